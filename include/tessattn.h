@@ -408,6 +408,38 @@ int tx_qwen3_forward(void *ctx, const TxQwen3Model *model, const uint32_t *ids,
                      float *pooled, uint32_t dimensions, void *workspace,
                      uint64_t workspace_bytes, void *stream);
 
+/* ---- encoder layers with other options ---------------------------------------------
+
+ * Operators for encoders whose layers differ from the two built in: the position rotation
+ * with its layouts and long-context frequencies, attention under a score rule, and a linear
+ * layer with bias, activation and residual.  No reference counterpart (the reference's
+ * layers are qwen3.py:191-280 and bert.py:191-231).  All pointers are device pointers unless
+ * said otherwise; strides are in elements; stream NULL: the context's stream. */
+
+/* One side of tx_rotary: `heads` heads of `dim` columns per token, each head contiguous.
+ * `out` may be `x` with the same strides (and dtype); otherwise the two must not overlap. */
+typedef struct {
+  const void *x;
+  void *out;
+  uint64_t x_token_stride, x_head_stride, out_token_stride, out_head_stride;
+  const uint16_t *norm_w; /* bf16 [dim] of an RMSNorm of each head first, or NULL */
+  uint32_t heads;
+} TxRotaryTensor;
+
+/* Rotates q and (unless NULL) k by their positions in one launch.  The first `rot_dim`
+ * columns of each head turn in pairs by the angle position * inv_freq[c] (an fp32 product,
+ * inv_freq device fp32 [rot_dim / 2]): columns (c, c + rot_dim / 2), or (2c, 2c + 1) with
+ * `interleaved`; cosine and sine are multiplied by `amplitude`, and `inverse` turns the other
+ * way.  Columns past rot_dim pass through.  A tensor with norm_w is first scaled by
+ * rsqrt(mean(x^2) + eps) * norm_w over all dim columns.  Positions: `positions` (device
+ * int32 [tokens], 0 <= position < 2^24), else the index inside the packed sequence
+ * (cu_seqlens, device int32 [nseq + 1], covering all tokens), else token % seq.  dtypes
+ * TX_F32 or TX_BF16; arithmetic is fp32, rounded once.  dim <= 256, rot_dim even, 2..dim. */
+int tx_rotary(void *ctx, const TxRotaryTensor *q, const TxRotaryTensor *k, int in_dtype,
+              int out_dtype, uint32_t tokens, uint32_t dim, uint32_t rot_dim, int interleaved,
+              int inverse, const int32_t *positions, const int32_t *cu_seqlens, uint32_t nseq,
+              uint32_t seq, const float *inv_freq, float amplitude, float eps, void *stream);
+
 /* ---- the BERT (BGE-small) fp32 forward around the head_dim-32 attention -------------
 
  * BertBackend.forward (bert.py:104-235) is built from these plus tx_linear (fmt TX_F32,

@@ -19,7 +19,8 @@ CSRC = PACKAGE / "csrc"
 LIBRARY = PACKAGE / "libtessattn.so"
 SOURCES = ["runtime.cu", "simt_kernels.cu", "attn_d32.cu", "attn_d32_tc.cu", "attn_f32_tc.cu", "attn_tc.cu", "attn_short.cu", "noalloc.cu",
            "pool.cu", "linear.cu", "qwen_ops.cu", "qwen3_model.cu",
-           "bert_ops.cu", "bert_model.cu"]
+           "bert_ops.cu", "bert_model.cu",
+           "rotary.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -154,6 +154,31 @@ cudaError_t launch_linear(const void *x, const void *x_lo, const void *w, const 
                           int mode, int fmt, uint32_t part, int *status, long long wait_cycles,
                           cudaStream_t stream);
 
+// ---- Encoder layers with other options (rotary.cu, attn_scored*.cu, linear_fused.cu) ----
+// One side (q or k) of the rotation: strides in elements, heads 0 when absent.
+struct RotaryTensor {
+  const void *x;
+  void *out;
+  uint64_t x_token, x_head, out_token, out_head;
+  const uint16_t *norm_w;  // bf16 [dim] or NULL
+  uint32_t heads;
+};
+struct RotaryProblem {
+  RotaryTensor q, k;
+  int in_dtype, out_dtype;
+  uint32_t tokens, dim, rot;
+  int interleaved;
+  int norm;                  // q or k has a norm weight
+  const int32_t *positions;  // [tokens], or NULL: from cu, or tok % seq
+  const int32_t *cu;
+  uint32_t nseq, seq;
+  const float *inv_freq;     // fp32 [rot / 2]
+  float amplitude, amplitude_sin;  // factors of cosine and sine (negated for the inverse)
+  float eps;
+};
+uint32_t rotary_vector(const RotaryProblem &p);
+cudaError_t launch_rotary(const RotaryProblem &p, cudaStream_t stream);
+
 // ---- BERT fp32 forward (bert_ops.cu) ----
 // Word + token-type-0 + absolute-position embeddings of `tokens` tokens, LayerNorm'd; the
 // position of a token is its index inside its packed sequence (cu, nseq) or t % seq.

@@ -24,7 +24,7 @@
 
 namespace {
 
-constexpr uint32_t kAbiVersion = 10;
+constexpr uint32_t kAbiVersion = 11;
 constexpr uint32_t kHostChunks = 8;              // most chunks of a host-buffer call
 constexpr size_t kHostChunkBytes = 16u << 20;     // bytes moved per chunk, at least
 // Padded layout, host-buffer calls: the valid k/v rows of consecutive sequences are
@@ -1642,6 +1642,57 @@ int tx_bert_embed(void *ctx, const uint32_t *ids, const int32_t *cu_seqlens, uin
   cudaSetDevice(c->device);
   cudaError_t e = tx::launch_bert_embed(p, stream ? (cudaStream_t)stream : c->stream);
   if (e != cudaSuccess) return cuda_fail(c, e, "bert_embed launch");
+  ++c->launches;
+  return TX_OK;
+}
+
+int tx_rotary(void *ctx, const TxRotaryTensor *q, const TxRotaryTensor *k, int in_dtype,
+              int out_dtype, uint32_t tokens, uint32_t dim, uint32_t rot_dim, int interleaved,
+              int inverse, const int32_t *positions, const int32_t *cu_seqlens, uint32_t nseq,
+              uint32_t seq, const float *inv_freq, float amplitude, float eps, void *stream) {
+  Ctx *c = (Ctx *)ctx;
+  if (!c) return TX_EINVAL;
+  std::lock_guard<std::recursive_mutex> g(c->mu);
+  if (!q || !inv_freq) return fail(c, TX_EINVAL, "rotary: null pointer");
+  if ((in_dtype != TX_F32 && in_dtype != TX_BF16) || (out_dtype != TX_F32 && out_dtype != TX_BF16))
+    return fail(c, TX_EINVAL, "rotary: bad dtype");
+  if (!dim || dim > 256 || rot_dim < 2 || rot_dim > dim || rot_dim % 2)
+    return fail(c, TX_EINVAL, "rotary: dim 1..256, rot_dim even, 2..dim");
+  if (!positions && cu_seqlens && !nseq) return fail(c, TX_EINVAL, "rotary: nseq must be positive");
+  if (!positions && !cu_seqlens && !seq)
+    return fail(c, TX_EINVAL, "rotary: positions, cu_seqlens or seq required");
+  if (!std::isfinite(amplitude) || !(eps >= 0.f) || !std::isfinite(eps))
+    return fail(c, TX_EINVAL, "rotary: bad amplitude or eps");
+  if (tokens > 0x7fffffffu) return fail(c, TX_EINVAL, "rotary: too many tokens");
+  const size_t ei = in_dtype == TX_BF16 ? 2 : 4, eo = out_dtype == TX_BF16 ? 2 : 4;
+  tx::RotaryProblem p{};
+  const TxRotaryTensor *side[2] = {q, k};
+  tx::RotaryTensor *to[2] = {&p.q, &p.k};
+  for (int i = 0; i < 2; ++i) {
+    const TxRotaryTensor *t = side[i];
+    if (!t) continue;
+    if (!t->x || !t->out || !t->heads || t->heads > 65535u)
+      return fail(c, TX_EINVAL, "rotary: a tensor needs x, out and 1..65535 heads");
+    if ((uintptr_t)t->x % ei || (uintptr_t)t->out % eo || (uintptr_t)t->norm_w % 2)
+      return fail(c, TX_EINVAL, "rotary: misaligned pointer");
+    if (t->x == t->out && (in_dtype != out_dtype || t->x_token_stride != t->out_token_stride ||
+                           t->x_head_stride != t->out_head_stride))
+      return fail(c, TX_EINVAL, "rotary: in place needs equal dtypes and strides");
+    if ((t->heads > 1 && t->out_head_stride < dim) || (tokens > 1 && t->out_token_stride < dim))
+      return fail(c, TX_EINVAL, "rotary: output rows overlap");
+    *to[i] = {t->x, t->out, t->x_token_stride, t->x_head_stride, t->out_token_stride,
+              t->out_head_stride, t->norm_w, t->heads};
+  }
+  p.in_dtype = in_dtype; p.out_dtype = out_dtype; p.tokens = tokens; p.dim = dim; p.rot = rot_dim;
+  p.interleaved = interleaved ? 1 : 0;
+  p.norm = p.q.norm_w || p.k.norm_w;
+  p.positions = positions; p.cu = cu_seqlens; p.nseq = nseq; p.seq = seq; p.inv_freq = inv_freq;
+  p.amplitude = amplitude; p.amplitude_sin = inverse ? -amplitude : amplitude; p.eps = eps;
+  if (!tokens) return TX_OK;
+  cudaSetDevice(c->device);
+  cudaError_t e = tx::launch_rotary(p, stream ? (cudaStream_t)stream : c->stream);
+  if (e != cudaSuccess) return cuda_fail(c, e, "rotary launch");
+  c->last_kernel = "rotary";
   ++c->launches;
   return TX_OK;
 }

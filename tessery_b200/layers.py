@@ -1,0 +1,162 @@
+"""NumPy-in / NumPy-out operators for encoder layers with other options than the two built
+in: the position rotation (layouts, part of the head, long-context frequencies, per-head
+norms), attention under a score rule (cap, distance bias, window, prefix, documents) and a
+linear layer with bias, activation and residual.
+
+float32 arrays, or uint16 arrays holding bf16 bit patterns, as in attention.py.  The same
+operators on device pointers are CudaRuntime.rotary_device, attention_scored_device and
+linear_fused_device.
+"""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+from numpy.typing import NDArray
+
+from . import native
+from .attention import _dtype_code, _upload, default_runtime
+from .errors import InvalidInputError
+from .runtime import CudaRuntime, _raise_for
+
+_NP = {native.TX_F32: np.float32, native.TX_BF16: np.uint16}
+
+
+def _out_code(name: str | None, default: int) -> int:
+    code = default if name is None else {"float32": native.TX_F32,
+                                         "bf16": native.TX_BF16}.get(name)
+    if code is None:
+        raise InvalidInputError()
+    return code
+
+
+def _read(rt: CudaRuntime, buffer, shape, code: int) -> NDArray:
+    out = np.empty(shape, dtype=_NP[code])
+    if out.size:
+        _raise_for(rt._lib.tx_read(buffer.pointer, out.ctypes.data, out.nbytes))
+    return out
+
+
+def rotary_frequencies(
+    rot_dim: int,
+    theta: float = 1e6,
+    *,
+    scaling: str = "none",
+    factor: float = 1.0,
+    original: int = 4096,
+    beta_fast: float = 32.0,
+    beta_slow: float = 1.0,
+) -> tuple[NDArray[np.float32], float]:
+    """(inverse frequencies [rot_dim / 2], amplitude) for rotary / rotary_device.
+
+    Column pair c turns by theta^(-2c / rot_dim) per position, rounded once from double.
+    `scaling` stretches that for contexts `factor` times the `original` positions trained on:
+
+    - "linear": every frequency divided by factor (position interpolation);
+    - "ntk": theta multiplied by factor^(rot_dim / (rot_dim - 2)), which leaves the fastest
+      pair as it is and divides the slowest by factor;
+    - "yarn": pairs that turn more than beta_fast times over the original positions are left,
+      those that turn less than beta_slow times divided by factor, with a linear ramp over the
+      pair index between the two; the amplitude is 0.1 ln(factor) + 1.
+    """
+    if rot_dim < 2 or rot_dim % 2 or not theta > 0 or not factor >= 1 or original < 1:
+        raise InvalidInputError()
+    c = np.arange(rot_dim // 2, dtype=np.float64)
+    amplitude = 1.0
+    if scaling == "ntk":
+        if rot_dim > 2:
+            theta = theta * factor ** (rot_dim / (rot_dim - 2))
+        freq = theta ** (-2.0 * c / rot_dim)
+    elif scaling in ("none", "linear"):
+        freq = theta ** (-2.0 * c / rot_dim) / (factor if scaling == "linear" else 1.0)
+    elif scaling == "yarn":
+        if not beta_fast > beta_slow > 0 or theta == 1.0:
+            raise InvalidInputError()
+        freq = theta ** (-2.0 * c / rot_dim)
+
+        def pair_with(turns: float) -> float:  # the (real) pair index that turns so often
+            return rot_dim * math.log(original / (2 * math.pi * turns)) / (2 * math.log(theta))
+
+        low = max(math.floor(pair_with(beta_fast)), 0)
+        high = min(math.ceil(pair_with(beta_slow)), rot_dim - 1)
+        ramp = np.clip((c - low) / max(high - low, 1e-3), 0.0, 1.0)
+        freq = freq * (1.0 - ramp) + freq / factor * ramp
+        amplitude = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+    else:
+        raise InvalidInputError()
+    return freq.astype(np.float32), amplitude
+
+
+def rotary(
+    q: NDArray,
+    k: NDArray | None = None,
+    *,
+    inv_freq: NDArray[np.float32],
+    amplitude: float = 1.0,
+    interleaved: bool = False,
+    inverse: bool = False,
+    positions: NDArray | None = None,
+    cu_seqlens: NDArray | None = None,
+    seq: int = 0,
+    q_norm_weight: NDArray | None = None,
+    k_norm_weight: NDArray | None = None,
+    eps: float = 1e-6,
+    out_dtype: str | None = None,
+    runtime: CudaRuntime | None = None,
+) -> tuple[NDArray, NDArray | None]:
+    """Rotates q [tokens, heads, dim] and k [tokens, kv_heads, dim] by their positions
+    (tx_rotary): the first 2 * len(inv_freq) columns of every head, half or interleaved
+    layout.  Positions: `positions` [tokens], or the index inside each packed sequence
+    (cu_seqlens), or token % seq.  Norm weights are bf16 bits [dim]."""
+    rt = runtime or default_runtime()
+    q = np.ascontiguousarray(q)
+    k = None if k is None else np.ascontiguousarray(k)
+    freq = np.ascontiguousarray(inv_freq, dtype=np.float32)
+    if q.ndim != 3 or freq.ndim != 1 or not freq.size:
+        raise InvalidInputError()
+    tokens, heads, dim = q.shape
+    code = _dtype_code(q)
+    if k is not None and (k.ndim != 3 or k.shape[0] != tokens or k.shape[2] != dim
+                          or _dtype_code(k) != code):
+        raise InvalidInputError()
+    out_code = _out_code(out_dtype, code)
+    if not tokens:
+        return (np.empty(q.shape, _NP[out_code]),
+                None if k is None else np.empty(k.shape, _NP[out_code]))
+    if sum(x is not None for x in (positions, cu_seqlens)) + bool(seq) != 1:
+        raise InvalidInputError()
+    pos_ptr = cu_ptr = None
+    nseq = 0
+    if positions is not None:
+        pos = np.ascontiguousarray(positions, dtype=np.int32)
+        if pos.shape != (tokens,) or pos.min() < 0 or pos.max() >= 1 << 24:
+            raise InvalidInputError()
+        pos_ptr = _upload(rt, "rotary_pos", pos)
+    elif cu_seqlens is not None:
+        cu = np.ascontiguousarray(cu_seqlens, dtype=np.int32)
+        if cu.ndim != 1 or cu.size < 2 or cu[0] != 0 or cu[-1] != tokens or np.any(np.diff(cu) < 0):
+            raise InvalidInputError()
+        cu_ptr, nseq = _upload(rt, "rotary_cu", cu), cu.size - 1
+    weights = []
+    for name, w in (("rotary_qw", q_norm_weight), ("rotary_kw", k_norm_weight)):
+        if w is not None:
+            w = np.ascontiguousarray(w, dtype=np.uint16)
+            if w.shape != (dim,):
+                raise InvalidInputError()
+        weights.append(None if w is None else _upload(rt, name, w))
+    size = 4 if out_code == native.TX_F32 else 2
+    q_out = rt.workspace("rotary_q_out", q.size * size)
+    k_out = None if k is None else rt.workspace("rotary_k_out", k.size * size)
+    rt.rotary_device(
+        _upload(rt, "rotary_q", q), None if k is None else _upload(rt, "rotary_k", k),
+        q_out.device_ptr, None if k_out is None else k_out.device_ptr, tokens=tokens, heads=heads,
+        kv_heads=0 if k is None else k.shape[1], dim=dim,
+        inv_freq=_upload(rt, "rotary_freq", freq), rot_dim=2 * freq.size, interleaved=interleaved,
+        inverse=inverse, amplitude=amplitude, positions=pos_ptr, cu_seqlens=cu_ptr, nseq=nseq,
+        seq=seq, q_norm_weight=weights[0], k_norm_weight=weights[1], eps=eps, in_dtype=code,
+        out_dtype=out_code,
+    )
+    rt.sync()
+    return (_read(rt, q_out, q.shape, out_code),
+            None if k is None else _read(rt, k_out, k.shape, out_code))

@@ -16,7 +16,7 @@ from typing import Any
 
 from .errors import NativeBuildError
 
-ABI_VERSION = 10
+ABI_VERSION = 11
 LIBRARY_NAME = "libtessattn.so"
 
 TX_OK, TX_EINVAL, TX_ECUDA, TX_ETIMEOUT = 0, 1, 2, 3
@@ -64,6 +64,17 @@ class TxBertModel(ct.Structure):
         ("eps", _f32), ("precise", _i32),
         ("words", _vp), ("positions", _vp), ("types", _vp), ("ln_w", _vp), ("ln_b", _vp),
         ("layer", ct.POINTER(TxBertLayer)),
+    ]
+
+
+class TxRotaryTensor(ct.Structure):
+    """One side of tx_rotary (TxRotaryTensor in tessattn.h)."""
+
+    _fields_ = [
+        ("x", _vp), ("out", _vp),
+        *[(name, _u64) for name in ("x_token_stride", "x_head_stride", "out_token_stride",
+                                    "out_head_stride")],
+        ("norm_w", _vp), ("heads", _u32),
     ]
 
 
@@ -143,6 +154,9 @@ SIGNATURES: dict[str, tuple[list[Any], Any]] = {
     "tx_rms_norm_rows": ([_vp, _vp, _vp, _vp, _i32, _u32, _u32, _f32, _vp], _i32),
     "tx_linear": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _i32, _i32, _u32, _vp],
                   _i32),
+    "tx_rotary": (
+        [_vp, ct.POINTER(TxRotaryTensor), ct.POINTER(TxRotaryTensor), _i32, _i32, _u32, _u32,
+         _u32, _i32, _i32, _vp, _vp, _u32, _u32, _vp, _f32, _f32, _vp], _i32),
     "tx_attention_padded_noalloc": (
         [_vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _i32, _i32, _f32, _vp, _f32,
          _f32, _vp, _vp],

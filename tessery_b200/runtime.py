@@ -707,6 +707,59 @@ class CudaRuntime:
                                              cu_host.ctypes.data, cu_host.size - 1, pooled,
                                              workspace, workspace_bytes, stream))
 
+    # ---- encoder layers with other options (device pointers) ----------------------------
+    def rotary_device(
+        self,
+        q: int,
+        k: int | None,
+        q_out: int,
+        k_out: int | None,
+        *,
+        tokens: int,
+        heads: int,
+        kv_heads: int = 0,
+        dim: int,
+        inv_freq: int,
+        rot_dim: int | None = None,
+        interleaved: bool = False,
+        inverse: bool = False,
+        amplitude: float = 1.0,
+        positions: int | None = None,
+        cu_seqlens: int | None = None,
+        nseq: int = 0,
+        seq: int = 0,
+        q_norm_weight: int | None = None,
+        k_norm_weight: int | None = None,
+        eps: float = 1e-6,
+        in_dtype: int = native.TX_BF16,
+        out_dtype: int = native.TX_BF16,
+        q_strides: Sequence[int] | None = None,
+        k_strides: Sequence[int] | None = None,
+        q_out_strides: Sequence[int] | None = None,
+        k_out_strides: Sequence[int] | None = None,
+        stream: int | None = None,
+    ) -> None:
+        """Queues the position rotation of q and k (k None: q alone), behind a per-head
+        RMSNorm where a norm weight is given (tx_rotary).  Strides are (token, head) in
+        elements, contiguous [tokens, heads, dim] by default; `inv_freq` (device fp32
+        [rot_dim / 2]) and `amplitude` come from layers.rotary_frequencies."""
+        self._check_open()
+
+        def side(x, out, n, xs, os, weight):
+            xt, xh = (n * dim, dim) if xs is None else xs
+            ot, oh = (n * dim, dim) if os is None else os
+            if min(xt, xh, ot, oh) < 0:
+                raise InvalidInputError()
+            return native.TxRotaryTensor(x, out, xt, xh, ot, oh, weight, n)
+
+        qt = side(q, q_out, heads, q_strides, q_out_strides, q_norm_weight)
+        kt = None if k is None else side(k, k_out, kv_heads, k_strides, k_out_strides,
+                                         k_norm_weight)
+        _raise_for(self._lib.tx_rotary(
+            self._pointer, qt, kt, in_dtype, out_dtype, tokens, dim,
+            dim if rot_dim is None else rot_dim, int(bool(interleaved)), int(bool(inverse)),
+            positions, cu_seqlens, nseq, seq, inv_freq, amplitude, eps, stream))
+
     def sync(self, stream: int | None = None) -> None:
         """Waits for queued work and reports kernel errors (tx_sync)."""
         self._check_open()
