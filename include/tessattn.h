@@ -440,6 +440,54 @@ int tx_rotary(void *ctx, const TxRotaryTensor *q, const TxRotaryTensor *k, int i
               int inverse, const int32_t *positions, const int32_t *cu_seqlens, uint32_t nseq,
               uint32_t seq, const float *inv_freq, float amplitude, float eps, void *stream);
 
+/* Attention under a score rule: row i of a sequence with nq query and nk key rows stands at
+ * position pos = i + nk - nq (the queries are the last positions: nq == nk for a whole text,
+ * nq == 1 for one new token against the keys kept for it), and
+ *   z_ij = scale * q_i . k_j;  z = softcap * tanh(z / softcap);  z += bias(head, j - pos)
+ *   out_i = sum over open j of softmax(z_i)_j v_j;  zeros where no key is open. */
+typedef struct {
+  float softcap;              /* > 0; 0: no cap */
+  const float *slopes;        /* fp32 [heads]: bias -slope * |j - pos|; or NULL */
+  const float *distance_bias; /* fp32 [heads, 2 * reach + 1]: entry clamp(j - pos, -reach, reach)
+                                 + reach; or NULL (at most one of the two biases).  -inf closes
+                                 a key; the lowest finite value does not */
+  uint32_t reach;             /* at most 2^20 */
+  int causal;                 /* keys j <= pos */
+  int32_t window_left, window_right; /* keys pos - left <= j <= pos + right; < 0: no limit */
+  const int32_t *prefix;      /* int32 [nseq]: keys j < prefix are open whatever causal and window
+                                 say; or NULL */
+  const int32_t *q_docs, *k_docs; /* int32 per q / k row (both or neither): a key is open only to
+                                 rows of its document; a negative id attends nothing and is
+                                 attended by none */
+} TxScoreRule;
+
+/* Rows of q, k or v: [rows, heads, dim] with strides in elements, each head contiguous. */
+typedef struct {
+  const void *data;
+  uint64_t row_stride, head_stride;
+} TxRows;
+
+/* Where the sequences lie: packed, sequence s at rows cu[s] .. cu[s + 1] - 1 (device int32
+ * [nseq + 1]); or cu NULL, sequence s at rows s * max_len with lengths[s] of them valid (device
+ * int32 [nseq], or NULL: all).  No sequence is longer than max_len; a device length that is, or
+ * that leaves the `rows`, is cut to fit and reported as TX_EINVAL by the next tx_sync. */
+typedef struct {
+  const int32_t *cu, *lengths;
+  uint32_t rows, max_len;
+} TxLayout;
+
+/* q [rows, heads, dim], k and v [rows, kv_heads, dim] (one layout), heads a multiple of kv_heads;
+ * out contiguous [q rows, heads, dim].  In a padded layout the query rows past a sequence's
+ * length get zeros; key and value rows past it, and those of other documents, may hold
+ * anything, NaN and Inf included.  in_dtype / out_dtype TX_F32 or TX_BF16; dim <= 256; scale
+ * finite.  bf16 with dim a multiple of 8 up to 128, strides multiples of 8 and 16-byte aligned
+ * pointers runs on the tensor-memory kernel (P rounded to bf16), everything else in fp32
+ * accuracy. */
+int tx_attention_scored(void *ctx, const TxRows *q, const TxRows *k, const TxRows *v, void *out,
+                        const TxLayout *q_layout, const TxLayout *k_layout, uint32_t nseq,
+                        uint32_t heads, uint32_t kv_heads, uint32_t dim, int in_dtype,
+                        int out_dtype, float scale, const TxScoreRule *rule, void *stream);
+
 /* ---- the BERT (BGE-small) fp32 forward around the head_dim-32 attention -------------
 
  * BertBackend.forward (bert.py:104-235) is built from these plus tx_linear (fmt TX_F32,

@@ -31,3 +31,66 @@ def rotary(x: NDArray, positions: NDArray, inv_freq: NDArray, *, amplitude: floa
         out[..., i] = y[..., i] * cos[..., c] - y[..., j] * sin[..., c]
         out[..., j] = y[..., j] * cos[..., c] + y[..., i] * sin[..., c]
     return out
+
+
+def open_keys(nq: int, nk: int, *, causal=False, window=(-1, -1), prefix=0, q_docs=None,
+              k_docs=None) -> NDArray:
+    """[nq, nk] truth values: the keys the rule leaves open to each query row."""
+    pos = np.arange(nq)[:, None] + nk - nq
+    j = np.arange(nk)[None, :]
+    seen = np.ones((nq, nk), bool)
+    if causal:
+        seen &= j <= pos
+    if window[0] >= 0:
+        seen &= j >= pos - window[0]
+    if window[1] >= 0:
+        seen &= j <= pos + window[1]
+    seen |= j < prefix
+    if q_docs is not None:
+        q_docs, k_docs = np.asarray(q_docs), np.asarray(k_docs)
+        seen &= (q_docs[:, None] == k_docs[None, :]) & (q_docs[:, None] >= 0)
+    return seen
+
+
+def attention_scored(q: NDArray, k: NDArray, v: NDArray, *, scale=None, softcap=0.0, slopes=None,
+                     table=None, **rule) -> tuple[NDArray, NDArray, float]:
+    """One sequence: q [nq, heads, dim], k and v [nk, kv_heads, dim] as float values.  Returns
+    the output, sum_j p_ij |v_j| (what the errors of the weights p are measured against) and the
+    largest finite |score| plus |scale| sum |q||k| met.  A key that is not open is never read."""
+    q, k, v = (np.asarray(a, np.float64) for a in (q, k, v))
+    nq, heads, dim = q.shape
+    nk, group = k.shape[0], heads // k.shape[1]
+    scale = dim ** -0.5 if scale is None else scale
+    seen = open_keys(nq, nk, **rule)
+    pos = np.arange(nq)[:, None] + nk - nq
+    dist = np.arange(nk)[None, :] - pos
+    out, mass, biggest = np.zeros((nq, heads, dim)), np.zeros((nq, heads, dim)), 0.0
+    for h in range(heads):
+        kh, vh = k[:, h // group], v[:, h // group]
+        for i in range(nq):
+            at = np.flatnonzero(seen[i])
+            if not at.size:
+                continue
+            with np.errstate(invalid="ignore", over="ignore"):
+                z = scale * (kh[at] @ q[i, h])
+                biggest = max(biggest, float(np.nanmax(
+                    abs(scale) * (np.abs(kh[at]) @ np.abs(q[i, h])), initial=0.0)))
+                if softcap:
+                    z = softcap * np.tanh(z / softcap)
+                if slopes is not None:
+                    z = z - float(slopes[h]) * np.abs(dist[i, at])
+                if table is not None:
+                    reach = (table.shape[1] - 1) // 2
+                    z = z + np.asarray(table[h], np.float64)[
+                        np.clip(dist[i, at], -reach, reach) + reach]
+                finite = np.abs(z[np.isfinite(z) & (np.abs(z) < 1e30)])
+                biggest = max(biggest, float(finite.max(initial=0.0)))
+                top = np.max(z)
+                if top == -np.inf:
+                    continue
+                p = np.exp(z - top)
+                p /= p.sum()
+                at, p = at[p != 0], p[p != 0]
+                out[i, h] = p @ vh[at]
+                mass[i, h] = p @ np.abs(vh[at])
+    return out, mass, biggest

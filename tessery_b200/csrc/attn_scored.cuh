@@ -1,0 +1,264 @@
+// What the kernels of attention under a score rule share: how a launch is cut into CTAs, which
+// key tiles a CTA visits, which keys a query row may see, and how partial results over a split
+// key range are joined.
+//
+// Rows.  A CTA's kRows rows are kRows / pack query tokens of `pack` heads that read the same
+// kv head (row r: token r / pack, head r % pack), so those heads share every key and value
+// tile; pack is the largest power of two that divides the heads per kv head (at most kRows).
+// Query token i of a sequence with nq queries and nk keys stands at position i + nk - nq.
+#pragma once
+
+#include "common.cuh"
+#include "kernels.h"
+
+namespace tx {
+namespace scored {
+
+constexpr int kKeys = 128;        // keys per tile
+constexpr uint32_t kDocWords = 1024;  // bits for the key tiles of a document mask: 32768 tiles
+
+struct Seq {
+  int q_row, k_row;  // first row of the sequence in q and k
+  int nq, nk;
+};
+
+// Rows of sequence s.  Offsets and lengths come from device arrays: they are held to the
+// tensors' rows, and a length above the stated maximum is reported.
+__device__ __forceinline__ Seq load_seq(const ScoredProblem &p, uint32_t s) {
+  Seq o;
+  auto side = [&](const int32_t *cu, const int32_t *len, uint32_t most, uint32_t rows, int *row,
+                  int *n) {
+    long long r0 = cu ? cu[s] : (long long)s * most;
+    long long c = cu ? (long long)cu[s + 1] - cu[s] : len ? (long long)len[s] : (long long)most;
+    if (c > (long long)most || r0 < 0 || c < 0 || r0 + c > (long long)rows) {
+      if (threadIdx.x == 0) report_status(p.status, kStatusBadArg);
+      r0 = min(max(r0, 0ll), (long long)rows);
+      c = min(min(max(c, 0ll), (long long)most), (long long)rows - r0);
+    }
+    *row = (int)r0;
+    *n = (int)c;
+  };
+  side(p.cu_q, p.q_lengths, p.max_q, p.rows_q, &o.q_row, &o.nq);
+  side(p.cu_k, p.k_lengths, p.max_k, p.rows_k, &o.k_row, &o.nk);
+  return o;
+}
+
+// One CTA's work.
+struct Unit {
+  Seq s;
+  uint32_t head0, kv;      // first query head of the pack, kv head
+  uint32_t split;          // which part of the key range
+  uint32_t slot;           // index of the unit without its split
+  int t0;                  // first query token
+  int tokens;              // query tokens of the sequence in this tile
+  int present;             // rows' tokens the layout has here: those past `tokens` get zeros
+  int prefix;              // keys [0, prefix) are open to every row
+  // key tiles in order: [0, a) then [b, ...), `count` in all; this CTA visits [first, last)
+  int a, b, first, last;
+};
+
+// Key range of a query position without the prefix: [lo, hi).
+__device__ __forceinline__ void row_range(const ScoredProblem &p, int pos, int nk, int *lo,
+                                          int *hi) {
+  int l = 0, h = nk;
+  if (p.left >= 0) l = max(l, pos - p.left);
+  if (p.causal) h = min(h, pos + 1);
+  if (p.right >= 0 && pos < 0x7fffffff - p.right) h = min(h, pos + p.right + 1);
+  *lo = l;
+  *hi = h;
+}
+
+// Blocks run the last token tiles first: under a causal rule they see the most keys.
+template <int kRows>
+__device__ __forceinline__ Unit make_unit(const ScoredProblem &p, uint32_t block) {
+  Unit u;
+  const uint32_t groups = p.heads / p.pack;
+  u.split = block % p.splits;
+  uint32_t rest = block / p.splits;
+  u.slot = rest;
+  const uint32_t hg = rest % groups;
+  rest /= groups;
+  const uint32_t s = rest % p.nseq, tile = p.tiles - 1 - rest / p.nseq;
+  u.s = load_seq(p, s);
+  u.head0 = hg * p.pack;
+  u.kv = u.head0 / (p.heads / p.kv_heads);
+  const int per = kRows / (int)p.pack;
+  u.t0 = (int)tile * per;
+  u.tokens = max(0, min(per, u.s.nq - u.t0));
+  u.present = p.cu_q ? u.tokens
+                     : max(0, min(per, min((int)p.max_q, (int)p.rows_q - u.s.q_row) - u.t0));
+  u.prefix = p.prefix ? min(max(p.prefix[s], 0), u.s.nk) : 0;
+  u.a = u.b = u.first = u.last = 0;
+  if (!u.tokens) return u;
+  const int p0 = u.t0 + u.s.nk - u.s.nq;
+  int lo, hi, x;
+  row_range(p, p0, u.s.nk, &lo, &x);                  // both ends grow with the position
+  row_range(p, p0 + u.tokens - 1, u.s.nk, &x, &hi);
+  u.a = (u.prefix + kKeys - 1) / kKeys;
+  u.b = max(u.a, lo / kKeys);
+  const int end = hi > lo ? (hi + kKeys - 1) / kKeys : 0;
+  const int count = u.a + max(0, end - u.b);
+  u.first = (int)((long long)count * u.split / p.splits);
+  u.last = (int)((long long)count * (u.split + 1) / p.splits);
+  return u;
+}
+__device__ __forceinline__ int key_tile(const Unit &u, int i) { return i < u.a ? i : i - u.a + u.b; }
+
+// With documents: the bits of the visited tiles that hold a key of a document that the unit's
+// rows may hold (their ids between the rows' least and greatest), by all threads of the CTA.
+// `words` holds (last - first + 31) / 32 words.  Ends with the threads in step.
+__device__ __forceinline__ void mark_tiles(const ScoredProblem &p, const Unit &u, uint32_t *words,
+                                           int *range) {
+  if (threadIdx.x == 0) {
+    range[0] = 0x7fffffff;
+    range[1] = -1;
+  }
+  for (int i = threadIdx.x; i < (u.last - u.first + 31) / 32; i += blockDim.x) words[i] = 0;
+  __syncthreads();
+  const int32_t *qd = p.q_docs + u.s.q_row + u.t0;
+  for (int i = threadIdx.x; i < u.tokens; i += blockDim.x)
+    if (qd[i] >= 0) {
+      atomicMin(&range[0], qd[i]);
+      atomicMax(&range[1], qd[i]);
+    }
+  __syncthreads();
+  const int lo = range[0], hi = range[1];
+  const int32_t *kd = p.k_docs + u.s.k_row;
+  for (int i = u.first + (int)(threadIdx.x >> 5); i < u.last; i += (int)(blockDim.x >> 5)) {
+    const int k0 = key_tile(u, i) * kKeys;
+    bool hit = false;
+#pragma unroll
+    for (int c = 0; c < kKeys / 32; ++c) {
+      const int j = k0 + c * 32 + (int)(threadIdx.x & 31);
+      if (j < u.s.nk) {
+        const int d = kd[j];
+        hit |= d >= lo && d <= hi;
+      }
+    }
+    if (__any_sync(0xffffffffu, hit) && (threadIdx.x & 31) == 0)
+      atomicOr(&words[(i - u.first) >> 5], 1u << ((i - u.first) & 31));
+  }
+  __syncthreads();
+}
+// Whether every key of the tile from k0 (up to the sequence's end) is open to every row of the
+// unit, as far as ranges tell.
+__device__ __forceinline__ bool whole_tile(const ScoredProblem &p, const Unit &u, int k0) {
+  if (p.q_docs) return false;
+  const int end = min(k0 + kKeys, u.s.nk), p0 = u.t0 + u.s.nk - u.s.nq;
+  if (end <= u.prefix) return true;
+  int lo, hi, x;
+  row_range(p, p0 + u.tokens - 1, u.s.nk, &lo, &x);
+  row_range(p, p0, u.s.nk, &x, &hi);
+  return k0 >= lo && end <= hi;
+}
+// The first visited tile at or after i (u.last when there is none).
+__device__ __forceinline__ int next_tile(const Unit &u, const uint32_t *words, int i) {
+  if (!words) return i;
+  while (i < u.last) {
+    const int at = i - u.first;
+    const uint32_t w = words[at >> 5] >> (at & 31);
+    if (w) return min(i + __ffs(w) - 1, u.last);
+    i = u.first + ((at >> 5) + 1) * 32;
+  }
+  return u.last;
+}
+
+// Bits t of [c0, c0 + 32) that lie in [lo, hi).
+__device__ __forceinline__ uint32_t interval_bits(int c0, int lo, int hi) {
+  const int l = min(max(lo - c0, 0), 32), h = min(max(hi - c0, 0), 32);
+  const uint32_t below_h = (uint32_t)((1ull << h) - 1), below_l = (uint32_t)((1ull << l) - 1);
+  return below_h & ~below_l;
+}
+
+// One row's view of the keys.
+struct Row {
+  int pos, lo, hi, prefix, doc;
+  __device__ __forceinline__ uint32_t bits(int c0) const {
+    return interval_bits(c0, lo, hi) | interval_bits(c0, 0, prefix);
+  }
+};
+__device__ __forceinline__ Row make_row(const ScoredProblem &p, const Unit &u, int token,
+                                        bool live) {
+  Row r;
+  r.pos = u.t0 + token + u.s.nk - u.s.nq;
+  row_range(p, r.pos, u.s.nk, &r.lo, &r.hi);
+  r.prefix = u.prefix;
+  r.doc = -1;
+  if (p.q_docs && live) r.doc = p.q_docs[u.s.q_row + u.t0 + token];
+  if (!live || (p.q_docs && r.doc < 0)) r.lo = r.hi = r.prefix = 0;
+  return r;
+}
+
+// Zeros for the query rows of a padded layout past the sequence's length.
+__device__ __forceinline__ void zero_padding(const ScoredProblem &p, const Unit &u) {
+  for (int t = u.tokens; t < u.present; ++t) {
+    const size_t at = ((size_t)(u.s.q_row + u.t0 + t) * p.heads + u.head0) * p.dim;
+    const uint32_t n = p.pack * p.dim;
+    for (uint32_t c = threadIdx.x; c < n; c += blockDim.x) {
+      if (p.out_dtype == 1)
+        static_cast<uint16_t *>(p.out)[at + c] = 0;
+      else
+        static_cast<float *>(p.out)[at + c] = 0.f;
+    }
+  }
+}
+
+// Joining a split key range.  Each CTA of a unit leaves, per row, its unnormalised sum O (fp32),
+// its reference m (log2 units; -inf when it saw no key) and row sum l; the CTA that arrives last
+// adds the parts in the order of the splits, so the result does not depend on which it was.
+//
+// Called by every thread of the CTA once its partials are written; true in the CTA that has to
+// join.  Every CTA arrives, whatever happened to it, so the counters always return to zero.
+__device__ __forceinline__ bool arrive_last(const ScoredProblem &p, const Unit &u,
+                                            uint32_t *flag) {
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const uint32_t n = atomicAdd(&p.part_arrived[u.slot], 1u);
+    *flag = n + 1 == p.splits;
+    if (*flag) p.part_arrived[u.slot] = 0;
+  }
+  __syncthreads();
+  const bool last = *flag != 0;
+  if (last) __threadfence();
+  return last;
+}
+
+__device__ __forceinline__ void store_out(const ScoredProblem &p, size_t at, float v) {
+  if (p.out_dtype == 1)
+    static_cast<uint16_t *>(p.out)[at] = f32_to_bf16_bits(v);
+  else
+    static_cast<float *>(p.out)[at] = v;
+}
+
+// One warp per row: weights of the splits first, then the columns.
+template <int kRows>
+__device__ __forceinline__ void join_parts(const ScoredProblem &p, const Unit &u) {
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const size_t base = (size_t)u.slot * p.splits * kRows;
+  for (int r = (int)warp; r < u.tokens * (int)p.pack; r += (int)warps) {
+    float m = -INFINITY;
+    for (uint32_t s = 0; s < p.splits; ++s) m = fmaxf(m, p.part_ml[base + s * kRows + r].x);
+    const float ref = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    for (uint32_t s = 0; s < p.splits; ++s) {
+      const float2 v = p.part_ml[base + s * kRows + r];
+      l += exp2f(v.x - ref) * v.y;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const size_t orow = ((size_t)(u.s.q_row + u.t0 + r / (int)p.pack) * p.heads + u.head0 +
+                         r % (int)p.pack) * p.dim;
+    for (uint32_t c = lane; c < p.dim; c += 32) {
+      float acc = 0.f;
+      for (uint32_t s = 0; s < p.splits; ++s) {
+        const float2 v = p.part_ml[base + s * kRows + r];
+        if (v.x != -INFINITY)
+          acc += exp2f(v.x - ref) * p.part_o[(base + s * kRows + r) * p.part_dp + c];
+      }
+      store_out(p, orow + c, acc * inv);
+    }
+  }
+}
+
+}  // namespace scored
+}  // namespace tx

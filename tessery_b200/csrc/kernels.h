@@ -177,6 +177,40 @@ struct RotaryProblem {
   float eps;
 };
 uint32_t rotary_vector(const RotaryProblem &p);
+
+// Attention under a score rule; strides in elements, out contiguous [rows_q, heads, dim].
+struct ScoredProblem {
+  const void *q, *k, *v;
+  void *out;
+  uint64_t q_row, q_head, k_row, k_head, v_row, v_head;
+  const int32_t *cu_q, *cu_k;            // packed rows, or NULL: sequence s starts at s * max
+  const int32_t *q_lengths, *k_lengths;  // rows of each sequence when not packed (NULL: max)
+  uint32_t nseq, rows_q, rows_k, max_q, max_k;
+  uint32_t heads, kv_heads, dim;
+  int in_dtype, out_dtype;
+  float scale;
+  // the rule
+  float softcap;                // > 0: z -> softcap * tanh(z / softcap)
+  const float *slopes;          // [heads]: z - slope * |distance|
+  const float *table;           // [heads][2 * reach + 1]: z + table[clamp(j - pos) + reach]
+  int reach;
+  int causal, left, right;      // left, right < 0: unlimited
+  const int32_t *prefix;        // [nseq]
+  const int32_t *q_docs, *k_docs;  // per row; < 0: attends nothing, attended by none
+  int *status;
+  long long wait_cycles;
+  // the cut (scored_plan)
+  uint32_t pack, tiles, splits, rows;    // rows: rows of a CTA
+  uint32_t part_dp;                      // columns of a partial row
+  float *part_o;
+  float2 *part_ml;
+  uint32_t *part_arrived;
+};
+// Fills the cut, without the partials; `tc`: the tensor-core kernel's.
+void scored_plan(ScoredProblem *p, bool tc, int num_sms);
+bool scored_tc_supported(const ScoredProblem &p);
+cudaError_t launch_scored_tc(const ScoredProblem &p, cudaStream_t stream);
+cudaError_t launch_scored_f32(const ScoredProblem &p, cudaStream_t stream);
 cudaError_t launch_rotary(const RotaryProblem &p, cudaStream_t stream);
 
 // ---- BERT fp32 forward (bert_ops.cu) ----

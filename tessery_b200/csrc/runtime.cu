@@ -153,6 +153,10 @@ struct Ctx {
   uint64_t units_key = 0;
   uint32_t units_count = 0;
   cudaEvent_t scratch_done = nullptr;  // last launch that read scratch
+  // split key ranges of tx_attention_scored: arrival counters (zero between calls), then the
+  // partial sums
+  uint8_t *part_mem = nullptr;
+  size_t part_bytes = 0, part_units = 0;
   std::set<Buf *> buffers;
   // Accounting of the buffers above: bytes live now, the most ever live at once, and
   // the number and bytes of every allocation made.
@@ -223,6 +227,25 @@ cudaError_t ensure_units(Ctx *c, size_t count) {
   e = cudaMalloc(&c->units, count * sizeof(uint32_t));
   if (e != cudaSuccess) return e;
   c->units_cap = count;
+  return cudaSuccess;
+}
+
+// Counters for `units` units (zeroed when made) and `bytes` of partial sums behind them.
+cudaError_t ensure_parts(Ctx *c, size_t units, size_t bytes) {
+  const size_t need_units = std::max(units, c->part_units);
+  const size_t counters = (need_units * 4 + 255) & ~(size_t)255;
+  if (c->part_units >= units && c->part_bytes >= counters + bytes) return cudaSuccess;
+  cudaError_t e = cudaDeviceSynchronize();
+  if (e != cudaSuccess) return e;
+  if (c->part_mem) cudaFree(c->part_mem);
+  c->part_mem = nullptr;
+  c->part_bytes = c->part_units = 0;
+  if ((e = cudaMalloc(&c->part_mem, counters + bytes)) != cudaSuccess) return e;
+  if ((e = cudaMemsetAsync(c->part_mem, 0, counters, c->stream)) != cudaSuccess ||
+      (e = cudaStreamSynchronize(c->stream)) != cudaSuccess)
+    return e;
+  c->part_bytes = counters + bytes;
+  c->part_units = need_units;
   return cudaSuccess;
 }
 
@@ -828,6 +851,7 @@ void tx_destroy(void *ctx) {
     c->buffers.clear();
     if (c->qk_scratch) cudaFree(c->qk_scratch);
     if (c->units) cudaFree(c->units);
+    if (c->part_mem) cudaFree(c->part_mem);
     if (c->status) cudaFree(c->status);
     for (cudaEvent_t ev : c->prof_events) cudaEventDestroy(ev);
     for (cudaEvent_t ev : c->kt_ev)
@@ -1693,6 +1717,93 @@ int tx_rotary(void *ctx, const TxRotaryTensor *q, const TxRotaryTensor *k, int i
   cudaError_t e = tx::launch_rotary(p, stream ? (cudaStream_t)stream : c->stream);
   if (e != cudaSuccess) return cuda_fail(c, e, "rotary launch");
   c->last_kernel = "rotary";
+  ++c->launches;
+  return TX_OK;
+}
+
+int tx_attention_scored(void *ctx, const TxRows *q, const TxRows *k, const TxRows *v, void *out,
+                        const TxLayout *q_layout, const TxLayout *k_layout, uint32_t nseq,
+                        uint32_t heads, uint32_t kv_heads, uint32_t dim, int in_dtype,
+                        int out_dtype, float scale, const TxScoreRule *rule, void *stream) {
+  Ctx *c = (Ctx *)ctx;
+  if (!c) return TX_EINVAL;
+  std::lock_guard<std::recursive_mutex> g(c->mu);
+  if (!q || !k || !v || !out || !q_layout || !k_layout || !rule || !q->data || !k->data || !v->data)
+    return fail(c, TX_EINVAL, "attention_scored: null pointer");
+  if (!heads || !kv_heads || heads % kv_heads)
+    return fail(c, TX_EINVAL, "attention_scored: heads must be a positive multiple of kv_heads");
+  if (!dim || dim > 256) return fail(c, TX_EINVAL, "attention_scored: head_dim must be in 1..256");
+  if ((in_dtype != TX_F32 && in_dtype != TX_BF16) || (out_dtype != TX_F32 && out_dtype != TX_BF16))
+    return fail(c, TX_EINVAL, "attention_scored: bad dtype");
+  if (!std::isfinite(scale)) return fail(c, TX_EINVAL, "attention_scored: scale must be finite");
+  const TxScoreRule &r = *rule;
+  if (!(r.softcap >= 0.f) || !std::isfinite(r.softcap))
+    return fail(c, TX_EINVAL, "attention_scored: softcap must be finite and >= 0");
+  if (r.slopes && r.distance_bias) return fail(c, TX_EINVAL, "attention_scored: one bias at most");
+  if (r.distance_bias && r.reach > (1u << 20))
+    return fail(c, TX_EINVAL, "attention_scored: reach at most 2^20");
+  if (!r.q_docs != !r.k_docs)
+    return fail(c, TX_EINVAL, "attention_scored: q_docs and k_docs go together");
+  const TxLayout *lay[2] = {q_layout, k_layout};
+  for (const TxLayout *l : lay) {
+    if (l->rows > 0x7fffffffu || l->max_len > 0x3fffffffu)
+      return fail(c, TX_EINVAL, "attention_scored: too many rows");
+    if (l->cu && l->lengths)
+      return fail(c, TX_EINVAL, "attention_scored: cu and lengths exclude one another");
+    if (!l->cu && (uint64_t)nseq * l->max_len > l->rows)
+      return fail(c, TX_EINVAL, "attention_scored: nseq * max_len exceeds the rows");
+  }
+  // Key tiles of a document mask are kept as bits on chip.
+  if (r.k_docs && k_layout->max_len > 128u * 32768u)
+    return fail(c, TX_EINVAL, "attention_scored: documents with at most 2^22 keys");
+  const size_t ei = in_dtype == TX_BF16 ? 2 : 4, eo = out_dtype == TX_BF16 ? 2 : 4;
+  if ((uintptr_t)q->data % ei || (uintptr_t)k->data % ei || (uintptr_t)v->data % ei ||
+      (uintptr_t)out % eo)
+    return fail(c, TX_EINVAL, "attention_scored: misaligned pointer");
+  if (!nseq || !q_layout->max_len || !q_layout->rows) return TX_OK;
+  tx::ScoredProblem p{};
+  p.q = q->data; p.k = k->data; p.v = v->data; p.out = out;
+  p.q_row = q->row_stride; p.k_row = k->row_stride; p.v_row = v->row_stride;
+  // The stride between heads says nothing where there is one.
+  p.q_head = heads == 1 ? dim : q->head_stride;
+  p.k_head = kv_heads == 1 ? dim : k->head_stride;
+  p.v_head = kv_heads == 1 ? dim : v->head_stride;
+  p.cu_q = q_layout->cu; p.cu_k = k_layout->cu;
+  p.q_lengths = q_layout->lengths; p.k_lengths = k_layout->lengths;
+  p.nseq = nseq; p.rows_q = q_layout->rows; p.rows_k = k_layout->rows;
+  p.max_q = q_layout->max_len; p.max_k = k_layout->max_len;
+  p.heads = heads; p.kv_heads = kv_heads; p.dim = dim;
+  p.in_dtype = in_dtype; p.out_dtype = out_dtype; p.scale = scale;
+  p.softcap = r.softcap; p.slopes = r.slopes; p.table = r.distance_bias; p.reach = (int)r.reach;
+  p.causal = r.causal ? 1 : 0;
+  p.left = r.window_left < 0 ? -1 : r.window_left;
+  p.right = r.window_right < 0 ? -1 : r.window_right;
+  p.prefix = r.prefix; p.q_docs = r.q_docs; p.k_docs = r.k_docs;
+  p.status = c->status;
+  p.wait_cycles = c->wait_cycles > 0 ? c->wait_cycles : 2000000000ll;
+  const bool tc = k_layout->rows && tx::scored_tc_supported(p);
+  tx::scored_plan(&p, tc, c->sms);
+  const uint64_t units = (uint64_t)p.tiles * nseq * (heads / p.pack);
+  if (units * p.splits > 0x7fffffffull)
+    return fail(c, TX_EINVAL, "attention_scored: problem too large");
+  cudaError_t e = cudaSetDevice(c->device);
+  if (e != cudaSuccess) return cuda_fail(c, e, "cudaSetDevice");
+  cudaStream_t st = stream ? (cudaStream_t)stream : c->stream;
+  if (p.splits > 1) {
+    const size_t rows = (size_t)units * p.splits * p.rows;
+    if ((e = ensure_parts(c, units, rows * ((size_t)p.part_dp * 4 + 8))) != cudaSuccess)
+      return cuda_fail(c, e, "partial sums allocation");
+    const size_t counters = (c->part_units * 4 + 255) & ~(size_t)255;
+    p.part_arrived = (uint32_t *)c->part_mem;
+    p.part_o = (float *)(c->part_mem + counters);
+    p.part_ml = (float2 *)(c->part_mem + counters + rows * p.part_dp * 4);
+    if ((e = scratch_acquire(c, st)) != cudaSuccess) return cuda_fail(c, e, "scratch wait");
+  }
+  e = tc ? tx::launch_scored_tc(p, st) : tx::launch_scored_f32(p, st);
+  if (e != cudaSuccess) return cuda_fail(c, e, "attention_scored launch");
+  if (p.splits > 1 && (e = scratch_release(c, st)) != cudaSuccess)
+    return cuda_fail(c, e, "scratch event");
+  c->last_kernel = tc ? "scored_tc" : "scored_f32";
   ++c->launches;
   return TX_OK;
 }

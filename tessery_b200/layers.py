@@ -160,3 +160,100 @@ def rotary(
     rt.sync()
     return (_read(rt, q_out, q.shape, out_code),
             None if k is None else _read(rt, k_out, k.shape, out_code))
+
+
+def attention_scored(
+    q: NDArray,
+    k: NDArray,
+    v: NDArray,
+    *,
+    cu_q: NDArray | None = None,
+    cu_k: NDArray | None = None,
+    q_lengths: NDArray | None = None,
+    k_lengths: NDArray | None = None,
+    scale: float | None = None,
+    causal: bool = True,
+    window: tuple[int, int] = (-1, -1),
+    softcap: float = 0.0,
+    slopes: NDArray | None = None,
+    distance_bias: NDArray | None = None,
+    prefix: NDArray | None = None,
+    q_docs: NDArray | None = None,
+    k_docs: NDArray | None = None,
+    out_dtype: str | None = None,
+    runtime: CudaRuntime | None = None,
+) -> NDArray:
+    """Attention under a score rule (tx_attention_scored).
+
+    Packed: q [Tq, H, d] with cu_q, k/v [Tk, Hkv, d] with cu_k (cu_k None: cu_q's).
+    Padded: q [B, Lq, H, d], k/v [B, Lk, Hkv, d] with lengths (None: all rows valid).
+    A sequence's queries are its last positions.  slopes [H]; distance_bias [H, 2R + 1];
+    prefix [B]; q_docs / k_docs int32 per row in q's / k's row layout (q_docs alone serves
+    both where the rows are the same).  Returns q's layout in q's dtype or `out_dtype`."""
+    rt = runtime or default_runtime()
+    q, k, v = (np.ascontiguousarray(a) for a in (q, k, v))
+    code = _dtype_code(q)
+    if _dtype_code(k) != code or _dtype_code(v) != code or k.shape != v.shape:
+        raise InvalidInputError()
+    out_code = _out_code(out_dtype, code)
+    packed = cu_q is not None
+    if q.ndim != (3 if packed else 4) or k.ndim != q.ndim or k.shape[-1] != q.shape[-1]:
+        raise InvalidInputError()
+    heads, dim = q.shape[-2:]
+    if slopes is not None and np.shape(slopes) != (heads,):
+        raise InvalidInputError()
+    if distance_bias is not None and (np.ndim(distance_bias) != 2 or distance_bias.shape[0] != heads
+                                      or distance_bias.shape[1] % 2 == 0):
+        raise InvalidInputError()
+    if q_docs is not None and k_docs is None:
+        k_docs = q_docs
+    kw: dict = {}
+
+    def layout(side: str, x: NDArray, cu, lengths) -> int:
+        """Uploads one side's layout; returns its number of sequences."""
+        if packed:
+            cu = np.ascontiguousarray(cu, dtype=np.int32)
+            if (lengths is not None or cu.ndim != 1 or cu.size < 2 or cu[0] != 0
+                    or cu[-1] != x.shape[0] or np.any(np.diff(cu) < 0)):
+                raise InvalidInputError()
+            kw["cu_" + side] = _upload(rt, "scored_cu_" + side, cu)
+            kw["rows_" + side], kw["max_" + side] = x.shape[0], int(np.diff(cu).max())
+            return cu.size - 1
+        if cu is not None:
+            raise InvalidInputError()
+        if lengths is not None:
+            n = np.ascontiguousarray(lengths, dtype=np.int32)
+            if n.shape != x.shape[:1] or np.any(n < 0) or np.any(n > x.shape[1]):
+                raise InvalidInputError()
+            kw[side + "_lengths"] = _upload(rt, f"scored_{side}_lengths", n) if n.size else None
+        kw["rows_" + side], kw["max_" + side] = x.shape[0] * x.shape[1], x.shape[1]
+        return x.shape[0]
+
+    nseq = layout("q", q, cu_q, q_lengths)
+    if layout("k", k, cu_q if packed and cu_k is None else cu_k, k_lengths) != nseq:
+        raise InvalidInputError()
+    if prefix is not None and np.shape(prefix) != (nseq,):
+        raise InvalidInputError()
+    for name, docs, x in (("q_docs", q_docs, q), ("k_docs", k_docs, k)):
+        if docs is not None:
+            docs = np.ascontiguousarray(docs, dtype=np.int32)
+            if docs.shape != x.shape[:-2]:
+                raise InvalidInputError()
+            kw[name] = _upload(rt, "scored_" + name, docs) if docs.size else None
+    if not q.size:
+        return np.empty(q.shape, _NP[out_code])
+    for name, a in (("slopes", slopes), ("distance_bias", distance_bias)):
+        if a is not None:
+            kw[name] = _upload(rt, "scored_" + name, np.ascontiguousarray(a, dtype=np.float32))
+    if prefix is not None:
+        kw["prefix"] = _upload(rt, "scored_prefix", np.ascontiguousarray(prefix, dtype=np.int32))
+    if not k.size:  # nothing to attend: every row is empty
+        return np.zeros(q.shape, _NP[out_code])
+    out = rt.workspace("scored_out", q.size * (4 if out_code == native.TX_F32 else 2))
+    rt.attention_scored_device(
+        _upload(rt, "scored_q", q), _upload(rt, "scored_k", k), _upload(rt, "scored_v", v),
+        out.device_ptr, nseq=nseq, heads=heads, kv_heads=k.shape[-2], dim=dim, in_dtype=code,
+        out_dtype=out_code, scale=scale, causal=causal, window=window, softcap=softcap,
+        reach=0 if distance_bias is None else distance_bias.shape[1] // 2, **kw)
+    rt.sync()
+    return _read(rt, out, q.shape, out_code)

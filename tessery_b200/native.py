@@ -78,6 +78,28 @@ class TxRotaryTensor(ct.Structure):
     ]
 
 
+class TxScoreRule(ct.Structure):
+    """The rule of tx_attention_scored (TxScoreRule in tessattn.h)."""
+
+    _fields_ = [
+        ("softcap", _f32), ("slopes", _vp), ("distance_bias", _vp), ("reach", _u32),
+        ("causal", _i32), ("window_left", ct.c_int32), ("window_right", ct.c_int32),
+        ("prefix", _vp), ("q_docs", _vp), ("k_docs", _vp),
+    ]
+
+
+class TxRows(ct.Structure):
+    """Rows of q, k or v with strides (TxRows in tessattn.h)."""
+
+    _fields_ = [("data", _vp), ("row_stride", _u64), ("head_stride", _u64)]
+
+
+class TxLayout(ct.Structure):
+    """Where the sequences lie (TxLayout in tessattn.h)."""
+
+    _fields_ = [("cu", _vp), ("lengths", _vp), ("rows", _u32), ("max_len", _u32)]
+
+
 SIGNATURES: dict[str, tuple[list[Any], Any]] = {
     "tx_abi_version": ([], _u32),
     "tx_create": ([_i32], _vp),
@@ -157,6 +179,10 @@ SIGNATURES: dict[str, tuple[list[Any], Any]] = {
     "tx_rotary": (
         [_vp, ct.POINTER(TxRotaryTensor), ct.POINTER(TxRotaryTensor), _i32, _i32, _u32, _u32,
          _u32, _i32, _i32, _vp, _vp, _u32, _u32, _vp, _f32, _f32, _vp], _i32),
+    "tx_attention_scored": (
+        [_vp, ct.POINTER(TxRows), ct.POINTER(TxRows), ct.POINTER(TxRows), _vp,
+         ct.POINTER(TxLayout), ct.POINTER(TxLayout), _u32, _u32, _u32, _u32, _i32, _i32, _f32,
+         ct.POINTER(TxScoreRule), _vp], _i32),
     "tx_attention_padded_noalloc": (
         [_vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _i32, _i32, _f32, _vp, _f32,
          _f32, _vp, _vp],

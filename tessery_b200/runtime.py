@@ -760,6 +760,67 @@ class CudaRuntime:
             dim if rot_dim is None else rot_dim, int(bool(interleaved)), int(bool(inverse)),
             positions, cu_seqlens, nseq, seq, inv_freq, amplitude, eps, stream))
 
+    def attention_scored_device(
+        self,
+        q: int,
+        k: int,
+        v: int,
+        out: int,
+        *,
+        nseq: int,
+        rows_q: int,
+        rows_k: int,
+        max_q: int,
+        max_k: int,
+        heads: int,
+        kv_heads: int,
+        dim: int,
+        cu_q: int | None = None,
+        cu_k: int | None = None,
+        q_lengths: int | None = None,
+        k_lengths: int | None = None,
+        in_dtype: int = native.TX_BF16,
+        out_dtype: int = native.TX_BF16,
+        scale: float | None = None,
+        causal: bool = True,
+        window: tuple[int, int] = (-1, -1),
+        softcap: float = 0.0,
+        slopes: int | None = None,
+        distance_bias: int | None = None,
+        reach: int = 0,
+        prefix: int | None = None,
+        q_docs: int | None = None,
+        k_docs: int | None = None,
+        q_strides: Sequence[int] | None = None,
+        k_strides: Sequence[int] | None = None,
+        v_strides: Sequence[int] | None = None,
+        stream: int | None = None,
+    ) -> None:
+        """Queues attention under a score rule (tx_attention_scored): a tanh cap, a bias by
+        distance (per-head slopes, or a table of 2 * reach + 1 values per head), causal order,
+        a (left, right) window, an open prefix per sequence, documents per row.  Packed rows
+        (cu_q, cu_k) or sequences of max_q / max_k rows (q_lengths, k_lengths); with fewer
+        query rows than keys the queries are the last positions.  Strides are (row, head) in
+        elements, contiguous by default."""
+        self._check_open()
+
+        def rows(x, n, strides):
+            r, h = (n * dim, dim) if strides is None else strides
+            if r < 0 or h < 0:
+                raise InvalidInputError()
+            return native.TxRows(x, r, h)
+
+        if min(nseq, rows_q, rows_k, max_q, max_k, reach) < 0 or dim < 1:
+            raise InvalidInputError()
+        rule = native.TxScoreRule(softcap, slopes, distance_bias, reach, int(bool(causal)),
+                                  max(int(window[0]), -1), max(int(window[1]), -1), prefix,
+                                  q_docs, k_docs)
+        _raise_for(self._lib.tx_attention_scored(
+            self._pointer, rows(q, heads, q_strides), rows(k, kv_heads, k_strides),
+            rows(v, kv_heads, v_strides), out, native.TxLayout(cu_q, q_lengths, rows_q, max_q),
+            native.TxLayout(cu_k, k_lengths, rows_k, max_k), nseq, heads, kv_heads, dim, in_dtype,
+            out_dtype, dim**-0.5 if scale is None else scale, rule, stream))
+
     def sync(self, stream: int | None = None) -> None:
         """Waits for queued work and reports kernel errors (tx_sync)."""
         self._check_open()
