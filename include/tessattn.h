@@ -488,6 +488,25 @@ int tx_attention_scored(void *ctx, const TxRows *q, const TxRows *k, const TxRow
                         uint32_t heads, uint32_t kv_heads, uint32_t dim, int in_dtype,
                         int out_dtype, float scale, const TxScoreRule *rule, void *stream);
 
+/* Activations of tx_linear_fused. */
+enum {
+  TX_ACT_NONE = 0,
+  TX_ACT_RELU = 1,
+  TX_ACT_GELU = 2,      /* y (1 + erf(y / sqrt 2)) / 2 */
+  TX_ACT_GELU_TANH = 3, /* y (1 + tanh(sqrt(2 / pi) (y + 0.044715 y^3))) / 2 */
+  TX_ACT_SILU = 4       /* y / (1 + exp(-y)) */
+};
+
+/* out = act(x w^T + bias) + residual: x [m, k] and w [n, k] bf16 with row strides ldx, ldw
+ * (elements), sums in fp32, bias fp32 [n] or NULL, residual [m, n] (TX_F32 or TX_BF16, row
+ * stride ldr) or NULL, out [m, n] (TX_F32 or TX_BF16, row stride ldo), rounded once.  residual
+ * may be out (same dtype and stride).  Any m, n, k; x and w 16-byte aligned with ldx and ldw
+ * multiples of 8 (columns past k may hold anything). */
+int tx_linear_fused(void *ctx, const void *x, uint64_t ldx, const void *w, uint64_t ldw,
+                    const float *bias, const void *residual, int residual_dtype, uint64_t ldr,
+                    void *out, int out_dtype, uint64_t ldo, uint32_t m, uint32_t n, uint32_t k,
+                    int activation, void *stream);
+
 /* ---- the BERT (BGE-small) fp32 forward around the head_dim-32 attention -------------
 
  * BertBackend.forward (bert.py:104-235) is built from these plus tx_linear (fmt TX_F32,

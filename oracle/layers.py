@@ -94,3 +94,27 @@ def attention_scored(q: NDArray, k: NDArray, v: NDArray, *, scale=None, softcap=
                 out[i, h] = p @ vh[at]
                 mass[i, h] = p @ np.abs(vh[at])
     return out, mass, biggest
+
+
+def activate(y: NDArray, name: str) -> NDArray:
+    if name == "none":
+        return y
+    if name == "relu":
+        return np.maximum(y, 0.0)
+    if name == "gelu":
+        return y * 0.5 * (1.0 + _erf(y / math.sqrt(2.0)))
+    if name == "gelu_tanh":
+        return y * 0.5 * (1.0 + np.tanh(math.sqrt(2.0 / math.pi) * (y + 0.044715 * y**3)))
+    if name == "silu":
+        return y / (1.0 + np.exp(-y))
+    raise ValueError(name)
+
+
+def linear_fused(x: NDArray, w: NDArray, *, bias=None, activation="none",
+                 residual=None) -> NDArray:
+    """act(x w^T + bias) + residual of float values."""
+    y = np.asarray(x, np.float64) @ np.asarray(w, np.float64).T
+    if bias is not None:
+        y = y + bias
+    y = activate(y, activation)
+    return y if residual is None else y + residual

@@ -213,6 +213,21 @@ cudaError_t launch_scored_tc(const ScoredProblem &p, cudaStream_t stream);
 cudaError_t launch_scored_f32(const ScoredProblem &p, cudaStream_t stream);
 cudaError_t launch_rotary(const RotaryProblem &p, cudaStream_t stream);
 
+// out = act(x w^T + bias) + residual; row strides in elements.
+struct LinearFusedProblem {
+  const void *x, *w;
+  const float *bias;
+  const void *residual;
+  void *out;
+  uint64_t ldx, ldw, ldr, ldo;
+  uint32_t m, n, k;
+  int residual_dtype, out_dtype, act;
+  bool out_vec, res_vec;  // rows on 16-byte boundaries (set by the launcher)
+  int *status;
+  long long wait_cycles;
+};
+cudaError_t launch_linear_fused(LinearFusedProblem p, int num_sms, cudaStream_t stream);
+
 // ---- BERT fp32 forward (bert_ops.cu) ----
 // Word + token-type-0 + absolute-position embeddings of `tokens` tokens, LayerNorm'd; the
 // position of a token is its index inside its packed sequence (cu, nseq) or t % seq.

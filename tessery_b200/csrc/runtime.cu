@@ -1808,6 +1808,48 @@ int tx_attention_scored(void *ctx, const TxRows *q, const TxRows *k, const TxRow
   return TX_OK;
 }
 
+int tx_linear_fused(void *ctx, const void *x, uint64_t ldx, const void *w, uint64_t ldw,
+                    const float *bias, const void *residual, int residual_dtype, uint64_t ldr,
+                    void *out, int out_dtype, uint64_t ldo, uint32_t m, uint32_t n, uint32_t k,
+                    int activation, void *stream) {
+  Ctx *c = (Ctx *)ctx;
+  if (!c) return TX_EINVAL;
+  std::lock_guard<std::recursive_mutex> g(c->mu);
+  if (!x || !w || !out) return fail(c, TX_EINVAL, "linear_fused: null pointer");
+  if ((out_dtype != TX_F32 && out_dtype != TX_BF16) ||
+      (residual && residual_dtype != TX_F32 && residual_dtype != TX_BF16))
+    return fail(c, TX_EINVAL, "linear_fused: bad dtype");
+  if (activation < TX_ACT_NONE || activation > TX_ACT_SILU)
+    return fail(c, TX_EINVAL, "linear_fused: bad activation");
+  if (!n || !k) return fail(c, TX_EINVAL, "linear_fused: n and k must be positive");
+  if (m > 0x7fffff00u || n > 0x7fffff00u || k > 0x7fffff00u)
+    return fail(c, TX_EINVAL, "linear_fused: sizes below 2^31");
+  const uint64_t most = 1ull << 38;
+  if (ldx < k || ldw < k || ldo < n || (residual && ldr < n) || ldx > most || ldw > most ||
+      ldo > most || (residual && ldr > most))
+    return fail(c, TX_EINVAL, "linear_fused: a row stride is shorter than its row");
+  if (ldx % 8 || ldw % 8 || (uintptr_t)x % 16 || (uintptr_t)w % 16)
+    return fail(c, TX_EINVAL, "linear_fused: rows of x and w on 16-byte boundaries");
+  const size_t eo = out_dtype == TX_BF16 ? 2 : 4, er = residual_dtype == TX_BF16 ? 2 : 4;
+  if ((uintptr_t)out % eo || (uintptr_t)bias % 4 || (residual && (uintptr_t)residual % er))
+    return fail(c, TX_EINVAL, "linear_fused: misaligned pointer");
+  if (residual == out && residual && (residual_dtype != out_dtype || ldr != ldo))
+    return fail(c, TX_EINVAL, "linear_fused: in place needs equal dtypes and strides");
+  if (!m) return TX_OK;
+  tx::LinearFusedProblem p{};
+  p.x = x; p.w = w; p.bias = bias; p.residual = residual; p.out = out;
+  p.ldx = ldx; p.ldw = ldw; p.ldr = ldr; p.ldo = ldo; p.m = m; p.n = n; p.k = k;
+  p.residual_dtype = residual_dtype; p.out_dtype = out_dtype; p.act = activation;
+  p.status = c->status;
+  p.wait_cycles = c->wait_cycles > 0 ? c->wait_cycles : 2000000000ll;
+  cudaSetDevice(c->device);
+  cudaError_t e = tx::launch_linear_fused(p, c->sms, stream ? (cudaStream_t)stream : c->stream);
+  if (e != cudaSuccess) return cuda_fail(c, e, "linear_fused launch");
+  c->last_kernel = "linear_fused";
+  ++c->launches;
+  return TX_OK;
+}
+
 int tx_device_count(void) {
   int n = 0;
   return cudaGetDeviceCount(&n) == cudaSuccess && n > 0 ? n : 0;

@@ -257,3 +257,53 @@ def attention_scored(
         reach=0 if distance_bias is None else distance_bias.shape[1] // 2, **kw)
     rt.sync()
     return _read(rt, out, q.shape, out_code)
+
+
+def linear_fused(
+    x: NDArray,
+    w: NDArray,
+    *,
+    bias: NDArray | None = None,
+    activation: str = "none",
+    residual: NDArray | None = None,
+    out_dtype: str = "bf16",
+    runtime: CudaRuntime | None = None,
+) -> NDArray:
+    """act(x w^T + bias) + residual (tx_linear_fused): x [m, k] and w [n, k] bf16 bits, bias
+    [n], residual [m, n] float32 or bf16 bits; activation none, relu, gelu, gelu_tanh, silu."""
+    rt = runtime or default_runtime()
+    x, w = np.asarray(x), np.asarray(w)
+    if (x.ndim != 2 or w.ndim != 2 or x.shape[1] != w.shape[1] or x.dtype != np.uint16
+            or w.dtype != np.uint16 or not w.size):
+        raise InvalidInputError()
+    (m, k), n = x.shape, w.shape[0]
+    out_code = _out_code(out_dtype, native.TX_BF16)
+    res_code = native.TX_F32
+    if bias is not None and np.shape(bias) != (n,):
+        raise InvalidInputError()
+    if residual is not None:
+        residual = np.ascontiguousarray(residual)
+        res_code = _dtype_code(residual)
+        if residual.shape != (m, n):
+            raise InvalidInputError()
+    if activation not in native.ACTIVATIONS:
+        raise InvalidInputError()
+    if not m:
+        return np.empty((m, n), _NP[out_code])
+    ld = -(-k // 8) * 8  # rows on 16-byte boundaries
+
+    def rows(name: str, a: NDArray) -> int:
+        padded = np.zeros((a.shape[0], ld), np.uint16)
+        padded[:, :k] = a
+        return _upload(rt, name, padded)
+
+    out = rt.workspace("linear_out", m * n * (4 if out_code == native.TX_F32 else 2))
+    rt.linear_fused_device(
+        rows("linear_x", x), rows("linear_w", w), out.device_ptr, m=m, n=n, k=k, ldx=ld, ldw=ld,
+        bias=None if bias is None else _upload(rt, "linear_bias",
+                                               np.ascontiguousarray(bias, np.float32)),
+        activation=activation,
+        residual=None if residual is None else _upload(rt, "linear_residual", residual),
+        residual_dtype=res_code, out_dtype=out_code)
+    rt.sync()
+    return _read(rt, out, (m, n), out_code)

@@ -23,6 +23,7 @@ TX_OK, TX_EINVAL, TX_ECUDA, TX_ETIMEOUT = 0, 1, 2, 3
 TX_F32, TX_BF16, TX_BF16X2 = 0, 1, 2
 TX_LINEAR_STORE_F32, TX_LINEAR_STORE_BF16, TX_LINEAR_ADD_F32, TX_LINEAR_GATED_BF16 = 0, 1, 2, 3
 TX_LINEAR_GELU_SPLIT = 4
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}  # TX_ACT_*
 
 _vp, _u32, _u64, _i32, _f32 = ct.c_void_p, ct.c_uint32, ct.c_uint64, ct.c_int, ct.c_float
 
@@ -183,6 +184,9 @@ SIGNATURES: dict[str, tuple[list[Any], Any]] = {
         [_vp, ct.POINTER(TxRows), ct.POINTER(TxRows), ct.POINTER(TxRows), _vp,
          ct.POINTER(TxLayout), ct.POINTER(TxLayout), _u32, _u32, _u32, _u32, _i32, _i32, _f32,
          ct.POINTER(TxScoreRule), _vp], _i32),
+    "tx_linear_fused": (
+        [_vp, _vp, _u64, _vp, _u64, _vp, _vp, _i32, _u64, _vp, _i32, _u64, _u32, _u32, _u32,
+         _i32, _vp], _i32),
     "tx_attention_padded_noalloc": (
         [_vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _i32, _i32, _f32, _vp, _f32,
          _f32, _vp, _vp],

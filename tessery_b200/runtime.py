@@ -821,6 +821,40 @@ class CudaRuntime:
             native.TxLayout(cu_k, k_lengths, rows_k, max_k), nseq, heads, kv_heads, dim, in_dtype,
             out_dtype, dim**-0.5 if scale is None else scale, rule, stream))
 
+    def linear_fused_device(
+        self,
+        x: int,
+        w: int,
+        out: int,
+        *,
+        m: int,
+        n: int,
+        k: int,
+        ldx: int | None = None,
+        ldw: int | None = None,
+        ldr: int | None = None,
+        ldo: int | None = None,
+        bias: int | None = None,
+        activation: str = "none",
+        residual: int | None = None,
+        residual_dtype: int = native.TX_F32,
+        out_dtype: int = native.TX_BF16,
+        stream: int | None = None,
+    ) -> None:
+        """Queues out = act(x w^T + bias) + residual (tx_linear_fused): x [m, k] and w [n, k]
+        bf16 with row strides ldx, ldw (multiples of 8; k by default), bias fp32 [n], residual
+        and out [m, n] fp32 or bf16 with row strides ldr, ldo (n by default); activation none,
+        relu, gelu, gelu_tanh or silu.  residual may be out."""
+        self._check_open()
+        act = native.ACTIVATIONS.get(activation)
+        ldx, ldw = k if ldx is None else ldx, k if ldw is None else ldw
+        ldr, ldo = n if ldr is None else ldr, n if ldo is None else ldo
+        if act is None or min(m, n, k, ldx, ldw, ldr, ldo) < 0:
+            raise InvalidInputError()
+        _raise_for(self._lib.tx_linear_fused(
+            self._pointer, x, ldx, w, ldw, bias, residual, residual_dtype, ldr, out, out_dtype, ldo,
+            m, n, k, act, stream))
+
     def sync(self, stream: int | None = None) -> None:
         """Waits for queued work and reports kernel errors (tx_sync)."""
         self._check_open()

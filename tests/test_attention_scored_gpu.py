@@ -364,3 +364,18 @@ def test_refusals(runtime):
         runtime.attention_scored_device(p, None, p, p, **ok)
     runtime.sync()
     b.close()
+
+
+def test_wait_limit_is_reported_and_the_runtime_goes_on(runtime):
+    """Waits that run out end the kernel with a status; a split call after it joins its parts as
+    ever (the arrival counters have returned to zero)."""
+    from tessery_b200 import DeviceTimeoutError
+
+    runtime.set_wait_limit(1)
+    try:
+        for lens_q, lens_k in (([300], [300]), ([1, 1], [3000, 900])):
+            with pytest.raises(DeviceTimeoutError):
+                run_packed(runtime, lens_q, lens_k, 4, 2, 128, "bf16")
+    finally:
+        runtime.set_wait_limit(0)
+    run_packed(runtime, [1, 1], [3000, 900], 4, 2, 128, "bf16", route="scored_tc")
