@@ -222,11 +222,12 @@ struct LinearFusedProblem {
   uint64_t ldx, ldw, ldr, ldo;
   uint32_t m, n, k;
   int residual_dtype, out_dtype, act;
-  bool out_vec, res_vec;  // rows on 16-byte boundaries (set by the launcher)
+  bool out_vec, res_vec, bias_vec;  // on 16-byte boundaries; epilogue: set by the launcher
+  int epilogue;
   int *status;
   long long wait_cycles;
 };
-cudaError_t launch_linear_fused(LinearFusedProblem p, int num_sms, cudaStream_t stream);
+cudaError_t launch_linear_fused(const LinearFusedProblem &p, int num_sms, cudaStream_t stream);
 
 // ---- BERT fp32 forward (bert_ops.cu) ----
 // Word + token-type-0 + absolute-position embeddings of `tokens` tokens, LayerNorm'd; the

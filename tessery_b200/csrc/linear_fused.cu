@@ -4,8 +4,10 @@
 //
 // linear_kernel: 128 x BN tiles on tcgen05 (kind::f16), K through a ring of 64-column stages
 // filled by TMA (128-byte swizzle; rows past m or n and columns past k arrive as zeros), two
-// accumulators in tensor memory so that four epilogue warps finish one tile while the next is
-// multiplied; persistent, one CTA per SM.
+// accumulators in tensor memory so that eight epilogue warps finish one tile while the next is
+// multiplied; persistent, one CTA per SM.  Results leave through shared memory and TMA stores
+// (whole 128-byte rows; a thread that stored its own row directly wrote 16 bytes to each of 32
+// rows per instruction), and a residual of the output's type comes in the same way, a box ahead.
 // gemv_kernel: a few rows (m <= 8) only stream w once: a warp per output column, w straight from
 // global memory into registers, the sums over lanes by shuffles.
 #include <cuda.h>
@@ -25,26 +27,33 @@ using namespace ptx;
 
 constexpr int kBM = 128;
 constexpr uint32_t kBK = 64;
-constexpr int kThreads = 192;  // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue
+constexpr int kThreads = 320;  // warp 0 TMA, warp 1 MMA, warps 2-9 epilogue
 constexpr int kMaxStages = 8;
+constexpr uint32_t kPart = 8;  // K stages (512 columns) of one partial sum
+constexpr uint32_t kBufBytes = 32 * 128;  // staging: 32 rows x 128 bytes, two per epilogue warp
 constexpr long long kDrainCycles = 2000000000ll;
 
 template <int kBN>
 struct Cfg {
   static constexpr uint32_t kABytes = kBM * 128, kBBytes = kBN * 128;
   static constexpr uint32_t kStageBytes = kABytes + kBBytes;
-  static constexpr int kFit = (int)((232448 - 1024) / kStageBytes);
+  static constexpr uint32_t kStaging = kBN >= 128 ? 8 * 2 * kBufBytes : 0;
+  static constexpr int kFit = (int)((232448 - 1024 - kStaging) / kStageBytes);
   static constexpr int kStages = kFit < kMaxStages ? kFit : kMaxStages;
-  static constexpr uint32_t kOffMisc = kStages * kStageBytes;
-  static constexpr uint32_t kSmemBytes = kOffMisc + 256;
+  static constexpr uint32_t kOffStaging = kStages * kStageBytes;
+  static constexpr uint32_t kOffMisc = kOffStaging + kStaging;
+  static constexpr uint32_t kSmemBytes = kOffMisc + 512;
   static constexpr uint32_t kTmemCols = 2 * kBN;
   static constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) |
                                      ((uint32_t)(kBN >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);
 };
 enum : uint32_t { kBarFull = 0, kBarEmpty = kMaxStages, kBarAcc = 2 * kMaxStages,
-                  kBarFree = kBarAcc + 2, kBarDrain = kBarFree + 2, kNumBars = kBarDrain + 1 };
+                  kBarFree = kBarAcc + 2, kBarDrain = kBarFree + 2,
+                  kBarRes = kBarDrain + 1,  // + 2 * epilogue warp + buffer: residual landed
+                  kNumBars = kBarRes + 16 };
 enum : uint32_t { kOffTmem = 8 * kNumBars, kOffAbort = kOffTmem + 4 };
-enum : int { kSiteEmpty = 1, kSiteFull = 2, kSiteAcc = 3, kSiteFree = 4 };
+static_assert(kOffAbort + 4 <= 512, "misc area");
+enum : int { kSiteEmpty = 1, kSiteFull = 2, kSiteAcc = 3, kSiteFree = 4, kSiteRes = 5 };
 
 __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile int *abort_flag,
                                          int *status, int site, long long limit) {
@@ -65,19 +74,44 @@ __device__ __forceinline__ void drain_bar(uint32_t bar, uint32_t parity) {
   while (!mbar_test(bar, parity) && clock64() - t0 < kDrainCycles) {
   }
 }
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, uint32_t src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(src), "r"(x), "r"(y)
+               : "memory");
+}
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
-__device__ __forceinline__ float activate(float y, int act) {
-  switch (act) {
-    case TX_ACT_RELU:
-      return y < 0.f ? 0.f : y;
-    case TX_ACT_GELU:
-      return 0.5f * y * (1.f + erff(y * 0.70710678118654752f));
-    case TX_ACT_GELU_TANH:  // (1 + tanh u) / 2 = 1 / (1 + e^(-2u))
-      return __fdividef(y, 1.f + __expf(-1.5957691216057308f * (y + 0.044715f * y * y * y)));
-    case TX_ACT_SILU:
-      return __fdividef(y, 1.f + __expf(-y));
-    default:
-      return y;
+// The hardware exponential and reciprocal (2^-22 of the value each) in place of exp and a
+// division: the epilogue's arithmetic is what bounds a layer of small k.
+template <int kAct>
+__device__ __forceinline__ float activate(float y) {
+  constexpr float kLog2e = 1.44269504088896341f;
+  if constexpr (kAct == TX_ACT_RELU) {
+    return y < 0.f ? 0.f : y;
+  } else if constexpr (kAct == TX_ACT_GELU) {
+    // 1 - erf(z), z = |y| / sqrt 2, as t P(t) exp(-z^2) with t = 1 / (1 + 0.3275911 z)
+    // (Abramowitz and Stegun 7.1.26, absolute error 1.5e-7); gelu = y - y tail / 2 for y > 0
+    // and y tail / 2 below, so the negative side does not cancel.
+    const float z = fabsf(y) * 0.70710678118654752f;
+    const float t = rcp(fmaf(0.3275911f, z, 1.f));
+    float q = fmaf(t, 1.061405429f, -1.453152027f);
+    q = fmaf(t, q, 1.421413741f);
+    q = fmaf(t, q, -0.284496736f);
+    q = fmaf(t, q, 0.254829592f) * t;
+    const float half = 0.5f * y * (q * ex2(z * z * -kLog2e));
+    return y > 0.f ? y - half : half;
+  } else if constexpr (kAct == TX_ACT_GELU_TANH) {  // (1 + tanh u) / 2 = 1 / (1 + e^(-2u))
+    const float u = y * fmaf(0.044715f, y * y, 1.f);
+    return y * rcp(1.f + ex2(u * (-1.5957691216057308f * kLog2e)));
+  } else if constexpr (kAct == TX_ACT_SILU) {
+    return y * rcp(1.f + ex2(y * -kLog2e));
+  } else {
+    return y;
   }
 }
 
@@ -92,9 +126,18 @@ __device__ __forceinline__ void store_at(const LinearFusedProblem &p, size_t i, 
     static_cast<float *>(p.out)[i] = v;
 }
 
-template <int kBN>
+// How the epilogue reaches global memory, chosen by the launcher.
+enum : int {
+  kDirect = 0,   // element by element or 16 bytes at a time, a thread per row
+  kStaged = 1,   // results through shared memory and TMA stores, the residual read directly
+  kStagedRes = 2 // the residual too: loaded by TMA into the buffer its sum leaves from
+};
+
+template <int kBN, int kAct>
 __global__ void __launch_bounds__(kThreads, 1)
     linear_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
+                  const __grid_constant__ CUtensorMap tm_res,
+                  const __grid_constant__ CUtensorMap tm_out,
                   const __grid_constant__ LinearFusedProblem p) {
   using C = Cfg<kBN>;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -103,7 +146,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + C::kOffMisc + kOffAbort);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t nt = (p.n + kBN - 1) / kBN, mt = (p.m + kBM - 1) / kBM, tiles = nt * mt;
-  const uint32_t nk = (p.k + kBK - 1) / kBK;
+  const uint32_t nk = (p.k + kBK - 1) / kBK, parts = (nk + kPart - 1) / kPart;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
@@ -112,9 +155,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(bar(kBarAcc + b), 1);
-      mbar_init(bar(kBarFree + b), 128);
+      mbar_init(bar(kBarFree + b), 256);
     }
     mbar_init(bar(kBarDrain), 1);
+    for (int b = 0; b < 16; ++b) mbar_init(bar(kBarRes + b), 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -155,113 +199,243 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else if (warp == 1) {
     if (lane == 0) {
-      uint32_t step = 0, done = 0;
+      uint32_t step = 0, done = 0;  // K stages, partial sums
       bool ok = true;
-      for (uint32_t tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, ++done) {
-        const uint32_t b = done & 1, acc = tmem + b * kBN;
-        if (done >= 2 && !(ok = wait_bar(bar(kBarFree + b), ((done >> 1) - 1) & 1, abort_flag,
-                                         p.status, kSiteFree, p.wait_cycles)))
-          break;
-        tc_fence_after();
-        for (uint32_t kb = 0; kb < nk; ++kb, ++step) {
-          const uint32_t s = step % C::kStages;
-          if (!(ok = wait_bar(bar(kBarFull + s), (step / C::kStages) & 1, abort_flag, p.status,
-                              kSiteFull, p.wait_cycles)))
+      for (uint32_t tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
+        for (uint32_t kb = 0; ok && kb < nk; ++done) {
+          const uint32_t b = done & 1, acc = tmem + b * kBN;
+          if (done >= 2 && !(ok = wait_bar(bar(kBarFree + b), ((done >> 1) - 1) & 1, abort_flag,
+                                           p.status, kSiteFree, p.wait_cycles)))
             break;
           tc_fence_after();
-          const uint32_t st = sbase + s * C::kStageBytes;
-          const uint64_t ad = sw128_desc(st, 16, 1024), bd = sw128_desc(st + C::kABytes, 16, 1024);
+          const uint32_t end = min(kb + kPart, nk);
+          for (uint32_t first = kb; kb < end; ++kb, ++step) {
+            const uint32_t s = step % C::kStages;
+            if (!(ok = wait_bar(bar(kBarFull + s), (step / C::kStages) & 1, abort_flag, p.status,
+                                kSiteFull, p.wait_cycles)))
+              break;
+            tc_fence_after();
+            const uint32_t st = sbase + s * C::kStageBytes;
+            const uint64_t ad = sw128_desc(st, 16, 1024), bd = sw128_desc(st + C::kABytes, 16, 1024);
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks)
-            umma(acc, ad + ks * 2, bd + ks * 2, C::kIdesc, kb > 0 || ks > 0);
-          umma_commit(bar(kBarEmpty + s));
+            for (int ks = 0; ks < 4; ++ks)
+              umma(acc, ad + ks * 2, bd + ks * 2, C::kIdesc, kb > first || ks > 0);
+            umma_commit(bar(kBarEmpty + s));
+          }
+          if (ok) umma_commit(bar(kBarAcc + b));
         }
-        if (ok) umma_commit(bar(kBarAcc + b));
       }
       umma_commit(bar(kBarDrain));
       drain_bar(bar(kBarDrain), 0);
     }
     __syncwarp();
   } else {
-    const uint32_t quarter = (uint32_t)warp & 3, r = quarter * 32 + lane;
-    const bool out16 = p.out_vec, res16 = p.res_vec;
-    uint32_t done = 0;
-    for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++done) {
-      const uint32_t b = done & 1, m = tile / nt * kBM + r, n0 = tile % nt * kBN;
-      if (!__all_sync(0xffffffffu, wait_bar(bar(kBarAcc + b), (done >> 1) & 1, abort_flag,
-                                            p.status, kSiteAcc, p.wait_cycles)))
-        break;
-      tc_fence_after();
-      const uint32_t t0 = tmem + b * kBN + ((quarter * 32u) << 16);
-#pragma unroll 1
-      for (uint32_t c = 0; c < kBN; c += 32) {
-        if (n0 + c >= p.n) break;
-        uint32_t a[32];
-        tmem_ld32(t0 + c, a);
-        tmem_ld_wait();
+    // Warp w finishes columns [half * kCols, +kCols) of the 32 rows of its tensor-memory quarter.
+    constexpr uint32_t kCols = kBN / 2;
+    const uint32_t quarter = (uint32_t)warp & 3, half = (uint32_t)(warp - 2) >> 2;
+    const uint32_t lane_row = quarter * 32 + lane;
+    const uint32_t staging = sbase + C::kOffStaging + (uint32_t)(warp - 2) * 2 * kBufBytes;
+    const uint32_t res_bar = kBarRes + 2 * (uint32_t)(warp - 2);
+    const int mode = kBN >= 128 ? p.epilogue : kDirect;
+    const bool f32_out = p.out_dtype == 0;
+    uint32_t done = 0, res_loads = 0, res_used = 0;  // residual boxes asked for and consumed
+    bool ok = true;
+    // Residual box number `res_loads` (columns from n, rows from m) into its buffer, once the
+    // store that last left from there has been read.
+    auto load_residual = [&](uint32_t n, uint32_t m) {
+      const uint32_t b = res_loads & 1;
+      if (lane == 0) {
+        bulk_wait_read<0>();
+        mbar_expect_tx(bar(res_bar + b), kBufBytes);
+        tma_load_2d(staging + b * kBufBytes, &tm_res, bar(res_bar + b), (int)n, (int)m);
+      }
+      ++res_loads;
+    };
+    for (uint32_t tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
+      const uint32_t m0 = tile / nt * kBM + quarter * 32, m = m0 + lane;
+      const uint32_t n0 = tile % nt * kBN + half * kCols;
+      const uint32_t box = f32_out ? 32 : 64;  // columns of a 128-byte staging row
+      const bool rows = m0 < p.m && n0 < p.n;  // this warp has something to write
+      if (mode == kStagedRes && rows) load_residual(n0, m0);
+      // The tile's sums: partial sums of 512 K are added in fp32 registers.  The accumulator cuts
+      // off bits at each of its additions, always towards zero: over 2048 K in one go that left
+      // an error of 2e-6 of the result, eight times that of fp32 products in fp32.
+      float v[kCols];
+      for (uint32_t part = 0; part < parts; ++part, ++done) {
+        const uint32_t b = done & 1;
+        if (!(ok = __all_sync(0xffffffffu, wait_bar(bar(kBarAcc + b), (done >> 1) & 1, abort_flag,
+                                                    p.status, kSiteAcc, p.wait_cycles))))
+          break;
+        tc_fence_after();
+        const uint32_t t0 = tmem + b * kBN + half * kCols + ((quarter * 32u) << 16);
+        if (part == 0) {
+          uint32_t a[kCols / 16][16];
+#pragma unroll
+          for (uint32_t c = 0; c < kCols / 16; ++c) tmem_ld16(t0 + 16 * c, a[c]);
+          tmem_ld_wait();
+#pragma unroll
+          for (uint32_t c = 0; c < kCols; ++c) {
+            asm volatile("" : "+r"(a[c / 16][c % 16]));  // no use above the wait
+            v[c] = __uint_as_float(a[c / 16][c % 16]);
+          }
+        } else {
+#pragma unroll
+          for (uint32_t c = 0; c < kCols; c += 16) {
+            uint32_t a[16];
+            tmem_ld16(t0 + c, a);
+            tmem_ld_wait();
+#pragma unroll
+            for (int t = 0; t < 16; ++t) v[c + t] += __uint_as_float(a[t]);
+          }
+        }
+        tc_fence_before();
+        mbar_arrive(bar(kBarFree + b));
+      }
+      if (!ok) break;
+      if (!rows) continue;
+#pragma unroll
+      for (uint32_t c = 0; c < kCols; c += 32) {
         const uint32_t n = n0 + c;
+        if (n < p.n && ok) {
         const bool whole = n + 32 <= p.n;
-        if (m < p.m) {
-          float v[32];
+        if (p.bias) {
+          if (whole && p.bias_vec) {
 #pragma unroll
-          for (int t = 0; t < 32; ++t) v[t] = __uint_as_float(a[t]);
-          if (p.bias) {
-#pragma unroll
-            for (int t = 0; t < 32; ++t)
-              if (whole || n + t < p.n) v[t] += __ldg(p.bias + n + t);
-          }
-          if (p.act) {
-#pragma unroll
-            for (int t = 0; t < 32; ++t) v[t] = activate(v[t], p.act);
-          }
-          if (p.residual) {
-            const size_t at = (size_t)m * p.ldr + n;
-            if (whole && res16 && p.residual_dtype == 0) {
-#pragma unroll
-              for (int t = 0; t < 8; ++t) {
-                const float4 q = reinterpret_cast<const float4 *>(
-                    static_cast<const float *>(p.residual) + at)[t];
-                v[4 * t] += q.x; v[4 * t + 1] += q.y; v[4 * t + 2] += q.z; v[4 * t + 3] += q.w;
-              }
-            } else if (whole && res16) {
-#pragma unroll
-              for (int t = 0; t < 4; ++t) {
-                const uint4 q = reinterpret_cast<const uint4 *>(
-                    static_cast<const uint16_t *>(p.residual) + at)[t];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  v[8 * t + 2 * e] += bf16_lo(u4_at(q, e));
-                  v[8 * t + 2 * e + 1] += bf16_hi(u4_at(q, e));
-                }
-              }
-            } else {
-#pragma unroll
-              for (int t = 0; t < 32; ++t)
-                if (whole || n + t < p.n) v[t] += residual_at(p, at + t);
+            for (int t = 0; t < 8; ++t) {
+              const float4 q = __ldg(reinterpret_cast<const float4 *>(p.bias + n) + t);
+              v[c + 4 * t] += q.x; v[c + 4 * t + 1] += q.y;
+              v[c + 4 * t + 2] += q.z; v[c + 4 * t + 3] += q.w;
             }
-          }
-          const size_t at = (size_t)m * p.ldo + n;
-          if (whole && out16 && p.out_dtype == 0) {
-#pragma unroll
-            for (int t = 0; t < 8; ++t)
-              reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at)[t] =
-                  make_float4(v[4 * t], v[4 * t + 1], v[4 * t + 2], v[4 * t + 3]);
-          } else if (whole && out16) {
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-              reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.out) + at)[t] = make_uint4(
-                  pack_bf16x2(v[8 * t], v[8 * t + 1]), pack_bf16x2(v[8 * t + 2], v[8 * t + 3]),
-                  pack_bf16x2(v[8 * t + 4], v[8 * t + 5]), pack_bf16x2(v[8 * t + 6], v[8 * t + 7]));
           } else {
 #pragma unroll
             for (int t = 0; t < 32; ++t)
-              if (whole || n + t < p.n) store_at(p, at + t, v[t]);
+              if (n + t < p.n) v[c + t] += __ldg(p.bias + n + t);
           }
         }
-        __syncwarp();
+#pragma unroll
+        for (int t = 0; t < 32; ++t) v[c + t] = activate<kAct>(v[c + t]);
+        if (p.residual && mode != kStagedRes && m < p.m) {
+          const size_t at = (size_t)m * p.ldr + n;
+          if (whole && p.res_vec && p.residual_dtype == 0) {
+#pragma unroll
+            for (int t = 0; t < 8; ++t) {
+              const float4 q = reinterpret_cast<const float4 *>(
+                  static_cast<const float *>(p.residual) + at)[t];
+              v[c + 4 * t] += q.x; v[c + 4 * t + 1] += q.y;
+              v[c + 4 * t + 2] += q.z; v[c + 4 * t + 3] += q.w;
+            }
+          } else if (whole && p.res_vec) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+              const uint4 q = reinterpret_cast<const uint4 *>(
+                  static_cast<const uint16_t *>(p.residual) + at)[t];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                v[c + 8 * t + 2 * e] += bf16_lo(u4_at(q, e));
+                v[c + 8 * t + 2 * e + 1] += bf16_hi(u4_at(q, e));
+              }
+            }
+          } else {
+#pragma unroll
+            for (int t = 0; t < 32; ++t)
+              if (n + t < p.n) v[c + t] += residual_at(p, at + t);
+          }
+        }
+        if (mode == kDirect) {
+          const size_t at = (size_t)m * p.ldo + n;
+          if (m >= p.m) {
+          } else if (whole && p.out_vec && f32_out) {
+#pragma unroll
+            for (int t = 0; t < 8; ++t)
+              reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at)[t] = make_float4(
+                  v[c + 4 * t], v[c + 4 * t + 1], v[c + 4 * t + 2], v[c + 4 * t + 3]);
+          } else if (whole && p.out_vec) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+              reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.out) + at)[t] =
+                  make_uint4(pack_bf16x2(v[c + 8 * t], v[c + 8 * t + 1]),
+                             pack_bf16x2(v[c + 8 * t + 2], v[c + 8 * t + 3]),
+                             pack_bf16x2(v[c + 8 * t + 4], v[c + 8 * t + 5]),
+                             pack_bf16x2(v[c + 8 * t + 6], v[c + 8 * t + 7]));
+          } else {
+#pragma unroll
+            for (int t = 0; t < 32; ++t)
+              if (n + t < p.n) store_at(p, at + t, v[c + t]);
+          }
+        } else if constexpr (kBN >= 128) {
+          // A staging row is 128 bytes of this lane's output row, its 16-byte pieces swizzled as
+          // the tensor map has them; bf16 takes two 32-column steps to fill one.
+          const bool starts = f32_out || c % 64 == 0, ends = f32_out || c % 64 == 32;
+          uint32_t b;
+          if (mode == kStagedRes) {
+            b = res_used & 1;
+            if (starts) {
+              // The next box, if this tile has one, travels while this one is finished.
+              if (c + box < kCols && n + box < p.n) load_residual(n + box, m0);
+              ok = __all_sync(0xffffffffu, wait_bar(bar(res_bar + b), (res_used >> 1) & 1,
+                                                    abort_flag, p.status, kSiteRes, p.wait_cycles));
+            }
+          } else {
+            b = (c / box) & 1;
+            if (starts) {
+              if (lane == 0) bulk_wait_read<1>();
+              __syncwarp();
+            }
+          }
+          const uint32_t row = staging + b * kBufBytes + (uint32_t)lane * 128, sw = lane & 7;
+          if (f32_out) {
+#pragma unroll
+            for (uint32_t q = 0; q < 8; ++q) {
+              const uint32_t at = row + ((q ^ sw) << 4);
+              if (mode == kStagedRes) {
+                const uint4 o = ld_shared_v4(at);
+                v[c + 4 * q] += __uint_as_float(o.x);
+                v[c + 4 * q + 1] += __uint_as_float(o.y);
+                v[c + 4 * q + 2] += __uint_as_float(o.z);
+                v[c + 4 * q + 3] += __uint_as_float(o.w);
+              }
+              st_shared_v4(at, __float_as_uint(v[c + 4 * q]), __float_as_uint(v[c + 4 * q + 1]),
+                           __float_as_uint(v[c + 4 * q + 2]), __float_as_uint(v[c + 4 * q + 3]));
+            }
+          } else {
+#pragma unroll
+            for (uint32_t q = 0; q < 4; ++q) {
+              const uint32_t at = row + (((q + (c % 64) / 8) ^ sw) << 4);
+              if (mode == kStagedRes) {
+                const uint4 o = ld_shared_v4(at);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  v[c + 8 * q + 2 * e] += bf16_lo(u4_at(o, e));
+                  v[c + 8 * q + 2 * e + 1] += bf16_hi(u4_at(o, e));
+                }
+              }
+              st_shared_v4(at, pack_bf16x2(v[c + 8 * q], v[c + 8 * q + 1]),
+                           pack_bf16x2(v[c + 8 * q + 2], v[c + 8 * q + 3]),
+                           pack_bf16x2(v[c + 8 * q + 4], v[c + 8 * q + 5]),
+                           pack_bf16x2(v[c + 8 * q + 6], v[c + 8 * q + 7]));
+            }
+          }
+          if (ends || n + 32 >= p.n) {
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(&tm_out, staging + b * kBufBytes, (int)(n - c % box), (int)m0);
+              bulk_commit();
+            }
+            if (mode == kStagedRes) ++res_used;
+          }
+        }
+        }
       }
-      tc_fence_before();
-      mbar_arrive(bar(kBarFree + b));
+    }
+    if (mode != kDirect) {
+      if (lane == 0) {
+        // Residual boxes that an abort left in flight, and every store, end before the CTA does.
+        for (; res_used < res_loads; ++res_used)
+          drain_bar(bar(res_bar + (res_used & 1)), (res_used >> 1) & 1);
+        bulk_wait_all();
+      }
+      __syncwarp();
     }
   }
 
@@ -278,7 +452,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 // One warp per output column; lane l takes columns 8l .. 8l+7 of every 256 of K.
 constexpr int kGemvWarps = 4;
 
-template <int kM>
+template <int kM, int kAct>
 __global__ void __launch_bounds__(32 * kGemvWarps) gemv_kernel(const __grid_constant__ LinearFusedProblem p) {
   const uint32_t lane = threadIdx.x & 31;
   const uint32_t n = blockIdx.x * kGemvWarps + (threadIdx.x >> 5);
@@ -318,15 +492,23 @@ __global__ void __launch_bounds__(32 * kGemvWarps) gemv_kernel(const __grid_cons
     if (lane == (uint32_t)i) y = sum[i];
   if (lane < p.m) {
     if (p.bias) y += p.bias[n];
-    y = activate(y, p.act);
+    y = activate<kAct>(y);
     if (p.residual) y += residual_at(p, (size_t)lane * p.ldr + n);
     store_at(p, (size_t)lane * p.ldo + n, y);
   }
 }
 
-template <int kM>
+template <int kAct>
 cudaError_t launch_gemv(const LinearFusedProblem &p, cudaStream_t stream) {
-  gemv_kernel<kM><<<(p.n + kGemvWarps - 1) / kGemvWarps, 32 * kGemvWarps, 0, stream>>>(p);
+  const uint32_t grid = (p.n + kGemvWarps - 1) / kGemvWarps, block = 32 * kGemvWarps;
+  if (p.m <= 1)
+    gemv_kernel<1, kAct><<<grid, block, 0, stream>>>(p);
+  else if (p.m <= 2)
+    gemv_kernel<2, kAct><<<grid, block, 0, stream>>>(p);
+  else if (p.m <= 4)
+    gemv_kernel<4, kAct><<<grid, block, 0, stream>>>(p);
+  else
+    gemv_kernel<8, kAct><<<grid, block, 0, stream>>>(p);
   return cudaGetLastError();
 }
 
@@ -342,50 +524,76 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   }();
   return fn;
 }
+// Row-major [rows, cols] of bf16 or fp32 with a row stride in elements; boxes of 128 bytes of
+// columns in the 128-byte swizzle.
 bool make_map(CUtensorMap *map, const void *base, uint32_t rows, uint32_t cols, uint64_t ld,
-              uint32_t box_rows) {
+              uint32_t box_rows, bool f32 = false) {
   auto fn = encode_fn();
   if (!fn) return false;
+  const uint32_t e = f32 ? 4 : 2;
   cuuint64_t dims[2] = {cols, rows};
-  cuuint64_t strides[1] = {ld * 2};
-  cuuint32_t box[2] = {kBK, box_rows};
+  cuuint64_t strides[1] = {ld * e};
+  cuuint32_t box[2] = {128 / e, box_rows};
   cuuint32_t elem[2] = {1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(base), dims, strides, box,
-            elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return fn(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+            const_cast<void *>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int kBN>
+template <int kBN, int kAct>
 cudaError_t launch_tiles(const LinearFusedProblem &p, int num_sms, cudaStream_t stream) {
   constexpr uint32_t smem = Cfg<kBN>::kSmemBytes;
-  CUtensorMap mx, mw;
+  CUtensorMap mx, mw, mr, mo;
   if (!make_map(&mx, p.x, p.m, p.k, p.ldx, kBM) || !make_map(&mw, p.w, p.n, p.k, p.ldw, kBN))
     return cudaErrorInvalidValue;
-  cudaError_t e = cudaFuncSetAttribute(linear_kernel<kBN>,
+  mr = mo = mx;
+  if (p.epilogue != kDirect && !make_map(&mo, p.out, p.m, p.n, p.ldo, 32, p.out_dtype == TX_F32))
+    return cudaErrorInvalidValue;
+  if (p.epilogue == kStagedRes &&
+      !make_map(&mr, p.residual, p.m, p.n, p.ldr, 32, p.out_dtype == TX_F32))
+    return cudaErrorInvalidValue;
+  cudaError_t e = cudaFuncSetAttribute(linear_kernel<kBN, kAct>,
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
   const uint64_t tiles = (uint64_t)((p.n + kBN - 1) / kBN) * ((p.m + kBM - 1) / kBM);
   if (tiles > 0x7fffffffull) return cudaErrorInvalidValue;
-  linear_kernel<kBN><<<(uint32_t)std::min<uint64_t>(tiles, (uint64_t)num_sms), kThreads, smem,
-                       stream>>>(mx, mw, p);
+  linear_kernel<kBN, kAct><<<(uint32_t)std::min<uint64_t>(tiles, (uint64_t)num_sms), kThreads,
+                             smem, stream>>>(mx, mw, mr, mo, p);
   return cudaGetLastError();
+}
+
+template <int kAct>
+cudaError_t launch_act(LinearFusedProblem p, int num_sms, cudaStream_t stream) {
+  if (p.m <= 8) return launch_gemv<kAct>(p, stream);
+  const uint32_t vo = p.out_dtype == TX_BF16 ? 8 : 4, vr = p.residual_dtype == TX_BF16 ? 8 : 4;
+  p.out_vec = (uintptr_t)p.out % 16 == 0 && p.ldo % vo == 0;
+  p.res_vec = p.residual && (uintptr_t)p.residual % 16 == 0 && p.ldr % vr == 0;
+  p.bias_vec = (uintptr_t)p.bias % 16 == 0;
+  p.epilogue = !p.out_vec ? kDirect
+               : p.residual && p.res_vec && p.residual_dtype == p.out_dtype ? kStagedRes : kStaged;
+  // The widest tile that still gives every SM one (a wide tile reads x fewer times).
+  const uint64_t mt = (p.m + kBM - 1) / kBM;
+  if (mt * ((p.n + 255) / 256) >= (uint64_t)num_sms) return launch_tiles<256, kAct>(p, num_sms, stream);
+  if (mt * ((p.n + 127) / 128) >= (uint64_t)num_sms) return launch_tiles<128, kAct>(p, num_sms, stream);
+  return launch_tiles<64, kAct>(p, num_sms, stream);
 }
 
 }  // namespace lfused
 
-cudaError_t launch_linear_fused(LinearFusedProblem p, int num_sms, cudaStream_t stream) {
-  if (p.m <= 1) return lfused::launch_gemv<1>(p, stream);
-  if (p.m <= 2) return lfused::launch_gemv<2>(p, stream);
-  if (p.m <= 4) return lfused::launch_gemv<4>(p, stream);
-  if (p.m <= 8) return lfused::launch_gemv<8>(p, stream);
-  const uint32_t vo = p.out_dtype == TX_BF16 ? 8 : 4, vr = p.residual_dtype == TX_BF16 ? 8 : 4;
-  p.out_vec = (uintptr_t)p.out % 16 == 0 && p.ldo % vo == 0;
-  p.res_vec = p.residual && (uintptr_t)p.residual % 16 == 0 && p.ldr % vr == 0;
-  // The widest tile that still gives every SM one (a wide tile reads x fewer times).
-  const uint64_t mt = (p.m + lfused::kBM - 1) / lfused::kBM;
-  if (mt * ((p.n + 255) / 256) >= (uint64_t)num_sms) return lfused::launch_tiles<256>(p, num_sms, stream);
-  if (mt * ((p.n + 127) / 128) >= (uint64_t)num_sms) return lfused::launch_tiles<128>(p, num_sms, stream);
-  return lfused::launch_tiles<64>(p, num_sms, stream);
+cudaError_t launch_linear_fused(const LinearFusedProblem &p, int num_sms, cudaStream_t stream) {
+  switch (p.act) {
+    case TX_ACT_RELU:
+      return lfused::launch_act<TX_ACT_RELU>(p, num_sms, stream);
+    case TX_ACT_GELU:
+      return lfused::launch_act<TX_ACT_GELU>(p, num_sms, stream);
+    case TX_ACT_GELU_TANH:
+      return lfused::launch_act<TX_ACT_GELU_TANH>(p, num_sms, stream);
+    case TX_ACT_SILU:
+      return lfused::launch_act<TX_ACT_SILU>(p, num_sms, stream);
+    default:
+      return lfused::launch_act<TX_ACT_NONE>(p, num_sms, stream);
+  }
 }
 
 }  // namespace tx
