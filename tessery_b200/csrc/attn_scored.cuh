@@ -15,6 +15,7 @@ namespace tx {
 namespace scored {
 
 constexpr int kKeys = 128;        // keys per tile
+constexpr uint32_t kTablePack = 4;  // most heads of a pack with a distance table (tensor-memory route)
 constexpr uint32_t kDocWords = 1024;  // bits for the key tiles of a document mask: 32768 tiles
 
 struct Seq {
@@ -55,6 +56,8 @@ struct Unit {
   int prefix;              // keys [0, prefix) are open to every row
   // key tiles in order: [0, a) then [b, ...), `count` in all; this CTA visits [first, last)
   int a, b, first, last;
+  // keys that all rows see: [whole_lo, whole_hi) and [0, whole_prefix) (none with documents)
+  int whole_lo, whole_hi, whole_prefix;
 };
 
 // Key range of a query position without the prefix: [lo, hi).
@@ -88,12 +91,17 @@ __device__ __forceinline__ Unit make_unit(const ScoredProblem &p, uint32_t block
   u.present = p.cu_q ? u.tokens
                      : max(0, min(per, min((int)p.max_q, (int)p.rows_q - u.s.q_row) - u.t0));
   u.prefix = p.prefix ? min(max(p.prefix[s], 0), u.s.nk) : 0;
-  u.a = u.b = u.first = u.last = 0;
+  u.a = u.b = u.first = u.last = u.whole_lo = u.whole_hi = u.whole_prefix = 0;
   if (!u.tokens) return u;
   const int p0 = u.t0 + u.s.nk - u.s.nq;
-  int lo, hi, x;
-  row_range(p, p0, u.s.nk, &lo, &x);                  // both ends grow with the position
-  row_range(p, p0 + u.tokens - 1, u.s.nk, &x, &hi);
+  int lo, hi, last_lo, first_hi;
+  row_range(p, p0, u.s.nk, &lo, &first_hi);           // both ends grow with the position
+  row_range(p, p0 + u.tokens - 1, u.s.nk, &last_lo, &hi);
+  if (!p.q_docs) {
+    u.whole_lo = last_lo;
+    u.whole_hi = first_hi;
+    u.whole_prefix = u.prefix;
+  }
   u.a = (u.prefix + kKeys - 1) / kKeys;
   u.b = max(u.a, lo / kKeys);
   const int end = hi > lo ? (hi + kKeys - 1) / kKeys : 0;
@@ -140,16 +148,11 @@ __device__ __forceinline__ void mark_tiles(const ScoredProblem &p, const Unit &u
   }
   __syncthreads();
 }
-// Whether every key of the tile from k0 (up to the sequence's end) is open to every row of the
-// unit, as far as ranges tell.
-__device__ __forceinline__ bool whole_tile(const ScoredProblem &p, const Unit &u, int k0) {
-  if (p.q_docs) return false;
-  const int end = min(k0 + kKeys, u.s.nk), p0 = u.t0 + u.s.nk - u.s.nq;
-  if (end <= u.prefix) return true;
-  int lo, hi, x;
-  row_range(p, p0 + u.tokens - 1, u.s.nk, &lo, &x);
-  row_range(p, p0, u.s.nk, &x, &hi);
-  return k0 >= lo && end <= hi;
+// Whether the tile from k0 holds kKeys keys and all are open to every row of the unit, as far as
+// ranges tell.
+__device__ __forceinline__ bool whole_tile(const Unit &u, int k0) {
+  const int end = k0 + kKeys;
+  return end <= u.whole_prefix || (k0 >= u.whole_lo && end <= u.whole_hi);
 }
 // The first visited tile at or after i (u.last when there is none).
 __device__ __forceinline__ int next_tile(const Unit &u, const uint32_t *words, int i) {
@@ -168,6 +171,19 @@ __device__ __forceinline__ uint32_t interval_bits(int c0, int lo, int hi) {
   const int l = min(max(lo - c0, 0), 32), h = min(max(hi - c0, 0), 32);
   const uint32_t below_h = (uint32_t)((1ull << h) - 1), below_l = (uint32_t)((1ull << l) - 1);
   return below_h & ~below_l;
+}
+
+// Bits of 32 keys, whose documents the lanes hold (lane = key), that lie in this lane's own
+// document: a pair of votes for each document that the warp's rows are in, most often one or two.
+__device__ __forceinline__ uint32_t doc_bits(int32_t key_doc, int32_t row_doc) {
+  uint32_t bits = 0, todo = __ballot_sync(0xffffffffu, row_doc >= 0);
+  while (todo) {
+    const int32_t d = __shfl_sync(0xffffffffu, row_doc, __ffs(todo) - 1);
+    const uint32_t same = __ballot_sync(0xffffffffu, key_doc == d);
+    if (row_doc == d) bits = same;
+    todo &= ~__ballot_sync(0xffffffffu, row_doc == d);
+  }
+  return bits;
 }
 
 // One row's view of the keys.

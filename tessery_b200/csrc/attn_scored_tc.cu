@@ -7,8 +7,10 @@
 // One CTA takes 128 rows (query tokens x the heads that share a kv head, attn_scored.cuh) and
 // walks the 128-key tiles that some row may see.  S = Q K^T and O += P V are tcgen05.mma
 // (M = 128) into tensor memory; thread t of the four softmax warps owns row t (tensor-memory
-// lane t): it reads S, applies cap, bias and mask, and writes P = exp2(z - m) as bf16 over S,
-// which is the A operand of P.V.  The reference m follows the row's running maximum lazily: O
+// lane t).  It walks S twice, 32 keys at a time: first the row's maximum (scores with a cap, a bias or a mask go back finished), then
+// P = exp2(z - m) as bf16 into tensor memory, the A operand of P.V.  Both walks are rolled loops:
+// the same work unrolled over the 128 keys (20 KB of code a tile) was bound by instruction
+// fetches.  The reference m follows the row's running maximum lazily: O
 // and the row sum are rescaled only when a tile's maximum exceeds it by more than 2^8, which
 // changes no result (P stays below 2^8 and the sum uses the same reference).  Two CTAs share an
 // SM, so one's products run beside the other's softmax.
@@ -36,10 +38,20 @@ using namespace scored;
 constexpr int kRows = 128;
 constexpr int kThreads = 192;  // warps 0-3 softmax, 4 TMA, 5 MMA
 constexpr int kTmaWarp = 4, kMmaWarp = 5;
-constexpr uint32_t kTmemCols = 256;  // S (128, P over it), O (head_dim); two CTAs per SM
-constexpr uint32_t kColO = 128;
+constexpr uint32_t kTmemCols = 256;  // of the 512 of an SM: two CTAs share it
+constexpr uint32_t kColO = 128;      // S in columns 0-127, O from here
 constexpr float kRescaleThreshold = 8.0f;  // log2 units
 constexpr float kLog2e = 1.44269504088896341f;
+
+// Distance biases of a warp's 32 rows over a key tile: 127 + 32 / pack distances of each of the
+// pack heads (at most kTablePack).  Heads lie 32 / pack words apart modulo 32, so that the rows of
+// a warp read different banks.
+__host__ __device__ constexpr uint32_t window_pitch(uint32_t pack) {
+  const uint32_t n = 127 + 32 / pack, step = 32 / pack;
+  return n + (32 + step - n % 32) % 32;
+}
+constexpr uint32_t kWindow = kTablePack * window_pitch(kTablePack);
+static_assert(window_pitch(1) <= kWindow && 2 * window_pitch(2) <= kWindow, "window area");
 
 template <int kDP>  // head_dim rounded up to whole 64-column (128-byte) blocks
 struct Cfg {
@@ -48,7 +60,11 @@ struct Cfg {
   static constexpr int kSlots = kDP == 64 ? 2 : 1;  // K slots, and V slots
   static constexpr uint32_t kOffQ = 0, kOffK = kTile, kOffV = kOffK + kSlots * kTile;
   static constexpr uint32_t kOffMisc = kOffV + kSlots * kTile;
-  static constexpr uint32_t kMiscBytes = 256 + kDocWords * 4 + 4 * kKeys * 4;
+  static constexpr uint32_t kMiscBytes = 256 + kDocWords * 4 + 4 * (kWindow + kKeys) * 4;
+  // head_dim up to 64 leaves columns for P beside S: the next tile's Q.K^T is issued as soon as S
+  // has been read.  Otherwise P lies over S, and it waits for P.V.
+  static constexpr bool kEarly = kDP == 64;
+  static constexpr uint32_t kColP = kEarly ? kColO + 64 : 0;
   static constexpr uint32_t kSmemBytes = kOffMisc + kMiscBytes;
   static_assert(2 * (kSmemBytes + 1024) <= 233472, "two CTAs per SM");
 };
@@ -56,12 +72,16 @@ struct Cfg {
 // Barriers at the start of the misc area.
 enum : uint32_t {
   kBarQ = 0, kBarKFull = 1, kBarKEmpty = 3, kBarVFull = 5, kBarVEmpty = 7, kBarS = 9, kBarP = 10,
-  kBarO = 11, kBarScan = 12, kBarHand = 13, kNumBars = 14
+  kBarO = 11, kBarScan = 12, kBarHand = 13, kBarSRead = 14, kBarPV = 15,
+  kNumBars = 16
 };
-enum : uint32_t { kOffTmem = 128, kOffAbort = 132, kOffFlag = 136, kOffRange = 144,
-                  kOffBad = 160, kOffWords = 256 };
+enum : uint32_t { kOffTmem = 128, kOffAbort = 132, kOffFlag = 136, kOffRange = 144, kOffBad = 160,
+                  kOffWords = 256,
+                  kOffWindow = kOffWords + kDocWords * 4,
+                  kOffDocs = kOffWindow + 4 * kWindow * 4 };
 enum : int { kSiteK = 1, kSiteV = 2, kSiteKFree = 3, kSiteVFree = 4, kSiteS = 5, kSiteP = 6,
-             kSiteO = 7, kSiteQ = 8, kSiteVRead = 9, kSiteScan = 10, kSiteHand = 11 };
+             kSiteO = 7, kSiteQ = 8, kSiteVRead = 9, kSiteScan = 10, kSiteHand = 11,
+             kSiteSRead = 12, kSitePV = 13 };
 
 struct Gate {  // a bounded wait that gives up once for the whole CTA
   volatile int *abort_flag;
@@ -126,23 +146,21 @@ __device__ __forceinline__ bool scan_values(uint32_t tile, int keys, uint32_t *b
 }
 
 // The value rows marked in `bad` added to O for the query rows with p > 0 (thread = row, all four
-// softmax warps), then zeroed.  `fresh`: O holds nothing yet.
+// softmax warps), then zeroed.  `fresh`: O holds nothing yet.  False where a wait gave up.
 template <int kDP>
-__device__ __noinline__ void add_by_hand(const volatile uint32_t *bad, uint32_t tile,
-                                         uint32_t atom, uint32_t tS, uint32_t tO, bool fresh,
-                                         int r, const Gate &gate, uint32_t done, uint32_t turn) {
+__device__ __noinline__ bool add_by_hand(const volatile uint32_t *bad, uint32_t tile,
+                                         uint32_t atom, uint32_t tP, uint32_t tO, bool fresh,
+                                         const Gate &gate, uint32_t read, uint32_t turn) {
   for (int j = 0; j < kKeys; ++j) {
     if (!((bad[j >> 5] >> (j & 31)) & 1)) continue;
-    uint32_t w;
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(w) : "r"(tS + j / 2));
-    tmem_ld_wait();
-    const float pj = j & 1 ? bf16_hi(w) : bf16_lo(w);
-    for (uint32_t c = 0; c < kDP; c += 32) {
-      uint32_t o[32];
-      tmem_ld32(tO + c, o);
-      tmem_ld_wait();
+    uint32_t w[1];
+    tmem_load(tP + j / 2, w);
+    const float pj = j & 1 ? bf16_hi(w[0]) : bf16_lo(w[0]);
+    for (uint32_t c = 0; c < kDP; c += 16) {
+      uint32_t o[16];
+      tmem_load(tO + c, o);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
+      for (int q = 0; q < 2; ++q) {
         const uint32_t chunk = (c & 63) / 8 + q;
         const uint4 v = ld_shared_v4(tile + (c >> 6) * atom + j * 128 +
                                      ((chunk ^ (uint32_t)(j & 7)) * 16));
@@ -153,19 +171,20 @@ __device__ __noinline__ void add_by_hand(const volatile uint32_t *bad, uint32_t 
           o[q * 8 + e] = __float_as_uint(pj == 0.f ? old : fmaf(pj, x, old));
         }
       }
-      tmem_st32(tO + c, o);
+      tmem_st16(tO + c, o);
     }
     tmem_st_wait();
     fresh = false;
   }
-  mbar_arrive(done);  // every thread has read the rows
-  if (!__all_sync(0xffffffffu, gate.wait(done, turn & 1, kSiteHand))) return;
-  for (int x = r; x < kKeys * (kDP / 8); x += 128) {
+  mbar_arrive(read);  // every thread has read the rows
+  if (!__all_sync(0xffffffffu, gate.wait(read, turn & 1, kSiteHand))) return false;
+  for (int x = (int)threadIdx.x; x < kKeys * (kDP / 8); x += 128) {
     const int row = x / (kDP / 8), ch = x % (kDP / 8);
     if ((bad[row >> 5] >> (row & 31)) & 1)
       st_shared_v4(tile + (ch >> 3) * atom + row * 128 + (ch & 7) * 16, 0, 0, 0, 0);
   }
   fence_proxy_async();
+  return true;
 }
 
 enum : int { kNoBias = 0, kSlopes = 1, kTable = 2 };
@@ -184,7 +203,6 @@ __global__ void __launch_bounds__(kThreads, 2)
   const uint32_t bars = sbase + C::kOffMisc;
   auto bar = [&](uint32_t i) { return bars + 8 * i; };
   uint32_t *words = reinterpret_cast<uint32_t *>(misc + kOffWords);
-  int32_t *doc_s = reinterpret_cast<int32_t *>(misc + kOffWords + kDocWords * 4);
   const Unit u = make_unit<kRows>(p, blockIdx.x);
   if (!u.present) return;  // whole units: every split of one takes the same way
   const bool docs = p.q_docs != nullptr;
@@ -209,6 +227,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       mbar_init(bar(kBarO), 1);
       mbar_init(bar(kBarScan), 1);
       mbar_init(bar(kBarHand), 128);
+      mbar_init(bar(kBarSRead), 4);
+      mbar_init(bar(kBarPV), 1);
       *gate.abort_flag = 0;
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -269,47 +289,64 @@ __global__ void __launch_bounds__(kThreads, 2)
       auto wait = [&](uint32_t b, uint32_t parity, int site) {
         return __all_sync(0xffffffffu, gate.wait(b, parity, site)) != 0;
       };
+      // Turn n issues Q.K^T of tile n and then P.V of the tile before it (kEarly: as soon as the
+      // softmax has read S; else S takes P's place, so P.V goes first).  One place in the code for
+      // each product: with two for Q.K^T the compiled code was wrong.
       bool ok = wait(bar(kBarQ), 0, kSiteQ);
+      bool more = true, odd = false;
+      int prev = first;  // the tile whose P.V is due
       uint32_t n = 0;
-      for (int i = first; ok && i < u.last; i = next_tile(u, marks, i + 1), ++n) {
+      for (int i = first; ok && (more || C::kEarly); ++n) {
         const uint32_t slot = n % C::kSlots, par = (n / C::kSlots) & 1;
-        const int k0 = key_tile(u, i) * kKeys, keys = min(u.s.nk - k0, kKeys);
-        if (!(ok = wait(bar(kBarKFull + slot), par, kSiteK))) break;
-        tc_fence_after();
-        const uint64_t kd = sw128_desc(sbase + C::kOffK + slot * C::kTile, 16, 1024);
-        if (lane == 0) {
+        if (more) {
+          if (!(ok = wait(bar(kBarKFull + slot), par, kSiteK))) break;
+          if (C::kEarly && n > 0 && !(ok = wait(bar(kBarSRead), (n - 1) & 1, kSiteSRead))) break;
+          tc_fence_after();
+          const uint64_t kd = sw128_desc(sbase + C::kOffK + slot * C::kTile, 16, 1024);
+          if (lane == 0) {
 #pragma unroll
-          for (uint32_t ks = 0; ks < kDP / 16; ++ks)
-            if (ks < dsteps) {
-              const uint64_t o = (uint64_t)((ks >> 2) * (C::kAtom >> 4) + (ks & 3) * 2);
-              umma(tmem, qd + o, kd + o, idesc_qk, ks > 0);
-            }
-          umma_commit(bar(kBarS));
-          umma_commit(bar(kBarKEmpty + slot));
-        }
-        __syncwarp();
-        if (!(ok = wait(bar(kBarVFull + slot), par, kSiteV))) break;
-        bool odd = false;
-        if (!whole_tile(p, u, k0)) {
-          odd = scan_values<C::kTile>(sbase + C::kOffV + slot * C::kTile, keys,
-                                      reinterpret_cast<uint32_t *>(misc + kOffBad), lane);
+            for (uint32_t ks = 0; ks < kDP / 16; ++ks)
+              if (ks < dsteps) {
+                const uint64_t o = (uint64_t)((ks >> 2) * (C::kAtom >> 4) + (ks & 3) * 2);
+                umma(tmem, qd + o, kd + o, idesc_qk, ks > 0);
+              }
+            umma_commit(bar(kBarS));
+            umma_commit(bar(kBarKEmpty + slot));
+          }
           __syncwarp();
-          if (lane == 0) mbar_arrive(bar(kBarScan));
         }
-        if (!(ok = wait(bar(kBarP), n & 1, kSiteP))) break;
-        tc_fence_after();
-        if (lane == 0) {
-          // 16-key steps up to the sequence's end (the probabilities past it are zero).
-          const uint32_t steps = (uint32_t)(keys + 15) / 16;
-          const uint64_t vd = sw128_desc(sbase + C::kOffV + slot * C::kTile, C::kAtom, 1024);
+        if (!C::kEarly || n > 0) {
+          const uint32_t t = C::kEarly ? n - 1 : n, vslot = t % C::kSlots;
+          const int k0 = key_tile(u, C::kEarly ? prev : i) * kKeys, keys = min(u.s.nk - k0, kKeys);
+          if (!(ok = wait(bar(kBarVFull + vslot), (t / C::kSlots) & 1, kSiteV))) break;
+          odd = false;
+          if (!whole_tile(u, k0)) {
+            odd = scan_values<C::kTile>(sbase + C::kOffV + vslot * C::kTile, keys,
+                                        reinterpret_cast<uint32_t *>(misc + kOffBad), lane);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(kBarScan));
+            __syncwarp();
+          }
+          if (!(ok = wait(bar(kBarP), t & 1, kSiteP))) break;
+          tc_fence_after();
+          if (lane == 0) {
+            // 16-key steps up to the sequence's end (the probabilities past it are zero).
+            const uint32_t steps = (uint32_t)(keys + 15) / 16;
+            const uint64_t vd = sw128_desc(sbase + C::kOffV + vslot * C::kTile, C::kAtom, 1024);
 #pragma unroll
-          for (uint32_t ks = 0; ks < 8; ++ks)
-            if (ks < steps)
-              umma_ts(tmem + kColO, tmem + ks * 8, vd + (uint64_t)(ks * (2048 >> 4)), idesc_pv,
-                      n > 0 || ks > 0 || odd);
-          umma_commit(bar(kBarVEmpty + slot));
+            for (uint32_t ks = 0; ks < 8; ++ks)
+              if (ks < steps)
+                umma_ts(tmem + kColO, tmem + C::kColP + ks * 8, vd + (uint64_t)(ks * (2048 >> 4)),
+                        idesc_pv, t > 0 || ks > 0 || odd);
+            umma_commit(bar(kBarVEmpty + vslot));
+            if (C::kEarly) umma_commit(bar(kBarPV));
+          }
+          __syncwarp();
+          if (C::kEarly && !more) break;
         }
-        __syncwarp();
+        prev = i;
+        i = next_tile(u, marks, i + 1);
+        more = i < u.last;
       }
       if (lane == 0) {
         umma_commit(bar(kBarO));
@@ -317,148 +354,220 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
       __syncwarp();
     } else {
-      const int r = warp * 32 + lane;
-      const uint32_t tS = tmem + ((uint32_t)(warp * 32) << 16), tO = tS + kColO;
+      const int r = (int)threadIdx.x;
+      const uint32_t tS = tmem + ((uint32_t)(warp * 32) << 16), tO = tS + kColO, tP = tS + C::kColP;
       const int token = r / (int)p.pack, head = (int)u.head0 + r % (int)p.pack;
       const bool live = token < u.tokens;
+      const bool busy = __any_sync(0xffffffffu, live);  // rows past the last token need nothing
       const Row row = make_row(p, u, token, live);
       const float scale2 = p.scale * kLog2e;
-      // cap: c2 tanh(s scale / cap) = c2 - 2 c2 / (1 + 2^(a s))
-      const float c2 = kCap ? p.softcap * kLog2e : 0.f;
-      const float cap_a = kCap ? 2.f * scale2 / p.softcap : 0.f;
+      // cap: c tanh(x scale / c) in log2 units = x (a0 + a1 x^2 + ... + a4 x^8) for arguments up to
+      // 3/4: a fit of degree 4 to tanh(u) / u in u^2 (weighted least squares refined to equal
+      // ripples, relative error 6e-7), which costs no special function.
+      const float cap_u = kCap ? p.scale / p.softcap : 0.f, cap2 = kCap ? p.softcap * kLog2e : 0.f;
+      const float cap_q = cap_u * cap_u;
+      const float a0 = scale2 * 0.999999435f, a1 = scale2 * -0.333282516f * cap_q,
+                  a2 = scale2 * 0.132589833f * cap_q * cap_q,
+                  a3 = scale2 * -0.0500563042f * cap_q * cap_q * cap_q,
+                  a4 = scale2 * 0.0129296325f * cap_q * cap_q * cap_q * cap_q;
+      auto cap_fit = [&](float x) {  // the factor of x
+        const float w = x * x;
+        return fmaf(fmaf(fmaf(fmaf(a4, w, a3), w, a2), w, a1), w, a0);
+      };
+      auto cap_exact = [&](float x) {  // tanh(u) = 1 - 2 / (1 + e^(2u))
+        return fmaf(-2.f * cap2, rcp(1.f + ex2(x * (2.f * kLog2e) * cap_u)), cap2);
+      };
       const float slope2 = kBias == kSlopes ? -p.slopes[head] * kLog2e : 0.f;
-      const float *table =
-          kBias == kTable ? p.table + (size_t)head * (2 * p.reach + 1) + p.reach : nullptr;
-      auto capped = [&](float s) {
-        return kCap ? fmaf(-2.f * c2, rcp(1.f + ex2(s * cap_a)), c2) : s * scale2;
-      };
-      // The score of key j in log2 units.  A finite bias too large for them stays finite.
-      auto score = [&](float s, int j) {
-        float z = capped(s);
-        if (kBias == kSlopes) z = fmaf(slope2, fabsf((float)(j - row.pos)), z);
-        if (kBias == kTable) {
-          const float b = __ldg(table + min(max(j - row.pos, -p.reach), p.reach));
-          z = b == -INFINITY ? b : fmaxf(fmaf(b, kLog2e, z), -3.402823466e38f);
-        }
-        return z;
-      };
+      // Table: this warp's window, and this row's place in it (its distance to the tile's key 0).
+      const uint32_t pitch = window_pitch(p.pack);
+      float *window = reinterpret_cast<float *>(misc + kOffWindow) + warp * kWindow;
+      const int warp_token = warp * 32 / (int)p.pack, span = 127 + 32 / (int)p.pack;
+      const float *window_row = window + (r % (int)p.pack) * pitch + (32 / (int)p.pack - 1) -
+                                (token - warp_token);
       bool ok = true;
       uint32_t n = 0, scans = 0, hands = 0;
-      for (int i = first; ok && i < u.last; i = next_tile(u, marks, i + 1), ++n) {
-        const int k0 = key_tile(u, i) * kKeys;
-        if (docs) {  // this tile's documents, a copy per warp
-          __syncwarp();
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int j = k0 + 32 * c + lane;
-            doc_s[warp * kKeys + 32 * c + lane] = j < u.s.nk ? p.k_docs[u.s.k_row + j] : -1;
-          }
-          __syncwarp();
-        }
-        uint32_t mask[4];
+      int32_t *doc_s = reinterpret_cast<int32_t *>(misc + kOffDocs) + warp * kKeys;
+      int32_t doc[4];  // documents of the next tile's keys, lane = key
+      auto load_docs = [&](int i) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          mask[c] = row.bits(k0 + 32 * c);
-          if (docs) {
-            uint32_t same = 0;
+          const int j = key_tile(u, i) * kKeys + 32 * c + lane;
+          doc[c] = i < u.last && j < u.s.nk ? p.k_docs[u.s.k_row + j] : -1;
+        }
+      };
+      if (docs && busy) load_docs(first);
+      for (int i = first, next; ok && i < u.last; i = next, ++n) {
+        next = next_tile(u, marks, i + 1);
+        const int k0 = key_tile(u, i) * kKeys;
+        const bool whole = whole_tile(u, k0);
+        if (docs && busy) {
+          __syncwarp();
 #pragma unroll
-            for (int t = 0; t < 32; ++t)
-              same |= (doc_s[warp * kKeys + c * 32 + t] == row.doc ? 1u : 0u) << t;
-            mask[c] &= same;
+          for (int c = 0; c < 4; ++c) doc_s[32 * c + lane] = doc[c];
+          load_docs(next);
+        }
+        if (kBias == kTable && busy) {
+          // In log2 units; a finite bias too large for them stays finite, so that only -inf closes
+          // a key.
+          const int d0 = k0 - row.pos + (token - warp_token) - (32 / (int)p.pack - 1);
+          __syncwarp();
+          for (int h = 0; h < (int)p.pack; ++h) {
+            const float *t = p.table + (size_t)((int)u.head0 + h) * (2 * p.reach + 1) + p.reach;
+            for (int x = lane; x < span; x += 32) {
+              const float b = __ldg(t + min(max(d0 + x, -p.reach), p.reach));
+              window[h * pitch + x] = b == -INFINITY ? b : fmaxf(b * kLog2e, -3.402823466e38f);
+            }
           }
         }
+        __syncwarp();
         if (!(ok = __all_sync(0xffffffffu, gate.wait(bar(kBarS), n & 1, kSiteS)))) break;
         tc_fence_after();
-        // First pass: the row's maximum; scores with a bias go back finished.
-        float top = -INFINITY;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          if (!__any_sync(0xffffffffu, mask[c])) continue;
-          uint32_t s[32];
-          tmem_ld32(tS + 32 * c, s);
-          tmem_ld_wait();
-#pragma unroll
-          for (int t = 0; t < 32; ++t) {
-            float z = __uint_as_float(s[t]);
-            if (kBias) z = score(z, k0 + 32 * c + t);
-            z = (mask[c] >> t) & 1 ? z : -INFINITY;
-            top = fmaxf(top, z);
-            if (kBias) s[t] = __float_as_uint(z);
+        // Walks the tile's four chunks of 32 keys.
+        auto walk = [&](auto each) {
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t s[32];
+            tmem_load(tS + 32 * c, s);
+            each(c, s);
           }
-          if (kBias) tmem_st32(tS + 32 * c, s);
+        };
+        float top = -INFINITY;
+        uint32_t open = 0;  // bit c: a key of chunk c is open to a row of the warp
+        if (busy)
+          walk([&](int c, uint32_t(&s)[32]) {
+            uint32_t mask = ~0u;
+            if (!whole) {
+              mask = row.bits(k0 + 32 * c);
+              if (docs) mask &= doc_bits(doc_s[32 * c + lane], row.doc);
+              if (!__any_sync(0xffffffffu, mask)) return;
+            }
+            open |= 1u << c;
+            if (kCap) {
+              float far = 0.f;
+#pragma unroll
+              for (int t = 0; t < 32; t += 2)
+                far = fmaxf(fmaxf(far, fabsf(__uint_as_float(s[t]))),
+                            fabsf(__uint_as_float(s[t + 1])));
+              if (__any_sync(0xffffffffu, far * cap_u > 0.75f)) {
+#pragma unroll
+                for (int t = 0; t < 32; ++t)
+                  s[t] = __float_as_uint(cap_exact(__uint_as_float(s[t])));
+              } else {
+#pragma unroll
+                for (int t = 0; t < 32; ++t) {
+                  const float x = __uint_as_float(s[t]);
+                  s[t] = __float_as_uint(x * cap_fit(x));
+                }
+              }
+            }
+            if (kBias == kSlopes) {
+              const float d0 = (float)(k0 + 32 * c - row.pos);
+#pragma unroll
+              for (int t = 0; t < 32; ++t) {
+                const float z = __uint_as_float(s[t]);
+                s[t] = __float_as_uint(fmaf(slope2, fabsf(d0 + (float)t), kCap ? z : z * scale2));
+              }
+            }
+            if (kBias == kTable) {
+#pragma unroll
+              for (int t = 0; t < 32; ++t) {
+                const float z = __uint_as_float(s[t]), b = window_row[32 * c + t];
+                s[t] = __float_as_uint(kCap ? z + b : fmaf(z, scale2, b));
+              }
+            }
+            if (!whole) {
+#pragma unroll
+              for (int t = 0; t < 32; ++t) s[t] = (mask >> t) & 1 ? s[t] : 0xff800000u;
+            }
+            float other = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < 32; t += 4) {
+              top = fmaxf(fmaxf(top, __uint_as_float(s[t])), __uint_as_float(s[t + 1]));
+              other = fmaxf(fmaxf(other, __uint_as_float(s[t + 2])), __uint_as_float(s[t + 3]));
+            }
+            top = fmaxf(top, other);
+            if (kCap || kBias || !whole) tmem_st32(tS + 32 * c, s);
+          });
+        if (kCap || kBias || !whole) tmem_st_wait();
+        if (!kCap && !kBias) top *= scale2;
+        if (C::kEarly && n > 0) {  // P and O are P.V's of the previous tile until it has run
+          ok = __all_sync(0xffffffffu, gate.wait(bar(kBarPV), (n - 1) & 1, kSitePV));
+          tc_fence_after();
         }
-        if (kBias) tmem_st_wait();
-        if (!kBias && top != -INFINITY) top = capped(top);  // increasing in the raw score
         const bool raise = top > m + kRescaleThreshold || (m == -INFINITY && top > m);
         if (__any_sync(0xffffffffu, raise)) {
           const float f = raise ? ex2(m - top) : 1.f;  // 0 where nothing was seen before
           if (raise) m = top;
           l *= f;
           if (n > 0) {
-#pragma unroll
-            for (int c = 0; c < kDP / 32; ++c) {
+#pragma unroll 1
+            for (uint32_t c = 0; c < kDP; c += 32) {
               uint32_t o[32];
-              tmem_ld32(tO + 32 * c, o);
-              tmem_ld_wait();
+              tmem_load(tO + c, o);
 #pragma unroll
               for (int t = 0; t < 32; ++t) o[t] = __float_as_uint(__uint_as_float(o[t]) * f);
-              tmem_st32(tO + 32 * c, o);
+              tmem_st32(tO + c, o);
             }
           }
         }
-        const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t w[16];
-          if (!__any_sync(0xffffffffu, mask[c])) {
-#pragma unroll
-            for (int t = 0; t < 16; ++t) w[t] = 0;
-          } else {
-            uint32_t s[32];
-            tmem_ld32(tS + 32 * c, s);
-            tmem_ld_wait();
-            float sum = 0.f;
-#pragma unroll
-            for (int t = 0; t < 32; ++t) {
-              float z = __uint_as_float(s[t]);
-              float e = kBias ? ex2(z - ref) : kCap ? ex2(capped(z) - ref) : ex2(fmaf(z, scale2, -ref));
-              if (!kBias) e = (mask[c] >> t) & 1 ? e : 0.f;
-              sum += e;
-              s[t] = __float_as_uint(e);
+        if (busy) {
+          const float ref = m == -INFINITY ? 0.f : m;
+          const float factor = kCap || kBias ? 1.f : scale2;
+          float sum[2] = {0.f, 0.f};
+          walk([&](int c, uint32_t(&s)[32]) {
+            if (C::kEarly && c == 3) {  // the last of S is in registers
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(bar(kBarSRead));
+              __syncwarp();  // together again before the warp-wide store below
             }
-            l += sum;
+            uint32_t w[16];
+            if ((open >> c) & 1) {
+              // Plain fp32 operations: the packed pairs (f32x2) take 3.3 to 3.9 cycles each against
+              // 0.9 to 1.4 of a single one, measured.
 #pragma unroll
-            for (int t = 0; t < 16; ++t)
-              w[t] = pack_bf16x2(__uint_as_float(s[2 * t]), __uint_as_float(s[2 * t + 1]));
-          }
-          tmem_st16(tS + 16 * c, w);
+              for (int t = 0; t < 16; ++t) {
+                const float a = ex2(fmaf(__uint_as_float(s[2 * t]), factor, -ref));
+                const float b = ex2(fmaf(__uint_as_float(s[2 * t + 1]), factor, -ref));
+                sum[0] += a;
+                sum[1] += b;
+                w[t] = pack_bf16x2(a, b);
+              }
+            } else {
+#pragma unroll
+              for (int t = 0; t < 16; ++t) w[t] = 0;
+            }
+            tmem_st16(tP + 16 * c, w);
+          });
+          l += sum[0] + sum[1];
+        } else if (C::kEarly) {
+          if (lane == 0) mbar_arrive(bar(kBarSRead));
+          __syncwarp();
         }
         // Rows of V past the sequence's end inside the last 16-key step: zero probabilities, but
         // zero times whatever lies there need not be zero.
+        const uint32_t slot = n % C::kSlots, tile_v = sbase + C::kOffV + slot * C::kTile;
         const int keys = min(u.s.nk - k0, kKeys), clear = (keys + 15) / 16 * 16;
         if (keys < clear) {
-          const uint32_t slot = n % C::kSlots;
-          ok = __all_sync(0xffffffffu, gate.wait(bar(kBarVFull + slot), (n / C::kSlots) & 1, kSiteVRead));
-          for (int x = keys * (kDP / 8) + r; x < clear * (kDP / 8); x += 128) {
-            const int vr = x / (kDP / 8), ch = x % (kDP / 8);
-            st_shared_v4(sbase + C::kOffV + slot * C::kTile + (ch >> 3) * C::kAtom + vr * 128 +
-                             (ch & 7) * 16,
+          ok = __all_sync(0xffffffffu, gate.wait(bar(kBarVFull + slot), (n / C::kSlots) & 1, kSiteVRead)) && ok;
+          for (int x = keys * (kDP / 8) + r; x < clear * (kDP / 8); x += 128)
+            st_shared_v4(tile_v + ((x % (kDP / 8)) >> 3) * C::kAtom + x / (kDP / 8) * 128 +
+                             (x & 7) * 16,
                          0, 0, 0, 0);
-          }
           fence_proxy_async();
         }
         tmem_st_wait();
-        if (!whole_tile(p, u, k0)) {
+        if (!whole) {
           ok = __all_sync(0xffffffffu, gate.wait(bar(kBarScan), scans++ & 1, kSiteScan)) && ok;
-          const volatile uint32_t *bad = reinterpret_cast<uint32_t *>(misc + kOffBad);
-          if (ok && (bad[0] | bad[1] | bad[2] | bad[3]))
-            add_by_hand<kDP>(bad, sbase + C::kOffV + (n % C::kSlots) * C::kTile, C::kAtom, tS, tO,
-                             n == 0, r, gate, bar(kBarHand), hands++);
+          const volatile uint32_t *odd = reinterpret_cast<uint32_t *>(misc + kOffBad);
+          if (ok && (odd[0] | odd[1] | odd[2] | odd[3]))
+            ok = add_by_hand<kDP>(odd, tile_v, C::kAtom, tP, tO, n == 0, gate, bar(kBarHand),
+                                  hands++);
         }
         tc_fence_before();
         mbar_arrive(bar(kBarP));
       }
-      ok = __all_sync(0xffffffffu, ok && gate.wait(bar(kBarO), 0, kSiteO));
+      ok = __all_sync(0xffffffffu, gate.wait(bar(kBarO), 0, kSiteO)) && ok;
       tc_fence_after();
       if (ok) {
         const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -469,8 +578,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         for (uint32_t c = 0; c < kDP; c += 32) {
           if (c >= p.dim) break;
           uint32_t o[32];
-          tmem_ld32(tO + c, o);
-          tmem_ld_wait();
+          tmem_load(tO + c, o);
           const int cols = min(32, (int)(p.dim - c));
           if (!part) {
 #pragma unroll
@@ -618,6 +726,7 @@ void scored_plan(ScoredProblem *p, bool tc, int num_sms) {
   p->rows = tc ? 128 : 64;
   p->pack = group & (0u - group);
   if (p->pack > p->rows) p->pack = p->rows;
+  if (tc && p->table && p->pack > scored::kTablePack) p->pack = scored::kTablePack;
   const uint32_t per = p->rows / p->pack;
   p->tiles = (p->max_q + per - 1) / per;
   const uint64_t units = (uint64_t)p->tiles * p->nseq * (p->heads / p->pack);

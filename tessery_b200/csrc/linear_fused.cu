@@ -233,7 +233,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     // Warp w finishes columns [half * kCols, +kCols) of the 32 rows of its tensor-memory quarter.
     constexpr uint32_t kCols = kBN / 2;
     const uint32_t quarter = (uint32_t)warp & 3, half = (uint32_t)(warp - 2) >> 2;
-    const uint32_t lane_row = quarter * 32 + lane;
     const uint32_t staging = sbase + C::kOffStaging + (uint32_t)(warp - 2) * 2 * kBufBytes;
     const uint32_t res_bar = kBarRes + 2 * (uint32_t)(warp - 2);
     const int mode = kBN >= 128 ? p.epilogue : kDirect;
@@ -268,25 +267,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           break;
         tc_fence_after();
         const uint32_t t0 = tmem + b * kBN + half * kCols + ((quarter * 32u) << 16);
-        if (part == 0) {
-          uint32_t a[kCols / 16][16];
 #pragma unroll
-          for (uint32_t c = 0; c < kCols / 16; ++c) tmem_ld16(t0 + 16 * c, a[c]);
-          tmem_ld_wait();
+        for (uint32_t c = 0; c < kCols; c += 16) {
+          uint32_t a[16];
+          tmem_load(t0 + c, a);
 #pragma unroll
-          for (uint32_t c = 0; c < kCols; ++c) {
-            asm volatile("" : "+r"(a[c / 16][c % 16]));  // no use above the wait
-            v[c] = __uint_as_float(a[c / 16][c % 16]);
-          }
-        } else {
-#pragma unroll
-          for (uint32_t c = 0; c < kCols; c += 16) {
-            uint32_t a[16];
-            tmem_ld16(t0 + c, a);
-            tmem_ld_wait();
-#pragma unroll
-            for (int t = 0; t < 16; ++t) v[c + t] += __uint_as_float(a[t]);
-          }
+          for (int t = 0; t < 16; ++t)
+            v[c + t] = part ? v[c + t] + __uint_as_float(a[t]) : __uint_as_float(a[t]);
         }
         tc_fence_before();
         mbar_arrive(bar(kBarFree + b));
