@@ -20,7 +20,7 @@ LIBRARY = PACKAGE / "libtessattn.so"
 SOURCES = ["runtime.cu", "simt_kernels.cu", "attn_d32.cu", "attn_d32_tc.cu", "attn_f32_tc.cu", "attn_tc.cu", "attn_short.cu", "noalloc.cu",
            "pool.cu", "linear.cu", "qwen_ops.cu", "qwen3_model.cu",
            "bert_ops.cu", "bert_model.cu",
-           "rotary.cu", "attn_scored_tc.cu", "attn_scored_f32.cu", "linear_fused.cu"]
+           "rotary.cu", "attn_scored_tc.cu", "attn_scored_f32.cu", "attn_scored_few.cu", "linear_fused.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

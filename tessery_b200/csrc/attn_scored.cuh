@@ -72,7 +72,8 @@ __device__ __forceinline__ void row_range(const ScoredProblem &p, int pos, int n
 }
 
 // Blocks run the last token tiles first: under a causal rule they see the most keys.
-template <int kRows>
+// kTile: keys of a visited tile.
+template <int kRows, int kTile = kKeys>
 __device__ __forceinline__ Unit make_unit(const ScoredProblem &p, uint32_t block) {
   Unit u;
   const uint32_t groups = p.heads / p.pack;
@@ -102,9 +103,9 @@ __device__ __forceinline__ Unit make_unit(const ScoredProblem &p, uint32_t block
     u.whole_hi = first_hi;
     u.whole_prefix = u.prefix;
   }
-  u.a = (u.prefix + kKeys - 1) / kKeys;
-  u.b = max(u.a, lo / kKeys);
-  const int end = hi > lo ? (hi + kKeys - 1) / kKeys : 0;
+  u.a = (u.prefix + kTile - 1) / kTile;
+  u.b = max(u.a, lo / kTile);
+  const int end = hi > lo ? (hi + kTile - 1) / kTile : 0;
   const int count = u.a + max(0, end - u.b);
   u.first = (int)((long long)count * u.split / p.splits);
   u.last = (int)((long long)count * (u.split + 1) / p.splits);

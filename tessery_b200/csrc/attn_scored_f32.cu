@@ -86,7 +86,7 @@ __device__ __forceinline__ bool stage(const ScoredProblem &p, float *dst, const 
 }
 
 template <int kDP>
-__global__ void __launch_bounds__(kThreads) scored_f32_kernel(const __grid_constant__ ScoredProblem p) {
+__global__ void __launch_bounds__(kThreads, kDP <= 64 ? 4 : 1) scored_f32_kernel(const __grid_constant__ ScoredProblem p) {
   using C = Cfg<kDP>;
   extern __shared__ __align__(16) uint8_t smem[];
   float *qs = reinterpret_cast<float *>(smem + C::kOffQ);

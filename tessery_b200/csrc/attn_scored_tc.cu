@@ -719,20 +719,33 @@ cudaError_t launch_scored_tc(const ScoredProblem &p, cudaStream_t stream) {
   return p.dim <= 64 ? scored_rule<64>(p, m, stream) : scored_rule<128>(p, m, stream);
 }
 
-// The cut of a launch.  Rows: the heads of a pack times tokens.  Splits of the key range: while
-// the units do not fill two CTAs per SM and a part would still hold two key tiles.
-void scored_plan(ScoredProblem *p, bool tc, int num_sms) {
+ScoredRoute scored_route(const ScoredProblem &p) {
+  if (p.rows_k && scored_few_supported(p)) return kScoredFew;
+  return p.rows_k && scored_tc_supported(p) ? kScoredTc : kScoredF32;
+}
+
+// The cut of a launch.  Rows: the heads of a pack times tokens (few rows: all heads of a kv head,
+// whatever their number).  Splits of the key range: as many as the CTAs that run at once leave
+// room for, while a part keeps a few key blocks.
+void scored_plan(ScoredProblem *p, ScoredRoute route, int num_sms) {
   const uint32_t group = p->heads / p->kv_heads;
-  p->rows = tc ? 128 : 64;
-  p->pack = group & (0u - group);
-  if (p->pack > p->rows) p->pack = p->rows;
-  if (tc && p->table && p->pack > scored::kTablePack) p->pack = scored::kTablePack;
+  uint32_t slots = 2 * (uint32_t)num_sms, least = 2 * scored::kKeys;  // CTAs at once, keys a part
+  if (route == kScoredFew) {
+    p->rows = 16;
+    p->pack = group;
+    least = 128;
+    slots = (uint32_t)(scored_few_resident(*p) * num_sms);
+  } else {
+    p->rows = route == kScoredTc ? 128 : 64;
+    p->pack = group & (0u - group);
+    if (p->pack > p->rows) p->pack = p->rows;
+    if (route == kScoredTc && p->table && p->pack > scored::kTablePack) p->pack = scored::kTablePack;
+  }
   const uint32_t per = p->rows / p->pack;
   p->tiles = (p->max_q + per - 1) / per;
   const uint64_t units = (uint64_t)p->tiles * p->nseq * (p->heads / p->pack);
-  const uint64_t want = (2ull * (uint64_t)num_sms + units - 1) / units;
-  const uint64_t parts = (p->max_k + 2 * scored::kKeys - 1) / (2 * scored::kKeys);
-  p->splits = units >= 2ull * (uint64_t)num_sms ? 1u : (uint32_t)(want < parts ? want : parts);
+  const uint64_t fit =  slots / units, parts = (p->max_k + least - 1) / least;
+  p->splits = (uint32_t)(fit < parts ? fit : parts);
   if (!p->splits) p->splits = 1;
   p->part_dp = (p->dim + 3) & ~3u;
 }

@@ -206,9 +206,15 @@ struct ScoredProblem {
   float2 *part_ml;
   uint32_t *part_arrived;
 };
-// Fills the cut, without the partials; `tc`: the tensor-core kernel's.
-void scored_plan(ScoredProblem *p, bool tc, int num_sms);
+// The kernel that takes a problem: few rows per kv head, tensor memory, or fp32 accuracy.
+enum ScoredRoute : int { kScoredFew = 0, kScoredTc = 1, kScoredF32 = 2 };
+ScoredRoute scored_route(const ScoredProblem &p);
+// Fills the cut, without the partials.
+void scored_plan(ScoredProblem *p, ScoredRoute route, int num_sms);
+bool scored_few_supported(const ScoredProblem &p);
+int scored_few_resident(const ScoredProblem &p);  // CTAs at once on an SM
 bool scored_tc_supported(const ScoredProblem &p);
+cudaError_t launch_scored_few(const ScoredProblem &p, cudaStream_t stream);
 cudaError_t launch_scored_tc(const ScoredProblem &p, cudaStream_t stream);
 cudaError_t launch_scored_f32(const ScoredProblem &p, cudaStream_t stream);
 cudaError_t launch_rotary(const RotaryProblem &p, cudaStream_t stream);

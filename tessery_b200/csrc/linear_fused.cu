@@ -237,7 +237,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t res_bar = kBarRes + 2 * (uint32_t)(warp - 2);
     const int mode = kBN >= 128 ? p.epilogue : kDirect;
     const bool f32_out = p.out_dtype == 0;
-    uint32_t done = 0, res_loads = 0, res_used = 0;  // residual boxes asked for and consumed
+    uint32_t done = 0, sent = 0;               // partial sums taken, boxes stored
+    uint32_t res_loads = 0, res_used = 0;      // residual boxes asked for and consumed
     bool ok = true;
     // Residual box number `res_loads` (columns from n, rows from m) into its buffer, once the
     // store that last left from there has been read.
@@ -256,51 +257,27 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t box = f32_out ? 32 : 64;  // columns of a 128-byte staging row
       const bool rows = m0 < p.m && n0 < p.n;  // this warp has something to write
       if (mode == kStagedRes && rows) load_residual(n0, m0);
-      // The tile's sums: partial sums of 512 K are added in fp32 registers.  The accumulator cuts
-      // off bits at each of its additions, always towards zero: over 2048 K in one go that left
-      // an error of 2e-6 of the result, eight times that of fp32 products in fp32.
-      float v[kCols];
-      for (uint32_t part = 0; part < parts; ++part, ++done) {
-        const uint32_t b = done & 1;
-        if (!(ok = __all_sync(0xffffffffu, wait_bar(bar(kBarAcc + b), (done >> 1) & 1, abort_flag,
-                                                    p.status, kSiteAcc, p.wait_cycles))))
-          break;
-        tc_fence_after();
-        const uint32_t t0 = tmem + b * kBN + half * kCols + ((quarter * 32u) << 16);
-#pragma unroll
-        for (uint32_t c = 0; c < kCols; c += 16) {
-          uint32_t a[16];
-          tmem_load(t0 + c, a);
-#pragma unroll
-          for (int t = 0; t < 16; ++t)
-            v[c + t] = part ? v[c + t] + __uint_as_float(a[t]) : __uint_as_float(a[t]);
-        }
-        tc_fence_before();
-        mbar_arrive(bar(kBarFree + b));
-      }
-      if (!ok) break;
-      if (!rows) continue;
-#pragma unroll
-      for (uint32_t c = 0; c < kCols; c += 32) {
+      // Bias, activation, residual and store of columns [c, c + 32) of this warp's share.
+      auto finish = [&](uint32_t c, float *v) {
         const uint32_t n = n0 + c;
-        if (n < p.n && ok) {
+        if (rows && n < p.n && ok) {
         const bool whole = n + 32 <= p.n;
         if (p.bias) {
           if (whole && p.bias_vec) {
 #pragma unroll
             for (int t = 0; t < 8; ++t) {
               const float4 q = __ldg(reinterpret_cast<const float4 *>(p.bias + n) + t);
-              v[c + 4 * t] += q.x; v[c + 4 * t + 1] += q.y;
-              v[c + 4 * t + 2] += q.z; v[c + 4 * t + 3] += q.w;
+              v[4 * t] += q.x; v[4 * t + 1] += q.y;
+              v[4 * t + 2] += q.z; v[4 * t + 3] += q.w;
             }
           } else {
 #pragma unroll
             for (int t = 0; t < 32; ++t)
-              if (n + t < p.n) v[c + t] += __ldg(p.bias + n + t);
+              if (n + t < p.n) v[t] += __ldg(p.bias + n + t);
           }
         }
 #pragma unroll
-        for (int t = 0; t < 32; ++t) v[c + t] = activate<kAct>(v[c + t]);
+        for (int t = 0; t < 32; ++t) v[t] = activate<kAct>(v[t]);
         if (p.residual && mode != kStagedRes && m < p.m) {
           const size_t at = (size_t)m * p.ldr + n;
           if (whole && p.res_vec && p.residual_dtype == 0) {
@@ -308,8 +285,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int t = 0; t < 8; ++t) {
               const float4 q = reinterpret_cast<const float4 *>(
                   static_cast<const float *>(p.residual) + at)[t];
-              v[c + 4 * t] += q.x; v[c + 4 * t + 1] += q.y;
-              v[c + 4 * t + 2] += q.z; v[c + 4 * t + 3] += q.w;
+              v[4 * t] += q.x; v[4 * t + 1] += q.y;
+              v[4 * t + 2] += q.z; v[4 * t + 3] += q.w;
             }
           } else if (whole && p.res_vec) {
 #pragma unroll
@@ -318,14 +295,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                   static_cast<const uint16_t *>(p.residual) + at)[t];
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                v[c + 8 * t + 2 * e] += bf16_lo(u4_at(q, e));
-                v[c + 8 * t + 2 * e + 1] += bf16_hi(u4_at(q, e));
+                v[8 * t + 2 * e] += bf16_lo(u4_at(q, e));
+                v[8 * t + 2 * e + 1] += bf16_hi(u4_at(q, e));
               }
             }
           } else {
 #pragma unroll
             for (int t = 0; t < 32; ++t)
-              if (n + t < p.n) v[c + t] += residual_at(p, at + t);
+              if (n + t < p.n) v[t] += residual_at(p, at + t);
           }
         }
         if (mode == kDirect) {
@@ -335,19 +312,19 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int t = 0; t < 8; ++t)
               reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at)[t] = make_float4(
-                  v[c + 4 * t], v[c + 4 * t + 1], v[c + 4 * t + 2], v[c + 4 * t + 3]);
+                  v[4 * t], v[4 * t + 1], v[4 * t + 2], v[4 * t + 3]);
           } else if (whole && p.out_vec) {
 #pragma unroll
             for (int t = 0; t < 4; ++t)
               reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.out) + at)[t] =
-                  make_uint4(pack_bf16x2(v[c + 8 * t], v[c + 8 * t + 1]),
-                             pack_bf16x2(v[c + 8 * t + 2], v[c + 8 * t + 3]),
-                             pack_bf16x2(v[c + 8 * t + 4], v[c + 8 * t + 5]),
-                             pack_bf16x2(v[c + 8 * t + 6], v[c + 8 * t + 7]));
+                  make_uint4(pack_bf16x2(v[8 * t], v[8 * t + 1]),
+                             pack_bf16x2(v[8 * t + 2], v[8 * t + 3]),
+                             pack_bf16x2(v[8 * t + 4], v[8 * t + 5]),
+                             pack_bf16x2(v[8 * t + 6], v[8 * t + 7]));
           } else {
 #pragma unroll
             for (int t = 0; t < 32; ++t)
-              if (n + t < p.n) store_at(p, at + t, v[c + t]);
+              if (n + t < p.n) store_at(p, at + t, v[t]);
           }
         } else if constexpr (kBN >= 128) {
           // A staging row is 128 bytes of this lane's output row, its 16-byte pieces swizzled as
@@ -363,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                                     abort_flag, p.status, kSiteRes, p.wait_cycles));
             }
           } else {
-            b = (c / box) & 1;
+            b = sent & 1;
             if (starts) {
               if (lane == 0) bulk_wait_read<1>();
               __syncwarp();
@@ -376,13 +353,13 @@ __global__ void __launch_bounds__(kThreads, 1)
               const uint32_t at = row + ((q ^ sw) << 4);
               if (mode == kStagedRes) {
                 const uint4 o = ld_shared_v4(at);
-                v[c + 4 * q] += __uint_as_float(o.x);
-                v[c + 4 * q + 1] += __uint_as_float(o.y);
-                v[c + 4 * q + 2] += __uint_as_float(o.z);
-                v[c + 4 * q + 3] += __uint_as_float(o.w);
+                v[4 * q] += __uint_as_float(o.x);
+                v[4 * q + 1] += __uint_as_float(o.y);
+                v[4 * q + 2] += __uint_as_float(o.z);
+                v[4 * q + 3] += __uint_as_float(o.w);
               }
-              st_shared_v4(at, __float_as_uint(v[c + 4 * q]), __float_as_uint(v[c + 4 * q + 1]),
-                           __float_as_uint(v[c + 4 * q + 2]), __float_as_uint(v[c + 4 * q + 3]));
+              st_shared_v4(at, __float_as_uint(v[4 * q]), __float_as_uint(v[4 * q + 1]),
+                           __float_as_uint(v[4 * q + 2]), __float_as_uint(v[4 * q + 3]));
             }
           } else {
 #pragma unroll
@@ -392,14 +369,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint4 o = ld_shared_v4(at);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                  v[c + 8 * q + 2 * e] += bf16_lo(u4_at(o, e));
-                  v[c + 8 * q + 2 * e + 1] += bf16_hi(u4_at(o, e));
+                  v[8 * q + 2 * e] += bf16_lo(u4_at(o, e));
+                  v[8 * q + 2 * e + 1] += bf16_hi(u4_at(o, e));
                 }
               }
-              st_shared_v4(at, pack_bf16x2(v[c + 8 * q], v[c + 8 * q + 1]),
-                           pack_bf16x2(v[c + 8 * q + 2], v[c + 8 * q + 3]),
-                           pack_bf16x2(v[c + 8 * q + 4], v[c + 8 * q + 5]),
-                           pack_bf16x2(v[c + 8 * q + 6], v[c + 8 * q + 7]));
+              st_shared_v4(at, pack_bf16x2(v[8 * q], v[8 * q + 1]),
+                           pack_bf16x2(v[8 * q + 2], v[8 * q + 3]),
+                           pack_bf16x2(v[8 * q + 4], v[8 * q + 5]),
+                           pack_bf16x2(v[8 * q + 6], v[8 * q + 7]));
             }
           }
           if (ends || n + 32 >= p.n) {
@@ -409,10 +386,60 @@ __global__ void __launch_bounds__(kThreads, 1)
               tma_store_2d(&tm_out, staging + b * kBufBytes, (int)(n - c % box), (int)m0);
               bulk_commit();
             }
+            ++sent;
             if (mode == kStagedRes) ++res_used;
           }
         }
         }
+        __syncwarp();
+      };
+      const uint32_t lanes = (quarter * 32u) << 16;
+      if (parts > 1) {
+        // Partial sums of 512 K are added in fp32 registers: the accumulator cuts off bits at each of
+        // its additions, always towards zero, and over 2048 K in one go that left an error of 2e-6
+        // of the result, eight times that of fp32 products in fp32.  The accumulator is free again
+        // before the epilogue (putting the sum back into it for the rolled loop below: 169 -> 194 us
+        // at 33500 x 1024 x 2048).
+        float v[kCols];
+        for (uint32_t part = 0; part < parts; ++part, ++done) {
+          const uint32_t b = done & 1, t0 = tmem + b * kBN + half * kCols + lanes;
+          if (!(ok = __all_sync(0xffffffffu, wait_bar(bar(kBarAcc + b), (done >> 1) & 1, abort_flag,
+                                                      p.status, kSiteAcc, p.wait_cycles))))
+            break;
+          tc_fence_after();
+#pragma unroll
+          for (uint32_t c = 0; c < kCols; c += 16) {
+            uint32_t a[16];
+            tmem_load(t0 + c, a);
+#pragma unroll
+            for (int t = 0; t < 16; ++t)
+              v[c + t] = part ? v[c + t] + __uint_as_float(a[t]) : __uint_as_float(a[t]);
+          }
+          tc_fence_before();
+          mbar_arrive(bar(kBarFree + b));
+        }
+#pragma unroll
+        for (uint32_t c = 0; c < kCols; c += 32) finish(c, v + c);
+      } else {
+        const uint32_t b = done & 1, t0 = tmem + b * kBN + half * kCols + lanes;
+        ok = __all_sync(0xffffffffu, wait_bar(bar(kBarAcc + b), (done >> 1) & 1, abort_flag,
+                                              p.status, kSiteAcc, p.wait_cycles));
+        if (!ok) break;
+        tc_fence_after();
+        ++done;
+        // Rolled: unrolled over the columns the epilogue did not stay in the instruction cache (36.5
+        // against 32.8 us at 8192 x 1536 x 384 with GELU).
+#pragma unroll 1
+        for (uint32_t c = 0; c < kCols; c += 32) {
+          uint32_t acc[32];
+          float v[32];
+          tmem_load(t0 + c, acc);
+#pragma unroll
+          for (int t = 0; t < 32; ++t) v[t] = __uint_as_float(acc[t]);
+          finish(c, v);
+        }
+        tc_fence_before();
+        mbar_arrive(bar(kBarFree + b));
       }
     }
     if (mode != kDirect) {

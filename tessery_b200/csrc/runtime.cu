@@ -1781,8 +1781,8 @@ int tx_attention_scored(void *ctx, const TxRows *q, const TxRows *k, const TxRow
   p.prefix = r.prefix; p.q_docs = r.q_docs; p.k_docs = r.k_docs;
   p.status = c->status;
   p.wait_cycles = c->wait_cycles > 0 ? c->wait_cycles : 2000000000ll;
-  const bool tc = k_layout->rows && tx::scored_tc_supported(p);
-  tx::scored_plan(&p, tc, c->sms);
+  const tx::ScoredRoute route = tx::scored_route(p);
+  tx::scored_plan(&p, route, c->sms);
   const uint64_t units = (uint64_t)p.tiles * nseq * (heads / p.pack);
   if (units * p.splits > 0x7fffffffull)
     return fail(c, TX_EINVAL, "attention_scored: problem too large");
@@ -1799,11 +1799,15 @@ int tx_attention_scored(void *ctx, const TxRows *q, const TxRows *k, const TxRow
     p.part_ml = (float2 *)(c->part_mem + counters + rows * p.part_dp * 4);
     if ((e = scratch_acquire(c, st)) != cudaSuccess) return cuda_fail(c, e, "scratch wait");
   }
-  e = tc ? tx::launch_scored_tc(p, st) : tx::launch_scored_f32(p, st);
+  e = route == tx::kScoredFew  ? tx::launch_scored_few(p, st)
+      : route == tx::kScoredTc ? tx::launch_scored_tc(p, st)
+                               : tx::launch_scored_f32(p, st);
   if (e != cudaSuccess) return cuda_fail(c, e, "attention_scored launch");
   if (p.splits > 1 && (e = scratch_release(c, st)) != cudaSuccess)
     return cuda_fail(c, e, "scratch event");
-  c->last_kernel = tc ? "scored_tc" : "scored_f32";
+  c->last_kernel = route == tx::kScoredFew  ? "scored_few"
+                   : route == tx::kScoredTc ? "scored_tc"
+                                            : "scored_f32";
   ++c->launches;
   return TX_OK;
 }

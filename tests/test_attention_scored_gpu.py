@@ -7,6 +7,9 @@ scale sum |q||k|) plus the cap:
   off by 2^-21 of sum |q||k| at worst (lo parts truncated to 2^-11, lo.lo dropped), the cap,
   bias, scaling to log2 units and exp2 by a few 2^-23 of Z; dz <= 2^-20 (Z + 1) covers them.
   P.V in split TF32 and the sums add 2^-20 A.  Gate: (2 (Z + 1) + 1) 2^-20 A.
+- Few-rows route: fp32 as above.  bf16: P is rounded to TF32, 2^-11 of each weight, and scores are
+  off by 2^-19 (Z + 1) (16 more additions in the tensor core, cut rather than rounded): gate
+  (2^-11 + (2 (Z + 1) + 1) 2^-19) A.
 - Tensor-memory route: bf16 inputs are exact, dz <= 2^-19 (Z + 1) (hardware exp2 and reciprocal);
   P is rounded to bf16, 2^-8 of each weight: 2^-8 A.  Gate: (2^-8 + 2^-18 (Z + 1)) A.
 - bf16 output: 2^-8 of the value more.  A term of 1e-30 admits exact zeros."""
@@ -27,9 +30,14 @@ def make(rng, shape, dtype, scale=1.0):
     return (to_bf16_bits(x), from_bf16_bits(to_bf16_bits(x))) if dtype == "bf16" else (x, x)
 
 
-def gate(want, mass, big, cap, route, bf16):
+def gate(want, mass, big, cap, route, bf16, dtype="bf16"):
     z = big + cap + 1
-    rel = (2 * z + 1) * 2.0**-20 if route == "scored_f32" else 2.0**-8 + z * 2.0**-18
+    if route == "scored_f32" or (route == "scored_few" and dtype == "f32"):
+        rel = (2 * z + 1) * 2.0**-20
+    elif route == "scored_few":
+        rel = 2.0**-11 + (2 * z + 1) * 2.0**-19
+    else:
+        rel = 2.0**-8 + z * 2.0**-18
     return rel * mass + (np.abs(want) * 2.0**-8 if bf16 else 0.0) + 1e-30
 
 
@@ -67,7 +75,7 @@ def run_packed(runtime, lens_q, lens_k, heads, kv_heads, dim, dtype, *, out=None
             qf[a], kf[b], vf[b], table=table, prefix=0 if prefix is None else int(prefix[s]),
             q_docs=None if docs is None else q_docs[a], k_docs=None if docs is None else k_docs[b],
             **rule)
-        tol = gate(want, mass, big, rule.get("softcap", 0.0), took, bf16)
+        tol = gate(want, mass, big, rule.get("softcap", 0.0), took, bf16, dtype)
         bad = ~(np.abs(gf[a] - want) <= tol) & ~(np.isnan(want) & np.isnan(gf[a])) \
             & ~(np.isinf(want) & (want == gf[a]))
         assert not bad.any(), (s, np.argwhere(bad)[:4], gf[a][bad][:4], want[bad][:4])
@@ -170,9 +178,28 @@ def test_new_tokens_against_kept_keys(runtime, dtype, new, shape):
     """Few query rows, long keys: the key range is split and joined."""
     lens_k = [1, 5, 700, 3000, 129, 2049]
     lens_q = [min(new, n) for n in lens_k]
-    run_packed(runtime, lens_q, lens_k, *shape, dtype)
-    run_packed(runtime, lens_q, lens_k, *shape, dtype, softcap=10.0, window=(900, -1),
+    few = new * (shape[0] // shape[1]) <= 16
+    route = "scored_few" if few else "scored_tc" if dtype == "bf16" else "scored_f32"
+    run_packed(runtime, lens_q, lens_k, *shape, dtype, route=route)
+    run_packed(runtime, lens_q, lens_k, *shape, dtype, route=route, softcap=10.0, window=(900, -1),
                prefix=np.array([1, 0, 3, 200, 0, 5], np.int32))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 2, 8), (10, 2, 40), (3, 1, 72), (16, 1, 256),
+                                                (7, 7, 136), (9, 3, 24)])
+def test_few_rows_of_any_group_and_dim(runtime, heads, kv_heads, dim, dtype):
+    """Groups that are no power of two, head_dims between the compiled ones, every rule."""
+    lens_k = [300, 1, 17, 1000]
+    kw = dict(route="scored_few")
+    run_packed(runtime, [1] * 4, lens_k, heads, kv_heads, dim, dtype, out="float32", **kw)
+    run_packed(runtime, [1] * 4, lens_k, heads, kv_heads, dim, dtype, slopes=slopes_of(heads),
+               softcap=9.0, window=(200, -1), **kw)
+    run_packed(runtime, [1] * 4, lens_k, heads, kv_heads, dim, dtype,
+               distance_bias=table_of(heads, 20), docs=lambda rng, n: rng.integers(-1, 3, size=n),
+               **kw)
+    run_packed(runtime, [1] * 4, lens_k, heads, kv_heads, dim, dtype, window=(30, 0),
+               prefix=np.array([40, 0, 17, 5], np.int32), qk_scale=3.0, **kw)
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
@@ -373,9 +400,9 @@ def test_wait_limit_is_reported_and_the_runtime_goes_on(runtime):
 
     runtime.set_wait_limit(1)
     try:
-        for lens_q, lens_k in (([300], [300]), ([1, 1], [3000, 900])):
+        for lens_q, lens_k in (([300], [300]), ([9, 9], [3000, 900])):
             with pytest.raises(DeviceTimeoutError):
                 run_packed(runtime, lens_q, lens_k, 4, 2, 128, "bf16")
     finally:
         runtime.set_wait_limit(0)
-    run_packed(runtime, [1, 1], [3000, 900], 4, 2, 128, "bf16", route="scored_tc")
+    run_packed(runtime, [9, 9], [3000, 900], 4, 2, 128, "bf16", route="scored_tc")

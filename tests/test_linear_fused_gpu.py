@@ -85,6 +85,21 @@ def test_wide_tiles(runtime):
               "none", r)
 
 
+@pytest.mark.parametrize("m,n,k", [(14000, 256, 72), (20000, 264, 600), (700, 1000, 1400)])
+@pytest.mark.parametrize("out", ["float32", "bf16"])
+def test_several_tiles_in_turn(runtime, m, n, k, out):
+    """CTAs that send several tiles through the same staging buffers; sums in several parts."""
+    rng = np.random.default_rng(m)
+    x, xf = bf16(rng, (m, k))
+    w, wf = bf16(rng, (n, k), k**-0.5)
+    bias = rng.standard_normal(n).astype(np.float32)
+    check(linear_fused(x, w, bias=bias, activation="gelu", out_dtype=out, runtime=runtime), xf, wf,
+          bias, "gelu", None)
+    r, rf = bf16(rng, (m, n))
+    r = rf if out == "float32" else r
+    check(linear_fused(x, w, residual=r, out_dtype=out, runtime=runtime), xf, wf, None, "none", rf)
+
+
 @pytest.mark.parametrize("m", [3, 150])
 @pytest.mark.parametrize("odd", [0, 1])
 @pytest.mark.parametrize("out", [TX_F32, TX_BF16])
