@@ -483,8 +483,8 @@ typedef struct {
  * finite.  bf16 with dim a multiple of 8 up to 128, strides multiples of 8 and 16-byte aligned
  * pointers runs on the tensor-memory kernel (P rounded to bf16), everything else in fp32
  * accuracy. */
-int tx_attention_scored(void *ctx, const TxRows *q, const TxRows *k, const TxRows *v, void *out,
-                        const TxLayout *q_layout, const TxLayout *k_layout, uint32_t nseq,
+int tx_attention_scored(void *ctx, const TxRows *qkv /* [3] */, void *out,
+                        const TxLayout *layouts /* [2]: q's, then k's and v's */, uint32_t nseq,
                         uint32_t heads, uint32_t kv_heads, uint32_t dim, int in_dtype,
                         int out_dtype, float scale, const TxScoreRule *rule, void *stream);
 

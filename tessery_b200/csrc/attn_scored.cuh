@@ -16,7 +16,7 @@ namespace scored {
 
 constexpr int kKeys = 128;        // keys per tile
 constexpr uint32_t kTablePack = 4;  // most heads of a pack with a distance table (tensor-memory route)
-constexpr uint32_t kDocWords = 1024;  // bits for the key tiles of a document mask: 32768 tiles
+constexpr uint32_t kDocWords = 512;  // bits for the key tiles of a document mask: 16384 tiles
 
 struct Seq {
   int q_row, k_row;  // first row of the sequence in q and k

@@ -314,8 +314,8 @@ __global__ void __launch_bounds__(kThreads, kDP <= 64 ? 4 : 1) scored_f32_kernel
 template <int kDP>
 cudaError_t launch(const ScoredProblem &p, cudaStream_t stream) {
   constexpr uint32_t smem = Cfg<kDP>::kSmemBytes;
-  cudaError_t e = cudaFuncSetAttribute(scored_f32_kernel<kDP>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static std::atomic<uint64_t> seen{0};
+  cudaError_t e = allow_smem((const void *)scored_f32_kernel<kDP>, (int)smem, seen);
   if (e != cudaSuccess) return e;
   const uint32_t grid = p.tiles * p.nseq * (p.heads / p.pack) * p.splits;
   scored_f32_kernel<kDP><<<grid, kThreads, smem, stream>>>(p);

@@ -447,8 +447,8 @@ __global__ void __launch_bounds__(Cfg<T, kDP>::kThreads)
 template <typename T, int kDP>
 cudaError_t launch(const ScoredProblem &p, cudaStream_t stream) {
   using C = Cfg<T, kDP>;
-  cudaError_t e = cudaFuncSetAttribute(scored_few_kernel<T, kDP>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+  static std::atomic<uint64_t> seen{0};
+  cudaError_t e = allow_smem((const void *)scored_few_kernel<T, kDP>, C::kSmemBytes, seen);
   if (e != cudaSuccess) return e;
   const uint32_t grid = p.tiles * p.nseq * (p.heads / p.pack) * p.splits;
   scored_few_kernel<T, kDP><<<grid, C::kThreads, C::kSmemBytes, stream>>>(p);

@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace tx {
 
 // One attention problem, in element units.  Pointers are device addresses.
@@ -155,6 +157,17 @@ cudaError_t launch_linear(const void *x, const void *x_lo, const void *w, const 
                           cudaStream_t stream);
 
 // ---- Encoder layers with other options (rotary.cu, attn_scored*.cu, linear_fused.cu) ----
+// Allows `kernel` its dynamic shared memory, once per device (`seen`: bit per device).
+inline cudaError_t allow_smem(const void *kernel, int bytes, std::atomic<uint64_t> &seen) {
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if (seen.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) seen.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
 // One side (q or k) of the rotation: strides in elements, heads 0 when absent.
 struct RotaryTensor {
   const void *x;

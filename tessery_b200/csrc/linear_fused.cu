@@ -567,8 +567,8 @@ cudaError_t launch_tiles(const LinearFusedProblem &p, int num_sms, cudaStream_t 
   if (p.epilogue == kStagedRes &&
       !make_map(&mr, p.residual, p.m, p.n, p.ldr, 32, p.out_dtype == TX_F32))
     return cudaErrorInvalidValue;
-  cudaError_t e = cudaFuncSetAttribute(linear_kernel<kBN, kAct>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static std::atomic<uint64_t> seen{0};
+  cudaError_t e = allow_smem((const void *)linear_kernel<kBN, kAct>, (int)smem, seen);
   if (e != cudaSuccess) return e;
   const uint64_t tiles = (uint64_t)((p.n + kBN - 1) / kBN) * ((p.m + kBM - 1) / kBM);
   if (tiles > 0x7fffffffull) return cudaErrorInvalidValue;

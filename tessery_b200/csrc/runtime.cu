@@ -1721,15 +1721,16 @@ int tx_rotary(void *ctx, const TxRotaryTensor *q, const TxRotaryTensor *k, int i
   return TX_OK;
 }
 
-int tx_attention_scored(void *ctx, const TxRows *q, const TxRows *k, const TxRows *v, void *out,
-                        const TxLayout *q_layout, const TxLayout *k_layout, uint32_t nseq,
-                        uint32_t heads, uint32_t kv_heads, uint32_t dim, int in_dtype,
+int tx_attention_scored(void *ctx, const TxRows *qkv, void *out, const TxLayout *layouts,
+                        uint32_t nseq, uint32_t heads, uint32_t kv_heads, uint32_t dim, int in_dtype,
                         int out_dtype, float scale, const TxScoreRule *rule, void *stream) {
   Ctx *c = (Ctx *)ctx;
   if (!c) return TX_EINVAL;
   std::lock_guard<std::recursive_mutex> g(c->mu);
-  if (!q || !k || !v || !out || !q_layout || !k_layout || !rule || !q->data || !k->data || !v->data)
+  if (!qkv || !out || !layouts || !rule || !qkv[0].data || !qkv[1].data || !qkv[2].data)
     return fail(c, TX_EINVAL, "attention_scored: null pointer");
+  const TxRows *q = qkv, *k = qkv + 1, *v = qkv + 2;
+  const TxLayout *q_layout = layouts, *k_layout = layouts + 1;
   if (!heads || !kv_heads || heads % kv_heads)
     return fail(c, TX_EINVAL, "attention_scored: heads must be a positive multiple of kv_heads");
   if (!dim || dim > 256) return fail(c, TX_EINVAL, "attention_scored: head_dim must be in 1..256");
@@ -1754,8 +1755,8 @@ int tx_attention_scored(void *ctx, const TxRows *q, const TxRows *k, const TxRow
       return fail(c, TX_EINVAL, "attention_scored: nseq * max_len exceeds the rows");
   }
   // Key tiles of a document mask are kept as bits on chip.
-  if (r.k_docs && k_layout->max_len > 128u * 32768u)
-    return fail(c, TX_EINVAL, "attention_scored: documents with at most 2^22 keys");
+  if (r.k_docs && k_layout->max_len > 128u * 16384u)
+    return fail(c, TX_EINVAL, "attention_scored: documents with at most 2^21 keys");
   const size_t ei = in_dtype == TX_BF16 ? 2 : 4, eo = out_dtype == TX_BF16 ? 2 : 4;
   if ((uintptr_t)q->data % ei || (uintptr_t)k->data % ei || (uintptr_t)v->data % ei ||
       (uintptr_t)out % eo)

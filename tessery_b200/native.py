@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes as ct
 import hashlib
+import struct
 import threading
 from pathlib import Path
 from typing import Any
@@ -68,37 +69,12 @@ class TxBertModel(ct.Structure):
     ]
 
 
-class TxRotaryTensor(ct.Structure):
-    """One side of tx_rotary (TxRotaryTensor in tessattn.h)."""
-
-    _fields_ = [
-        ("x", _vp), ("out", _vp),
-        *[(name, _u64) for name in ("x_token_stride", "x_head_stride", "out_token_stride",
-                                    "out_head_stride")],
-        ("norm_w", _vp), ("heads", _u32),
-    ]
-
-
-class TxScoreRule(ct.Structure):
-    """The rule of tx_attention_scored (TxScoreRule in tessattn.h)."""
-
-    _fields_ = [
-        ("softcap", _f32), ("slopes", _vp), ("distance_bias", _vp), ("reach", _u32),
-        ("causal", _i32), ("window_left", ct.c_int32), ("window_right", ct.c_int32),
-        ("prefix", _vp), ("q_docs", _vp), ("k_docs", _vp),
-    ]
-
-
-class TxRows(ct.Structure):
-    """Rows of q, k or v with strides (TxRows in tessattn.h)."""
-
-    _fields_ = [("data", _vp), ("row_stride", _u64), ("head_stride", _u64)]
-
-
-class TxLayout(ct.Structure):
-    """Where the sequences lie (TxLayout in tessattn.h)."""
-
-    _fields_ = [("cu", _vp), ("lengths", _vp), ("rows", _u32), ("max_len", _u32)]
+# Small descriptions that go with every call, packed as the C structures of tessattn.h lay them
+# out (a ctypes.Structure per call costs several microseconds).
+TX_ROTARY_TENSOR = struct.Struct("QQQQQQQI4x")  # x, out, four strides, norm_w, heads
+TX_ROWS = struct.Struct("9Q")  # [3]: data, row_stride, head_stride
+TX_LAYOUTS = struct.Struct("QQIIQQII")  # [2]: cu, lengths, rows, max_len
+TX_SCORE_RULE = struct.Struct("f4xQQIiiiQQQ")  # softcap .. k_docs, in their order
 
 
 SIGNATURES: dict[str, tuple[list[Any], Any]] = {
@@ -178,12 +154,11 @@ SIGNATURES: dict[str, tuple[list[Any], Any]] = {
     "tx_linear": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _i32, _i32, _u32, _vp],
                   _i32),
     "tx_rotary": (
-        [_vp, ct.POINTER(TxRotaryTensor), ct.POINTER(TxRotaryTensor), _i32, _i32, _u32, _u32,
+        [_vp, ct.c_char_p, ct.c_char_p, _i32, _i32, _u32, _u32,
          _u32, _i32, _i32, _vp, _vp, _u32, _u32, _vp, _f32, _f32, _vp], _i32),
     "tx_attention_scored": (
-        [_vp, ct.POINTER(TxRows), ct.POINTER(TxRows), ct.POINTER(TxRows), _vp,
-         ct.POINTER(TxLayout), ct.POINTER(TxLayout), _u32, _u32, _u32, _u32, _i32, _i32, _f32,
-         ct.POINTER(TxScoreRule), _vp], _i32),
+        [_vp, ct.c_char_p, _vp, ct.c_char_p, _u32, _u32, _u32, _u32, _i32, _i32, _f32, ct.c_char_p,
+         _vp], _i32),
     "tx_linear_fused": (
         [_vp, _vp, _u64, _vp, _u64, _vp, _vp, _i32, _u64, _vp, _i32, _u64, _u32, _u32, _u32,
          _i32, _vp], _i32),

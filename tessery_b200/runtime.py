@@ -748,16 +748,16 @@ class CudaRuntime:
         def side(x, out, n, xs, os, weight):
             xt, xh = (n * dim, dim) if xs is None else xs
             ot, oh = (n * dim, dim) if os is None else os
-            if min(xt, xh, ot, oh) < 0:
+            if min(xt, xh, ot, oh, n) < 0 or not x or not out:
                 raise InvalidInputError()
-            return native.TxRotaryTensor(x, out, xt, xh, ot, oh, weight, n)
+            return native.TX_ROTARY_TENSOR.pack(x, out, xt, xh, ot, oh, weight or 0, n)
 
         qt = side(q, q_out, heads, q_strides, q_out_strides, q_norm_weight)
         kt = None if k is None else side(k, k_out, kv_heads, k_strides, k_out_strides,
                                          k_norm_weight)
         _raise_for(self._lib.tx_rotary(
             self._pointer, qt, kt, in_dtype, out_dtype, tokens, dim,
-            dim if rot_dim is None else rot_dim, int(bool(interleaved)), int(bool(inverse)),
+            dim if rot_dim is None else rot_dim, 1 if interleaved else 0, 1 if inverse else 0,
             positions, cu_seqlens, nseq, seq, inv_freq, amplitude, eps, stream))
 
     def attention_scored_device(
@@ -804,22 +804,24 @@ class CudaRuntime:
         elements, contiguous by default."""
         self._check_open()
 
-        def rows(x, n, strides):
-            r, h = (n * dim, dim) if strides is None else strides
-            if r < 0 or h < 0:
-                raise InvalidInputError()
-            return native.TxRows(x, r, h)
-
-        if min(nseq, rows_q, rows_k, max_q, max_k, reach) < 0 or dim < 1:
+        qr, qh = (heads * dim, dim) if q_strides is None else q_strides
+        kr, kh = (kv_heads * dim, dim) if k_strides is None else k_strides
+        vr, vh = (kv_heads * dim, dim) if v_strides is None else v_strides
+        left, right = window
+        if (min(nseq, rows_q, rows_k, max_q, max_k, reach, qr, qh, kr, kh, vr, vh) < 0 or dim < 1
+                or max(rows_q, rows_k, max_q, max_k, reach) > 0x7FFFFFFF
+                or max(left, right) > 0x7FFFFFFF or not (q and k and v)):
             raise InvalidInputError()
-        rule = native.TxScoreRule(softcap, slopes, distance_bias, reach, int(bool(causal)),
-                                  max(int(window[0]), -1), max(int(window[1]), -1), prefix,
-                                  q_docs, k_docs)
         _raise_for(self._lib.tx_attention_scored(
-            self._pointer, rows(q, heads, q_strides), rows(k, kv_heads, k_strides),
-            rows(v, kv_heads, v_strides), out, native.TxLayout(cu_q, q_lengths, rows_q, max_q),
-            native.TxLayout(cu_k, k_lengths, rows_k, max_k), nseq, heads, kv_heads, dim, in_dtype,
-            out_dtype, dim**-0.5 if scale is None else scale, rule, stream))
+            self._pointer, native.TX_ROWS.pack(q, qr, qh, k, kr, kh, v, vr, vh), out,
+            native.TX_LAYOUTS.pack(cu_q or 0, q_lengths or 0, rows_q, max_q, cu_k or 0,
+                                   k_lengths or 0, rows_k, max_k),
+            nseq, heads, kv_heads, dim, in_dtype, out_dtype,
+            dim**-0.5 if scale is None else scale,
+            native.TX_SCORE_RULE.pack(softcap, slopes or 0, distance_bias or 0, reach,
+                                      1 if causal else 0, left if left >= 0 else -1,
+                                      right if right >= 0 else -1, prefix or 0, q_docs or 0,
+                                      k_docs or 0), stream))
 
     def linear_fused_device(
         self,
