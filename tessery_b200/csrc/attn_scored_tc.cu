@@ -6,8 +6,8 @@
 //
 // One CTA takes 128 rows (query tokens x the heads that share a kv head, attn_scored.cuh) and
 // walks the 128-key tiles that some row may see.  S = Q K^T and O += P V are tcgen05.mma
-// (M = 128) into tensor memory.  Eight softmax warps: two threads share a row (tensor-memory lane),
-// 64 keys each.  A thread walks its part of S twice, 32 keys at a time: first the row's maximum (scores with a cap, a bias or a mask go back finished), then
+// (M = 128) into tensor memory; thread t of the four softmax warps owns row t (tensor-memory
+// lane t).  It walks S twice, 32 keys at a time: first the row's maximum (scores with a cap, a bias or a mask go back finished), then
 // P = exp2(z - m) as bf16 into tensor memory, the A operand of P.V.  Both walks are rolled loops:
 // the same work unrolled over the 128 keys (20 KB of code a tile) was bound by instruction
 // fetches.  The reference m follows the row's running maximum lazily: O
@@ -36,18 +36,18 @@ using namespace ptx;
 using namespace scored;
 
 constexpr int kRows = 128;
-constexpr int kThreads = 320;  // warps 0-7 softmax, 8 TMA, 9 MMA
-constexpr int kTmaWarp = 8, kMmaWarp = 9;
+constexpr int kThreads = 192;  // warps 0-3 softmax, 4 TMA, 5 MMA
+constexpr int kTmaWarp = 4, kMmaWarp = 5;
 constexpr uint32_t kTmemCols = 256;  // of the 512 of an SM: two CTAs share it
 constexpr uint32_t kColO = 128;      // S in columns 0-127, O from here
 constexpr float kRescaleThreshold = 8.0f;  // log2 units
 constexpr float kLog2e = 1.44269504088896341f;
 
-// Distance biases of a warp's 32 rows over its 64 keys: 63 + 32 / pack distances of each of the
+// Distance biases of a warp's 32 rows over a key tile: 127 + 32 / pack distances of each of the
 // pack heads (at most kTablePack).  Heads lie 32 / pack words apart modulo 32, so that the rows of
 // a warp read different banks.
 __host__ __device__ constexpr uint32_t window_pitch(uint32_t pack) {
-  const uint32_t n = 63 + 32 / pack, step = 32 / pack;
+  const uint32_t n = 127 + 32 / pack, step = 32 / pack;
   return n + (32 + step - n % 32) % 32;
 }
 constexpr uint32_t kWindow = kTablePack * window_pitch(kTablePack);
@@ -63,13 +63,11 @@ struct Cfg {
   // head_dim up to 64 has room for a table of distances.
   static constexpr uint32_t kTable = kDP == 64 ? 4096 : 0;
   static constexpr uint32_t kMiscBytes =
-      256 + kDocWords * 4 + 8 * (kWindow + 64) * 4 + 2 * 2 * kRows * 4 + kTable * 4;
+      256 + kDocWords * 4 + 4 * (kWindow + kKeys) * 4 + kTable * 4;
   // head_dim up to 64 leaves columns for P beside S: the next tile's Q.K^T is issued as soon as S
   // has been read.  Otherwise P lies over S, and it waits for P.V.
   static constexpr bool kEarly = kDP == 64;
-  // P of a half's 64 keys, 32 columns: over the first columns of the S that its own threads have
-  // read, or beside S.
-  static constexpr uint32_t kColP = kEarly ? kColO + 64 : 0, kHalfP = kEarly ? 32 : 64;
+  static constexpr uint32_t kColP = kEarly ? kColO + 64 : 0;
   static constexpr uint32_t kSmemBytes = kOffMisc + kMiscBytes;
   static_assert(2 * (kSmemBytes + 1024) <= 233472, "two CTAs per SM");
 };
@@ -83,8 +81,7 @@ enum : uint32_t {
 enum : uint32_t { kOffTmem = 128, kOffAbort = 132, kOffFlag = 136, kOffRange = 144, kOffBad = 160,
                   kOffWords = 256,
                   kOffWindow = kOffWords + kDocWords * 4,
-                  kOffDocs = kOffWindow + 8 * kWindow * 4, kOffRows = kOffDocs + 8 * 64 * 4,
-                  kOffTable = kOffRows + 2 * 2 * kRows * 4 };
+                  kOffDocs = kOffWindow + 4 * kWindow * 4, kOffTable = kOffDocs + 4 * kKeys * 4 };
 enum : int { kSiteK = 1, kSiteV = 2, kSiteKFree = 3, kSiteVFree = 4, kSiteS = 5, kSiteP = 6,
              kSiteO = 7, kSiteQ = 8, kSiteVRead = 9, kSiteScan = 10, kSiteHand = 11,
              kSiteSRead = 12, kSitePV = 13 };
@@ -151,27 +148,18 @@ __device__ __forceinline__ bool scan_values(uint32_t tile, int keys, uint32_t *b
   return __any_sync(0xffffffffu, any) != 0;
 }
 
-// The value rows marked in `bad` added to O for the query rows with p > 0 (all eight softmax warps,
-// each thread half of its row's columns), then zeroed.  `fresh`: O holds nothing yet.  False where
-// a wait gave up.
-template <int kDP, uint32_t kHalfP>
+// The value rows marked in `bad` added to O for the query rows with p > 0 (thread = row, all four
+// softmax warps), then zeroed.  `fresh`: O holds nothing yet.  False where a wait gave up.
+template <int kDP>
 __device__ __noinline__ bool add_by_hand(const volatile uint32_t *bad, uint32_t tile,
                                          uint32_t atom, uint32_t tP, uint32_t tO, bool fresh,
-                                         uint32_t half, const Gate &gate, uint32_t step) {
-  auto in_step = [&](uint32_t parity) {  // all 256 threads, two phases a call
-    tc_fence_before();
-    mbar_arrive(step);
-    const bool ok = __all_sync(0xffffffffu, gate.wait(step, parity, kSiteHand));
-    tc_fence_after();
-    return ok;
-  };
-  if (!in_step(0)) return false;  // both halves of P are there
+                                         const Gate &gate, uint32_t read, uint32_t turn) {
   for (int j = 0; j < kKeys; ++j) {
     if (!((bad[j >> 5] >> (j & 31)) & 1)) continue;
     uint32_t w[1];
-    tmem_load(tP + (j >> 6) * kHalfP + (j & 63) / 2, w);
+    tmem_load(tP + j / 2, w);
     const float pj = j & 1 ? bf16_hi(w[0]) : bf16_lo(w[0]);
-    for (uint32_t c = half * (kDP / 2); c < (half + 1) * (kDP / 2); c += 16) {
+    for (uint32_t c = 0; c < kDP; c += 16) {
       uint32_t o[16];
       tmem_load(tO + c, o);
 #pragma unroll
@@ -191,28 +179,15 @@ __device__ __noinline__ bool add_by_hand(const volatile uint32_t *bad, uint32_t 
     tmem_st_wait();
     fresh = false;
   }
-  if (!in_step(1)) return false;  // every thread has read the rows
-  for (int x = (int)threadIdx.x; x < kKeys * (kDP / 8); x += 256) {
+  mbar_arrive(read);  // every thread has read the rows
+  if (!__all_sync(0xffffffffu, gate.wait(read, turn & 1, kSiteHand))) return false;
+  for (int x = (int)threadIdx.x; x < kKeys * (kDP / 8); x += 128) {
     const int row = x / (kDP / 8), ch = x % (kDP / 8);
     if ((bad[row >> 5] >> (row & 31)) & 1)
       st_shared_v4(tile + (ch >> 3) * atom + row * 128 + (ch & 7) * 16, 0, 0, 0, 0);
   }
   fence_proxy_async();
   return true;
-}
-
-// The 64 threads of the two warps that share rows, in step; true if any of them says so.
-__device__ __forceinline__ bool pair_vote(uint32_t quarter, bool say) {
-  uint32_t any;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.u32 q, %1, 0;\n\t"
-      "barrier.cta.red.or.pred p, %2, 64, q;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(any)
-      : "r"((uint32_t)say), "r"(1 + quarter)
-      : "memory");
-  return any != 0;
 }
 
 enum : int { kNoBias = 0, kSlopes = 1, kTable = 2 };
@@ -258,11 +233,11 @@ __global__ void __launch_bounds__(kThreads, 2)
         mbar_init(bar(kBarVEmpty + i), 1);
       }
       mbar_init(bar(kBarS), 1);
-      mbar_init(bar(kBarP), 256);
+      mbar_init(bar(kBarP), 128);
       mbar_init(bar(kBarO), 1);
       mbar_init(bar(kBarScan), 1);
-      mbar_init(bar(kBarHand), 256);
-      mbar_init(bar(kBarSRead), 8);
+      mbar_init(bar(kBarHand), 128);
+      mbar_init(bar(kBarSRead), 4);
       mbar_init(bar(kBarPV), 1);
       *gate.abort_flag = 0;
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -377,8 +352,8 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
             for (uint32_t ks = 0; ks < 8; ++ks)
               if (ks < steps)
-                umma_ts(tmem + kColO, tmem + C::kColP + (ks >> 2) * C::kHalfP + (ks & 3) * 8,
-                        vd + (uint64_t)(ks * (2048 >> 4)), idesc_pv, t > 0 || ks > 0 || odd);
+                umma_ts(tmem + kColO, tmem + C::kColP + ks * 8, vd + (uint64_t)(ks * (2048 >> 4)),
+                        idesc_pv, t > 0 || ks > 0 || odd);
             umma_commit(bar(kBarVEmpty + vslot));
             if (C::kEarly) umma_commit(bar(kBarPV));
           }
@@ -395,10 +370,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
       __syncwarp();
     } else {
-      const uint32_t quarter = (uint32_t)warp & 3, half = (uint32_t)warp >> 2;
-      const int r = (int)quarter * 32 + lane;
-      const uint32_t lanes = tmem + ((quarter * 32) << 16);
-      const uint32_t tS = lanes + 64 * half, tO = lanes + kColO, tP = lanes + C::kColP;
+      const int r = (int)threadIdx.x;
+      const uint32_t tS = tmem + ((uint32_t)(warp * 32) << 16), tO = tS + kColO, tP = tS + C::kColP;
       const int token = r / (int)p.pack, head = (int)u.head0 + r % (int)p.pack;
       const bool live = token < u.tokens;
       const bool busy = __any_sync(0xffffffffu, live);  // rows past the last token need nothing
@@ -424,7 +397,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       // Table: this warp's window, and this row's place in it (its distance to the tile's key 0).
       const uint32_t pitch = window_pitch(p.pack);
       float *window = reinterpret_cast<float *>(misc + kOffWindow) + warp * kWindow;
-      const int warp_token = (int)quarter * 32 / (int)p.pack, span = 63 + 32 / (int)p.pack;
+      const int warp_token = warp * 32 / (int)p.pack, span = 127 + 32 / (int)p.pack;
       const float *window_row = window + (r % (int)p.pack) * pitch + (32 / (int)p.pack - 1) -
                                 (token - warp_token);
       // Tables small enough lie in shared memory.
@@ -432,27 +405,26 @@ __global__ void __launch_bounds__(kThreads, 2)
       const float *table = kBias != kTable ? nullptr
                            : near ? reinterpret_cast<const float *>(misc + kOffTable) + p.reach
                                   : p.table + (size_t)u.head0 * (2 * p.reach + 1) + p.reach;
-      bool bad = false;
-      uint32_t n = 0, scans = 0;
-      int32_t *doc_s = reinterpret_cast<int32_t *>(misc + kOffDocs) + warp * 64;
-      float *row_s = reinterpret_cast<float *>(misc + kOffRows);  // [2 buffers][2 halves][rows]
-      int32_t doc[2];  // documents of this half of the next tile's keys, lane = key
+      bool ok = true;
+      uint32_t n = 0, scans = 0, hands = 0;
+      int32_t *doc_s = reinterpret_cast<int32_t *>(misc + kOffDocs) + warp * kKeys;
+      int32_t doc[4];  // documents of the next tile's keys, lane = key
       auto load_docs = [&](int i) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int j = key_tile(u, i) * kKeys + 64 * (int)half + 32 * c + lane;
+        for (int c = 0; c < 4; ++c) {
+          const int j = key_tile(u, i) * kKeys + 32 * c + lane;
           doc[c] = i < u.last && j < u.s.nk ? p.k_docs[u.s.k_row + j] : -1;
         }
       };
       if (docs && busy) load_docs(first);
-      for (int i = first, next; i < u.last; i = next, ++n) {
+      for (int i = first, next; ok && i < u.last; i = next, ++n) {
         next = next_tile(u, marks, i + 1);
-        const int t0 = key_tile(u, i) * kKeys, k0 = t0 + 64 * (int)half;  // the tile's, this half's
-        const bool whole = whole_tile(u, t0);
+        const int k0 = key_tile(u, i) * kKeys;
+        const bool whole = whole_tile(u, k0);
         if (docs && busy) {
           __syncwarp();
-          doc_s[lane] = doc[0];
-          doc_s[32 + lane] = doc[1];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) doc_s[32 * c + lane] = doc[c];
           load_docs(next);
         }
         if (kBias == kTable && busy) {
@@ -469,12 +441,12 @@ __global__ void __launch_bounds__(kThreads, 2)
           }
         }
         __syncwarp();
-        bad = !__all_sync(0xffffffffu, gate.wait(bar(kBarS), n & 1, kSiteS)) || bad;
+        if (!(ok = __all_sync(0xffffffffu, gate.wait(bar(kBarS), n & 1, kSiteS)))) break;
         tc_fence_after();
-        // Walks this half's two chunks of 32 keys.
+        // Walks the tile's four chunks of 32 keys.
         auto walk = [&](auto each) {
 #pragma unroll 1
-          for (int c = 0; c < 2; ++c) {
+          for (int c = 0; c < 4; ++c) {
             uint32_t s[32];
             tmem_load(tS + 32 * c, s);
             each(c, s);
@@ -539,17 +511,8 @@ __global__ void __launch_bounds__(kThreads, 2)
           });
         if (kCap || kBias || !whole) tmem_st_wait();
         if (!kCap && !kBias) top *= scale2;
-        // The row's maximum over both halves.  The two warps leave together when a wait of either
-        // gave up.
-        float *rows = row_s + (n & 1) * 2 * kRows;
-        rows[half * kRows + r] = top;
-        if (pair_vote(quarter, bad)) {
-          bad = true;
-          break;
-        }
-        top = fmaxf(top, rows[(half ^ 1) * kRows + r]);
         if (C::kEarly && n > 0) {  // P and O are P.V's of the previous tile until it has run
-          bad = !__all_sync(0xffffffffu, gate.wait(bar(kBarPV), (n - 1) & 1, kSitePV));
+          ok = __all_sync(0xffffffffu, gate.wait(bar(kBarPV), (n - 1) & 1, kSitePV));
           tc_fence_after();
         }
         const bool raise = top > m + kRescaleThreshold || (m == -INFINITY && top > m);
@@ -559,7 +522,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           l *= f;
           if (n > 0) {
 #pragma unroll 1
-            for (uint32_t c = half * (kDP / 2); c < (half + 1) * (kDP / 2); c += 32) {
+            for (uint32_t c = 0; c < kDP; c += 32) {
               uint32_t o[32];
               tmem_load(tO + c, o);
 #pragma unroll
@@ -573,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           const float factor = kCap || kBias ? 1.f : scale2;
           float sum[2] = {0.f, 0.f};
           walk([&](int c, uint32_t(&s)[32]) {
-            if (C::kEarly && c == 1) {  // the last of this half of S is in registers
+            if (C::kEarly && c == 3) {  // the last of S is in registers
               tc_fence_before();
               __syncwarp();
               if (lane == 0) mbar_arrive(bar(kBarSRead));
@@ -595,7 +558,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
               for (int t = 0; t < 16; ++t) w[t] = 0;
             }
-            tmem_st16(tP + C::kHalfP * half + 16 * c, w);
+            tmem_st16(tP + 16 * c, w);
           });
           l += sum[0] + sum[1];
         } else if (C::kEarly) {
@@ -605,11 +568,10 @@ __global__ void __launch_bounds__(kThreads, 2)
         // Rows of V past the sequence's end inside the last 16-key step: zero probabilities, but
         // zero times whatever lies there need not be zero.
         const uint32_t slot = n % C::kSlots, tile_v = sbase + C::kOffV + slot * C::kTile;
-        const int keys = min(u.s.nk - t0, kKeys), clear = (keys + 15) / 16 * 16;
+        const int keys = min(u.s.nk - k0, kKeys), clear = (keys + 15) / 16 * 16;
         if (keys < clear) {
-          bad = !__all_sync(0xffffffffu, gate.wait(bar(kBarVFull + slot), (n / C::kSlots) & 1,
-                                                   kSiteVRead)) || bad;
-          for (int x = keys * (kDP / 8) + (int)threadIdx.x; x < clear * (kDP / 8); x += 256)
+          ok = __all_sync(0xffffffffu, gate.wait(bar(kBarVFull + slot), (n / C::kSlots) & 1, kSiteVRead)) && ok;
+          for (int x = keys * (kDP / 8) + r; x < clear * (kDP / 8); x += 128)
             st_shared_v4(tile_v + ((x % (kDP / 8)) >> 3) * C::kAtom + x / (kDP / 8) * 128 +
                              (x & 7) * 16,
                          0, 0, 0, 0);
@@ -617,27 +579,24 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
         tmem_st_wait();
         if (!whole) {
-          bad = !__all_sync(0xffffffffu, gate.wait(bar(kBarScan), scans++ & 1, kSiteScan)) || bad;
+          ok = __all_sync(0xffffffffu, gate.wait(bar(kBarScan), scans++ & 1, kSiteScan)) && ok;
           const volatile uint32_t *odd = reinterpret_cast<uint32_t *>(misc + kOffBad);
-          if (!bad && (odd[0] | odd[1] | odd[2] | odd[3]))
-            bad = !add_by_hand<kDP, C::kHalfP>(odd, tile_v, C::kAtom, tP, tO, n == 0, half, gate,
-                                               bar(kBarHand));
+          if (ok && (odd[0] | odd[1] | odd[2] | odd[3]))
+            ok = add_by_hand<kDP>(odd, tile_v, C::kAtom, tP, tO, n == 0, gate, bar(kBarHand),
+                                  hands++);
         }
         tc_fence_before();
         mbar_arrive(bar(kBarP));
       }
-      bad = !__all_sync(0xffffffffu, gate.wait(bar(kBarO), 0, kSiteO)) || bad;
+      ok = __all_sync(0xffffffffu, gate.wait(bar(kBarO), 0, kSiteO)) && ok;
       tc_fence_after();
-      float *rows = row_s + (n & 1) * 2 * kRows;
-      rows[half * kRows + r] = l;
-      if (!pair_vote(quarter, bad)) {
-        l += rows[(half ^ 1) * kRows + r];
+      if (ok) {
         const float inv = l == 0.f ? 0.f : 1.f / l;
         const size_t orow = ((size_t)(u.s.q_row + u.t0 + token) * p.heads + head) * p.dim;
         float *part = p.splits > 1 ? p.part_o + (((size_t)u.slot * p.splits + u.split) * kRows + r) * p.part_dp
                                    : nullptr;
 #pragma unroll 1
-        for (uint32_t c = half * (kDP / 2); c < (half + 1) * (kDP / 2); c += 32) {
+        for (uint32_t c = 0; c < kDP; c += 32) {
           if (c >= p.dim) break;
           uint32_t o[32];
           tmem_load(tO + c, o);
