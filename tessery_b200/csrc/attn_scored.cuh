@@ -118,6 +118,8 @@ __device__ __forceinline__ int key_tile(const Unit &u, int i) { return i < u.a ?
 // `words` holds (last - first + 31) / 32 words.  Ends with the threads in step.
 __device__ __forceinline__ void mark_tiles(const ScoredProblem &p, const Unit &u, uint32_t *words,
                                            int *range) {
+  const int lane = (int)(threadIdx.x & 31), warp = (int)(threadIdx.x >> 5),
+            warps = (int)(blockDim.x >> 5);
   if (threadIdx.x == 0) {
     range[0] = 0x7fffffff;
     range[1] = -1;
@@ -125,27 +127,39 @@ __device__ __forceinline__ void mark_tiles(const ScoredProblem &p, const Unit &u
   for (int i = threadIdx.x; i < (u.last - u.first + 31) / 32; i += blockDim.x) words[i] = 0;
   __syncthreads();
   const int32_t *qd = p.q_docs + u.s.q_row + u.t0;
-  for (int i = threadIdx.x; i < u.tokens; i += blockDim.x)
-    if (qd[i] >= 0) {
-      atomicMin(&range[0], qd[i]);
-      atomicMax(&range[1], qd[i]);
+  for (int i = warp * 32; i < u.tokens; i += warps * 32) {
+    const int d = i + lane < u.tokens ? qd[i + lane] : -1;
+    const int least = __reduce_min_sync(0xffffffffu, d < 0 ? 0x7fffffff : d);
+    const int most = __reduce_max_sync(0xffffffffu, d);
+    if (lane == 0 && most >= 0) {
+      atomicMin(&range[0], least);
+      atomicMax(&range[1], most);
     }
+  }
   __syncthreads();
   const int lo = range[0], hi = range[1];
   const int32_t *kd = p.k_docs + u.s.k_row;
-  for (int i = u.first + (int)(threadIdx.x >> 5); i < u.last; i += (int)(blockDim.x >> 5)) {
-    const int k0 = key_tile(u, i) * kKeys;
-    bool hit = false;
+  constexpr int kAhead = 4;  // tiles whose loads are in flight
+  for (int i0 = u.first + warp; i0 < u.last; i0 += warps * kAhead) {
+    int d[kAhead][kKeys / 32];
 #pragma unroll
-    for (int c = 0; c < kKeys / 32; ++c) {
-      const int j = k0 + c * 32 + (int)(threadIdx.x & 31);
-      if (j < u.s.nk) {
-        const int d = kd[j];
-        hit |= d >= lo && d <= hi;
+    for (int a = 0; a < kAhead; ++a) {
+      const int i = i0 + a * warps;
+#pragma unroll
+      for (int c = 0; c < kKeys / 32; ++c) {
+        const int j = key_tile(u, i) * kKeys + c * 32 + lane;
+        d[a][c] = i < u.last && j < u.s.nk ? kd[j] : -1;
       }
     }
-    if (__any_sync(0xffffffffu, hit) && (threadIdx.x & 31) == 0)
-      atomicOr(&words[(i - u.first) >> 5], 1u << ((i - u.first) & 31));
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      bool hit = false;
+#pragma unroll
+      for (int c = 0; c < kKeys / 32; ++c) hit |= d[a][c] >= lo && d[a][c] <= hi;
+      const int at = i0 + a * warps - u.first;
+      if (__any_sync(0xffffffffu, hit) && lane == 0)
+        atomicOr(&words[at >> 5], 1u << (at & 31));
+    }
   }
   __syncthreads();
 }

@@ -43,14 +43,18 @@ constexpr uint32_t kColO = 128;      // S in columns 0-127, O from here
 constexpr float kRescaleThreshold = 8.0f;  // log2 units
 constexpr float kLog2e = 1.44269504088896341f;
 
-// Distance biases of a warp's 32 rows over a key tile: 127 + 32 / pack distances of each of the
-// pack heads (at most kTablePack).  Heads lie 32 / pack words apart modulo 32, so that the rows of
-// a warp read different banks.
-__host__ __device__ constexpr uint32_t window_pitch(uint32_t pack) {
-  const uint32_t n = 127 + 32 / pack, step = 32 / pack;
-  return n + (32 + step - n % 32) % 32;
+// Distance biases lie in shared memory in log2 units.  A table small enough lies there once per CTA
+// with kKeys copies of its ends on either side, so that a row reads a tile's 128 distances from one
+// place; otherwise each warp lays out, tile by tile, the 127 + 32 / pack distances that its rows
+// need.  The pack (at most kTablePack) heads' parts lie 32 / pack words apart modulo 32, so that
+// the rows of a warp read different banks.
+__host__ __device__ constexpr uint32_t bias_pitch(uint32_t n, uint32_t pack) {
+  return n + (32 + 32 / pack - n % 32) % 32;
 }
-constexpr uint32_t kWindow = kTablePack * window_pitch(kTablePack);
+__host__ __device__ constexpr uint32_t window_pitch(uint32_t pack) {
+  return bias_pitch(127 + 32 / pack, pack);
+}
+constexpr uint32_t kWindow = kTablePack * window_pitch(kTablePack);  // a warp's
 static_assert(window_pitch(1) <= kWindow && 2 * window_pitch(2) <= kWindow, "window area");
 
 template <int kDP>  // head_dim rounded up to whole 64-column (128-byte) blocks
@@ -60,10 +64,9 @@ struct Cfg {
   static constexpr int kSlots = kDP == 64 ? 2 : 1;  // K slots, and V slots
   static constexpr uint32_t kOffQ = 0, kOffK = kTile, kOffV = kOffK + kSlots * kTile;
   static constexpr uint32_t kOffMisc = kOffV + kSlots * kTile;
-  // head_dim up to 64 has room for a table of distances.
-  static constexpr uint32_t kTable = kDP == 64 ? 4096 : 0;
-  static constexpr uint32_t kMiscBytes =
-      256 + kDocWords * 4 + 4 * (kWindow + kKeys) * 4 + kTable * 4;
+  static constexpr uint32_t kBiases = kDP == 64 ? 7168 : 3200;  // floats for distance biases
+  static constexpr uint32_t kMiscBytes = 256 + kDocWords * 4 + 4 * kKeys * 4 + kBiases * 4;
+  static_assert(4 * kWindow <= kBiases, "a window for each warp");
   // head_dim up to 64 leaves columns for P beside S: the next tile's Q.K^T is issued as soon as S
   // has been read.  Otherwise P lies over S, and it waits for P.V.
   static constexpr bool kEarly = kDP == 64;
@@ -80,8 +83,7 @@ enum : uint32_t {
 };
 enum : uint32_t { kOffTmem = 128, kOffAbort = 132, kOffFlag = 136, kOffRange = 144, kOffBad = 160,
                   kOffWords = 256,
-                  kOffWindow = kOffWords + kDocWords * 4,
-                  kOffDocs = kOffWindow + 4 * kWindow * 4, kOffTable = kOffDocs + 4 * kKeys * 4 };
+                  kOffDocs = kOffWords + kDocWords * 4, kOffBias = kOffDocs + 4 * kKeys * 4 };
 enum : int { kSiteK = 1, kSiteV = 2, kSiteKFree = 3, kSiteVFree = 4, kSiteS = 5, kSiteP = 6,
              kSiteO = 7, kSiteQ = 8, kSiteVRead = 9, kSiteScan = 10, kSiteHand = 11,
              kSiteSRead = 12, kSitePV = 13 };
@@ -115,6 +117,12 @@ __device__ __forceinline__ float rcp(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// A distance bias in log2 units.  A finite bias too large for them stays finite: only -inf closes a
+// key.
+__device__ __forceinline__ float bias_log2(float b) {
+  return b == -INFINITY ? b : fmaxf(b * kLog2e, -3.402823466e38f);
 }
 
 // Looks over `keys` rows of a value tile (one warp).  Returns whether any value is not finite;
@@ -214,14 +222,19 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int first = next_tile(u, marks, u.first);
   const bool work = u.tokens > 0 && first < u.last;
 
+  // Whether the whole table is to lie in shared memory, and at which pitch.
+  const uint32_t table_pitch = bias_pitch(2 * ((uint32_t)p.reach + kKeys) + 1, p.pack);
+  const bool near = kBias == kTable && p.reach <= (int)C::kBiases && p.pack * table_pitch <= C::kBiases;
+
   float m = -INFINITY, l = 0.f;  // softmax threads: the row's reference and sum
   if (work) {
-    if (kBias == kTable) {
-      const uint32_t n = p.pack * (2 * (uint32_t)p.reach + 1);
-      float *t = reinterpret_cast<float *>(misc + kOffTable);
-      if (n <= C::kTable)
-        for (uint32_t x = threadIdx.x; x < n; x += kThreads)
-          t[x] = p.table[(size_t)u.head0 * (2 * p.reach + 1) + x];
+    if (near) {
+      float *t = reinterpret_cast<float *>(misc + kOffBias);
+      for (uint32_t h = 0; h < p.pack; ++h) {
+        const float *from = p.table + (size_t)(u.head0 + h) * (2 * p.reach + 1);
+        for (int x = (int)threadIdx.x; x <= 2 * (p.reach + kKeys); x += kThreads)
+          t[h * table_pitch + x] = bias_log2(from[min(max(x - kKeys, 0), 2 * p.reach)]);
+      }
     }
     const Gate gate{reinterpret_cast<volatile int *>(misc + kOffAbort), p.status, p.wait_cycles};
     if (threadIdx.x == 0) {
@@ -395,16 +408,12 @@ __global__ void __launch_bounds__(kThreads, 2)
       };
       const float slope2 = kBias == kSlopes ? -p.slopes[head] * kLog2e : 0.f;
       // Table: this warp's window, and this row's place in it (its distance to the tile's key 0).
-      const uint32_t pitch = window_pitch(p.pack);
-      float *window = reinterpret_cast<float *>(misc + kOffWindow) + warp * kWindow;
+      const uint32_t pitch = near ? table_pitch : window_pitch(p.pack);
+      float *biases = reinterpret_cast<float *>(misc + kOffBias) + (near ? 0 : warp * kWindow);
       const int warp_token = warp * 32 / (int)p.pack, span = 127 + 32 / (int)p.pack;
-      const float *window_row = window + (r % (int)p.pack) * pitch + (32 / (int)p.pack - 1) -
-                                (token - warp_token);
-      // Tables small enough lie in shared memory.
-      const bool near = C::kTable > 0 && p.pack * (2 * (uint32_t)p.reach + 1) <= C::kTable;
-      const float *table = kBias != kTable ? nullptr
-                           : near ? reinterpret_cast<const float *>(misc + kOffTable) + p.reach
-                                  : p.table + (size_t)u.head0 * (2 * p.reach + 1) + p.reach;
+      const float *bias_row = biases + (r % (int)p.pack) * pitch +
+                              (near ? p.reach + kKeys
+                                    : (32 / (int)p.pack - 1) - (token - warp_token));
       bool ok = true;
       uint32_t n = 0, scans = 0, hands = 0;
       int32_t *doc_s = reinterpret_cast<int32_t *>(misc + kOffDocs) + warp * kKeys;
@@ -427,17 +436,16 @@ __global__ void __launch_bounds__(kThreads, 2)
           for (int c = 0; c < 4; ++c) doc_s[32 * c + lane] = doc[c];
           load_docs(next);
         }
-        if (kBias == kTable && busy) {
-          // In log2 units; a finite bias too large for them stays finite, so that only -inf closes
-          // a key.
+        const float *bias = bias_row;
+        if (near) {
+          bias += min(max(k0 - row.pos, -(p.reach + kKeys)), p.reach + 1);
+        } else if (kBias == kTable && busy) {
           const int d0 = k0 - row.pos + (token - warp_token) - (32 / (int)p.pack - 1);
           __syncwarp();
           for (int h = 0; h < (int)p.pack; ++h) {
-            const float *t = table + h * (2 * p.reach + 1);
-            for (int x = lane; x < span; x += 32) {
-              const float b = t[min(max(d0 + x, -p.reach), p.reach)];
-              window[h * pitch + x] = b == -INFINITY ? b : fmaxf(b * kLog2e, -3.402823466e38f);
-            }
+            const float *t = p.table + (size_t)((int)u.head0 + h) * (2 * p.reach + 1) + p.reach;
+            for (int x = lane; x < span; x += 32)
+              biases[h * pitch + x] = bias_log2(__ldg(t + min(max(d0 + x, -p.reach), p.reach)));
           }
         }
         __syncwarp();
@@ -457,10 +465,12 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (busy)
           walk([&](int c, uint32_t(&s)[32]) {
             uint32_t mask = ~0u;
+            bool full = true;  // every key of the chunk is open to every row of the warp
             if (!whole) {
               mask = row.bits(k0 + 32 * c);
               if (docs) mask &= doc_bits(doc_s[32 * c + lane], row.doc);
               if (!__any_sync(0xffffffffu, mask)) return;
+              full = __all_sync(0xffffffffu, mask == ~0u);
             }
             open |= 1u << c;
             if (kCap) {
@@ -492,11 +502,11 @@ __global__ void __launch_bounds__(kThreads, 2)
             if (kBias == kTable) {
 #pragma unroll
               for (int t = 0; t < 32; ++t) {
-                const float z = __uint_as_float(s[t]), b = window_row[32 * c + t];
+                const float z = __uint_as_float(s[t]), b = bias[32 * c + t];
                 s[t] = __float_as_uint(kCap ? z + b : fmaf(z, scale2, b));
               }
             }
-            if (!whole) {
+            if (!full) {
 #pragma unroll
               for (int t = 0; t < 32; ++t) s[t] = (mask >> t) & 1 ? s[t] : 0xff800000u;
             }
