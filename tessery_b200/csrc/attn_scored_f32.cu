@@ -18,11 +18,13 @@
 #include "attn_scored.cuh"
 #include "common.cuh"
 #include "kernels.h"
+#include "tcgen05.cuh"
 
 namespace tx {
 namespace scored_f32 {
 
 using namespace scored;
+using ptx::ex2;
 
 constexpr int kRows = 64, kThreads = 128, kStep = 64;  // kStep keys staged at a time
 constexpr float kLog2e = 1.44269504088896341f;
@@ -56,34 +58,33 @@ __device__ __forceinline__ float elem(const ScoredProblem &p, const void *x, siz
                          : static_cast<const float *>(x)[i];
 }
 
-// Rows [0, rows) of `x` (row r at r * row + off; rows past `live` zero) into `dst` with `pitch`,
-// columns past dim zero.  Returns whether this thread met a value that is not finite.
-template <int kDP, int kPitch>
-__device__ __forceinline__ bool stage(const ScoredProblem &p, float *dst, const void *x,
-                                      size_t off, uint64_t row, int live, bool vec) {
-  bool odd = false;
-  if (vec) {  // fp32, 16-byte rows
+// kStep rows into `dst` with kPitch, the columns past dim zero.  `at(r)` is row r's first element in
+// x, or -1 for a row of zeros.  `vec`: fp32 rows on 16-byte boundaries, copied asynchronously (the
+// caller waits for them).
+template <int kDP, int kPitch, typename At>
+__device__ __forceinline__ void stage(const ScoredProblem &p, float *dst, const void *x, bool vec,
+                                      At at) {
+  if (vec) {
+    const uint32_t to = ptx::smem_addr(dst);
 #pragma unroll 4
     for (int i = threadIdx.x; i < kStep * (kDP / 4); i += kThreads) {
       const int r = i / (kDP / 4), c = i % (kDP / 4) * 4;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (r < live && c < (int)p.dim)
-        v = *reinterpret_cast<const float4 *>(static_cast<const float *>(x) + off + r * row + c);
-      *reinterpret_cast<float4 *>(dst + r * kPitch + c) = v;
-      odd |= !(fabsf(v.x) < INFINITY && fabsf(v.y) < INFINITY && fabsf(v.z) < INFINITY &&
-               fabsf(v.w) < INFINITY);
+      const long long from = at(r);
+      const bool have = from >= 0 && c < (int)p.dim;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + (r * kPitch + c) * 4),
+                   "l"(static_cast<const float *>(x) + (have ? from + c : 0)), "r"(have ? 16 : 0)
+                   : "memory");
     }
   } else {
 #pragma unroll 4
     for (int i = threadIdx.x; i < kStep * kDP; i += kThreads) {
       const int r = i / kDP, c = i % kDP;
-      const float v = r < live && c < (int)p.dim ? elem(p, x, off + r * row + c) : 0.f;
-      dst[r * kPitch + c] = v;
-      odd |= !(fabsf(v) < INFINITY);
+      const long long from = at(r);
+      dst[r * kPitch + c] = from >= 0 && c < (int)p.dim ? elem(p, x, from + c) : 0.f;
     }
   }
-  return odd;
 }
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 template <int kDP>
 __global__ void __launch_bounds__(kThreads, kDP <= 64 ? 4 : 1) scored_f32_kernel(const __grid_constant__ ScoredProblem p) {
@@ -125,33 +126,49 @@ __global__ void __launch_bounds__(kThreads, kDP <= 64 ? 4 : 1) scored_f32_kernel
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
 
-  const bool f32 = p.in_dtype == 0;
-  const bool vk = f32 && p.dim % 4 == 0 && ((uintptr_t)p.k % 16) == 0 && p.k_row % 4 == 0 && p.k_head % 4 == 0;
-  const bool vv = f32 && p.dim % 4 == 0 && ((uintptr_t)p.v % 16) == 0 && p.v_row % 4 == 0 && p.v_head % 4 == 0;
-  if (first < u.last) {
-    // Query rows; packed heads of a token follow one another.
-    for (int i = threadIdx.x; i < kRows * kDP; i += kThreads) {
-      const int r = i / kDP, c = i % kDP;
-      float v = 0.f;
-      if (r / pack < u.tokens && c < (int)p.dim)
-        v = elem(p, p.q, (size_t)(u.s.q_row + u.t0 + r / pack) * p.q_row +
-                             (size_t)(u.head0 + r % pack) * p.q_head + c);
-      qs[r * C::kQP + c] = v;
-    }
-  }
+  // 16-byte copies: fp32, and every row of the tensor on a 16-byte boundary.
+  auto aligned = [&](const void *x, uint64_t row_stride, uint64_t head_stride) {
+    return p.in_dtype == 0 && ((p.dim | row_stride | head_stride) & 3) == 0 && ((uintptr_t)x & 15) == 0;
+  };
+  const bool vk = aligned(p.k, p.k_row, p.k_head), vv = aligned(p.v, p.v_row, p.v_head);
+  const bool busy = warp * 16 / pack < u.tokens;  // this warp has rows
+  if (first < u.last)  // query rows; packed heads of a token follow one another
+    stage<kDP, C::kQP>(p, qs, p.q, aligned(p.q, p.q_row, p.q_head), [&](int r) -> long long {
+      if (r / pack >= u.tokens) return -1;
+      return (long long)((size_t)(u.s.q_row + u.t0 + r / pack) * p.q_row +
+                         (size_t)(u.head0 + r % pack) * p.q_head);
+    });
   for (int i = first; i < u.last; i = next_tile(u, marks, i + 1)) {
     const int tile0 = key_tile(u, i) * kKeys;
     for (int k0 = tile0; k0 < min(tile0 + kKeys, u.s.nk); k0 += kStep) {
       const int live = min(kStep, u.s.nk - k0);
       __syncthreads();  // the previous step's rows have been read
       const size_t kr = (size_t)(u.s.k_row + k0);
-      stage<kDP, C::kQP>(p, ks, p.k, kr * p.k_row + (size_t)u.kv * p.k_head, p.k_row, live, vk);
-      const bool odd = stage<kDP, C::kVP>(p, vs, p.v, kr * p.v_row + (size_t)u.kv * p.v_head,
-                                          p.v_row, live, vv);
+      stage<kDP, C::kQP>(p, ks, p.k, vk, [&](int r) -> long long {
+        return r < live ? (long long)((kr + r) * p.k_row + (size_t)u.kv * p.k_head) : -1;
+      });
+      stage<kDP, C::kVP>(p, vs, p.v, vv, [&](int r) -> long long {
+        return r < live ? (long long)((kr + r) * p.v_row + (size_t)u.kv * p.v_head) : -1;
+      });
       if (docs)
         for (int j = threadIdx.x; j < kStep; j += kThreads)
           doc_s[j] = j < live ? p.k_docs[kr + j] : -1;
-      const bool any_odd = __syncthreads_or(odd);
+      copies_done();
+      // Whether a value is not finite: each thread looks over the ones that it copied.
+      float taint = 0.f;  // x * 0 is NaN exactly where x is not finite, and then the sum stays NaN
+      if (vv) {
+#pragma unroll 4
+        for (int x = threadIdx.x; x < kStep * (kDP / 4); x += kThreads) {
+          const float4 v = *reinterpret_cast<const float4 *>(vs + x / (kDP / 4) * C::kVP + x % (kDP / 4) * 4);
+          taint = fmaf(v.x, 0.f, fmaf(v.y, 0.f, fmaf(v.z, 0.f, fmaf(v.w, 0.f, taint))));
+        }
+      } else {
+#pragma unroll 4
+        for (int x = threadIdx.x; x < kStep * kDP; x += kThreads)
+          taint = fmaf(vs[x / kDP * C::kVP + x % kDP], 0.f, taint);
+      }
+      const bool any_odd = __syncthreads_or(taint != 0.f);
+      if (!busy && !any_odd) continue;  // the hand sums below keep the CTA in step
 
       // S = Q K^T
       float s[kStep / 8][4];
@@ -170,6 +187,7 @@ __global__ void __launch_bounds__(kThreads, kDP <= 64 ? 4 : 1) scored_f32_kernel
         split(q1.y, ah[3], al[3]);
 #pragma unroll
         for (int n = 0; n < kStep / 8; ++n) {
+          if (n * 8 >= live) break;
           const float2 b = *reinterpret_cast<const float2 *>(ks + (n * 8 + g) * C::kQP + kk * 8 + 2 * t);
           uint32_t bh0, bl0, bh1, bl1;
           split(b.x, bh0, bl0);
@@ -180,25 +198,47 @@ __global__ void __launch_bounds__(kThreads, kDP <= 64 ? 4 : 1) scored_f32_kernel
         }
       }
 
-      // Scores in log2 units, masked; then the running maximum and the probabilities.
-      float top[2] = {-INFINITY, -INFINITY};
+      // Scores in log2 units, masked; then the running maximum and the probabilities.  One branch
+      // per part of the rule around the loop over the scores.
+      auto each = [&](auto change) {
 #pragma unroll
-      for (int n = 0; n < kStep / 8; ++n)
+        for (int n = 0; n < kStep / 8; ++n) {
+          if (n * 8 >= live) break;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int h = e >> 1, jj = n * 8 + 2 * t + (e & 1), j = k0 + jj;
+          for (int e = 0; e < 4; ++e) s[n][e] = change(s[n][e], e >> 1, n * 8 + 2 * t + (e & 1));
+        }
+      };
+      if (p.softcap > 0.f) {
+        each([&](float z, int, int) { return p.softcap * tanhf(z * p.scale / p.softcap); });
+      } else {
+        each([&](float z, int, int) { return z * p.scale; });
+      }
+      if (p.slopes)
+        each([&](float z, int h, int j) {
+          return fmaf(-slope[h], fabsf((float)(k0 + j - row[h].pos)), z);
+        });
+      if (p.table)
+        each([&](float z, int h, int j) {
+          return z + __ldg(table[h] + min(max(k0 + j - row[h].pos, -p.reach), p.reach));
+        });
+      // A finite score that log2 units cannot hold stays finite.
+      each([&](float z, int, int) {
+        return fabsf(z) < INFINITY ? fmaxf(z * kLog2e, -3.402823466e38f) : z;
+      });
+      const int end = k0 + kStep;
+      if (!(end <= u.whole_prefix || (k0 >= u.whole_lo && end <= u.whole_hi)))
+        each([&](float z, int h, int jj) {
           const Row &w = row[h];
-          float z = s[n][e] * p.scale;
-          if (p.softcap > 0.f) z = p.softcap * tanhf(z / p.softcap);
-          if (p.slopes) z = fmaf(-slope[h], fabsf((float)(j - w.pos)), z);
-          if (p.table) z += __ldg(table[h] + min(max(j - w.pos, -p.reach), p.reach));
-          // A finite score that log2 units cannot hold stays finite.
-          z = fabsf(z) < INFINITY ? fmaxf(z * kLog2e, -3.402823466e38f) : z;
+          const int j = k0 + jj;
           bool open = j < w.prefix || (j >= w.lo && j < w.hi);
           if (docs) open = open && doc_s[jj] == w.doc;
-          s[n][e] = open ? z : -INFINITY;
-          top[h] = fmaxf(top[h], s[n][e]);
-        }
+          return open ? z : -INFINITY;
+        });
+      float top[2] = {-INFINITY, -INFINITY};
+      each([&](float z, int h, int) {
+        top[h] = fmaxf(top[h], z);
+        return z;
+      });
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
@@ -218,13 +258,11 @@ __global__ void __launch_bounds__(kThreads, kDP <= 64 ? 4 : 1) scored_f32_kernel
           o[n][2 * h + 1] *= f;
         }
       }
-#pragma unroll
-      for (int n = 0; n < kStep / 8; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[n][e] = exp2f(s[n][e] - ref[e >> 1]);
-          l[e >> 1] += s[n][e];
-        }
+      each([&](float z, int h, int) {
+        const float pj = ex2(z - ref[h]);  // 0 below 2^-126: nothing beside the row's largest, 1
+        l[h] += pj;
+        return pj;
+      });
 
       if (any_odd) {
         // A value of v in this step is not finite: its key counts for the rows that see it and
@@ -264,6 +302,7 @@ __global__ void __launch_bounds__(kThreads, kDP <= 64 ? 4 : 1) scored_f32_kernel
       // O += P V
 #pragma unroll
       for (int kk = 0; kk < kStep / 8; ++kk) {
+        if (kk * 8 >= live) break;
         uint32_t ah[4], al[4];
         split(s[kk][0], ah[0], al[0]);
         split(s[kk][2], ah[1], al[1]);
