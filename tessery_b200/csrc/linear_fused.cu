@@ -133,7 +133,9 @@ enum : int {
   kStagedRes = 2 // the residual too: loaded by TMA into the buffer its sum leaves from
 };
 
-template <int kBN, int kAct>
+// kLong: k takes more than one partial sum.  Kernels of their own, since the sums' registers and
+// the rolled loop in one kernel left spills in the first (178 against 169 us at 33500 x 1024 x 2048).
+template <int kBN, int kAct, bool kLong>
 __global__ void __launch_bounds__(kThreads, 1)
     linear_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                   const __grid_constant__ CUtensorMap tm_res,
@@ -394,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
       };
       const uint32_t lanes = (quarter * 32u) << 16;
-      if (parts > 1) {
+      if constexpr (kLong) {
         // Partial sums of 512 K are added in fp32 registers: the accumulator cuts off bits at each of
         // its additions, always towards zero, and over 2048 K in one go that left an error of 2e-6
         // of the result, eight times that of fp32 products in fp32.  The accumulator is free again
@@ -555,7 +557,7 @@ bool make_map(CUtensorMap *map, const void *base, uint32_t rows, uint32_t cols, 
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int kBN, int kAct>
+template <int kBN, int kAct, bool kLong>
 cudaError_t launch_tiles(const LinearFusedProblem &p, int num_sms, cudaStream_t stream) {
   constexpr uint32_t smem = Cfg<kBN>::kSmemBytes;
   CUtensorMap mx, mw, mr, mo;
@@ -568,13 +570,30 @@ cudaError_t launch_tiles(const LinearFusedProblem &p, int num_sms, cudaStream_t 
       !make_map(&mr, p.residual, p.m, p.n, p.ldr, 32, p.out_dtype == TX_F32))
     return cudaErrorInvalidValue;
   static std::atomic<uint64_t> seen{0};
-  cudaError_t e = allow_smem((const void *)linear_kernel<kBN, kAct>, (int)smem, seen);
+  cudaError_t e = allow_smem((const void *)linear_kernel<kBN, kAct, kLong>, (int)smem, seen);
   if (e != cudaSuccess) return e;
   const uint64_t tiles = (uint64_t)((p.n + kBN - 1) / kBN) * ((p.m + kBM - 1) / kBM);
   if (tiles > 0x7fffffffull) return cudaErrorInvalidValue;
-  linear_kernel<kBN, kAct><<<(uint32_t)std::min<uint64_t>(tiles, (uint64_t)num_sms), kThreads,
+  linear_kernel<kBN, kAct, kLong><<<(uint32_t)std::min<uint64_t>(tiles, (uint64_t)num_sms), kThreads,
                              smem, stream>>>(mx, mw, mr, mo, p);
   return cudaGetLastError();
+}
+
+template <int kAct, bool kLong>
+cudaError_t launch_wide(const LinearFusedProblem &p, int num_sms, cudaStream_t stream) {
+  // Tile width: waves of tiles over the SMs times a tile's cost, and what its first stages and last
+  // epilogue add, in microseconds measured at k = 1024 (k = 384 orders the widths alike).  At
+  // k = 1024 widths 64 / 128 / 256 take 33 / 29 / 39 us for 33500 x 100, 115 / 71 / 75 us for
+  // 33500 x 640, 178 / 107 / 96 us for 33500 x 1024, 21 / 16 / 28 us for 2048 x 1024 and
+  // 13 / 15 / 27 us for 777 x 128.
+  const uint64_t mt = (p.m + kBM - 1) / kBM;
+  auto cost = [&](uint64_t bn, uint64_t wave, uint64_t once) {
+    return (mt * ((p.n + bn - 1) / bn) + num_sms - 1) / num_sms * wave + once;
+  };
+  const uint64_t c64 = cost(64, 6, 0), c128 = cost(128, 7, 2), c256 = cost(256, 12, 7);
+  if (c256 < c128 && c256 < c64) return launch_tiles<256, kAct, kLong>(p, num_sms, stream);
+  if (c128 < c64) return launch_tiles<128, kAct, kLong>(p, num_sms, stream);
+  return launch_tiles<64, kAct, kLong>(p, num_sms, stream);
 }
 
 template <int kAct>
@@ -586,11 +605,8 @@ cudaError_t launch_act(LinearFusedProblem p, int num_sms, cudaStream_t stream) {
   p.bias_vec = (uintptr_t)p.bias % 16 == 0;
   p.epilogue = !p.out_vec ? kDirect
                : p.residual && p.res_vec && p.residual_dtype == p.out_dtype ? kStagedRes : kStaged;
-  // The widest tile that still gives every SM one (a wide tile reads x fewer times).
-  const uint64_t mt = (p.m + kBM - 1) / kBM;
-  if (mt * ((p.n + 255) / 256) >= (uint64_t)num_sms) return launch_tiles<256, kAct>(p, num_sms, stream);
-  if (mt * ((p.n + 127) / 128) >= (uint64_t)num_sms) return launch_tiles<128, kAct>(p, num_sms, stream);
-  return launch_tiles<64, kAct>(p, num_sms, stream);
+  return p.k > kPart * kBK ? launch_wide<kAct, true>(p, num_sms, stream)
+                           : launch_wide<kAct, false>(p, num_sms, stream);
 }
 
 }  // namespace lfused
