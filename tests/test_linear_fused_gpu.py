@@ -100,6 +100,22 @@ def test_several_tiles_in_turn(runtime, m, n, k, out):
     check(linear_fused(x, w, residual=r, out_dtype=out, runtime=runtime), xf, wf, None, "none", rf)
 
 
+@pytest.mark.parametrize("k", [72, 600])
+@pytest.mark.parametrize("out", ["float32", "bf16"])
+def test_widest_tiles(runtime, k, out):
+    """Enough tiles of 128 x 256 for several per CTA, the last of each row ragged; sums in one part
+    and in two."""
+    rng = np.random.default_rng(k)
+    m, n = 9400, 1530
+    x, xf = bf16(rng, (m, k))
+    w, wf = bf16(rng, (n, k), k**-0.5)
+    bias = rng.standard_normal(n).astype(np.float32)
+    r, rf = bf16(rng, (m, n))
+    r = rf if out == "float32" else r
+    check(linear_fused(x, w, bias=bias, activation="relu", residual=r, out_dtype=out,
+                       runtime=runtime), xf, wf, bias, "relu", rf)
+
+
 @pytest.mark.parametrize("m", [3, 150])
 @pytest.mark.parametrize("odd", [0, 1])
 @pytest.mark.parametrize("out", [TX_F32, TX_BF16])
