@@ -262,31 +262,66 @@ __device__ __forceinline__ void store_out(const ScoredProblem &p, size_t at, flo
     static_cast<float *>(p.out)[at] = v;
 }
 
-// One warp per row: weights of the splits first, then the columns.
+// One warp per row.  The splits' weights first, lane = split; then 16 bytes of the row per lane, the
+// lanes that a row leaves over (dim below 128) taking every second, fourth or eighth split, with
+// eight loads in flight each.  (Walked split by split with one load in flight, 37 parts of 16 rows
+// took 90 us of the 145 us at 16384 keys.)
 template <int kRows>
 __device__ __forceinline__ void join_parts(const ScoredProblem &p, const Unit &u) {
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const size_t base = (size_t)u.slot * p.splits * kRows;
+  const uint32_t need = (p.part_dp + 3) / 4;  // lanes for a row
+  const uint32_t width = need > 16 ? 32 : need > 8 ? 16 : need > 4 ? 8 : 4, sets = 32 / width;
+  const uint32_t set = lane / width;
   for (int r = (int)warp; r < u.tokens * (int)p.pack; r += (int)warps) {
+    auto part = [&](uint32_t s) { return base + (size_t)s * kRows + r; };
     float m = -INFINITY;
-    for (uint32_t s = 0; s < p.splits; ++s) m = fmaxf(m, p.part_ml[base + s * kRows + r].x);
+    for (uint32_t s = lane; s < p.splits; s += 32) m = fmaxf(m, p.part_ml[part(s)].x);
+    m = warp_max(m);
     const float ref = m == -INFINITY ? 0.f : m;
     float l = 0.f;
-    for (uint32_t s = 0; s < p.splits; ++s) {
-      const float2 v = p.part_ml[base + s * kRows + r];
+    for (uint32_t s = lane; s < p.splits; s += 32) {
+      const float2 v = p.part_ml[part(s)];
       l += exp2f(v.x - ref) * v.y;
     }
+    l = warp_sum(l);
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const size_t orow = ((size_t)(u.s.q_row + u.t0 + r / (int)p.pack) * p.heads + u.head0 +
                          r % (int)p.pack) * p.dim;
-    for (uint32_t c = lane; c < p.dim; c += 32) {
-      float acc = 0.f;
-      for (uint32_t s = 0; s < p.splits; ++s) {
-        const float2 v = p.part_ml[base + s * kRows + r];
-        if (v.x != -INFINITY)
-          acc += exp2f(v.x - ref) * p.part_o[(base + s * kRows + r) * p.part_dp + c];
+    for (uint32_t c0 = 0; c0 < p.dim; c0 += 4 * width) {
+      const uint32_t c = c0 + 4 * (lane % width);
+      float acc[4] = {0.f, 0.f, 0.f, 0.f};
+      for (uint32_t s0 = 0; s0 < p.splits; s0 += 32) {
+        float weight = 0.f;  // of split s0 + lane; one that saw no key has left no sum
+        if (s0 + lane < p.splits) weight = exp2f(p.part_ml[part(s0 + lane)].x - ref);
+        const uint32_t end = min(32u, p.splits - s0);
+        for (uint32_t x0 = 0; x0 < end; x0 += 8 * sets) {
+          float4 v[8];
+#pragma unroll
+          for (uint32_t x = 0; x < 8; ++x) {
+            const uint32_t s = x0 + x * sets + set;
+            v[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (s < end && c < p.part_dp)
+              v[x] = *reinterpret_cast<const float4 *>(p.part_o + part(s0 + s) * p.part_dp + c);
+          }
+#pragma unroll
+          for (uint32_t x = 0; x < 8; ++x) {
+            const float f = __shfl_sync(0xffffffffu, weight, (x0 + x * sets + set) & 31);
+            if (f != 0.f && x0 + x * sets + set < end) {
+              acc[0] = fmaf(f, v[x].x, acc[0]);
+              acc[1] = fmaf(f, v[x].y, acc[1]);
+              acc[2] = fmaf(f, v[x].z, acc[2]);
+              acc[3] = fmaf(f, v[x].w, acc[3]);
+            }
+          }
+        }
       }
-      store_out(p, orow + c, acc * inv);
+      for (uint32_t o = width; o < 32; o <<= 1)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor_sync(0xffffffffu, acc[e], o);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (set == 0 && c + e < p.dim) store_out(p, orow + c + e, acc[e] * inv);
     }
   }
 }
