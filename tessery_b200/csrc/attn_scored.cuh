@@ -275,12 +275,14 @@ __device__ __forceinline__ void join_parts(const ScoredProblem &p, const Unit &u
   const uint32_t set = lane / width;
   for (int r = (int)warp; r < u.tokens * (int)p.pack; r += (int)warps) {
     auto part = [&](uint32_t s) { return base + (size_t)s * kRows + r; };
-    float m = -INFINITY;
-    for (uint32_t s = lane; s < p.splits; s += 32) m = fmaxf(m, p.part_ml[part(s)].x);
+    const float2 none = make_float2(-INFINITY, 0.f);
+    const float2 ml = lane < p.splits ? p.part_ml[part(lane)] : none;
+    float m = ml.x;
+    for (uint32_t s = lane + 32; s < p.splits; s += 32) m = fmaxf(m, p.part_ml[part(s)].x);
     m = warp_max(m);
     const float ref = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
-    for (uint32_t s = lane; s < p.splits; s += 32) {
+    float l = exp2f(ml.x - ref) * ml.y;
+    for (uint32_t s = lane + 32; s < p.splits; s += 32) {
       const float2 v = p.part_ml[part(s)];
       l += exp2f(v.x - ref) * v.y;
     }
@@ -292,8 +294,9 @@ __device__ __forceinline__ void join_parts(const ScoredProblem &p, const Unit &u
       const uint32_t c = c0 + 4 * (lane % width);
       float acc[4] = {0.f, 0.f, 0.f, 0.f};
       for (uint32_t s0 = 0; s0 < p.splits; s0 += 32) {
-        float weight = 0.f;  // of split s0 + lane; one that saw no key has left no sum
-        if (s0 + lane < p.splits) weight = exp2f(p.part_ml[part(s0 + lane)].x - ref);
+        // Of split s0 + lane; 0 for one that saw no key.
+        const float at = s0 == 0 ? ml.x : s0 + lane < p.splits ? p.part_ml[part(s0 + lane)].x : none.x;
+        const float weight = exp2f(at - ref);
         const uint32_t end = min(32u, p.splits - s0);
         for (uint32_t x0 = 0; x0 < end; x0 += 8 * sets) {
           float4 v[8];

@@ -7,8 +7,12 @@
 // warps of a CTA and the CTAs of a split key range are joined at the end (in this order, so the
 // result is the same every time).  Both products run on mma.sync with the rows as M: bf16 on
 // m16n8k16, the probabilities as two bf16 parts (hi + lo, error 2^-17); fp32 on m16n8k8 TF32 with
-// split operands (hi + lo, three products, error 2^-22).  A 128-row tensor-memory tile would hold these few rows in one warp's
-// lanes and walk its keys one warp at a time (8 new tokens over up to 2048 keys: 38 us there).
+// split operands (hi + lo, three products, error 2^-22).  The 64-row fp32 kernel would compute 64
+// rows for these (when this one takes which call: scored_route in attn_scored_tc.cu).
+//
+// Measured: 8 new tokens, 16 query and 8 kv heads of 128, a cap, 300 to 2048 keys each: 25 us
+// between events, of which some 6 are the launch's; 32 texts of 1024 keys, 12 heads of 64 (101 MB):
+// 39 us, 2.6 TB/s.  More parts than CTAs that run at once gave no gain.
 #include <cuda_runtime.h>
 
 #include "../../include/tessattn.h"
@@ -101,7 +105,7 @@ __device__ __forceinline__ bool finite_word(uint32_t w, bool f32) {
 }
 
 template <typename T, int kDP>
-__global__ void __launch_bounds__(Cfg<T, kDP>::kThreads)
+__global__ void __launch_bounds__(Cfg<T, kDP>::kThreads, Cfg<T, kDP>::kResident)
     scored_few_kernel(const __grid_constant__ ScoredProblem p) {
   using C = Cfg<T, kDP>;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -112,46 +116,6 @@ __global__ void __launch_bounds__(Cfg<T, kDP>::kThreads)
   const Unit u = make_unit<kRows, kBlock>(p, blockIdx.x);
   if (!u.present) return;
   const int pack = (int)p.pack, rows = u.tokens * pack;
-
-  for (int i = threadIdx.x; i < kRows * kDP; i += C::kThreads) {
-    const int r = i / kDP, c = i % kDP;
-    T v = 0;
-    if (r < rows && c < (int)p.dim)
-      v = static_cast<const T *>(p.q)[(size_t)(u.s.q_row + u.t0 + r / pack) * p.q_row +
-                                      (size_t)(u.head0 + r % pack) * p.q_head + c];
-    qs[r * C::kQP + c] = v;
-  }
-  __syncthreads();
-  // bf16: the query rows as they enter the product, in registers (head_dim 256: read each time).
-  constexpr bool kQRegs = !C::kF32 && kDP <= 128;
-  uint32_t qa[kQRegs ? C::kChunks / 2 : 1][4];
-  auto q_words = [&](int q, int j, uint32_t(&a)[4]) {  // step j of piece group q
-    const int c = (4 * q + t) * 8 + 4 * j;
-    const uint2 x = *reinterpret_cast<const uint2 *>(qs + g * C::kQP + c);
-    const uint2 y = *reinterpret_cast<const uint2 *>(qs + (g + 8) * C::kQP + c);
-    a[0] = x.x; a[1] = y.x; a[2] = x.y; a[3] = y.y;
-  };
-  if constexpr (kQRegs) {
-#pragma unroll
-    for (int i = 0; i < C::kChunks / 2; ++i) q_words(i / 2, i % 2, qa[i]);
-  }
-
-  Row row[2];
-  const float *table[2];
-  float slope[2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int r = g + 8 * h, head = (int)u.head0 + r % pack;
-    row[h] = make_row(p, u, r / pack, r < rows);
-    table[h] = p.table ? p.table + (size_t)head * (2 * p.reach + 1) + p.reach : nullptr;
-    slope[h] = p.slopes ? p.slopes[head] : 0.f;
-  }
-  const float cap_a = p.softcap > 0.f ? 2.f * kLog2e / p.softcap : 0.f;
-  float o[kDP / 8][4];
-#pragma unroll
-  for (int n = 0; n < kDP / 8; ++n)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
 
   // Warp w takes blocks first + w, first + w + kWarps, ...
   const T *kp = static_cast<const T *>(p.k) + (size_t)u.kv * p.k_head;
@@ -192,6 +156,56 @@ __global__ void __launch_bounds__(Cfg<T, kDP>::kThreads)
   int ahead = u.first + warp;
 #pragma unroll
   for (int s = 0; s < kStages - 1; ++s, ahead += C::kWarps) fetch(ahead, s);
+  // Query rows, behind the first key blocks; a batch of loads in flight at a time.
+  constexpr int kBatch = 16;
+  for (int i0 = threadIdx.x; i0 < kRows * kDP; i0 += C::kThreads * kBatch) {
+    T v[kBatch];
+#pragma unroll
+    for (int x = 0; x < kBatch; ++x) {
+      const int i = i0 + x * C::kThreads, r = i / kDP, c = i % kDP;
+      v[x] = 0;
+      if (r < rows && c < (int)p.dim)
+        v[x] = static_cast<const T *>(p.q)[(size_t)(u.s.q_row + u.t0 + r / pack) * p.q_row +
+                                           (size_t)(u.head0 + r % pack) * p.q_head + c];
+    }
+#pragma unroll
+    for (int x = 0; x < kBatch; ++x) {
+      const int i = i0 + x * C::kThreads;
+      if (i < kRows * kDP) qs[i / kDP * C::kQP + i % kDP] = v[x];
+    }
+  }
+  __syncthreads();
+  // bf16: the query rows as they enter the product, in registers (head_dim 256: read each time).
+  constexpr bool kQRegs = !C::kF32 && kDP <= 128;
+  uint32_t qa[kQRegs ? C::kChunks / 2 : 1][4];
+  auto q_words = [&](int q, int j, uint32_t(&a)[4]) {  // step j of piece group q
+    const int c = (4 * q + t) * 8 + 4 * j;
+    const uint2 x = *reinterpret_cast<const uint2 *>(qs + g * C::kQP + c);
+    const uint2 y = *reinterpret_cast<const uint2 *>(qs + (g + 8) * C::kQP + c);
+    a[0] = x.x; a[1] = y.x; a[2] = x.y; a[3] = y.y;
+  };
+  if constexpr (kQRegs) {
+#pragma unroll
+    for (int i = 0; i < C::kChunks / 2; ++i) q_words(i / 2, i % 2, qa[i]);
+  }
+
+  Row row[2];
+  const float *table[2];
+  float slope[2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int r = g + 8 * h, head = (int)u.head0 + r % pack;
+    row[h] = make_row(p, u, r / pack, r < rows);
+    table[h] = p.table ? p.table + (size_t)head * (2 * p.reach + 1) + p.reach : nullptr;
+    slope[h] = p.slopes ? p.slopes[head] : 0.f;
+  }
+  const float cap_a = p.softcap > 0.f ? 2.f * kLog2e / p.softcap : 0.f;
+  float o[kDP / 8][4];
+#pragma unroll
+  for (int n = 0; n < kDP / 8; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
+
   int stage = 0;
   for (int i = u.first + warp; i < u.last; i += C::kWarps) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");

@@ -750,9 +750,16 @@ cudaError_t launch_scored_tc(const ScoredProblem &p, cudaStream_t stream) {
   return p.dim <= 64 ? scored_rule<64>(p, m, stream) : scored_rule<128>(p, m, stream);
 }
 
+// Few rows: up to 8 per kv head for head_dim up to 64 or with a cap, and up to 16 where the
+// tensor-memory kernel does not take the call.  Few-rows against tensor-memory kernel, one token of
+// 8 texts over 2048 keys: 27 / 28 us at 12 heads of 64, 27 / 34 us with a cap; of 32 texts over 1024
+// keys 39 / 46 us.  8 heads of 128, 2 rows each: 29 / 28 us, with a cap 29 / 30 us; 16 rows: 35 / 30
+// and 35 / 34 us.  fp32, 16 rows of 128 over 2048 keys: 68 us against 146 in the 64-row kernel.
 ScoredRoute scored_route(const ScoredProblem &p) {
-  if (p.rows_k && scored_few_supported(p)) return kScoredFew;
-  return p.rows_k && scored_tc_supported(p) ? kScoredTc : kScoredF32;
+  const bool tc = p.rows_k && scored_tc_supported(p), few = p.rows_k && scored_few_supported(p);
+  const uint64_t rows = (uint64_t)p.max_q * (p.heads / p.kv_heads);
+  if (few && (!tc || (rows <= 8 && (p.dim <= 64 || p.softcap > 0.f)))) return kScoredFew;
+  return tc ? kScoredTc : kScoredF32;
 }
 
 // The cut of a launch.  Rows: the heads of a pack times tokens (few rows: all heads of a kv head,

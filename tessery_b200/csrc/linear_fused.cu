@@ -8,8 +8,8 @@
 // multiplied; persistent, one CTA per SM.  Results leave through shared memory and TMA stores
 // (whole 128-byte rows; a thread that stored its own row directly wrote 16 bytes to each of 32
 // rows per instruction), and a residual of the output's type comes in the same way, a box ahead.
-// gemv_kernel: a few rows (m <= 8) only stream w once: a warp per output column, w straight from
-// global memory into registers, the sums over lanes by shuffles.
+// gemv_kernel: a few rows (m <= 8) only stream w once: one or four warps per output column, w
+// straight from global memory into registers, the sums over lanes by shuffles.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -465,48 +465,65 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // ---- a few rows -----------------------------------------------------------------------------
-// One warp per output column; lane l takes columns 8l .. 8l+7 of every 256 of K.
-constexpr int kGemvWarps = 4;
+// One warp per output column, or the block's four warps with a quarter of K each (kSplit = 4); lane l
+// takes columns 8l .. 8l+7 of every 256 of its part.
+constexpr uint32_t kGemvWarps = 4;
 
-template <int kM, int kAct>
+template <int kM, uint32_t kSplit, int kAct>
 __global__ void __launch_bounds__(32 * kGemvWarps) gemv_kernel(const __grid_constant__ LinearFusedProblem p) {
-  const uint32_t lane = threadIdx.x & 31;
-  const uint32_t n = blockIdx.x * kGemvWarps + (threadIdx.x >> 5);
-  if (n >= p.n) return;
-  const uint16_t *x = static_cast<const uint16_t *>(p.x);
-  const uint16_t *w = static_cast<const uint16_t *>(p.w) + (size_t)n * p.ldw;
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t n = (blockIdx.x * kGemvWarps + warp) / kSplit, part = warp % kSplit;
+  __shared__ float parts[kSplit][kM];
+  const bool live = n < p.n;
   float sum[kM];
 #pragma unroll
   for (int i = 0; i < kM; ++i) sum[i] = 0.f;
+  if (live) {
+    const uint16_t *x = static_cast<const uint16_t *>(p.x);
+    const uint16_t *w = static_cast<const uint16_t *>(p.w) + (size_t)n * p.ldw;
 #pragma unroll 4
-  for (uint32_t c = lane * 8; c < p.k; c += 256) {
-    const uint4 wv = __ldg(reinterpret_cast<const uint4 *>(w + c));
-    float wf[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t q = u4_at(wv, e / 2);
-      wf[e] = c + e < p.k ? (e & 1 ? bf16_hi(q) : bf16_lo(q)) : 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < kM; ++i) {
-      if ((uint32_t)i >= p.m) break;
-      const uint4 xv = __ldg(reinterpret_cast<const uint4 *>(x + (size_t)i * p.ldx + c));
+    for (uint32_t c = part * 256 + lane * 8; c < p.k; c += 256 * kSplit) {
+      const uint4 wv = __ldg(reinterpret_cast<const uint4 *>(w + c));
+      float wf[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const uint32_t q = u4_at(xv, e / 2);
-        const float xf = c + e < p.k ? (e & 1 ? bf16_hi(q) : bf16_lo(q)) : 0.f;
-        sum[i] = fmaf(xf, wf[e], sum[i]);
+        const uint32_t q = u4_at(wv, e / 2);
+        wf[e] = c + e < p.k ? (e & 1 ? bf16_hi(q) : bf16_lo(q)) : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < kM; ++i) {
+        if ((uint32_t)i >= p.m) break;
+        const uint4 xv = __ldg(reinterpret_cast<const uint4 *>(x + (size_t)i * p.ldx + c));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t q = u4_at(xv, e / 2);
+          const float xf = c + e < p.k ? (e & 1 ? bf16_hi(q) : bf16_lo(q)) : 0.f;
+          sum[i] = fmaf(xf, wf[e], sum[i]);
+        }
       }
     }
   }
 #pragma unroll
   for (int i = 0; i < kM; ++i) sum[i] = warp_sum(sum[i]);
+  if constexpr (kSplit > 1) {
+#pragma unroll
+    for (int i = 0; i < kM; ++i)
+      if (lane == 0) parts[part][i] = sum[i];
+    __syncthreads();
+    if (part) return;
+#pragma unroll
+    for (int i = 0; i < kM; ++i) {
+      sum[i] = parts[0][i];
+#pragma unroll
+      for (uint32_t s = 1; s < kSplit; ++s) sum[i] += parts[s][i];
+    }
+  }
   // Lane i finishes row i.
   float y = 0.f;
 #pragma unroll
   for (int i = 0; i < kM; ++i)
     if (lane == (uint32_t)i) y = sum[i];
-  if (lane < p.m) {
+  if (live && lane < p.m) {
     if (p.bias) y += p.bias[n];
     y = activate<kAct>(y);
     if (p.residual) y += residual_at(p, (size_t)lane * p.ldr + n);
@@ -514,18 +531,22 @@ __global__ void __launch_bounds__(32 * kGemvWarps) gemv_kernel(const __grid_cons
   }
 }
 
+template <int kM, uint32_t kSplit, int kAct>
+cudaError_t launch_columns(const LinearFusedProblem &p, cudaStream_t stream) {
+  constexpr uint32_t columns = kGemvWarps / kSplit;
+  gemv_kernel<kM, kSplit, kAct><<<(p.n + columns - 1) / columns, 32 * kGemvWarps, 0, stream>>>(p);
+  return cudaGetLastError();
+}
+
+// Four warps a column against one: 10.1 / 14.3 us for 1 x 1024 x 4096, 10 / 23 us for 2 x 1024 x 4096,
+// 10.2 / 10.2 us for 1 x 4096 x 1024, but 18.5 / 14.4 us for 1 x 16384 x 1024.
 template <int kAct>
 cudaError_t launch_gemv(const LinearFusedProblem &p, cudaStream_t stream) {
-  const uint32_t grid = (p.n + kGemvWarps - 1) / kGemvWarps, block = 32 * kGemvWarps;
-  if (p.m <= 1)
-    gemv_kernel<1, kAct><<<grid, block, 0, stream>>>(p);
-  else if (p.m <= 2)
-    gemv_kernel<2, kAct><<<grid, block, 0, stream>>>(p);
-  else if (p.m <= 4)
-    gemv_kernel<4, kAct><<<grid, block, 0, stream>>>(p);
-  else
-    gemv_kernel<8, kAct><<<grid, block, 0, stream>>>(p);
-  return cudaGetLastError();
+  if (p.m == 1)
+    return p.n > 8192 ? launch_columns<1, 1, kAct>(p, stream) : launch_columns<1, 4, kAct>(p, stream);
+  return p.m <= 2   ? launch_columns<2, 4, kAct>(p, stream)
+         : p.m <= 4 ? launch_columns<4, 4, kAct>(p, stream)
+                    : launch_columns<8, 4, kAct>(p, stream);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
@@ -598,7 +619,10 @@ cudaError_t launch_wide(const LinearFusedProblem &p, int num_sms, cudaStream_t s
 
 template <int kAct>
 cudaError_t launch_act(LinearFusedProblem p, int num_sms, cudaStream_t stream) {
-  if (p.m <= 8) return launch_gemv<kAct>(p, stream);
+  // A few rows stream w once; with more outputs than these the conversions and sums of every row
+  // cost more than a tile's: 10 against 14 us for 8 x 1024 x 1024, 27 against 34 us for
+  // 4 x 4096 x 4096, but 43 against 33 us for 8 x 4096 x 4096.
+  if (p.m == 1 || (p.m <= 8 && (uint64_t)p.m * p.n <= 16384)) return launch_gemv<kAct>(p, stream);
   const uint32_t vo = p.out_dtype == TX_BF16 ? 8 : 4, vr = p.residual_dtype == TX_BF16 ? 8 : 4;
   p.out_vec = (uintptr_t)p.out % 16 == 0 && p.ldo % vo == 0;
   p.res_vec = p.residual && (uintptr_t)p.residual % 16 == 0 && p.ldr % vr == 0;

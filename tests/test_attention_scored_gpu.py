@@ -171,6 +171,15 @@ def test_documents_skip_many_tiles(runtime):
     run_packed(runtime, [2500], [2500], 2, 1, 32, "f32", docs=docs, causal=False)
 
 
+def few_rows_route(rows, dim, dtype, cap=False):
+    """The kernel that takes `rows` query rows per kv head, 16-byte rows of k and v."""
+    if dtype == "f32":
+        return "scored_few" if rows <= 16 else "scored_f32"
+    if dim <= 128:
+        return "scored_few" if rows <= 8 and (dim <= 64 or cap) else "scored_tc"
+    return "scored_few" if rows <= 16 else "scored_f32"
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("new", [1, 2, 5, 17])
 @pytest.mark.parametrize("shape", [(16, 8, 128), (8, 1, 64), (3, 3, 32), (6, 2, 80)])
@@ -178,11 +187,12 @@ def test_new_tokens_against_kept_keys(runtime, dtype, new, shape):
     """Few query rows, long keys: the key range is split and joined."""
     lens_k = [1, 5, 700, 3000, 129, 2049]
     lens_q = [min(new, n) for n in lens_k]
-    few = new * (shape[0] // shape[1]) <= 16
-    route = "scored_few" if few else "scored_tc" if dtype == "bf16" else "scored_f32"
-    run_packed(runtime, lens_q, lens_k, *shape, dtype, route=route)
-    run_packed(runtime, lens_q, lens_k, *shape, dtype, route=route, softcap=10.0, window=(900, -1),
-               prefix=np.array([1, 0, 3, 200, 0, 5], np.int32))
+    rows = new * (shape[0] // shape[1])
+    run_packed(runtime, lens_q, lens_k, *shape, dtype,
+               route=few_rows_route(rows, shape[2], dtype))
+    run_packed(runtime, lens_q, lens_k, *shape, dtype,
+               route=few_rows_route(rows, shape[2], dtype, cap=True), softcap=10.0,
+               window=(900, -1), prefix=np.array([1, 0, 3, 200, 0, 5], np.int32))
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
@@ -191,10 +201,10 @@ def test_new_tokens_against_kept_keys(runtime, dtype, new, shape):
 def test_few_rows_of_any_group_and_dim(runtime, heads, kv_heads, dim, dtype):
     """Groups that are no power of two, head_dims between the compiled ones, every rule."""
     lens_k = [300, 1, 17, 1000]
-    kw = dict(route="scored_few")
+    kw = dict(route=few_rows_route(heads // kv_heads, dim, dtype))
     run_packed(runtime, [1] * 4, lens_k, heads, kv_heads, dim, dtype, out="float32", **kw)
     run_packed(runtime, [1] * 4, lens_k, heads, kv_heads, dim, dtype, slopes=slopes_of(heads),
-               softcap=9.0, window=(200, -1), **kw)
+               softcap=9.0, window=(200, -1), route="scored_few")
     run_packed(runtime, [1] * 4, lens_k, heads, kv_heads, dim, dtype,
                distance_bias=table_of(heads, 20), docs=lambda rng, n: rng.integers(-1, 3, size=n),
                **kw)
