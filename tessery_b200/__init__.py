@@ -15,6 +15,7 @@ from .errors import (
     InvalidInputError,
     NativeBuildError,
 )
+from .layers import attention_scored, linear_fused, rotary, rotary_frequencies
 from .native import TX_BF16, TX_F32
 from .partition import gather_shard, pack, shard_sequences
 from .runtime import Buffer, CudaRuntime
@@ -32,12 +33,16 @@ __all__ = [
     "TX_BF16",
     "TX_F32",
     "attention",
+    "attention_scored",
     "default_runtime",
     "gather_shard",
+    "linear_fused",
     "pack",
     "pack_rows",
     "pool_project",
     "qk_norm_rope",
+    "rotary",
+    "rotary_frequencies",
     "shard_sequences",
     "unpack_rows",
     "varlen_batches",
