@@ -70,7 +70,8 @@ int tx_device_sms(void *ctx);
 int tx_set_wait_limit(void *ctx, int64_t cycles);
 
 /* Name of the last attention kernel this context launched ("tc_bf16_d128",
- * "simt", "d32_f32") or "" -- the route a call took, as the reference's tests read
+ * "simt", "d32_f32"; tx_attention_scored: "scored_tc", "scored_few", "scored_f32"), "rotary",
+ * "linear_fused" or "" -- the route a call took, as the reference's tests read
  * kernel names from MetalRuntime.diagnostics()["dispatches"] (metal.py:208-234). */
 const char *tx_last_kernel(void *ctx);
 
@@ -481,8 +482,12 @@ typedef struct {
  * length get zeros; key and value rows past it, and those of other documents, may hold
  * anything, NaN and Inf included.  in_dtype / out_dtype TX_F32 or TX_BF16; dim <= 256; scale
  * finite.  bf16 with dim a multiple of 8 up to 128, strides multiples of 8 and 16-byte aligned
- * pointers runs on the tensor-memory kernel (P rounded to bf16), everything else in fp32
- * accuracy. */
+ * pointers runs on the tensor-memory kernel (P rounded to bf16).  A few query rows per kv head
+ * (max_len of q times heads / kv_heads: 8, with bf16 wider than 128 or fp32 16) run in a kernel of
+ * their own, P in two bf16 parts or fp32.  Everything else runs in fp32 accuracy.  With documents a
+ * sequence has at most 2^21 keys.  A long key range is cut into parts that are joined by the last
+ * to end, in a fixed order: a call's result does not change from run to run.  The parts' scratch
+ * belongs to the context; a call that needs more than any before it allocates. */
 int tx_attention_scored(void *ctx, const TxRows *qkv /* [3] */, void *out,
                         const TxLayout *layouts /* [2]: q's, then k's and v's */, uint32_t nseq,
                         uint32_t heads, uint32_t kv_heads, uint32_t dim, int in_dtype,

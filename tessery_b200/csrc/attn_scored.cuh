@@ -120,28 +120,11 @@ __device__ __forceinline__ void mark_tiles(const ScoredProblem &p, const Unit &u
                                            int *range) {
   const int lane = (int)(threadIdx.x & 31), warp = (int)(threadIdx.x >> 5),
             warps = (int)(blockDim.x >> 5);
-  if (threadIdx.x == 0) {
-    range[0] = 0x7fffffff;
-    range[1] = -1;
-  }
-  for (int i = threadIdx.x; i < (u.last - u.first + 31) / 32; i += blockDim.x) words[i] = 0;
-  __syncthreads();
-  const int32_t *qd = p.q_docs + u.s.q_row + u.t0;
-  for (int i = warp * 32; i < u.tokens; i += warps * 32) {
-    const int d = i + lane < u.tokens ? qd[i + lane] : -1;
-    const int least = __reduce_min_sync(0xffffffffu, d < 0 ? 0x7fffffff : d);
-    const int most = __reduce_max_sync(0xffffffffu, d);
-    if (lane == 0 && most >= 0) {
-      atomicMin(&range[0], least);
-      atomicMax(&range[1], most);
-    }
-  }
-  __syncthreads();
-  const int lo = range[0], hi = range[1];
+  // Documents of kAhead tiles a warp, the first of them on their way while the rows' range is found.
+  constexpr int kAhead = 4;
   const int32_t *kd = p.k_docs + u.s.k_row;
-  constexpr int kAhead = 4;  // tiles whose loads are in flight
-  for (int i0 = u.first + warp; i0 < u.last; i0 += warps * kAhead) {
-    int d[kAhead][kKeys / 32];
+  int d[kAhead][kKeys / 32];
+  auto load = [&](int i0) {
 #pragma unroll
     for (int a = 0; a < kAhead; ++a) {
       const int i = i0 + a * warps;
@@ -151,6 +134,28 @@ __device__ __forceinline__ void mark_tiles(const ScoredProblem &p, const Unit &u
         d[a][c] = i < u.last && j < u.s.nk ? kd[j] : -1;
       }
     }
+  };
+  load(u.first + warp);
+  if (threadIdx.x == 0) {
+    range[0] = 0x7fffffff;
+    range[1] = -1;
+  }
+  for (int i = threadIdx.x; i < (u.last - u.first + 31) / 32; i += blockDim.x) words[i] = 0;
+  __syncthreads();
+  const int32_t *qd = p.q_docs + u.s.q_row + u.t0;
+  for (int i = warp * 32; i < u.tokens; i += warps * 32) {
+    const int id = i + lane < u.tokens ? qd[i + lane] : -1;
+    const int least = __reduce_min_sync(0xffffffffu, id < 0 ? 0x7fffffff : id);
+    const int most = __reduce_max_sync(0xffffffffu, id);
+    if (lane == 0 && most >= 0) {
+      atomicMin(&range[0], least);
+      atomicMax(&range[1], most);
+    }
+  }
+  __syncthreads();
+  const int lo = range[0], hi = range[1];
+  for (int i0 = u.first + warp; i0 < u.last; i0 += warps * kAhead) {
+    if (i0 != u.first + warp) load(i0);
 #pragma unroll
     for (int a = 0; a < kAhead; ++a) {
       bool hit = false;

@@ -216,57 +216,44 @@ __global__ void __launch_bounds__(kThreads, 2)
   uint32_t *words = reinterpret_cast<uint32_t *>(misc + kOffWords);
   const Unit u = make_unit<kRows>(p, blockIdx.x);
   if (!u.present) return;  // whole units: every split of one takes the same way
+  const Gate gate{reinterpret_cast<volatile int *>(misc + kOffAbort), p.status, p.wait_cycles};
+  if (threadIdx.x == 0) {
+    mbar_init(bar(kBarQ), 1);
+    for (uint32_t i = 0; i < 2; ++i) {
+      mbar_init(bar(kBarKFull + i), 1);
+      mbar_init(bar(kBarKEmpty + i), 1);
+      mbar_init(bar(kBarVFull + i), 1);
+      mbar_init(bar(kBarVEmpty + i), 1);
+    }
+    mbar_init(bar(kBarS), 1);
+    mbar_init(bar(kBarP), 128);
+    mbar_init(bar(kBarO), 1);
+    mbar_init(bar(kBarScan), 1);
+    mbar_init(bar(kBarHand), 128);
+    mbar_init(bar(kBarSRead), 4);
+    mbar_init(bar(kBarPV), 1);
+    *gate.abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     bars + kOffTmem),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
   const bool docs = p.q_docs != nullptr;
   if (docs) mark_tiles(p, u, words, reinterpret_cast<int *>(misc + kOffRange));
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<uint32_t *>(misc + kOffTmem);
   const uint32_t *marks = docs ? words : nullptr;
   const int first = next_tile(u, marks, u.first);
   const bool work = u.tokens > 0 && first < u.last;
 
-  // Whether the whole table is to lie in shared memory, and at which pitch.
-  const uint32_t table_pitch = bias_pitch(2 * ((uint32_t)p.reach + kKeys) + 1, p.pack);
-  const bool near = kBias == kTable && p.reach <= (int)C::kBiases && p.pack * table_pitch <= C::kBiases;
-
   float m = -INFINITY, l = 0.f;  // softmax threads: the row's reference and sum
   if (work) {
-    if (near) {
-      float *t = reinterpret_cast<float *>(misc + kOffBias);
-      for (uint32_t h = 0; h < p.pack; ++h) {
-        const float *from = p.table + (size_t)(u.head0 + h) * (2 * p.reach + 1);
-        for (int x = (int)threadIdx.x; x <= 2 * (p.reach + kKeys); x += kThreads)
-          t[h * table_pitch + x] = bias_log2(from[min(max(x - kKeys, 0), 2 * p.reach)]);
-      }
-    }
-    const Gate gate{reinterpret_cast<volatile int *>(misc + kOffAbort), p.status, p.wait_cycles};
-    if (threadIdx.x == 0) {
-      mbar_init(bar(kBarQ), 1);
-      for (uint32_t i = 0; i < 2; ++i) {
-        mbar_init(bar(kBarKFull + i), 1);
-        mbar_init(bar(kBarKEmpty + i), 1);
-        mbar_init(bar(kBarVFull + i), 1);
-        mbar_init(bar(kBarVEmpty + i), 1);
-      }
-      mbar_init(bar(kBarS), 1);
-      mbar_init(bar(kBarP), 128);
-      mbar_init(bar(kBarO), 1);
-      mbar_init(bar(kBarScan), 1);
-      mbar_init(bar(kBarHand), 128);
-      mbar_init(bar(kBarSRead), 4);
-      mbar_init(bar(kBarPV), 1);
-      *gate.abort_flag = 0;
-      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    if (warp == kMmaWarp) {
-      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                       bars + kOffTmem),
-                   "r"(kTmemCols)
-                   : "memory");
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = *reinterpret_cast<uint32_t *>(misc + kOffTmem);
-
     if (warp == kTmaWarp) {
       if (lane == 0) {
         mbar_expect_tx(bar(kBarQ), C::kTile);
@@ -407,6 +394,19 @@ __global__ void __launch_bounds__(kThreads, 2)
         return fmaf(-2.f * cap2, rcp(1.f + ex2(x * (2.f * kLog2e) * cap_u)), cap2);
       };
       const float slope2 = kBias == kSlopes ? -p.slopes[head] * kLog2e : 0.f;
+      // Whether the whole table lies in shared memory, and at which pitch.
+      const uint32_t table_pitch = bias_pitch(2 * ((uint32_t)p.reach + kKeys) + 1, p.pack);
+      const bool near = kBias == kTable && p.reach <= (int)C::kBiases &&
+                        p.pack * table_pitch <= C::kBiases;
+      if (near) {  // laid out while the first tiles travel
+        float *t = reinterpret_cast<float *>(misc + kOffBias);
+        for (uint32_t h = 0; h < p.pack; ++h) {
+          const float *from = p.table + (size_t)(u.head0 + h) * (2 * p.reach + 1);
+          for (int x = (int)threadIdx.x; x <= 2 * (p.reach + kKeys); x += 128)
+            t[h * table_pitch + x] = bias_log2(from[min(max(x - kKeys, 0), 2 * p.reach)]);
+        }
+        asm volatile("barrier.cta.sync 1, 128;" ::: "memory");  // the softmax warps
+      }
       // Table: this warp's window, and this row's place in it (its distance to the tile's key 0).
       const uint32_t pitch = near ? table_pitch : window_pitch(p.pack);
       float *biases = reinterpret_cast<float *>(misc + kOffBias) + (near ? 0 : warp * kWindow);
@@ -648,11 +648,11 @@ __global__ void __launch_bounds__(kThreads, 2)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == kMmaWarp)
-      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
-                   "r"(kTmemCols)
-                   : "memory");
   }
+  if (warp == kMmaWarp)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "r"(kTmemCols)
+                 : "memory");
   if (p.splits > 1) {
     const int r = (int)threadIdx.x;
     if (r < u.tokens * (int)p.pack)
