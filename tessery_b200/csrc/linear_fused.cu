@@ -94,17 +94,22 @@ __device__ __forceinline__ float activate(float y) {
   if constexpr (kAct == TX_ACT_RELU) {
     return y < 0.f ? 0.f : y;
   } else if constexpr (kAct == TX_ACT_GELU) {
-    // 1 - erf(z), z = |y| / sqrt 2, as t P(t) exp(-z^2) with t = 1 / (1 + 0.3275911 z)
-    // (Abramowitz and Stegun 7.1.26, absolute error 1.5e-7); gelu = y - y tail / 2 for y > 0
-    // and y tail / 2 below, so the negative side does not cancel.
-    const float z = fabsf(y) * 0.70710678118654752f;
-    const float t = rcp(fmaf(0.3275911f, z, 1.f));
-    float q = fmaf(t, 1.061405429f, -1.453152027f);
-    q = fmaf(t, q, 1.421413741f);
-    q = fmaf(t, q, -0.284496736f);
-    q = fmaf(t, q, 0.254829592f) * t;
-    const float half = 0.5f * y * (q * ex2(z * z * -kLog2e));
-    return y > 0.f ? y - half : half;
+    // 1 - erf(z), z = |y| / sqrt 2, as 1 / (1 + a1 z + ... + a6 z^6)^16 (Abramowitz and Stegun
+    // 7.1.28, absolute error 3e-7), the coefficients here for |y|; gelu = y (1 - tail / 2) for
+    // y > 0 and y tail / 2 below, so the negative side does not cancel.  One special function
+    // (7.1.26 takes an exponential as well: 26.7 against 25.0 us at 8192 x 1536 x 384).
+    const float z = fabsf(y);
+    float q = fmaf(z, 5.38297500e-06f, 4.88906374e-05f);
+    q = fmaf(z, q, 3.80035750e-05f);
+    q = fmaf(z, q, 3.27762630e-03f);
+    q = fmaf(z, q, 2.11410062e-02f);
+    q = fmaf(z, q, 4.98673469e-02f);
+    q = rcp(fmaf(z, q, 1.f));
+    q *= q;
+    q *= q;
+    q *= q;
+    const float tail = 0.5f * (q * q);
+    return y * (y > 0.f ? 1.f - tail : tail);
   } else if constexpr (kAct == TX_ACT_GELU_TANH) {  // (1 + tanh u) / 2 = 1 / (1 + e^(-2u))
     const float u = y * fmaf(0.044715f, y * y, 1.f);
     return y * rcp(1.f + ex2(u * (-1.5957691216057308f * kLog2e)));

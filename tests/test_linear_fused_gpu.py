@@ -100,6 +100,20 @@ def test_several_tiles_in_turn(runtime, m, n, k, out):
     check(linear_fused(x, w, residual=r, out_dtype=out, runtime=runtime), xf, wf, None, "none", rf)
 
 
+@pytest.mark.parametrize("m", [2, 40])
+@pytest.mark.parametrize("act", ACTS)
+def test_infinite_sums_stay_infinite(runtime, m, act):
+    rng = np.random.default_rng(m)
+    x, xf = bf16(rng, (m, 64))
+    w, wf = bf16(rng, (40, 64), 0.1)
+    bias = np.zeros(40, np.float32)
+    bias[7] = np.inf
+    got = linear_fused(x, w, bias=bias, activation=act, out_dtype="float32", runtime=runtime)
+    assert np.isposinf(got[:, 7]).all()
+    rest = np.arange(40) != 7
+    check(got[:, rest], xf, wf[rest], None, act, None)
+
+
 @pytest.mark.parametrize("k", [72, 600])
 @pytest.mark.parametrize("out", ["float32", "bf16"])
 def test_widest_tiles(runtime, k, out):
