@@ -240,7 +240,7 @@ __device__ __forceinline__ void zero_padding(const ScoredProblem &p, const Unit 
 }
 
 // Joining a split key range.  Each CTA of a unit leaves, per row, its unnormalised sum O (fp32),
-// its reference m (log2 units; -inf when it saw no key) and row sum l; the CTA that arrives last
+// its reference m (in the kernel's units of the score; -inf when it saw no key) and row sum l; the CTA that arrives last
 // adds the parts in the order of the splits, so the result does not depend on which it was.
 //
 // Called by every thread of the CTA once its partials are written; true in the CTA that has to
@@ -271,8 +271,9 @@ __device__ __forceinline__ void store_out(const ScoredProblem &p, size_t at, flo
 // lanes that a row leaves over (dim below 128) taking every second, fourth or eighth split, with
 // eight loads in flight each.  (Walked split by split with one load in flight, 37 parts of 16 rows
 // took 90 us of the 145 us at 16384 keys.)
+// `log2e`: the factor of m's units to log2 units.
 template <int kRows>
-__device__ __forceinline__ void join_parts(const ScoredProblem &p, const Unit &u) {
+__device__ __forceinline__ void join_parts(const ScoredProblem &p, const Unit &u, float log2e) {
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const size_t base = (size_t)u.slot * p.splits * kRows;
   const uint32_t need = (p.part_dp + 3) / 4;  // lanes for a row
@@ -286,10 +287,10 @@ __device__ __forceinline__ void join_parts(const ScoredProblem &p, const Unit &u
     for (uint32_t s = lane + 32; s < p.splits; s += 32) m = fmaxf(m, p.part_ml[part(s)].x);
     m = warp_max(m);
     const float ref = m == -INFINITY ? 0.f : m;
-    float l = exp2f(ml.x - ref) * ml.y;
+    float l = exp2f((ml.x - ref) * log2e) * ml.y;
     for (uint32_t s = lane + 32; s < p.splits; s += 32) {
       const float2 v = p.part_ml[part(s)];
-      l += exp2f(v.x - ref) * v.y;
+      l += exp2f((v.x - ref) * log2e) * v.y;
     }
     l = warp_sum(l);
     const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -301,7 +302,7 @@ __device__ __forceinline__ void join_parts(const ScoredProblem &p, const Unit &u
       for (uint32_t s0 = 0; s0 < p.splits; s0 += 32) {
         // Of split s0 + lane; 0 for one that saw no key.
         const float at = s0 == 0 ? ml.x : s0 + lane < p.splits ? p.part_ml[part(s0 + lane)].x : none.x;
-        const float weight = exp2f(at - ref);
+        const float weight = exp2f((at - ref) * log2e);
         const uint32_t end = min(32u, p.splits - s0);
         for (uint32_t x0 = 0; x0 < end; x0 += 8 * sets) {
           float4 v[8];

@@ -10,7 +10,7 @@
 // split operands (hi + lo, three products, error 2^-22).  The 64-row fp32 kernel would compute 64
 // rows for these (when this one takes which call: scored_route in attn_scored_tc.cu).
 //
-// Measured: 8 new tokens, 16 query and 8 kv heads of 128, a cap, 300 to 2048 keys each: 25 us
+// Measured: 8 new tokens, 16 query and 8 kv heads of 128, a cap, 64 to 2048 keys each: 25 us
 // between events, of which some 6 are the launch's; 32 texts of 1024 keys, 12 heads of 64 (101 MB):
 // 39 us, 2.6 TB/s.  More parts than CTAs that run at once gave no gain.
 #include <cuda_runtime.h>
@@ -30,7 +30,7 @@ using ptx::ld_shared_v4;
 
 constexpr int kRows = 16, kBlock = 16, kStages = 3;
 constexpr float kLog2e = 1.44269504088896341f;
-constexpr float kRescaleThreshold = 8.0f;  // log2 units
+constexpr float kRescaleThreshold = 5.5f;  // e^5.5 = 2^7.9
 
 template <typename T, int kDP>
 struct Cfg {
@@ -84,15 +84,20 @@ __device__ __forceinline__ void split(float x, uint32_t &hi, uint32_t &lo) {
   hi = round_tf32(x) & 0xffffe000u;
   lo = __float_as_uint(x - __uint_as_float(hi));
 }
-// c += a b for fp32 operands given as raw bits, through their splits.
+// c += a b for fp32 operands given as raw bits, through their splits.  Added to c in fp32: the
+// tensor core cuts bits off at each of its own additions, always towards zero (8 heads of 128 on one
+// kv head, up to 774 keys: off by 9e-7 that way and 1.9e-7 this way, for 18.5 and 20.5 us).
 __device__ __forceinline__ void mma_split(float (&c)[4], const uint32_t (&ah)[4],
                                           const uint32_t (&al)[4], float b0, float b1) {
   uint32_t h0, l0, h1, l1;
   split(b0, h0, l0);
   split(b1, h1, l1);
-  mma(c, al, h0, h1);
-  mma(c, ah, l0, l1);
-  mma(c, ah, h0, h1);
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  mma(sum, al, h0, h1);
+  mma(sum, ah, l0, l1);
+  mma(sum, ah, h0, h1);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) c[e] += sum[e];
 }
 __device__ __forceinline__ float rcp(float x) {
   float y;
@@ -253,7 +258,8 @@ __global__ void __launch_bounds__(Cfg<T, kDP>::kThreads, Cfg<T, kDP>::kResident)
       }
     }
 
-    // Scores in log2 units, masked.
+    // Scores, masked.  The step to log2 units comes behind the subtraction of the reference: a large
+    // score times log2 e would be rounded before it.
     bool all = true;
     float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
@@ -271,8 +277,6 @@ __global__ void __launch_bounds__(Cfg<T, kDP>::kThreads, Cfg<T, kDP>::kResident)
         }
         if (p.slopes) z = fmaf(-slope[h], fabsf((float)(j - w.pos)), z);
         if (p.table) z += __ldg(table[h] + min(max(j - w.pos, -p.reach), p.reach));
-        // A finite score that log2 units cannot hold stays finite.
-        z = fabsf(z) < INFINITY ? fmaxf(z * kLog2e, -3.402823466e38f) : z;
         bool open = j < w.prefix || (j >= w.lo && j < w.hi);
         if (p.k_docs) open = open && p.k_docs[u.s.k_row + j] == w.doc;
         all = all && (open || g + 8 * h >= rows);
@@ -290,7 +294,7 @@ __global__ void __launch_bounds__(Cfg<T, kDP>::kThreads, Cfg<T, kDP>::kResident)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const float now = fmaxf(m[h], top[h]);
-        const float f = m[h] == -INFINITY ? 0.f : exp2f(m[h] - now);
+        const float f = m[h] == -INFINITY ? 0.f : exp2f((m[h] - now) * kLog2e);
         m[h] = now;
         l[h] *= f;
 #pragma unroll
@@ -305,7 +309,7 @@ __global__ void __launch_bounds__(Cfg<T, kDP>::kThreads, Cfg<T, kDP>::kResident)
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        s[n][e] = ex2(s[n][e] - ref[e >> 1]);
+        s[n][e] = ex2((s[n][e] - ref[e >> 1]) * kLog2e);
         l[e >> 1] += s[n][e];
       }
 
@@ -434,7 +438,7 @@ __global__ void __launch_bounds__(Cfg<T, kDP>::kThreads, Cfg<T, kDP>::kResident)
 #pragma unroll
     for (int w = 0; w < C::kWarps; ++w) {
       const float2 v = sml[w * kRows + r];
-      f[w] = v.x == -INFINITY ? 0.f : exp2f(v.x - ref);
+      f[w] = v.x == -INFINITY ? 0.f : exp2f((v.x - ref) * kLog2e);
       ll += v.x == -INFINITY ? v.y : f[w] * v.y;
     }
     const size_t part = ((size_t)u.slot * p.splits + u.split) * kRows + r;
@@ -453,7 +457,7 @@ __global__ void __launch_bounds__(Cfg<T, kDP>::kThreads, Cfg<T, kDP>::kResident)
     }
   }
   if (p.splits == 1 || arrive_last(p, u, flag)) {
-    if (p.splits > 1) join_parts<kRows>(p, u);
+    if (p.splits > 1) join_parts<kRows>(p, u, kLog2e);
     zero_padding(p, u);
   }
 }

@@ -212,6 +212,21 @@ def test_few_rows_of_any_group_and_dim(runtime, heads, kv_heads, dim, dtype):
                prefix=np.array([40, 0, 17, 5], np.int32), qk_scale=3.0, **kw)
 
 
+@pytest.mark.parametrize("new,heads,kv_heads,dim", [(0, 3, 1, 80), (1, 8, 1, 128)])
+def test_fp32_sums_over_many_keys(runtime, new, heads, kv_heads, dim):
+    """Sums over many keys round to nearest: n / 8 partial sums, each off by 2^-24 / sqrt(3) of the
+    sum so far in the mean square, are off by sqrt(2200 / 8) 2^-24 / sqrt(3) = 5.7e-7 of it at most,
+    taken over the whole result.  Sums that cut bits off always towards zero are off by 2e-6."""
+    rng = np.random.default_rng(3)
+    n = 2200
+    q = rng.standard_normal((new or n, heads, dim)).astype(np.float32)
+    k, v = (rng.standard_normal((n, kv_heads, dim)).astype(np.float32) for _ in range(2))
+    got = attention_scored(q, k, v, cu_q=[0, len(q)], cu_k=[0, n], causal=False, runtime=runtime)
+    rows = slice(0, None, 97)
+    want = oracle.attention_scored(q[rows], k, v)[0]
+    assert np.linalg.norm(got[rows] - want) < 6e-7 * np.linalg.norm(want)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_more_queries_than_keys_leaves_rows_empty(runtime, dtype):
     """nq > nk: causal rows at negative positions see nothing and are zeros."""
