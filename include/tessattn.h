@@ -506,7 +506,9 @@ enum {
  * (elements), sums in fp32, bias fp32 [n] or NULL, residual [m, n] (TX_F32 or TX_BF16, row
  * stride ldr) or NULL, out [m, n] (TX_F32 or TX_BF16, row stride ldo), rounded once.  residual
  * may be out (same dtype and stride).  Any m, n, k; x and w 16-byte aligned with ldx and ldw
- * multiples of 8 (columns past k may hold anything). */
+ * multiples of 8 (columns past k may hold anything).  With few output tiles and a long k the sum is
+ * cut over CTAs and joined in a fixed order in the context's scratch; a call that needs more of it
+ * than any before allocates. */
 int tx_linear_fused(void *ctx, const void *x, uint64_t ldx, const void *w, uint64_t ldw,
                     const float *bias, const void *residual, int residual_dtype, uint64_t ldr,
                     void *out, int out_dtype, uint64_t ldo, uint32_t m, uint32_t n, uint32_t k,

@@ -243,9 +243,15 @@ struct LinearFusedProblem {
   int residual_dtype, out_dtype, act;
   bool out_vec, res_vec, bias_vec;  // on 16-byte boundaries; epilogue: set by the launcher
   int epilogue;
+  uint32_t splits;    // parts of k that CTAs of their own sum (linear_fused_splits)
+  float *part;        // [tile][split][epilogue warp][32 columns][32 rows] with splits > 1
+  uint32_t *arrived;  // [tile][epilogue warp], zero between calls
   int *status;
   long long wait_cycles;
 };
+// How many parts of k a call is cut into, and with more than one the tiles (8 counters and
+// splits * 8192 floats of scratch each).
+uint32_t linear_fused_splits(const LinearFusedProblem &p, int num_sms, uint32_t *tiles);
 cudaError_t launch_linear_fused(const LinearFusedProblem &p, int num_sms, cudaStream_t stream);
 
 // ---- BERT fp32 forward (bert_ops.cu) ----

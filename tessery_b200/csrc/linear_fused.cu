@@ -11,6 +11,7 @@
 // Bound: for large k the tiles' way from L2 to shared memory (9.8 TB/s at 128 x 256), for small k
 // the epilogue.  Measured: 33500 x 1024 x 2048 into an fp32 residual 166 us, 847 TFLOP/s; 8192 x
 // 1536 x 384 with GELU 25 us, 387 TFLOP/s; 777 x 1000 x 1001 12.3 us.
+// Few tiles of long k: k is cut over CTAs, whose partial sums the last to arrive adds up.
 // gemv_kernel: a few rows (m <= 8) only stream w once: one or four warps per output column, w
 // straight from global memory into registers, the sums over lanes by shuffles.
 #include <cuda.h>
@@ -156,7 +157,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + C::kOffMisc + kOffAbort);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t nt = (p.n + kBN - 1) / kBN, mt = (p.m + kBM - 1) / kBM, tiles = nt * mt;
-  const uint32_t nk = (p.k + kBK - 1) / kBK, parts = (nk + kPart - 1) / kPart;
+  const uint32_t nk_all = (p.k + kBK - 1) / kBK;
+  // With a split k (64 columns, long k) a CTA has one tile and one part of k.
+  constexpr bool kSplits = kLong && kBN == 64;
+  const uint32_t splits = kSplits ? p.splits : 1, split = kSplits ? blockIdx.x % splits : 0;
+  const uint32_t tile_first = kSplits ? blockIdx.x / splits : blockIdx.x;
+  const uint32_t tile_step = kSplits && splits > 1 ? tiles : gridDim.x;
+  const uint32_t kb_first = kSplits ? nk_all * split / splits : 0;
+  const uint32_t nk = kSplits ? nk_all * (split + 1) / splits : nk_all;
+  const uint32_t parts = (nk - kb_first + kPart - 1) / kPart;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
@@ -188,9 +197,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       uint32_t fills = 0;
       bool ok = true;
-      for (uint32_t tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
+      for (uint32_t tile = tile_first; ok && tile < tiles; tile += tile_step) {
         const int m0 = (int)(tile / nt * kBM), n0 = (int)(tile % nt * kBN);
-        for (uint32_t kb = 0; kb < nk; ++kb) {
+        for (uint32_t kb = kb_first; kb < nk; ++kb) {
           const uint32_t s = fills % C::kStages, round = fills / C::kStages;
           if (round && !(ok = wait_bar(bar(kBarEmpty + s), (round - 1) & 1, abort_flag, p.status,
                                        kSiteEmpty, p.wait_cycles)))
@@ -211,8 +220,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       uint32_t step = 0, done = 0;  // K stages, partial sums
       bool ok = true;
-      for (uint32_t tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
-        for (uint32_t kb = 0; ok && kb < nk; ++done) {
+      for (uint32_t tile = tile_first; ok && tile < tiles; tile += tile_step) {
+        for (uint32_t kb = kb_first; ok && kb < nk; ++done) {
           const uint32_t b = done & 1, acc = tmem + b * kBN;
           if (done >= 2 && !(ok = wait_bar(bar(kBarFree + b), ((done >> 1) - 1) & 1, abort_flag,
                                            p.status, kSiteFree, p.wait_cycles)))
@@ -261,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       ++res_loads;
     };
-    for (uint32_t tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
+    for (uint32_t tile = tile_first; ok && tile < tiles; tile += tile_step) {
       const uint32_t m0 = tile / nt * kBM + quarter * 32, m = m0 + lane;
       const uint32_t n0 = tile % nt * kBN + half * kCols;
       const uint32_t box = f32_out ? 32 : 64;  // columns of a 128-byte staging row
@@ -428,8 +437,41 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_fence_before();
           mbar_arrive(bar(kBarFree + b));
         }
+        bool mine = true;
+        if constexpr (kSplits) {
+          // Every warp leaves its part of the tile; the one that arrives last adds them in the order
+          // of the splits and finishes.  All arrive, whatever happened, so that the counters return
+          // to zero.
+          if (splits > 1) {
+            const uint32_t w = (uint32_t)warp - 2;
+            auto at = [&](uint32_t s) {
+              return p.part + ((((size_t)tile * splits + s) * 8 + w) * kCols) * 32 + lane;
+            };
+            float *to = at(split);
 #pragma unroll
-        for (uint32_t c = 0; c < kCols; c += 32) finish(c, v + c);
+            for (uint32_t c = 0; c < kCols; ++c) to[c * 32] = v[c];
+            __threadfence();
+            __syncwarp();
+            uint32_t before = 0;
+            if (lane == 0) before = atomicAdd(&p.arrived[tile * 8 + w], 1u);
+            mine = __shfl_sync(0xffffffffu, before, 0) + 1 == splits;
+            if (mine) {
+              if (lane == 0) p.arrived[tile * 8 + w] = 0;
+              __threadfence();
+#pragma unroll
+              for (uint32_t c = 0; c < kCols; ++c) v[c] = 0.f;
+              for (uint32_t s = 0; s < splits; ++s) {
+                const float *from = at(s);
+#pragma unroll
+                for (uint32_t c = 0; c < kCols; ++c) v[c] += __ldcg(from + c * 32);
+              }
+            }
+          }
+        }
+        if (mine) {
+#pragma unroll
+          for (uint32_t c = 0; c < kCols; c += 32) finish(c, v + c);
+        }
       } else {
         const uint32_t b = done & 1, t0 = tmem + b * kBN + half * kCols + lanes;
         ok = __all_sync(0xffffffffu, wait_bar(bar(kBarAcc + b), (done >> 1) & 1, abort_flag,
@@ -603,8 +645,9 @@ cudaError_t launch_tiles(const LinearFusedProblem &p, int num_sms, cudaStream_t 
   if (e != cudaSuccess) return e;
   const uint64_t tiles = (uint64_t)((p.n + kBN - 1) / kBN) * ((p.m + kBM - 1) / kBM);
   if (tiles > 0x7fffffffull) return cudaErrorInvalidValue;
-  linear_kernel<kBN, kAct, kLong><<<(uint32_t)std::min<uint64_t>(tiles, (uint64_t)num_sms), kThreads,
-                             smem, stream>>>(mx, mw, mr, mo, p);
+  const uint32_t grid = p.splits > 1 ? (uint32_t)tiles * p.splits
+                                     : (uint32_t)std::min<uint64_t>(tiles, (uint64_t)num_sms);
+  linear_kernel<kBN, kAct, kLong><<<grid, kThreads, smem, stream>>>(mx, mw, mr, mo, p);
   return cudaGetLastError();
 }
 
@@ -615,6 +658,7 @@ cudaError_t launch_wide(const LinearFusedProblem &p, int num_sms, cudaStream_t s
   // k = 1024 widths 64 / 128 / 256 take 33 / 29 / 39 us for 33500 x 100, 115 / 71 / 75 us for
   // 33500 x 640, 178 / 107 / 96 us for 33500 x 1024, 21 / 16 / 28 us for 2048 x 1024 and
   // 13 / 15 / 27 us for 777 x 128.
+  if (p.splits > 1) return launch_tiles<64, kAct, kLong>(p, num_sms, stream);
   const uint64_t mt = (p.m + kBM - 1) / kBM;
   auto cost = [&](uint64_t bn, uint64_t wave, uint64_t once) {
     return (mt * ((p.n + bn - 1) / bn) + num_sms - 1) / num_sms * wave + once;
@@ -625,12 +669,18 @@ cudaError_t launch_wide(const LinearFusedProblem &p, int num_sms, cudaStream_t s
   return launch_tiles<64, kAct, kLong>(p, num_sms, stream);
 }
 
+// A few rows stream w once; past these sizes the conversions and sums of every row cost more than
+// a tile's.  By columns against tiles: 10 / 14 us for 8 x 1024 x 1024, 14 / 18 us for
+// 4 x 1024 x 4096, 18 / 22 us for 2 x 4096 x 4096, but 22 / 18 us for 8 x 1024 x 4096, 27 / 22 us
+// for 4 x 4096 x 4096 and 22 / 20 us for 2 x 16384 x 1024.
+bool by_columns(const LinearFusedProblem &p) {
+  return p.m == 1 || (p.m == 2 && p.n <= 8192) ||
+         (p.m <= 8 && p.k <= 4096 && (uint64_t)p.m * p.n * p.k <= 1 << 24);
+}
+
 template <int kAct>
 cudaError_t launch_act(LinearFusedProblem p, int num_sms, cudaStream_t stream) {
-  // A few rows stream w once; with more outputs than these the conversions and sums of every row
-  // cost more than a tile's: 10 against 14 us for 8 x 1024 x 1024, 27 against 34 us for
-  // 4 x 4096 x 4096, but 43 against 33 us for 8 x 4096 x 4096.
-  if (p.m == 1 || (p.m <= 8 && (uint64_t)p.m * p.n <= 16384)) return launch_gemv<kAct>(p, stream);
+  if (by_columns(p)) return launch_gemv<kAct>(p, stream);
   const uint32_t vo = p.out_dtype == TX_BF16 ? 8 : 4, vr = p.residual_dtype == TX_BF16 ? 8 : 4;
   p.out_vec = (uintptr_t)p.out % 16 == 0 && p.ldo % vo == 0;
   p.res_vec = p.residual && (uintptr_t)p.residual % 16 == 0 && p.ldr % vr == 0;
@@ -642,6 +692,18 @@ cudaError_t launch_act(LinearFusedProblem p, int num_sms, cudaStream_t stream) {
 }
 
 }  // namespace lfused
+
+// k is cut where the 64-column tiles would leave half the SMs without one: as many parts as SMs for
+// each tile, of 256 columns at least.  16 x 1024 x 4096 29 -> 18 us, 773 x 117 x 3754 33 -> 22 us,
+// 16 x 1024 x 1024 14.3 us either way.
+uint32_t linear_fused_splits(const LinearFusedProblem &p, int num_sms, uint32_t *tiles) {
+  using namespace lfused;
+  const uint64_t t = (uint64_t)((p.m + kBM - 1) / kBM) * ((p.n + 63) / 64);
+  *tiles = 0;
+  if (by_columns(p) || p.k <= kPart * kBK || 2 * t > (uint64_t)num_sms) return 1;
+  *tiles = (uint32_t)t;
+  return std::min<uint32_t>((uint32_t)(num_sms / t), (p.k + kBK - 1) / kBK / 4);
+}
 
 cudaError_t launch_linear_fused(const LinearFusedProblem &p, int num_sms, cudaStream_t stream) {
   switch (p.act) {

@@ -1847,9 +1847,22 @@ int tx_linear_fused(void *ctx, const void *x, uint64_t ldx, const void *w, uint6
   p.residual_dtype = residual_dtype; p.out_dtype = out_dtype; p.act = activation;
   p.status = c->status;
   p.wait_cycles = c->wait_cycles > 0 ? c->wait_cycles : 2000000000ll;
-  cudaSetDevice(c->device);
-  cudaError_t e = tx::launch_linear_fused(p, c->sms, stream ? (cudaStream_t)stream : c->stream);
+  cudaError_t e = cudaSetDevice(c->device);
+  if (e != cudaSuccess) return cuda_fail(c, e, "cudaSetDevice");
+  cudaStream_t st = stream ? (cudaStream_t)stream : c->stream;
+  uint32_t tiles;
+  p.splits = tx::linear_fused_splits(p, c->sms, &tiles);
+  if (p.splits > 1) {
+    if ((e = ensure_parts(c, 8 * (size_t)tiles, (size_t)tiles * p.splits * 8192 * 4)) != cudaSuccess)
+      return cuda_fail(c, e, "partial sums allocation");
+    p.arrived = (uint32_t *)c->part_mem;
+    p.part = (float *)(c->part_mem + ((c->part_units * 4 + 255) & ~(size_t)255));
+    if ((e = scratch_acquire(c, st)) != cudaSuccess) return cuda_fail(c, e, "scratch wait");
+  }
+  e = tx::launch_linear_fused(p, c->sms, st);
   if (e != cudaSuccess) return cuda_fail(c, e, "linear_fused launch");
+  if (p.splits > 1 && (e = scratch_release(c, st)) != cudaSuccess)
+    return cuda_fail(c, e, "scratch event");
   c->last_kernel = "linear_fused";
   ++c->launches;
   return TX_OK;

@@ -100,6 +100,23 @@ def test_several_tiles_in_turn(runtime, m, n, k, out):
     check(linear_fused(x, w, residual=r, out_dtype=out, runtime=runtime), xf, wf, None, "none", rf)
 
 
+@pytest.mark.parametrize("m,n,k", [(9, 4096, 513), (40, 65, 4097), (130, 343, 1024), (773, 117, 3754),
+                                   (16, 1024, 4096), (20, 1, 9000)])
+@pytest.mark.parametrize("out", ["float32", "bf16"])
+def test_few_tiles_of_long_k(runtime, m, n, k, out):
+    """k cut into parts that CTAs of their own sum: right, the same every time, and the counters as
+    they were before."""
+    rng = np.random.default_rng(m + k)
+    x, xf = bf16(rng, (m, k))
+    w, wf = bf16(rng, (n, k), k**-0.5)
+    bias = rng.standard_normal(n).astype(np.float32)
+    r, rf = bf16(rng, (m, n))
+    got = [linear_fused(x, w, bias=bias, activation="silu", residual=r, out_dtype=out,
+                        runtime=runtime) for _ in range(3)]
+    check(got[0], xf, wf, bias, "silu", rf)
+    assert np.array_equal(got[0], got[1]) and np.array_equal(got[0], got[2])
+
+
 @pytest.mark.parametrize("m", [2, 40])
 @pytest.mark.parametrize("act", ACTS)
 def test_infinite_sums_stay_infinite(runtime, m, act):
