@@ -10,9 +10,10 @@
 // split operands (hi + lo, three products, error 2^-22).  The 64-row fp32 kernel would compute 64
 // rows for these (when this one takes which call: scored_route in attn_scored_tc.cu).
 //
-// Measured: 8 new tokens, 16 query and 8 kv heads of 128, a cap, 64 to 2048 keys each: 25 us
+// Measured: 8 new tokens, 16 query and 8 kv heads of 128, a cap, 64 to 2048 keys each: 23 us
 // between events, of which some 6 are the launch's; 32 texts of 1024 keys, 12 heads of 64 (101 MB):
-// 39 us, 2.6 TB/s.  More parts than CTAs that run at once gave no gain.
+// 39 us, 2.6 TB/s.  11 texts of 1428 to 6289 keys, 32 / 8 heads of 128 in fp32
+// (437 MB): 249 us, bound by the split operands' products.
 #include <cuda_runtime.h>
 
 #include "../../include/tessattn.h"
