@@ -63,8 +63,10 @@ struct Unit {
 // Key range of a query position without the prefix: [lo, hi).
 __device__ __forceinline__ void row_range(const ScoredProblem &p, int pos, int nk, int *lo,
                                           int *hi) {
+  // Neither end may pass 32 bits: a position is negative where there are more queries than keys, and
+  // a reach may be any int.
   int l = 0, h = nk;
-  if (p.left >= 0) l = max(l, pos - p.left);
+  if (p.left >= 0 && pos > p.left) l = pos - p.left;
   if (p.causal) h = min(h, pos + 1);
   if (p.right >= 0 && pos < 0x7fffffff - p.right) h = min(h, pos + p.right + 1);
   *lo = l;

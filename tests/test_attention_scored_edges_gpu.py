@@ -1,0 +1,127 @@
+"""Attention under a score rule at the ends of its arguments: queries before the first key with
+windows of any reach, infinite and largest finite values, caps of any size, distance tables with
+special values and of every place they are kept in.  Against the formula in 64 bits.
+
+Tolerances, per element, from each row's own scores: A = sum_j p_j |v_j|, Z = the largest
+scale sum |q||k| over finite products of the row, or the largest finite |score| if that is more (a
+cap adds nothing: a capped score is off relative to itself).  As in test_attention_scored_gpu,
+a score is off by at most 2^-20 (Z + 1) in the fp32 kernels and 2^-19 (Z + 1) in the bf16 ones,
+which moves the output by twice that times A, and P.V adds 2^-20 A in fp32, 2^-16 A where P is held
+in two bf16 parts (2^-17 each) and 2^-8 A where it is rounded to bf16 once."""
+
+import numpy as np
+import pytest
+
+from oracle import layers as oracle
+from tessery_b200.layers import attention_scored
+from tessery_b200.workloads import from_bf16_bits, to_bf16_bits
+
+pytestmark = pytest.mark.gpu
+
+LARGE = 2**31 - 1
+
+
+def exact(q, k, v, *, softcap=0.0, slopes=None, table=None, **rule):
+    """One sequence in 64 bits: the output, A and Z per row [nq, heads, dim] / [nq, heads, 1]."""
+    q, k, v = (np.asarray(x, np.float64) for x in (q, k, v))
+    (nq, heads, dim), nk = q.shape, k.shape[0]
+    group, scale = heads // k.shape[1], dim**-0.5
+    seen = oracle.open_keys(nq, nk, **rule)
+    dist = np.arange(nk)[None] - (np.arange(nq)[:, None] + nk - nq)
+    out, mass, size = np.zeros((nq, heads, dim)), np.zeros((nq, heads, dim)), np.zeros((nq, heads, 1))
+    with np.errstate(invalid="ignore", over="ignore"):
+        for h in range(heads):
+            for i in range(nq):
+                at = np.flatnonzero(seen[i])
+                if not at.size:
+                    continue
+                kh, vh = k[at, h // group], v[at, h // group]
+                products = scale * kh * q[i, h]
+                z = products.sum(-1)
+                size[i, h] = np.where(np.isfinite(products), np.abs(products), 0).sum(-1).max()
+                if softcap:
+                    z = softcap * np.tanh(z / softcap)
+                if slopes is not None:
+                    z = z - float(slopes[h]) * np.abs(dist[i, at])
+                if table is not None:
+                    reach = table.shape[1] // 2
+                    z = z + np.asarray(table[h], np.float64)[
+                        np.clip(dist[i, at], -reach, reach) + reach]
+                common = np.abs(z[np.abs(z) < 1e30])
+                size[i, h] = max(size[i, h, 0], common.max(initial=0.0))
+                if np.max(z) == -np.inf:
+                    continue
+                p = np.exp(z - np.max(z))
+                p /= p.sum()
+                used = p != 0
+                out[i, h], mass[i, h] = p[used] @ vh[used], p[used] @ np.abs(vh[used])
+    return out, mass, size
+
+
+def relative(took, dtype, size):
+    f32 = took == "scored_f32" or dtype == "f32"
+    scores = 2 * (size + 1) * (2.0**-20 if f32 else 2.0**-19)
+    return scores + (2.0**-20 if f32 else 2.0**-16 if took == "scored_few" else 2.0**-8)
+
+
+def check(runtime, q, k, v, dtype, *, route=None, distance_bias=None, **rule):
+    """Runs one sequence of float values with fp32 output and compares every element."""
+    if dtype == "bf16":
+        held = [to_bf16_bits(x) for x in (q, k, v)]
+        q, k, v = (from_bf16_bits(x) for x in held)
+    else:
+        held = [np.asarray(x, np.float32) for x in (q, k, v)]
+    host = dict(rule)
+    if "prefix" in host:
+        host["prefix"] = np.array([host["prefix"]])
+    got = attention_scored(*held, cu_q=np.array([0, len(q)]), cu_k=np.array([0, len(k)]),
+                           distance_bias=distance_bias, out_dtype="float32", runtime=runtime, **host)
+    took = runtime.last_kernel()
+    if route:
+        assert took == route
+    rule.setdefault("causal", True)
+    want, mass, size = exact(q, k, v, table=distance_bias, **rule)
+    finite = np.isfinite(want)
+    np.testing.assert_array_equal(np.isnan(got), np.isnan(want))
+    np.testing.assert_array_equal(got[np.isinf(want)], want[np.isinf(want)])
+    with np.errstate(invalid="ignore"):
+        bad = finite & ~(np.abs(got - want) <= relative(took, dtype, size) * mass + 1e-30)
+    assert not bad.any(), (took, np.argwhere(bad)[:4], got[bad][:4], want[bad][:4])
+    return got
+
+
+def normal(seed, nq, nk, heads, kv_heads, dim):
+    rng = np.random.default_rng(seed)
+    return (rng.standard_normal((nq, heads, dim)).astype(np.float32),
+            *(rng.standard_normal((nk, kv_heads, dim)).astype(np.float32) for _ in range(2)))
+
+
+# ROUTES: (kernel, dtype, query rows, heads, kv_heads, dim)
+ROUTES = [("scored_tc", "bf16", 40, 2, 1, 64), ("scored_tc", "bf16", 40, 4, 2, 128),
+          ("scored_f32", "f32", 40, 2, 1, 64), ("scored_f32", "bf16", 40, 2, 1, 160),
+          ("scored_few", "bf16", 6, 1, 1, 64), ("scored_few", "f32", 6, 2, 1, 64),
+          ("scored_few", "bf16", 5, 3, 1, 136)]
+
+
+@pytest.mark.parametrize("kernel,dtype,nq,heads,kv_heads,dim", ROUTES)
+@pytest.mark.parametrize("rule", [
+    dict(causal=False, window=(LARGE, -1)), dict(causal=False, window=(LARGE, LARGE)),
+    dict(causal=False, window=(LARGE - 1, 0)), dict(window=(LARGE, LARGE)),
+    dict(causal=False, window=(2, 3)), dict(causal=False, window=(-1, 1)),
+    dict(causal=False, window=(0, 4), prefix=2), dict(causal=False, slopes=True),
+    dict(causal=False, table=True), dict(causal=False, docs=True),
+    dict(causal=False, docs=True, window=(LARGE, 2), slopes=True)])
+def test_queries_before_the_first_key(runtime, kernel, dtype, nq, heads, kv_heads, dim, rule):
+    """More query rows than keys: the first ones stand at negative positions."""
+    rule = dict(rule)
+    if rule.pop("slopes", False):
+        rule["slopes"] = (0.5 ** np.arange(1, heads + 1)).astype(np.float32)
+    if rule.pop("table", False):
+        rule["distance_bias"] = np.random.default_rng(1).standard_normal(
+            (heads, 2 * 4 + 1)).astype(np.float32)
+    for nk in (3, 1):
+        q, k, v = normal(nk, nq, nk, heads, kv_heads, dim)
+        if rule.pop("docs", False) or "k_docs" in rule:
+            rule["k_docs"] = np.arange(nk, dtype=np.int32) % 2
+            rule["q_docs"] = (np.arange(nq, dtype=np.int32) % 3) - 1
+        check(runtime, q, k, v, dtype, route=kernel, **rule)
