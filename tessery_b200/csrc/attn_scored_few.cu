@@ -16,6 +16,8 @@
 // (437 MB): 249 us, bound by the split operands' products.
 #include <cuda_runtime.h>
 
+#include <type_traits>
+
 #include "../../include/tessattn.h"
 #include "attn_scored.cuh"
 #include "common.cuh"
@@ -207,205 +209,230 @@ __global__ void __launch_bounds__(Cfg<T, kDP>::kThreads, Cfg<T, kDP>::kResident)
   }
   const float cap_a = p.softcap > 0.f ? 2.f * kLog2e / p.softcap : 0.f;
   float o[kDP / 8][4];
+
+  // Values that are not finite.  A key closed to a row has p = 0 there, and the product would turn
+  // 0 * Inf or 0 * NaN into NaN; and a part of an operand times Inf need not be what the whole gives
+  // (a lo part is 0 or below it as often as above).  So a warp whose sums come out not finite (rare)
+  // walks its keys once more, carefully: with weights of at most 1, and with the value rows that
+  // hold such a value added by hand where p > 0 and zeroed before the product.  (The careful part
+  // kept out of the first walk: 32 texts of 1024 keys, 12 heads of 64, take 37.0 us in bf16 either
+  // way, 11 texts in fp32 208 against 251 us with values looked over in every block with a
+  // closed key.)
+  auto walk = [&](auto how) {
+    constexpr bool careful = decltype(how)::value;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) m[h] = -INFINITY, l[h] = 0.f;
+#pragma unroll
+    for (int n = 0; n < kDP / 8; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
+    int stage = 0;
+    for (int i = u.first + warp; i < u.last; i += C::kWarps) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+      __syncwarp();  // every lane's pieces are there, and the stage to fill has been read
+      fetch(ahead, (stage + kStages - 1) % kStages);
+      ahead += C::kWarps;
+      const uint32_t ks = ring + stage * C::kStageBytes, vs = ks + kBlock * C::kRowBytes;
+      stage = (stage + 1) % kStages;
+      const int k0 = (i < u.a ? i : i - u.a + u.b) * kBlock;
+
+      // S = Q K^T; a 16-byte piece of a key row is lane t's share of two steps (of 16 columns in
+      // bf16, 8 in fp32), in the order in which it lies: the query rows are read alike.
+      float s[2][4] = {};
+#pragma unroll
+      for (int q = 0; q < C::kChunks / 4; ++q) {
+        uint4 kw[2];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) kw[n] = ld_shared_v4(ks + C::k_at(8 * n + g, 4 * q + t));
+        if constexpr (C::kF32) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int c = (4 * q + t) * 4 + 2 * j;
+            const float2 q0 = *reinterpret_cast<const float2 *>(qs + g * C::kQP + c);
+            const float2 q1 = *reinterpret_cast<const float2 *>(qs + (g + 8) * C::kQP + c);
+            uint32_t ah[4], al[4];
+            split(q0.x, ah[0], al[0]);
+            split(q1.x, ah[1], al[1]);
+            split(q0.y, ah[2], al[2]);
+            split(q1.y, ah[3], al[3]);
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+              mma_split(s[n], ah, al, __uint_as_float(ptx::u4_at(kw[n], 2 * j)),
+                        __uint_as_float(ptx::u4_at(kw[n], 2 * j + 1)));
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            uint32_t a[4];
+            if constexpr (!kQRegs) q_words(q, j, a);
+            const uint32_t(&qw)[4] = kQRegs ? qa[kQRegs ? 2 * q + j : 0] : a;
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+              mma_bf16(s[n], qw, ptx::u4_at(kw[n], 2 * j), ptx::u4_at(kw[n], 2 * j + 1));
+          }
+        }
+      }
+
+      // Scores, masked.  The step to log2 units comes behind the subtraction of the reference: a
+      // large score times log2 e would be rounded before it.
+      float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int h = e >> 1, j = k0 + 8 * n + 2 * t + (e & 1);
+          const Row &w = row[h];
+          float z = s[n][e] * p.scale;
+          if (p.softcap > 0.f) {
+            if constexpr (C::kF32)
+              z = p.softcap * tanhf(z / p.softcap);
+            else  // 1 - 2 / (1 + e^(2u)) by hardware: 2^-21 of the cap
+              z = fmaf(-2.f * p.softcap, rcp(1.f + ex2(z * cap_a)), p.softcap);
+          }
+          if (p.slopes) z = fmaf(-slope[h], fabsf((float)(j - w.pos)), z);
+          if (p.table) z += __ldg(table[h] + min(max(j - w.pos, -p.reach), p.reach));
+          bool open = j < w.prefix || (j >= w.lo && j < w.hi);
+          if (p.k_docs) open = open && p.k_docs[u.s.k_row + j] == w.doc;
+          s[n][e] = open ? z : -INFINITY;
+          top[h] = fmaxf(top[h], s[n][e]);
+        }
+      bool raise = false;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+        raise = raise || top[h] > m[h] + (careful ? 0.f : kRescaleThreshold) ||
+                (m[h] == -INFINITY && top[h] > m[h]);
+      }
+      if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float now = fmaxf(m[h], top[h]);
+          const float f = m[h] == -INFINITY ? 0.f : exp2f((m[h] - now) * kLog2e);
+          m[h] = now;
+          l[h] *= f;
+#pragma unroll
+          for (int n = 0; n < kDP / 8; ++n) {
+            o[n][2 * h] *= f;
+            o[n][2 * h + 1] *= f;
+          }
+        }
+      }
+      const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[n][e] = ex2((s[n][e] - ref[e >> 1]) * kLog2e);
+          l[e >> 1] += s[n][e];
+        }
+
+      if constexpr (careful) {
+        uint32_t bad = 0;
+#pragma unroll 4
+        for (int x = lane; x < kBlock * C::kChunks; x += 32) {
+          const uint4 w = ld_shared_v4(vs + x * 16);
+          if (!(finite_word(w.x, C::kF32) && finite_word(w.y, C::kF32) &&
+                finite_word(w.z, C::kF32) && finite_word(w.w, C::kF32)))
+            bad |= 1u << (x / C::kChunks);
+        }
+        bad = __reduce_or_sync(0xffffffffu, bad);
+        while (bad) {
+          const int j = __ffs(bad) - 1;
+          bad &= bad - 1;
+          float pj[2];  // this row's weight of key j, from the lane that has it
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float mine = 0.f;
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                if (j == 8 * n + (j & 6) + e) mine = s[n][2 * h + e];
+            pj[h] = __shfl_sync(0xffffffffu, mine, (lane & ~3) | ((j & 7) >> 1));
+          }
+#pragma unroll
+          for (int n = 0; n < kDP / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              // fp32: column 8n + 2t + (e & 1); bf16: see P.V below
+              const int c = C::kF32 ? 8 * n + 2 * t + (e & 1)
+                                    : 16 * (n / 2) + 2 * (2 * t + (e & 1)) + (n & 1);
+              const int byte = c * (int)sizeof(T);
+              const float x = Elem<T>::load(
+                  reinterpret_cast<const T *>(smem + (vs - ptx::smem_addr(smem)) +
+                                              C::v_at(j, byte / 16) + byte % 16), 0);
+              if (!(pj[e >> 1] == 0.f)) o[n][e] = fmaf(pj[e >> 1], x, o[n][e]);
+            }
+          __syncwarp();
+          for (int x = lane; x < C::kChunks; x += 32)
+            ptx::st_shared_v4(vs + j * C::kRowBytes + x * 16, 0, 0, 0, 0);
+          __syncwarp();
+        }
+      }
+
+      // O += P V.  S's accumulator holds keys 2t and 2t + 1 of each 8 of a row: how P enters.
+      const int sw = (t << 1) & (C::kChunks - 1);  // the rows' exchange of pieces
+      const uint32_t vr = vs + 2 * t * C::kRowBytes + (g >> 2) * 16 + (g & 3) * 4;
+      auto word = [&](int row, int piece) {
+        uint32_t w;
+        asm volatile("ld.shared.b32 %0, [%1];"
+                     : "=r"(w)
+                     : "r"(vr + row * C::kRowBytes + (piece ^ sw) * 16)
+                     : "memory");
+        return w;
+      };
+      if constexpr (C::kF32) {
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+          uint32_t ah[4], al[4];
+          split(s[kk][0], ah[0], al[0]);
+          split(s[kk][2], ah[1], al[1]);
+          split(s[kk][1], ah[2], al[2]);
+          split(s[kk][3], ah[3], al[3]);
+#pragma unroll
+          for (int n = 0; n < kDP / 8; ++n)
+            mma_split(o[n], ah, al, __uint_as_float(word(8 * kk, 2 * n)),
+                      __uint_as_float(word(8 * kk + 1, 2 * n)));
+        }
+      } else {
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const float a = s[x >> 1][2 * (x & 1)], b = s[x >> 1][2 * (x & 1) + 1];
+          hi[x] = pack_bf16x2(a, b);
+          lo[x] = pack_bf16x2(a - ptx::bf16_lo(hi[x]), b - ptx::bf16_hi(hi[x]));
+        }
+        // A word holds columns 16i + 2g and 16i + 2g + 1 of a key: the even ones go to accumulator
+        // 2i, the odd ones to 2i + 1.
+#pragma unroll
+        for (int i2 = 0; i2 < kDP / 16; ++i2) {
+          const uint32_t w0 = word(0, 2 * i2), w1 = word(1, 2 * i2), w2 = word(8, 2 * i2),
+                         w3 = word(9, 2 * i2);
+          const uint32_t e0 = __byte_perm(w0, w1, 0x5410), e1 = __byte_perm(w2, w3, 0x5410);
+          const uint32_t d0 = __byte_perm(w0, w1, 0x7632), d1 = __byte_perm(w2, w3, 0x7632);
+          mma_bf16(o[2 * i2], lo, e0, e1);
+          mma_bf16(o[2 * i2 + 1], lo, d0, d1);
+          mma_bf16(o[2 * i2], hi, e0, e1);
+          mma_bf16(o[2 * i2 + 1], hi, d0, d1);
+        }
+      }
+    }
+  };
+  walk(std::false_type());
+  float taint[2] = {0.f, 0.f};  // NaN where a sum is not finite
 #pragma unroll
   for (int n = 0; n < kDP / 8; ++n)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
-
-  int stage = 0;
-  for (int i = u.first + warp; i < u.last; i += C::kWarps) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-    __syncwarp();  // every lane's pieces are there, and the stage to fill has been read
-    fetch(ahead, (stage + kStages - 1) % kStages);
-    ahead += C::kWarps;
-    const uint32_t ks = ring + stage * C::kStageBytes, vs = ks + kBlock * C::kRowBytes;
-    stage = (stage + 1) % kStages;
-    const int k0 = (i < u.a ? i : i - u.a + u.b) * kBlock;
-
-    // S = Q K^T; a 16-byte piece of a key row is lane t's share of two steps (of 16 columns in bf16,
-    // 8 in fp32), in the order in which it lies: the query rows are read alike.
-    float s[2][4] = {};
-#pragma unroll
-    for (int q = 0; q < C::kChunks / 4; ++q) {
-      uint4 kw[2];
-#pragma unroll
-      for (int n = 0; n < 2; ++n) kw[n] = ld_shared_v4(ks + C::k_at(8 * n + g, 4 * q + t));
-      if constexpr (C::kF32) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int c = (4 * q + t) * 4 + 2 * j;
-          const float2 q0 = *reinterpret_cast<const float2 *>(qs + g * C::kQP + c);
-          const float2 q1 = *reinterpret_cast<const float2 *>(qs + (g + 8) * C::kQP + c);
-          uint32_t ah[4], al[4];
-          split(q0.x, ah[0], al[0]);
-          split(q1.x, ah[1], al[1]);
-          split(q0.y, ah[2], al[2]);
-          split(q1.y, ah[3], al[3]);
-#pragma unroll
-          for (int n = 0; n < 2; ++n)
-            mma_split(s[n], ah, al, __uint_as_float(ptx::u4_at(kw[n], 2 * j)),
-                      __uint_as_float(ptx::u4_at(kw[n], 2 * j + 1)));
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          uint32_t a[4];
-          if constexpr (!kQRegs) q_words(q, j, a);
-          const uint32_t(&qw)[4] = kQRegs ? qa[kQRegs ? 2 * q + j : 0] : a;
-#pragma unroll
-          for (int n = 0; n < 2; ++n)
-            mma_bf16(s[n], qw, ptx::u4_at(kw[n], 2 * j), ptx::u4_at(kw[n], 2 * j + 1));
-        }
-      }
-    }
-
-    // Scores, masked.  The step to log2 units comes behind the subtraction of the reference: a large
-    // score times log2 e would be rounded before it.
-    bool all = true;
-    float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int h = e >> 1, j = k0 + 8 * n + 2 * t + (e & 1);
-        const Row &w = row[h];
-        float z = s[n][e] * p.scale;
-        if (p.softcap > 0.f) {
-          if constexpr (C::kF32)
-            z = p.softcap * tanhf(z / p.softcap);
-          else  // 1 - 2 / (1 + e^(2u)) by hardware: 2^-21 of the cap
-            z = fmaf(-2.f * p.softcap, rcp(1.f + ex2(z * cap_a)), p.softcap);
-        }
-        if (p.slopes) z = fmaf(-slope[h], fabsf((float)(j - w.pos)), z);
-        if (p.table) z += __ldg(table[h] + min(max(j - w.pos, -p.reach), p.reach));
-        bool open = j < w.prefix || (j >= w.lo && j < w.hi);
-        if (p.k_docs) open = open && p.k_docs[u.s.k_row + j] == w.doc;
-        all = all && (open || g + 8 * h >= rows);
-        s[n][e] = open ? z : -INFINITY;
-        top[h] = fmaxf(top[h], s[n][e]);
-      }
-    bool raise = false;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-      top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
-      raise = raise || top[h] > m[h] + kRescaleThreshold || (m[h] == -INFINITY && top[h] > m[h]);
-    }
-    if (__any_sync(0xffffffffu, raise)) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float now = fmaxf(m[h], top[h]);
-        const float f = m[h] == -INFINITY ? 0.f : exp2f((m[h] - now) * kLog2e);
-        m[h] = now;
-        l[h] *= f;
-#pragma unroll
-        for (int n = 0; n < kDP / 8; ++n) {
-          o[n][2 * h] *= f;
-          o[n][2 * h + 1] *= f;
-        }
-      }
-    }
-    const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[n][e] = ex2((s[n][e] - ref[e >> 1]) * kLog2e);
-        l[e >> 1] += s[n][e];
-      }
-
-    // A key closed to a row has p = 0 there, but zero times a value that is not finite would not be
-    // zero: value rows with such a value (rare) are added by hand where p > 0 and then zeroed.
-    // Looked for only where some key is closed to some row.
-    if (__any_sync(0xffffffffu, !all)) {
-      uint32_t bad = 0;
-#pragma unroll 4
-      for (int x = lane; x < kBlock * C::kChunks; x += 32) {
-        const uint4 w = ld_shared_v4(vs + x * 16);
-        if (!(finite_word(w.x, C::kF32) && finite_word(w.y, C::kF32) &&
-              finite_word(w.z, C::kF32) && finite_word(w.w, C::kF32)))
-          bad |= 1u << (x / C::kChunks);
-      }
-      bad = __reduce_or_sync(0xffffffffu, bad);
-      while (bad) {
-        const int j = __ffs(bad) - 1;
-        bad &= bad - 1;
-        float pj[2];  // this row's weight of key j, from the lane that has it
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float mine = 0.f;
-#pragma unroll
-          for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-              if (j == 8 * n + (j & 6) + e) mine = s[n][2 * h + e];
-          pj[h] = __shfl_sync(0xffffffffu, mine, (lane & ~3) | ((j & 7) >> 1));
-        }
-#pragma unroll
-        for (int n = 0; n < kDP / 8; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            // fp32: column 8n + 2t + (e & 1); bf16: see P.V below
-            const int c = C::kF32 ? 8 * n + 2 * t + (e & 1)
-                                  : 16 * (n / 2) + 2 * (2 * t + (e & 1)) + (n & 1);
-            const int byte = c * (int)sizeof(T);
-            const float x = Elem<T>::load(
-                reinterpret_cast<const T *>(smem + (vs - ptx::smem_addr(smem)) +
-                                            C::v_at(j, byte / 16) + byte % 16), 0);
-            if (!(pj[e >> 1] == 0.f)) o[n][e] = fmaf(pj[e >> 1], x, o[n][e]);
-          }
-        __syncwarp();
-        for (int x = lane; x < C::kChunks; x += 32) ptx::st_shared_v4(vs + j * C::kRowBytes + x * 16, 0, 0, 0, 0);
-        __syncwarp();
-      }
-    }
-
-    // O += P V.  S's accumulator holds keys 2t and 2t + 1 of each 8 of a row, which is how P enters.
-    const int sw = (t << 1) & (C::kChunks - 1);  // the rows' exchange of pieces
-    const uint32_t vr = vs + 2 * t * C::kRowBytes + (g >> 2) * 16 + (g & 3) * 4;
-    auto word = [&](int row, int piece) {
-      uint32_t w;
-      asm volatile("ld.shared.b32 %0, [%1];"
-                   : "=r"(w)
-                   : "r"(vr + row * C::kRowBytes + (piece ^ sw) * 16)
-                   : "memory");
-      return w;
-    };
-    if constexpr (C::kF32) {
-#pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
-        uint32_t ah[4], al[4];
-        split(s[kk][0], ah[0], al[0]);
-        split(s[kk][2], ah[1], al[1]);
-        split(s[kk][1], ah[2], al[2]);
-        split(s[kk][3], ah[3], al[3]);
-#pragma unroll
-        for (int n = 0; n < kDP / 8; ++n)
-          mma_split(o[n], ah, al, __uint_as_float(word(8 * kk, 2 * n)),
-                    __uint_as_float(word(8 * kk + 1, 2 * n)));
-      }
-    } else {
-      uint32_t hi[4], lo[4];
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const float a = s[x >> 1][2 * (x & 1)], b = s[x >> 1][2 * (x & 1) + 1];
-        hi[x] = pack_bf16x2(a, b);
-        lo[x] = pack_bf16x2(a - ptx::bf16_lo(hi[x]), b - ptx::bf16_hi(hi[x]));
-      }
-      // A word holds columns 16i + 2g and 16i + 2g + 1 of a key: the even ones go to accumulator
-      // 2i, the odd ones to 2i + 1.
-#pragma unroll
-      for (int i2 = 0; i2 < kDP / 16; ++i2) {
-        const uint32_t w0 = word(0, 2 * i2), w1 = word(1, 2 * i2), w2 = word(8, 2 * i2),
-                       w3 = word(9, 2 * i2);
-        const uint32_t e0 = __byte_perm(w0, w1, 0x5410), e1 = __byte_perm(w2, w3, 0x5410);
-        const uint32_t d0 = __byte_perm(w0, w1, 0x7632), d1 = __byte_perm(w2, w3, 0x7632);
-        mma_bf16(o[2 * i2], lo, e0, e1);
-        mma_bf16(o[2 * i2 + 1], lo, d0, d1);
-        mma_bf16(o[2 * i2], hi, e0, e1);
-        mma_bf16(o[2 * i2 + 1], hi, d0, d1);
-      }
-    }
+    for (int e = 0; e < 4; ++e) taint[e >> 1] = fmaf(o[n][e], 0.f, taint[e >> 1]);
+  const bool odd = (g < rows && taint[0] != 0.f) || (g + 8 < rows && taint[1] != 0.f);
+  if (__any_sync(0xffffffffu, odd)) {
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncwarp();  // the ring is free
+    ahead = u.first + warp;
+#pragma unroll 1
+    for (int s = 0; s < kStages - 1; ++s, ahead += C::kWarps) fetch(ahead, s);
+    walk(std::true_type());
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll

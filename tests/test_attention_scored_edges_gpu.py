@@ -125,3 +125,15 @@ def test_queries_before_the_first_key(runtime, kernel, dtype, nq, heads, kv_head
             rule["k_docs"] = np.arange(nk, dtype=np.int32) % 2
             rule["q_docs"] = (np.arange(nq, dtype=np.int32) % 3) - 1
         check(runtime, q, k, v, dtype, route=kernel, **rule)
+
+
+@pytest.mark.parametrize("kernel,dtype,nq,heads,kv_heads,dim", ROUTES)
+def test_infinite_values_that_a_row_sees(runtime, kernel, dtype, nq, heads, kv_heads, dim):
+    """An infinite value of v makes its column infinite, two of both signs make it NaN, and the
+    other columns are as ever, whether or not a key near it is closed."""
+    q, k, v = normal(3, nq, 300, heads, kv_heads, dim)
+    v[20, :, 1], v[20, :, 2], v[150, :, 4] = np.inf, -np.inf, np.inf
+    v[20, :, 5], v[21, :, 5], v[77, :, 7] = np.inf, -np.inf, np.nan
+    check(runtime, q, k, v, dtype, route=kernel, causal=False)
+    check(runtime, q, k, v, dtype, route=kernel)
+    check(runtime, q, k, v, dtype, route=kernel, window=(200, -1), prefix=30)
