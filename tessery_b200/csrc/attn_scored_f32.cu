@@ -19,6 +19,8 @@
 // slopes: 45 us (43 % of issue slots); 32 keys a step with half as many CTAs again: 46.5 us.
 #include <cuda_runtime.h>
 
+#include <type_traits>
+
 #include "../../include/tessattn.h"
 #include "attn_scored.cuh"
 #include "common.cuh"
@@ -33,6 +35,7 @@ using ptx::ex2;
 
 constexpr int kRows = 64, kThreads = 128, kStep = 64;  // kStep keys staged at a time
 constexpr float kLog2e = 1.44269504088896341f;
+constexpr float kOdd = 0x1p127f;  // values from here on are added by hand
 
 // Row pitches (floats) that keep the fragment reads free of bank conflicts: Q and K are read as
 // pairs (8 words between rows modulo 32), V by single values of every second row (4 words).
@@ -128,7 +131,7 @@ __global__ void __launch_bounds__(kThreads, kDP <= 64 ? 4 : 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 
   // This thread's two rows.
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  float m[2], l[2];
   Row row[2];
   int head[2];
   const float *table[2];
@@ -142,10 +145,6 @@ __global__ void __launch_bounds__(kThreads, kDP <= 64 ? 4 : 1)
     slope[h] = p.slopes ? p.slopes[head[h]] : 0.f;
   }
   float o[kDP / 8][4];
-#pragma unroll
-  for (int i = 0; i < kDP / 8; ++i)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
 
   // 16-byte copies: fp32, and every row of the tensor on a 16-byte boundary.
   auto aligned = [&](const void *x, uint64_t row_stride, uint64_t head_stride) {
@@ -159,182 +158,233 @@ __global__ void __launch_bounds__(kThreads, kDP <= 64 ? 4 : 1)
       return (long long)((size_t)(u.s.q_row + u.t0 + r / pack) * p.q_row +
                          (size_t)(u.head0 + r % pack) * p.q_head);
     });
-  for (int i = first; i < u.last; i = next_tile(u, marks, i + 1)) {
-    const int tile0 = key_tile(u, i) * kKeys;
-    for (int k0 = tile0; k0 < min(tile0 + kKeys, u.s.nk); k0 += kStep) {
-      const int live = min(kStep, u.s.nk - k0);
-      __syncthreads();  // the previous step's rows have been read
-      const size_t kr = (size_t)(u.s.k_row + k0);
-      stage<kDP, C::kQP>(p, ks, p.k, vk, [&](int r) -> long long {
-        return r < live ? (long long)((kr + r) * p.k_row + (size_t)u.kv * p.k_head) : -1;
-      });
-      stage<kDP, C::kVP>(p, vs, p.v, vv, [&](int r) -> long long {
-        return r < live ? (long long)((kr + r) * p.v_row + (size_t)u.kv * p.v_head) : -1;
-      });
-      if (docs)
-        for (int j = threadIdx.x; j < kStep; j += kThreads)
-          doc_s[j] = j < live ? p.k_docs[kr + j] : -1;
-      copies_done();
-      // Whether a value is not finite: each thread looks over the ones that it copied.
-      float taint = 0.f;  // x * 0 is NaN exactly where x is not finite, and then the sum stays NaN
-      if (vv) {
+
+  // Values that are not finite.  A key closed to a row has p = 0 there, and the product would turn
+  // 0 * Inf or 0 * NaN into NaN; and the parts of an infinite operand make NaN where the whole need
+  // not.  So a CTA whose sums come out not finite (rare) walks its keys once more, carefully: with
+  // NaN scores taken again whole, and with the value rows that hold such a value added by hand where
+  // p > 0 and zeroed before the product.
+  auto walk = [&](auto how) {
+    constexpr bool careful = decltype(how)::value;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) m[h] = -INFINITY, l[h] = 0.f;
+#pragma unroll
+    for (int i = 0; i < kDP / 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+    for (int i = first; i < u.last; i = next_tile(u, marks, i + 1)) {
+      const int tile0 = key_tile(u, i) * kKeys;
+      for (int k0 = tile0; k0 < min(tile0 + kKeys, u.s.nk); k0 += kStep) {
+        const int live = min(kStep, u.s.nk - k0);
+        __syncthreads();  // the previous step's rows have been read
+        const size_t kr = (size_t)(u.s.k_row + k0);
+        stage<kDP, C::kQP>(p, ks, p.k, vk, [&](int r) -> long long {
+          return r < live ? (long long)((kr + r) * p.k_row + (size_t)u.kv * p.k_head) : -1;
+        });
+        stage<kDP, C::kVP>(p, vs, p.v, vv, [&](int r) -> long long {
+          return r < live ? (long long)((kr + r) * p.v_row + (size_t)u.kv * p.v_head) : -1;
+        });
+        if (docs)
+          for (int j = threadIdx.x; j < kStep; j += kThreads)
+            doc_s[j] = j < live ? p.k_docs[kr + j] : -1;
+        copies_done();
+        bool any_odd = false;
+        if constexpr (careful) {
+          // Whether a value is not finite, or as good as that to the split below (2^127 or more):
+          // each thread looks over the ones that it copied.  x * 2 * 0 is NaN exactly there, and
+          // then the sum stays NaN.
+          float taint = 0.f;
+          auto look = [&](float x) { taint = fmaf(x * 2.f, 0.f, taint); };
+          if (vv) {
 #pragma unroll 4
-        for (int x = threadIdx.x; x < kStep * (kDP / 4); x += kThreads) {
-          const float4 v = *reinterpret_cast<const float4 *>(vs + x / (kDP / 4) * C::kVP + x % (kDP / 4) * 4);
-          taint = fmaf(v.x, 0.f, fmaf(v.y, 0.f, fmaf(v.z, 0.f, fmaf(v.w, 0.f, taint))));
-        }
-      } else {
+            for (int x = threadIdx.x; x < kStep * (kDP / 4); x += kThreads) {
+              const float4 v = *reinterpret_cast<const float4 *>(vs + x / (kDP / 4) * C::kVP +
+                                                                 x % (kDP / 4) * 4);
+              look(v.x), look(v.y), look(v.z), look(v.w);
+            }
+          } else {
 #pragma unroll 4
-        for (int x = threadIdx.x; x < kStep * kDP; x += kThreads)
-          taint = fmaf(vs[x / kDP * C::kVP + x % kDP], 0.f, taint);
-      }
-      const bool any_odd = __syncthreads_or(taint != 0.f);
-      if (!busy && !any_odd) continue;  // the hand sums below keep the CTA in step
-
-      // S = Q K^T
-      float s[kStep / 8][4];
-#pragma unroll
-      for (int n = 0; n < kStep / 8; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
-#pragma unroll 2
-      for (int kk = 0; kk < kDP / 8; ++kk) {
-        uint32_t ah[4], al[4];
-        const float2 q0 = *reinterpret_cast<const float2 *>(qs + (warp * 16 + g) * C::kQP + kk * 8 + 2 * t);
-        const float2 q1 = *reinterpret_cast<const float2 *>(qs + (warp * 16 + g + 8) * C::kQP + kk * 8 + 2 * t);
-        split(q0.x, ah[0], al[0]);
-        split(q1.x, ah[1], al[1]);
-        split(q0.y, ah[2], al[2]);
-        split(q1.y, ah[3], al[3]);
-#pragma unroll
-        for (int n = 0; n < kStep / 8; ++n) {
-          if (n * 8 >= live) break;
-          const float2 b = *reinterpret_cast<const float2 *>(ks + (n * 8 + g) * C::kQP + kk * 8 + 2 * t);
-          uint32_t bh0, bl0, bh1, bl1;
-          split(b.x, bh0, bl0);
-          split(b.y, bh1, bl1);
-          mma_split(s[n], ah, al, bh0, bl0, bh1, bl1);
+            for (int x = threadIdx.x; x < kStep * kDP; x += kThreads)
+              look(vs[x / kDP * C::kVP + x % kDP]);
+          }
+          any_odd = __syncthreads_or(taint != 0.f);
+        } else {
+          __syncthreads();
         }
-      }
+        if (!busy && !any_odd) continue;  // the hand sums below keep the CTA in step
 
-      // Scores, masked; then the running maximum and the probabilities.  One branch per part of the
-      // rule around the loop over the scores.  The step to log2 units comes behind the subtraction
-      // of the reference: a large score times log2 e would be rounded before it.
-      auto each = [&](auto change) {
-#pragma unroll
-        for (int n = 0; n < kStep / 8; ++n) {
-          if (n * 8 >= live) break;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[n][e] = change(s[n][e], e >> 1, n * 8 + 2 * t + (e & 1));
-        }
-      };
-      if (p.softcap > 0.f) {
-        each([&](float z, int, int) { return p.softcap * tanhf(z * p.scale / p.softcap); });
-      } else {
-        each([&](float z, int, int) { return z * p.scale; });
-      }
-      if (p.slopes)
-        each([&](float z, int h, int j) {
-          return fmaf(-slope[h], fabsf((float)(k0 + j - row[h].pos)), z);
-        });
-      if (p.table)
-        each([&](float z, int h, int j) {
-          return z + __ldg(table[h] + min(max(k0 + j - row[h].pos, -p.reach), p.reach));
-        });
-      const int end = k0 + kStep;
-      if (!(end <= u.whole_prefix || (k0 >= u.whole_lo && end <= u.whole_hi)))
-        each([&](float z, int h, int jj) {
-          const Row &w = row[h];
-          const int j = k0 + jj;
-          bool open = j < w.prefix || (j >= w.lo && j < w.hi);
-          if (docs) open = open && doc_s[jj] == w.doc;
-          return open ? z : -INFINITY;
-        });
-      float top[2] = {-INFINITY, -INFINITY};
-      each([&](float z, int h, int) {
-        top[h] = fmaxf(top[h], z);
-        return z;
-      });
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
-      }
-      float ref[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float now = fmaxf(m[h], top[h]);
-        ref[h] = now == -INFINITY ? 0.f : now;
-        const float f = m[h] == -INFINITY ? 0.f : exp2f((m[h] - now) * kLog2e);
-        m[h] = now;
-        l[h] *= f;
-#pragma unroll
-        for (int n = 0; n < kDP / 8; ++n) {
-          o[n][2 * h] *= f;
-          o[n][2 * h + 1] *= f;
-        }
-      }
-      each([&](float z, int h, int) {
-        const float pj = ex2((z - ref[h]) * kLog2e);  // 0 below 2^-126: nothing beside the row's largest, 1
-        l[h] += pj;
-        return pj;
-      });
-
-      if (any_odd) {
-        // A value of v in this step is not finite: its key counts for the rows that see it and
-        // for no other, and zero times it would not be zero.  Such keys (rare) are added by
-        // hand where p > 0 and taken out of the product.
-        __syncthreads();  // the K rows are free: P goes there
-        constexpr int kPP = kStep + 1;
+        // S = Q K^T
+        float s[kStep / 8][4];
 #pragma unroll
         for (int n = 0; n < kStep / 8; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            ks[(warp * 16 + g + 8 * (e >> 1)) * kPP + n * 8 + 2 * t + (e & 1)] = s[n][e];
-        __syncwarp();
-        uint32_t bad[kStep / 32];
-        for (int x = 0; x < kStep / 32; ++x) {
-          bool not_finite = false;
-          for (int c = 0; c < kDP; ++c) not_finite |= !(fabsf(vs[(x * 32 + lane) * C::kVP + c]) < INFINITY);
-          bad[x] = __ballot_sync(0xffffffffu, not_finite);
-        }
-        for (int jj = 0; jj < kStep; ++jj) {
-          if (!((bad[jj >> 5] >> (jj & 31)) & 1)) continue;
+          for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+#pragma unroll 2
+        for (int kk = 0; kk < kDP / 8; ++kk) {
+          uint32_t ah[4], al[4];
+          const float *qr = qs + (warp * 16 + g) * C::kQP + kk * 8 + 2 * t;
+          const float2 q0 = *reinterpret_cast<const float2 *>(qr);
+          const float2 q1 = *reinterpret_cast<const float2 *>(qr + 8 * C::kQP);
+          split(q0.x, ah[0], al[0]);
+          split(q1.x, ah[1], al[1]);
+          split(q0.y, ah[2], al[2]);
+          split(q1.y, ah[3], al[3]);
 #pragma unroll
-          for (int n = 0; n < kDP / 8; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float pj = ks[(warp * 16 + g + 8 * (e >> 1)) * kPP + jj];
-              if (!(pj == 0.f)) o[n][e] = fmaf(pj, vs[jj * C::kVP + n * 8 + 2 * t + (e & 1)], o[n][e]);
-            }
+          for (int n = 0; n < kStep / 8; ++n) {
+            if (n * 8 >= live) break;
+            const float2 b =
+                *reinterpret_cast<const float2 *>(ks + (n * 8 + g) * C::kQP + kk * 8 + 2 * t);
+            uint32_t bh0, bl0, bh1, bl1;
+            split(b.x, bh0, bl0);
+            split(b.y, bh1, bl1);
+            mma_split(s[n], ah, al, bh0, bl0, bh1, bl1);
+          }
         }
-        __syncthreads();  // every warp has read the rows
-        for (int jj = warp; jj < kStep; jj += kThreads / 32)
-          if ((bad[jj >> 5] >> (jj & 31)) & 1)
-            for (int c = lane; c < kDP; c += 32) vs[jj * C::kVP + c] = 0.f;
-        __syncthreads();
-      }
 
-      // O += P V
+        if constexpr (careful) {
+          // An infinite q or k, or one whose upper part rounds up to infinity, makes NaN of its
+          // products' parts where the product itself need not be NaN: such scores are taken whole.
 #pragma unroll
-      for (int kk = 0; kk < kStep / 8; ++kk) {
-        if (kk * 8 >= live) break;
-        uint32_t ah[4], al[4];
-        split(s[kk][0], ah[0], al[0]);
-        split(s[kk][2], ah[1], al[1]);
-        split(s[kk][1], ah[2], al[2]);
-        split(s[kk][3], ah[3], al[3]);
+          for (int n = 0; n < kStep / 8; ++n)
 #pragma unroll
-        for (int n = 0; n < kDP / 8; ++n) {
-          const float *v0 = vs + (kk * 8 + 2 * t) * C::kVP + n * 8 + g;
-          uint32_t bh0, bl0, bh1, bl1;
-          split(v0[0], bh0, bl0);
-          split(v0[C::kVP], bh1, bl1);
-          mma_split(o[n], ah, al, bh0, bl0, bh1, bl1);
+            for (int e = 0; e < 4; ++e)
+              if (s[n][e] != s[n][e]) {
+                const float *a = qs + (warp * 16 + g + 8 * (e >> 1)) * C::kQP;
+                const float *b = ks + (n * 8 + 2 * t + (e & 1)) * C::kQP;
+                s[n][e] = 0.f;
+#pragma unroll 1
+                for (int c = 0; c < kDP; ++c) s[n][e] = fmaf(a[c], b[c], s[n][e]);
+              }
+        }
+
+        // Scores, masked; then the running maximum and the probabilities.  One branch per part of the
+        // rule around the loop over the scores.  The step to log2 units comes behind the subtraction
+        // of the reference: a large score times log2 e would be rounded before it.
+        auto each = [&](auto change) {
+#pragma unroll
+          for (int n = 0; n < kStep / 8; ++n) {
+            if (n * 8 >= live) break;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[n][e] = change(s[n][e], e >> 1, n * 8 + 2 * t + (e & 1));
+          }
+        };
+        if (p.softcap > 0.f) {
+          each([&](float z, int, int) { return p.softcap * tanhf(z * p.scale / p.softcap); });
+        } else {
+          each([&](float z, int, int) { return z * p.scale; });
+        }
+        if (p.slopes)
+          each([&](float z, int h, int j) {
+            return fmaf(-slope[h], fabsf((float)(k0 + j - row[h].pos)), z);
+          });
+        if (p.table)
+          each([&](float z, int h, int j) {
+            return z + __ldg(table[h] + min(max(k0 + j - row[h].pos, -p.reach), p.reach));
+          });
+        const int end = k0 + kStep;
+        if (!(end <= u.whole_prefix || (k0 >= u.whole_lo && end <= u.whole_hi)))
+          each([&](float z, int h, int jj) {
+            const Row &w = row[h];
+            const int j = k0 + jj;
+            bool open = j < w.prefix || (j >= w.lo && j < w.hi);
+            if (docs) open = open && doc_s[jj] == w.doc;
+            return open ? z : -INFINITY;
+          });
+        float top[2] = {-INFINITY, -INFINITY};
+        each([&](float z, int h, int) {
+          top[h] = fmaxf(top[h], z);
+          return z;
+        });
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+          top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+        }
+        float ref[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float now = fmaxf(m[h], top[h]);
+          ref[h] = now == -INFINITY ? 0.f : now;
+          const float f = m[h] == -INFINITY ? 0.f : exp2f((m[h] - now) * kLog2e);
+          m[h] = now;
+          l[h] *= f;
+#pragma unroll
+          for (int n = 0; n < kDP / 8; ++n) {
+            o[n][2 * h] *= f;
+            o[n][2 * h + 1] *= f;
+          }
+        }
+        each([&](float z, int h, int) {
+          const float pj = ex2((z - ref[h]) * kLog2e);  // 0 below 2^-126: nothing beside the row's largest, 1
+          l[h] += pj;
+          return pj;
+        });
+
+        if (careful && any_odd) {
+          // A value of v in this step is not finite (or near that): its key counts for the rows that
+          // see it and for no other, and zero times it would not be zero.  Such keys (rare) are added by
+          // hand where p > 0 and taken out of the product.
+          __syncthreads();  // the K rows are free: P goes there
+          constexpr int kPP = kStep + 1;
+#pragma unroll
+          for (int n = 0; n < kStep / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              ks[(warp * 16 + g + 8 * (e >> 1)) * kPP + n * 8 + 2 * t + (e & 1)] = s[n][e];
+          __syncwarp();
+          uint32_t bad[kStep / 32];
+          for (int x = 0; x < kStep / 32; ++x) {
+            bool odd = false;
+            for (int c = 0; c < kDP; ++c) odd |= !(fabsf(vs[(x * 32 + lane) * C::kVP + c]) < kOdd);
+            bad[x] = __ballot_sync(0xffffffffu, odd);
+          }
+          for (int jj = 0; jj < kStep; ++jj) {
+            if (!((bad[jj >> 5] >> (jj & 31)) & 1)) continue;
+#pragma unroll
+            for (int n = 0; n < kDP / 8; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float pj = ks[(warp * 16 + g + 8 * (e >> 1)) * kPP + jj];
+                if (!(pj == 0.f)) o[n][e] = fmaf(pj, vs[jj * C::kVP + n * 8 + 2 * t + (e & 1)], o[n][e]);
+              }
+          }
+          __syncthreads();  // every warp has read the rows
+          for (int jj = warp; jj < kStep; jj += kThreads / 32)
+            if ((bad[jj >> 5] >> (jj & 31)) & 1)
+              for (int c = lane; c < kDP; c += 32) vs[jj * C::kVP + c] = 0.f;
+          __syncthreads();
+        }
+
+        // O += P V
+#pragma unroll
+        for (int kk = 0; kk < kStep / 8; ++kk) {
+          if (kk * 8 >= live) break;
+          uint32_t ah[4], al[4];
+          split(s[kk][0], ah[0], al[0]);
+          split(s[kk][2], ah[1], al[1]);
+          split(s[kk][1], ah[2], al[2]);
+          split(s[kk][3], ah[3], al[3]);
+#pragma unroll
+          for (int n = 0; n < kDP / 8; ++n) {
+            const float *v0 = vs + (kk * 8 + 2 * t) * C::kVP + n * 8 + g;
+            uint32_t bh0, bl0, bh1, bl1;
+            split(v0[0], bh0, bl0);
+            split(v0[C::kVP], bh1, bl1);
+            mma_split(o[n], ah, al, bh0, bl0, bh1, bl1);
+          }
         }
       }
     }
-  }
+  };
+  walk(std::false_type());
+  float taint = 0.f;  // NaN where a sum is not finite
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    if ((warp * 16 + g + 8 * h) / pack < u.tokens)
+#pragma unroll
+      for (int n = 0; n < kDP / 8; ++n)
+        taint = fmaf(o[n][2 * h], 0.f, fmaf(o[n][2 * h + 1], 0.f, taint));
+  if (__syncthreads_or(taint != 0.f)) walk(std::true_type());
 
 #pragma unroll
   for (int h = 0; h < 2; ++h) {

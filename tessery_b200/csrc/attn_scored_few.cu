@@ -107,8 +107,10 @@ __device__ __forceinline__ float rcp(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Whether a word of values is safe in the products: finite, and in fp32 below 2^127, so that the upper
+// part of the split is finite too.
 __device__ __forceinline__ bool finite_word(uint32_t w, bool f32) {
-  if (f32) return (w & 0x7f800000u) != 0x7f800000u;
+  if (f32) return (w & 0x7fffffffu) < 0x7f000000u;
   return (w & 0x7f80u) != 0x7f80u && (w & 0x7f800000u) != 0x7f800000u;
 }
 
@@ -213,8 +215,9 @@ __global__ void __launch_bounds__(Cfg<T, kDP>::kThreads, Cfg<T, kDP>::kResident)
   // Values that are not finite.  A key closed to a row has p = 0 there, and the product would turn
   // 0 * Inf or 0 * NaN into NaN; and a part of an operand times Inf need not be what the whole gives
   // (a lo part is 0 or below it as often as above).  So a warp whose sums come out not finite (rare)
-  // walks its keys once more, carefully: with weights of at most 1, and with the value rows that
-  // hold such a value added by hand where p > 0 and zeroed before the product.  (The careful part
+  // walks its keys once more, carefully: with weights of at most 1, with NaN scores taken again
+  // whole (fp32), and with the value rows that hold such a value added by hand where p > 0 and
+  // zeroed before the product.  (The careful part
   // kept out of the first walk: 32 texts of 1024 keys, 12 heads of 64, take 37.0 us in bf16 either
   // way, 11 texts in fp32 208 against 251 us with values looked over in every block with a
   // closed key.)
@@ -271,6 +274,25 @@ __global__ void __launch_bounds__(Cfg<T, kDP>::kThreads, Cfg<T, kDP>::kResident)
               mma_bf16(s[n], qw, ptx::u4_at(kw[n], 2 * j), ptx::u4_at(kw[n], 2 * j + 1));
           }
         }
+      }
+
+      if constexpr (careful && C::kF32) {
+        // An infinite q or k, or one whose upper part rounds up to infinity, makes NaN of its
+        // products' parts where the product itself need not be NaN: such scores are taken whole.
+        const uint8_t *kb = smem + (ks - ptx::smem_addr(smem));
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (s[n][e] != s[n][e]) {
+              const int key = 8 * n + 2 * t + (e & 1);
+              const T *a = qs + (g + 8 * (e >> 1)) * C::kQP;
+              s[n][e] = 0.f;
+#pragma unroll 1
+              for (int c = 0; c < kDP; ++c)
+                s[n][e] = fmaf(a[c], reinterpret_cast<const float *>(kb + C::k_at(key, c / 4))[c % 4],
+                               s[n][e]);
+            }
       }
 
       // Scores, masked.  The step to log2 units comes behind the subtraction of the reference: a

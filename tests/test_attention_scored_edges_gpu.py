@@ -137,3 +137,39 @@ def test_infinite_values_that_a_row_sees(runtime, kernel, dtype, nq, heads, kv_h
     check(runtime, q, k, v, dtype, route=kernel, causal=False)
     check(runtime, q, k, v, dtype, route=kernel)
     check(runtime, q, k, v, dtype, route=kernel, window=(200, -1), prefix=30)
+
+
+@pytest.mark.parametrize("kernel,dtype,nq,heads,kv_heads,dim", ROUTES)
+def test_infinite_scores(runtime, kernel, dtype, nq, heads, kv_heads, dim):
+    """A score of -inf weighs nothing and leaves its row as it is; one of +inf makes the row NaN; a cap
+    makes both finite."""
+    q, k, v = normal(4, nq, 200, heads, kv_heads, dim)
+    q[..., 3] = np.abs(q[..., 3]) + 0.5
+    k[17, :, 3] = -np.inf
+    check(runtime, q, k, v, dtype, route=kernel, causal=False)
+    q[2, :, 3] *= -1  # this row's score is +inf
+    check(runtime, q, k, v, dtype, route=kernel, causal=False)
+    check(runtime, q, k, v, dtype, causal=False, softcap=4.0)
+    k[17] = 0.0
+    k[17, :, 3] = 1.0
+    k[..., 5] = np.abs(k[..., 5]) + 0.5
+    q[..., 5] = 0.25
+    q[3, :, 5], q[4, :, 5] = -np.inf, np.inf  # every score of these rows
+    got = check(runtime, q, k, v, dtype, route=kernel, causal=False)
+    assert not got[3].any() and np.isnan(got[4]).all()
+    check(runtime, q, k, v, dtype, causal=False, softcap=4.0)
+
+
+@pytest.mark.parametrize("kernel,nq,dim", [("scored_f32", 40, 64), ("scored_few", 6, 64),
+                                           ("scored_few", 6, 160)])
+def test_largest_finite_values(runtime, kernel, nq, dim):
+    """fp32 values whose upper TF32 part would be infinite."""
+    big = np.finfo(np.float32).max
+    q, k, v = normal(5, nq, 100, 2, 1, dim)
+    q[..., 1] = 2.0**-126
+    k[::7, :, 1] = big
+    k[3::7, :, 1] = -big
+    v[:, :, 0] = np.abs(v[:, :, 0])
+    v[11, :, 0], v[50, :, 3] = big, -big
+    check(runtime, q, k, v, "f32", route=kernel, causal=False)
+    check(runtime, q, k, v, "f32", route=kernel, causal=False, softcap=10.0)
