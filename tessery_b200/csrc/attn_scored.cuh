@@ -10,6 +10,7 @@
 
 #include "common.cuh"
 #include "kernels.h"
+#include "tcgen05.cuh"
 
 namespace tx {
 namespace scored {
@@ -225,6 +226,40 @@ __device__ __forceinline__ Row make_row(const ScoredProblem &p, const Unit &u, i
   if (p.q_docs && live) r.doc = p.q_docs[u.s.q_row + u.t0 + token];
   if (!live || (p.q_docs && r.doc < 0)) r.lo = r.hi = r.prefix = 0;
   return r;
+}
+
+// c tanh(z / c) for a cap c.  For arguments u = z / c up to kCapFit by a fit of degree 4 to tanh(u) / u
+// in u^2 (weighted least squares refined to equal ripples, relative error 6e-7), beyond as
+// 1 - 2 / (1 + e^(2u)) by hardware, 2^-21 of the cap: either is off relative to the result, whatever
+// the cap (the second form alone is off by 1.2e-3 for scores below 8 under a cap of 1e4).
+constexpr float kCapFit = 0.75f;
+struct CapPoly {  // a tanh(u) / u with u^2 = q w
+  float a0, a1, a2, a3, a4;
+  __device__ __forceinline__ void set(float a, float q) {
+    a0 = a * 0.999999435f;
+    a1 = a * -0.333282516f * q;
+    a2 = a * 0.132589833f * q * q;
+    a3 = a * -0.0500563042f * q * q * q;
+    a4 = a * 0.0129296325f * q * q * q * q;
+  }
+  __device__ __forceinline__ float operator()(float w) const {
+    return fmaf(fmaf(fmaf(fmaf(a4, w, a3), w, a2), w, a1), w, a0);
+  }
+};
+__device__ __forceinline__ float cap_exact(float u, float c) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + ptx::ex2(u * (2.f * 1.44269504088896341f))));
+  return fmaf(-2.f * c, r, c);
+}
+__device__ __forceinline__ float cap_scaled(float z, float u, float c) {
+  CapPoly fit;
+  fit.set(1.f, 1.f);
+  return fabsf(u) <= kCapFit ? z * fit(u * u) : cap_exact(u, c);
+}
+// The factor from x to u where z = scale x; finite, so that a score of zero stays zero under the
+// smallest of caps.
+__device__ __forceinline__ float cap_factor(float scale, float c) {
+  return c > 0.f ? fminf(scale / c, 3.402823466e38f) : 0.f;
 }
 
 // Zeros for the query rows of a padded layout past the sequence's length.

@@ -102,11 +102,6 @@ __device__ __forceinline__ void mma_split(float (&c)[4], const uint32_t (&ah)[4]
 #pragma unroll
   for (int e = 0; e < 4; ++e) c[e] += sum[e];
 }
-__device__ __forceinline__ float rcp(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // Whether a word of values is safe in the products: finite, and in fp32 below 2^127, so that the upper
 // part of the split is finite too.
 __device__ __forceinline__ bool finite_word(uint32_t w, bool f32) {
@@ -209,7 +204,9 @@ __global__ void __launch_bounds__(Cfg<T, kDP>::kThreads, Cfg<T, kDP>::kResident)
     table[h] = p.table ? p.table + (size_t)head * (2 * p.reach + 1) + p.reach : nullptr;
     slope[h] = p.slopes ? p.slopes[head] : 0.f;
   }
-  const float cap_a = p.softcap > 0.f ? 2.f * kLog2e / p.softcap : 0.f;
+  const float cap_u = cap_factor(1.f, p.softcap);
+  CapPoly cap_fit;
+  cap_fit.set(1.f, 1.f);
   float o[kDP / 8][4];
 
   // Values that are not finite.  A key closed to a row has p = 0 there, and the product would turn
@@ -297,6 +294,32 @@ __global__ void __launch_bounds__(Cfg<T, kDP>::kThreads, Cfg<T, kDP>::kResident)
 
       // Scores, masked.  The step to log2 units comes behind the subtraction of the reference: a
       // large score times log2 e would be rounded before it.
+      if constexpr (!C::kF32) {
+        if (p.softcap > 0.f) {  // fp32: tanhf below
+          float most = 0.f;
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              s[n][e] *= p.scale;
+              most = fmaxf(most, fabsf(s[n][e]));
+            }
+          if (__any_sync(0xffffffffu, most * cap_u > kCapFit)) {
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[n][e] = cap_scaled(s[n][e], s[n][e] * cap_u, p.softcap);
+          } else {
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float x = s[n][e] * cap_u;
+                s[n][e] *= cap_fit(x * x);
+              }
+          }
+        }
+      }
       float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
       for (int n = 0; n < 2; ++n)
@@ -304,13 +327,8 @@ __global__ void __launch_bounds__(Cfg<T, kDP>::kThreads, Cfg<T, kDP>::kResident)
         for (int e = 0; e < 4; ++e) {
           const int h = e >> 1, j = k0 + 8 * n + 2 * t + (e & 1);
           const Row &w = row[h];
-          float z = s[n][e] * p.scale;
-          if (p.softcap > 0.f) {
-            if constexpr (C::kF32)
-              z = p.softcap * tanhf(z / p.softcap);
-            else  // 1 - 2 / (1 + e^(2u)) by hardware: 2^-21 of the cap
-              z = fmaf(-2.f * p.softcap, rcp(1.f + ex2(z * cap_a)), p.softcap);
-          }
+          float z = !C::kF32 && p.softcap > 0.f ? s[n][e] : s[n][e] * p.scale;
+          if (C::kF32 && p.softcap > 0.f) z = p.softcap * tanhf(z / p.softcap);
           if (p.slopes) z = fmaf(-slope[h], fabsf((float)(j - w.pos)), z);
           if (p.table) z += __ldg(table[h] + min(max(j - w.pos, -p.reach), p.reach));
           bool open = j < w.prefix || (j >= w.lo && j < w.hi);

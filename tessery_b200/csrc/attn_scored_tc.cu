@@ -121,12 +121,6 @@ struct Gate {  // a bounded wait that gives up once for the whole CTA
   }
 };
 
-__device__ __forceinline__ float rcp(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // A distance bias in log2 units.  A finite bias too large for them stays finite: only -inf closes a
 // key.
 __device__ __forceinline__ float bias_log2(float b) {
@@ -385,22 +379,15 @@ __global__ void __launch_bounds__(kThreads, 2)
       const bool busy = __any_sync(0xffffffffu, live);  // rows past the last token need nothing
       const Row row = make_row(p, u, token, live);
       const float scale2 = p.scale * kLog2e;
-      // cap: c tanh(x scale / c) in log2 units = x (a0 + a1 x^2 + ... + a4 x^8) for arguments up to
-      // 3/4: a fit of degree 4 to tanh(u) / u in u^2 (weighted least squares refined to equal
-      // ripples, relative error 6e-7), which costs no special function.
-      const float cap_u = kCap ? p.scale / p.softcap : 0.f, cap2 = kCap ? p.softcap * kLog2e : 0.f;
-      const float cap_q = cap_u * cap_u;
-      const float a0 = scale2 * 0.999999435f, a1 = scale2 * -0.333282516f * cap_q,
-                  a2 = scale2 * 0.132589833f * cap_q * cap_q,
-                  a3 = scale2 * -0.0500563042f * cap_q * cap_q * cap_q,
-                  a4 = scale2 * 0.0129296325f * cap_q * cap_q * cap_q * cap_q;
-      auto cap_fit = [&](float x) {  // the factor of x
-        const float w = x * x;
-        return fmaf(fmaf(fmaf(fmaf(a4, w, a3), w, a2), w, a1), w, a0);
-      };
-      auto cap_exact = [&](float x) {  // tanh(u) = 1 - 2 / (1 + e^(2u))
-        return fmaf(-2.f * cap2, rcp(1.f + ex2(x * (2.f * kLog2e) * cap_u)), cap2);
-      };
+      // cap: c tanh(u) in log2 units, u = x cap_u.  Scores up to cap_near: x times a polynomial in x^2 (6
+      // instructions, no special function), where its coefficients keep inside of fp32's range.
+      // Beyond, for a cap up to 512, the hardware's form for the whole chunk: 2^-21 of the cap is
+      // 2^-12 at most, beside P's 2^-9.  A larger cap takes each score by its own size.
+      const float cap_u = kCap ? cap_factor(p.scale, p.softcap) : 0.f;
+      const float cap2 = kCap ? p.softcap * kLog2e : 0.f;
+      const float cap_near = cap_u > 5e-5f && cap_u < 3e4f ? kCapFit / cap_u : -1.f;
+      CapPoly cap_x;
+      if (kCap) cap_x.set(scale2, cap_u * cap_u);
       const float slope2 = kBias == kSlopes ? -p.slopes[head] * kLog2e : 0.f;
       // Whether the whole table lies in shared memory, and at which pitch.
       const uint32_t table_pitch = bias_pitch(2 * ((uint32_t)p.reach + kKeys) + 1, p.pack);
@@ -487,15 +474,21 @@ __global__ void __launch_bounds__(kThreads, 2)
               for (int t = 0; t < 32; t += 2)
                 far = fmaxf(fmaxf(far, fabsf(__uint_as_float(s[t]))),
                             fabsf(__uint_as_float(s[t + 1])));
-              if (__any_sync(0xffffffffu, far * cap_u > 0.75f)) {
+              if (!__any_sync(0xffffffffu, far > cap_near)) {
+#pragma unroll
+                for (int t = 0; t < 32; ++t) {
+                  const float x = __uint_as_float(s[t]);
+                  s[t] = __float_as_uint(x * cap_x(x * x));
+                }
+              } else if (p.softcap <= 512.f) {
 #pragma unroll
                 for (int t = 0; t < 32; ++t)
-                  s[t] = __float_as_uint(cap_exact(__uint_as_float(s[t])));
+                  s[t] = __float_as_uint(cap_exact(__uint_as_float(s[t]) * cap_u, cap2));
               } else {
 #pragma unroll
                 for (int t = 0; t < 32; ++t) {
                   const float x = __uint_as_float(s[t]);
-                  s[t] = __float_as_uint(x * cap_fit(x));
+                  s[t] = __float_as_uint(cap_scaled(x * scale2, x * cap_u, cap2));
                 }
               }
             }

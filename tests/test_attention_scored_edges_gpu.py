@@ -173,3 +173,18 @@ def test_largest_finite_values(runtime, kernel, nq, dim):
     v[11, :, 0], v[50, :, 3] = big, -big
     check(runtime, q, k, v, "f32", route=kernel, causal=False)
     check(runtime, q, k, v, "f32", route=kernel, causal=False, softcap=10.0)
+
+
+@pytest.mark.parametrize("kernel,dtype,nq,heads,kv_heads,dim", ROUTES)
+@pytest.mark.parametrize("cap", [1e-9, 1e-3, 0.5, 30.0, 1e4, 1e6, 1e30])
+def test_caps_of_any_size(runtime, kernel, dtype, nq, heads, kv_heads, dim, cap):
+    """A capped score is off relative to itself, not to the cap; rows whose scores reach the cap do not
+    touch the others."""
+    q, k, v = normal(6, nq, 150, heads, kv_heads, dim)
+    q[1] = 0.0
+    q[2] *= 3.0
+    check(runtime, q, k, v, dtype, causal=False, softcap=cap)
+    if 1 < cap < 1e10:
+        q[3] *= cap  # scores that reach the cap, in the same warps
+        check(runtime, q, k, v, dtype, causal=False, softcap=cap)
+    check(runtime, 0 * q, k, v, dtype, causal=False, softcap=cap)
