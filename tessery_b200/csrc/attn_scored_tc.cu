@@ -121,10 +121,12 @@ struct Gate {  // a bounded wait that gives up once for the whole CTA
   }
 };
 
-// A distance bias in log2 units.  A finite bias too large for them stays finite: only -inf closes a
+// A distance bias in log2 units.  A finite bias too large for them, at either end, stays finite (those
+// from 2.36e38 on are one value), and NaN and the infinities stay what they are: only -inf closes a
 // key.
 __device__ __forceinline__ float bias_log2(float b) {
-  return b == -INFINITY ? b : fmaxf(b * kLog2e, -3.402823466e38f);
+  const float most = 3.402823466e38f;
+  return fabsf(b) <= most ? fminf(fmaxf(b * kLog2e, -most), most) : b;
 }
 
 // Looks over `keys` rows of a value tile (one warp).  Returns whether any value is not finite;
@@ -388,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       const float cap_near = cap_u > 5e-5f && cap_u < 3e4f ? kCapFit / cap_u : -1.f;
       CapPoly cap_x;
       if (kCap) cap_x.set(scale2, cap_u * cap_u);
-      const float slope2 = kBias == kSlopes ? -p.slopes[head] * kLog2e : 0.f;
+      const float slope2 = kBias == kSlopes ? bias_log2(-p.slopes[head]) : 0.f;
       // Whether the whole table lies in shared memory, and at which pitch.
       const uint32_t table_pitch = bias_pitch(2 * ((uint32_t)p.reach + kKeys) + 1, p.pack);
       const bool near = kBias == kTable && p.reach <= (int)C::kBiases &&

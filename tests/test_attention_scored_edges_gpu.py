@@ -188,3 +188,21 @@ def test_caps_of_any_size(runtime, kernel, dtype, nq, heads, kv_heads, dim, cap)
         q[3] *= cap  # scores that reach the cap, in the same warps
         check(runtime, q, k, v, dtype, causal=False, softcap=cap)
     check(runtime, 0 * q, k, v, dtype, causal=False, softcap=cap)
+
+
+@pytest.mark.parametrize("kernel,dtype,nq,heads,kv_heads,dim", ROUTES)
+@pytest.mark.parametrize("reach", [3, 1500])
+def test_special_values_of_a_table(runtime, kernel, dtype, nq, heads, kv_heads, dim, reach):
+    """NaN reaches the rows that see it and no others; the largest finite value takes all the weight;
+    -inf closes a key."""
+    big = np.finfo(np.float32).max
+    q, k, v = normal(7, nq, 140, heads, kv_heads, dim)
+    for what in (np.nan, big, -big, -np.inf, np.inf):
+        t = np.zeros((heads, 2 * reach + 1), np.float32)
+        t[:, reach - 2] = what  # two keys before the query
+        check(runtime, q, k, v, dtype, distance_bias=t, causal=False)
+        t[:] = 0.0
+        t[:, 0] = what  # and everything farther to the left
+        check(runtime, q, k, v, dtype, distance_bias=t)
+    t[:] = np.linspace(-2, 2, 2 * reach + 1)
+    check(runtime, q, k, v, dtype, distance_bias=t, causal=False, softcap=5.0)
