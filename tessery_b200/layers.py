@@ -10,6 +10,7 @@ linear_fused_device.
 
 from __future__ import annotations
 
+import functools
 import math
 
 import numpy as np
@@ -36,6 +37,20 @@ def _read(rt: CudaRuntime, buffer, shape, code: int) -> NDArray:
     if out.size:
         _raise_for(rt._lib.tx_read(buffer.pointer, out.ctypes.data, out.nbytes))
     return out
+
+
+def _one_at_a_time(operator):
+    """Holds the runtime for a whole call.  The named workspaces that inputs and results go through
+    are the runtime's: between an upload and the read-back another thread's call would overwrite
+    them, or close one for a larger."""
+
+    @functools.wraps(operator)
+    def call(*args, runtime: CudaRuntime | None = None, **options):
+        rt = runtime or default_runtime()
+        with rt._lock:
+            return operator(*args, runtime=rt, **options)
+
+    return call
 
 
 def rotary_frequencies(
@@ -88,6 +103,7 @@ def rotary_frequencies(
     return freq.astype(np.float32), amplitude
 
 
+@_one_at_a_time
 def rotary(
     q: NDArray,
     k: NDArray | None = None,
@@ -162,6 +178,7 @@ def rotary(
             None if k is None else _read(rt, k_out, k.shape, out_code))
 
 
+@_one_at_a_time
 def attention_scored(
     q: NDArray,
     k: NDArray,
@@ -259,6 +276,7 @@ def attention_scored(
     return _read(rt, out, q.shape, out_code)
 
 
+@_one_at_a_time
 def linear_fused(
     x: NDArray,
     w: NDArray,
