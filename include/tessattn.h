@@ -487,7 +487,8 @@ typedef struct {
  * their own, P in two bf16 parts or fp32.  Everything else runs in fp32 accuracy.  With documents a
  * sequence has at most 2^21 keys.  A long key range is cut into parts that are joined by the last
  * to end, in a fixed order: a call's result does not change from run to run.  The parts' scratch
- * belongs to the context; a call that needs more than any before it allocates. */
+ * belongs to the context; a call that needs more than any before it allocates.  On a stream that is
+ * being captured the graph gets scratch of its own (allocation and free nodes). */
 int tx_attention_scored(void *ctx, const TxRows *qkv /* [3] */, void *out,
                         const TxLayout *layouts /* [2]: q's, then k's and v's */, uint32_t nseq,
                         uint32_t heads, uint32_t kv_heads, uint32_t dim, int in_dtype,
@@ -508,7 +509,7 @@ enum {
  * may be out (same dtype and stride).  Any m, n, k; x and w 16-byte aligned with ldx and ldw
  * multiples of 8 (columns past k may hold anything).  With few output tiles and a long k the sum is
  * cut over CTAs and joined in a fixed order in the context's scratch; a call that needs more of it
- * than any before allocates. */
+ * than any before allocates, and one on a stream that is being captured gives the graph its own. */
 int tx_linear_fused(void *ctx, const void *x, uint64_t ldx, const void *w, uint64_t ldw,
                     const float *bias, const void *residual, int residual_dtype, uint64_t ldr,
                     void *out, int out_dtype, uint64_t ldo, uint32_t m, uint32_t n, uint32_t k,

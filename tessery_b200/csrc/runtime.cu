@@ -153,8 +153,8 @@ struct Ctx {
   uint64_t units_key = 0;
   uint32_t units_count = 0;
   cudaEvent_t scratch_done = nullptr;  // last launch that read scratch
-  // split key ranges of tx_attention_scored: arrival counters (zero between calls), then the
-  // partial sums
+  // partial sums of the calls that cut a range over CTAs (tx_attention_scored its keys,
+  // tx_linear_fused its k): arrival counters (zero between calls), then the sums
   uint8_t *part_mem = nullptr;
   size_t part_bytes = 0, part_units = 0;
   std::set<Buf *> buffers;
@@ -247,6 +247,37 @@ cudaError_t ensure_parts(Ctx *c, size_t units, size_t bytes) {
   c->part_bytes = counters + bytes;
   c->part_units = need_units;
   return cudaSuccess;
+}
+
+// The counters and partial sums of one call: the context's, or, where the stream is being captured,
+// memory that the graph allocates and frees around the kernel at each launch.  (The context's would
+// be freed under the graph by a later call that needs more, and its event cannot be waited for across
+// the capture's border.)
+struct Parts {
+  uint32_t *arrived = nullptr;
+  uint8_t *sums = nullptr;
+  void *captured = nullptr;
+};
+cudaError_t parts_acquire(Ctx *c, cudaStream_t stream, size_t units, size_t bytes, Parts *p) {
+  cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+  cudaError_t e = cudaStreamIsCapturing(stream, &capturing);
+  if (e != cudaSuccess) return e;
+  if (capturing != cudaStreamCaptureStatusNone) {
+    const size_t counters = (units * 4 + 255) & ~(size_t)255;
+    if ((e = cudaMallocAsync(&p->captured, counters + bytes, stream)) != cudaSuccess) return e;
+    p->arrived = (uint32_t *)p->captured;
+    p->sums = (uint8_t *)p->captured + counters;
+    e = cudaMemsetAsync(p->captured, 0, counters, stream);
+    if (e != cudaSuccess) cudaFreeAsync(p->captured, stream);
+    return e;
+  }
+  if ((e = ensure_parts(c, units, bytes)) != cudaSuccess) return e;
+  p->arrived = (uint32_t *)c->part_mem;
+  p->sums = c->part_mem + ((c->part_units * 4 + 255) & ~(size_t)255);
+  return scratch_acquire(c, stream);
+}
+cudaError_t parts_release(Ctx *c, cudaStream_t stream, const Parts &p) {
+  return p.captured ? cudaFreeAsync(p.captured, stream) : scratch_release(c, stream);
 }
 
 uint64_t fnv1a(uint64_t h, const void *data, size_t n) {
@@ -1790,22 +1821,21 @@ int tx_attention_scored(void *ctx, const TxRows *qkv, void *out, const TxLayout 
   cudaError_t e = cudaSetDevice(c->device);
   if (e != cudaSuccess) return cuda_fail(c, e, "cudaSetDevice");
   cudaStream_t st = stream ? (cudaStream_t)stream : c->stream;
+  Parts parts;
   if (p.splits > 1) {
     const size_t rows = (size_t)units * p.splits * p.rows;
-    if ((e = ensure_parts(c, units, rows * ((size_t)p.part_dp * 4 + 8))) != cudaSuccess)
-      return cuda_fail(c, e, "partial sums allocation");
-    const size_t counters = (c->part_units * 4 + 255) & ~(size_t)255;
-    p.part_arrived = (uint32_t *)c->part_mem;
-    p.part_o = (float *)(c->part_mem + counters);
-    p.part_ml = (float2 *)(c->part_mem + counters + rows * p.part_dp * 4);
-    if ((e = scratch_acquire(c, st)) != cudaSuccess) return cuda_fail(c, e, "scratch wait");
+    if ((e = parts_acquire(c, st, units, rows * ((size_t)p.part_dp * 4 + 8), &parts)) != cudaSuccess)
+      return cuda_fail(c, e, "partial sums");
+    p.part_arrived = parts.arrived;
+    p.part_o = (float *)parts.sums;
+    p.part_ml = (float2 *)(parts.sums + rows * p.part_dp * 4);
   }
   e = route == tx::kScoredFew  ? tx::launch_scored_few(p, st)
       : route == tx::kScoredTc ? tx::launch_scored_tc(p, st)
                                : tx::launch_scored_f32(p, st);
+  const cudaError_t released = p.splits > 1 ? parts_release(c, st, parts) : cudaSuccess;
   if (e != cudaSuccess) return cuda_fail(c, e, "attention_scored launch");
-  if (p.splits > 1 && (e = scratch_release(c, st)) != cudaSuccess)
-    return cuda_fail(c, e, "scratch event");
+  if (released != cudaSuccess) return cuda_fail(c, released, "partial sums");
   c->last_kernel = route == tx::kScoredFew  ? "scored_few"
                    : route == tx::kScoredTc ? "scored_tc"
                                             : "scored_f32";
@@ -1852,17 +1882,17 @@ int tx_linear_fused(void *ctx, const void *x, uint64_t ldx, const void *w, uint6
   cudaStream_t st = stream ? (cudaStream_t)stream : c->stream;
   uint32_t tiles;
   p.splits = tx::linear_fused_splits(p, c->sms, &tiles);
+  Parts parts;
   if (p.splits > 1) {
-    if ((e = ensure_parts(c, 8 * (size_t)tiles, (size_t)tiles * p.splits * 8192 * 4)) != cudaSuccess)
-      return cuda_fail(c, e, "partial sums allocation");
-    p.arrived = (uint32_t *)c->part_mem;
-    p.part = (float *)(c->part_mem + ((c->part_units * 4 + 255) & ~(size_t)255));
-    if ((e = scratch_acquire(c, st)) != cudaSuccess) return cuda_fail(c, e, "scratch wait");
+    e = parts_acquire(c, st, 8 * (size_t)tiles, (size_t)tiles * p.splits * 8192 * 4, &parts);
+    if (e != cudaSuccess) return cuda_fail(c, e, "partial sums");
+    p.arrived = parts.arrived;
+    p.part = (float *)parts.sums;
   }
   e = tx::launch_linear_fused(p, c->sms, st);
+  const cudaError_t released = p.splits > 1 ? parts_release(c, st, parts) : cudaSuccess;
   if (e != cudaSuccess) return cuda_fail(c, e, "linear_fused launch");
-  if (p.splits > 1 && (e = scratch_release(c, st)) != cudaSuccess)
-    return cuda_fail(c, e, "scratch event");
+  if (released != cudaSuccess) return cuda_fail(c, released, "partial sums");
   c->last_kernel = "linear_fused";
   ++c->launches;
   return TX_OK;
