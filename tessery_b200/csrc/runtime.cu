@@ -1719,6 +1719,8 @@ int tx_rotary(void *ctx, const TxRotaryTensor *q, const TxRotaryTensor *k, int i
   if (!std::isfinite(amplitude) || !(eps >= 0.f) || !std::isfinite(eps))
     return fail(c, TX_EINVAL, "rotary: bad amplitude or eps");
   if (tokens > 0x7fffffffu) return fail(c, TX_EINVAL, "rotary: too many tokens");
+  if ((uintptr_t)positions % 4 || (uintptr_t)cu_seqlens % 4 || (uintptr_t)inv_freq % 4)
+    return fail(c, TX_EINVAL, "rotary: misaligned pointer");
   const size_t ei = in_dtype == TX_BF16 ? 2 : 4, eo = out_dtype == TX_BF16 ? 2 : 4;
   tx::RotaryProblem p{};
   const TxRotaryTensor *side[2] = {q, k};
@@ -1792,6 +1794,10 @@ int tx_attention_scored(void *ctx, const TxRows *qkv, void *out, const TxLayout 
   if ((uintptr_t)q->data % ei || (uintptr_t)k->data % ei || (uintptr_t)v->data % ei ||
       (uintptr_t)out % eo)
     return fail(c, TX_EINVAL, "attention_scored: misaligned pointer");
+  const void *words[] = {q_layout->cu, q_layout->lengths, k_layout->cu, k_layout->lengths, r.slopes,
+                         r.distance_bias, r.prefix, r.q_docs, r.k_docs};
+  for (const void *w : words)
+    if ((uintptr_t)w % 4) return fail(c, TX_EINVAL, "attention_scored: misaligned pointer");
   if (!nseq || !q_layout->max_len || !q_layout->rows) return TX_OK;
   tx::ScoredProblem p{};
   p.q = q->data; p.k = k->data; p.v = v->data; p.out = out;
