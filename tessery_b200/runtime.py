@@ -49,6 +49,20 @@ def _raise_for(rc: int) -> None:
     raise InferenceError()
 
 
+# The C calls take counts as 32 bits and strides as 64; ctypes would wrap what lies outside.
+_COUNT, _STRIDE, _F32_MAX = 2**31 - 1, 2**63 - 1, 3.4028234663852886e38
+
+
+def _check_counts(*counts: int) -> None:
+    if min(counts) < 0 or max(counts) > _COUNT:
+        raise InvalidInputError()
+
+
+def _check_strides(*strides: int) -> None:
+    if min(strides) < 0 or max(strides) > _STRIDE:
+        raise InvalidInputError()
+
+
 class Buffer:
     """Handle of one device allocation made by the native context (the role of
     metal.py:94-119's Buffer).  The context owns the memory and its accounting
@@ -744,11 +758,14 @@ class CudaRuntime:
         elements, contiguous [tokens, heads, dim] by default; `inv_freq` (device fp32
         [rot_dim / 2]) and `amplitude` come from layers.rotary_frequencies."""
         self._check_open()
+        rot = dim if rot_dim is None else rot_dim
+        _check_counts(tokens, heads, kv_heads, dim, rot, nseq, seq)
 
         def side(x, out, n, xs, os, weight):
             xt, xh = (n * dim, dim) if xs is None else xs
             ot, oh = (n * dim, dim) if os is None else os
-            if min(xt, xh, ot, oh, n) < 0 or not x or not out:
+            _check_strides(xt, xh, ot, oh)
+            if not x or not out:
                 raise InvalidInputError()
             return native.TX_ROTARY_TENSOR.pack(x, out, xt, xh, ot, oh, weight or 0, n)
 
@@ -756,9 +773,9 @@ class CudaRuntime:
         kt = None if k is None else side(k, k_out, kv_heads, k_strides, k_out_strides,
                                          k_norm_weight)
         _raise_for(self._lib.tx_rotary(
-            self._pointer, qt, kt, in_dtype, out_dtype, tokens, dim,
-            dim if rot_dim is None else rot_dim, 1 if interleaved else 0, 1 if inverse else 0,
-            positions, cu_seqlens, nseq, seq, inv_freq, amplitude, eps, stream))
+            self._pointer, qt, kt, in_dtype, out_dtype, tokens, dim, rot,
+            1 if interleaved else 0, 1 if inverse else 0, positions, cu_seqlens, nseq, seq, inv_freq,
+            amplitude, eps, stream))
 
     def attention_scored_device(
         self,
@@ -808,9 +825,9 @@ class CudaRuntime:
         kr, kh = (kv_heads * dim, dim) if k_strides is None else k_strides
         vr, vh = (kv_heads * dim, dim) if v_strides is None else v_strides
         left, right = window
-        if (min(nseq, rows_q, rows_k, max_q, max_k, reach, qr, qh, kr, kh, vr, vh) < 0 or dim < 1
-                or max(rows_q, rows_k, max_q, max_k, reach) > 0x7FFFFFFF
-                or max(left, right) > 0x7FFFFFFF or not (q and k and v)):
+        _check_counts(nseq, rows_q, rows_k, max_q, max_k, heads, kv_heads, dim, reach)
+        _check_strides(qr, qh, kr, kh, vr, vh)
+        if dim < 1 or max(left, right) > _COUNT or abs(softcap) > _F32_MAX or not (q and k and v):
             raise InvalidInputError()
         _raise_for(self._lib.tx_attention_scored(
             self._pointer, native.TX_ROWS.pack(q, qr, qh, k, kr, kh, v, vr, vh), out,
@@ -851,7 +868,9 @@ class CudaRuntime:
         act = native.ACTIVATIONS.get(activation)
         ldx, ldw = k if ldx is None else ldx, k if ldw is None else ldw
         ldr, ldo = n if ldr is None else ldr, n if ldo is None else ldo
-        if act is None or min(m, n, k, ldx, ldw, ldr, ldo) < 0:
+        _check_counts(m, n, k)
+        _check_strides(ldx, ldw, ldr, ldo)
+        if act is None:
             raise InvalidInputError()
         _raise_for(self._lib.tx_linear_fused(
             self._pointer, x, ldx, w, ldw, bias, residual, residual_dtype, ldr, out, out_dtype, ldo,
