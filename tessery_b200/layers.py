@@ -39,6 +39,17 @@ def _read(rt: CudaRuntime, buffer, shape, code: int) -> NDArray:
     return out
 
 
+def _int32(a) -> NDArray[np.int32]:
+    """`a` as int32, refused where that changes a value: a document id or a position that wrapped
+    would be another one."""
+    a = np.asarray(a)
+    with np.errstate(invalid="ignore"):
+        held = np.ascontiguousarray(a, dtype=np.int32)
+    if np.any(held != a):
+        raise InvalidInputError()
+    return held
+
+
 def _one_at_a_time(operator):
     """Holds the runtime for a whole call.  The named workspaces that inputs and results go through
     are the runtime's: between an upload and the read-back another thread's call would overwrite
@@ -145,21 +156,22 @@ def rotary(
     pos_ptr = cu_ptr = None
     nseq = 0
     if positions is not None:
-        pos = np.ascontiguousarray(positions, dtype=np.int32)
+        pos = _int32(positions)
         if pos.shape != (tokens,) or pos.min() < 0 or pos.max() >= 1 << 24:
             raise InvalidInputError()
         pos_ptr = _upload(rt, "rotary_pos", pos)
     elif cu_seqlens is not None:
-        cu = np.ascontiguousarray(cu_seqlens, dtype=np.int32)
+        cu = _int32(cu_seqlens)
         if cu.ndim != 1 or cu.size < 2 or cu[0] != 0 or cu[-1] != tokens or np.any(np.diff(cu) < 0):
             raise InvalidInputError()
         cu_ptr, nseq = _upload(rt, "rotary_cu", cu), cu.size - 1
     weights = []
     for name, w in (("rotary_qw", q_norm_weight), ("rotary_kw", k_norm_weight)):
         if w is not None:
-            w = np.ascontiguousarray(w, dtype=np.uint16)
-            if w.shape != (dim,):
+            w = np.asarray(w)
+            if w.shape != (dim,) or w.dtype.kind == "f":  # bit patterns, not values
                 raise InvalidInputError()
+            w = w.astype(np.uint16)
         weights.append(None if w is None else _upload(rt, name, w))
     size = 4 if out_code == native.TX_F32 else 2
     q_out = rt.workspace("rotary_q_out", q.size * size)
@@ -229,7 +241,7 @@ def attention_scored(
     def layout(side: str, x: NDArray, cu, lengths) -> int:
         """Uploads one side's layout; returns its number of sequences."""
         if packed:
-            cu = np.ascontiguousarray(cu, dtype=np.int32)
+            cu = _int32(cu)
             if (lengths is not None or cu.ndim != 1 or cu.size < 2 or cu[0] != 0
                     or cu[-1] != x.shape[0] or np.any(np.diff(cu) < 0)):
                 raise InvalidInputError()
@@ -239,7 +251,7 @@ def attention_scored(
         if cu is not None:
             raise InvalidInputError()
         if lengths is not None:
-            n = np.ascontiguousarray(lengths, dtype=np.int32)
+            n = _int32(lengths)
             if n.shape != x.shape[:1] or np.any(n < 0) or np.any(n > x.shape[1]):
                 raise InvalidInputError()
             kw[side + "_lengths"] = _upload(rt, f"scored_{side}_lengths", n) if n.size else None
@@ -253,7 +265,7 @@ def attention_scored(
         raise InvalidInputError()
     for name, docs, x in (("q_docs", q_docs, q), ("k_docs", k_docs, k)):
         if docs is not None:
-            docs = np.ascontiguousarray(docs, dtype=np.int32)
+            docs = _int32(docs)
             if docs.shape != x.shape[:-2]:
                 raise InvalidInputError()
             kw[name] = _upload(rt, "scored_" + name, docs) if docs.size else None
@@ -263,7 +275,7 @@ def attention_scored(
         if a is not None:
             kw[name] = _upload(rt, "scored_" + name, np.ascontiguousarray(a, dtype=np.float32))
     if prefix is not None:
-        kw["prefix"] = _upload(rt, "scored_prefix", np.ascontiguousarray(prefix, dtype=np.int32))
+        kw["prefix"] = _upload(rt, "scored_prefix", _int32(prefix))
     if not k.size:  # nothing to attend: every row is empty
         return np.zeros(q.shape, _NP[out_code])
     out = rt.workspace("scored_out", q.size * (4 if out_code == native.TX_F32 else 2))
