@@ -1701,6 +1701,25 @@ int tx_bert_embed(void *ctx, const uint32_t *ids, const int32_t *cu_seqlens, uin
   return TX_OK;
 }
 
+// Whether two of the heads [token, head] of `dim` elements share an element: within a token or a head
+// where its stride is below dim, otherwise where a multiple of one stride comes closer than dim to a
+// multiple of the other.
+static bool heads_overlap(uint64_t tokens, uint64_t heads, uint64_t token_stride,
+                          uint64_t head_stride, uint64_t dim) {
+  if ((heads > 1 && head_stride < dim) || (tokens > 1 && token_stride < dim)) return true;
+  if (heads < 2 || tokens < 2) return false;
+  using wide = unsigned __int128;
+  if (token_stride >= (wide)(heads - 1) * head_stride + dim) return false;  // tokens apart
+  for (uint64_t h = 1; h < heads; ++h) {
+    const wide at = (wide)h * head_stride;
+    const wide token = at / token_stride, past = at % token_stride;
+    if (token >= tokens) break;
+    if (token && past < dim) return true;
+    if (token + 1 < tokens && token_stride - past < dim) return true;
+  }
+  return false;
+}
+
 int tx_rotary(void *ctx, const TxRotaryTensor *q, const TxRotaryTensor *k, int in_dtype,
               int out_dtype, uint32_t tokens, uint32_t dim, uint32_t rot_dim, int interleaved,
               int inverse, const int32_t *positions, const int32_t *cu_seqlens, uint32_t nseq,
@@ -1735,11 +1754,12 @@ int tx_rotary(void *ctx, const TxRotaryTensor *q, const TxRotaryTensor *k, int i
     if (t->x == t->out && (in_dtype != out_dtype || t->x_token_stride != t->out_token_stride ||
                            t->x_head_stride != t->out_head_stride))
       return fail(c, TX_EINVAL, "rotary: in place needs equal dtypes and strides");
-    if ((t->heads > 1 && t->out_head_stride < dim) || (tokens > 1 && t->out_token_stride < dim))
+    if (heads_overlap(tokens, t->heads, t->out_token_stride, t->out_head_stride, dim))
       return fail(c, TX_EINVAL, "rotary: output rows overlap");
     *to[i] = {t->x, t->out, t->x_token_stride, t->x_head_stride, t->out_token_stride,
               t->out_head_stride, t->norm_w, t->heads};
   }
+  if (p.q.out == p.k.out) return fail(c, TX_EINVAL, "rotary: q and k share an output");
   p.in_dtype = in_dtype; p.out_dtype = out_dtype; p.tokens = tokens; p.dim = dim; p.rot = rot_dim;
   p.interleaved = interleaved ? 1 : 0;
   p.norm = p.q.norm_w || p.k.norm_w;
