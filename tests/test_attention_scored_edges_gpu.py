@@ -206,3 +206,25 @@ def test_special_values_of_a_table(runtime, kernel, dtype, nq, heads, kv_heads, 
         check(runtime, q, k, v, dtype, distance_bias=t)
     t[:] = np.linspace(-2, 2, 2 * reach + 1)
     check(runtime, q, k, v, dtype, distance_bias=t, causal=False, softcap=5.0)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,reach", [
+    (4, 2, 128, 700), (2, 1, 64, 1700), (4, 1, 128, 300), (4, 1, 64, 800), (8, 1, 128, 40),
+    (8, 1, 64, 900), (3, 3, 128, 1500), (1, 1, 64, 3500), (4, 1, 96, 255), (2, 1, 80, 671),
+    (2, 1, 128, 672)])
+@pytest.mark.parametrize("rule", [dict(causal=False), dict(window=(1100, 5), causal=False, prefix=9),
+                                  dict(softcap=6.0)])
+def test_tables_of_every_length(runtime, heads, kv_heads, dim, reach, rule):
+    """Tables that fit on chip whole and tables of which each warp keeps the part it needs, for packs
+    of one, two and four heads."""
+    q, k, v = normal(reach, 70, 1900, heads, kv_heads, dim)
+    t = np.random.default_rng(reach).standard_normal((heads, 2 * reach + 1)).astype(np.float32)
+    check(runtime, q, k, v, "bf16", route="scored_tc", distance_bias=t, **rule)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,rule", [
+    (1, 1, 64, {}), (8, 1, 64, {}), (4, 1, 32, {}), (2, 1, 128, dict(softcap=20.0)),
+    (8, 1, 128, dict(softcap=20.0)), (16, 1, 256, {}), (3, 1, 136, {})])
+def test_few_rows_hold_the_weights_in_two_parts(runtime, heads, kv_heads, dim, rule):
+    q, k, v = normal(8, 1, 1500, heads, kv_heads, dim)
+    check(runtime, q, k, v, "bf16", route="scored_few", **rule)
