@@ -1,4 +1,4 @@
-"""The encoder-layer operators in CUDA graphs (needs a B200).  A call that cuts its range over CTAs has
+"""The encoder-layer operators in CUDA graphs and on several streams (needs a B200).  A call that cuts its range over CTAs has
 scratch; a graph has to keep its own, whatever calls come after the capture."""
 
 import numpy as np
@@ -78,3 +78,26 @@ def test_split_calls_in_a_graph(runtime, make, small, large):
     assert np.isfinite(out.cpu().numpy()).all()
     del graph
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("make,size", [(attention, 3000), (linear, 4096)])
+def test_split_calls_on_two_streams(runtime, make, size):
+    """Calls in turn on two streams and the runtime's own share the scratch one after another."""
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    calls = [make(runtime, size + 512 * i) for i in range(3)]
+    torch.cuda.synchronize()
+    want = []
+    for call, _, out in calls:
+        call(streams[0].cuda_stream)
+        runtime.sync(streams[0].cuda_stream)
+        want.append(out.clone())
+        out.zero_()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for (call, _, _), stream in zip(calls, (*streams, None), strict=True):
+            call(stream.cuda_stream if stream else 0)
+    for s in (*(s.cuda_stream for s in streams), 0):
+        runtime.sync(s)
+    torch.cuda.synchronize()
+    for (_, _, out), w in zip(calls, want, strict=True):
+        assert torch.equal(out, w)
