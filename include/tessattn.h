@@ -481,14 +481,22 @@ typedef struct {
  * out contiguous [q rows, heads, dim].  In a padded layout the query rows past a sequence's
  * length get zeros; key and value rows past it, and those of other documents, may hold
  * anything, NaN and Inf included.  in_dtype / out_dtype TX_F32 or TX_BF16; dim <= 256; scale
- * finite.  bf16 with dim a multiple of 8 up to 128, strides multiples of 8 and 16-byte aligned
- * pointers runs on the tensor-memory kernel (P rounded to bf16).  A few query rows per kv head
- * (max_len of q times heads / kv_heads: 8, with bf16 wider than 128 or fp32 16) run in a kernel of
- * their own, P in two bf16 parts or fp32.  Everything else runs in fp32 accuracy.  With documents a
- * sequence has at most 2^21 keys.  A long key range is cut into parts that are joined by the last
- * to end, in a fixed order: a call's result does not change from run to run.  The parts' scratch
- * belongs to the context; a call that needs more than any before it allocates.  On a stream that is
- * being captured the graph gets scratch of its own (allocation and free nodes). */
+ * finite.
+ *
+ * Which kernel.  bf16 with dim a multiple of 8 up to 128, scale > 0, strides multiples of 8 and
+ * 16-byte aligned pointers: tensor memory, P rounded to bf16 (2^-9 of each weight).  Few query rows
+ * per kv head (max_len of q times heads / kv_heads), with 16-byte rows of k and v: a kernel of their
+ * own, P in two bf16 parts (2^-17) or fp32; up to 8 rows where the call could run on tensor memory
+ * and dim is at most 64 or there is a cap, up to 16 where it could not.  Everything else, bf16 wider
+ * than 128 among it, runs in fp32 accuracy, many times slower than tensor memory (8 / 4 heads of
+ * 256, causal with a cap, 4 texts of 500 to 1000 tokens: 3.2 ms).  In all three the weighted sum of v
+ * is taken before the division by the weights' sum, with weights up to 2^8: it has to stay within
+ * fp32's range.
+ *
+ * With documents a sequence has at most 2^21 keys.  A long key range is cut into parts that are
+ * joined by the last to end, in a fixed order: a call's result does not change from run to run.  The
+ * parts' scratch belongs to the context; a call that needs more than any before it allocates.  On a
+ * stream that is being captured the graph gets scratch of its own (allocation and free nodes). */
 int tx_attention_scored(void *ctx, const TxRows *qkv /* [3] */, void *out,
                         const TxLayout *layouts /* [2]: q's, then k's and v's */, uint32_t nseq,
                         uint32_t heads, uint32_t kv_heads, uint32_t dim, int in_dtype,

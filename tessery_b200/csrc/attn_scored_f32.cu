@@ -16,7 +16,8 @@
 // Bound: issue slots and latency (the operands' splits are half of the products' instructions).
 // Rows arrive by asynchronous copies, K, V and Q at once; warps without rows and blocks of 8 keys
 // past the end are skipped.  Measured: 64 texts of 16 to 128 tokens, 12 heads of 32, distance
-// slopes: 45 us (43 % of issue slots); 32 keys a step with half as many CTAs again: 46.5 us.
+// slopes: 45.6 us (44 % of issue slots); 32 keys a step with half as many CTAs again: 46.5 us against
+// 44.6 when that was measured.
 #include <cuda_runtime.h>
 
 #include <type_traits>

@@ -10,10 +10,11 @@
 // split operands (hi + lo, three products, error 2^-22).  The 64-row fp32 kernel would compute 64
 // rows for these (when this one takes which call: scored_route in attn_scored_tc.cu).
 //
-// Measured: 8 new tokens, 16 query and 8 kv heads of 128, a cap, 64 to 2048 keys each: 23 us
-// between events, of which some 6 are the launch's; 32 texts of 1024 keys, 12 heads of 64 (101 MB):
-// 39 us, 2.6 TB/s.  11 texts of 1428 to 6289 keys, 32 / 8 heads of 128 in fp32
-// (437 MB): 249 us, bound by the split operands' products.
+// Measured: 8 new tokens, 16 query and 8 kv heads of 128, a cap, 64 to 2048 keys each: 22.6 us
+// between events; in a graph, from warm caches, 6.9 us with 16 keys each, 14.4 with 256 (start-up,
+// split and join) and 24.4 with 2048.  32 texts of 1024 keys, 12 heads of 64 (101 MB): 37 us,
+// 2.7 TB/s.  11 texts of 1428 to 6289 keys, 32 / 8 heads of 128 in fp32 (392 MB): 204 us, bound by the
+// split operands' products.
 #include <cuda_runtime.h>
 
 #include <type_traits>
@@ -214,10 +215,9 @@ __global__ void __launch_bounds__(Cfg<T, kDP>::kThreads, Cfg<T, kDP>::kResident)
   // (a lo part is 0 or below it as often as above).  So a warp whose sums come out not finite (rare)
   // walks its keys once more, carefully: with weights of at most 1, with NaN scores taken again
   // whole (fp32), and with the value rows that hold such a value added by hand where p > 0 and
-  // zeroed before the product.  (The careful part
-  // kept out of the first walk: 32 texts of 1024 keys, 12 heads of 64, take 37.0 us in bf16 either
-  // way, 11 texts in fp32 208 against 251 us with values looked over in every block with a
-  // closed key.)
+  // zeroed before the product.  The first walk holds nothing of this: with values looked over in
+  // every block with a closed key 11 texts in fp32 (above) took 251 us, and with the second walk a
+  // flag of one loop 8 new tokens with a cap 24.6.
   auto walk = [&](auto how) {
     constexpr bool careful = decltype(how)::value;
 #pragma unroll

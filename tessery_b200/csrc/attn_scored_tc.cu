@@ -19,9 +19,9 @@
 // Bound: the softmax warps, by the latency of their chain (two warps per scheduler): 5500 cycles a
 // tile and CTA, 7000 with head_dim 128 and a cap.  Two threads a row (eight warps) took 298 against
 // 291 us with a long window, 85 against 77 us with a cap, 171 against 181 us with documents (since
-// at 163).  Measured: 8192 tokens, window 4096, 16 / 8 heads of 128: 290 us, 710 TFLOP/s of open
-// pairs (42 % of the measured bf16 rate); causal with a cap, packed, 16 / 8 heads of 128: 77 us; 8
-// texts of 1500 to 2048 in documents with a table, 12 heads of 64: 163 us.
+// at 164).  Measured: 8192 tokens, window 4096, 16 / 8 heads of 128: 290 us, 710 TFLOP/s of open
+// pairs (42 % of the measured bf16 rate); causal with a cap, packed, 16 / 8 heads of 128: 78 us; 8
+// texts of 1500 to 2048 in documents with a table, 12 heads of 64: 164 us.
 //
 // Values that are not finite.  A key that the rule closes to a row has p = 0 there, and the
 // product would turn 0 * Inf or 0 * NaN in its value row into NaN.  In tiles that are not wholly
@@ -305,7 +305,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       };
       // Turn n issues Q.K^T of tile n and then P.V of the tile before it (kEarly: as soon as the
       // softmax has read S; else S takes P's place, so P.V goes first).  One place in the code for
-      // each product: with two for Q.K^T the compiled code was wrong.
+      // each product.  A form with two places for Q.K^T, each right by reading, gave NaN or a fault
+      // where only the first was reached; the cause is not known, so the loop keeps to one.
       bool ok = wait(bar(kBarQ), 0, kSiteQ);
       bool more = true, odd = false;
       int prev = first;  // the tile whose P.V is due

@@ -9,7 +9,7 @@
 // (whole 128-byte rows; a thread that stored its own row directly wrote 16 bytes to each of 32
 // rows per instruction), and a residual of the output's type comes in the same way, a box ahead.
 // Bound: for large k the tiles' way from L2 to shared memory (9.8 TB/s at 128 x 256), for small k
-// the epilogue.  Measured: 33500 x 1024 x 2048 into an fp32 residual 166 us, 847 TFLOP/s; 8192 x
+// the epilogue.  Measured: 33500 x 1024 x 2048 into an fp32 residual 170 us, 827 TFLOP/s; 8192 x
 // 1536 x 384 with GELU 25 us, 387 TFLOP/s; 777 x 1000 x 1001 12.3 us.
 // Few tiles of long k: k is cut over CTAs, whose partial sums the last to arrive adds up.
 // gemv_kernel: a few rows (m <= 8) only stream w once: one or four warps per output column, w

@@ -11,8 +11,9 @@
 //
 // Bound: HBM, one read and one write of every element; ~6 flops per element.  A warp per token, so
 // that the sines and cosines serve every head, and no shared memory.  Measured: 65536 packed tokens,
-// 16 + 8 heads of 128 in bf16 with both norms (805 MB): 148 us, 5.4 TB/s; 8192 tokens, 12 + 12
-// heads of 32 in fp32 (50 MB): 12.6 us, 4.0 TB/s; 8 tokens: 11.5 us, the host's part of the call.
+// 16 + 8 heads of 128 in bf16 with both norms (805 MB): 151 us, 5.3 TB/s; 8192 tokens, 12 + 12
+// heads of 32 in fp32 (50 MB): 12.6 us, 4.0 TB/s; 8 tokens: 9.2 us from cold caches and 5.1 us from
+// warm ones, a warp's 12 steps through its token's 24 heads (queueing the call takes the host 6.7 us).
 #include <cuda_runtime.h>
 
 #include "../../include/tessattn.h"

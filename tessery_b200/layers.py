@@ -82,7 +82,8 @@ def rotary_frequencies(
     - "linear": every frequency divided by factor (position interpolation);
     - "ntk": theta multiplied by factor^(rot_dim / (rot_dim - 2)), which leaves the fastest
       pair as it is and divides the slowest by factor;
-    - "yarn": pairs that turn more than beta_fast times over the original positions are left,
+    - "yarn" (Peng et al., "YaRN: Efficient Context Window Extension of Large Language Models", 2023):
+      pairs that turn more than beta_fast times over the original positions are left,
       those that turn less than beta_slow times divided by factor, with a linear ramp over the
       pair index between the two; the amplitude is 0.1 ln(factor) + 1.
     """
