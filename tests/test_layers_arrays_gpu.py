@@ -1,10 +1,12 @@
-"""The encoder-layer operators on arrays one after another, each given what the one before returns (a
-B200), against the formulas in 64 bits.
+"""The encoder-layer operators on arrays (a B200): one after another, each given what the one before
+returns, against the formulas in 64 bits; and from several threads on one runtime.
 
-Tolerance, over the whole result: q, k, the attention's output and its weights are rounded to bf16, each
+Tolerance of the former, over the whole result: q, k, the attention's output and its weights are rounded to bf16, each
 by 2^-9 / sqrt(3) = 2^-9.8 of its values in the mean square.  A rounding of q or k moves scores of
 variance about 1 by as much, and so the output, whose values the weights average, by no more than that;
 four of them make 2^-8.8.  The gate is 2^-8."""
+
+import threading
 
 import numpy as np
 import pytest
@@ -49,3 +51,35 @@ def test_attention_block_on_arrays(runtime):
                                      k_docs=docs[at])[0]
         want[at] = oracle.linear_fused(ea.reshape(len(pos), -1), from_bf16_bits(w), bias=b)
     assert np.linalg.norm(y - x - want) < 2.0**-8 * np.linalg.norm(want - b)
+
+
+def test_threads_on_one_runtime(runtime):
+    """Three threads, three sizes: each call's result is the one it has alone."""
+    rng = np.random.default_rng(1)
+    cases = []
+    for n in (40, 300, 1100):
+        x = to_bf16_bits(rng.standard_normal((n, 4, 64)).astype(np.float32))
+        w = to_bf16_bits(rng.standard_normal((96, 256)).astype(np.float32))
+        freq = tx.rotary_frequencies(64)[0]
+        cases.append((
+            lambda x=x: tx.attention_scored(x, x, x, cu_q=np.array([0, len(x)]), runtime=runtime),
+            lambda x=x, f=freq: tx.rotary(x, x, inv_freq=f, seq=len(x), runtime=runtime)[1],
+            lambda x=x, w=w: tx.linear_fused(x.reshape(len(x), -1), w, runtime=runtime)))
+    want = [[call() for call in case] for case in cases]
+    wrong = []
+
+    def work(i):
+        try:
+            for _ in range(15):
+                for call, w in zip(cases[i], want[i], strict=True):
+                    if not np.array_equal(call(), w):
+                        wrong.append(i)
+        except Exception as e:  # noqa: BLE001 - reported below
+            wrong.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
