@@ -523,6 +523,113 @@ int tx_linear_fused(void *ctx, const void *x, uint64_t ldx, const void *w, uint6
                     void *out, int out_dtype, uint64_t ldo, uint32_t m, uint32_t n, uint32_t k,
                     int activation, void *stream);
 
+/* ---- layers of experts, norms on both sides of a block, positions with several axes ----
+
+ * What further encoders need beside the operators above: a feed-forward part made of experts of
+ * which each token takes a few, norms after a block as well as before it, and tokens that stand at
+ * a time, a row and a column.  No reference counterpart. */
+
+/* tx_rotary with a position on each of `axes` axes: positions device int32 [axes, axis_stride], of
+ * which the first `tokens` of every axis count (-2^24 < position < 2^24); pair_axes device int32
+ * [rot_dim / 2] names the axis by whose position a pair of columns turns (an axis >= axes counts as
+ * position 0 and is reported as TX_EINVAL by the next tx_sync). */
+int tx_rotary_axes(void *ctx, const TxRotaryTensor *q, const TxRotaryTensor *k, int in_dtype,
+                   int out_dtype, uint32_t tokens, uint32_t dim, uint32_t rot_dim, int interleaved,
+                   int inverse, const int32_t *positions, uint64_t axis_stride, uint32_t axes,
+                   const int32_t *pair_axes, const float *inv_freq, float amplitude, float eps,
+                   void *stream);
+
+enum { TX_SCORES_SOFTMAX = 0, TX_SCORES_SIGMOID = 1 };
+
+/* Routing of each token to top_k of `experts` experts.  Scores s = softmax(l) or 1 / (1 + e^-l) of the
+ * token's logits; the experts with the largest s + bias are chosen, in that order, the lower index
+ * first among equals.  With groups > 1 (experts / groups experts side by side each) only the experts
+ * of the top_groups groups are eligible whose best group_best (1 or 2) values of s + bias have the
+ * largest sums.  A weight is the expert's s, divided by the sum of the chosen ones' with `renormalise`,
+ * times scale.  The choice is that of exact arithmetic on the fp32 values of logits and bias.  An
+ * expert whose logit or bias is -inf is closed; NaN ranks below every number and counts in no group's
+ * sum.  Where a token has fewer open experts than top_k, and for the rows of a padded batch past their
+ * sequence's length, the remaining entries are expert -1 with weight 0. */
+typedef struct {
+  const void *logits;      /* [tokens, experts] TX_F32 or TX_BF16 */
+  uint64_t ld;             /* row stride in elements */
+  int dtype, scores;       /* TX_SCORES_* */
+  const float *bias;       /* fp32 [experts], for the choice alone; or NULL */
+  uint32_t groups, top_groups, group_best;
+  int renormalise;
+  float scale;
+  uint32_t seq;            /* with lengths: rows of each sequence */
+  const int32_t *lengths;  /* int32 [ceil(tokens / seq)]: valid rows of each; or NULL: all */
+  int32_t *chosen;         /* [tokens, top_k] */
+  float *weights;          /* [tokens, top_k] */
+  int32_t *offsets;        /* the plan (all three or none).  offsets [experts + 1]: expert e's rows are */
+  int32_t *order;          /* offsets[e] .. offsets[e + 1] - 1.  order [tokens * top_k]: the pair token *
+                              top_k + j of each row, rising inside an expert; entries past
+                              offsets[experts] are left as they were */
+  int32_t *places;         /* [tokens, top_k]: the row of each pair, or -1 */
+} TxRoute;
+
+/* experts at most 1024, top_k at most 32 and at most the eligible experts, tokens * top_k below 2^31.
+ * More than a few hundred tokens take two launches and scratch of the context (or, on a stream that is
+ * being captured, of the graph). */
+int tx_experts_route(void *ctx, const TxRoute *route, uint32_t tokens, uint32_t experts,
+                     uint32_t top_k, void *stream);
+
+/* The experts' products over rows that lie by expert: row r of expert e (offsets[e] <= r <
+ * offsets[e + 1], device int32 [experts + 1]) is
+ *   out[r] = act(x[i] w_e^T + b_e),   gated: act(x[i] g_e^T + bg_e) * (x[i] u_e^T + bu_e),
+ * i = order[r] / top_k (device int32 [rows]), or r with order NULL.  x [x_rows, k] and w [experts,
+ * n, k] bf16, gated w [experts, 2 n, k] with an expert's n gate rows before its n up rows; bias fp32
+ * [experts, n or 2 n] or NULL; out [rows, n] TX_F32 or TX_BF16; sums in fp32, rounded once.  Any n and
+ * k; x and w 16-byte aligned with ldx, ldw and expert_stride multiples of 8 (columns past k may hold
+ * anything).  experts at most 1024.  Rows past offsets[experts] are left as they were.  An offset that
+ * falls or leaves 0 .. rows is cut to fit, a row of x that is not there replaced by the last; both are
+ * reported as TX_EINVAL by the next tx_sync. */
+int tx_experts_linear(void *ctx, const void *x, uint64_t ldx, uint32_t x_rows, const void *w,
+                      uint64_t ldw, uint64_t expert_stride, const float *bias, void *out,
+                      int out_dtype, uint64_t ldo, const int32_t *offsets, const int32_t *order,
+                      uint32_t rows, uint32_t experts, uint32_t top_k, uint32_t n, uint32_t k,
+                      int gated, int activation, void *stream);
+
+enum { TX_NORM_NONE = 0, TX_NORM_RMS = 1, TX_NORM_LAYER = 2 };
+
+/* v inv (weight + offset) + bias: inv = 1 / sqrt(mean(v^2) + eps), for TX_NORM_LAYER of v - mean(v). */
+typedef struct {
+  const void *weight, *bias; /* [cols] of `dtype`, or NULL: 1 and 0 */
+  int kind, dtype;           /* TX_NORM_*; TX_F32 or TX_BF16 */
+  float eps, offset;
+} TxNorm;
+
+typedef struct {
+  const void *data;
+  uint64_t ld; /* row stride in elements */
+  int dtype;   /* TX_F32 or TX_BF16 */
+} TxMatrix;
+
+/* The rows between two blocks of a layer: with z = y, or z[t] = sum_j weights[t, j] y[places[t, j]]
+ * (the experts' rows joined, a negative place left out),
+ *   out = x_scale x + y_scale gate * after(z)   and   h = before(out),
+ * computed in fp32 and rounded once each (h from out before its rounding). */
+typedef struct {
+  TxMatrix x, y;             /* the residual rows and the block's; one may have data NULL (zeros) */
+  TxMatrix out, h;           /* one may have data NULL (not wanted) */
+  const int32_t *places;     /* int32 [rows, top_k] into the y_rows rows of y, or NULL */
+  const float *weights;      /* fp32 [rows, top_k] */
+  uint32_t top_k, y_rows;
+  const void *gate;          /* [gate_rows, cols], or NULL: 1 */
+  uint64_t ldg;
+  int gate_dtype;
+  uint32_t gate_rows;
+  const int32_t *cu_seqlens; /* int32 [gate_rows + 1]: a packed sequence's rows take its row of gate */
+  uint32_t seq;              /* else row / seq; with neither gate has one row, for all */
+  float x_scale, y_scale;
+  TxNorm after, before;
+} TxBlockNorm;
+
+/* cols at most 16384.  out or h may be x, or y without places, with the same dtype and row stride.  A
+ * place >= y_rows is left out and reported as TX_EINVAL by the next tx_sync. */
+int tx_block_norm(void *ctx, const TxBlockNorm *block, uint32_t rows, uint32_t cols, void *stream);
+
 /* ---- the BERT (BGE-small) fp32 forward around the head_dim-32 attention -------------
 
  * BertBackend.forward (bert.py:104-235) is built from these plus tx_linear (fmt TX_F32,

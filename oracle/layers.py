@@ -118,3 +118,116 @@ def linear_fused(x: NDArray, w: NDArray, *, bias=None, activation="none",
         y = y + bias
     y = activate(y, activation)
     return y if residual is None else y + residual
+
+
+def rotary_axes(x: NDArray, positions: NDArray, pair_axes: NDArray, inv_freq: NDArray,
+                **options) -> NDArray:
+    """rotary, pair by pair: pair c alone turns, by the positions of its axis."""
+    parts = []
+    for a, c in zip(np.asarray(pair_axes), range(len(inv_freq)), strict=True):
+        alone = np.zeros(len(inv_freq), np.float32)
+        alone[c] = inv_freq[c]
+        parts.append(rotary(x, np.asarray(positions)[a], alone, **options))
+    # Where pair c stands in part c; a column of no pair is the same in all.
+    out, half = parts[0].copy(), len(inv_freq)
+    for c, part in enumerate(parts):
+        for i in (2 * c, 2 * c + 1) if options.get("interleaved") else (c, c + half):
+            out[..., i] = part[..., i]
+    return out
+
+
+def experts_route(logits: NDArray, top_k: int, *, scores="softmax", bias=None, groups=1,
+                  top_groups=1, group_best=2, renormalise=True, scale=1.0, lengths=None, seq=0):
+    """(experts, weights, offsets, order, places) of float logits, token by token."""
+    logits = np.asarray(logits, np.float64)
+    tokens, n = logits.shape
+    bias = np.zeros(n) if bias is None else np.asarray(bias, np.float64)
+    chosen, weights = np.full((tokens, top_k), -1), np.zeros((tokens, top_k))
+    for t in range(tokens):
+        if lengths is not None and t % seq >= lengths[t // seq]:
+            continue
+        row = logits[t]
+        open_ = [e for e in range(n) if row[e] != -np.inf and bias[e] != -np.inf]
+        if not open_:
+            continue
+        with np.errstate(over="ignore", invalid="ignore"):
+            if scores == "softmax":
+                s = np.exp(row - np.nanmax(row[open_]))
+                s = s / s[open_].sum()
+            else:
+                s = 1.0 / (1.0 + np.exp(-row))
+        c = s + bias
+        if groups > 1:
+            per, sums = n // groups, []
+            for g in range(groups):
+                inside = sorted((c[e] for e in open_ if e // per == g and not np.isnan(c[e])),
+                                reverse=True)
+                sums.append(sum(inside[:group_best]) if inside else -np.inf)
+            kept = sorted(range(groups), key=lambda g: (-sums[g], g))[:top_groups]
+            open_ = [e for e in open_ if e // per in kept]
+        order = sorted(open_, key=lambda e: (np.isnan(c[e]), 0 if np.isnan(c[e]) else -c[e], e))
+        for j, e in enumerate(order[:top_k]):
+            chosen[t, j], weights[t, j] = e, s[e]
+        if renormalise and order:
+            weights[t] /= weights[t].sum()
+        weights[t] *= scale
+    order, offsets, places = [], [0], np.full(tokens * top_k, -1)
+    for e in range(n):
+        for pair in np.flatnonzero(chosen.reshape(-1) == e):
+            places[pair] = len(order)
+            order.append(pair)
+        offsets.append(len(order))
+    order += [-1] * (tokens * top_k - len(order))
+    return (chosen, weights, np.array(offsets), np.array(order, dtype=np.int64),
+            places.reshape(tokens, top_k))
+
+
+def experts_linear(x: NDArray, w: NDArray, offsets, *, order=None, top_k=1, gated=False,
+                   activation="none", bias=None) -> tuple[NDArray, NDArray]:
+    """(out, what its errors are measured against) [rows, n] of float values, row by row; rows of no
+    expert are zeros.  The measure is |x| |w| + |bias| of a row, gated the product's two terms."""
+    x, w = np.asarray(x, np.float64), np.asarray(w, np.float64)
+    rows = len(x) if order is None else len(x) * top_k
+    n = w.shape[1] // (2 if gated else 1)
+    out, mass = np.zeros((rows, n)), np.zeros((rows, n))
+    for e in range(w.shape[0]):
+        for r in range(offsets[e], offsets[e + 1]):
+            xr = x[r if order is None else order[r] // top_k]
+            y, m = w[e] @ xr, np.abs(w[e]) @ np.abs(xr)
+            if bias is not None:
+                y, m = y + bias[e], m + np.abs(bias[e])
+            if gated:
+                a = activate(y[:n], activation)
+                out[r] = a * y[n:]
+                mass[r] = np.abs(a) * m[n:] + m[:n] * np.abs(y[n:])
+            else:
+                out[r], mass[r] = activate(y, activation), m
+    return out, mass
+
+
+def norm(v: NDArray, *, kind, weight=None, bias=None, eps=1e-6, offset=0.0) -> NDArray:
+    if kind == "layer":
+        v = v - v.mean(axis=-1, keepdims=True)
+    v = v / np.sqrt(np.mean(v * v, axis=-1, keepdims=True) + eps)
+    v = v * (1.0 if weight is None else weight + offset)
+    return v if bias is None else v + bias
+
+
+def block_norm(x, y=None, *, after=None, before=None, x_scale=1.0, y_scale=1.0, gate=None,
+               gate_row=None, places=None, weights=None) -> tuple[NDArray, NDArray]:
+    """(out, h) of float values; gate_row: the row of gate of each row."""
+    z = None if y is None else np.asarray(y, np.float64)
+    if places is not None:
+        joined = np.zeros((len(places), z.shape[1]))
+        for t, row in enumerate(places):
+            for j, place in enumerate(row):
+                if place >= 0:
+                    joined[t] += float(weights[t, j]) * z[place]
+        z = joined
+    if z is not None and after is not None:
+        z = norm(z, **after)
+    if z is not None and gate is not None:
+        z = z * np.asarray(gate, np.float64)[gate_row]
+    out = (0.0 if z is None else y_scale * z) + (
+        0.0 if x is None else x_scale * np.asarray(x, np.float64))
+    return out, out if before is None else norm(out, **before)

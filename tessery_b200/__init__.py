@@ -15,7 +15,18 @@ from .errors import (
     InvalidInputError,
     NativeBuildError,
 )
-from .layers import attention_scored, linear_fused, rotary, rotary_frequencies
+from .layers import (
+    Routes,
+    attention_scored,
+    block_norm,
+    experts_linear,
+    experts_route,
+    linear_fused,
+    rotary,
+    rotary_axes,
+    rotary_frequencies,
+    rotary_pair_axes,
+)
 from .native import TX_BF16, TX_F32
 from .partition import gather_shard, pack, shard_sequences
 from .runtime import Buffer, CudaRuntime
@@ -30,11 +41,15 @@ __all__ = [
     "InferenceError",
     "InvalidInputError",
     "NativeBuildError",
+    "Routes",
     "TX_BF16",
     "TX_F32",
     "attention",
     "attention_scored",
+    "block_norm",
     "default_runtime",
+    "experts_linear",
+    "experts_route",
     "gather_shard",
     "linear_fused",
     "pack",
@@ -42,7 +57,9 @@ __all__ = [
     "pool_project",
     "qk_norm_rope",
     "rotary",
+    "rotary_axes",
     "rotary_frequencies",
+    "rotary_pair_axes",
     "shard_sequences",
     "unpack_rows",
     "varlen_batches",

@@ -59,6 +59,23 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
+// The sequence of packed row `tok`: the last s in [0, nseq) with cu[s] <= tok, by a search
+// whose 32 lanes probe at once (two dependent loads for up to 1024 sequences).
+__device__ __forceinline__ uint32_t warp_find_seq(const int32_t *cu, uint32_t nseq, uint32_t tok,
+                                                  uint32_t lane) {
+  uint32_t lo = 0, n = nseq;  // the answer is in [lo, lo + n)
+  while (n > 1) {
+    const uint32_t step = (n + 31) / 32;
+    const uint32_t at = lane * step;
+    const bool le = at < n && (uint32_t)cu[lo + at] <= tok;
+    const uint32_t hits = __popc(__ballot_sync(0xffffffffu, le));  // le is monotone in lane
+    const uint32_t skip = (hits ? hits - 1 : 0) * step;
+    lo += skip;
+    n = min(step, n - skip);
+  }
+  return lo;
+}
+
 // sin and cos of a float angle (a RoPE angle, position x inverse frequency): Cody-Waite
 // reduction by 2*pi (2*pi split into a float head and a float tail; each product k * part
 // is exact inside its fma) to [-pi, pi], then the hardware approximations, accurate to

@@ -188,6 +188,11 @@ struct RotaryProblem {
   const float *inv_freq;     // fp32 [rot / 2]
   float amplitude, amplitude_sin;  // factors of cosine and sine (negated for the inverse)
   float eps;
+  // with axes > 0: positions [axes][axis_stride], and the axis of each pair [rot / 2]
+  uint32_t axes;
+  uint64_t axis_stride;
+  const int32_t *pair_axes;
+  int *status;
 };
 uint32_t rotary_vector(const RotaryProblem &p);
 
@@ -253,6 +258,67 @@ struct LinearFusedProblem {
 // splits * 8192 floats of scratch each).
 uint32_t linear_fused_splits(const LinearFusedProblem &p, int num_sms, uint32_t *tiles);
 cudaError_t launch_linear_fused(const LinearFusedProblem &p, int num_sms, cudaStream_t stream);
+
+// ---- Layers of experts and norms on both sides (experts_*.cu, block_norm.cu) ----
+struct RouteProblem {
+  const void *logits;
+  uint64_t ld;
+  int logits_dtype, softmax, renormalise;
+  const float *bias;
+  uint32_t tokens, experts, top_k, groups, top_groups, group_best;
+  float scale;
+  const int32_t *lengths;  // valid rows of each sequence of `seq` rows, or NULL
+  uint32_t seq;
+  int32_t *chosen;         // [tokens, top_k]
+  float *weights;
+  int32_t *offsets, *order, *places;  // the plan, or NULL
+  uint32_t run, blocks;    // tokens of a block (route_plan)
+  uint32_t *counts;        // [blocks][experts] with blocks > 1
+  uint32_t off_groups, off_places;  // shared memory, set by the launcher
+};
+void route_plan(RouteProblem *p, int num_sms);
+cudaError_t launch_experts_route(const RouteProblem &p, cudaStream_t stream);
+
+struct ExpertsProblem {
+  const void *x, *w;
+  const float *bias;
+  void *out;
+  uint64_t ldx, ldw, expert_stride, ldo;
+  const int32_t *offsets, *order;
+  uint32_t x_rows, rows, experts, top_k, n, k;
+  int gated, act, out_dtype;
+  bool out_vec;  // on 16-byte boundaries: set by the launcher
+  int *status;
+  long long wait_cycles;
+};
+cudaError_t launch_experts_linear(ExpertsProblem p, int num_sms, cudaStream_t stream);
+
+struct BlockNorm {
+  int kind, dtype;
+  const void *weight, *bias;
+  float eps, offset;
+};
+struct BlockNormProblem {
+  const void *x, *y;
+  void *out, *h;
+  uint64_t ldx, ldy, ldo, ldh;
+  int x_dtype, y_dtype, out_dtype, h_dtype;
+  uint32_t rows, cols;
+  const int32_t *places;  // [rows, top_k], or NULL: y has a row for each
+  const float *weights;
+  uint32_t top_k, y_rows;
+  const void *gate;
+  uint64_t ldg;
+  int gate_dtype;
+  uint32_t gate_rows;
+  const int32_t *cu;  // the gate's row of a row: by packed sequence, by seq rows, or 0
+  uint32_t seq;
+  float x_scale, y_scale;
+  BlockNorm after, before;
+  bool vec;  // 16-byte accesses: set by the launcher
+  int *status;
+};
+cudaError_t launch_block_norm(BlockNormProblem p, cudaStream_t stream);
 
 // ---- BERT fp32 forward (bert_ops.cu) ----
 // Word + token-type-0 + absolute-position embeddings of `tokens` tokens, LayerNorm'd; the

@@ -83,21 +83,15 @@ __device__ __forceinline__ void store_vec(uint16_t *p, const float (&f)[V]) {
     p[0] = f32_to_bf16_bits(f[0]);
 }
 
-// The sequence of packed row `tok`: the last s in [0, nseq) with cu[s] <= tok, by a search
-// whose 32 lanes probe at once (two dependent loads for up to 1024 sequences).
-__device__ __forceinline__ uint32_t warp_find_seq(const int32_t *cu, uint32_t nseq, uint32_t tok,
-                                                  uint32_t lane) {
-  uint32_t lo = 0, n = nseq;  // the answer is in [lo, lo + n)
-  while (n > 1) {
-    const uint32_t step = (n + 31) / 32;
-    const uint32_t at = lane * step;
-    const bool le = at < n && (uint32_t)cu[lo + at] <= tok;
-    const uint32_t hits = __popc(__ballot_sync(0xffffffffu, le));  // le is monotone in lane
-    const uint32_t skip = (hits ? hits - 1 : 0) * step;
-    lo += skip;
-    n = min(step, n - skip);
+// The position by which pair `pair` of token `tok` turns; an axis that is not there counts as position 0
+// and is reported.
+__device__ __forceinline__ float axis_position(const RotaryProblem &p, uint32_t pair, uint32_t tok) {
+  const uint32_t axis = (uint32_t)__ldg(p.pair_axes + pair);
+  if (axis >= p.axes) {
+    report_status(p.status, kStatusBadArg);
+    return 0.f;
   }
-  return lo;
+  return (float)__ldg(p.positions + axis * p.axis_stride + tok);
 }
 
 // A head is cut into slots of 2V columns, held by one lane as two vectors of V: in a rotated
@@ -105,7 +99,8 @@ __device__ __forceinline__ uint32_t warp_find_seq(const int32_t *cu, uint32_t ns
 // (interleaved).  kLanes lanes cover a head with kSlots slots each, so a warp takes
 // 32 / kLanes heads at a time; one warp per token, so the sines and cosines of a lane's slots
 // serve every head of the token.
-template <typename TI, typename TO, int V, int kLanes, int kSlots>
+// kAxes: a pair turns by its own axis' position of the token.
+template <typename TI, typename TO, int V, int kLanes, int kSlots, bool kAxes>
 __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ RotaryProblem p) {
   constexpr uint32_t kHeads = 32 / kLanes;  // heads per step of a warp
   const uint32_t lane = threadIdx.x & 31;
@@ -152,8 +147,9 @@ __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ Rot
   };
   fetch(0);
 
-  uint32_t pos;
-  if (p.positions)
+  uint32_t pos = 0;
+  if constexpr (kAxes) {
+  } else if (p.positions)
     pos = (uint32_t)p.positions[tok];
   else if (p.cu)
     pos = tok - (uint32_t)p.cu[warp_find_seq(p.cu, p.nseq, tok, lane)];
@@ -166,8 +162,9 @@ __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ Rot
     if (turned[s]) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        float sn, cs;
-        rope_sincos(__fmul_rn((float)pos, __ldg(p.inv_freq + slot * V + i)), &sn, &cs);
+        float sn, cs, at = (float)pos;
+        if constexpr (kAxes) at = axis_position(p, slot * V + i, tok);
+        rope_sincos(__fmul_rn(at, __ldg(p.inv_freq + slot * V + i)), &sn, &cs);
         co[s][i] = cs * p.amplitude;
         si[s][i] = sn * p.amplitude_sin;
       }
@@ -247,8 +244,11 @@ template <typename TI, typename TO, int V, int kLanes, int kSlots>
 cudaError_t run(const RotaryProblem &p, cudaStream_t stream) {
   // Few tokens: a warp per block, so that they spread over the SMs.
   const uint32_t warps = p.tokens >= 8 * 148 ? 8 : 1;
-  rotary_kernel<TI, TO, V, kLanes, kSlots>
-      <<<(p.tokens + warps - 1) / warps, 32 * warps, 0, stream>>>(p);
+  const uint32_t blocks = (p.tokens + warps - 1) / warps;
+  if (p.axes)
+    rotary_kernel<TI, TO, V, kLanes, kSlots, true><<<blocks, 32 * warps, 0, stream>>>(p);
+  else
+    rotary_kernel<TI, TO, V, kLanes, kSlots, false><<<blocks, 32 * warps, 0, stream>>>(p);
   return cudaGetLastError();
 }
 

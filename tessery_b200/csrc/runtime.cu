@@ -24,7 +24,7 @@
 
 namespace {
 
-constexpr uint32_t kAbiVersion = 11;
+constexpr uint32_t kAbiVersion = 12;
 constexpr uint32_t kHostChunks = 8;              // most chunks of a host-buffer call
 constexpr size_t kHostChunkBytes = 16u << 20;     // bytes moved per chunk, at least
 // Padded layout, host-buffer calls: the valid k/v rows of consecutive sequences are
@@ -1720,28 +1720,26 @@ static bool heads_overlap(uint64_t tokens, uint64_t heads, uint64_t token_stride
   return false;
 }
 
-int tx_rotary(void *ctx, const TxRotaryTensor *q, const TxRotaryTensor *k, int in_dtype,
-              int out_dtype, uint32_t tokens, uint32_t dim, uint32_t rot_dim, int interleaved,
-              int inverse, const int32_t *positions, const int32_t *cu_seqlens, uint32_t nseq,
-              uint32_t seq, const float *inv_freq, float amplitude, float eps, void *stream) {
-  Ctx *c = (Ctx *)ctx;
-  if (!c) return TX_EINVAL;
-  std::lock_guard<std::recursive_mutex> g(c->mu);
+// The checks and launch of both rotations; p carries where the positions come from.
+static int rotary_call(Ctx *c, const TxRotaryTensor *q, const TxRotaryTensor *k, int in_dtype,
+                       int out_dtype, uint32_t tokens, uint32_t dim, uint32_t rot_dim,
+                       int interleaved, int inverse, const float *inv_freq, float amplitude,
+                       float eps, tx::RotaryProblem p, const char *name, void *stream) {
   if (!q || !inv_freq) return fail(c, TX_EINVAL, "rotary: null pointer");
   if ((in_dtype != TX_F32 && in_dtype != TX_BF16) || (out_dtype != TX_F32 && out_dtype != TX_BF16))
     return fail(c, TX_EINVAL, "rotary: bad dtype");
   if (!dim || dim > 256 || rot_dim < 2 || rot_dim > dim || rot_dim % 2)
     return fail(c, TX_EINVAL, "rotary: dim 1..256, rot_dim even, 2..dim");
-  if (!positions && cu_seqlens && !nseq) return fail(c, TX_EINVAL, "rotary: nseq must be positive");
-  if (!positions && !cu_seqlens && !seq)
+  if (!p.positions && p.cu && !p.nseq) return fail(c, TX_EINVAL, "rotary: nseq must be positive");
+  if (!p.positions && !p.cu && !p.seq)
     return fail(c, TX_EINVAL, "rotary: positions, cu_seqlens or seq required");
   if (!std::isfinite(amplitude) || !(eps >= 0.f) || !std::isfinite(eps))
     return fail(c, TX_EINVAL, "rotary: bad amplitude or eps");
   if (tokens > 0x7fffffffu) return fail(c, TX_EINVAL, "rotary: too many tokens");
-  if ((uintptr_t)positions % 4 || (uintptr_t)cu_seqlens % 4 || (uintptr_t)inv_freq % 4)
+  if ((uintptr_t)p.positions % 4 || (uintptr_t)p.cu % 4 || (uintptr_t)inv_freq % 4 ||
+      (uintptr_t)p.pair_axes % 4)
     return fail(c, TX_EINVAL, "rotary: misaligned pointer");
   const size_t ei = in_dtype == TX_BF16 ? 2 : 4, eo = out_dtype == TX_BF16 ? 2 : 4;
-  tx::RotaryProblem p{};
   const TxRotaryTensor *side[2] = {q, k};
   tx::RotaryTensor *to[2] = {&p.q, &p.k};
   for (int i = 0; i < 2; ++i) {
@@ -1763,16 +1761,49 @@ int tx_rotary(void *ctx, const TxRotaryTensor *q, const TxRotaryTensor *k, int i
   p.in_dtype = in_dtype; p.out_dtype = out_dtype; p.tokens = tokens; p.dim = dim; p.rot = rot_dim;
   p.interleaved = interleaved ? 1 : 0;
   p.norm = p.q.norm_w || p.k.norm_w;
-  p.positions = positions; p.cu = cu_seqlens; p.nseq = nseq; p.seq = seq; p.inv_freq = inv_freq;
+  p.inv_freq = inv_freq;
   p.amplitude = amplitude; p.amplitude_sin = inverse ? -amplitude : amplitude; p.eps = eps;
   if (!tokens) return TX_OK;
   cudaSetDevice(c->device);
   cudaError_t e = tx::launch_rotary(p, stream ? (cudaStream_t)stream : c->stream);
   if (e != cudaSuccess) return cuda_fail(c, e, "rotary launch");
-  c->last_kernel = "rotary";
+  c->last_kernel = name;
   ++c->launches;
   return TX_OK;
 }
+
+int tx_rotary(void *ctx, const TxRotaryTensor *q, const TxRotaryTensor *k, int in_dtype,
+              int out_dtype, uint32_t tokens, uint32_t dim, uint32_t rot_dim, int interleaved,
+              int inverse, const int32_t *positions, const int32_t *cu_seqlens, uint32_t nseq,
+              uint32_t seq, const float *inv_freq, float amplitude, float eps, void *stream) {
+  Ctx *c = (Ctx *)ctx;
+  if (!c) return TX_EINVAL;
+  std::lock_guard<std::recursive_mutex> g(c->mu);
+  tx::RotaryProblem p{};
+  p.positions = positions; p.cu = cu_seqlens; p.nseq = nseq; p.seq = seq;
+  return rotary_call(c, q, k, in_dtype, out_dtype, tokens, dim, rot_dim, interleaved, inverse,
+                     inv_freq, amplitude, eps, p, "rotary", stream);
+}
+
+int tx_rotary_axes(void *ctx, const TxRotaryTensor *q, const TxRotaryTensor *k, int in_dtype,
+                   int out_dtype, uint32_t tokens, uint32_t dim, uint32_t rot_dim, int interleaved,
+                   int inverse, const int32_t *positions, uint64_t axis_stride, uint32_t axes,
+                   const int32_t *pair_axes, const float *inv_freq, float amplitude, float eps,
+                   void *stream) {
+  Ctx *c = (Ctx *)ctx;
+  if (!c) return TX_EINVAL;
+  std::lock_guard<std::recursive_mutex> g(c->mu);
+  if (!positions || !pair_axes || !axes)
+    return fail(c, TX_EINVAL, "rotary_axes: positions, pair_axes and axes required");
+  if (axes > 1 && (axis_stride < tokens || axis_stride > 1ull << 38))
+    return fail(c, TX_EINVAL, "rotary_axes: an axis' positions overlap the next one's");
+  tx::RotaryProblem p{};
+  p.positions = positions; p.axes = axes; p.axis_stride = axis_stride; p.pair_axes = pair_axes;
+  p.status = c->status;
+  return rotary_call(c, q, k, in_dtype, out_dtype, tokens, dim, rot_dim, interleaved, inverse,
+                     inv_freq, amplitude, eps, p, "rotary_axes", stream);
+}
+
 
 int tx_attention_scored(void *ctx, const TxRows *qkv, void *out, const TxLayout *layouts,
                         uint32_t nseq, uint32_t heads, uint32_t kv_heads, uint32_t dim, int in_dtype,
@@ -1920,6 +1951,198 @@ int tx_linear_fused(void *ctx, const void *x, uint64_t ldx, const void *w, uint6
   if (e != cudaSuccess) return cuda_fail(c, e, "linear_fused launch");
   if (released != cudaSuccess) return cuda_fail(c, released, "partial sums");
   c->last_kernel = "linear_fused";
+  ++c->launches;
+  return TX_OK;
+}
+
+int tx_experts_route(void *ctx, const TxRoute *route, uint32_t tokens, uint32_t experts,
+                     uint32_t top_k, void *stream) {
+  Ctx *c = (Ctx *)ctx;
+  if (!c) return TX_EINVAL;
+  std::lock_guard<std::recursive_mutex> g(c->mu);
+  if (!route || !route->logits || !route->chosen || !route->weights)
+    return fail(c, TX_EINVAL, "experts_route: null pointer");
+  const TxRoute &r = *route;
+  if (r.dtype != TX_F32 && r.dtype != TX_BF16) return fail(c, TX_EINVAL, "experts_route: bad dtype");
+  if (r.scores != TX_SCORES_SOFTMAX && r.scores != TX_SCORES_SIGMOID)
+    return fail(c, TX_EINVAL, "experts_route: bad scores");
+  if (!experts || experts > 1024) return fail(c, TX_EINVAL, "experts_route: 1..1024 experts");
+  if (!r.groups || experts % r.groups || !r.top_groups || r.top_groups > r.groups ||
+      (r.groups > 1 && r.group_best != 1 && r.group_best != 2))
+    return fail(c, TX_EINVAL, "experts_route: groups divide the experts, top_groups 1..groups, "
+                              "group_best 1 or 2");
+  if (!top_k || top_k > 32 || top_k > experts / r.groups * r.top_groups)
+    return fail(c, TX_EINVAL, "experts_route: top_k 1..32, at most the eligible experts");
+  if (r.ld < experts || r.ld > 1ull << 38)
+    return fail(c, TX_EINVAL, "experts_route: a row stride is shorter than its row");
+  if (!std::isfinite(r.scale)) return fail(c, TX_EINVAL, "experts_route: scale must be finite");
+  if (r.lengths && !r.seq) return fail(c, TX_EINVAL, "experts_route: lengths need seq");
+  if ((uint64_t)tokens * top_k > 0x7fffffffull)
+    return fail(c, TX_EINVAL, "experts_route: too many tokens");
+  if (!r.offsets != !r.order || !r.offsets != !r.places)
+    return fail(c, TX_EINVAL, "experts_route: offsets, order and places go together");
+  const void *words[] = {r.bias, r.lengths, r.chosen, r.weights, r.offsets, r.order, r.places};
+  for (const void *w : words)
+    if ((uintptr_t)w % 4) return fail(c, TX_EINVAL, "experts_route: misaligned pointer");
+  if ((uintptr_t)r.logits % (r.dtype == TX_BF16 ? 2 : 4))
+    return fail(c, TX_EINVAL, "experts_route: misaligned pointer");
+  cudaError_t e = cudaSetDevice(c->device);
+  if (e != cudaSuccess) return cuda_fail(c, e, "cudaSetDevice");
+  cudaStream_t st = stream ? (cudaStream_t)stream : c->stream;
+  if (!tokens) {  // a plan without rows
+    if (r.offsets && (e = cudaMemsetAsync(r.offsets, 0, 4 * (experts + 1), st)) != cudaSuccess)
+      return cuda_fail(c, e, "experts_route offsets");
+    return TX_OK;
+  }
+  tx::RouteProblem p{};
+  p.logits = r.logits; p.ld = r.ld; p.logits_dtype = r.dtype;
+  p.softmax = r.scores == TX_SCORES_SOFTMAX; p.renormalise = r.renormalise ? 1 : 0;
+  p.bias = r.bias; p.tokens = tokens; p.experts = experts; p.top_k = top_k;
+  p.groups = r.groups; p.top_groups = r.top_groups; p.group_best = r.group_best;
+  p.scale = r.scale; p.lengths = r.lengths; p.seq = r.seq;
+  p.chosen = r.chosen; p.weights = r.weights;
+  p.offsets = r.offsets; p.order = r.order; p.places = r.places;
+  tx::route_plan(&p, c->sms);
+  Parts parts;
+  const bool scratch = p.order && p.blocks > 1;
+  if (scratch) {
+    e = parts_acquire(c, st, 1, (size_t)p.blocks * experts * 4, &parts);
+    if (e != cudaSuccess) return cuda_fail(c, e, "routing counts");
+    p.counts = (uint32_t *)parts.sums;
+  }
+  e = tx::launch_experts_route(p, st);
+  const cudaError_t released = scratch ? parts_release(c, st, parts) : cudaSuccess;
+  if (e != cudaSuccess) return cuda_fail(c, e, "experts_route launch");
+  if (released != cudaSuccess) return cuda_fail(c, released, "routing counts");
+  c->last_kernel = "experts_route";
+  c->launches += scratch ? 2 : 1;
+  return TX_OK;
+}
+
+int tx_experts_linear(void *ctx, const void *x, uint64_t ldx, uint32_t x_rows, const void *w,
+                      uint64_t ldw, uint64_t expert_stride, const float *bias, void *out,
+                      int out_dtype, uint64_t ldo, const int32_t *offsets, const int32_t *order,
+                      uint32_t rows, uint32_t experts, uint32_t top_k, uint32_t n, uint32_t k,
+                      int gated, int activation, void *stream) {
+  Ctx *c = (Ctx *)ctx;
+  if (!c) return TX_EINVAL;
+  std::lock_guard<std::recursive_mutex> g(c->mu);
+  if (!x || !w || !out || !offsets) return fail(c, TX_EINVAL, "experts_linear: null pointer");
+  if (out_dtype != TX_F32 && out_dtype != TX_BF16)
+    return fail(c, TX_EINVAL, "experts_linear: bad dtype");
+  if (activation < TX_ACT_NONE || activation > TX_ACT_SILU)
+    return fail(c, TX_EINVAL, "experts_linear: bad activation");
+  if (!n || !k || !top_k) return fail(c, TX_EINVAL, "experts_linear: n, k and top_k must be positive");
+  if (!experts || experts > 1024) return fail(c, TX_EINVAL, "experts_linear: 1..1024 experts");
+  if (x_rows > 0x7fffff00u || rows > 0x7fffff00u || n > 0x3fffff00u || k > 0x7fffff00u ||
+      (rows / 128 + (uint64_t)experts) * ((uint64_t)n / 32 + 1) > 0x7fffffffull)
+    return fail(c, TX_EINVAL, "experts_linear: problem too large");
+  const uint64_t most = 1ull << 38, wide = (uint64_t)n * (gated ? 2 : 1);
+  if (ldx < k || ldw < k || ldo < n || ldx > most || ldw > most || ldo > most)
+    return fail(c, TX_EINVAL, "experts_linear: a row stride is shorter than its row");
+  if (experts > 1 && (expert_stride < (wide - 1) * ldw + k || expert_stride > most))
+    return fail(c, TX_EINVAL, "experts_linear: an expert's weights overlap the next one's");
+  if (experts == 1) expert_stride = wide * ldw;
+  if (ldx % 8 || ldw % 8 || expert_stride % 8 || (uintptr_t)x % 16 || (uintptr_t)w % 16)
+    return fail(c, TX_EINVAL, "experts_linear: rows of x and w on 16-byte boundaries");
+  if ((uintptr_t)out % (out_dtype == TX_BF16 ? 2 : 4) || (uintptr_t)bias % 4 ||
+      (uintptr_t)offsets % 4 || (uintptr_t)order % 4)
+    return fail(c, TX_EINVAL, "experts_linear: misaligned pointer");
+  if (x == out) return fail(c, TX_EINVAL, "experts_linear: out may not be x");
+  if (!order && x_rows < rows) return fail(c, TX_EINVAL, "experts_linear: x has fewer rows than out");
+  if (!rows) return TX_OK;
+  if (!x_rows) return fail(c, TX_EINVAL, "experts_linear: x has no rows");
+  tx::ExpertsProblem p{};
+  p.x = x; p.w = w; p.bias = bias; p.out = out;
+  p.ldx = ldx; p.ldw = ldw; p.expert_stride = expert_stride; p.ldo = ldo;
+  p.offsets = offsets; p.order = order; p.x_rows = x_rows; p.rows = rows; p.experts = experts;
+  p.top_k = top_k; p.n = n; p.k = k; p.gated = gated ? 1 : 0; p.act = activation;
+  p.out_dtype = out_dtype; p.status = c->status;
+  p.wait_cycles = c->wait_cycles > 0 ? c->wait_cycles : 2000000000ll;
+  cudaError_t e = cudaSetDevice(c->device);
+  if (e != cudaSuccess) return cuda_fail(c, e, "cudaSetDevice");
+  e = tx::launch_experts_linear(p, c->sms, stream ? (cudaStream_t)stream : c->stream);
+  if (e != cudaSuccess) return cuda_fail(c, e, "experts_linear launch");
+  c->last_kernel = "experts_linear";
+  ++c->launches;
+  return TX_OK;
+}
+
+int tx_block_norm(void *ctx, const TxBlockNorm *block, uint32_t rows, uint32_t cols, void *stream) {
+  Ctx *c = (Ctx *)ctx;
+  if (!c) return TX_EINVAL;
+  std::lock_guard<std::recursive_mutex> g(c->mu);
+  static_assert(sizeof(TxBlockNorm) == 232, "the layout that bindings pack");
+  if (!block) return fail(c, TX_EINVAL, "block_norm: null pointer");
+  const TxBlockNorm &b = *block;
+  if ((!b.x.data && !b.y.data) || (!b.out.data && !b.h.data))
+    return fail(c, TX_EINVAL, "block_norm: x or y, and out or h required");
+  if (!cols || cols > 16384) return fail(c, TX_EINVAL, "block_norm: 1..16384 columns");
+  if (rows > 0x7fffffffu) return fail(c, TX_EINVAL, "block_norm: too many rows");
+  const TxMatrix *all[] = {&b.x, &b.y, &b.out, &b.h};
+  for (const TxMatrix *m : all) {
+    if (!m->data) continue;
+    if (m->dtype != TX_F32 && m->dtype != TX_BF16) return fail(c, TX_EINVAL, "block_norm: bad dtype");
+    if (m->ld < cols || m->ld > 1ull << 38)
+      return fail(c, TX_EINVAL, "block_norm: a row stride is shorter than its row");
+    if ((uintptr_t)m->data % (m->dtype == TX_BF16 ? 2 : 4))
+      return fail(c, TX_EINVAL, "block_norm: misaligned pointer");
+  }
+  if (b.out.data == b.h.data) return fail(c, TX_EINVAL, "block_norm: out and h are one");
+  for (const TxMatrix *o : {&b.out, &b.h})
+    for (const TxMatrix *i : {&b.x, &b.y})
+      if (o->data && o->data == i->data &&
+          (o->dtype != i->dtype || o->ld != i->ld || (i == &b.y && b.places)))
+        return fail(c, TX_EINVAL, "block_norm: in place needs equal dtypes and strides, and no places");
+  if (b.places && (!b.y.data || !b.weights || !b.top_k || b.y_rows > 0x7fffffffu))
+    return fail(c, TX_EINVAL, "block_norm: places need y, weights and top_k");
+  if (b.gate) {
+    if (b.gate_dtype != TX_F32 && b.gate_dtype != TX_BF16)
+      return fail(c, TX_EINVAL, "block_norm: bad dtype");
+    if (!b.gate_rows || b.gate_rows > 0x7fffffffu || b.ldg < cols || b.ldg > 1ull << 38)
+      return fail(c, TX_EINVAL, "block_norm: a row stride is shorter than its row");
+    if ((uintptr_t)b.gate % (b.gate_dtype == TX_BF16 ? 2 : 4))
+      return fail(c, TX_EINVAL, "block_norm: misaligned pointer");
+    if (b.cu_seqlens && b.seq)
+      return fail(c, TX_EINVAL, "block_norm: cu_seqlens and seq exclude one another");
+    if (b.cu_seqlens ? false : b.seq ? (uint64_t)b.gate_rows * b.seq < rows : b.gate_rows != 1)
+      return fail(c, TX_EINVAL, "block_norm: gate_rows do not cover the rows");
+  }
+  for (const TxNorm *n : {&b.after, &b.before}) {
+    if (n->kind < TX_NORM_NONE || n->kind > TX_NORM_LAYER)
+      return fail(c, TX_EINVAL, "block_norm: bad norm");
+    if (n->kind == TX_NORM_NONE) continue;
+    if (n->dtype != TX_F32 && n->dtype != TX_BF16) return fail(c, TX_EINVAL, "block_norm: bad dtype");
+    if (!(n->eps >= 0.f) || !std::isfinite(n->eps) || !std::isfinite(n->offset))
+      return fail(c, TX_EINVAL, "block_norm: bad eps or offset");
+    const size_t size = n->dtype == TX_BF16 ? 2 : 4;
+    if ((uintptr_t)n->weight % size || (uintptr_t)n->bias % size)
+      return fail(c, TX_EINVAL, "block_norm: misaligned pointer");
+  }
+  if (!std::isfinite(b.x_scale) || !std::isfinite(b.y_scale))
+    return fail(c, TX_EINVAL, "block_norm: scales must be finite");
+  if ((uintptr_t)b.places % 4 || (uintptr_t)b.weights % 4 || (uintptr_t)b.cu_seqlens % 4)
+    return fail(c, TX_EINVAL, "block_norm: misaligned pointer");
+  if (!rows) return TX_OK;
+  tx::BlockNormProblem p{};
+  p.x = b.x.data; p.y = b.y.data; p.out = (void *)b.out.data; p.h = (void *)b.h.data;
+  p.ldx = b.x.ld; p.ldy = b.y.ld; p.ldo = b.out.ld; p.ldh = b.h.ld;
+  p.x_dtype = b.x.dtype; p.y_dtype = b.y.dtype; p.out_dtype = b.out.dtype; p.h_dtype = b.h.dtype;
+  p.rows = rows; p.cols = cols; p.places = b.places; p.weights = b.weights; p.top_k = b.top_k;
+  p.y_rows = b.y_rows; p.gate = b.gate; p.ldg = b.ldg; p.gate_dtype = b.gate_dtype;
+  p.gate_rows = b.gate_rows; p.cu = b.cu_seqlens; p.seq = b.seq;
+  p.x_scale = b.x_scale; p.y_scale = b.y_scale;
+  const TxNorm *norms[2] = {&b.after, &b.before};
+  tx::BlockNorm *to[2] = {&p.after, &p.before};
+  for (int i = 0; i < 2; ++i)
+    *to[i] = {norms[i]->kind, norms[i]->dtype, norms[i]->weight, norms[i]->bias, norms[i]->eps,
+              norms[i]->offset};
+  p.status = c->status;
+  cudaError_t e = cudaSetDevice(c->device);
+  if (e != cudaSuccess) return cuda_fail(c, e, "cudaSetDevice");
+  e = tx::launch_block_norm(p, stream ? (cudaStream_t)stream : c->stream);
+  if (e != cudaSuccess) return cuda_fail(c, e, "block_norm launch");
+  c->last_kernel = "block_norm";
   ++c->launches;
   return TX_OK;
 }

@@ -17,7 +17,7 @@ from typing import Any
 
 from .errors import NativeBuildError
 
-ABI_VERSION = 11
+ABI_VERSION = 12
 LIBRARY_NAME = "libtessattn.so"
 
 TX_OK, TX_EINVAL, TX_ECUDA, TX_ETIMEOUT = 0, 1, 2, 3
@@ -25,6 +25,8 @@ TX_F32, TX_BF16, TX_BF16X2 = 0, 1, 2
 TX_LINEAR_STORE_F32, TX_LINEAR_STORE_BF16, TX_LINEAR_ADD_F32, TX_LINEAR_GATED_BF16 = 0, 1, 2, 3
 TX_LINEAR_GELU_SPLIT = 4
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}  # TX_ACT_*
+SCORES = {"softmax": 0, "sigmoid": 1}  # TX_SCORES_*
+NORMS = {"rms": 1, "layer": 2}  # TX_NORM_*
 
 _vp, _u32, _u64, _i32, _f32 = ct.c_void_p, ct.c_uint32, ct.c_uint64, ct.c_int, ct.c_float
 
@@ -75,6 +77,9 @@ TX_ROTARY_TENSOR = struct.Struct("QQQQQQQI4x")  # x, out, four strides, norm_w, 
 TX_ROWS = struct.Struct("9Q")  # [3]: data, row_stride, head_stride
 TX_LAYOUTS = struct.Struct("QQIIQQII")  # [2]: cu, lengths, rows, max_len
 TX_SCORE_RULE = struct.Struct("f4xQQIiiiQQQ")  # softcap .. k_docs, in their order
+TX_ROUTE = struct.Struct("QQiiQIIIifIQQQQQQ")  # logits .. places, in their order
+# x, y, out, h; places .. y_scale; the norms after and before
+TX_BLOCK_NORM = struct.Struct("QQi4x" * 4 + "QQIIQQiIQIff4x" + "QQiiff" * 2)
 
 
 SIGNATURES: dict[str, tuple[list[Any], Any]] = {
@@ -156,6 +161,14 @@ SIGNATURES: dict[str, tuple[list[Any], Any]] = {
     "tx_rotary": (
         [_vp, ct.c_char_p, ct.c_char_p, _i32, _i32, _u32, _u32,
          _u32, _i32, _i32, _vp, _vp, _u32, _u32, _vp, _f32, _f32, _vp], _i32),
+    "tx_rotary_axes": (
+        [_vp, ct.c_char_p, ct.c_char_p, _i32, _i32, _u32, _u32, _u32, _i32, _i32, _vp, _u64, _u32,
+         _vp, _vp, _f32, _f32, _vp], _i32),
+    "tx_experts_route": ([_vp, ct.c_char_p, _u32, _u32, _u32, _vp], _i32),
+    "tx_experts_linear": (
+        [_vp, _vp, _u64, _u32, _vp, _u64, _u64, _vp, _vp, _i32, _u64, _vp, _vp, _u32, _u32, _u32,
+         _u32, _u32, _i32, _i32, _vp], _i32),
+    "tx_block_norm": ([_vp, ct.c_char_p, _u32, _u32, _vp], _i32),
     "tx_attention_scored": (
         [_vp, ct.c_char_p, _vp, ct.c_char_p, _u32, _u32, _u32, _u32, _i32, _i32, _f32, ct.c_char_p,
          _vp], _i32),

@@ -13,7 +13,7 @@ from __future__ import annotations
 import ctypes as ct
 import threading
 from collections import Counter
-from collections.abc import Iterator, Sequence
+from collections.abc import Iterator, Mapping, Sequence
 from contextlib import contextmanager
 from typing import Any
 from weakref import WeakSet
@@ -50,6 +50,7 @@ def _raise_for(rc: int) -> None:
 
 
 _F32_MAX = 3.4028234663852886e38
+_NORM_KEYS = frozenset(("kind", "weight", "bias", "dtype", "eps", "offset"))
 
 
 # The C calls take counts as 32 bits and strides as 64, and ctypes would wrap what lies outside: each
@@ -63,6 +64,19 @@ def _check_counts(values: int) -> None:
 def _check_strides(values: int) -> None:
     if values >> 63:
         raise InvalidInputError()
+
+
+def _norm_fields(norm: Mapping[str, Any] | None) -> tuple:
+    """weight, bias, kind, dtype, eps, offset of a norm as TxNorm has them."""
+    if norm is None:
+        return 0, 0, 0, 0, 0.0, 0.0
+    kind = native.NORMS.get(norm.get("kind"))
+    eps, offset = norm.get("eps", 1e-6), norm.get("offset", 0.0)
+    if (kind is None or not norm.keys() <= _NORM_KEYS
+            or max(abs(eps), abs(offset)) > _F32_MAX):
+        raise InvalidInputError()
+    return (norm.get("weight") or 0, norm.get("bias") or 0, kind, norm.get("dtype", native.TX_F32),
+            eps, offset)
 
 
 class Buffer:
@@ -724,6 +738,15 @@ class CudaRuntime:
                                              workspace, workspace_bytes, stream))
 
     # ---- encoder layers with other options (device pointers) ----------------------------
+    @staticmethod
+    def _rotary_side(x, out, n, dim, xs, os, weight) -> bytes:
+        xt, xh = (n * dim, dim) if xs is None else xs
+        ot, oh = (n * dim, dim) if os is None else os
+        _check_strides(xt | xh | ot | oh)
+        if not x or not out:
+            raise InvalidInputError()
+        return native.TX_ROTARY_TENSOR.pack(x, out, xt, xh, ot, oh, weight or 0, n)
+
     def rotary_device(
         self,
         q: int,
@@ -762,18 +785,9 @@ class CudaRuntime:
         self._check_open()
         rot = dim if rot_dim is None else rot_dim
         _check_counts(tokens | heads | kv_heads | dim | rot | nseq | seq)
-
-        def side(x, out, n, xs, os, weight):
-            xt, xh = (n * dim, dim) if xs is None else xs
-            ot, oh = (n * dim, dim) if os is None else os
-            _check_strides(xt | xh | ot | oh)
-            if not x or not out:
-                raise InvalidInputError()
-            return native.TX_ROTARY_TENSOR.pack(x, out, xt, xh, ot, oh, weight or 0, n)
-
-        qt = side(q, q_out, heads, q_strides, q_out_strides, q_norm_weight)
-        kt = None if k is None else side(k, k_out, kv_heads, k_strides, k_out_strides,
-                                         k_norm_weight)
+        qt = self._rotary_side(q, q_out, heads, dim, q_strides, q_out_strides, q_norm_weight)
+        kt = None if k is None else self._rotary_side(k, k_out, kv_heads, dim, k_strides,
+                                                      k_out_strides, k_norm_weight)
         _raise_for(self._lib.tx_rotary(
             self._pointer, qt, kt, in_dtype, out_dtype, tokens, dim, rot,
             1 if interleaved else 0, 1 if inverse else 0, positions, cu_seqlens, nseq, seq, inv_freq,
@@ -877,6 +891,200 @@ class CudaRuntime:
         _raise_for(self._lib.tx_linear_fused(
             self._pointer, x, ldx, w, ldw, bias, residual, residual_dtype, ldr, out, out_dtype, ldo,
             m, n, k, act, stream))
+
+    # ---- layers of experts, norms on both sides, positions with several axes ------------------
+    def rotary_axes_device(
+        self,
+        q: int,
+        k: int | None,
+        q_out: int,
+        k_out: int | None,
+        *,
+        tokens: int,
+        heads: int,
+        kv_heads: int = 0,
+        dim: int,
+        inv_freq: int,
+        pair_axes: int,
+        positions: int,
+        axes: int,
+        axis_stride: int | None = None,
+        rot_dim: int | None = None,
+        interleaved: bool = False,
+        inverse: bool = False,
+        amplitude: float = 1.0,
+        q_norm_weight: int | None = None,
+        k_norm_weight: int | None = None,
+        eps: float = 1e-6,
+        in_dtype: int = native.TX_BF16,
+        out_dtype: int = native.TX_BF16,
+        q_strides: Sequence[int] | None = None,
+        k_strides: Sequence[int] | None = None,
+        q_out_strides: Sequence[int] | None = None,
+        k_out_strides: Sequence[int] | None = None,
+        stream: int | None = None,
+    ) -> None:
+        """rotary_device for tokens with a position on each of several axes (tx_rotary_axes):
+        `positions` device int32 [axes, axis_stride] (axis_stride: tokens by default), negative
+        ones among them, and `pair_axes` device int32 [rot_dim / 2] the axis each pair of columns
+        turns by (layers.rotary_pair_axes)."""
+        self._check_open()
+        rot = dim if rot_dim is None else rot_dim
+        stride = tokens if axis_stride is None else axis_stride
+        _check_counts(tokens | heads | kv_heads | dim | rot | axes)
+        _check_strides(stride)
+        qt = self._rotary_side(q, q_out, heads, dim, q_strides, q_out_strides, q_norm_weight)
+        kt = None if k is None else self._rotary_side(k, k_out, kv_heads, dim, k_strides,
+                                                      k_out_strides, k_norm_weight)
+        _raise_for(self._lib.tx_rotary_axes(
+            self._pointer, qt, kt, in_dtype, out_dtype, tokens, dim, rot, 1 if interleaved else 0,
+            1 if inverse else 0, positions, stride, axes, pair_axes, inv_freq, amplitude, eps,
+            stream))
+
+    def experts_route_device(
+        self,
+        logits: int,
+        experts: int,
+        weights: int,
+        *,
+        tokens: int,
+        num_experts: int,
+        top_k: int,
+        ld: int | None = None,
+        logits_dtype: int = native.TX_F32,
+        bias: int | None = None,
+        scores: str = "softmax",
+        groups: int = 1,
+        top_groups: int = 1,
+        group_best: int = 2,
+        renormalise: bool = True,
+        scale: float = 1.0,
+        lengths: int | None = None,
+        seq: int = 0,
+        offsets: int | None = None,
+        order: int | None = None,
+        places: int | None = None,
+        stream: int | None = None,
+    ) -> None:
+        """Queues the routing of tokens to experts (tx_experts_route): `experts` int32 and
+        `weights` fp32 [tokens, top_k] from the logits [tokens, num_experts], by softmax or sigmoid
+        scores, with a bias for the choice, groups, renormalised and scaled weights, and padded
+        rows (lengths of sequences of `seq` rows) left out.  With offsets [num_experts + 1], order
+        [tokens * top_k] and places [tokens, top_k] (int32, all three or none) it also plans the
+        rows of experts_linear_device."""
+        self._check_open()
+        by = native.SCORES.get(scores)
+        ld = num_experts if ld is None else ld
+        _check_counts(tokens | num_experts | top_k | groups | top_groups | group_best | seq)
+        _check_strides(ld)
+        if by is None or abs(scale) > _F32_MAX or not (logits and experts and weights):
+            raise InvalidInputError()
+        _raise_for(self._lib.tx_experts_route(
+            self._pointer,
+            native.TX_ROUTE.pack(logits, ld, logits_dtype, by, bias or 0, groups, top_groups,
+                                 group_best, 1 if renormalise else 0, scale, seq, lengths or 0,
+                                 experts, weights, offsets or 0, order or 0, places or 0),
+            tokens, num_experts, top_k, stream))
+
+    def experts_linear_device(
+        self,
+        x: int,
+        w: int,
+        out: int,
+        *,
+        offsets: int,
+        tokens: int,
+        top_k: int,
+        num_experts: int,
+        n: int,
+        k: int,
+        order: int | None = None,
+        gated: bool = False,
+        activation: str = "none",
+        bias: int | None = None,
+        ldx: int | None = None,
+        ldw: int | None = None,
+        expert_stride: int | None = None,
+        ldo: int | None = None,
+        out_dtype: int = native.TX_BF16,
+        stream: int | None = None,
+    ) -> None:
+        """Queues the experts' products (tx_experts_linear) over the tokens * top_k rows that
+        experts_route_device planned: out[r] = act(x[i] w_e^T + bias_e), or gated, act of the first
+        n rows of w_e times the other n.  With `order`, x is [tokens, k] and i the row's token;
+        without, x is [tokens * top_k, k], by expert like out.  w [num_experts, n or 2 n, k] bf16
+        with strides expert_stride and ldw."""
+        self._check_open()
+        act = native.ACTIVATIONS.get(activation)
+        wide = 2 * n if gated else n
+        ldx, ldw = k if ldx is None else ldx, k if ldw is None else ldw
+        expert_stride = wide * ldw if expert_stride is None else expert_stride
+        ldo = n if ldo is None else ldo
+        _check_counts(tokens | top_k | num_experts | n | k)
+        _check_strides(ldx | ldw | expert_stride | ldo)
+        rows = tokens * top_k
+        _check_counts(rows)
+        if act is None:
+            raise InvalidInputError()
+        _raise_for(self._lib.tx_experts_linear(
+            self._pointer, x, ldx, rows if order is None else tokens, w, ldw, expert_stride, bias,
+            out, out_dtype, ldo, offsets, order, rows, num_experts, top_k, n, k, 1 if gated else 0,
+            act, stream))
+
+    def block_norm_device(
+        self,
+        x: int | None,
+        y: int | None,
+        *,
+        rows: int,
+        cols: int,
+        out: int | None = None,
+        h: int | None = None,
+        x_dtype: int = native.TX_F32,
+        y_dtype: int = native.TX_BF16,
+        out_dtype: int = native.TX_F32,
+        h_dtype: int = native.TX_BF16,
+        after: Mapping[str, Any] | None = None,
+        before: Mapping[str, Any] | None = None,
+        x_scale: float = 1.0,
+        y_scale: float = 1.0,
+        gate: int | None = None,
+        gate_dtype: int = native.TX_F32,
+        gate_rows: int = 1,
+        cu_seqlens: int | None = None,
+        seq: int = 0,
+        places: int | None = None,
+        weights: int | None = None,
+        top_k: int = 0,
+        y_rows: int = 0,
+        ldx: int | None = None,
+        ldy: int | None = None,
+        ldo: int | None = None,
+        ldh: int | None = None,
+        ldg: int | None = None,
+        stream: int | None = None,
+    ) -> None:
+        """Queues the rows between two blocks (tx_block_norm): out = x_scale x + y_scale gate *
+        after(y) and h = before(out); x or y, and out or h, may be None.  A norm is a mapping with
+        `kind` ("rms" or "layer"), `weight` and `bias` (device addresses of [cols] of `dtype`, fp32
+        by default; None: 1 and 0), `eps` and `offset` (added to the weight).  With places and
+        weights [rows, top_k] (experts_route_device), y holds y_rows experts' rows and is joined
+        first.  gate [gate_rows, cols]: one row for all, or one for each packed sequence
+        (cu_seqlens) or for every `seq` rows."""
+        self._check_open()
+        ldx, ldy, ldo, ldh, ldg = (cols if ld is None else ld for ld in (ldx, ldy, ldo, ldh, ldg))
+        _check_counts(rows | cols | gate_rows | seq | top_k | y_rows)
+        _check_strides(ldx | ldy | ldo | ldh | ldg)
+        if max(abs(x_scale), abs(y_scale)) > _F32_MAX:
+            raise InvalidInputError()
+        _raise_for(self._lib.tx_block_norm(
+            self._pointer,
+            native.TX_BLOCK_NORM.pack(
+                x or 0, ldx, x_dtype, y or 0, ldy, y_dtype, out or 0, ldo, out_dtype, h or 0, ldh,
+                h_dtype, places or 0, weights or 0, top_k, y_rows, gate or 0, ldg, gate_dtype,
+                gate_rows, cu_seqlens or 0, seq, x_scale, y_scale, *_norm_fields(after),
+                *_norm_fields(before)),
+            rows, cols, stream))
 
     def sync(self, stream: int | None = None) -> None:
         """Waits for queued work and reports kernel errors (tx_sync)."""
