@@ -3,9 +3,15 @@
 // e the expert whose range offsets[e] .. offsets[e + 1] - 1 holds r, row(r) = order[r] / top_k or r.
 //
 // 128 x BN tiles on tcgen05 as in linear_fused.cu: one tile is up to 128 rows of one expert, and with the
-// ranges known on the device alone each CTA counts the tiles of every expert first.  The rows of x come by
-// TMA gathers of four rows, as many as the tile has, so nothing is sorted into memory first; a gated tile
-// holds BN / 2 gate columns and the same up columns side by side in tensor memory.
+// ranges known on the device alone each CTA counts the tiles of every expert first.  Rows of x that do not
+// lie by expert are gathered by four warps with 16-byte asynchronous copies into the layout that TMA
+// writes, so nothing is sorted into memory first.  (TMA gathers of four rows took 80 cycles each, 2600 a
+// stage where the products take 512: 336 against 138 us for the largest case.)  A gated tile holds BN / 2
+// gate columns and the same up columns side by side in tensor memory.
+// pair_kernel: 256 x 256 tiles by two CTAs, for calls of many rows.
+//
+// Measured: 65536 rows over 64 experts, gated, n 512, k 1024, gathered: 118 us, 1160 TFLOP/s (128 x 256
+// tiles: 121 us); n 1024, k 512, rows by expert: 68 us, 1010 TFLOP/s and 3.9 TB/s (78 us).
 #include <cuda.h>
 
 #include <algorithm>
@@ -24,20 +30,23 @@ using namespace lfused;
 
 constexpr int kBM = 128;
 constexpr uint32_t kBK = 64;
-constexpr int kThreads = 320;  // warp 0 TMA, warp 1 MMA, warps 2-9 epilogue
+// warp 0 TMA, warp 1 MMA, warps 2-9 epilogue, and to gather rows warps 10-13
+constexpr int kThreads = 320, kGatherThreads = 448;
 constexpr int kMaxStages = 8;
 constexpr uint32_t kPart = 8;  // K stages (512 columns) of one partial sum
-constexpr uint32_t kMaxExperts = 1024;
+constexpr uint32_t kBufBytes = 32 * 64;  // staging of an epilogue warp: 32 rows of 64 bytes
 constexpr uint32_t kFull = 0xffffffffu;
 
 template <int kBN>
 struct Cfg {
   static constexpr uint32_t kABytes = kBM * 128, kBBytes = kBN * 128;
   static constexpr uint32_t kStageBytes = kABytes + kBBytes;
+  static constexpr uint32_t kMaxExperts = 1024;
   static constexpr uint32_t kTables = 2 * (kMaxExperts + 1) * 4;
-  static constexpr int kFit = (int)((232448 - 1024 - 512 - kTables) / kStageBytes);
+  static constexpr int kFit = (int)((232448 - 512 - kTables - 8 * kBufBytes) / kStageBytes);
   static constexpr int kStages = kFit < kMaxStages ? kFit : kMaxStages;
-  static constexpr uint32_t kOffMisc = kStages * kStageBytes;
+  static constexpr uint32_t kOffStaging = kStages * kStageBytes;
+  static constexpr uint32_t kOffMisc = kOffStaging + 8 * kBufBytes;
   static constexpr uint32_t kOffTables = kOffMisc + 512;
   static constexpr uint32_t kSmemBytes = kOffTables + kTables;
   static constexpr uint32_t kTmemCols = 2 * kBN;
@@ -50,19 +59,78 @@ enum : uint32_t { kOffTmem = 8 * kNumBars, kOffAbort = kOffTmem + 4 };
 static_assert(kOffAbort + 4 <= 512, "misc area");
 enum : int { kSiteEmpty = 1, kSiteFull = 2, kSiteAcc = 3, kSiteFree = 4 };
 
-// Columns x .. x + 63 of four rows, 512 bytes in the 128-byte swizzle.
-__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x,
-                                            const int (&r)[4]) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(r[0]), "r"(r[1]), "r"(r[2]),
-      "r"(r[3])
-      : "memory");
+// wait_bar by a whole warp, with one answer.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag,
+                                          const ExpertsProblem &p, int site) {
+  return __all_sync(kFull, wait_bar(bar, parity, abort_flag, p.status, site, p.wait_cycles));
+}
+// 16 bytes from global to shared memory, of which the first `bytes` are read and the others zeros.
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+               : "memory");
+}
+// Arrives at `bar` when this thread's copies so far have landed.  (The barrier counts every such arrival;
+// who waits for it makes the copies visible to the tensor core with fence_proxy_async.)
+__device__ __forceinline__ void copies_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-// The tables of a launch: start[e] is offsets[e] cut to 0 .. rows and never falling, tiles[e] the row
-// tiles of the experts before e.  One warp fills them.
+// The rows that four warps gather for a tile.  Eight lanes copy a row's 128 bytes of a stage, a warp 32 rows
+// in eight steps, into the 128-byte swizzle.  A tile's entries of `order` are fetched while the tile before
+// it is copied: waiting for them at its start took 3400 cycles, more than the stages ahead last.
+struct Gather {
+  const uint16_t *from[8];
+  int32_t pair[8];
+  uint32_t first, chunk, rows, next_rows;
+  // warp: 0 .. 3
+  __device__ __forceinline__ explicit Gather(uint32_t warp) {
+    const uint32_t lane = threadIdx.x & 31;
+    first = warp * 32 + lane / 8;
+    chunk = lane % 8;
+    next_rows = 0;
+  }
+  // The next tile's first row here is r0, and `tile_rows` rows of it exist.
+  __device__ __forceinline__ void fetch(const ExpertsProblem &p, uint32_t r0, uint32_t tile_rows) {
+    next_rows = tile_rows;
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i)
+      pair[i] = first + i * 4 < tile_rows ? __ldg(p.order + r0 + first + i * 4) : 0;
+  }
+  // Turns to the tile fetched last.
+  __device__ __forceinline__ void turn(const ExpertsProblem &p) {
+    rows = next_rows;
+    const uint16_t *x = static_cast<const uint16_t *>(p.x) + chunk * 8;
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+      // pair / top_k by the reciprocal floor(2^32 / top_k) + 1, which is one too much at most.
+      uint32_t at = p.top_k > 1 ? __umulhi((uint32_t)pair[i], p.top_k_inv) : (uint32_t)pair[i];
+      if (at * p.top_k > (uint32_t)pair[i]) --at;
+      if (at >= p.x_rows) {
+        report_status(p.status, kStatusBadArg);
+        at = p.x_rows - 1;
+      }
+      from[i] = x + (size_t)at * p.ldx;
+    }
+  }
+  // Columns kb * kBK .. + kBK - 1, those past k as zeros.
+  __device__ __forceinline__ void stage(const ExpertsProblem &p, uint32_t dst, uint32_t kb) const {
+    const uint32_t col = kb * kBK + chunk * 8;
+    const uint32_t bytes = col < p.k ? min((p.k - col) * 2, 16u) : 0;
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+      const uint32_t r = first + i * 4;
+      if (r < rows)
+        copy16(dst + r * 128 + ((chunk ^ (r & 7)) << 4), bytes ? from[i] + kb * kBK : from[i], bytes);
+    }
+  }
+};
+
+// The tables of a launch: start[e] is offsets[e] cut to 0 .. rows and never falling, tiles[e] the tiles
+// of kRows rows of the experts before e.  One warp fills them.
+template <uint32_t kRows>
 __device__ __forceinline__ void fill_tables(const ExpertsProblem &p, uint32_t *start, uint32_t *tiles) {
   const uint32_t lane = threadIdx.x & 31;
   uint32_t edge = 0, count = 0;
@@ -79,7 +147,7 @@ __device__ __forceinline__ void fill_tables(const ExpertsProblem &p, uint32_t *s
     if (e <= p.experts && v != (uint32_t)raw) report_status(p.status, kStatusBadArg);
     uint32_t before = __shfl_up_sync(kFull, v, 1);
     if (lane == 0) before = e0 ? edge : v;
-    uint32_t n = e <= p.experts ? (v - before + kBM - 1) / kBM : 0;  // tiles of expert e - 1
+    uint32_t n = e <= p.experts ? (v - before + kRows - 1) / kRows : 0;  // tiles of expert e - 1
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const uint32_t u = __shfl_up_sync(kFull, n, o);
@@ -123,9 +191,106 @@ __device__ __forceinline__ void activate_all(float (&v)[kN], int act) {
   }
 }
 
+// What an epilogue warp finishes: rows r0 + lane of the output, of which the first `rows` exist.
+struct Finish {
+  uint32_t r0, rows, staging;
+  const float *bias;  // of the tile's expert, or NULL
+};
+// Stores 32 staged rows of kPieces 16-byte pieces (elements of kSize bytes) from column n on.
+template <uint32_t kSize, uint32_t kPieces>
+__device__ __forceinline__ void store_staged(const ExpertsProblem &p, const Finish &f, uint32_t n) {
+  constexpr uint32_t kEach = 16 / kSize;
+  const uint32_t lane = threadIdx.x & 31, piece = lane & 3, col = n + piece * kEach;
+  if (piece >= kPieces || col >= p.n) return;
+  uint8_t *to = static_cast<uint8_t *>(p.out) + ((size_t)f.r0 * p.ldo + col) * kSize;
+  const bool whole = col + kEach <= p.n;
+#pragma unroll
+  for (uint32_t r = lane >> 2; r < 32; r += 8) {
+    if (r >= f.rows) break;
+    const uint4 o = ld_shared_v4(f.staging + r * 64 + ((piece ^ ((r >> 1) & 3)) << 4));
+    uint8_t *at = to + (size_t)r * p.ldo * kSize;
+    if (whole) {
+      *reinterpret_cast<uint4 *>(at) = o;
+    } else {
+      for (uint32_t t = 0; col + t < p.n; ++t) {
+        if constexpr (kSize == 4)
+          reinterpret_cast<uint32_t *>(at)[t] = u4_at(o, t);
+        else
+          reinterpret_cast<uint16_t *>(at)[t] = (uint16_t)(u4_at(o, t / 2) >> (16 * (t & 1)));
+      }
+    }
+  }
+}
+// Bias, activation, gate and store of columns n .. n + kStep - 1 of 32 rows, one a lane; u is the up half.
+// The whole warp calls it.
+template <bool kGated, uint32_t kStep>
+__device__ __forceinline__ void finish_columns(const ExpertsProblem &p, const Finish &f, uint32_t n,
+                                               float (&v)[kStep], float (&u)[kGated ? kStep : 1]) {
+  if (!f.rows || n >= p.n) return;
+  const uint32_t lane = threadIdx.x & 31;
+  if (f.bias) {
+    const bool whole = n + kStep <= p.n;
+#pragma unroll
+    for (uint32_t t = 0; t < kStep; ++t)
+      if (whole || n + t < p.n) {
+        v[t] += __ldg(f.bias + n + t);
+        if constexpr (kGated) u[t] += __ldg(f.bias + p.n + n + t);
+      }
+  }
+  activate_all(v, p.act);
+  if constexpr (kGated) {
+#pragma unroll
+    for (uint32_t t = 0; t < kStep; ++t) v[t] *= u[t];
+  }
+  if (p.out_vec) {
+    // Through shared memory, so that a warp stores rows of 64 bytes.  The 16-byte pieces of a row are
+    // swapped so that neither side meets a bank twice.
+    const uint32_t sw = (lane >> 1) & 3, mine = f.staging + lane * 64;
+    if (p.out_dtype == TX_F32) {
+#pragma unroll
+      for (uint32_t h = 0; h < kStep; h += 16) {
+        __syncwarp();
+#pragma unroll
+        for (uint32_t q = 0; q < 4; ++q)
+          st_shared_v4(mine + ((q ^ sw) << 4), __float_as_uint(v[h + 4 * q]),
+                       __float_as_uint(v[h + 4 * q + 1]), __float_as_uint(v[h + 4 * q + 2]),
+                       __float_as_uint(v[h + 4 * q + 3]));
+        __syncwarp();
+        store_staged<4, 4>(p, f, n + h);
+      }
+    } else {
+      __syncwarp();
+#pragma unroll
+      for (uint32_t q = 0; q < kStep / 8; ++q)
+        st_shared_v4(mine + ((q ^ sw) << 4), pack_bf16x2(v[8 * q], v[8 * q + 1]),
+                     pack_bf16x2(v[8 * q + 2], v[8 * q + 3]), pack_bf16x2(v[8 * q + 4], v[8 * q + 5]),
+                     pack_bf16x2(v[8 * q + 6], v[8 * q + 7]));
+      __syncwarp();
+      store_staged<2, kStep / 8>(p, f, n);
+    }
+  } else if (lane < f.rows) {
+    const size_t at = (size_t)(f.r0 + lane) * p.ldo + n;
+#pragma unroll
+    for (uint32_t t = 0; t < kStep; ++t)
+      if (n + t < p.n) {
+        if (p.out_dtype == TX_F32)
+          static_cast<float *>(p.out)[at + t] = v[t];
+        else
+          static_cast<uint16_t *>(p.out)[at + t] = f32_to_bf16_bits(v[t]);
+      }
+  }
+}
+template <uint32_t kStep>
+__device__ __forceinline__ void load_columns(uint32_t at, float (&v)[kStep]) {
+  uint32_t a[kStep];
+  tmem_load(at, a);
+#pragma unroll
+  for (uint32_t t = 0; t < kStep; ++t) v[t] = __uint_as_float(a[t]);
+}
+
 // kLong: the sum is taken in parts of 512 K that are added in fp32 registers.
-template <int kBN, bool kGated, bool kLong>
-__global__ void __launch_bounds__(kThreads, 1)
+template <int kBN, bool kGated, bool kLong, bool kGather>
+__global__ void __launch_bounds__(kGather ? kGatherThreads : kThreads, 1)
     experts_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                    const __grid_constant__ ExpertsProblem p) {
   using C = Cfg<kBN>;
@@ -135,12 +300,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto bar = [&](uint32_t i) { return bars + 8u * i; };
   volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + C::kOffMisc + kOffAbort);
   uint32_t *start = reinterpret_cast<uint32_t *>(smem + C::kOffTables);
-  uint32_t *tiles = start + kMaxExperts + 1;
+  uint32_t *tiles = start + C::kMaxExperts + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(bar(kBarFull + s), 1);
+      mbar_init(bar(kBarFull + s), kGather ? 129 : 1);  // the TMA copies, and each gathering thread
       mbar_init(bar(kBarEmpty + s), 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -158,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  if (warp == 2) fill_tables(p, start, tiles);
+  if (warp == 2) fill_tables<kBM>(p, start, tiles);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -172,145 +337,104 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (uint32_t tile = blockIdx.x; ok && tile < total; tile += gridDim.x) {
       const uint32_t mt = tile / nt;
       e = expert_of(tiles, p.experts, mt, e);
-      const uint32_t r0 = start[e] + (mt - tiles[e]) * kBM, rows = min(start[e + 1] - r0, (uint32_t)kBM);
-      const int n0 = (int)(tile % nt * kOut);
-      const uint32_t gathers = (rows + 3) / 4;
-      int row[4];  // the rows that this lane gathers; past the tile's last its last again
-#pragma unroll
-      for (uint32_t i = 0; i < 4; ++i) {
-        const uint32_t r = r0 + min((uint32_t)lane * 4 + i, rows - 1);
-        row[i] = (int)r;
-        if (p.order) {
-          const uint32_t at = (uint32_t)__ldg(p.order + r) / p.top_k;
-          if (at >= p.x_rows) report_status(p.status, kStatusBadArg);
-          row[i] = (int)min(at, p.x_rows - 1);
-        }
-      }
+      const int r0 = (int)(start[e] + (mt - tiles[e]) * kBM), n0 = (int)(tile % nt * kOut);
       for (uint32_t kb = 0; kb < nk; ++kb) {
         const uint32_t s = fills % C::kStages, round = fills / C::kStages;
-        if (round && !(ok = wait_bar(bar(kBarEmpty + s), (round - 1) & 1, abort_flag, p.status,
-                                     kSiteEmpty, p.wait_cycles)))
+        if (round &&
+            !(ok = warp_wait(bar(kBarEmpty + s), (round - 1) & 1, abort_flag, p, kSiteEmpty)))
           break;
-        const uint32_t dst = sbase + s * C::kStageBytes;
-        if (lane == 0) {
-          mbar_expect_tx(bar(kBarFull + s), gathers * 512 + C::kBBytes);
-          if constexpr (kGated) {
-            tma_load_3d(dst + C::kABytes, &tm_w, bar(kBarFull + s), (int)(kb * kBK), n0, (int)e);
-            tma_load_3d(dst + C::kABytes + C::kBBytes / 2, &tm_w, bar(kBarFull + s), (int)(kb * kBK),
+        const uint32_t dst = sbase + s * C::kStageBytes, x = kb * kBK;
+        if (elect_one()) {
+          mbar_expect_tx(bar(kBarFull + s), kGather ? C::kBBytes : C::kStageBytes);
+          if constexpr (!kGather) tma_load_2d(dst, &tm_x, bar(kBarFull + s), (int)x, r0);
+          tma_load_3d(dst + C::kABytes, &tm_w, bar(kBarFull + s), (int)x, n0, (int)e);
+          if constexpr (kGated)
+            tma_load_3d(dst + C::kABytes + C::kBBytes / 2, &tm_w, bar(kBarFull + s), (int)x,
                         (int)p.n + n0, (int)e);
-          } else {
-            tma_load_3d(dst + C::kABytes, &tm_w, bar(kBarFull + s), (int)(kb * kBK), n0, (int)e);
-          }
         }
         __syncwarp();
-        if ((uint32_t)lane < gathers)
-          tma_gather4(dst + (uint32_t)lane * 512, &tm_x, bar(kBarFull + s), (int)(kb * kBK), row);
         ++fills;
       }
-      ok = __all_sync(kFull, ok);
     }
     // No copy may land after the CTA has gone.
     if (lane == 0)
       for (uint32_t s = 0; s < (uint32_t)C::kStages && s < fills; ++s)
         drain_bar(bar(kBarFull + s), ((fills - 1 - s) / C::kStages) & 1);
     __syncwarp();
+  } else if (kGather && warp >= 10) {
+    uint32_t fills = 0, e = 0;
+    bool ok = true;
+    Gather rows((uint32_t)warp - 10);
+    auto fetch = [&](uint32_t tile) {
+      if (tile >= total) return;
+      e = expert_of(tiles, p.experts, tile / nt, e);
+      const uint32_t r0 = start[e] + (tile / nt - tiles[e]) * kBM;
+      rows.fetch(p, r0, min(start[e + 1] - r0, (uint32_t)kBM));
+    };
+    fetch(blockIdx.x);
+    for (uint32_t tile = blockIdx.x; ok && tile < total; tile += gridDim.x) {
+      rows.turn(p);
+      fetch(tile + gridDim.x);
+      for (uint32_t kb = 0; kb < nk; ++kb) {
+        const uint32_t s = fills % C::kStages, round = fills / C::kStages;
+        if (round &&
+            !(ok = warp_wait(bar(kBarEmpty + s), (round - 1) & 1, abort_flag, p, kSiteEmpty)))
+          break;
+        rows.stage(p, sbase + s * C::kStageBytes, kb);
+        copies_arrive(bar(kBarFull + s));
+        ++fills;
+      }
+    }
+    copies_wait();
   } else if (warp == 1) {
-    if (lane == 0) {
-      uint32_t step = 0, done = 0;  // K stages, partial sums
-      bool ok = true;
-      for (uint32_t tile = blockIdx.x; ok && tile < total; tile += gridDim.x) {
-        for (uint32_t kb = 0; ok && kb < nk; ++done) {
-          const uint32_t b = done & 1, acc = tmem + b * kBN;
-          if (done >= 2 && !(ok = wait_bar(bar(kBarFree + b), ((done >> 1) - 1) & 1, abort_flag,
-                                           p.status, kSiteFree, p.wait_cycles)))
+    uint32_t step = 0, done = 0;  // K stages, partial sums
+    bool ok = true;
+    for (uint32_t tile = blockIdx.x; ok && tile < total; tile += gridDim.x) {
+      for (uint32_t kb = 0; ok && kb < nk; ++done) {
+        const uint32_t b = done & 1, acc = tmem + b * kBN;
+        if (done >= 2 &&
+            !(ok = warp_wait(bar(kBarFree + b), ((done >> 1) - 1) & 1, abort_flag, p, kSiteFree)))
+          break;
+        tc_fence_after();
+        const uint32_t end = kLong ? min(kb + kPart, nk) : nk;
+        for (uint32_t first = kb; kb < end; ++kb, ++step) {
+          const uint32_t s = step % C::kStages;
+          if (!(ok = warp_wait(bar(kBarFull + s), (step / C::kStages) & 1, abort_flag, p, kSiteFull)))
             break;
+          if constexpr (kGather) fence_proxy_async();
           tc_fence_after();
-          const uint32_t end = kLong ? min(kb + kPart, nk) : nk;
-          for (uint32_t first = kb; kb < end; ++kb, ++step) {
-            const uint32_t s = step % C::kStages;
-            if (!(ok = wait_bar(bar(kBarFull + s), (step / C::kStages) & 1, abort_flag, p.status,
-                                kSiteFull, p.wait_cycles)))
-              break;
-            tc_fence_after();
-            const uint32_t st = sbase + s * C::kStageBytes;
-            const uint64_t ad = sw128_desc(st, 16, 1024), bd = sw128_desc(st + C::kABytes, 16, 1024);
+          const uint32_t st = sbase + s * C::kStageBytes;
+          const uint64_t ad = sw128_desc(st, 16, 1024), bd = sw128_desc(st + C::kABytes, 16, 1024);
+          if (elect_one()) {
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks)
               umma(acc, ad + ks * 2, bd + ks * 2, C::kIdesc, kb > first || ks > 0);
             umma_commit(bar(kBarEmpty + s));
           }
-          if (ok) umma_commit(bar(kBarAcc + b));
+          __syncwarp();
         }
+        if (ok && elect_one()) umma_commit(bar(kBarAcc + b));
+        __syncwarp();
       }
-      umma_commit(bar(kBarDrain));
-      drain_bar(bar(kBarDrain), 0);
     }
+    if (elect_one()) umma_commit(bar(kBarDrain));
     __syncwarp();
+    drain_bar(bar(kBarDrain), 0);
   } else {
     // Warp w finishes output columns [half * kCols, +kCols) of the 32 rows of its tensor-memory quarter.
     constexpr uint32_t kCols = kOut / 2, kStep = kCols < 32 ? kCols : 32;
     const uint32_t quarter = (uint32_t)warp & 3, half = (uint32_t)(warp - 2) >> 2;
     const uint32_t lanes = (quarter * 32u) << 16;
-    const bool f32_out = p.out_dtype == TX_F32;
+    const uint32_t staging = sbase + C::kOffStaging + (uint32_t)(warp - 2) * kBufBytes;
     uint32_t done = 0, e = 0;
     bool ok = true;
     for (uint32_t tile = blockIdx.x; ok && tile < total; tile += gridDim.x) {
       const uint32_t mt = tile / nt;
       e = expert_of(tiles, p.experts, mt, e);
       const uint32_t r0 = start[e] + (mt - tiles[e]) * kBM, rows = min(start[e + 1] - r0, (uint32_t)kBM);
-      const uint32_t n0 = tile % nt * kOut + half * kCols, mine = quarter * 32 + lane;
-      const float *bias = p.bias ? p.bias + (size_t)e * (kGated ? 2 : 1) * p.n : nullptr;
-      // Bias, activation, gate and store of columns [c, c + kStep); u is the up half.
-      auto finish = [&](uint32_t c, float (&v)[kStep], float (&u)[kGated ? kStep : 1]) {
-        const uint32_t n = n0 + c;
-        if (mine >= rows || n >= p.n) return;
-        const bool whole = n + kStep <= p.n;
-        if (bias) {
-#pragma unroll
-          for (uint32_t t = 0; t < kStep; ++t)
-            if (whole || n + t < p.n) {
-              v[t] += __ldg(bias + n + t);
-              if constexpr (kGated) u[t] += __ldg(bias + p.n + n + t);
-            }
-        }
-        activate_all(v, p.act);
-        if constexpr (kGated) {
-#pragma unroll
-          for (uint32_t t = 0; t < kStep; ++t) v[t] *= u[t];
-        }
-        const size_t at = (size_t)(r0 + mine) * p.ldo + n;
-        if (whole && p.out_vec && f32_out) {
-#pragma unroll
-          for (uint32_t t = 0; t < kStep / 4; ++t)
-            reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at)[t] =
-                make_float4(v[4 * t], v[4 * t + 1], v[4 * t + 2], v[4 * t + 3]);
-        } else if (whole && p.out_vec) {
-#pragma unroll
-          for (uint32_t t = 0; t < kStep / 8; ++t)
-            reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.out) + at)[t] =
-                make_uint4(pack_bf16x2(v[8 * t], v[8 * t + 1]), pack_bf16x2(v[8 * t + 2], v[8 * t + 3]),
-                           pack_bf16x2(v[8 * t + 4], v[8 * t + 5]),
-                           pack_bf16x2(v[8 * t + 6], v[8 * t + 7]));
-        } else {
-#pragma unroll
-          for (uint32_t t = 0; t < kStep; ++t)
-            if (n + t < p.n) {
-              if (f32_out)
-                static_cast<float *>(p.out)[at + t] = v[t];
-              else
-                static_cast<uint16_t *>(p.out)[at + t] = f32_to_bf16_bits(v[t]);
-            }
-        }
-      };
-      auto load = [&](uint32_t at, float (&v)[kStep]) {
-#pragma unroll
-        for (uint32_t c = 0; c < kStep; c += 16) {
-          uint32_t a[16];
-          tmem_load(at + c, a);
-#pragma unroll
-          for (int t = 0; t < 16; ++t) v[c + t] = __uint_as_float(a[t]);
-        }
-      };
+      const uint32_t n0 = tile % nt * kOut + half * kCols;
+      const Finish f{r0 + quarter * 32, rows > quarter * 32 ? min(rows - quarter * 32, 32u) : 0, staging,
+                     p.bias ? p.bias + (size_t)e * (kGated ? 2 : 1) * p.n : nullptr};
       if constexpr (kLong) {
         constexpr uint32_t kHeld = kCols / kStep;
         float v[kHeld][kStep], u[kGated ? kHeld : 1][kGated ? kStep : 1];
@@ -324,11 +448,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (uint32_t c = 0; c < kHeld; ++c) {
             float a[kStep];
-            load(t0 + c * kStep, a);
+            load_columns<kStep>(t0 + c * kStep, a);
 #pragma unroll
             for (uint32_t t = 0; t < kStep; ++t) v[c][t] = part ? v[c][t] + a[t] : a[t];
             if constexpr (kGated) {
-              load(t0 + kOut + c * kStep, a);
+              load_columns<kStep>(t0 + kOut + c * kStep, a);
 #pragma unroll
               for (uint32_t t = 0; t < kStep; ++t) u[c][t] = part ? u[c][t] + a[t] : a[t];
             }
@@ -338,7 +462,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (!ok) break;
 #pragma unroll
-        for (uint32_t c = 0; c < kHeld; ++c) finish(c * kStep, v[c], u[kGated ? c : 0]);
+        for (uint32_t c = 0; c < kHeld; ++c)
+          finish_columns<kGated, kStep>(p, f, n0 + c * kStep, v[c], u[kGated ? c : 0]);
       } else {
         const uint32_t b = done & 1, t0 = tmem + b * kBN + half * kCols + lanes;
         ok = __all_sync(kFull, wait_bar(bar(kBarAcc + b), (done >> 1) & 1, abort_flag, p.status,
@@ -349,9 +474,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
         for (uint32_t c = 0; c < kCols; c += kStep) {
           float v[kStep], u[kGated ? kStep : 1];
-          load(t0 + c, v);
-          if constexpr (kGated) load(t0 + kOut + c, u);
-          finish(c, v, u);
+          load_columns<kStep>(t0 + c, v);
+          if constexpr (kGated) load_columns<kStep>(t0 + kOut + c, u);
+          finish_columns<kGated, kStep>(p, f, n0 + c, v, u);
           __syncwarp();
         }
         tc_fence_before();
@@ -369,14 +494,227 @@ __global__ void __launch_bounds__(kThreads, 1)
                  : "memory");
 }
 
-// x [rows, k] read one row a box, and w [experts, wide, k] in boxes of box_rows rows; 64 columns of bf16
-// in the 128-byte swizzle.
+// ---- two CTAs a tile ------------------------------------------------------------------------
+// 256 rows x 256 columns of products a tile, by the two CTAs of a cluster (cta_group::2): each brings and
+// holds 128 of the rows and 128 of the columns, so that a stage of 64 K takes 32 KB of shared memory a CTA
+// where the tiles above take 48 KB: with those the way from L2 into shared memory is the bound.
+namespace pair {
+constexpr int kStages = 6;
+constexpr uint32_t kHalfBytes = 128 * 128, kStageBytes = 2 * kHalfBytes;
+constexpr uint32_t kRows = 256, kWide = 256, kMaxExperts = 1024;
+constexpr uint32_t kOffStaging = kStages * kStageBytes, kOffMisc = kOffStaging + 8 * kBufBytes;
+constexpr uint32_t kOffTables = kOffMisc + 512;
+constexpr uint32_t kSmemBytes = kOffTables + 2 * (kMaxExperts + 1) * 4;
+static_assert(kSmemBytes <= 232448, "shared memory");
+constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | ((kWide >> 3) << 17) |
+                            ((kRows >> 4) << 24);
+// kFull: of the even CTA, the copies of both (and the odd one's gathered rows); kGathered: this CTA's.
+enum : uint32_t { kFullBar = 0, kGathered = kStages, kEmpty = 2 * kStages, kAcc = 3 * kStages,
+                  kFree = kAcc + 2, kDrain = kFree + 2, kBars = kDrain + 1 };
+static_assert(8 * kBars + 8 <= 512, "misc area");
+enum : int { kSiteGathered = 5 };
+}  // namespace pair
+
+template <bool kGated, bool kGather>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGather ? kGatherThreads : kThreads, 1)
+    pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
+                const __grid_constant__ ExpertsProblem p) {
+  using namespace pair;
+  constexpr uint32_t kOut = kGated ? kWide / 2 : kWide;  // output columns of a tile
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t sbase = smem_addr(smem), bars = sbase + kOffMisc;
+  auto bar = [&](uint32_t i) { return bars + 8u * i; };
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + kOffMisc + 8 * kBars + 4);
+  uint32_t *start = reinterpret_cast<uint32_t *>(smem + kOffTables);
+  uint32_t *tiles = start + kMaxExperts + 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank(), first_tile = blockIdx.x / 2, tile_step = gridDim.x / 2;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(bar(kFullBar + s), kGather ? 2 : 1);
+      mbar_init(bar(kGathered + s), 128);
+      mbar_init(bar(kEmpty + s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(bar(kAcc + b), 1);
+      mbar_init(bar(kFree + b), 16);  // the epilogue warps of both CTAs
+    }
+    mbar_init(bar(kDrain), 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     bars + 8 * kBars),
+                 "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  if (warp == 2) fill_tables<kRows>(p, start, tiles);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<uint32_t *>(smem + kOffMisc + 8 * kBars);
+  const uint32_t nt = (p.n + kOut - 1) / kOut, total = tiles[p.experts] * nt;
+  const uint32_t nk = (p.k + kBK - 1) / kBK;
+  auto full_at_even = [&](uint32_t s) { return cluster_addr(bar(kFullBar + s), 0); };
+
+  if (warp == 0) {
+    // This CTA's rows (unless gathered) and columns of every stage.
+    uint32_t fills = 0, e = 0;
+    bool ok = true;
+    for (uint32_t tile = first_tile; ok && tile < total; tile += tile_step) {
+      const uint32_t mt = tile / nt;
+      e = expert_of(tiles, p.experts, mt, e);
+      const int r0 = (int)(start[e] + (mt - tiles[e]) * kRows + rank * 128);
+      const int n0 = (int)(tile % nt * kOut + rank * (kGated ? p.n : 128));
+      for (uint32_t kb = 0; kb < nk; ++kb) {
+        const uint32_t s = fills % kStages, round = fills / kStages;
+        if (round && !(ok = warp_wait(bar(kEmpty + s), (round - 1) & 1, abort_flag, p, kSiteEmpty)))
+          break;
+        const uint32_t dst = sbase + s * kStageBytes, full = full_at_even(s);
+        if (elect_one()) {
+          if (rank == 0) mbar_expect_tx(bar(kFullBar + s), (kGather ? 2 : 4) * kHalfBytes);
+          if constexpr (!kGather) tma_load_2d_pair(dst, &tm_x, full, (int)(kb * kBK), r0);
+          tma_load_3d_pair(dst + kHalfBytes, &tm_w, full, (int)(kb * kBK), n0, (int)e);
+        }
+        __syncwarp();
+        ++fills;
+      }
+    }
+    // No copy may land after the CTAs have gone.
+    if (lane == 0 && rank == 0)
+      for (uint32_t s = 0; s < (uint32_t)kStages && s < fills; ++s)
+        drain_bar(bar(kFullBar + s), ((fills - 1 - s) / kStages) & 1);
+    __syncwarp();
+  } else if (kGather && warp >= 10) {
+    uint32_t fills = 0, e = 0;
+    bool ok = true;
+    Gather rows((uint32_t)warp - 10);
+    auto fetch = [&](uint32_t tile) {
+      if (tile >= total) return;
+      e = expert_of(tiles, p.experts, tile / nt, e);
+      const uint32_t r0 = start[e] + (tile / nt - tiles[e]) * kRows + rank * 128;
+      rows.fetch(p, r0, start[e + 1] > r0 ? min(start[e + 1] - r0, 128u) : 0);
+    };
+    fetch(first_tile);
+    for (uint32_t tile = first_tile; ok && tile < total; tile += tile_step) {
+      rows.turn(p);
+      fetch(tile + tile_step);
+      for (uint32_t kb = 0; kb < nk; ++kb) {
+        const uint32_t s = fills % kStages, round = fills / kStages;
+        if (round && !(ok = warp_wait(bar(kEmpty + s), (round - 1) & 1, abort_flag, p, kSiteEmpty)))
+          break;
+        rows.stage(p, sbase + s * kStageBytes, kb);
+        copies_arrive(bar(kGathered + s));
+        ++fills;
+      }
+    }
+    copies_wait();
+  } else if (warp == 1) {
+    if (rank == 0) {
+      uint32_t step = 0, done = 0;
+      bool ok = true;
+      for (uint32_t tile = first_tile; ok && tile < total; tile += tile_step, ++done) {
+        const uint32_t b = done & 1, acc = tmem + b * kWide;
+        if (done >= 2 && !(ok = warp_wait(bar(kFree + b), ((done >> 1) - 1) & 1, abort_flag, p, kSiteFree)))
+          break;
+        tc_fence_after();
+        for (uint32_t kb = 0; kb < nk; ++kb, ++step) {
+          const uint32_t s = step % kStages, parity = (step / kStages) & 1;
+          if (!(ok = warp_wait(bar(kFullBar + s), parity, abort_flag, p, kSiteFull))) break;
+          if constexpr (kGather) {
+            if (!(ok = warp_wait(bar(kGathered + s), parity, abort_flag, p, kSiteGathered))) break;
+            fence_proxy_async();
+          }
+          tc_fence_after();
+          const uint32_t st = sbase + s * kStageBytes;
+          const uint64_t ad = sw128_desc(st, 16, 1024), bd = sw128_desc(st + kHalfBytes, 16, 1024);
+          if (elect_one()) {
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)
+              umma_pair(acc, ad + ks * 2, bd + ks * 2, kIdesc, kb > 0 || ks > 0);
+            umma_commit_pair(bar(kEmpty + s));
+          }
+          __syncwarp();
+        }
+        if (ok && elect_one()) umma_commit_pair(bar(kAcc + b));
+        __syncwarp();
+      }
+      if (elect_one()) umma_commit_pair(bar(kDrain));
+      __syncwarp();
+    } else if constexpr (kGather) {
+      // The odd CTA's gathered rows, passed on to the thread that multiplies.
+      uint32_t step = 0;
+      bool ok = true;
+      for (uint32_t tile = first_tile; ok && tile < total; tile += tile_step)
+        for (uint32_t kb = 0; kb < nk; ++kb, ++step) {
+          const uint32_t s = step % kStages;
+          if (!(ok = warp_wait(bar(kGathered + s), (step / kStages) & 1, abort_flag, p, kSiteGathered)))
+            break;
+          fence_proxy_async();
+          if (elect_one()) mbar_arrive_cluster(full_at_even(s));
+          __syncwarp();
+        }
+    }
+    drain_bar(bar(kDrain), 0);
+  } else {
+    // Warp w finishes output columns [half * kCols, +kCols) of the 32 rows of its tensor-memory quarter.
+    constexpr uint32_t kCols = kOut / 2, kStep = 32;
+    const uint32_t quarter = (uint32_t)warp & 3, half = (uint32_t)(warp - 2) >> 2;
+    const uint32_t lanes = (quarter * 32u) << 16;
+    const uint32_t staging = sbase + kOffStaging + (uint32_t)(warp - 2) * kBufBytes;
+    uint32_t done = 0, e = 0;
+    bool ok = true;
+    for (uint32_t tile = first_tile; ok && tile < total; tile += tile_step) {
+      const uint32_t mt = tile / nt;
+      e = expert_of(tiles, p.experts, mt, e);
+      const uint32_t r0 = start[e] + (mt - tiles[e]) * kRows + rank * 128 + quarter * 32;
+      const uint32_t n0 = tile % nt * kOut + half * kCols;
+      const Finish f{r0, start[e + 1] > r0 ? min(start[e + 1] - r0, 32u) : 0, staging,
+                     p.bias ? p.bias + (size_t)e * (kGated ? 2 : 1) * p.n : nullptr};
+      const uint32_t b = done & 1, t0 = tmem + b * kWide + half * kCols + lanes;
+      ok = __all_sync(kFull, wait_bar(bar(kAcc + b), (done >> 1) & 1, abort_flag, p.status,
+                                              kSiteAcc, p.wait_cycles));
+      if (!ok) break;
+      tc_fence_after();
+      ++done;
+      if (f.rows) {
+#pragma unroll 1
+        for (uint32_t c = 0; c < kCols; c += kStep) {
+          float v[kStep], u[kGated ? kStep : 1];
+          load_columns<kStep>(t0 + c, v);
+          if constexpr (kGated) load_columns<kStep>(t0 + kOut + c, u);
+          finish_columns<kGated, kStep>(p, f, n0 + c, v, u);
+          __syncwarp();
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(cluster_addr(bar(kFree + b), 0));
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  // Neither CTA leaves, nor gives its tensor memory back, while the other may still reach it.
+  cluster_sync();
+  tc_fence_after();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512)
+                 : "memory");
+}
+
+// x [rows, k] in boxes of a tile's rows, and w [experts, wide, k] in boxes of box_rows rows; 64 columns
+// of bf16 in the 128-byte swizzle.
 bool make_maps(CUtensorMap *mx, CUtensorMap *mw, const ExpertsProblem &p, uint32_t box_rows) {
   auto fn = encode_fn();
   if (!fn) return false;
   const uint32_t wide = p.n * (p.gated ? 2 : 1);
   cuuint64_t xd[2] = {p.k, p.x_rows}, xs[1] = {p.ldx * 2};
-  cuuint32_t xb[2] = {64, 1}, one[3] = {1, 1, 1};
+  cuuint32_t xb[2] = {64, kBM}, one[3] = {1, 1, 1};
   cuuint64_t wd[3] = {p.k, wide, p.experts}, ws[2] = {p.ldw * 2, p.expert_stride * 2};
   cuuint32_t wb[3] = {64, box_rows, 1};
   return fn(mx, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(p.x), xd, xs, xb, one,
@@ -387,25 +725,44 @@ bool make_maps(CUtensorMap *mx, CUtensorMap *mw, const ExpertsProblem &p, uint32
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int kBN, bool kGated, bool kLong>
+template <int kBN, bool kGated, bool kLong, bool kGather>
 cudaError_t launch_tiles(const ExpertsProblem &p, int num_sms, cudaStream_t stream) {
   constexpr uint32_t smem = Cfg<kBN>::kSmemBytes;
   CUtensorMap mx, mw;
   if (!make_maps(&mx, &mw, p, kGated ? kBN / 2 : kBN)) return cudaErrorInvalidValue;
   static std::atomic<uint64_t> seen{0};
-  cudaError_t e = allow_smem((const void *)experts_kernel<kBN, kGated, kLong>, (int)smem, seen);
+  cudaError_t e =
+      allow_smem((const void *)experts_kernel<kBN, kGated, kLong, kGather>, (int)smem, seen);
   if (e != cudaSuccess) return e;
-  experts_kernel<kBN, kGated, kLong><<<num_sms, kThreads, smem, stream>>>(mx, mw, p);
+  experts_kernel<kBN, kGated, kLong, kGather>
+      <<<num_sms, kGather ? kGatherThreads : kThreads, smem, stream>>>(mx, mw, p);
   return cudaGetLastError();
 }
 
-template <bool kGated, bool kLong>
+template <bool kGated, bool kGather>
+cudaError_t launch_pairs(const ExpertsProblem &p, int num_sms, cudaStream_t stream) {
+  CUtensorMap mx, mw;
+  if (!make_maps(&mx, &mw, p, 128)) return cudaErrorInvalidValue;
+  static std::atomic<uint64_t> seen{0};
+  cudaError_t e = allow_smem((const void *)pair_kernel<kGated, kGather>, (int)pair::kSmemBytes, seen);
+  if (e != cudaSuccess) return e;
+  pair_kernel<kGated, kGather><<<num_sms / 2 * 2, kGather ? kGatherThreads : kThreads, pair::kSmemBytes,
+                                 stream>>>(mx, mw, p);
+  return cudaGetLastError();
+}
+
+template <bool kGated, bool kLong, bool kGather>
 cudaError_t launch_wide(const ExpertsProblem &p, int num_sms, cudaStream_t stream) {
   const uint32_t wide = p.n * (kGated ? 2 : 1);
-  if (wide <= 64) return launch_tiles<64, kGated, kLong>(p, num_sms, stream);
+  if (wide <= 64) return launch_tiles<64, kGated, kLong, kGather>(p, num_sms, stream);
   if constexpr (!kLong)
-    if (wide > 128 && p.rows > 128 * 64) return launch_tiles<256, kGated, kLong>(p, num_sms, stream);
-  return launch_tiles<128, kGated, kLong>(p, num_sms, stream);
+    if (wide > 128 && p.rows > 128 * 64) return launch_pairs<kGated, kGather>(p, num_sms, stream);
+  return launch_tiles<128, kGated, kLong, kGather>(p, num_sms, stream);
+}
+template <bool kGated, bool kLong>
+cudaError_t launch_rows(const ExpertsProblem &p, int num_sms, cudaStream_t stream) {
+  return p.order ? launch_wide<kGated, kLong, true>(p, num_sms, stream)
+                 : launch_wide<kGated, kLong, false>(p, num_sms, stream);
 }
 
 }  // namespace experts
@@ -413,15 +770,16 @@ cudaError_t launch_wide(const ExpertsProblem &p, int num_sms, cudaStream_t strea
 cudaError_t launch_experts_linear(ExpertsProblem p, int num_sms, cudaStream_t stream) {
   using namespace experts;
   p.out_vec = (uintptr_t)p.out % 16 == 0 && p.ldo % (p.out_dtype == TX_BF16 ? 8 : 4) == 0;
+  p.top_k_inv = p.top_k > 1 ? (uint32_t)((1ull << 32) / p.top_k) + 1 : 0;
   if (p.act == TX_ACT_GELU && p.out_dtype == TX_F32) p.act = kGeluF32;
   // The accumulator cuts bits off at each of its additions: over 512 K that is far below bf16's rounding,
   // for an fp32 result it is not.
   const bool parts = p.out_dtype == TX_F32 && p.k > kPart * kBK;
   if (p.gated)
-    return parts ? launch_wide<true, true>(p, num_sms, stream)
-                 : launch_wide<true, false>(p, num_sms, stream);
-  return parts ? launch_wide<false, true>(p, num_sms, stream)
-               : launch_wide<false, false>(p, num_sms, stream);
+    return parts ? launch_rows<true, true>(p, num_sms, stream)
+                 : launch_rows<true, false>(p, num_sms, stream);
+  return parts ? launch_rows<false, true>(p, num_sms, stream)
+               : launch_rows<false, false>(p, num_sms, stream);
 }
 
 }  // namespace tx

@@ -287,7 +287,8 @@ struct ExpertsProblem {
   const int32_t *offsets, *order;
   uint32_t x_rows, rows, experts, top_k, n, k;
   int gated, act, out_dtype;
-  bool out_vec;  // on 16-byte boundaries: set by the launcher
+  bool out_vec;        // on 16-byte boundaries, and what divides by top_k: set by the launcher
+  uint32_t top_k_inv;
   int *status;
   long long wait_cycles;
 };
