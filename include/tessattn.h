@@ -569,7 +569,8 @@ typedef struct {
   int32_t *places;         /* [tokens, top_k]: the row of each pair, or -1 */
 } TxRoute;
 
-/* experts at most 1024, top_k at most 32 and at most the eligible experts, tokens * top_k below 2^31.
+/* experts at most 1024, groups at most 64, top_k at most 32 and at most the eligible experts, tokens *
+ * top_k below 2^31.
  * More than a few hundred tokens take two launches and scratch of the context (or, on a stream that is
  * being captured, of the graph). */
 int tx_experts_route(void *ctx, const TxRoute *route, uint32_t tokens, uint32_t experts,

@@ -5,17 +5,22 @@
 // the largest sums; the weights are the chosen experts' s, divided by their sum where asked, times scale.
 // The plan lists the pairs token * top_k + j by expert, ascending inside an expert: a stable counting sort.
 //
-// The choice is that of exact arithmetic: without bias and groups c grows with l, so the logits themselves
-// are compared; otherwise c is taken in fp32, and a token with two candidates closer than fp32's error at
-// a border that decides (and not equal in logit and bias) takes its scores again in 64 bits.  In 64 bits
-// alone the exponentials would cost several times the rest.
+// kLanes lanes take a token, each with `per_lane` (at most V) consecutive experts.  A lane sorts its
+// candidates once, as 32-bit keys whose lowest bits name the expert of the lane, and each round takes the
+// largest head: 2 instructions a comparison, and no search for what won.  The bits that the name covers are
+// looked at where they matter: the choice is that of exact arithmetic, and a token with two neighbours in
+// the order that the keys do not tell apart (or, where c is computed, closer than fp32's error) is chosen
+// again by choose_exact: in fp32, and where that cannot tell either, with scores in 64 bits.
 //
-// kLanes lanes take a token, each with V consecutive experts.  A block takes a run of tokens and counts its
-// pairs by expert; the second kernel sums the counts of the runs before its own and places its pairs.
-// A few tokens are one block, which does both.
+// The plan: a warp takes tokens side by side and counts its pairs by expert as it goes, which gives a pair
+// its rank among the warp's; place_kernel adds what lies before, of the warps and blocks before it.  A few
+// tokens are one block, which does both.
+//
+// Bound: instructions (HBM would take 3 to 4 us of the measured ones).
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/tessattn.h"
 #include "common.cuh"
@@ -24,11 +29,17 @@
 namespace tx {
 namespace {
 
-constexpr uint32_t kFull = 0xffffffffu;
-constexpr int kWarps = 16, kThreads = 32 * kWarps;
+constexpr uint32_t kFull = 0xffffffffu, kNone = 0xffffffffu;
 constexpr uint32_t kMaxK = 32;
+constexpr int kMostWarps = 32;  // of a block
 
-// Values as unsigned integers of the same order: 0 is closed, 1 is NaN (below every number).
+// Values as unsigned integers of the same order: 0 is closed, 1 is NaN (below every number).  The quick
+// keys of the kernel know neither: its closed experts are -inf, below kLowest, and a NaN is chosen exactly.
+constexpr uint32_t kLowest = 0x00800000u;  // the key of fp32's lowest value
+__device__ __forceinline__ uint32_t quick_key(float c) {
+  const uint32_t u = __float_as_uint(c + 0.f);  // -0 as 0
+  return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+}
 __device__ __forceinline__ uint32_t key_of(float c) {
   const uint32_t u = __float_as_uint(c + 0.f);  // -0 as 0
   if (c != c) return 1;
@@ -43,9 +54,21 @@ __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float(key >> 31 ? key & 0x7fffffffu : ~key);
 }
 
-__device__ __forceinline__ float sigmoid(float l) { return 1.f / (1.f + expf(-l)); }
+constexpr float kLog2e = 1.44269504088896341f;
+// The hardware exponential (2^-22) and reciprocal (2^-23).
+__device__ __forceinline__ float quick_exp(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * kLog2e));
+  return y;
+}
+__device__ __forceinline__ float quick_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float sigmoid(float l) { return quick_rcp(1.f + quick_exp(-l)); }
 __device__ __forceinline__ double sigmoid(double l) { return 1.0 / (1.0 + exp(-l)); }
-__device__ __forceinline__ float exp_of(float x) { return expf(x); }
+__device__ __forceinline__ float exp_of(float x) { return quick_exp(x); }
 __device__ __forceinline__ double exp_of(double x) { return exp(x); }
 
 template <int kLanes, typename S>
@@ -60,6 +83,164 @@ __device__ __forceinline__ float lanes_max(float v) {
   for (int o = kLanes / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
   return v;
 }
+template <int kLanes>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+  if constexpr (kLanes == 32) {
+    return __reduce_max_sync(kFull, v);
+  } else {
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(kFull, v, o));
+    return v;
+  }
+}
+
+__device__ __forceinline__ float logit_at(const RouteProblem &p, size_t token, uint32_t e) {
+  const size_t at = token * p.ld + e;
+  return p.logits_dtype == TX_BF16 ? bf16_bits_to_f32(static_cast<const uint16_t *>(p.logits)[at])
+                                   : static_cast<const float *>(p.logits)[at];
+}
+
+// What two fp32 scores together may be off by.  Softmax: the sum over V values and lanes, the exponential's
+// 4 units of 2^-24 and its argument's rounding, the reciprocal and the product make (V + 16) 2^-24 of a score,
+// and none is above 1 / sum.  Sigmoid: 2^-21.4 (a quarter of the exponential's error, the sum's and the
+// reciprocal's rounding).
+template <int V>
+__device__ __forceinline__ float score_tolerance(bool softmax, float inv_sum) {
+  return softmax ? (float)((V + 16) * 1.1920929e-7f) * inv_sum : 7.2e-7f;
+}
+
+template <typename S>
+__device__ __forceinline__ S larger(S a, S b) {
+  return a > b ? a : b;
+}
+template <typename S>
+__device__ __forceinline__ S smaller(S a, S b) {
+  return a < b ? a : b;
+}
+// keep_groups for groups that cut through lanes: one after the other over all lanes.
+template <int kLanes, int V, typename S>
+__device__ __noinline__ uint32_t keep_any_groups(const RouteProblem &p, uint32_t sub, uint32_t slot,
+                                                 const S (&c)[V], float tol, bool *near) {
+  const S none = -(S)INFINITY;
+  const uint32_t per = p.experts / p.groups;
+  auto sum_of = [&](uint32_t g) {
+    S a = none, b = none;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const uint32_t e = sub * p.per_lane + i;
+      const S v = i < (int)p.per_lane && e >= g * per && e < (g + 1) * per ? c[i] : none;
+      b = larger(b, smaller(a, v));
+      a = larger(a, v);
+    }
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) {
+      const S x = __shfl_xor_sync(kFull, a, o), y = __shfl_xor_sync(kFull, b, o);
+      b = larger(smaller(a, x), larger(b, y));
+      a = larger(a, x);
+    }
+    return p.group_best > 1 && b > none ? a + b : a;
+  };
+  // The lane keeps the sums of groups sub, sub + kLanes, ...: 64 groups at most.
+  constexpr int kSums = 64 / kLanes;
+  S sums[kSums];
+  uint32_t before[kSums];
+#pragma unroll
+  for (int m = 0; m < kSums; ++m) {
+    sums[m] = none;
+    before[m] = 0;
+  }
+  for (uint32_t g = 0; g < p.groups; ++g) {
+    const S s = sum_of(g);
+#pragma unroll
+    for (int m = 0; m < kSums; ++m)
+      if (g == sub + m * kLanes) sums[m] = s;
+  }
+  for (uint32_t h = 0; h < p.groups; ++h) {
+    S other = none;
+#pragma unroll
+    for (int m = 0; m < kSums; ++m)
+      if (h / kLanes == m) other = sums[m];
+    other = __shfl_sync(kFull, other, slot * kLanes + h % kLanes);
+#pragma unroll
+    for (int m = 0; m < kSums; ++m)
+      before[m] += other > sums[m] || (other == sums[m] && h < sub + m * kLanes);
+  }
+  uint32_t mask = 0;
+  S low = (S)INFINITY, high = none;  // the lowest sum kept, the highest left out
+  for (uint32_t g = 0; g < p.groups; ++g) {
+    S s = none;
+    uint32_t n = 0;
+#pragma unroll
+    for (int m = 0; m < kSums; ++m)
+      if (g / kLanes == m) {
+        s = sums[m];
+        n = before[m];
+      }
+    s = __shfl_sync(kFull, s, slot * kLanes + g % kLanes);
+    n = __shfl_sync(kFull, n, slot * kLanes + g % kLanes);
+    if (n < p.top_groups) {
+      low = smaller(low, s);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const uint32_t e = sub * p.per_lane + i;
+        if (e >= g * per && e < (g + 1) * per) mask |= 1u << i;
+      }
+    } else {
+      high = larger(high, s);
+    }
+  }
+  if (sizeof(S) == 4 && high > none)
+    *near |= low - high <= (S)(3.f * tol) + (low < 0 ? -low : low) * (S)2.4e-7f;
+  return mask;
+}
+// Whether the lane's experts lie in a group that stays, bit i for its i-th; c[i] is -inf where closed or
+// NaN.  near: whether a sum that stays and one that does not are closer than tol (fp32 only).
+template <int kLanes, int V, typename S>
+__device__ __forceinline__ uint32_t keep_groups(const RouteProblem &p, uint32_t sub, uint32_t slot,
+                                                const S (&c)[V], float tol, bool *near) {
+  const S none = -(S)INFINITY;
+  if (p.group_lanes) {
+    // A group is group_lanes lanes: the best two of a lane, then of its group, then the group's place among
+    // the others.
+    S a = none, b = none;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      b = larger(b, smaller(a, c[i]));
+      a = larger(a, c[i]);
+    }
+    const uint32_t g = sub / p.group_lanes, at = sub - g * p.group_lanes;
+    const uint32_t base = slot * kLanes + g * p.group_lanes;
+    S best = a, second = b;
+    for (uint32_t t = 1; t < p.group_lanes; ++t) {
+      const uint32_t from = at + t < p.group_lanes ? at + t : at + t - p.group_lanes;
+      const S x = __shfl_sync(kFull, a, (base + from) & 31);
+      const S y = __shfl_sync(kFull, b, (base + from) & 31);
+      second = larger(smaller(best, x), larger(second, y));
+      best = larger(best, x);
+    }
+    const S sum = p.group_best > 1 && second > none ? best + second : best;
+    const S close = (S)(3.f * tol) + (sum < 0 ? -sum : sum) * (S)2.4e-7f;
+    uint32_t before = 0;
+    bool touch = false;
+    for (uint32_t h = 0; h < p.groups; ++h) {
+      const S other = __shfl_sync(kFull, sum, slot * kLanes + h * p.group_lanes);
+      before += other > sum || (other == sum && h < g);
+      touch |= h != g && other <= sum + close && other >= sum - close;
+    }
+    const bool kept = before < p.top_groups;
+    if (sizeof(S) == 4 && __any_sync(kFull, touch && g < p.groups && sum > none)) {
+      for (uint32_t h = 0; h < p.groups; ++h) {
+        const S other = __shfl_sync(kFull, sum, slot * kLanes + h * p.group_lanes);
+        const bool stays = __shfl_sync(kFull, (int)kept, slot * kLanes + h * p.group_lanes);
+        *near |= g < p.groups && sum > none && stays != kept && other <= sum + close &&
+                 other >= sum - close;
+      }
+    }
+    return kept ? kFull : 0;
+  }
+  return keep_any_groups<kLanes, V, S>(p, sub, slot, c, tol, near);
+}
+
 template <typename S>
 struct KeyOf {
   using type = uint32_t;
@@ -69,84 +250,65 @@ struct KeyOf<double> {
   using type = uint64_t;
 };
 
-__device__ __forceinline__ float logit_at(const RouteProblem &p, size_t token, uint32_t e) {
-  const size_t at = token * p.ld + e;
-  return p.logits_dtype == TX_BF16 ? bf16_bits_to_f32(static_cast<const uint16_t *>(p.logits)[at])
-                                   : static_cast<const float *>(p.logits)[at];
-}
-
-// What a token's lanes share in shared memory.
-struct Shared {
-  uint32_t *chosen;  // [kMaxK]
-  void *c;           // [experts] of S (groups only)
-  void *sum;         // [groups] of S
-  uint32_t *kept;    // [groups]
-};
-
-// The choice of one token among candidates c: key[i] of expert sub * V + i, 0 where closed.  Leaves the
-// chosen experts in sh.chosen (kNone behind the last) and returns whether fp32 could not decide.
-constexpr uint32_t kNone = 0xffffffffu;
-
+// The choice of the warp's tokens with whole keys: of the logits as they are (S float), or of scores in 64
+// bits.  Reads the logits again and leaves the chosen experts in `chosen`, kNone behind the last.
 template <int kLanes, int V, typename S>
-__device__ bool choose(const RouteProblem &p, const Shared &sh, size_t token, uint32_t sub,
-                       typename KeyOf<S>::type (&key)[V], const S (&c)[V], float tol) {
+__device__ __noinline__ void choose_exact(const RouteProblem &p, uint32_t *chosen, uint32_t token,
+                                          bool valid, uint32_t sub, uint32_t slot) {
   using Key = typename KeyOf<S>::type;
-  bool unsure = false;
-  if (p.groups > 1) {
-    const uint32_t per = p.experts / p.groups;
-    S *cs = static_cast<S *>(sh.c), *sum = static_cast<S *>(sh.sum);
-    const S none = -(S)INFINITY;
+  const bool scored = sizeof(S) == 8;
+  S c[V];
+  bool open[V];
+  S sum = 0;
+  float top_l = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (sub * V + i < p.experts) cs[sub * V + i] = key[i] > 1 ? c[i] : none;
-    __syncwarp();
-    for (uint32_t g = sub; g < p.groups; g += kLanes) {
-      S a = none, b = none;
-      for (uint32_t e = g * per; e < (g + 1) * per; ++e) {
-        const S v = cs[e];
-        if (v > a) {
-          b = a;
-          a = v;
-        } else if (v > b) {
-          b = v;
-        }
-      }
-      sum[g] = p.group_best > 1 && b > none ? a + b : a;
-    }
-    __syncwarp();
-    for (uint32_t g = sub; g < p.groups; g += kLanes) {
-      uint32_t before = 0;
-      for (uint32_t h = 0; h < p.groups; ++h)
-        before += sum[h] > sum[g] || (sum[h] == sum[g] && h < g);
-      sh.kept[g] = before < p.top_groups;
-    }
-    __syncwarp();
-    if (tol > 0.f) {
-      S low = (S)INFINITY, high = none;  // the lowest sum kept, the highest left out
-      for (uint32_t g = 0; g < p.groups; ++g) {
-        if (sh.kept[g])
-          low = low < sum[g] ? low : sum[g];
-        else
-          high = high > sum[g] ? high : sum[g];
-      }
-      const S size = (low < 0 ? -low : low) * (S)2.4e-7f;
-      unsure |= high > none && low - high <= 3 * (S)tol + size;
-    }
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (sub * V + i < p.experts && !sh.kept[(sub * V + i) / per]) key[i] = 0;
+  for (int i = 0; i < V; ++i) {
+    const uint32_t e = sub * p.per_lane + i;
+    open[i] = valid && i < (int)p.per_lane && e < p.experts;
+    float l = open[i] ? logit_at(p, token, e) : -INFINITY;
+    open[i] = l != -INFINITY && !(p.bias && p.bias[e] == -INFINITY);
+    if (open[i]) top_l = fmaxf(top_l, l);
+    c[i] = (S)l;
   }
-  Key last = 0;
-  uint32_t last_e = kNone;
-  bool done = false;  // (the rounds are the warp's; a token that needs no more of them idles)
-  for (uint32_t j = 0;; ++j) {
+  if (scored) {
+    if (p.softmax) {
+      top_l = lanes_max<kLanes>(top_l);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        if (open[i]) c[i] = exp_of(c[i] - (S)top_l);
+        if (open[i]) sum += c[i];
+      }
+      sum = lanes_sum<kLanes>(sum);
+#pragma unroll
+      for (int i = 0; i < V; ++i) c[i] /= sum;
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (open[i]) c[i] = sigmoid(c[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (open[i] && p.bias) c[i] += (S)p.bias[sub * p.per_lane + i];
+  }
+  uint32_t kept = kFull;
+  if (p.groups > 1) {
+    S g[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) g[i] = open[i] && c[i] == c[i] ? c[i] : -(S)INFINITY;
+    bool none;
+    kept = keep_groups<kLanes, V, S>(p, sub, slot, g, 0.f, &none);
+  }
+  Key key[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) key[i] = open[i] && (kept >> i & 1) ? key_of(c[i]) : 0;
+  for (uint32_t j = 0; j < p.top_k; ++j) {
     Key top = 0;
     uint32_t at = 0;
 #pragma unroll
     for (int i = 0; i < V; ++i)
       if (key[i] > top) {
         top = key[i];
-        at = sub * V + i;
+        at = sub * p.per_lane + i;
       }
 #pragma unroll
     for (int o = kLanes / 2; o > 0; o >>= 1) {
@@ -157,72 +319,78 @@ __device__ bool choose(const RouteProblem &p, const Shared &sh, size_t token, ui
         at = at2;
       }
     }
-    bool same = false;
-    if (sizeof(S) == 4 && tol > 0.f && j && !done && top > 1) {
-      const float v = value_of((uint32_t)top), w = value_of((uint32_t)last);
-      if (!(w - v > tol + 1.2e-7f * fabsf(w))) {
-        same = logit_at(p, token, at) == logit_at(p, token, last_e) &&
-               (!p.bias || p.bias[at] == p.bias[last_e]);
-        unsure |= !same;
-      }
-    }
-    if (j < p.top_k && sub == 0) sh.chosen[j] = top ? at : kNone;
-    // Past the last one only equals of it may be followed by a candidate too close to tell.
-    done |= !top || (j >= p.top_k && !same);
-    if (j + 1 >= p.top_k && !(sizeof(S) == 4 && tol > 0.f)) break;
-    if (j >= p.top_k && __all_sync(kFull, done)) break;
-    if (!done) {
-      last = top;
-      last_e = at;
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (sub * V + i == at) key[i] = 0;
-    }
-  }
-  __syncwarp();
-  return unsure;
-}
-
-template <int kLanes, int V, typename S>
-__device__ bool score_and_choose(const RouteProblem &p, const Shared &sh, size_t token, uint32_t sub,
-                                 const float (&l)[V], const bool (&open)[V]) {
-  S s[V];
-  float tol = 0.f;
-  if (p.softmax) {
-    float top = -INFINITY;
+    if (sub == 0) chosen[j] = top ? at : kNone;
 #pragma unroll
     for (int i = 0; i < V; ++i)
-      if (open[i]) top = fmaxf(top, l[i]);
-    top = lanes_max<kLanes>(top);
-    S sum = 0;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      s[i] = open[i] ? exp_of((S)l[i] - (S)top) : (S)0;
-      sum += s[i];
-    }
-    sum = lanes_sum<kLanes>(sum);
-    const S inv = (S)1 / sum;
-#pragma unroll
-    for (int i = 0; i < V; ++i) s[i] *= inv;
-    // A score is off by (V + 12) 2^-24 of itself at most, and none is above 1 / sum: the sum over V
-    // values and lanes, the exponential (2 units), its argument's rounding, the reciprocal and product.
-    tol = (float)((V + 12) * 1.1920929e-7f) * (float)inv;
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) s[i] = open[i] ? sigmoid((S)l[i]) : (S)0;
-    tol = 7.2e-7f;  // two scores, each off by 2^-21.4
+      if (sub * p.per_lane + i == at) key[i] = 0;
   }
-  using Key = typename KeyOf<S>::type;
-  Key key[V];
-  S c[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    c[i] = s[i];
-    if (p.bias && sub * V + i < p.experts) c[i] += (S)__ldg(p.bias + sub * V + i);
-    key[i] = open[i] ? key_of(c[i]) : 0;
-  }
-  return choose<kLanes, V, S>(p, sh, token, sub, key, c, sizeof(S) == 4 ? tol : 0.f);
+  __syncwarp();
 }
+
+// Sorts V keys, the largest first: Batcher's odd-even merge network.
+template <int V>
+__device__ __forceinline__ void sort_keys(uint32_t (&k)[V]) {
+#pragma unroll
+  for (int p = 1; p < V; p *= 2)
+#pragma unroll
+    for (int q = p; q >= 1; q /= 2)
+#pragma unroll
+      for (int j = q % p; j <= V - 1 - q; j += 2 * q)
+#pragma unroll
+        for (int i = 0; i < q; ++i)
+          if (i + j + q < V && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+            const uint32_t a = k[i + j], b = k[i + j + q];
+            k[i + j] = max(a, b);
+            k[i + j + q] = min(a, b);
+          }
+}
+
+// The logits of a lane's experts, as they lie.
+template <int V>
+struct Logits {
+  uint32_t w[V];
+  // -inf where there is none; here: whether the token has logits
+  __device__ __forceinline__ void load(const RouteProblem &p, size_t token, uint32_t sub, bool here) {
+    const uint32_t e0 = sub * p.per_lane;
+    const size_t at = token * p.ld + e0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) w[i] = 0xff800000u;
+    if constexpr (V >= 4) {
+      if (p.vec && p.logits_dtype == TX_F32) {  // per_lane == V, on 16-byte boundaries
+#pragma unroll
+        for (int i = 0; i < V; i += 4)
+          if (here && e0 + i < p.experts) {
+            const uint4 q = *reinterpret_cast<const uint4 *>(static_cast<const float *>(p.logits) + at + i);
+            w[i] = q.x; w[i + 1] = q.y; w[i + 2] = q.z; w[i + 3] = q.w;
+          }
+        return;
+      }
+    }
+    if constexpr (V >= 8) {
+      if (p.vec) {
+#pragma unroll
+        for (int i = 0; i < V; i += 8)
+          if (here && e0 + i < p.experts) {
+            const uint4 q =
+                *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.logits) + at + i);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+              const uint32_t u = t == 0 ? q.x : t == 1 ? q.y : t == 2 ? q.z : q.w;
+              w[i + 2 * t] = u << 16;
+              w[i + 2 * t + 1] = u & 0xffff0000u;
+            }
+          }
+        return;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (here && i < (int)p.per_lane && e0 + i < p.experts)
+        w[i] = p.logits_dtype == TX_BF16
+                   ? (uint32_t) static_cast<const uint16_t *>(p.logits)[at + i] << 16
+                   : static_cast<const uint32_t *>(p.logits)[at + i];
+  }
+};
 
 // ---- the plan -------------------------------------------------------------------------------
 // Exclusive sums of count[experts] into offset[experts + 1]; all threads of the block call it.
@@ -244,158 +412,281 @@ __device__ void scan_counts(const uint32_t *count, uint32_t *offset, uint32_t ex
   }
   __syncthreads();
 }
-
-// Places the pairs [first, end): base[e] is where this run's pairs of expert e start.
-__device__ void place_pairs(const RouteProblem &p, uint64_t first, uint64_t end, const uint32_t *base,
-                            uint32_t *by_warp /* [kWarps][experts] */) {
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint64_t per = ((end - first + kWarps - 1) / kWarps + 31) / 32 * 32;
-  const uint64_t a = first + warp * per, b = min(end, a + per);
-  uint32_t *mine = by_warp + (size_t)warp * p.experts;
-  for (uint32_t i = threadIdx.x; i < kWarps * p.experts; i += kThreads) by_warp[i] = 0;
-  __syncthreads();
-  for (uint64_t i = a; i < b; i += 32) {
-    const int32_t e = i + lane < b ? p.chosen[i + lane] : -1;
-    const uint32_t peers = __match_any_sync(kFull, e);
-    if (e >= 0 && lane == __ffs(peers) - 1) mine[e] += __popc(peers);
-    __syncwarp();
-  }
-  __syncthreads();
-  for (uint32_t e = threadIdx.x; e < p.experts; e += kThreads) {
-    uint32_t run = base[e];
-    for (uint32_t w = 0; w < kWarps; ++w) {
-      uint32_t *at = by_warp + (size_t)w * p.experts + e;
-      const uint32_t n = *at;
-      *at = run;
-      run += n;
-    }
-  }
-  __syncthreads();
-  for (uint64_t i = a; i < b; i += 32) {
-    const int32_t e = i + lane < b ? p.chosen[i + lane] : -1;
-    const uint32_t peers = __match_any_sync(kFull, e);
-    uint32_t at = 0;
-    if (e >= 0) at = mine[e] + __popc(peers & ((1u << lane) - 1));
-    __syncwarp();
-    if (e >= 0 && lane == __ffs(peers) - 1) mine[e] += __popc(peers);
-    __syncwarp();
-    if (i + lane < b) {
-      p.places[i + lane] = e >= 0 ? (int32_t)at : -1;
-      if (e >= 0) p.order[at] = (int32_t)(i + lane);
+// The tokens of warp `warp` in the run of block `block`: [*first, *end).
+__device__ __forceinline__ void warp_tokens(const RouteProblem &p, uint32_t block, uint32_t warp,
+                                            uint32_t *first, uint32_t *end) {
+  const uint64_t run = (uint64_t)block * p.run, last = min(run + p.run, (uint64_t)p.tokens);
+  *first = (uint32_t)min(run + (uint64_t)warp * p.run_warp, last);
+  *end = (uint32_t)min((uint64_t)*first + p.run_warp, last);
+}
+// A warp's pairs, whose ranks among them lie in p.places, go to their rows: before[e] is where the warp's
+// rows of expert e start.
+__device__ __forceinline__ void place_pairs(const RouteProblem &p, uint32_t first, uint32_t end,
+                                            const uint32_t *before) {
+  const uint64_t b = (uint64_t)end * p.top_k;
+#pragma unroll 4
+  for (uint64_t i = (uint64_t)first * p.top_k + (threadIdx.x & 31); i < b; i += 32) {
+    const int32_t e = p.chosen[i], rank = p.places[i];
+    if (e >= 0) {
+      const uint32_t at = before[e] + (uint32_t)rank;
+      p.places[i] = (int32_t)at;
+      p.order[at] = (int32_t)i;
     }
   }
 }
 
-// kLanes lanes a token, V experts a lane.  Shared memory: the chosen of every token in work, with groups
-// their candidates and sums, the block's counts by expert, and for a plan in one block its places.
-template <int kLanes, int V>
-__global__ void __launch_bounds__(kThreads) route_kernel(const __grid_constant__ RouteProblem p) {
+// Shared memory: by_warp [kWarps][experts], offset [experts + 1], and for every token in work its chosen
+// experts and their keys, one more than there may be.
+constexpr uint32_t kSlotWords = 2 * (kMaxK + 1);
+
+template <int kLanes, int V, bool kScored, int kWarps>
+__global__ void __launch_bounds__(32 * kWarps, 1)
+    route_kernel(const __grid_constant__ RouteProblem p) {
+  constexpr uint32_t kThreads = 32 * kWarps;
   constexpr uint32_t kTokens = 32 / kLanes;  // of a warp at a time
+  // The low bits of a key: V - 1 - i for expert i of the lane, or, where the keys' lowest 16 bits are alike
+  // (bf16 logits compared as they are), kNameAll - e for expert e.  The latter lose nothing and put equals
+  // in their order.
+  constexpr uint32_t kName = V - 1, kNameAll = 0xffff;
+  constexpr int kMine = kMaxK / kLanes;  // chosen experts a lane weighs
   extern __shared__ __align__(16) uint8_t smem[];
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane % kLanes;
-  const uint32_t slot = warp * kTokens + lane / kLanes;
-  uint32_t *count = reinterpret_cast<uint32_t *>(smem);
-  uint32_t *offset = count + p.experts;
-  uint32_t *chosen = offset + p.experts + 1;
-  Shared sh;
-  sh.chosen = chosen + slot * kMaxK;
-  uint8_t *more = smem + p.off_groups;
-  const uint32_t group_bytes = p.groups > 1 ? p.experts * 8 + p.groups * 12 + (p.groups & 1) * 4 : 0;
-  sh.c = more + (size_t)slot * group_bytes;
-  sh.sum = more + (size_t)slot * group_bytes + p.experts * 8;
-  sh.kept = reinterpret_cast<uint32_t *>(more + (size_t)slot * group_bytes + p.experts * 8 +
-                                         p.groups * 8);
-  for (uint32_t e = threadIdx.x; e < p.experts; e += kThreads) count[e] = 0;
-  __syncthreads();
-  const uint32_t first = min((uint64_t)blockIdx.x * p.run, (uint64_t)p.tokens);
-  const uint32_t end = min((uint64_t)first + p.run, (uint64_t)p.tokens);
-  for (uint32_t t0 = first + warp * kTokens; t0 < end; t0 += kWarps * kTokens) {
-    const uint32_t token = t0 + lane / kLanes;
-    const bool here = token < end;
-    bool valid = here;
-    if (here && p.lengths) valid = (int64_t)(token % p.seq) < (int64_t)p.lengths[token / p.seq];
-    float l[V];
-    bool open[V];
+  const uint32_t slot = lane / kLanes, group_mask = (kLanes == 32 ? kFull : (1u << kLanes) - 1)
+                                                   << (slot * kLanes);
+  uint32_t *by_warp = reinterpret_cast<uint32_t *>(smem), *words = by_warp + warp * p.experts;
+  uint32_t *offset = by_warp + kWarps * p.experts;
+  uint32_t *chosen = offset + p.experts + 1 + (warp * kTokens + slot) * kSlotWords;
+  uint32_t *chosen_key = chosen + kMaxK + 1;
+  if (p.order) {
+    for (uint32_t e = lane; e < p.experts; e += 32) words[e] = 0;
+    __syncwarp();
+  }
+  uint32_t first, end;
+  warp_tokens(p, blockIdx.x, warp, &first, &end);
+  const bool told = !kScored && p.logits_dtype == TX_BF16;
+  // Where the next token to load stands in its sequence, and how many rows of that are valid.
+  uint32_t next = first + slot, row = 0, seq = 0, length = 0;
+  if (p.lengths && next < end) {
+    seq = next / p.seq;
+    row = next - seq * p.seq;
+    length = (uint32_t)max(p.lengths[seq], 0);
+  }
+  Logits<V> raw;
+  bool valid = next < end && (!p.lengths || row < length);
+  raw.load(p, next, sub, valid);
+  for (uint32_t t0 = first; t0 < end; t0 += kTokens) {
+    const uint32_t token = t0 + slot;
+    const bool here = token < end, had = valid;
+    float l[V], tol = 0.f;
+    uint32_t key[V];
+    bool near = false;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const uint32_t e = sub * V + i;
-      open[i] = valid && e < p.experts;
-      l[i] = open[i] ? logit_at(p, token, e) : -INFINITY;
-      open[i] = open[i] && l[i] != -INFINITY;
-      if (open[i] && p.bias) open[i] = __ldg(p.bias + e) != -INFINITY;
+    for (int i = 0; i < V; ++i) l[i] = __uint_as_float(raw.w[i]);
+    // The next tokens' logits travel meanwhile.
+    next += kTokens;
+    if (p.lengths && next < end) {
+      row += kTokens;
+      if (row >= p.seq) {
+        seq = next / p.seq;
+        row = next - seq * p.seq;
+        length = (uint32_t)max(p.lengths[seq], 0);
+      }
     }
-    if (p.bias || p.groups > 1) {
-      const bool unsure = score_and_choose<kLanes, V, float>(p, sh, token, sub, l, open);
-      if (__any_sync(kFull, unsure)) score_and_choose<kLanes, V, double>(p, sh, token, sub, l, open);
-    } else {
-      uint32_t key[V];
+    valid = next < end && (!p.lengths || row < length);
+    raw.load(p, next, sub, valid);
+    if constexpr (!kScored) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) key[i] = open[i] ? key_of(l[i]) : 0;
-      choose<kLanes, V, float>(p, sh, token, sub, key, l, 0.f);
+      for (int i = 0; i < V; ++i) {
+        near |= l[i] != l[i];
+        key[i] = told ? (quick_key(l[i]) & ~kNameAll) | (kNameAll - sub * p.per_lane - i)
+                      : (quick_key(l[i]) & ~kName) | (V - 1 - i);
+      }
+    } else {
+      float c[V];
+      if (p.bias) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const uint32_t e = sub * p.per_lane + i;
+          c[i] = i < (int)p.per_lane && e < p.experts ? __ldg(p.bias + e) : 0.f;
+          if (c[i] == -INFINITY) l[i] = -INFINITY;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) c[i] = 0.f;
+      }
+      float inv = 1.f;
+      if (p.softmax) {
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) top = fmaxf(top, l[i]);
+        top = lanes_max<kLanes>(top);
+#pragma unroll
+        for (int i = 0; i < V; ++i) sum += l[i] == -INFINITY ? 0.f : quick_exp(l[i] - top);
+        inv = quick_rcp(lanes_sum<kLanes>(sum));
+#pragma unroll
+        for (int i = 0; i < V; ++i) c[i] = fmaf(quick_exp(l[i] - top), inv, c[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) c[i] += sigmoid(l[i]);
+      }
+      tol = score_tolerance<V>(p.softmax, inv);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        c[i] = l[i] == -INFINITY ? -INFINITY : c[i];
+        near |= c[i] != c[i];
+      }
+      uint32_t kept = kFull;
+      if (p.groups > 1) kept = keep_groups<kLanes, V, float>(p, sub, slot, c, tol, &near);
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        key[i] = kept >> i & 1 ? (quick_key(c[i]) & ~kName) | (V - 1 - i) : 0;
+    }
+    sort_keys(key);
+    // The lowest lane with the largest head, names apart, has the next expert.
+    const uint32_t names = told ? 0 : kName;
+    for (uint32_t j = 0; j < p.top_k + !told; ++j) {
+      const uint32_t head = key[0] | names, top = lanes_max<kLanes>(head);
+      if (lane == __ffs(__ballot_sync(kFull, head == top) & group_mask) - 1) {
+        chosen[j] = told ? kNameAll - (key[0] & kNameAll) : sub * p.per_lane + kName - (key[0] & kName);
+        chosen_key[j] = key[0];
+#pragma unroll
+        for (int i = 0; i + 1 < V; ++i) key[i] = key[i + 1];
+        key[V - 1] = 0;
+      }
+    }
+    __syncwarp();
+    uint32_t e[kMine];
+#pragma unroll
+    for (int m = 0; m < kMine; ++m) {
+      const uint32_t j = sub + m * kLanes;
+      e[m] = kNone;
+      if (j >= p.top_k) continue;
+      const uint32_t own = chosen_key[j];
+      if (own >= kLowest) e[m] = chosen[j];
+      if (told || own < kLowest) continue;
+      const uint32_t after = chosen_key[j + 1];
+      const float w = value_of(own & ~kName), v = value_of(after & ~kName);
+      if (after >= kLowest && !(w - v > tol + fabsf(w) * (V * 2.4e-7f))) {
+        // Equal in logit and bias they are in the right order, but behind the last there may be another.
+        const uint32_t f = chosen[j + 1];
+        near |= j + 1 == p.top_k || logit_at(p, token, e[m]) != logit_at(p, token, f) ||
+                (p.bias && p.bias[e[m]] != p.bias[f]);
+      }
+    }
+    if (__any_sync(kFull, near)) {
+      __syncwarp();
+      choose_exact<kLanes, V, typename std::conditional<kScored, double, float>::type>(
+          p, chosen, token, had, sub, slot);
+#pragma unroll
+      for (int m = 0; m < kMine; ++m)
+        if (sub + m * kLanes < p.top_k) e[m] = chosen[sub + m * kLanes];
+      __syncwarp();
     }
     // Weights.  With a common factor taken out first: e^l by the largest l, and for the sigmoid
     // e^min(l, 0) / (1 + e^-|l|) by the largest of the numerators; renormalised it cancels.
-    float top = -INFINITY, total = 1.f;
-    if (p.softmax && !p.renormalise) {
-      float sum = 0.f;
+    float x[kMine], top = -INFINITY, total = 1.f;
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (open[i]) top = fmaxf(top, l[i]);
+    for (int m = 0; m < kMine; ++m) {
+      x[m] = e[m] != kNone ? logit_at(p, token, e[m]) : -INFINITY;
+      if (e[m] != kNone) top = fmaxf(top, p.softmax ? x[m] : fminf(x[m], 0.f));
+    }
+    if (p.renormalise) {
       top = lanes_max<kLanes>(top);
+    } else if (p.softmax) {
+      top = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (open[i]) sum += expf(l[i] - top);
-      total = lanes_sum<kLanes>(sum);
-    } else if (p.renormalise) {
-      for (uint32_t j = sub; j < p.top_k; j += kLanes)
-        if (sh.chosen[j] != kNone) {
-          const float x = logit_at(p, token, sh.chosen[j]);
-          top = fmaxf(top, p.softmax ? x : fminf(x, 0.f));
-        }
+      for (int i = 0; i < V; ++i) top = fmaxf(top, l[i]);
       top = lanes_max<kLanes>(top);
     } else {
       top = 0.f;
     }
-    auto score = [&](uint32_t e) {
-      const float x = logit_at(p, token, e);
-      return p.softmax ? expf(x - top) : expf(fminf(x, 0.f) - top) / (1.f + expf(-fabsf(x)));
-    };
+    float s[kMine], sum = 0.f;
+#pragma unroll
+    for (int m = 0; m < kMine; ++m) {
+      s[m] = 0.f;
+      if (e[m] == kNone) continue;
+      s[m] = p.softmax ? expf(x[m] - top)
+                       : expf(fminf(x[m], 0.f) - top) / (1.f + expf(-fabsf(x[m])));
+      sum += s[m];
+    }
     if (p.renormalise) {
-      float sum = 0.f;
-      for (uint32_t j = sub; j < p.top_k; j += kLanes)
-        if (sh.chosen[j] != kNone) sum += score(sh.chosen[j]);
+      total = lanes_sum<kLanes>(sum);
+    } else if (p.softmax) {
+      sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (l[i] != -INFINITY) sum += expf(l[i] - top);
       total = lanes_sum<kLanes>(sum);
     }
-    if (here) {
-      for (uint32_t j = sub; j < p.top_k; j += kLanes) {
-        const uint32_t e = sh.chosen[j];
-        const size_t at = (size_t)token * p.top_k + j;
-        p.chosen[at] = e == kNone ? -1 : (int32_t)e;
-        p.weights[at] = e == kNone ? 0.f : score(e) / total * p.scale;
-        if (p.order && e != kNone) atomicAdd(count + e, 1u);
-      }
+    const float factor = p.scale / total;
+#pragma unroll
+    for (int m = 0; m < kMine; ++m) {
+      const uint32_t j = sub + m * kLanes;
+      if (!here || j >= p.top_k) continue;
+      const size_t at = (size_t)token * p.top_k + j;
+      p.chosen[at] = e[m] == kNone ? -1 : (int32_t)e[m];
+      p.weights[at] = e[m] == kNone ? 0.f : s[m] * factor;
     }
+    if (!p.order) continue;
+    // The rank of a pair among the warp's of its expert: words[e] holds those of the tokens before in its
+    // lower bits, and bit 24 + t for token t of these.  (A token has an expert once.)
+#pragma unroll
+    for (int m = 0; m < kMine; ++m)
+      if (e[m] != kNone) atomicOr(words + e[m], 1u << (24 + slot));
+    __syncwarp();
+    uint32_t word[kMine];
+#pragma unroll
+    for (int m = 0; m < kMine; ++m) {
+      const uint32_t j = sub + m * kLanes;
+      word[m] = e[m] != kNone ? words[e[m]] : 0;
+      if (here && j < p.top_k)
+        p.places[(size_t)token * p.top_k + j] =
+            e[m] == kNone ? -1
+                          : (int32_t)((word[m] & 0xffffffu) +
+                                      __popc(word[m] >> 24 & ((1u << slot) - 1)));
+    }
+    __syncwarp();
+#pragma unroll
+    for (int m = 0; m < kMine; ++m)
+      if (e[m] != kNone && !(word[m] >> 24 & ((1u << slot) - 1)))
+        words[e[m]] = (word[m] & 0xffffffu) + __popc(word[m] >> 24);
     __syncwarp();
   }
   if (!p.order) return;
   __syncthreads();
+  // The counts of the warps before each warp, and of the block.
+  for (uint32_t e = threadIdx.x; e < p.experts; e += kThreads) {
+    uint32_t run = 0;
+    for (uint32_t w = 0; w < kWarps; ++w) {
+      const uint32_t n = by_warp[w * p.experts + e];
+      by_warp[w * p.experts + e] = run;
+      run += n;
+    }
+    offset[e] = run;
+    if (gridDim.x > 1) p.counts[(size_t)blockIdx.x * p.experts + e] = run;
+  }
+  __syncthreads();
   if (gridDim.x > 1) {
-    for (uint32_t e = threadIdx.x; e < p.experts; e += kThreads)
-      p.counts[(size_t)blockIdx.x * p.experts + e] = count[e];
+    uint32_t *to = p.counts + ((size_t)gridDim.x + (size_t)blockIdx.x * kWarps) * p.experts;
+    for (uint32_t i = threadIdx.x; i < kWarps * p.experts; i += kThreads) to[i] = by_warp[i];
     return;
   }
-  scan_counts(count, offset, p.experts);
+  scan_counts(offset, offset, p.experts);
   for (uint32_t e = threadIdx.x; e <= p.experts; e += kThreads) p.offsets[e] = (int32_t)offset[e];
-  place_pairs(p, 0, (uint64_t)p.tokens * p.top_k, offset,
-              reinterpret_cast<uint32_t *>(smem + p.off_places));
+  for (uint32_t e = lane; e < p.experts; e += 32) words[e] += offset[e];
+  __syncwarp();
+  place_pairs(p, first, end, words);
 }
 
 // Places the pairs of run blockIdx.x behind those of the runs before it.
-__global__ void __launch_bounds__(kThreads) place_kernel(const __grid_constant__ RouteProblem p) {
+__global__ void __launch_bounds__(1024, 1) place_kernel(const __grid_constant__ RouteProblem p) {
   extern __shared__ __align__(16) uint8_t smem[];
-  uint32_t *total = reinterpret_cast<uint32_t *>(smem), *base = total + p.experts;
-  uint32_t *offset = base + p.experts;
+  const uint32_t kWarps = p.warps, kThreads = blockDim.x;
+  uint32_t *by_warp = reinterpret_cast<uint32_t *>(smem), *total = by_warp + kWarps * p.experts;
+  uint32_t *base = total + p.experts, *offset = base + p.experts;
   for (uint32_t e = threadIdx.x; e < p.experts; e += kThreads) total[e] = base[e] = 0;
+  const uint32_t *from = p.counts + ((size_t)gridDim.x + (size_t)blockIdx.x * kWarps) * p.experts;
+  for (uint32_t i = threadIdx.x; i < kWarps * p.experts; i += kThreads) by_warp[i] = __ldcg(from + i);
   __syncthreads();
   // Threads side by side take experts, the rest of them runs.
   uint32_t wide = 32;
@@ -414,52 +705,73 @@ __global__ void __launch_bounds__(kThreads) place_kernel(const __grid_constant__
   }
   __syncthreads();
   scan_counts(total, offset, p.experts);
-  for (uint32_t e = threadIdx.x; e < p.experts; e += kThreads) base[e] += offset[e];
   if (blockIdx.x == 0)
     for (uint32_t e = threadIdx.x; e <= p.experts; e += kThreads) p.offsets[e] = (int32_t)offset[e];
-  __syncthreads();
-  const uint64_t first = min((uint64_t)blockIdx.x * p.run, (uint64_t)p.tokens);
-  const uint64_t end = min(first + p.run, (uint64_t)p.tokens);
-  place_pairs(p, first * p.top_k, end * p.top_k, base, offset + p.experts + 1);
+  const uint32_t warp = threadIdx.x >> 5;
+  uint32_t *before = by_warp + warp * p.experts;
+  for (uint32_t e = threadIdx.x & 31; e < p.experts; e += 32) before[e] += offset[e] + base[e];
+  __syncwarp();
+  uint32_t first, end;
+  warp_tokens(p, blockIdx.x, warp, &first, &end);
+  place_pairs(p, first, end, before);
 }
 
-template <int kLanes, int V>
-cudaError_t run(RouteProblem p, cudaStream_t stream) {
-  constexpr uint32_t kTokens = kWarps * (32 / kLanes);  // a block's at a time
-  uint32_t bytes = (2 * p.experts + 1 + kTokens * kMaxK) * 4;
-  bytes = (bytes + 15) / 16 * 16;
-  p.off_groups = bytes;
-  if (p.groups > 1) bytes += kTokens * (p.experts * 8 + p.groups * 12 + (p.groups & 1) * 4);
-  // One block plans from the same memory once its tokens are routed.
-  p.off_places = p.off_groups;
-  const uint32_t places = kWarps * p.experts * 4;
-  if (p.blocks == 1 && p.order) bytes = std::max(bytes, p.off_places + places);
+template <int kLanes, int V, bool kScored, int kWarps>
+cudaError_t run_warps(RouteProblem p, cudaStream_t stream) {
+  constexpr uint32_t kTokens = 32 / kLanes;
+  p.warps = kWarps;
+  p.run_warp = ((p.run + kWarps - 1) / kWarps + kTokens - 1) / kTokens * kTokens;
+  const size_t size = p.logits_dtype == TX_BF16 ? 2 : 4;
+  p.vec = p.per_lane == V && V * size % 16 == 0 && p.experts % (16 / size) == 0 &&
+          p.ld * size % 16 == 0 && (uintptr_t)p.logits % 16 == 0;
+  const uint32_t bytes = ((kWarps + 1) * p.experts + 1 + kWarps * kTokens * kSlotWords) * 4;
   static std::atomic<uint64_t> seen{0}, seen_place{0};
-  cudaError_t e = allow_smem((const void *)route_kernel<kLanes, V>, 232448, seen);
+  cudaError_t e = allow_smem((const void *)route_kernel<kLanes, V, kScored, kWarps>, 232448, seen);
   if (e != cudaSuccess) return e;
-  route_kernel<kLanes, V><<<p.blocks, kThreads, bytes, stream>>>(p);
+  route_kernel<kLanes, V, kScored, kWarps><<<p.blocks, 32 * kWarps, bytes, stream>>>(p);
   if ((e = cudaGetLastError()) != cudaSuccess || p.blocks == 1 || !p.order) return e;
   if ((e = allow_smem((const void *)place_kernel, 232448, seen_place)) != cudaSuccess) return e;
-  place_kernel<<<p.blocks, kThreads, (3 * p.experts + 1) * 4 + places, stream>>>(p);
+  place_kernel<<<p.blocks, 32 * kWarps, ((kWarps + 3) * p.experts + 1) * 4, stream>>>(p);
   return cudaGetLastError();
+}
+template <int kLanes, int V>
+cudaError_t run(const RouteProblem &p, cudaStream_t stream) {
+  constexpr int kWarps = V <= 8 ? kMostWarps : kMostWarps / 2;  // as registers allow
+  return p.bias || p.groups > 1 ? run_warps<kLanes, V, true, kWarps>(p, stream)
+                                : run_warps<kLanes, V, false, kWarps>(p, stream);
 }
 
 }  // namespace
 
 // Runs of tokens: one while a single block is the faster way, else a block for each SM.
-void route_plan(RouteProblem *p, int num_sms) {
+size_t route_plan(RouteProblem *p, int num_sms) {
   p->run = std::max<uint32_t>(128, (uint32_t)(((uint64_t)p->tokens + num_sms - 1) / num_sms));
   p->blocks = (p->tokens + p->run - 1) / p->run;
+  return p->order && p->blocks > 1 ? (size_t)p->blocks * (kMostWarps + 1) * p->experts * 4 : 0;
 }
 
-cudaError_t launch_experts_route(const RouteProblem &p, cudaStream_t stream) {
-  if (p.experts <= 16) return run<4, 4>(p, stream);
-  if (p.experts <= 32) return run<8, 4>(p, stream);
-  if (p.experts <= 64) return run<8, 8>(p, stream);
-  if (p.experts <= 128) return run<16, 8>(p, stream);
-  if (p.experts <= 256) return run<32, 8>(p, stream);
-  if (p.experts <= 512) return run<32, 16>(p, stream);
-  return run<32, 32>(p, stream);
+cudaError_t launch_experts_route(RouteProblem p, cudaStream_t stream) {
+  // Experts of a lane: as few lanes as 8 (4 of up to 16, 16 or 32 of many) experts each allow.  With
+  // groups a group has to be whole lanes; where no number does that, group_lanes is 0.
+  uint32_t most = p.experts <= 16 ? 4 : p.experts <= 256 ? 8 : p.experts <= 512 ? 16 : 32;
+  p.per_lane = most;
+  p.group_lanes = 0;
+  if (p.groups > 1) {
+    const uint32_t per = p.experts / p.groups;
+    for (uint32_t v = std::min(most, per); v && !p.group_lanes; --v)
+      if (per % v == 0 && p.experts / v <= 32) {
+        p.per_lane = v;
+        p.group_lanes = per / v;
+      }
+  }
+  const uint32_t lanes = (p.experts + p.per_lane - 1) / p.per_lane;
+  if (most == 4 && lanes <= 4) return run<4, 4>(p, stream);
+  if (most == 32) return run<32, 32>(p, stream);
+  if (most == 16) return run<32, 16>(p, stream);
+  if (lanes <= 4) return run<4, 8>(p, stream);
+  if (lanes <= 8) return run<8, 8>(p, stream);
+  if (lanes <= 16) return run<16, 8>(p, stream);
+  return run<32, 8>(p, stream);
 }
 
 }  // namespace tx

@@ -273,11 +273,15 @@ struct RouteProblem {
   float *weights;
   int32_t *offsets, *order, *places;  // the plan, or NULL
   uint32_t run, blocks;    // tokens of a block (route_plan)
-  uint32_t *counts;        // [blocks][experts] with blocks > 1
-  uint32_t off_groups, off_places;  // shared memory, set by the launcher
+  uint32_t *counts;        // scratch with blocks > 1: [blocks][experts], then [blocks][warps][experts]
+  // set by the launcher
+  uint32_t warps, run_warp;        // of a block, and the tokens of a warp
+  uint32_t per_lane, group_lanes;  // experts of a lane, lanes of a group
+  bool vec;                        // 16-byte loads
 };
-void route_plan(RouteProblem *p, int num_sms);
-cudaError_t launch_experts_route(const RouteProblem &p, cudaStream_t stream);
+// Cuts the tokens into runs; returns the bytes of scratch that the plan needs.
+size_t route_plan(RouteProblem *p, int num_sms);
+cudaError_t launch_experts_route(RouteProblem p, cudaStream_t stream);
 
 struct ExpertsProblem {
   const void *x, *w;

@@ -1967,9 +1967,9 @@ int tx_experts_route(void *ctx, const TxRoute *route, uint32_t tokens, uint32_t 
   if (r.scores != TX_SCORES_SOFTMAX && r.scores != TX_SCORES_SIGMOID)
     return fail(c, TX_EINVAL, "experts_route: bad scores");
   if (!experts || experts > 1024) return fail(c, TX_EINVAL, "experts_route: 1..1024 experts");
-  if (!r.groups || experts % r.groups || !r.top_groups || r.top_groups > r.groups ||
+  if (!r.groups || r.groups > 64 || experts % r.groups || !r.top_groups || r.top_groups > r.groups ||
       (r.groups > 1 && r.group_best != 1 && r.group_best != 2))
-    return fail(c, TX_EINVAL, "experts_route: groups divide the experts, top_groups 1..groups, "
+    return fail(c, TX_EINVAL, "experts_route: 1..64 groups that divide the experts, top_groups 1..groups, "
                               "group_best 1 or 2");
   if (!top_k || top_k > 32 || top_k > experts / r.groups * r.top_groups)
     return fail(c, TX_EINVAL, "experts_route: top_k 1..32, at most the eligible experts");
@@ -2002,11 +2002,10 @@ int tx_experts_route(void *ctx, const TxRoute *route, uint32_t tokens, uint32_t 
   p.scale = r.scale; p.lengths = r.lengths; p.seq = r.seq;
   p.chosen = r.chosen; p.weights = r.weights;
   p.offsets = r.offsets; p.order = r.order; p.places = r.places;
-  tx::route_plan(&p, c->sms);
+  const size_t scratch = tx::route_plan(&p, c->sms);
   Parts parts;
-  const bool scratch = p.order && p.blocks > 1;
   if (scratch) {
-    e = parts_acquire(c, st, 1, (size_t)p.blocks * experts * 4, &parts);
+    e = parts_acquire(c, st, 1, scratch, &parts);
     if (e != cudaSuccess) return cuda_fail(c, e, "routing counts");
     p.counts = (uint32_t *)parts.sums;
   }
