@@ -393,23 +393,33 @@ struct Logits {
 };
 
 // ---- the plan -------------------------------------------------------------------------------
-// Exclusive sums of count[experts] into offset[experts + 1]; all threads of the block call it.
-__device__ void scan_counts(const uint32_t *count, uint32_t *offset, uint32_t experts) {
-  if (threadIdx.x < 32) {
-    uint32_t carry = 0;
-    for (uint32_t e0 = 0; e0 < experts; e0 += 32) {
-      const uint32_t e = e0 + threadIdx.x, own = e < experts ? count[e] : 0;
-      uint32_t v = own;
+// Exclusive sums of count[experts] into offset[experts + 1] (which may be count); parts is scratch of a
+// word for each warp.  All threads of the block call it.
+__device__ void scan_counts(const uint32_t *count, uint32_t *offset, uint32_t experts, uint32_t *parts) {
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x / 32;
+  uint32_t carry = 0;
+  for (uint32_t e0 = 0; e0 < experts; e0 += blockDim.x) {
+    const uint32_t e = e0 + threadIdx.x, own = e < experts ? count[e] : 0;
+    uint32_t v = own;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t u = __shfl_up_sync(kFull, v, o);
-        if ((int)threadIdx.x >= o) v += u;
-      }
-      if (e < experts) offset[e] = carry + v - own;
-      carry += __shfl_sync(kFull, v, 31);
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t u = __shfl_up_sync(kFull, v, o);
+      if ((int)lane >= o) v += u;
     }
-    if (threadIdx.x == 0) offset[experts] = carry;
+    if (lane == 31) parts[warp] = v;
+    __syncthreads();
+    uint32_t before = lane < warps ? parts[lane] : 0, all = before;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t u = __shfl_up_sync(kFull, all, o);
+      if ((int)lane >= o) all += u;
+    }
+    before = carry + __shfl_sync(kFull, all - before, warp);
+    if (e < experts) offset[e] = before + v - own;
+    carry += __shfl_sync(kFull, all, 31);
+    __syncthreads();
   }
+  if (threadIdx.x == 0) offset[experts] = carry;
   __syncthreads();
 }
 // The tokens of warp `warp` in the run of block `block`: [*first, *end).
@@ -419,8 +429,9 @@ __device__ __forceinline__ void warp_tokens(const RouteProblem &p, uint32_t bloc
   *first = (uint32_t)min(run + (uint64_t)warp * p.run_warp, last);
   *end = (uint32_t)min((uint64_t)*first + p.run_warp, last);
 }
-// A warp's pairs, whose ranks among them lie in p.places, go to their rows: before[e] is where the warp's
-// rows of expert e start.
+// A warp's pairs, whose ranks lie in p.places: before[e] is added to those of expert e, and, where that is
+// their row, the row filled.
+template <bool kRows>
 __device__ __forceinline__ void place_pairs(const RouteProblem &p, uint32_t first, uint32_t end,
                                             const uint32_t *before) {
   const uint64_t b = (uint64_t)end * p.top_k;
@@ -430,13 +441,13 @@ __device__ __forceinline__ void place_pairs(const RouteProblem &p, uint32_t firs
     if (e >= 0) {
       const uint32_t at = before[e] + (uint32_t)rank;
       p.places[i] = (int32_t)at;
-      p.order[at] = (int32_t)i;
+      if (kRows) p.order[at] = (int32_t)i;
     }
   }
 }
 
-// Shared memory: by_warp [kWarps][experts], offset [experts + 1], and for every token in work its chosen
-// experts and their keys, one more than there may be.
+// Shared memory: by_warp [kWarps][experts], offset [experts + 1], a word for each warp, the bias, for every
+// token in work its chosen experts and their keys, one more than there may be, and the lanes' sorted keys.
 constexpr uint32_t kSlotWords = 2 * (kMaxK + 1);
 
 template <int kLanes, int V, bool kScored, int kWarps>
@@ -449,18 +460,32 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
   // in their order.
   constexpr uint32_t kName = V - 1, kNameAll = 0xffff;
   constexpr int kMine = kMaxK / kLanes;  // chosen experts a lane weighs
+  constexpr bool kListed = V > 8;        // sorted keys behind the first in shared memory
   extern __shared__ __align__(16) uint8_t smem[];
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane % kLanes;
   const uint32_t slot = lane / kLanes, group_mask = (kLanes == 32 ? kFull : (1u << kLanes) - 1)
                                                    << (slot * kLanes);
   uint32_t *by_warp = reinterpret_cast<uint32_t *>(smem), *words = by_warp + warp * p.experts;
   uint32_t *offset = by_warp + kWarps * p.experts;
-  uint32_t *chosen = offset + p.experts + 1 + (warp * kTokens + slot) * kSlotWords;
+  uint32_t *parts = offset + p.experts + 1;
+  float *bias = reinterpret_cast<float *>(parts + kWarps);
+  uint32_t *chosen = reinterpret_cast<uint32_t *>(bias + (kScored ? kLanes * V : 0)) +
+                     (warp * kTokens + slot) * kSlotWords;
   uint32_t *chosen_key = chosen + kMaxK + 1;
-  if (p.order) {
+  uint32_t *list = chosen - (warp * kTokens + slot) * kSlotWords + kWarps * kTokens * kSlotWords +
+                   warp * V * 32 + lane;
+  if (p.order)
     for (uint32_t e = lane; e < p.experts; e += 32) words[e] = 0;
-    __syncwarp();
+  if constexpr (kScored) {
+    for (uint32_t e = threadIdx.x; e < kLanes * V; e += kThreads)
+      {
+        // by the lane last, so that lanes side by side meet banks side by side
+        const uint32_t at = e % kLanes * p.per_lane + e / kLanes;
+        bias[e] = p.bias && e / kLanes < p.per_lane && at < p.experts ? p.bias[at] : 0.f;
+      }
+    __syncthreads();
   }
+  __syncwarp();
   uint32_t first, end;
   warp_tokens(p, blockIdx.x, warp, &first, &end);
   const bool told = !kScored && p.logits_dtype == TX_BF16;
@@ -477,11 +502,55 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
   for (uint32_t t0 = first; t0 < end; t0 += kTokens) {
     const uint32_t token = t0 + slot;
     const bool here = token < end, had = valid;
-    float l[V], tol = 0.f;
+    float tol = 0.f, all_top = 0.f, all_sum = 1.f;  // of all logits, where the weights need them
     uint32_t key[V];
     bool near = false;
+    {
+      float c[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) l[i] = __uint_as_float(raw.w[i]);
+      for (int i = 0; i < V; ++i) {
+        c[i] = __uint_as_float(raw.w[i]);
+        if constexpr (kScored)
+          if (bias[i * kLanes + sub] == -INFINITY) c[i] = -INFINITY;
+      }
+      if (p.softmax && (kScored || !p.renormalise)) {
+        all_top = c[0];
+#pragma unroll
+        for (int i = 1; i < V; ++i) all_top = fmaxf(all_top, c[i]);
+        all_top = lanes_max<kLanes>(all_top);
+        float sum = 0.f;
+        if (!p.renormalise) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) sum += c[i] == -INFINITY ? 0.f : expf(c[i] - all_top);
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; ++i) sum += c[i] == -INFINITY ? 0.f : quick_exp(c[i] - all_top);
+        }
+        all_sum = lanes_sum<kLanes>(sum);
+      }
+      if constexpr (!kScored) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          near |= c[i] != c[i];
+          key[i] = told ? (quick_key(c[i]) & ~kNameAll) | (kNameAll - sub * p.per_lane - i)
+                        : (quick_key(c[i]) & ~kName) | (V - 1 - i);
+        }
+      } else {
+        const float inv = p.softmax ? quick_rcp(all_sum) : 1.f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float s = p.softmax ? quick_exp(c[i] - all_top) * inv : sigmoid(c[i]);
+          c[i] = c[i] == -INFINITY ? -INFINITY : s + bias[i * kLanes + sub];
+          near |= c[i] != c[i];
+        }
+        tol = score_tolerance<V>(p.softmax, inv);
+        uint32_t kept = kFull;
+        if (p.groups > 1) kept = keep_groups<kLanes, V, float>(p, sub, slot, c, tol, &near);
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          key[i] = kept >> i & 1 ? (quick_key(c[i]) & ~kName) | (V - 1 - i) : 0;
+      }
+    }
     // The next tokens' logits travel meanwhile.
     next += kTokens;
     if (p.lengths && next < end) {
@@ -494,64 +563,27 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
     }
     valid = next < end && (!p.lengths || row < length);
     raw.load(p, next, sub, valid);
-    if constexpr (!kScored) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        near |= l[i] != l[i];
-        key[i] = told ? (quick_key(l[i]) & ~kNameAll) | (kNameAll - sub * p.per_lane - i)
-                      : (quick_key(l[i]) & ~kName) | (V - 1 - i);
-      }
-    } else {
-      float c[V];
-      if (p.bias) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const uint32_t e = sub * p.per_lane + i;
-          c[i] = i < (int)p.per_lane && e < p.experts ? __ldg(p.bias + e) : 0.f;
-          if (c[i] == -INFINITY) l[i] = -INFINITY;
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) c[i] = 0.f;
-      }
-      float inv = 1.f;
-      if (p.softmax) {
-        float top = -INFINITY, sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < V; ++i) top = fmaxf(top, l[i]);
-        top = lanes_max<kLanes>(top);
-#pragma unroll
-        for (int i = 0; i < V; ++i) sum += l[i] == -INFINITY ? 0.f : quick_exp(l[i] - top);
-        inv = quick_rcp(lanes_sum<kLanes>(sum));
-#pragma unroll
-        for (int i = 0; i < V; ++i) c[i] = fmaf(quick_exp(l[i] - top), inv, c[i]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) c[i] += sigmoid(l[i]);
-      }
-      tol = score_tolerance<V>(p.softmax, inv);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        c[i] = l[i] == -INFINITY ? -INFINITY : c[i];
-        near |= c[i] != c[i];
-      }
-      uint32_t kept = kFull;
-      if (p.groups > 1) kept = keep_groups<kLanes, V, float>(p, sub, slot, c, tol, &near);
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        key[i] = kept >> i & 1 ? (quick_key(c[i]) & ~kName) | (V - 1 - i) : 0;
-    }
     sort_keys(key);
+    if constexpr (kListed) {
+#pragma unroll
+      for (int i = 1; i < V; ++i)
+        if (i <= (int)p.top_k) list[i * 32] = key[i];
+    }
     // The lowest lane with the largest head, names apart, has the next expert.
     const uint32_t names = told ? 0 : kName;
+    uint32_t taken = 0;
     for (uint32_t j = 0; j < p.top_k + !told; ++j) {
-      const uint32_t head = key[0] | names, top = lanes_max<kLanes>(head);
-      if (lane == __ffs(__ballot_sync(kFull, head == top) & group_mask) - 1) {
-        chosen[j] = told ? kNameAll - (key[0] & kNameAll) : sub * p.per_lane + kName - (key[0] & kName);
-        chosen_key[j] = key[0];
+      const uint32_t head = key[0], named = head | names, top = lanes_max<kLanes>(named);
+      if (lane == __ffs(__ballot_sync(kFull, named == top) & group_mask) - 1) {
+        chosen[j] = told ? kNameAll - (head & kNameAll) : sub * p.per_lane + kName - (head & kName);
+        chosen_key[j] = head;
+        if constexpr (kListed) {
+          key[0] = ++taken < V ? list[taken * 32] : 0;
+        } else {
 #pragma unroll
-        for (int i = 0; i + 1 < V; ++i) key[i] = key[i + 1];
-        key[V - 1] = 0;
+          for (int i = 0; i + 1 < V; ++i) key[i] = key[i + 1];
+          key[V - 1] = 0;
+        }
       }
     }
     __syncwarp();
@@ -584,41 +616,23 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
     }
     // Weights.  With a common factor taken out first: e^l by the largest l, and for the sigmoid
     // e^min(l, 0) / (1 + e^-|l|) by the largest of the numerators; renormalised it cancels.
-    float x[kMine], top = -INFINITY, total = 1.f;
+    float x[kMine], top = -INFINITY;
 #pragma unroll
     for (int m = 0; m < kMine; ++m) {
       x[m] = e[m] != kNone ? logit_at(p, token, e[m]) : -INFINITY;
       if (e[m] != kNone) top = fmaxf(top, p.softmax ? x[m] : fminf(x[m], 0.f));
     }
-    if (p.renormalise) {
-      top = lanes_max<kLanes>(top);
-    } else if (p.softmax) {
-      top = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < V; ++i) top = fmaxf(top, l[i]);
-      top = lanes_max<kLanes>(top);
-    } else {
-      top = 0.f;
-    }
+    top = p.renormalise ? lanes_max<kLanes>(top) : p.softmax ? all_top : 0.f;
     float s[kMine], sum = 0.f;
 #pragma unroll
     for (int m = 0; m < kMine; ++m) {
       s[m] = 0.f;
       if (e[m] == kNone) continue;
       s[m] = p.softmax ? expf(x[m] - top)
-                       : expf(fminf(x[m], 0.f) - top) / (1.f + expf(-fabsf(x[m])));
+                       : expf(fminf(x[m], 0.f) - top) * quick_rcp(1.f + expf(-fabsf(x[m])));
       sum += s[m];
     }
-    if (p.renormalise) {
-      total = lanes_sum<kLanes>(sum);
-    } else if (p.softmax) {
-      sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (l[i] != -INFINITY) sum += expf(l[i] - top);
-      total = lanes_sum<kLanes>(sum);
-    }
-    const float factor = p.scale / total;
+    const float factor = p.scale * quick_rcp(p.renormalise ? lanes_sum<kLanes>(sum) : all_sum);
 #pragma unroll
     for (int m = 0; m < kMine; ++m) {
       const uint32_t j = sub + m * kLanes;
@@ -657,81 +671,89 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
   // The counts of the warps before each warp, and of the block.
   for (uint32_t e = threadIdx.x; e < p.experts; e += kThreads) {
     uint32_t run = 0;
+#pragma unroll 8
     for (uint32_t w = 0; w < kWarps; ++w) {
       const uint32_t n = by_warp[w * p.experts + e];
       by_warp[w * p.experts + e] = run;
       run += n;
     }
     offset[e] = run;
-    if (gridDim.x > 1) p.counts[(size_t)blockIdx.x * p.experts + e] = run;
+    if (gridDim.x > 1) p.counts[(size_t)e * gridDim.x + blockIdx.x] = run;
   }
   __syncthreads();
   if (gridDim.x > 1) {
-    uint32_t *to = p.counts + ((size_t)gridDim.x + (size_t)blockIdx.x * kWarps) * p.experts;
-    for (uint32_t i = threadIdx.x; i < kWarps * p.experts; i += kThreads) to[i] = by_warp[i];
+    place_pairs<false>(p, first, end, words);
     return;
   }
-  scan_counts(offset, offset, p.experts);
+  scan_counts(offset, offset, p.experts, parts);
   for (uint32_t e = threadIdx.x; e <= p.experts; e += kThreads) p.offsets[e] = (int32_t)offset[e];
   for (uint32_t e = lane; e < p.experts; e += 32) words[e] += offset[e];
   __syncwarp();
-  place_pairs(p, first, end, words);
+  place_pairs<true>(p, first, end, words);
 }
 
-// Places the pairs of run blockIdx.x behind those of the runs before it.
-__global__ void __launch_bounds__(1024, 1) place_kernel(const __grid_constant__ RouteProblem p) {
-  extern __shared__ __align__(16) uint8_t smem[];
-  const uint32_t kWarps = p.warps, kThreads = blockDim.x;
-  uint32_t *by_warp = reinterpret_cast<uint32_t *>(smem), *total = by_warp + kWarps * p.experts;
-  uint32_t *base = total + p.experts, *offset = base + p.experts;
-  for (uint32_t e = threadIdx.x; e < p.experts; e += kThreads) total[e] = base[e] = 0;
-  const uint32_t *from = p.counts + ((size_t)gridDim.x + (size_t)blockIdx.x * kWarps) * p.experts;
-  for (uint32_t i = threadIdx.x; i < kWarps * p.experts; i += kThreads) by_warp[i] = __ldcg(from + i);
-  __syncthreads();
-  // Threads side by side take experts, the rest of them runs.
-  uint32_t wide = 32;
-  while (wide < p.experts && wide < kThreads) wide *= 2;
-  const uint32_t part = threadIdx.x / wide, parts = kThreads / wide;
-  for (uint32_t e = threadIdx.x % wide; e < p.experts; e += wide) {
-    uint32_t all = 0, before = 0;
-#pragma unroll 8
-    for (uint32_t b = part; b < gridDim.x; b += parts) {
-      const uint32_t n = __ldcg(p.counts + (size_t)b * p.experts + e);
-      all += n;
-      if (b < blockIdx.x) before += n;
+// Places the pairs of run blockIdx.x, ranked within it, behind those of the runs before it.
+constexpr int kPlaceThreads = 1024;
+__global__ void __launch_bounds__(kPlaceThreads, 1)
+    place_kernel(const __grid_constant__ RouteProblem p) {
+  __shared__ uint32_t total[1024], base[1024], offset[1025], parts[32];
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, runs = gridDim.x;
+  // A warp sums the counts of an expert over the runs, and of those before this one; the loads of four
+  // experts are on their way at once.
+  for (uint32_t e0 = warp * 4; e0 < p.experts; e0 += kPlaceThreads / 8) {
+    uint32_t all[4] = {}, before[4] = {};
+    for (uint32_t b = lane; b < runs; b += 32) {
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i) {
+        const uint32_t n = e0 + i < p.experts ? __ldcg(p.counts + (size_t)(e0 + i) * runs + b) : 0;
+        all[i] += n;
+        before[i] += b < blockIdx.x ? n : 0;
+      }
     }
-    atomicAdd(total + e, all);
-    atomicAdd(base + e, before);
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+      const uint32_t a = __reduce_add_sync(kFull, all[i]), b = __reduce_add_sync(kFull, before[i]);
+      if (lane == 0 && e0 + i < p.experts) {
+        total[e0 + i] = a;
+        base[e0 + i] = b;
+      }
+    }
   }
   __syncthreads();
-  scan_counts(total, offset, p.experts);
+  scan_counts(total, offset, p.experts, parts);
   if (blockIdx.x == 0)
-    for (uint32_t e = threadIdx.x; e <= p.experts; e += kThreads) p.offsets[e] = (int32_t)offset[e];
-  const uint32_t warp = threadIdx.x >> 5;
-  uint32_t *before = by_warp + warp * p.experts;
-  for (uint32_t e = threadIdx.x & 31; e < p.experts; e += 32) before[e] += offset[e] + base[e];
-  __syncwarp();
-  uint32_t first, end;
-  warp_tokens(p, blockIdx.x, warp, &first, &end);
-  place_pairs(p, first, end, before);
+    for (uint32_t e = threadIdx.x; e <= p.experts; e += kPlaceThreads) p.offsets[e] = (int32_t)offset[e];
+  for (uint32_t e = threadIdx.x; e < p.experts; e += kPlaceThreads) base[e] += offset[e];
+  __syncthreads();
+  const uint64_t first = min((uint64_t)blockIdx.x * p.run, (uint64_t)p.tokens) * p.top_k;
+  const uint64_t end = min((uint64_t)(blockIdx.x + 1) * p.run, (uint64_t)p.tokens) * p.top_k;
+#pragma unroll 4
+  for (uint64_t i = first + threadIdx.x; i < end; i += kPlaceThreads) {
+    const int32_t e = p.chosen[i], rank = p.places[i];
+    if (e >= 0) {
+      const uint32_t at = base[e] + (uint32_t)rank;
+      p.places[i] = (int32_t)at;
+      p.order[at] = (int32_t)i;
+    }
+  }
 }
 
 template <int kLanes, int V, bool kScored, int kWarps>
 cudaError_t run_warps(RouteProblem p, cudaStream_t stream) {
   constexpr uint32_t kTokens = 32 / kLanes;
-  p.warps = kWarps;
   p.run_warp = ((p.run + kWarps - 1) / kWarps + kTokens - 1) / kTokens * kTokens;
   const size_t size = p.logits_dtype == TX_BF16 ? 2 : 4;
   p.vec = p.per_lane == V && V * size % 16 == 0 && p.experts % (16 / size) == 0 &&
           p.ld * size % 16 == 0 && (uintptr_t)p.logits % 16 == 0;
-  const uint32_t bytes = ((kWarps + 1) * p.experts + 1 + kWarps * kTokens * kSlotWords) * 4;
-  static std::atomic<uint64_t> seen{0}, seen_place{0};
+  const uint32_t bytes = ((kWarps + 1) * p.experts + 1 + kWarps + (kScored ? kLanes * V : 0) +
+                          kWarps * kTokens * kSlotWords + (V > 8 ? kWarps * V * 32 : 0)) *
+                         4;
+  static std::atomic<uint64_t> seen{0};
   cudaError_t e = allow_smem((const void *)route_kernel<kLanes, V, kScored, kWarps>, 232448, seen);
   if (e != cudaSuccess) return e;
   route_kernel<kLanes, V, kScored, kWarps><<<p.blocks, 32 * kWarps, bytes, stream>>>(p);
   if ((e = cudaGetLastError()) != cudaSuccess || p.blocks == 1 || !p.order) return e;
-  if ((e = allow_smem((const void *)place_kernel, 232448, seen_place)) != cudaSuccess) return e;
-  place_kernel<<<p.blocks, 32 * kWarps, ((kWarps + 3) * p.experts + 1) * 4, stream>>>(p);
+  place_kernel<<<p.blocks, kPlaceThreads, 0, stream>>>(p);
   return cudaGetLastError();
 }
 template <int kLanes, int V>
@@ -745,15 +767,17 @@ cudaError_t run(const RouteProblem &p, cudaStream_t stream) {
 
 // Runs of tokens: one while a single block is the faster way, else a block for each SM.
 size_t route_plan(RouteProblem *p, int num_sms) {
-  p->run = std::max<uint32_t>(128, (uint32_t)(((uint64_t)p->tokens + num_sms - 1) / num_sms));
+  p->run = std::max<uint32_t>(p->tokens <= 256 ? 256 : 32,
+                              (uint32_t)(((uint64_t)p->tokens + num_sms - 1) / num_sms));
   p->blocks = (p->tokens + p->run - 1) / p->run;
-  return p->order && p->blocks > 1 ? (size_t)p->blocks * (kMostWarps + 1) * p->experts * 4 : 0;
+  return p->order && p->blocks > 1 ? (size_t)p->blocks * p->experts * 4 : 0;
 }
 
 cudaError_t launch_experts_route(RouteProblem p, cudaStream_t stream) {
-  // Experts of a lane: as few lanes as 8 (4 of up to 16, 16 or 32 of many) experts each allow.  With
-  // groups a group has to be whole lanes; where no number does that, group_lanes is 0.
-  uint32_t most = p.experts <= 16 ? 4 : p.experts <= 256 ? 8 : p.experts <= 512 ? 16 : 32;
+  // Experts of a lane: 8 where 32 lanes can hold them.  (16 make a third fewer instructions a token but
+  // leave too few tokens in work: 66 / 48 us for 16384 tokens and 256 experts in groups.)  With groups a
+  // group has to be whole lanes; where no number of experts a lane does that, group_lanes is 0.
+  const uint32_t most = p.experts <= 256 ? 8 : p.experts <= 512 ? 16 : 32;
   p.per_lane = most;
   p.group_lanes = 0;
   if (p.groups > 1) {
@@ -765,7 +789,6 @@ cudaError_t launch_experts_route(RouteProblem p, cudaStream_t stream) {
       }
   }
   const uint32_t lanes = (p.experts + p.per_lane - 1) / p.per_lane;
-  if (most == 4 && lanes <= 4) return run<4, 4>(p, stream);
   if (most == 32) return run<32, 32>(p, stream);
   if (most == 16) return run<32, 16>(p, stream);
   if (lanes <= 4) return run<4, 8>(p, stream);

@@ -273,9 +273,9 @@ struct RouteProblem {
   float *weights;
   int32_t *offsets, *order, *places;  // the plan, or NULL
   uint32_t run, blocks;    // tokens of a block (route_plan)
-  uint32_t *counts;        // scratch with blocks > 1: [blocks][experts], then [blocks][warps][experts]
+  uint32_t *counts;        // scratch with blocks > 1: [experts][blocks]
   // set by the launcher
-  uint32_t warps, run_warp;        // of a block, and the tokens of a warp
+  uint32_t run_warp;               // tokens of a warp
   uint32_t per_lane, group_lanes;  // experts of a lane, lanes of a group
   bool vec;                        // 16-byte loads
 };
