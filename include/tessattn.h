@@ -627,7 +627,7 @@ typedef struct {
   TxNorm after, before;
 } TxBlockNorm;
 
-/* cols at most 16384.  out or h may be x, or y without places, with the same dtype and row stride.  A
+/* cols at most 16384, top_k at most 32.  out or h may be x, or y without places, with the same dtype and row stride.  A
  * place >= y_rows is left out and reported as TX_EINVAL by the next tx_sync. */
 int tx_block_norm(void *ctx, const TxBlockNorm *block, uint32_t rows, uint32_t cols, void *stream);
 

@@ -5,9 +5,13 @@
 // none.  Everything is fp32 from the loads to the one rounding of each output; h is the norm of r as it
 // is before r is rounded.  The joined sum runs in the order of j, and a row whose place is negative is not read.
 //
-// Bound: HBM, each row read once and written once.  A row lives in the registers of the threads that take
-// it, so that the mean and the deviations of a LayerNorm are two passes over registers.
+// Bound: HBM, each row read once and written once.  A row is W warps with C vectors of V elements a thread in
+// registers, so that the mean and the deviations of a LayerNorm are two passes over registers.  Few
+// registers a thread and a row's words loaded a row ahead keep enough of them on their way: a warp a row
+// (100 registers) left 16 warps an SM and took 66 / ?? us for 8192 joined rows of 1024.
 #include <cuda_runtime.h>
+
+#include <algorithm>
 
 #include "../../include/tessattn.h"
 #include "common.cuh"
@@ -21,12 +25,16 @@ template <int V, typename T>
 struct Words {
   static constexpr int kWords = V * (int)sizeof(T) / 4;
   uint32_t w[kWords ? kWords : 1];
-  __device__ __forceinline__ void load(const T *p) {
+  __device__ __forceinline__ void load(const void *base, int, size_t at) {
+    const T *p = static_cast<const T *>(base) + at;
     if constexpr (V == 1) {
       if constexpr (sizeof(T) == 4)
         w[0] = __float_as_uint(*p);
       else
         w[0] = (uint32_t)*p << 16;
+    } else if constexpr (kWords == 2) {
+      const uint2 v = *reinterpret_cast<const uint2 *>(p);
+      w[0] = v.x; w[1] = v.y;
     } else {
 #pragma unroll
       for (int i = 0; i < kWords; i += 4) {
@@ -42,6 +50,26 @@ struct Words {
       return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
   }
 };
+// The same with the type looked up as they are loaded.
+struct Any {};
+template <int V>
+struct Words<V, Any> {
+  float f[V];
+  __device__ __forceinline__ void load(const void *base, int dtype, size_t at) {
+    if (dtype == TX_BF16) {
+      Words<V, uint16_t> r;
+      r.load(base, dtype, at);
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[i] = r.at(i);
+    } else {
+      Words<V, float> r;
+      r.load(base, dtype, at);
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[i] = r.at(i);
+    }
+  }
+  __device__ __forceinline__ float at(int i) const { return f[i]; }
+};
 
 template <int V>
 __device__ __forceinline__ void store_as(void *base, int dtype, size_t at, const float *f) {
@@ -51,59 +79,59 @@ __device__ __forceinline__ void store_as(void *base, int dtype, size_t at, const
     else
       static_cast<float *>(base)[at] = f[0];
   } else if (dtype == TX_BF16) {
-    *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(base) + at) =
-        make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
-                   pack_bf16x2(f[6], f[7]));
+    uint16_t *p = static_cast<uint16_t *>(base) + at;
+    if constexpr (V == 4)
+      *reinterpret_cast<uint2 *>(p) = make_uint2(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]));
+    else
+      *reinterpret_cast<uint4 *>(p) = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]),
+                                                 pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
   } else {
     float4 *p = reinterpret_cast<float4 *>(static_cast<float *>(base) + at);
-    p[0] = make_float4(f[0], f[1], f[2], f[3]);
-    p[1] = make_float4(f[4], f[5], f[6], f[7]);
+#pragma unroll
+    for (int i = 0; i < V; i += 4) p[i / 4] = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
   }
 }
 template <int V>
 __device__ __forceinline__ void load_as(const void *base, int dtype, size_t at, float *f) {
-  if (dtype == TX_BF16) {
-    Words<V, uint16_t> r;
-    r.load(static_cast<const uint16_t *>(base) + at);
+  Words<V, Any> r;
+  r.load(base, dtype, at);
 #pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = r.at(i);
-  } else {
-    Words<V, float> r;
-    r.load(static_cast<const float *>(base) + at);
-#pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = r.at(i);
-  }
+  for (int i = 0; i < V; ++i) f[i] = r.at(i);
 }
 
-// The sum of v over the kThreads threads of a row; `turn` numbers the row's sums, so that two sums in turn
-// use buffers of their own.
-template <int kThreads>
-__device__ __forceinline__ float row_sum(float v, float (*buf)[32], int &turn) {
-  v = warp_sum(v);
-  if constexpr (kThreads > 32) {
-    float *b = buf[turn++ & 1];
-    if ((threadIdx.x & 31) == 0) b[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = b[0];
+// The W warps of a row: their sums meet in shared memory, in two buffers by turns (who writes one again has
+// passed the barrier of the other, before which all had read it).
+template <int W>
+struct RowTeam {
+  float (*buf)[W];  // [2][W]
+  uint32_t barrier;  // of its own among the block's
+  int turn;
+  __device__ __forceinline__ float sum(float v) {
+    v = warp_sum(v);
+    if constexpr (W > 1) {
+      float *b = buf[turn++ & 1];
+      if ((threadIdx.x & 31) == 0) b[threadIdx.x / 32 % W] = v;
+      asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(32 * W) : "memory");
+      v = b[0];
 #pragma unroll
-    for (int i = 1; i < kThreads / 32; ++i) v += b[i];
+      for (int i = 1; i < W; ++i) v += b[i];
+    }
+    return v;
   }
-  return v;
-}
+};
 
-// A row's elements: thread t holds vectors t, t + kThreads, ... of V elements.
-template <int kThreads, int V, int C>
+template <int W, int V, int C>
 __device__ __forceinline__ void apply_norm(const BlockNorm &n, float (&v)[C][V], uint32_t cols,
-                                           uint32_t t, float (*buf)[32], int &turn) {
+                                           float inv_cols, uint32_t t, RowTeam<W> &team) {
   if (n.kind == TX_NORM_NONE) return;
-  auto in = [&](int c) { return (t + c * kThreads) * V < cols; };
+  auto in = [&](int c) { return (t + c * 32 * W) * V < cols; };
   if (n.kind == TX_NORM_LAYER) {
     float s = 0.f;
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
       for (int i = 0; i < V; ++i) s += v[c][i];
-    const float mean = row_sum<kThreads>(s, buf, turn) / (float)cols;
+    const float mean = team.sum(s) * inv_cols;
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -114,11 +142,11 @@ __device__ __forceinline__ void apply_norm(const BlockNorm &n, float (&v)[C][V],
   for (int c = 0; c < C; ++c)
 #pragma unroll
     for (int i = 0; i < V; ++i) ss = fmaf(v[c][i], v[c][i], ss);
-  const float inv = rsqrtf(row_sum<kThreads>(ss, buf, turn) / (float)cols + n.eps);
+  const float inv = rsqrtf(fmaf(team.sum(ss), inv_cols, n.eps));
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     if (!in(c)) continue;
-    const size_t at = (size_t)(t + c * kThreads) * V;
+    const size_t at = (size_t)(t + c * 32 * W) * V;
     float w[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) w[i] = 1.f;
@@ -137,134 +165,184 @@ __device__ __forceinline__ void apply_norm(const BlockNorm &n, float (&v)[C][V],
   }
 }
 
-template <typename XT, typename YT, int kThreads, int V, int C>
-__global__ void __launch_bounds__(kThreads > 32 ? kThreads : 256)
+// Rows of a block, and blocks of an SM at 64 registers a thread.
+template <int W>
+struct Shape {
+  static constexpr int kRows = W >= 4 ? 1 : W == 1 ? 4 : 2;
+  static constexpr int kThreads = 32 * W * kRows;
+  static constexpr int kResident = 1024 / kThreads;
+};
+
+template <typename XT, typename YT, int W, int V, int C, bool kJoin>
+__global__ void __launch_bounds__(Shape<W>::kThreads, Shape<W>::kResident)
     block_norm_kernel(const __grid_constant__ BlockNormProblem p) {
-  __shared__ float buf[2][32];
-  int turn = 0;
-  const uint32_t t = kThreads > 32 ? threadIdx.x : threadIdx.x & 31;
-  const uint32_t row = kThreads > 32 ? blockIdx.x : blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (row >= p.rows) return;
-  auto in = [&](int c) { return (t + c * kThreads) * V < p.cols; };
+  constexpr int kRows = Shape<W>::kRows;
+  constexpr int kAhead = V * C > 8 ? 2 : sizeof(YT) == 4 ? 4 : 8;  // joined rows on their way at once
+  __shared__ float buf[kRows][2][W];
+  const uint32_t own = threadIdx.x / (32 * W), t = threadIdx.x % (32 * W), lane = threadIdx.x & 31;
+  RowTeam<W> team{buf[own], 1 + own, 0};
+  const uint32_t step = gridDim.x * kRows;
+  const float inv_cols = 1.f / (float)p.cols;
+  auto in = [&](int c) { return (t + c * 32 * W) * V < p.cols; };
   Words<V, XT> x[C];
-  if (p.x) {
-    const XT *from = static_cast<const XT *>(p.x) + (size_t)row * p.ldx;
-#pragma unroll
-    for (int c = 0; c < C; ++c)
-      if (in(c)) x[c].load(from + (size_t)(t + c * kThreads) * V);
-  }
-  float v[C][V];
-#pragma unroll
-  for (int c = 0; c < C; ++c)
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[c][i] = 0.f;
-  if (p.places) {
-#pragma unroll 2
-    for (uint32_t j = 0; j < p.top_k; ++j) {
-      const int32_t place = __ldg(p.places + (size_t)row * p.top_k + j);
-      if (place < 0) continue;
-      if ((uint32_t)place >= p.y_rows) {
-        report_status(p.status, kStatusBadArg);
-        continue;
-      }
-      const float w = __ldg(p.weights + (size_t)row * p.top_k + j);
-      const YT *from = static_cast<const YT *>(p.y) + (size_t)place * p.ldy;
-      Words<V, YT> y[C];
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-        if (in(c)) y[c].load(from + (size_t)(t + c * kThreads) * V);
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-        if (in(c))
-#pragma unroll
-          for (int i = 0; i < V; ++i) v[c][i] = fmaf(w, y[c].at(i), v[c][i]);
-    }
-  } else if (p.y) {
-    const YT *from = static_cast<const YT *>(p.y) + (size_t)row * p.ldy;
-#pragma unroll
-    for (int c = 0; c < C; ++c)
-      if (in(c)) {
-        Words<V, YT> y;
-        y.load(from + (size_t)(t + c * kThreads) * V);
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[c][i] = y.at(i);
-      }
-  }
-  if (p.y) apply_norm<kThreads, V, C>(p.after, v, p.cols, t, buf, turn);
-  if (p.gate) {
-    uint32_t g = 0;
-    if (p.cu)
-      g = warp_find_seq(p.cu, p.gate_rows, row, threadIdx.x & 31);
-    else if (p.seq)
-      g = row / p.seq;
+  Words<V, YT> y[C];
+  int32_t place = -1;
+  float weight = 0.f;
+  auto fetch = [&](uint32_t row) {
+    if (row >= p.rows) return;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       if (!in(c)) continue;
-      float f[V];
-      load_as<V>(p.gate, p.gate_dtype, (size_t)g * p.ldg + (size_t)(t + c * kThreads) * V, f);
-#pragma unroll
-      for (int i = 0; i < V; ++i) v[c][i] *= f[i];
+      const size_t at = (size_t)(t + c * 32 * W) * V;
+      if (p.x) x[c].load(p.x, p.x_dtype, (size_t)row * p.ldx + at);
+      if (!kJoin && p.y) y[c].load(p.y, p.y_dtype, (size_t)row * p.ldy + at);
     }
-  }
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    if (!in(c)) continue;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      v[c][i] = p.y ? v[c][i] * p.y_scale : 0.f;
-      if (p.x) v[c][i] = fmaf(p.x_scale, x[c].at(i), v[c][i]);
+    if (kJoin && lane < p.top_k) {
+      place = __ldg(p.places + (size_t)row * p.top_k + lane);
+      weight = __ldg(p.weights + (size_t)row * p.top_k + lane);
     }
-    if (p.out)
-      store_as<V>(p.out, p.out_dtype, (size_t)row * p.ldo + (size_t)(t + c * kThreads) * V, v[c]);
-  }
-  if (!p.h) return;
-  apply_norm<kThreads, V, C>(p.before, v, p.cols, t, buf, turn);
+  };
+  uint32_t row = blockIdx.x * kRows + own;
+  fetch(row);
+  for (; row < p.rows; row += step) {
+    float v[C][V], r[C][V];
 #pragma unroll
-  for (int c = 0; c < C; ++c)
-    if (in(c))
-      store_as<V>(p.h, p.h_dtype, (size_t)row * p.ldh + (size_t)(t + c * kThreads) * V, v[c]);
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        v[c][i] = !kJoin && p.y && in(c) ? y[c].at(i) : 0.f;
+        r[c][i] = p.x && in(c) ? p.x_scale * x[c].at(i) : 0.f;
+      }
+    const int32_t here = place;
+    const float here_weight = weight;
+    fetch(row + step);
+    if constexpr (kJoin) {
+      if (lane < p.top_k && here >= 0 && (uint32_t)here >= p.y_rows)
+        report_status(p.status, kStatusBadArg);
+      for (uint32_t j0 = 0; j0 < p.top_k; j0 += kAhead) {
+        Words<V, YT> z[kAhead][C];
+        float w[kAhead];
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+          const uint32_t j = j0 + a;
+          const uint32_t at = (uint32_t)__shfl_sync(0xffffffffu, here, j & 31);
+          w[a] = __shfl_sync(0xffffffffu, here_weight, j & 31);
+          const bool is = j < p.top_k && at < p.y_rows;  // a negative place is beyond all rows
+          if (!is) w[a] = 0.f;
+#pragma unroll
+          for (int c = 0; c < C; ++c) {
+            if (is && in(c)) {
+              z[a][c].load(p.y, p.y_dtype, (size_t)at * p.ldy + (size_t)(t + c * 32 * W) * V);
+            } else {
+              z[a][c] = {};
+            }
+          }
+        }
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+          for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[c][i] = fmaf(w[a], z[a][c].at(i), v[c][i]);
+      }
+    }
+    if (p.y) {
+      apply_norm<W, V, C>(p.after, v, p.cols, inv_cols, t, team);
+      uint32_t g = 0;
+      if (p.gate)
+        g = p.cu ? warp_find_seq(p.cu, p.gate_rows, row, lane) : p.seq ? row / p.seq : 0;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        if (!in(c)) continue;
+        float f[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[i] = 1.f;
+        if (p.gate)
+          load_as<V>(p.gate, p.gate_dtype, (size_t)g * p.ldg + (size_t)(t + c * 32 * W) * V, f);
+#pragma unroll
+        for (int i = 0; i < V; ++i) r[c][i] = fmaf(p.y_scale, v[c][i] * f[i], r[c][i]);
+      }
+    }
+    if (p.out) {
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+        if (in(c))
+          store_as<V>(p.out, p.out_dtype, (size_t)row * p.ldo + (size_t)(t + c * 32 * W) * V, r[c]);
+    }
+    if (!p.h) continue;
+    apply_norm<W, V, C>(p.before, r, p.cols, inv_cols, t, team);
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if (in(c))
+        store_as<V>(p.h, p.h_dtype, (size_t)row * p.ldh + (size_t)(t + c * 32 * W) * V, r[c]);
+  }
 }
 
-template <typename XT, typename YT, int kThreads, int V, int C>
-cudaError_t run(const BlockNormProblem &p, cudaStream_t stream) {
-  const uint32_t blocks = kThreads > 32 ? p.rows : (p.rows + 7) / 8;
-  block_norm_kernel<XT, YT, kThreads, V, C>
-      <<<blocks, kThreads > 32 ? kThreads : 256, 0, stream>>>(p);
+template <typename XT, typename YT, int W, int V, int C>
+cudaError_t run(const BlockNormProblem &p, int num_sms, cudaStream_t stream) {
+  using S = Shape<W>;
+  const uint32_t blocks = std::min<uint32_t>((p.rows + S::kRows - 1) / S::kRows,
+                                             (uint32_t)(num_sms * S::kResident));
+  if (p.places)
+    block_norm_kernel<XT, YT, W, V, C, true><<<blocks, S::kThreads, 0, stream>>>(p);
+  else
+    block_norm_kernel<XT, YT, W, V, C, false><<<blocks, S::kThreads, 0, stream>>>(p);
   return cudaGetLastError();
 }
 
+// As many warps as the row has vectors for, up to 16.
 template <typename XT, typename YT>
-cudaError_t run_types(const BlockNormProblem &p, cudaStream_t stream) {
-  if (!p.vec) {
-    if (p.cols <= 32 * 8) return run<XT, YT, 32, 1, 8>(p, stream);
-    if (p.cols <= 128 * 16) return run<XT, YT, 128, 1, 16>(p, stream);
-    return run<XT, YT, 512, 1, 32>(p, stream);
-  }
-  if (p.cols <= 32 * 8) return run<XT, YT, 32, 8, 1>(p, stream);
-  if (p.cols <= 32 * 16) return run<XT, YT, 32, 8, 2>(p, stream);
-  if (p.cols <= 32 * 32) return run<XT, YT, 32, 8, 4>(p, stream);
-  if (p.cols <= 128 * 16) return run<XT, YT, 128, 8, 2>(p, stream);
-  if (p.cols <= 128 * 32) return run<XT, YT, 128, 8, 4>(p, stream);
-  return run<XT, YT, 512, 8, 4>(p, stream);
+cudaError_t run_vectors(const BlockNormProblem &p, int num_sms, cudaStream_t stream) {
+  const uint32_t warps = (p.cols + 255) / 256;
+  if (warps <= 1) return run<XT, YT, 1, 8, 1>(p, num_sms, stream);
+  if (warps <= 2) return run<XT, YT, 2, 8, 1>(p, num_sms, stream);
+  if (warps <= 3) return run<XT, YT, 3, 8, 1>(p, num_sms, stream);
+  if (warps <= 4) return run<XT, YT, 4, 8, 1>(p, num_sms, stream);
+  if (warps <= 8) return run<XT, YT, 8, 8, 1>(p, num_sms, stream);
+  if (warps <= 16) return run<XT, YT, 8, 8, 2>(p, num_sms, stream);
+  if (warps <= 32) return run<XT, YT, 16, 8, 2>(p, num_sms, stream);
+  return run<XT, YT, 16, 8, 4>(p, num_sms, stream);
+}
+cudaError_t run_fours(const BlockNormProblem &p, int num_sms, cudaStream_t stream) {
+  const uint32_t warps = (p.cols + 127) / 128;
+  if (warps <= 1) return run<Any, Any, 1, 4, 1>(p, num_sms, stream);
+  if (warps <= 4) return run<Any, Any, 4, 4, 1>(p, num_sms, stream);
+  if (warps <= 16) return run<Any, Any, 8, 4, 2>(p, num_sms, stream);
+  return run<Any, Any, 16, 4, 8>(p, num_sms, stream);
+}
+cudaError_t run_ones(const BlockNormProblem &p, int num_sms, cudaStream_t stream) {
+  if (p.cols <= 32 * 8) return run<Any, Any, 1, 1, 8>(p, num_sms, stream);
+  if (p.cols <= 128 * 8) return run<Any, Any, 4, 1, 8>(p, num_sms, stream);
+  if (p.cols <= 512 * 8) return run<Any, Any, 16, 1, 8>(p, num_sms, stream);
+  return run<Any, Any, 16, 1, 32>(p, num_sms, stream);
 }
 
 }  // namespace
 
-cudaError_t launch_block_norm(BlockNormProblem p, cudaStream_t stream) {
-  p.vec = p.cols % 8 == 0;
-  auto row = [&](const void *base, uint64_t ld) {
-    if (base && ((uintptr_t)base % 16 || ld % 8)) p.vec = false;
+cudaError_t launch_block_norm(const BlockNormProblem &p, int num_sms, cudaStream_t stream) {
+  // The widest of 8, 4 and 1 elements in which every row is whole vectors on their boundaries.
+  uint32_t v = p.cols % 8 == 0 ? 8 : p.cols % 4 == 0 ? 4 : 1;
+  auto row = [&](const void *base, uint64_t ld, int dtype) {
+    if (!base) return;
+    while (v > 1 && (ld % v || (uintptr_t)base % std::min<uint64_t>(16, v * (dtype == TX_BF16 ? 2 : 4))))
+      v = v == 8 ? 4 : 1;
   };
-  row(p.x, p.ldx); row(p.y, p.ldy); row(p.out, p.ldo); row(p.h, p.ldh); row(p.gate, p.ldg);
+  row(p.x, p.ldx, p.x_dtype);
+  row(p.y, p.ldy, p.y_dtype);
+  row(p.out, p.ldo, p.out_dtype);
+  row(p.h, p.ldh, p.h_dtype);
+  row(p.gate, p.ldg, p.gate_dtype);
   for (const BlockNorm *n : {&p.after, &p.before}) {
-    row(n->weight, 0);
-    row(n->bias, 0);
+    row(n->weight, 0, n->dtype);
+    row(n->bias, 0, n->dtype);
   }
+  if (v == 1) return run_ones(p, num_sms, stream);
+  if (v == 4) return run_fours(p, num_sms, stream);
   if (p.x_dtype == TX_F32)
-    return p.y_dtype == TX_F32 ? run_types<float, float>(p, stream)
-                               : run_types<float, uint16_t>(p, stream);
-  return p.y_dtype == TX_F32 ? run_types<uint16_t, float>(p, stream)
-                             : run_types<uint16_t, uint16_t>(p, stream);
+    return p.y_dtype == TX_F32 ? run_vectors<float, float>(p, num_sms, stream)
+                               : run_vectors<float, uint16_t>(p, num_sms, stream);
+  return p.y_dtype == TX_F32 ? run_vectors<uint16_t, float>(p, num_sms, stream)
+                             : run_vectors<uint16_t, uint16_t>(p, num_sms, stream);
 }
 
 }  // namespace tx

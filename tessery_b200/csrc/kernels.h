@@ -320,10 +320,9 @@ struct BlockNormProblem {
   uint32_t seq;
   float x_scale, y_scale;
   BlockNorm after, before;
-  bool vec;  // 16-byte accesses: set by the launcher
   int *status;
 };
-cudaError_t launch_block_norm(BlockNormProblem p, cudaStream_t stream);
+cudaError_t launch_block_norm(const BlockNormProblem &p, int num_sms, cudaStream_t stream);
 
 // ---- BERT fp32 forward (bert_ops.cu) ----
 // Word + token-type-0 + absolute-position embeddings of `tokens` tokens, LayerNorm'd; the

@@ -2093,8 +2093,8 @@ int tx_block_norm(void *ctx, const TxBlockNorm *block, uint32_t rows, uint32_t c
       if (o->data && o->data == i->data &&
           (o->dtype != i->dtype || o->ld != i->ld || (i == &b.y && b.places)))
         return fail(c, TX_EINVAL, "block_norm: in place needs equal dtypes and strides, and no places");
-  if (b.places && (!b.y.data || !b.weights || !b.top_k || b.y_rows > 0x7fffffffu))
-    return fail(c, TX_EINVAL, "block_norm: places need y, weights and top_k");
+  if (b.places && (!b.y.data || !b.weights || !b.top_k || b.top_k > 32 || b.y_rows > 0x7fffffffu))
+    return fail(c, TX_EINVAL, "block_norm: places need y, weights and top_k 1..32");
   if (b.gate) {
     if (b.gate_dtype != TX_F32 && b.gate_dtype != TX_BF16)
       return fail(c, TX_EINVAL, "block_norm: bad dtype");
@@ -2139,7 +2139,7 @@ int tx_block_norm(void *ctx, const TxBlockNorm *block, uint32_t rows, uint32_t c
   p.status = c->status;
   cudaError_t e = cudaSetDevice(c->device);
   if (e != cudaSuccess) return cuda_fail(c, e, "cudaSetDevice");
-  e = tx::launch_block_norm(p, stream ? (cudaStream_t)stream : c->stream);
+  e = tx::launch_block_norm(p, c->sms, stream ? (cudaStream_t)stream : c->stream);
   if (e != cudaSuccess) return cuda_fail(c, e, "block_norm launch");
   c->last_kernel = "block_norm";
   ++c->launches;
