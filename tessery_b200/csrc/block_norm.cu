@@ -6,9 +6,11 @@
 // is before r is rounded.  The joined sum runs in the order of j, and a row whose place is negative is not read.
 //
 // Bound: HBM, each row read once and written once.  A row is W warps with C vectors of V elements a thread in
-// registers, so that the mean and the deviations of a LayerNorm are two passes over registers.  Few
-// registers a thread and a row's words loaded a row ahead keep enough of them on their way: a warp a row
-// (100 registers) left 16 warps an SM and took 66 / ?? us for 8192 joined rows of 1024.
+// registers, so that the mean and the deviations of a LayerNorm are two passes over registers, and its words
+// are loaded a row ahead.  Measured: 33500 rows of 1024, normed on both sides (412 MB): 71 us, 5.8 TB/s; 8192
+// rows of 1024 joined from 8 experts' with a gate by sequence (219 MB): 48 us, 4.5 TB/s; 8 rows: 8 us.  A warp
+// a row without loads ahead (100 registers, 16 warps an SM) took 79 and 66 us; rows through a ring in shared
+// memory filled by bulk copies 112 and 60 us; half as many warps with twice the vectors 76 and 68 us.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -16,6 +18,7 @@
 #include "../../include/tessattn.h"
 #include "common.cuh"
 #include "kernels.h"
+#include "tcgen05.cuh"
 
 namespace tx {
 namespace {
@@ -71,32 +74,113 @@ struct Words<V, Any> {
   __device__ __forceinline__ float at(int i) const { return f[i]; }
 };
 
+// V values in fp32, in pairs that one instruction works on (one value: alone).
 template <int V>
-__device__ __forceinline__ void store_as(void *base, int dtype, size_t at, const float *f) {
-  if constexpr (V == 1) {
-    if (dtype == TX_BF16)
-      static_cast<uint16_t *>(base)[at] = f32_to_bf16_bits(f[0]);
-    else
-      static_cast<float *>(base)[at] = f[0];
-  } else if (dtype == TX_BF16) {
-    uint16_t *p = static_cast<uint16_t *>(base) + at;
-    if constexpr (V == 4)
-      *reinterpret_cast<uint2 *>(p) = make_uint2(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]));
-    else
-      *reinterpret_cast<uint4 *>(p) = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]),
-                                                 pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
-  } else {
-    float4 *p = reinterpret_cast<float4 *>(static_cast<float *>(base) + at);
+struct Row {
+  uint64_t p[V / 2];
+  __device__ __forceinline__ void fill(float x) {
 #pragma unroll
-    for (int i = 0; i < V; i += 4) p[i / 4] = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+    for (int i = 0; i < V / 2; ++i) p[i] = ptx::f2(x, x);
   }
-}
-template <int V>
-__device__ __forceinline__ void load_as(const void *base, int dtype, size_t at, float *f) {
-  Words<V, Any> r;
-  r.load(base, dtype, at);
+  template <typename W>
+  __device__ __forceinline__ void from(const W &w) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) f[i] = r.at(i);
+    for (int i = 0; i < V / 2; ++i) p[i] = ptx::f2(w.at(2 * i), w.at(2 * i + 1));
+  }
+  __device__ __forceinline__ void add(float x) {
+    const uint64_t y = ptx::f2(x, x);
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) p[i] = ptx::add2(p[i], y);
+  }
+  __device__ __forceinline__ void add(const Row &b) {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) p[i] = ptx::add2(p[i], b.p[i]);
+  }
+  __device__ __forceinline__ void mul(float x) {
+    const uint64_t y = ptx::f2(x, x);
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) p[i] = ptx::mul2(p[i], y);
+  }
+  __device__ __forceinline__ void mul(const Row &b) {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) p[i] = ptx::mul2(p[i], b.p[i]);
+  }
+  // this + x b
+  __device__ __forceinline__ void fma(float x, const Row &b) {
+    const uint64_t y = ptx::f2(x, x);
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) p[i] = ptx::fma2(y, b.p[i], p[i]);
+  }
+  __device__ __forceinline__ float sum() const {
+    uint64_t s = p[0];
+#pragma unroll
+    for (int i = 1; i < V / 2; ++i) s = ptx::add2(s, p[i]);
+    const float2 f = ptx::f2_unpack(s);
+    return f.x + f.y;
+  }
+  __device__ __forceinline__ float squares() const {
+    uint64_t s = ptx::mul2(p[0], p[0]);
+#pragma unroll
+    for (int i = 1; i < V / 2; ++i) s = ptx::fma2(p[i], p[i], s);
+    const float2 f = ptx::f2_unpack(s);
+    return f.x + f.y;
+  }
+  __device__ __forceinline__ void store(void *base, int dtype, size_t at) const {
+    float2 f[V / 2];
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) f[i] = ptx::f2_unpack(p[i]);
+    if (dtype == TX_BF16) {
+      uint16_t *to = static_cast<uint16_t *>(base) + at;
+      if constexpr (V == 4)
+        *reinterpret_cast<uint2 *>(to) =
+            make_uint2(pack_bf16x2(f[0].x, f[0].y), pack_bf16x2(f[1].x, f[1].y));
+      else
+        *reinterpret_cast<uint4 *>(to) =
+            make_uint4(pack_bf16x2(f[0].x, f[0].y), pack_bf16x2(f[1].x, f[1].y),
+                       pack_bf16x2(f[2].x, f[2].y), pack_bf16x2(f[3].x, f[3].y));
+    } else {
+      float4 *to = reinterpret_cast<float4 *>(static_cast<float *>(base) + at);
+#pragma unroll
+      for (int i = 0; i < V / 4; ++i)
+        to[i] = make_float4(f[2 * i].x, f[2 * i].y, f[2 * i + 1].x, f[2 * i + 1].y);
+    }
+  }
+};
+template <>
+struct Row<1> {
+  float s;
+  __device__ __forceinline__ void fill(float x) { s = x; }
+  template <typename W>
+  __device__ __forceinline__ void from(const W &w) {
+    s = w.at(0);
+  }
+  __device__ __forceinline__ void add(float x) { s += x; }
+  __device__ __forceinline__ void add(const Row &b) { s += b.s; }
+  __device__ __forceinline__ void mul(float x) { s *= x; }
+  __device__ __forceinline__ void mul(const Row &b) { s *= b.s; }
+  __device__ __forceinline__ void fma(float x, const Row &b) { s = fmaf(x, b.s, s); }
+  __device__ __forceinline__ float sum() const { return s; }
+  __device__ __forceinline__ float squares() const { return s * s; }
+  __device__ __forceinline__ void store(void *base, int dtype, size_t at) const {
+    if (dtype == TX_BF16)
+      static_cast<uint16_t *>(base)[at] = f32_to_bf16_bits(s);
+    else
+      static_cast<float *>(base)[at] = s;
+  }
+};
+template <int V>
+__device__ __forceinline__ Row<V> load_row(const void *base, int dtype, size_t at) {
+  Row<V> r;
+  if (dtype == TX_BF16) {
+    Words<V, uint16_t> w;
+    w.load(base, dtype, at);
+    r.from(w);
+  } else {
+    Words<V, float> w;
+    w.load(base, dtype, at);
+    r.from(w);
+  }
+  return r;
 }
 
 // The W warps of a row: their sums meet in shared memory, in two buffers by turns (who writes one again has
@@ -104,14 +188,19 @@ __device__ __forceinline__ void load_as(const void *base, int dtype, size_t at, 
 template <int W>
 struct RowTeam {
   float (*buf)[W];  // [2][W]
-  uint32_t barrier;  // of its own among the block's
+  uint32_t barrier;  // 1 or 2
   int turn;
   __device__ __forceinline__ float sum(float v) {
     v = warp_sum(v);
     if constexpr (W > 1) {
       float *b = buf[turn++ & 1];
       if ((threadIdx.x & 31) == 0) b[threadIdx.x / 32 % W] = v;
-      asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(32 * W) : "memory");
+      // (Barriers by a number that the compiler knows: otherwise a block holds all 16 of them, and four
+      // blocks an SM's.)
+      if (barrier == 1)
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * W) : "memory");
+      else
+        asm volatile("bar.sync 2, %0;" ::"n"(32 * W) : "memory");
       v = b[0];
 #pragma unroll
       for (int i = 1; i < W; ++i) v += b[i];
@@ -120,64 +209,64 @@ struct RowTeam {
   }
 };
 
+// scale: a factor of all that comes out.
 template <int W, int V, int C>
-__device__ __forceinline__ void apply_norm(const BlockNorm &n, float (&v)[C][V], uint32_t cols,
-                                           float inv_cols, uint32_t t, RowTeam<W> &team) {
-  if (n.kind == TX_NORM_NONE) return;
+__device__ __forceinline__ void apply_norm(const BlockNorm &n, Row<V> (&v)[C], uint32_t cols,
+                                           float inv_cols, uint32_t t, RowTeam<W> &team, float scale) {
   auto in = [&](int c) { return (t + c * 32 * W) * V < cols; };
+  if (n.kind == TX_NORM_NONE) {
+    if (scale != 1.f) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) v[c].mul(scale);
+    }
+    return;
+  }
   if (n.kind == TX_NORM_LAYER) {
     float s = 0.f;
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-      for (int i = 0; i < V; ++i) s += v[c][i];
+    for (int c = 0; c < C; ++c) s += v[c].sum();
     const float mean = team.sum(s) * inv_cols;
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-      for (int i = 0; i < V; ++i) v[c][i] = in(c) ? v[c][i] - mean : 0.f;
+    for (int c = 0; c < C; ++c) {
+      if (in(c))
+        v[c].add(-mean);
+      else
+        v[c].fill(0.f);
+    }
   }
   float ss = 0.f;
 #pragma unroll
-  for (int c = 0; c < C; ++c)
-#pragma unroll
-    for (int i = 0; i < V; ++i) ss = fmaf(v[c][i], v[c][i], ss);
-  const float inv = rsqrtf(fmaf(team.sum(ss), inv_cols, n.eps));
+  for (int c = 0; c < C; ++c) ss += v[c].squares();
+  const float inv = rsqrtf(fmaf(team.sum(ss), inv_cols, n.eps)) * scale;
 #pragma unroll
   for (int c = 0; c < C; ++c) {
+    v[c].mul(inv);
     if (!in(c)) continue;
     const size_t at = (size_t)(t + c * 32 * W) * V;
-    float w[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) w[i] = 1.f;
     if (n.weight) {
-      load_as<V>(n.weight, n.dtype, at, w);
-#pragma unroll
-      for (int i = 0; i < V; ++i) w[i] += n.offset;
+      Row<V> w = load_row<V>(n.weight, n.dtype, at);
+      if (n.offset != 0.f) w.add(n.offset);
+      v[c].mul(w);
     }
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[c][i] = v[c][i] * inv * w[i];
-    if (n.bias) {
-      load_as<V>(n.bias, n.dtype, at, w);
-#pragma unroll
-      for (int i = 0; i < V; ++i) v[c][i] += w[i];
-    }
+    if (n.bias) v[c].fma(scale, load_row<V>(n.bias, n.dtype, at));
   }
 }
 
-// Rows of a block, and blocks of an SM at 64 registers a thread.
-template <int W>
+// Rows of a block, and blocks of an SM as registers allow.
+template <int W, int C, int V>
 struct Shape {
   static constexpr int kRows = W >= 4 ? 1 : W == 1 ? 4 : 2;
   static constexpr int kThreads = 32 * W * kRows;
-  static constexpr int kResident = 1024 / kThreads;
+  static constexpr int kWide = C * V >= 32 ? 512 : C * V >= 16 ? 768 : 1024;
+  static constexpr int kResident = kWide / kThreads > 0 ? kWide / kThreads : 1;
 };
 
 template <typename XT, typename YT, int W, int V, int C, bool kJoin>
-__global__ void __launch_bounds__(Shape<W>::kThreads, Shape<W>::kResident)
+__global__ void __launch_bounds__(Shape<W, C, V>::kThreads, Shape<W, C, V>::kResident)
     block_norm_kernel(const __grid_constant__ BlockNormProblem p) {
-  constexpr int kRows = Shape<W>::kRows;
-  constexpr int kAhead = V * C > 8 ? 2 : sizeof(YT) == 4 ? 4 : 8;  // joined rows on their way at once
+  constexpr int kRows = Shape<W, C, V>::kRows;
+  constexpr int kFit = (W < 4 ? 64 : 128) / (C * (int)sizeof(Words<V, YT>));
+  constexpr int kAhead = kFit < 1 ? 1 : kFit > 8 ? 8 : kFit;  // joined rows on their way at once
   __shared__ float buf[kRows][2][W];
   const uint32_t own = threadIdx.x / (32 * W), t = threadIdx.x % (32 * W), lane = threadIdx.x & 31;
   RowTeam<W> team{buf[own], 1 + own, 0};
@@ -205,14 +294,17 @@ __global__ void __launch_bounds__(Shape<W>::kThreads, Shape<W>::kResident)
   uint32_t row = blockIdx.x * kRows + own;
   fetch(row);
   for (; row < p.rows; row += step) {
-    float v[C][V], r[C][V];
+    Row<V> v[C], r[C];
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        v[c][i] = !kJoin && p.y && in(c) ? y[c].at(i) : 0.f;
-        r[c][i] = p.x && in(c) ? p.x_scale * x[c].at(i) : 0.f;
+    for (int c = 0; c < C; ++c) {
+      v[c].fill(0.f);
+      r[c].fill(0.f);
+      if (in(c)) {
+        if (!kJoin && p.y) v[c].from(y[c]);
+        if (p.x) r[c].from(x[c]);
       }
+      r[c].mul(p.x_scale);
+    }
     const int32_t here = place;
     const float here_weight = weight;
     fetch(row + step);
@@ -241,46 +333,42 @@ __global__ void __launch_bounds__(Shape<W>::kThreads, Shape<W>::kResident)
 #pragma unroll
         for (int a = 0; a < kAhead; ++a)
 #pragma unroll
-          for (int c = 0; c < C; ++c)
-#pragma unroll
-            for (int i = 0; i < V; ++i) v[c][i] = fmaf(w[a], z[a][c].at(i), v[c][i]);
+          for (int c = 0; c < C; ++c) {
+            Row<V> f;
+            f.from(z[a][c]);
+            v[c].fma(w[a], f);
+          }
       }
     }
     if (p.y) {
-      apply_norm<W, V, C>(p.after, v, p.cols, inv_cols, t, team);
-      uint32_t g = 0;
-      if (p.gate)
-        g = p.cu ? warp_find_seq(p.cu, p.gate_rows, row, lane) : p.seq ? row / p.seq : 0;
+      apply_norm<W, V, C>(p.after, v, p.cols, inv_cols, t, team, p.y_scale);
+      if (p.gate) {
+        const uint32_t g = p.cu ? warp_find_seq(p.cu, p.gate_rows, row, lane) : p.seq ? row / p.seq : 0;
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        if (!in(c)) continue;
-        float f[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) f[i] = 1.f;
-        if (p.gate)
-          load_as<V>(p.gate, p.gate_dtype, (size_t)g * p.ldg + (size_t)(t + c * 32 * W) * V, f);
-#pragma unroll
-        for (int i = 0; i < V; ++i) r[c][i] = fmaf(p.y_scale, v[c][i] * f[i], r[c][i]);
+        for (int c = 0; c < C; ++c)
+          if (in(c))
+            v[c].mul(load_row<V>(p.gate, p.gate_dtype, (size_t)g * p.ldg + (size_t)(t + c * 32 * W) * V));
       }
+#pragma unroll
+      for (int c = 0; c < C; ++c) r[c].add(v[c]);
     }
     if (p.out) {
 #pragma unroll
       for (int c = 0; c < C; ++c)
         if (in(c))
-          store_as<V>(p.out, p.out_dtype, (size_t)row * p.ldo + (size_t)(t + c * 32 * W) * V, r[c]);
+          r[c].store(p.out, p.out_dtype, (size_t)row * p.ldo + (size_t)(t + c * 32 * W) * V);
     }
     if (!p.h) continue;
-    apply_norm<W, V, C>(p.before, r, p.cols, inv_cols, t, team);
+    apply_norm<W, V, C>(p.before, r, p.cols, inv_cols, t, team, 1.f);
 #pragma unroll
     for (int c = 0; c < C; ++c)
-      if (in(c))
-        store_as<V>(p.h, p.h_dtype, (size_t)row * p.ldh + (size_t)(t + c * 32 * W) * V, r[c]);
+      if (in(c)) r[c].store(p.h, p.h_dtype, (size_t)row * p.ldh + (size_t)(t + c * 32 * W) * V);
   }
 }
 
 template <typename XT, typename YT, int W, int V, int C>
 cudaError_t run(const BlockNormProblem &p, int num_sms, cudaStream_t stream) {
-  using S = Shape<W>;
+  using S = Shape<W, C, V>;
   const uint32_t blocks = std::min<uint32_t>((p.rows + S::kRows - 1) / S::kRows,
                                              (uint32_t)(num_sms * S::kResident));
   if (p.places)
