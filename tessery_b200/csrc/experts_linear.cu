@@ -196,28 +196,57 @@ struct Finish {
   uint32_t r0, rows, staging;
   const float *bias;  // of the tile's expert, or NULL
 };
-// Stores 32 staged rows of kPieces 16-byte pieces (elements of kSize bytes) from column n on.
+// Stores 32 staged rows of kPieces 16-byte pieces (elements of kSize bytes) from column n on, in pieces of 16
+// bytes where the rows of out start on such, otherwise of 4, and bf16 rows at odd elements one by one.
 template <uint32_t kSize, uint32_t kPieces>
 __device__ __forceinline__ void store_staged(const ExpertsProblem &p, const Finish &f, uint32_t n) {
-  constexpr uint32_t kEach = 16 / kSize;
-  const uint32_t lane = threadIdx.x & 31, piece = lane & 3, col = n + piece * kEach;
-  if (piece >= kPieces || col >= p.n) return;
-  uint8_t *to = static_cast<uint8_t *>(p.out) + ((size_t)f.r0 * p.ldo + col) * kSize;
-  const bool whole = col + kEach <= p.n;
+  const uint32_t lane = threadIdx.x & 31;
+  auto piece_of = [&](uint32_t r, uint32_t piece) {
+    return f.staging + r * 64 + ((piece ^ ((r >> 1) & 3)) << 4);
+  };
+  uint8_t *to = static_cast<uint8_t *>(p.out) + ((size_t)f.r0 * p.ldo + n) * kSize;
+  const size_t pitch = (size_t)p.ldo * kSize;
+  if (p.out_step == 16) {
+    constexpr uint32_t kEach = 16 / kSize;
+    const uint32_t piece = lane & 3, col = n + piece * kEach;
+    if (piece >= kPieces || col >= p.n) return;
+    const bool whole = col + kEach <= p.n;
 #pragma unroll
-  for (uint32_t r = lane >> 2; r < 32; r += 8) {
-    if (r >= f.rows) break;
-    const uint4 o = ld_shared_v4(f.staging + r * 64 + ((piece ^ ((r >> 1) & 3)) << 4));
-    uint8_t *at = to + (size_t)r * p.ldo * kSize;
-    if (whole) {
-      *reinterpret_cast<uint4 *>(at) = o;
-    } else {
-      for (uint32_t t = 0; col + t < p.n; ++t) {
-        if constexpr (kSize == 4)
-          reinterpret_cast<uint32_t *>(at)[t] = u4_at(o, t);
-        else
-          reinterpret_cast<uint16_t *>(at)[t] = (uint16_t)(u4_at(o, t / 2) >> (16 * (t & 1)));
+    for (uint32_t r = lane >> 2; r < 32; r += 8) {
+      if (r >= f.rows) break;
+      const uint4 o = ld_shared_v4(piece_of(r, piece));
+      uint8_t *at = to + r * pitch + piece * 16;
+      if (whole) {
+        *reinterpret_cast<uint4 *>(at) = o;
+      } else {
+        for (uint32_t t = 0; col + t < p.n; ++t) {
+          if constexpr (kSize == 4)
+            reinterpret_cast<uint32_t *>(at)[t] = u4_at(o, t);
+          else
+            reinterpret_cast<uint16_t *>(at)[t] = (uint16_t)(u4_at(o, t / 2) >> (16 * (t & 1)));
+        }
       }
+    }
+  } else if (p.out_step == 4) {
+    // 16 lanes a row: the words of 64 bytes.
+    const uint32_t word = lane & 15, col = n + word * (4 / kSize);
+    if (word >= 4 * kPieces || col >= p.n) return;
+    const bool whole = col + 4 / kSize <= p.n;
+#pragma unroll 4
+    for (uint32_t r = lane >> 4; r < f.rows; r += 2) {
+      const uint32_t o = ld_shared(piece_of(r, word >> 2) + (word & 3) * 4);
+      uint8_t *at = to + r * pitch + word * 4;
+      if (whole)
+        *reinterpret_cast<uint32_t *>(at) = o;
+      else
+        *reinterpret_cast<uint16_t *>(at) = (uint16_t)o;
+    }
+  } else if constexpr (kSize == 2) {
+    if (lane >= 8 * kPieces || n + lane >= p.n) return;
+#pragma unroll 4
+    for (uint32_t r = 0; r < f.rows; ++r) {
+      const uint32_t o = ld_shared(piece_of(r, lane >> 3) + (lane & 6) * 2);
+      *reinterpret_cast<uint16_t *>(to + r * pitch + lane * 2) = (uint16_t)(o >> (16 * (lane & 1)));
     }
   }
 }
@@ -242,42 +271,30 @@ __device__ __forceinline__ void finish_columns(const ExpertsProblem &p, const Fi
 #pragma unroll
     for (uint32_t t = 0; t < kStep; ++t) v[t] *= u[t];
   }
-  if (p.out_vec) {
-    // Through shared memory, so that a warp stores rows of 64 bytes.  The 16-byte pieces of a row are
-    // swapped so that neither side meets a bank twice.
-    const uint32_t sw = (lane >> 1) & 3, mine = f.staging + lane * 64;
-    if (p.out_dtype == TX_F32) {
+  // Through shared memory, so that a warp stores rows of 64 bytes.  The 16-byte pieces of a row are
+  // swapped so that neither side meets a bank twice.
+  const uint32_t sw = (lane >> 1) & 3, mine = f.staging + lane * 64;
+  if (p.out_dtype == TX_F32) {
 #pragma unroll
-      for (uint32_t h = 0; h < kStep; h += 16) {
-        __syncwarp();
-#pragma unroll
-        for (uint32_t q = 0; q < 4; ++q)
-          st_shared_v4(mine + ((q ^ sw) << 4), __float_as_uint(v[h + 4 * q]),
-                       __float_as_uint(v[h + 4 * q + 1]), __float_as_uint(v[h + 4 * q + 2]),
-                       __float_as_uint(v[h + 4 * q + 3]));
-        __syncwarp();
-        store_staged<4, 4>(p, f, n + h);
-      }
-    } else {
+    for (uint32_t h = 0; h < kStep; h += 16) {
       __syncwarp();
 #pragma unroll
-      for (uint32_t q = 0; q < kStep / 8; ++q)
-        st_shared_v4(mine + ((q ^ sw) << 4), pack_bf16x2(v[8 * q], v[8 * q + 1]),
-                     pack_bf16x2(v[8 * q + 2], v[8 * q + 3]), pack_bf16x2(v[8 * q + 4], v[8 * q + 5]),
-                     pack_bf16x2(v[8 * q + 6], v[8 * q + 7]));
+      for (uint32_t q = 0; q < 4; ++q)
+        st_shared_v4(mine + ((q ^ sw) << 4), __float_as_uint(v[h + 4 * q]),
+                     __float_as_uint(v[h + 4 * q + 1]), __float_as_uint(v[h + 4 * q + 2]),
+                     __float_as_uint(v[h + 4 * q + 3]));
       __syncwarp();
-      store_staged<2, kStep / 8>(p, f, n);
+      if (n + h < p.n) store_staged<4, 4>(p, f, n + h);
     }
-  } else if (lane < f.rows) {
-    const size_t at = (size_t)(f.r0 + lane) * p.ldo + n;
+  } else {
+    __syncwarp();
 #pragma unroll
-    for (uint32_t t = 0; t < kStep; ++t)
-      if (n + t < p.n) {
-        if (p.out_dtype == TX_F32)
-          static_cast<float *>(p.out)[at + t] = v[t];
-        else
-          static_cast<uint16_t *>(p.out)[at + t] = f32_to_bf16_bits(v[t]);
-      }
+    for (uint32_t q = 0; q < kStep / 8; ++q)
+      st_shared_v4(mine + ((q ^ sw) << 4), pack_bf16x2(v[8 * q], v[8 * q + 1]),
+                   pack_bf16x2(v[8 * q + 2], v[8 * q + 3]), pack_bf16x2(v[8 * q + 4], v[8 * q + 5]),
+                   pack_bf16x2(v[8 * q + 6], v[8 * q + 7]));
+    __syncwarp();
+    store_staged<2, kStep / 8>(p, f, n);
   }
 }
 template <uint32_t kStep>
@@ -769,7 +786,9 @@ cudaError_t launch_rows(const ExpertsProblem &p, int num_sms, cudaStream_t strea
 
 cudaError_t launch_experts_linear(ExpertsProblem p, int num_sms, cudaStream_t stream) {
   using namespace experts;
-  p.out_vec = (uintptr_t)p.out % 16 == 0 && p.ldo % (p.out_dtype == TX_BF16 ? 8 : 4) == 0;
+  const uint32_t size = p.out_dtype == TX_BF16 ? 2 : 4;
+  p.out_step = 16;
+  while ((uintptr_t)p.out % p.out_step || p.ldo * size % p.out_step) p.out_step = p.out_step == 16 ? 4 : 2;
   p.top_k_inv = p.top_k > 1 ? (uint32_t)((1ull << 32) / p.top_k) + 1 : 0;
   if (p.act == TX_ACT_GELU && p.out_dtype == TX_F32) p.act = kGeluF32;
   // The accumulator cuts bits off at each of its additions: over 512 K that is far below bf16's rounding,

@@ -291,8 +291,8 @@ struct ExpertsProblem {
   const int32_t *offsets, *order;
   uint32_t x_rows, rows, experts, top_k, n, k;
   int gated, act, out_dtype;
-  bool out_vec;        // on 16-byte boundaries, and what divides by top_k: set by the launcher
-  uint32_t top_k_inv;
+  // set by the launcher: bytes that rows of out start on a multiple of (16, 4 or 2), what divides by top_k
+  uint32_t out_step, top_k_inv;
   int *status;
   long long wait_cycles;
 };
