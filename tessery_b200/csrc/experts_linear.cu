@@ -35,6 +35,7 @@ constexpr int kThreads = 320, kGatherThreads = 448;
 constexpr int kMaxStages = 8;
 constexpr uint32_t kPart = 8;  // K stages (512 columns) of one partial sum
 constexpr uint32_t kBufBytes = 32 * 64;  // staging of an epilogue warp: 32 rows of 64 bytes
+constexpr uint32_t kBiasBytes = 512;     // of an epilogue warp: its columns' bias
 constexpr uint32_t kFull = 0xffffffffu;
 
 template <int kBN>
@@ -43,10 +44,11 @@ struct Cfg {
   static constexpr uint32_t kStageBytes = kABytes + kBBytes;
   static constexpr uint32_t kMaxExperts = 1024;
   static constexpr uint32_t kTables = 2 * (kMaxExperts + 1) * 4;
-  static constexpr int kFit = (int)((232448 - 512 - kTables - 8 * kBufBytes) / kStageBytes);
+  static constexpr int kFit =
+      (int)((232448 - 512 - kTables - 8 * (kBufBytes + kBiasBytes)) / kStageBytes);
   static constexpr int kStages = kFit < kMaxStages ? kFit : kMaxStages;
   static constexpr uint32_t kOffStaging = kStages * kStageBytes;
-  static constexpr uint32_t kOffMisc = kOffStaging + 8 * kBufBytes;
+  static constexpr uint32_t kOffMisc = kOffStaging + 8 * (kBufBytes + kBiasBytes);
   static constexpr uint32_t kOffTables = kOffMisc + 512;
   static constexpr uint32_t kSmemBytes = kOffTables + kTables;
   static constexpr uint32_t kTmemCols = 2 * kBN;
@@ -133,10 +135,17 @@ struct Gather {
 template <uint32_t kRows>
 __device__ __forceinline__ void fill_tables(const ExpertsProblem &p, uint32_t *start, uint32_t *tiles) {
   const uint32_t lane = threadIdx.x & 31;
+  constexpr uint32_t kAhead = 4;  // loads on their way at once
   uint32_t edge = 0, count = 0;
+  int32_t ahead[kAhead];
   for (uint32_t e0 = 0; e0 <= p.experts; e0 += 32) {
-    const uint32_t e = e0 + lane;
-    int32_t raw = e <= p.experts ? __ldg(p.offsets + e) : 0;
+    const uint32_t e = e0 + lane, turn = e0 / 32 % kAhead;
+    if (turn == 0) {
+#pragma unroll
+      for (uint32_t a = 0; a < kAhead; ++a)
+        ahead[a] = e + a * 32 <= p.experts ? __ldg(p.offsets + e + a * 32) : 0;
+    }
+    const int32_t raw = turn == 0 ? ahead[0] : turn == 1 ? ahead[1] : turn == 2 ? ahead[2] : ahead[3];
     uint32_t v = min((uint32_t)max(raw, 0), p.rows);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {  // the largest so far
@@ -194,8 +203,30 @@ __device__ __forceinline__ void activate_all(float (&v)[kN], int act) {
 // What an epilogue warp finishes: rows r0 + lane of the output, of which the first `rows` exist.
 struct Finish {
   uint32_t r0, rows, staging;
-  const float *bias;  // of the tile's expert, or NULL
+  uint32_t bias;  // in shared memory: its columns', gated the gate's and then the up's
 };
+// The bias of the warp's kCols columns from n on into shared memory, fetched while the products are made: at
+// their end a first look at it took as long as a small tile.
+template <bool kGated, uint32_t kCols>
+__device__ __forceinline__ void fetch_bias(const ExpertsProblem &p, uint32_t to, uint32_t e, uint32_t n) {
+  const uint32_t lane = threadIdx.x & 31;
+  const float *bias = p.bias + (size_t)e * (kGated ? 2 : 1) * p.n;
+  float v[(kCols + 31) / 32], u[(kCols + 31) / 32];
+#pragma unroll
+  for (uint32_t c = 0; c < kCols; c += 32) {
+    const bool in = c + lane < kCols && n + c + lane < p.n;
+    v[c / 32] = in ? __ldg(bias + n + c + lane) : 0.f;
+    if constexpr (kGated) u[c / 32] = in ? __ldg(bias + p.n + n + c + lane) : 0.f;
+  }
+  __syncwarp();
+#pragma unroll
+  for (uint32_t c = 0; c < kCols; c += 32) {
+    if (c + lane >= kCols) continue;
+    st_shared(to + (c + lane) * 4, __float_as_uint(v[c / 32]));
+    if constexpr (kGated) st_shared(to + (kCols + c + lane) * 4, __float_as_uint(u[c / 32]));
+  }
+  __syncwarp();
+}
 // Stores 32 staged rows of kPieces 16-byte pieces (elements of kSize bytes) from column n on, in pieces of 16
 // bytes where the rows of out start on such, otherwise of 4, and bf16 rows at odd elements one by one.
 template <uint32_t kSize, uint32_t kPieces>
@@ -250,21 +281,27 @@ __device__ __forceinline__ void store_staged(const ExpertsProblem &p, const Fini
     }
   }
 }
-// Bias, activation, gate and store of columns n .. n + kStep - 1 of 32 rows, one a lane; u is the up half.
-// The whole warp calls it.
-template <bool kGated, uint32_t kStep>
-__device__ __forceinline__ void finish_columns(const ExpertsProblem &p, const Finish &f, uint32_t n,
-                                               float (&v)[kStep], float (&u)[kGated ? kStep : 1]) {
+// Bias, activation, gate and store of columns c .. c + kStep - 1 of the warp's kCols from n0 on, of 32 rows,
+// one a lane; u is the up half.  The whole warp calls it.
+template <bool kGated, uint32_t kCols, uint32_t kStep>
+__device__ __forceinline__ void finish_columns(const ExpertsProblem &p, const Finish &f, uint32_t n0,
+                                               uint32_t c, float (&v)[kStep],
+                                               float (&u)[kGated ? kStep : 1]) {
+  const uint32_t n = n0 + c;
   if (!f.rows || n >= p.n) return;
   const uint32_t lane = threadIdx.x & 31;
-  if (f.bias) {
-    const bool whole = n + kStep <= p.n;
+  if (p.bias) {
 #pragma unroll
-    for (uint32_t t = 0; t < kStep; ++t)
-      if (whole || n + t < p.n) {
-        v[t] += __ldg(f.bias + n + t);
-        if constexpr (kGated) u[t] += __ldg(f.bias + p.n + n + t);
+    for (uint32_t t = 0; t < kStep; t += 4) {
+      const uint4 q = ld_shared_v4(f.bias + (c + t) * 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[t + i] += __uint_as_float(u4_at(q, i));
+      if constexpr (kGated) {
+        const uint4 r = ld_shared_v4(f.bias + (kCols + c + t) * 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) u[t + i] += __uint_as_float(u4_at(r, i));
       }
+    }
   }
   activate_all(v, p.act);
   if constexpr (kGated) {
@@ -321,6 +358,8 @@ __global__ void __launch_bounds__(kGather ? kGatherThreads : kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
+    prefetch_tmap(&tm_x);
+    prefetch_tmap(&tm_w);
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(bar(kBarFull + s), kGather ? 129 : 1);  // the TMA copies, and each gathering thread
       mbar_init(bar(kBarEmpty + s), 1);
@@ -443,6 +482,8 @@ __global__ void __launch_bounds__(kGather ? kGatherThreads : kThreads, 1)
     const uint32_t quarter = (uint32_t)warp & 3, half = (uint32_t)(warp - 2) >> 2;
     const uint32_t lanes = (quarter * 32u) << 16;
     const uint32_t staging = sbase + C::kOffStaging + (uint32_t)(warp - 2) * kBufBytes;
+    const uint32_t bias = sbase + C::kOffStaging + 8 * kBufBytes + (uint32_t)(warp - 2) * kBiasBytes;
+    static_assert(kCols * (kGated ? 8 : 4) <= kBiasBytes, "bias area");
     uint32_t done = 0, e = 0;
     bool ok = true;
     for (uint32_t tile = blockIdx.x; ok && tile < total; tile += gridDim.x) {
@@ -451,7 +492,8 @@ __global__ void __launch_bounds__(kGather ? kGatherThreads : kThreads, 1)
       const uint32_t r0 = start[e] + (mt - tiles[e]) * kBM, rows = min(start[e + 1] - r0, (uint32_t)kBM);
       const uint32_t n0 = tile % nt * kOut + half * kCols;
       const Finish f{r0 + quarter * 32, rows > quarter * 32 ? min(rows - quarter * 32, 32u) : 0, staging,
-                     p.bias ? p.bias + (size_t)e * (kGated ? 2 : 1) * p.n : nullptr};
+                     bias};
+      if (p.bias && f.rows) fetch_bias<kGated, kCols>(p, bias, e, n0);
       if constexpr (kLong) {
         constexpr uint32_t kHeld = kCols / kStep;
         float v[kHeld][kStep], u[kGated ? kHeld : 1][kGated ? kStep : 1];
@@ -480,7 +522,7 @@ __global__ void __launch_bounds__(kGather ? kGatherThreads : kThreads, 1)
         if (!ok) break;
 #pragma unroll
         for (uint32_t c = 0; c < kHeld; ++c)
-          finish_columns<kGated, kStep>(p, f, n0 + c * kStep, v[c], u[kGated ? c : 0]);
+          finish_columns<kGated, kCols, kStep>(p, f, n0, c * kStep, v[c], u[kGated ? c : 0]);
       } else {
         const uint32_t b = done & 1, t0 = tmem + b * kBN + half * kCols + lanes;
         ok = __all_sync(kFull, wait_bar(bar(kBarAcc + b), (done >> 1) & 1, abort_flag, p.status,
@@ -493,7 +535,7 @@ __global__ void __launch_bounds__(kGather ? kGatherThreads : kThreads, 1)
           float v[kStep], u[kGated ? kStep : 1];
           load_columns<kStep>(t0 + c, v);
           if constexpr (kGated) load_columns<kStep>(t0 + kOut + c, u);
-          finish_columns<kGated, kStep>(p, f, n0 + c, v, u);
+          finish_columns<kGated, kCols, kStep>(p, f, n0, c, v, u);
           __syncwarp();
         }
         tc_fence_before();
@@ -519,7 +561,8 @@ namespace pair {
 constexpr int kStages = 6;
 constexpr uint32_t kHalfBytes = 128 * 128, kStageBytes = 2 * kHalfBytes;
 constexpr uint32_t kRows = 256, kWide = 256, kMaxExperts = 1024;
-constexpr uint32_t kOffStaging = kStages * kStageBytes, kOffMisc = kOffStaging + 8 * kBufBytes;
+constexpr uint32_t kOffStaging = kStages * kStageBytes;
+constexpr uint32_t kOffMisc = kOffStaging + 8 * (kBufBytes + kBiasBytes);
 constexpr uint32_t kOffTables = kOffMisc + 512;
 constexpr uint32_t kSmemBytes = kOffTables + 2 * (kMaxExperts + 1) * 4;
 static_assert(kSmemBytes <= 232448, "shared memory");
@@ -548,6 +591,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGather ? kGatherThr
   const uint32_t rank = cluster_rank(), first_tile = blockIdx.x / 2, tile_step = gridDim.x / 2;
 
   if (threadIdx.x == 0) {
+    prefetch_tmap(&tm_x);
+    prefetch_tmap(&tm_w);
     for (int s = 0; s < kStages; ++s) {
       mbar_init(bar(kFullBar + s), kGather ? 2 : 1);
       mbar_init(bar(kGathered + s), 128);
@@ -683,6 +728,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGather ? kGatherThr
     const uint32_t quarter = (uint32_t)warp & 3, half = (uint32_t)(warp - 2) >> 2;
     const uint32_t lanes = (quarter * 32u) << 16;
     const uint32_t staging = sbase + kOffStaging + (uint32_t)(warp - 2) * kBufBytes;
+    const uint32_t bias = sbase + kOffStaging + 8 * kBufBytes + (uint32_t)(warp - 2) * kBiasBytes;
+    static_assert(kCols * (kGated ? 8 : 4) <= kBiasBytes, "bias area");
     uint32_t done = 0, e = 0;
     bool ok = true;
     for (uint32_t tile = first_tile; ok && tile < total; tile += tile_step) {
@@ -690,8 +737,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGather ? kGatherThr
       e = expert_of(tiles, p.experts, mt, e);
       const uint32_t r0 = start[e] + (mt - tiles[e]) * kRows + rank * 128 + quarter * 32;
       const uint32_t n0 = tile % nt * kOut + half * kCols;
-      const Finish f{r0, start[e + 1] > r0 ? min(start[e + 1] - r0, 32u) : 0, staging,
-                     p.bias ? p.bias + (size_t)e * (kGated ? 2 : 1) * p.n : nullptr};
+      const Finish f{r0, start[e + 1] > r0 ? min(start[e + 1] - r0, 32u) : 0, staging, bias};
+      if (p.bias && f.rows) fetch_bias<kGated, kCols>(p, bias, e, n0);
       const uint32_t b = done & 1, t0 = tmem + b * kWide + half * kCols + lanes;
       ok = __all_sync(kFull, wait_bar(bar(kAcc + b), (done >> 1) & 1, abort_flag, p.status,
                                               kSiteAcc, p.wait_cycles));
@@ -704,7 +751,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGather ? kGatherThr
           float v[kStep], u[kGated ? kStep : 1];
           load_columns<kStep>(t0 + c, v);
           if constexpr (kGated) load_columns<kStep>(t0 + kOut + c, u);
-          finish_columns<kGated, kStep>(p, f, n0 + c, v, u);
+          finish_columns<kGated, kCols, kStep>(p, f, n0, c, v, u);
           __syncwarp();
         }
       }
@@ -771,9 +818,14 @@ cudaError_t launch_pairs(const ExpertsProblem &p, int num_sms, cudaStream_t stre
 template <bool kGated, bool kLong, bool kGather>
 cudaError_t launch_wide(const ExpertsProblem &p, int num_sms, cudaStream_t stream) {
   const uint32_t wide = p.n * (kGated ? 2 : 1);
-  if (wide <= 64) return launch_tiles<64, kGated, kLong, kGather>(p, num_sms, stream);
   if constexpr (!kLong)
     if (wide > 128 && p.rows > 128 * 64) return launch_pairs<kGated, kGather>(p, num_sms, stream);
+  // 64 columns a tile where tiles of 128 would leave half the SMs without one (the expert ranges are not
+  // known here: at most a tile for each row or expert, and one for every 128 rows): 18 / 12 us for 2 to 32
+  // rows over 8 experts, n 768, k 768; but 27 / 35 us for 64 rows over 64 experts, gated, n 512, k 1024.
+  const uint64_t tiles = ((uint64_t)std::min(p.rows, p.experts) + p.rows / kBM) * ((wide + 127) / 128);
+  if (wide <= 64 || 2 * tiles <= (uint64_t)num_sms)
+    return launch_tiles<64, kGated, kLong, kGather>(p, num_sms, stream);
   return launch_tiles<128, kGated, kLong, kGather>(p, num_sms, stream);
 }
 template <bool kGated, bool kLong>
