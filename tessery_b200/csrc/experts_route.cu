@@ -345,6 +345,42 @@ __device__ __forceinline__ void sort_keys(uint32_t (&k)[V]) {
           }
 }
 
+// The 8 largest of V keys in their order, largest first: halves sorted, and the larger of each key of one and
+// its counterpart from the other's end, which rise and then fall.
+__device__ __forceinline__ void sort_bitonic(uint32_t (&t)[8]) {
+#pragma unroll
+  for (int d = 4; d; d /= 2)
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (!(i & d)) {
+        const uint32_t a = t[i], b = t[i + d];
+        t[i] = max(a, b);
+        t[i + d] = min(a, b);
+      }
+}
+template <int V>
+__device__ __forceinline__ void top_keys(const uint32_t (&k)[V], uint32_t (&t)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) t[i] = k[i];
+  sort_keys(t);
+  if constexpr (V == 16) {
+    uint32_t b[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) b[i] = k[8 + i];
+    sort_keys(b);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = max(t[i], b[7 - i]);
+    sort_bitonic(t);
+  }
+}
+// t[i] for an i that is known only here.
+__device__ __forceinline__ uint32_t pick(const uint32_t (&t)[8], uint32_t i) {
+  const uint32_t a = i & 1 ? t[1] : t[0], b = i & 1 ? t[3] : t[2], c = i & 1 ? t[5] : t[4],
+                 d = i & 1 ? t[7] : t[6];
+  const uint32_t x = i & 2 ? b : a, y = i & 2 ? d : c;
+  return i & 4 ? y : x;
+}
+
 // The logits of a lane's experts, as they lie.
 template <int V>
 struct Logits {
@@ -450,7 +486,10 @@ __device__ __forceinline__ void place_pairs(const RouteProblem &p, uint32_t firs
 // token in work its chosen experts and their keys, one more than there may be, and the lanes' sorted keys.
 constexpr uint32_t kSlotWords = 2 * (kMaxK + 1);
 
-template <int kLanes, int V, bool kScored, int kWarps>
+// kTop8: up to 8 experts a token, chosen by their logits alone.  Every lane's 8 largest meet those of the
+// other lanes in steps of a shuffle for each (8 maxima and a sort of 8), after which every lane has the
+// token's 8, without a round for each or a branch.  Their keys name the expert in all lanes.
+template <int kLanes, int V, bool kScored, int kWarps, bool kTop8>
 __global__ void __launch_bounds__(32 * kWarps, 1)
     route_kernel(const __grid_constant__ RouteProblem p) {
   constexpr uint32_t kThreads = 32 * kWarps;
@@ -458,8 +497,9 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
   // The low bits of a key: V - 1 - i for expert i of the lane, or, where the keys' lowest 16 bits are alike
   // (bf16 logits compared as they are), kNameAll - e for expert e.  The latter lose nothing and put equals
   // in their order.
-  constexpr uint32_t kName = V - 1, kNameAll = 0xffff;
-  constexpr int kMine = kMaxK / kLanes;  // chosen experts a lane weighs
+  // Of kTop8 the others' name is kName - e.
+  constexpr uint32_t kName = kTop8 ? kLanes * V - 1 : V - 1, kNameAll = 0xffff;
+  constexpr int kMine = ((kTop8 ? 8 : kMaxK) + kLanes - 1) / kLanes;  // chosen experts a lane weighs
   constexpr bool kListed = V > 8;        // sorted keys behind the first in shared memory
   extern __shared__ __align__(16) uint8_t smem[];
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane % kLanes;
@@ -488,7 +528,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
   __syncwarp();
   uint32_t first, end;
   warp_tokens(p, blockIdx.x, warp, &first, &end);
-  const bool told = !kScored && p.logits_dtype == TX_BF16;
+  bool told = !kScored && p.logits_dtype == TX_BF16;
   // Where the next token to load stands in its sequence, and how many rows of that are valid.
   uint32_t next = first + slot, row = 0, seq = 0, length = 0;
   if (p.lengths && next < end) {
@@ -496,6 +536,9 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
     row = next - seq * p.seq;
     length = (uint32_t)max(p.lengths[seq], 0);
   }
+  // A block that is alone, each warp with one round of tokens, places its pairs from registers.
+  const bool once = gridDim.x == 1 && p.run_warp <= kTokens;
+  uint32_t kept_e[kMine], kept_rank[kMine];
   Logits<V> raw;
   bool valid = next < end && (!p.lengths || row < length);
   raw.load(p, next, sub, valid);
@@ -528,12 +571,19 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
         }
         all_sum = lanes_sum<kLanes>(sum);
       }
+      if constexpr (kTop8) {
+        // fp32 logits that were bf16 are many equals: they are told apart as well.
+        uint32_t low = 0;
+#pragma unroll
+        for (int i = 0; i < V; ++i) low |= __float_as_uint(c[i]);
+        told = !__any_sync(kFull, low & kNameAll);
+      }
       if constexpr (!kScored) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           near |= c[i] != c[i];
           key[i] = told ? (quick_key(c[i]) & ~kNameAll) | (kNameAll - sub * p.per_lane - i)
-                        : (quick_key(c[i]) & ~kName) | (V - 1 - i);
+                        : (quick_key(c[i]) & ~kName) | (kName - (kTop8 ? sub * p.per_lane : 0) - i);
         }
       } else {
         const float inv = p.softmax ? quick_rcp(all_sum) : 1.f;
@@ -552,57 +602,94 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
       }
     }
     // The next tokens' logits travel meanwhile.
-    next += kTokens;
-    if (p.lengths && next < end) {
-      row += kTokens;
-      if (row >= p.seq) {
-        seq = next / p.seq;
-        row = next - seq * p.seq;
-        length = (uint32_t)max(p.lengths[seq], 0);
-      }
-    }
-    valid = next < end && (!p.lengths || row < length);
-    raw.load(p, next, sub, valid);
-    sort_keys(key);
-    if constexpr (kListed) {
-#pragma unroll
-      for (int i = 1; i < V; ++i)
-        if (i <= (int)p.top_k) list[i * 32] = key[i];
-    }
-    // The lowest lane with the largest head, names apart, has the next expert.
-    const uint32_t names = told ? 0 : kName;
-    uint32_t taken = 0;
-    for (uint32_t j = 0; j < p.top_k + !told; ++j) {
-      const uint32_t head = key[0], named = head | names, top = lanes_max<kLanes>(named);
-      if (lane == __ffs(__ballot_sync(kFull, named == top) & group_mask) - 1) {
-        chosen[j] = told ? kNameAll - (head & kNameAll) : sub * p.per_lane + kName - (head & kName);
-        chosen_key[j] = head;
-        if constexpr (kListed) {
-          key[0] = ++taken < V ? list[taken * 32] : 0;
-        } else {
-#pragma unroll
-          for (int i = 0; i + 1 < V; ++i) key[i] = key[i + 1];
-          key[V - 1] = 0;
+    auto load_next = [&] {
+      next += kTokens;
+      if (p.lengths && next < end) {
+        row += kTokens;
+        if (row >= p.seq) {
+          seq = next / p.seq;
+          row = next - seq * p.seq;
+          length = (uint32_t)max(p.lengths[seq], 0);
         }
       }
-    }
-    __syncwarp();
+      valid = next < end && (!p.lengths || row < length);
+      raw.load(p, next, sub, valid);
+    };
     uint32_t e[kMine];
+    if constexpr (kTop8) {
+      uint32_t t[8], own[8];
+      top_keys<V>(key, t);
 #pragma unroll
-    for (int m = 0; m < kMine; ++m) {
-      const uint32_t j = sub + m * kLanes;
-      e[m] = kNone;
-      if (j >= p.top_k) continue;
-      const uint32_t own = chosen_key[j];
-      if (own >= kLowest) e[m] = chosen[j];
-      if (told || own < kLowest) continue;
-      const uint32_t after = chosen_key[j + 1];
-      const float w = value_of(own & ~kName), v = value_of(after & ~kName);
-      if (after >= kLowest && !(w - v > tol + fabsf(w) * (V * 2.4e-7f))) {
-        // Equal in logit and bias they are in the right order, but behind the last there may be another.
-        const uint32_t f = chosen[j + 1];
-        near |= j + 1 == p.top_k || logit_at(p, token, e[m]) != logit_at(p, token, f) ||
-                (p.bias && p.bias[e[m]] != p.bias[f]);
+      for (int i = 0; i < 8; ++i) own[i] = t[i];
+#pragma unroll
+      for (int o = 1; o < kLanes; o *= 2) {
+        uint32_t b[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) b[i] = __shfl_xor_sync(kFull, t[i], o);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] = max(t[i], b[7 - i]);
+        sort_bitonic(t);
+      }
+      load_next();
+      uint32_t ninth = 0;
+      if (!told) {
+        // The largest that is left, or, where a lane's 8 are all among the token's, that lane's next may be.
+#pragma unroll
+        for (int i = 7; i >= 0; --i) ninth = own[i] < t[7] ? max(ninth, own[i]) : ninth;
+        ninth = lanes_max<kLanes>(own[7] >= t[7] && t[7] >= kLowest && V > 8 ? t[7] : ninth);
+      }
+      const uint32_t names = told ? kNameAll : kName;
+#pragma unroll
+      for (int m = 0; m < kMine; ++m) {
+        const uint32_t j = sub + m * kLanes;
+        e[m] = kNone;
+        if (j >= p.top_k) continue;
+        const uint32_t mine = pick(t, j), after = j < 7 ? pick(t, j + 1) : ninth;
+        if (mine >= kLowest) e[m] = names - (mine & names);
+        near |= !told && mine >= kLowest && (mine & ~kName) == (after & ~kName);
+      }
+    } else {
+      load_next();
+      sort_keys(key);
+      if constexpr (kListed) {
+#pragma unroll
+        for (int i = 1; i < V; ++i)
+          if (i <= (int)p.top_k) list[i * 32] = key[i];
+      }
+      // The lowest lane with the largest head, names apart, has the next expert.
+      const uint32_t names = told ? 0 : kName;
+      uint32_t taken = 0;
+      for (uint32_t j = 0; j < p.top_k + !told; ++j) {
+        const uint32_t head = key[0], named = head | names, top = lanes_max<kLanes>(named);
+        if (lane == __ffs(__ballot_sync(kFull, named == top) & group_mask) - 1) {
+          chosen[j] = told ? kNameAll - (head & kNameAll) : sub * p.per_lane + kName - (head & kName);
+          chosen_key[j] = head;
+          if constexpr (kListed) {
+            key[0] = ++taken < V ? list[taken * 32] : 0;
+          } else {
+#pragma unroll
+            for (int i = 0; i + 1 < V; ++i) key[i] = key[i + 1];
+            key[V - 1] = 0;
+          }
+        }
+      }
+      __syncwarp();
+#pragma unroll
+      for (int m = 0; m < kMine; ++m) {
+        const uint32_t j = sub + m * kLanes;
+        e[m] = kNone;
+        if (j >= p.top_k) continue;
+        const uint32_t own = chosen_key[j];
+        if (own >= kLowest) e[m] = chosen[j];
+        if (told || own < kLowest) continue;
+        const uint32_t after = chosen_key[j + 1];
+        const float w = value_of(own & ~kName), v = value_of(after & ~kName);
+        if (after >= kLowest && !(w - v > tol + fabsf(w) * (V * 2.4e-7f))) {
+          // Equal in logit and bias they are in the right order, but behind the last there may be another.
+          const uint32_t f = chosen[j + 1];
+          near |= j + 1 == p.top_k || logit_at(p, token, e[m]) != logit_at(p, token, f) ||
+                  (p.bias && p.bias[e[m]] != p.bias[f]);
+        }
       }
     }
     if (__any_sync(kFull, near)) {
@@ -653,11 +740,11 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
     for (int m = 0; m < kMine; ++m) {
       const uint32_t j = sub + m * kLanes;
       word[m] = e[m] != kNone ? words[e[m]] : 0;
-      if (here && j < p.top_k)
-        p.places[(size_t)token * p.top_k + j] =
-            e[m] == kNone ? -1
-                          : (int32_t)((word[m] & 0xffffffu) +
-                                      __popc(word[m] >> 24 & ((1u << slot) - 1)));
+      const uint32_t rank = (word[m] & 0xffffffu) + __popc(word[m] >> 24 & ((1u << slot) - 1));
+      kept_e[m] = here ? e[m] : kNone;
+      kept_rank[m] = rank;
+      if (here && j < p.top_k && !(once && e[m] != kNone))
+        p.places[(size_t)token * p.top_k + j] = e[m] == kNone ? -1 : (int32_t)rank;
     }
     __syncwarp();
 #pragma unroll
@@ -689,7 +776,18 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
   for (uint32_t e = threadIdx.x; e <= p.experts; e += kThreads) p.offsets[e] = (int32_t)offset[e];
   for (uint32_t e = lane; e < p.experts; e += 32) words[e] += offset[e];
   __syncwarp();
-  place_pairs<true>(p, first, end, words);
+  if (!once) {
+    place_pairs<true>(p, first, end, words);
+  } else if (first < end) {
+#pragma unroll
+    for (int m = 0; m < kMine; ++m) {
+      if (kept_e[m] == kNone) continue;
+      const uint32_t at = words[kept_e[m]] + kept_rank[m];
+      const size_t pair = (size_t)(first + slot) * p.top_k + sub + m * kLanes;
+      p.places[pair] = (int32_t)at;
+      p.order[at] = (int32_t)pair;
+    }
+  }
 }
 
 // Places the pairs of run blockIdx.x, ranked within it, behind those of the runs before it.
@@ -738,29 +836,36 @@ __global__ void __launch_bounds__(kPlaceThreads, 1)
   }
 }
 
-template <int kLanes, int V, bool kScored, int kWarps>
+template <int kLanes, int V, bool kScored, int kWarps, bool kTop8>
 cudaError_t run_warps(RouteProblem p, cudaStream_t stream) {
   constexpr uint32_t kTokens = 32 / kLanes;
-  p.run_warp = ((p.run + kWarps - 1) / kWarps + kTokens - 1) / kTokens * kTokens;
+  const uint32_t run = std::min(p.run, p.tokens);
+  p.run_warp = ((run + kWarps - 1) / kWarps + kTokens - 1) / kTokens * kTokens;
   const size_t size = p.logits_dtype == TX_BF16 ? 2 : 4;
   p.vec = p.per_lane == V && V * size % 16 == 0 && p.experts % (16 / size) == 0 &&
           p.ld * size % 16 == 0 && (uintptr_t)p.logits % 16 == 0;
   const uint32_t bytes = ((kWarps + 1) * p.experts + 1 + kWarps + (kScored ? kLanes * V : 0) +
-                          kWarps * kTokens * kSlotWords + (V > 8 ? kWarps * V * 32 : 0)) *
+                          kWarps * kTokens * kSlotWords + (V > 8 && !kTop8 ? kWarps * V * 32 : 0)) *
                          4;
   static std::atomic<uint64_t> seen{0};
-  cudaError_t e = allow_smem((const void *)route_kernel<kLanes, V, kScored, kWarps>, 232448, seen);
+  cudaError_t e = allow_smem((const void *)route_kernel<kLanes, V, kScored, kWarps, kTop8>, 232448, seen);
   if (e != cudaSuccess) return e;
-  route_kernel<kLanes, V, kScored, kWarps><<<p.blocks, 32 * kWarps, bytes, stream>>>(p);
+  route_kernel<kLanes, V, kScored, kWarps, kTop8><<<p.blocks, 32 * kWarps, bytes, stream>>>(p);
   if ((e = cudaGetLastError()) != cudaSuccess || p.blocks == 1 || !p.order) return e;
   place_kernel<<<p.blocks, kPlaceThreads, 0, stream>>>(p);
   return cudaGetLastError();
 }
-template <int kLanes, int V>
+// Few warps where a round of theirs takes all tokens: a block of 32 is slower to start and to add up.
+template <int kLanes, int V, bool kScored, bool kTop8>
 cudaError_t run(const RouteProblem &p, cudaStream_t stream) {
-  constexpr int kWarps = V <= 8 ? kMostWarps : kMostWarps / 2;  // as registers allow
-  return p.bias || p.groups > 1 ? run_warps<kLanes, V, true, kWarps>(p, stream)
-                                : run_warps<kLanes, V, false, kWarps>(p, stream);
+  constexpr int kWarps = V <= 8 || kTop8 ? kMostWarps : kMostWarps / 2;  // as registers allow
+  if (p.tokens <= 4 * (32 / kLanes)) return run_warps<kLanes, V, kScored, 4, kTop8>(p, stream);
+  return run_warps<kLanes, V, kScored, kWarps, kTop8>(p, stream);
+}
+template <int kLanes, int V>
+cudaError_t run_rounds(const RouteProblem &p, cudaStream_t stream) {
+  return p.bias || p.groups > 1 ? run<kLanes, V, true, false>(p, stream)
+                                : run<kLanes, V, false, false>(p, stream);
 }
 
 }  // namespace
@@ -774,6 +879,15 @@ size_t route_plan(RouteProblem *p, int num_sms) {
 }
 
 cudaError_t launch_experts_route(RouteProblem p, cudaStream_t stream) {
+  if (!p.bias && p.groups == 1 && p.top_k <= 8 && p.experts <= 512) {
+    p.group_lanes = 0;
+    p.per_lane = p.experts <= 32 ? 8 : 16;
+    if (p.experts <= 32) return run<4, 8, false, true>(p, stream);
+    if (p.experts <= 64) return run<4, 16, false, true>(p, stream);
+    if (p.experts <= 128) return run<8, 16, false, true>(p, stream);
+    if (p.experts <= 256) return run<16, 16, false, true>(p, stream);
+    return run<32, 16, false, true>(p, stream);
+  }
   // Experts of a lane: 8 where 32 lanes can hold them.  (16 make a third fewer instructions a token but
   // leave too few tokens in work: 66 / 48 us for 16384 tokens and 256 experts in groups.)  With groups a
   // group has to be whole lanes; where no number of experts a lane does that, group_lanes is 0.
@@ -789,12 +903,12 @@ cudaError_t launch_experts_route(RouteProblem p, cudaStream_t stream) {
       }
   }
   const uint32_t lanes = (p.experts + p.per_lane - 1) / p.per_lane;
-  if (most == 32) return run<32, 32>(p, stream);
-  if (most == 16) return run<32, 16>(p, stream);
-  if (lanes <= 4) return run<4, 8>(p, stream);
-  if (lanes <= 8) return run<8, 8>(p, stream);
-  if (lanes <= 16) return run<16, 8>(p, stream);
-  return run<32, 8>(p, stream);
+  if (most == 32) return run_rounds<32, 32>(p, stream);
+  if (most == 16) return run_rounds<32, 16>(p, stream);
+  if (lanes <= 4) return run_rounds<4, 8>(p, stream);
+  if (lanes <= 8) return run_rounds<8, 8>(p, stream);
+  if (lanes <= 16) return run_rounds<16, 8>(p, stream);
+  return run_rounds<32, 8>(p, stream);
 }
 
 }  // namespace tx

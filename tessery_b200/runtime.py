@@ -70,13 +70,12 @@ def _norm_fields(norm: Mapping[str, Any] | None) -> tuple:
     """weight, bias, kind, dtype, eps, offset of a norm as TxNorm has them."""
     if norm is None:
         return 0, 0, 0, 0, 0.0, 0.0
-    kind = native.NORMS.get(norm.get("kind"))
-    eps, offset = norm.get("eps", 1e-6), norm.get("offset", 0.0)
-    if (kind is None or not norm.keys() <= _NORM_KEYS
-            or max(abs(eps), abs(offset)) > _F32_MAX):
+    get = norm.get
+    kind, eps, offset = native.NORMS.get(get("kind")), get("eps", 1e-6), get("offset", 0.0)
+    if (kind is None or not _NORM_KEYS.issuperset(norm) or not -_F32_MAX <= eps <= _F32_MAX
+            or not -_F32_MAX <= offset <= _F32_MAX):
         raise InvalidInputError()
-    return (norm.get("weight") or 0, norm.get("bias") or 0, kind, norm.get("dtype", native.TX_F32),
-            eps, offset)
+    return get("weight") or 0, get("bias") or 0, kind, get("dtype", native.TX_F32), eps, offset
 
 
 class Buffer:
