@@ -20,7 +20,6 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
-#include <type_traits>
 
 #include "../../include/tessattn.h"
 #include "common.cuh"
@@ -33,22 +32,12 @@ constexpr uint32_t kFull = 0xffffffffu, kNone = 0xffffffffu;
 constexpr uint32_t kMaxK = 32;
 constexpr int kMostWarps = 32;  // of a block
 
-// Values as unsigned integers of the same order: 0 is closed, 1 is NaN (below every number).  The quick
-// keys of the kernel know neither: its closed experts are -inf, below kLowest, and a NaN is chosen exactly.
+// Values as unsigned integers of the same order.  Closed experts are -inf, below kLowest; of a token with a NaN
+// the experts are chosen by choose_exact.
 constexpr uint32_t kLowest = 0x00800000u;  // the key of fp32's lowest value
-__device__ __forceinline__ uint32_t quick_key(float c) {
-  const uint32_t u = __float_as_uint(c + 0.f);  // -0 as 0
-  return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
-}
 __device__ __forceinline__ uint32_t key_of(float c) {
   const uint32_t u = __float_as_uint(c + 0.f);  // -0 as 0
-  if (c != c) return 1;
-  return u >> 31 ? ~u : u | 0x80000000u;
-}
-__device__ __forceinline__ uint64_t key_of(double c) {
-  const uint64_t u = (uint64_t)__double_as_longlong(c + 0.0);
-  if (c != c) return 1;
-  return u >> 63 ? ~u : u | 0x8000000000000000ull;
+  return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float(key >> 31 ? key & 0x7fffffffu : ~key);
@@ -67,9 +56,36 @@ __device__ __forceinline__ float quick_rcp(float x) {
   return y;
 }
 __device__ __forceinline__ float sigmoid(float l) { return quick_rcp(1.f + quick_exp(-l)); }
-__device__ __forceinline__ double sigmoid(double l) { return 1.0 / (1.0 + exp(-l)); }
-__device__ __forceinline__ float exp_of(float x) { return quick_exp(x); }
-__device__ __forceinline__ double exp_of(double x) { return exp(x); }
+// e^x in 64 bits without a branch, so that a lane's many overlap: x = k ln 2 + r with ln 2 in two parts, the
+// Taylor series of e^r to r^13 (|r| < 0.35: 4e-18 is left), and k into the exponent.  To 0 below -700.
+__device__ __forceinline__ double exp_of(double x) {
+  const double z = fmin(fmax(x, -700.0), 700.0), k = rint(z * 1.4426950408889634);
+  const double r = fma(k, -1.9082149292705877e-10, fma(k, -0.693147180369123816490, z));
+  double y = 1.0 / 6227020800.0;
+  y = fma(y, r, 1.0 / 479001600.0);
+  y = fma(y, r, 1.0 / 39916800.0);
+  y = fma(y, r, 1.0 / 3628800.0);
+  y = fma(y, r, 1.0 / 362880.0);
+  y = fma(y, r, 1.0 / 40320.0);
+  y = fma(y, r, 1.0 / 5040.0);
+  y = fma(y, r, 1.0 / 720.0);
+  y = fma(y, r, 1.0 / 120.0);
+  y = fma(y, r, 1.0 / 24.0);
+  y = fma(y, r, 1.0 / 6.0);
+  y = fma(y, r, 0.5);
+  y = fma(y, r, 1.0);
+  y = fma(y, r, 1.0);
+  y = __longlong_as_double(__double_as_longlong(y) + ((long long)(int)k << 52));
+  return x != x ? x : y;
+}
+// 1 / (1 + e^-l): the reciprocal by Newton's steps from the hardware's.
+__device__ __forceinline__ double sigmoid(double l) {
+  const double t = exp_of(-fabs(l)), d = 1.0 + t;  // 1 .. 2
+  double y = (double)quick_rcp((float)d);
+  y = fma(y, fma(-d, y, 1.0), y);
+  y = fma(y, fma(-d, y, 1.0), y);
+  return l < 0 ? t * y : y;
+}
 
 template <int kLanes, typename S>
 __device__ __forceinline__ S lanes_sum(S v) {
@@ -109,40 +125,32 @@ __device__ __forceinline__ float score_tolerance(bool softmax, float inv_sum) {
   return softmax ? (float)((V + 16) * 1.1920929e-7f) * inv_sum : 7.2e-7f;
 }
 
-template <typename S>
-__device__ __forceinline__ S larger(S a, S b) {
-  return a > b ? a : b;
-}
-template <typename S>
-__device__ __forceinline__ S smaller(S a, S b) {
-  return a < b ? a : b;
-}
 // keep_groups for groups that cut through lanes: one after the other over all lanes.
-template <int kLanes, int V, typename S>
+template <int kLanes, int V>
 __device__ __noinline__ uint32_t keep_any_groups(const RouteProblem &p, uint32_t sub, uint32_t slot,
-                                                 const S (&c)[V], float tol, bool *near) {
-  const S none = -(S)INFINITY;
+                                                 const float (&c)[V], float tol, bool *near) {
+  const float none = -INFINITY;
   const uint32_t per = p.experts / p.groups;
   auto sum_of = [&](uint32_t g) {
-    S a = none, b = none;
+    float a = none, b = none;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const uint32_t e = sub * p.per_lane + i;
-      const S v = i < (int)p.per_lane && e >= g * per && e < (g + 1) * per ? c[i] : none;
-      b = larger(b, smaller(a, v));
-      a = larger(a, v);
+      const float v = i < (int)p.per_lane && e >= g * per && e < (g + 1) * per ? c[i] : none;
+      b = fmaxf(b, fminf(a, v));
+      a = fmaxf(a, v);
     }
 #pragma unroll
     for (int o = kLanes / 2; o > 0; o >>= 1) {
-      const S x = __shfl_xor_sync(kFull, a, o), y = __shfl_xor_sync(kFull, b, o);
-      b = larger(smaller(a, x), larger(b, y));
-      a = larger(a, x);
+      const float x = __shfl_xor_sync(kFull, a, o), y = __shfl_xor_sync(kFull, b, o);
+      b = fmaxf(fminf(a, x), fmaxf(b, y));
+      a = fmaxf(a, x);
     }
     return p.group_best > 1 && b > none ? a + b : a;
   };
   // The lane keeps the sums of groups sub, sub + kLanes, ...: 64 groups at most.
   constexpr int kSums = 64 / kLanes;
-  S sums[kSums];
+  float sums[kSums];
   uint32_t before[kSums];
 #pragma unroll
   for (int m = 0; m < kSums; ++m) {
@@ -150,13 +158,13 @@ __device__ __noinline__ uint32_t keep_any_groups(const RouteProblem &p, uint32_t
     before[m] = 0;
   }
   for (uint32_t g = 0; g < p.groups; ++g) {
-    const S s = sum_of(g);
+    const float s = sum_of(g);
 #pragma unroll
     for (int m = 0; m < kSums; ++m)
       if (g == sub + m * kLanes) sums[m] = s;
   }
   for (uint32_t h = 0; h < p.groups; ++h) {
-    S other = none;
+    float other = none;
 #pragma unroll
     for (int m = 0; m < kSums; ++m)
       if (h / kLanes == m) other = sums[m];
@@ -166,9 +174,9 @@ __device__ __noinline__ uint32_t keep_any_groups(const RouteProblem &p, uint32_t
       before[m] += other > sums[m] || (other == sums[m] && h < sub + m * kLanes);
   }
   uint32_t mask = 0;
-  S low = (S)INFINITY, high = none;  // the lowest sum kept, the highest left out
+  float low = INFINITY, high = none;  // the lowest sum kept, the highest left out
   for (uint32_t g = 0; g < p.groups; ++g) {
-    S s = none;
+    float s = none;
     uint32_t n = 0;
 #pragma unroll
     for (int m = 0; m < kSums; ++m)
@@ -179,58 +187,58 @@ __device__ __noinline__ uint32_t keep_any_groups(const RouteProblem &p, uint32_t
     s = __shfl_sync(kFull, s, slot * kLanes + g % kLanes);
     n = __shfl_sync(kFull, n, slot * kLanes + g % kLanes);
     if (n < p.top_groups) {
-      low = smaller(low, s);
+      low = fminf(low, s);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const uint32_t e = sub * p.per_lane + i;
         if (e >= g * per && e < (g + 1) * per) mask |= 1u << i;
       }
     } else {
-      high = larger(high, s);
+      high = fmaxf(high, s);
     }
   }
-  if (sizeof(S) == 4 && high > none)
-    *near |= low - high <= (S)(3.f * tol) + (low < 0 ? -low : low) * (S)2.4e-7f;
+  if (high > none)
+    *near |= low - high <= 3.f * tol + fabsf(low) * 2.4e-7f;
   return mask;
 }
 // Whether the lane's experts lie in a group that stays, bit i for its i-th; c[i] is -inf where closed or
-// NaN.  near: whether a sum that stays and one that does not are closer than tol (fp32 only).
-template <int kLanes, int V, typename S>
+// NaN.  near: whether a sum that stays and one that does not are closer than fp32 tells.
+template <int kLanes, int V>
 __device__ __forceinline__ uint32_t keep_groups(const RouteProblem &p, uint32_t sub, uint32_t slot,
-                                                const S (&c)[V], float tol, bool *near) {
-  const S none = -(S)INFINITY;
+                                                const float (&c)[V], float tol, bool *near) {
+  const float none = -INFINITY;
   if (p.group_lanes) {
     // A group is group_lanes lanes: the best two of a lane, then of its group, then the group's place among
     // the others.
-    S a = none, b = none;
+    float a = none, b = none;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      b = larger(b, smaller(a, c[i]));
-      a = larger(a, c[i]);
+      b = fmaxf(b, fminf(a, c[i]));
+      a = fmaxf(a, c[i]);
     }
     const uint32_t g = sub / p.group_lanes, at = sub - g * p.group_lanes;
     const uint32_t base = slot * kLanes + g * p.group_lanes;
-    S best = a, second = b;
+    float best = a, second = b;
     for (uint32_t t = 1; t < p.group_lanes; ++t) {
       const uint32_t from = at + t < p.group_lanes ? at + t : at + t - p.group_lanes;
-      const S x = __shfl_sync(kFull, a, (base + from) & 31);
-      const S y = __shfl_sync(kFull, b, (base + from) & 31);
-      second = larger(smaller(best, x), larger(second, y));
-      best = larger(best, x);
+      const float x = __shfl_sync(kFull, a, (base + from) & 31);
+      const float y = __shfl_sync(kFull, b, (base + from) & 31);
+      second = fmaxf(fminf(best, x), fmaxf(second, y));
+      best = fmaxf(best, x);
     }
-    const S sum = p.group_best > 1 && second > none ? best + second : best;
-    const S close = (S)(3.f * tol) + (sum < 0 ? -sum : sum) * (S)2.4e-7f;
+    const float sum = p.group_best > 1 && second > none ? best + second : best;
+    const float close = 3.f * tol + fabsf(sum) * 2.4e-7f;
     uint32_t before = 0;
     bool touch = false;
     for (uint32_t h = 0; h < p.groups; ++h) {
-      const S other = __shfl_sync(kFull, sum, slot * kLanes + h * p.group_lanes);
+      const float other = __shfl_sync(kFull, sum, slot * kLanes + h * p.group_lanes);
       before += other > sum || (other == sum && h < g);
       touch |= h != g && other <= sum + close && other >= sum - close;
     }
     const bool kept = before < p.top_groups;
-    if (sizeof(S) == 4 && __any_sync(kFull, touch && g < p.groups && sum > none)) {
+    if (__any_sync(kFull, touch && g < p.groups && sum > none)) {
       for (uint32_t h = 0; h < p.groups; ++h) {
-        const S other = __shfl_sync(kFull, sum, slot * kLanes + h * p.group_lanes);
+        const float other = __shfl_sync(kFull, sum, slot * kLanes + h * p.group_lanes);
         const bool stays = __shfl_sync(kFull, (int)kept, slot * kLanes + h * p.group_lanes);
         *near |= g < p.groups && sum > none && stays != kept && other <= sum + close &&
                  other >= sum - close;
@@ -238,91 +246,117 @@ __device__ __forceinline__ uint32_t keep_groups(const RouteProblem &p, uint32_t 
     }
     return kept ? kFull : 0;
   }
-  return keep_any_groups<kLanes, V, S>(p, sub, slot, c, tol, near);
+  return keep_any_groups<kLanes, V>(p, sub, slot, c, tol, near);
 }
 
-template <typename S>
-struct KeyOf {
-  using type = uint32_t;
-};
-template <>
-struct KeyOf<double> {
-  using type = uint64_t;
-};
-
-// The choice of the warp's tokens with whole keys: of the logits as they are (S float), or of scores in 64
-// bits.  Reads the logits again and leaves the chosen experts in `chosen`, kNone behind the last.
-template <int kLanes, int V, typename S>
+// The choice of the warp's tokens with whole values: of the logits as they are, or of scores in 64 bits.  Reads
+// the logits again and leaves the chosen experts in `chosen`, kNone behind the last.  Few tokens come here, and
+// then the code does for the first time: loops over values in local memory, little unrolled.
+template <int kLanes, int V, bool kScored>
 __device__ __noinline__ void choose_exact(const RouteProblem &p, uint32_t *chosen, uint32_t token,
                                           bool valid, uint32_t sub, uint32_t slot) {
-  using Key = typename KeyOf<S>::type;
-  const bool scored = sizeof(S) == 8;
-  S c[V];
-  bool open[V];
-  S sum = 0;
-  float top_l = -INFINITY;
-#pragma unroll
+  double c[V];  // -inf: closed
+  uint32_t nan = 0;
+  float top = -INFINITY;
+  const uint32_t first = sub * p.per_lane;
+#pragma unroll 4
   for (int i = 0; i < V; ++i) {
-    const uint32_t e = sub * p.per_lane + i;
-    open[i] = valid && i < (int)p.per_lane && e < p.experts;
-    float l = open[i] ? logit_at(p, token, e) : -INFINITY;
-    open[i] = l != -INFINITY && !(p.bias && p.bias[e] == -INFINITY);
-    if (open[i]) top_l = fmaxf(top_l, l);
-    c[i] = (S)l;
+    const uint32_t e = first + i;
+    float l = valid && i < (int)p.per_lane && e < p.experts ? logit_at(p, token, e) : -INFINITY;
+    if (l != -INFINITY && p.bias && p.bias[e] == -INFINITY) l = -INFINITY;
+    top = fmaxf(top, l);
+    c[i] = l;
   }
-  if (scored) {
-    if (p.softmax) {
-      top_l = lanes_max<kLanes>(top_l);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        if (open[i]) c[i] = exp_of(c[i] - (S)top_l);
-        if (open[i]) sum += c[i];
-      }
-      sum = lanes_sum<kLanes>(sum);
-#pragma unroll
-      for (int i = 0; i < V; ++i) c[i] /= sum;
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (open[i]) c[i] = sigmoid(c[i]);
+  if constexpr (kScored) {
+    top = lanes_max<kLanes>(top);
+    double sum = 0.0;
+#pragma unroll 4
+    for (int i = 0; i < V; ++i) {
+      const double s = p.softmax ? exp_of(c[i] - (double)top) : sigmoid(c[i]);
+      const bool is = c[i] != -INFINITY;
+      c[i] = is ? s : c[i];
+      sum += is ? s : 0.0;
     }
-#pragma unroll
+    const double inv = p.softmax ? 1.0 / lanes_sum<kLanes>(sum) : 1.0;
+#pragma unroll 1
     for (int i = 0; i < V; ++i)
-      if (open[i] && p.bias) c[i] += (S)p.bias[sub * p.per_lane + i];
+      if (c[i] != -INFINITY) c[i] = c[i] * inv + (p.bias ? (double)p.bias[first + i] : 0.0);
   }
+  // NaN ranks below every number: -inf from here on, with a mark.
+#pragma unroll 1
+  for (int i = 0; i < V; ++i)
+    if (c[i] != c[i]) {
+      nan |= 1u << i;
+      c[i] = -INFINITY;
+    }
   uint32_t kept = kFull;
   if (p.groups > 1) {
-    S g[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) g[i] = open[i] && c[i] == c[i] ? c[i] : -(S)INFINITY;
-    bool none;
-    kept = keep_groups<kLanes, V, S>(p, sub, slot, g, 0.f, &none);
-  }
-  Key key[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) key[i] = open[i] && (kept >> i & 1) ? key_of(c[i]) : 0;
-  for (uint32_t j = 0; j < p.top_k; ++j) {
-    Key top = 0;
-    uint32_t at = 0;
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (key[i] > top) {
-        top = key[i];
-        at = sub * p.per_lane + i;
+    // One group after the other: its best two over all lanes.  The lane keeps the sums of groups sub,
+    // sub + kLanes, ...: 64 at most.
+    const uint32_t per = p.experts / p.groups;
+    constexpr int kSums = 64 / kLanes;
+    double sums[kSums];
+#pragma unroll 1
+    for (uint32_t g = 0; g < p.groups; ++g) {
+      double a = -INFINITY, b = -INFINITY;
+#pragma unroll 4
+      for (uint32_t e = max(g * per, first); e < min((g + 1) * per, first + p.per_lane); ++e) {
+        const double v = c[e - first];
+        b = fmax(b, fmin(a, v));
+        a = fmax(a, v);
       }
+#pragma unroll 1
+      for (int o = kLanes / 2; o > 0; o >>= 1) {
+        const double x = __shfl_xor_sync(kFull, a, o), y = __shfl_xor_sync(kFull, b, o);
+        b = fmax(fmin(a, x), fmax(b, y));
+        a = fmax(a, x);
+      }
+      if (g % kLanes == sub) sums[g / kLanes] = p.group_best > 1 && b > -INFINITY ? a + b : a;
+    }
+    kept = 0;
+#pragma unroll 1
+    for (uint32_t g = 0; g < p.groups; ++g) {
+      const double own = __shfl_sync(kFull, sums[g / kLanes], slot * kLanes + g % kLanes);
+      uint32_t before = 0;
+#pragma unroll 1
+      for (uint32_t h = sub; h < p.groups; h += kLanes)
+        before += sums[h / kLanes] > own || (sums[h / kLanes] == own && h < g);
+      __syncwarp();
 #pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) before += __shfl_xor_sync(kFull, before, o);
+      if (before < p.top_groups)
+#pragma unroll 1
+        for (uint32_t e = max(g * per, first); e < min((g + 1) * per, first + p.per_lane); ++e)
+          kept |= 1u << (e - first);
+    }
+  }
+  // Taken experts lose their bit; the NaN that are left rank behind all numbers, by index.
+  uint32_t open = 0;
+#pragma unroll 1
+  for (int i = 0; i < V; ++i)
+    if (c[i] > -INFINITY || (nan >> i & 1)) open |= 1u << i;
+  open &= kept;
+#pragma unroll 1
+  for (uint32_t j = 0; j < p.top_k; ++j) {
+    double best = -INFINITY;
+    uint32_t at = kNone;  // what is left, numbers first, then the lower index
+#pragma unroll 4
+    for (int i = 0; i < V; ++i)
+      if ((open >> i & 1) && (at == kNone || c[i] > best)) {
+        best = c[i];
+        at = first + i;
+      }
+#pragma unroll 1
     for (int o = kLanes / 2; o > 0; o >>= 1) {
-      const Key k2 = __shfl_xor_sync(kFull, top, o);
+      const double other = __shfl_xor_sync(kFull, best, o);
       const uint32_t at2 = __shfl_xor_sync(kFull, at, o);
-      if (k2 > top || (k2 == top && at2 < at)) {
-        top = k2;
+      if (other > best || (other == best && at2 < at)) {
+        best = other;
         at = at2;
       }
     }
-    if (sub == 0) chosen[j] = top ? at : kNone;
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (sub * p.per_lane + i == at) key[i] = 0;
+    if (sub == 0) chosen[j] = at;
+    if (at >= first && at < first + p.per_lane) open &= ~(1u << (at - first));
   }
   __syncwarp();
 }
@@ -486,7 +520,7 @@ __device__ __forceinline__ void place_pairs(const RouteProblem &p, uint32_t firs
 // token in work its chosen experts and their keys, one more than there may be, and the lanes' sorted keys.
 constexpr uint32_t kSlotWords = 2 * (kMaxK + 1);
 
-// kTop8: up to 8 experts a token, chosen by their logits alone.  Every lane's 8 largest meet those of the
+// kTop8: up to 8 experts a token.  Every lane's 8 largest meet those of the
 // other lanes in steps of a shuffle for each (8 maxima and a sort of 8), after which every lane has the
 // token's 8, without a round for each or a branch.  Their keys name the expert in all lanes.
 template <int kLanes, int V, bool kScored, int kWarps, bool kTop8>
@@ -547,7 +581,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
     const bool here = token < end, had = valid;
     float tol = 0.f, all_top = 0.f, all_sum = 1.f;  // of all logits, where the weights need them
     uint32_t key[V];
-    bool near = false;
+    bool near = false, far = false;  // neighbours to put in order; a choice to make again
     {
       float c[V];
 #pragma unroll
@@ -571,7 +605,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
         }
         all_sum = lanes_sum<kLanes>(sum);
       }
-      if constexpr (kTop8) {
+      if constexpr (kTop8 && !kScored) {
         // fp32 logits that were bf16 are many equals: they are told apart as well.
         uint32_t low = 0;
 #pragma unroll
@@ -581,9 +615,9 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
       if constexpr (!kScored) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          near |= c[i] != c[i];
-          key[i] = told ? (quick_key(c[i]) & ~kNameAll) | (kNameAll - sub * p.per_lane - i)
-                        : (quick_key(c[i]) & ~kName) | (kName - (kTop8 ? sub * p.per_lane : 0) - i);
+          far |= c[i] != c[i];
+          key[i] = told ? (key_of(c[i]) & ~kNameAll) | (kNameAll - sub * p.per_lane - i)
+                        : (key_of(c[i]) & ~kName) | (kName - (kTop8 ? sub * p.per_lane : 0) - i);
         }
       } else {
         const float inv = p.softmax ? quick_rcp(all_sum) : 1.f;
@@ -591,14 +625,16 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
         for (int i = 0; i < V; ++i) {
           const float s = p.softmax ? quick_exp(c[i] - all_top) * inv : sigmoid(c[i]);
           c[i] = c[i] == -INFINITY ? -INFINITY : s + bias[i * kLanes + sub];
-          near |= c[i] != c[i];
+          far |= c[i] != c[i];
         }
         tol = score_tolerance<V>(p.softmax, inv);
         uint32_t kept = kFull;
-        if (p.groups > 1) kept = keep_groups<kLanes, V, float>(p, sub, slot, c, tol, &near);
+        if (p.groups > 1) kept = keep_groups<kLanes, V>(p, sub, slot, c, tol, &far);
 #pragma unroll
         for (int i = 0; i < V; ++i)
-          key[i] = kept >> i & 1 ? (quick_key(c[i]) & ~kName) | (V - 1 - i) : 0;
+          key[i] = kept >> i & 1
+                       ? (key_of(c[i]) & ~kName) | (kName - (kTop8 ? sub * p.per_lane : 0) - i)
+                       : 0;
       }
     }
     // The next tokens' logits travel meanwhile.
@@ -631,22 +667,81 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
         sort_bitonic(t);
       }
       load_next();
-      uint32_t ninth = 0;
-      if (!told) {
-        // The largest that is left, or, where a lane's 8 are all among the token's, that lane's next may be.
-#pragma unroll
-        for (int i = 7; i >= 0; --i) ninth = own[i] < t[7] ? max(ninth, own[i]) : ninth;
-        ninth = lanes_max<kLanes>(own[7] >= t[7] && t[7] >= kLowest && V > 8 ? t[7] : ninth);
-      }
       const uint32_t names = told ? kNameAll : kName;
 #pragma unroll
       for (int m = 0; m < kMine; ++m) {
-        const uint32_t j = sub + m * kLanes;
-        e[m] = kNone;
-        if (j >= p.top_k) continue;
-        const uint32_t mine = pick(t, j), after = j < 7 ? pick(t, j + 1) : ninth;
-        if (mine >= kLowest) e[m] = names - (mine & names);
-        near |= !told && mine >= kLowest && (mine & ~kName) == (after & ~kName);
+        const uint32_t j = sub + m * kLanes, mine = pick(t, j & 7);
+        e[m] = j < p.top_k && mine >= kLowest ? names - (mine & names) : kNone;
+      }
+      if (!told) {
+        // The largest behind the 8.
+        uint32_t ninth = 0;
+#pragma unroll
+        for (int i = 7; i >= 0; --i) ninth = own[i] < t[7] ? max(ninth, own[i]) : ninth;
+        ninth = lanes_max<kLanes>(ninth);
+        auto key_at = [&](uint32_t j) { return j < 8 ? pick(t, j) : ninth; };
+        auto close = [&](uint32_t a, uint32_t b) {  // whether the order of a and b below it is in doubt
+          const float w = value_of(a & ~kName), v = value_of(b & ~kName);
+          return b >= kLowest && !(w - v > tol + fabsf(w) * ((kName + 1) * 1.3e-7f));
+        };
+#pragma unroll
+        for (int m = 0; m < kMine; ++m) {
+          const uint32_t j = sub + m * kLanes;
+          near |= e[m] != kNone && close(key_at(j), key_at(j + 1));
+        }
+        // (Where a lane's 8 are all among the token's, its next are not known.)
+        near |= V > 8 && own[7] >= t[7] && t[7] >= kLowest;
+        if (__any_sync(kFull, near)) {
+          // All that may belong among the chosen are put in the order of their logits, where scores grow with
+          // them, or of sigmoids in 64 bits.  Softmax scores with a bias need the sum in 64 bits too.
+          constexpr uint32_t kMost = 16;
+          constexpr int kEach = (kMost + kLanes - 1) / kLanes;
+          const uint32_t last = key_at(p.top_k - 1);
+          uint32_t count = 0;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const bool is = own[i] >= kLowest && (own[i] >= last || last < kLowest || close(last, own[i]));
+            const uint32_t all = __ballot_sync(kFull, is) & group_mask;
+            const uint32_t at = count + __popc(all & ((1u << lane) - 1));
+            if (is && at < kMost) chosen[at] = kName - (own[i] & kName);
+            count += __popc(all);
+            if (i == 7) far |= V > 8 && is;
+          }
+          far |= count > kMost || (near && kScored && p.softmax && p.bias);
+          __syncwarp();
+          if (!__any_sync(kFull, far)) {
+            double c[kEach];
+            uint32_t of[kEach], place[kEach], *high = chosen_key, *low = chosen_key + kMost;
+#pragma unroll
+            for (int m = 0; m < kEach; ++m) {
+              const uint32_t j = sub + m * kLanes;
+              of[m] = j < count ? chosen[j] : kNone;
+              place[m] = 0;
+              if (of[m] == kNone) continue;
+              c[m] = logit_at(p, token, of[m]);
+              if (kScored && p.bias) c[m] = sigmoid(c[m]) + (double)p.bias[of[m]];
+              high[j] = (uint32_t)((uint64_t)__double_as_longlong(c[m]) >> 32);
+              low[j] = (uint32_t)__double_as_longlong(c[m]);
+            }
+            __syncwarp();
+            for (uint32_t j = 0; j < count; ++j) {
+              const double other = __longlong_as_double((long long)((uint64_t)high[j] << 32 | low[j]));
+              const uint32_t other_e = chosen[j];
+#pragma unroll
+              for (int m = 0; m < kEach; ++m)
+                place[m] += of[m] != kNone && (other > c[m] || (other == c[m] && other_e < of[m]));
+            }
+            __syncwarp();
+#pragma unroll
+            for (int m = 0; m < kEach; ++m)
+              if (of[m] != kNone) chosen[place[m]] = of[m];
+            __syncwarp();
+#pragma unroll
+            for (int m = 0; m < kMine; ++m)
+              if (e[m] != kNone) e[m] = chosen[sub + m * kLanes];
+            __syncwarp();
+          }
+        }
       }
     } else {
       load_next();
@@ -687,15 +782,14 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
         if (after >= kLowest && !(w - v > tol + fabsf(w) * (V * 2.4e-7f))) {
           // Equal in logit and bias they are in the right order, but behind the last there may be another.
           const uint32_t f = chosen[j + 1];
-          near |= j + 1 == p.top_k || logit_at(p, token, e[m]) != logit_at(p, token, f) ||
+          far |= j + 1 == p.top_k || logit_at(p, token, e[m]) != logit_at(p, token, f) ||
                   (p.bias && p.bias[e[m]] != p.bias[f]);
         }
       }
     }
-    if (__any_sync(kFull, near)) {
+    if (__any_sync(kFull, far)) {
       __syncwarp();
-      choose_exact<kLanes, V, typename std::conditional<kScored, double, float>::type>(
-          p, chosen, token, had, sub, slot);
+      choose_exact<kLanes, V, kScored>(p, chosen, token, had, sub, slot);
 #pragma unroll
       for (int m = 0; m < kMine; ++m)
         if (sub + m * kLanes < p.top_k) e[m] = chosen[sub + m * kLanes];
@@ -863,6 +957,11 @@ cudaError_t run(const RouteProblem &p, cudaStream_t stream) {
   return run_warps<kLanes, V, kScored, kWarps, kTop8>(p, stream);
 }
 template <int kLanes, int V>
+cudaError_t run_top8(const RouteProblem &p, cudaStream_t stream) {
+  return p.bias || p.groups > 1 ? run<kLanes, V, true, true>(p, stream)
+                                : run<kLanes, V, false, true>(p, stream);
+}
+template <int kLanes, int V>
 cudaError_t run_rounds(const RouteProblem &p, cudaStream_t stream) {
   return p.bias || p.groups > 1 ? run<kLanes, V, true, false>(p, stream)
                                 : run<kLanes, V, false, false>(p, stream);
@@ -879,35 +978,36 @@ size_t route_plan(RouteProblem *p, int num_sms) {
 }
 
 cudaError_t launch_experts_route(RouteProblem p, cudaStream_t stream) {
-  if (!p.bias && p.groups == 1 && p.top_k <= 8 && p.experts <= 512) {
+  // Experts of a lane.  With groups a group has to be whole lanes; where no number of experts a lane does
+  // that, group_lanes is 0.
+  auto cut = [&](uint32_t most) {
+    p.per_lane = most;
     p.group_lanes = 0;
-    p.per_lane = p.experts <= 32 ? 8 : 16;
-    if (p.experts <= 32) return run<4, 8, false, true>(p, stream);
-    if (p.experts <= 64) return run<4, 16, false, true>(p, stream);
-    if (p.experts <= 128) return run<8, 16, false, true>(p, stream);
-    if (p.experts <= 256) return run<16, 16, false, true>(p, stream);
-    return run<32, 16, false, true>(p, stream);
-  }
-  // Experts of a lane: 8 where 32 lanes can hold them.  (16 make a third fewer instructions a token but
-  // leave too few tokens in work: 66 / 48 us for 16384 tokens and 256 experts in groups.)  With groups a
-  // group has to be whole lanes; where no number of experts a lane does that, group_lanes is 0.
-  const uint32_t most = p.experts <= 256 ? 8 : p.experts <= 512 ? 16 : 32;
-  p.per_lane = most;
-  p.group_lanes = 0;
-  if (p.groups > 1) {
+    if (p.groups < 2) return;
     const uint32_t per = p.experts / p.groups;
     for (uint32_t v = std::min(most, per); v && !p.group_lanes; --v)
       if (per % v == 0 && p.experts / v <= 32) {
         p.per_lane = v;
         p.group_lanes = per / v;
       }
+  };
+  auto lanes = [&] { return (p.experts + p.per_lane - 1) / p.per_lane; };
+  if (p.top_k <= 8 && p.experts <= 512) {
+    cut(p.experts <= 32 ? 8 : 16);
+    if (p.experts <= 32 && lanes() <= 4) return run_top8<4, 8>(p, stream);
+    if (lanes() <= 4) return run_top8<4, 16>(p, stream);
+    if (lanes() <= 8) return run_top8<8, 16>(p, stream);
+    if (lanes() <= 16) return run_top8<16, 16>(p, stream);
+    return run_top8<32, 16>(p, stream);
   }
-  const uint32_t lanes = (p.experts + p.per_lane - 1) / p.per_lane;
+  // Rounds: 8 experts a lane where 32 lanes can hold them.
+  const uint32_t most = p.experts <= 256 ? 8 : p.experts <= 512 ? 16 : 32;
+  cut(most);
   if (most == 32) return run_rounds<32, 32>(p, stream);
   if (most == 16) return run_rounds<32, 16>(p, stream);
-  if (lanes <= 4) return run_rounds<4, 8>(p, stream);
-  if (lanes <= 8) return run_rounds<8, 8>(p, stream);
-  if (lanes <= 16) return run_rounds<16, 8>(p, stream);
+  if (lanes() <= 4) return run_rounds<4, 8>(p, stream);
+  if (lanes() <= 8) return run_rounds<8, 8>(p, stream);
+  if (lanes() <= 16) return run_rounds<16, 8>(p, stream);
   return run_rounds<32, 8>(p, stream);
 }
 
