@@ -202,10 +202,12 @@ __device__ __noinline__ uint32_t keep_any_groups(const RouteProblem &p, uint32_t
   return mask;
 }
 // Whether the lane's experts lie in a group that stays, bit i for its i-th; c[i] is -inf where closed or
-// NaN.  near: whether a sum that stays and one that does not are closer than fp32 tells.
+// NaN, top the largest logit of softmax scores.  near: whether a sum that stays and one that does not are
+// closer than fp32 tells, unless that is settled here.
 template <int kLanes, int V>
 __device__ __forceinline__ uint32_t keep_groups(const RouteProblem &p, uint32_t sub, uint32_t slot,
-                                                const float (&c)[V], float tol, bool *near) {
+                                                const float (&c)[V], float tol, size_t token, float top,
+                                                bool *near) {
   const float none = -INFINITY;
   if (p.group_lanes) {
     // A group is group_lanes lanes: the best two of a lane, then of its group, then the group's place among
@@ -235,13 +237,53 @@ __device__ __forceinline__ uint32_t keep_groups(const RouteProblem &p, uint32_t 
       before += other > sum || (other == sum && h < g);
       touch |= h != g && other <= sum + close && other >= sum - close;
     }
-    const bool kept = before < p.top_groups;
+    bool kept = before < p.top_groups;
     if (__any_sync(kFull, touch && g < p.groups && sum > none)) {
+      bool doubt = false;
       for (uint32_t h = 0; h < p.groups; ++h) {
         const float other = __shfl_sync(kFull, sum, slot * kLanes + h * p.group_lanes);
         const bool stays = __shfl_sync(kFull, (int)kept, slot * kLanes + h * p.group_lanes);
-        *near |= g < p.groups && sum > none && stays != kept && other <= sum + close &&
+        doubt |= g < p.groups && sum > none && stays != kept && other <= sum + close &&
                  other >= sum - close;
+      }
+      if (p.softmax && p.bias) {
+        *near |= doubt;  // the scores' sum is needed in 64 bits
+      } else if (__any_sync(kFull, doubt)) {
+        // The sums again in 64 bits, of the few experts that may be among a group's best two (softmax scores
+        // but for their common factor).
+        const float cut = (second > none ? second : best) - 2.f * tol - fabsf(second) * 2.4e-7f;
+        uint32_t left = 0;
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (c[i] > none && !(c[i] < cut)) left |= 1u << i;
+        double a2 = none, b2 = none;
+        while (__any_sync(kFull, left != 0)) {
+          if (left) {
+            const uint32_t e = sub * p.per_lane + __ffs(left) - 1;
+            left &= left - 1;
+            const double l = logit_at(p, token, e);
+            const double v = p.softmax ? exp_of(l - (double)top)
+                                       : sigmoid(l) + (p.bias ? (double)p.bias[e] : 0.0);
+            b2 = fmax(b2, fmin(a2, v));
+            a2 = fmax(a2, v);
+          }
+          __syncwarp();
+        }
+        double best2 = a2, second2 = b2;
+        for (uint32_t t = 1; t < p.group_lanes; ++t) {
+          const uint32_t from = at + t < p.group_lanes ? at + t : at + t - p.group_lanes;
+          const double x = __shfl_sync(kFull, a2, (base + from) & 31);
+          const double y = __shfl_sync(kFull, b2, (base + from) & 31);
+          second2 = fmax(fmin(best2, x), fmax(second2, y));
+          best2 = fmax(best2, x);
+        }
+        const double sum2 = p.group_best > 1 && second2 > none ? best2 + second2 : best2;
+        before = 0;
+        for (uint32_t h = 0; h < p.groups; ++h) {
+          const double other = __shfl_sync(kFull, sum2, slot * kLanes + h * p.group_lanes);
+          before += other > sum2 || (other == sum2 && h < g);
+        }
+        kept = before < p.top_groups;
       }
     }
     return kept ? kFull : 0;
@@ -629,7 +671,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
         }
         tol = score_tolerance<V>(p.softmax, inv);
         uint32_t kept = kFull;
-        if (p.groups > 1) kept = keep_groups<kLanes, V>(p, sub, slot, c, tol, &far);
+        if (p.groups > 1) kept = keep_groups<kLanes, V>(p, sub, slot, c, tol, token, all_top, &far);
 #pragma unroll
         for (int i = 0; i < V; ++i)
           key[i] = kept >> i & 1
