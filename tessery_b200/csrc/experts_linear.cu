@@ -413,9 +413,11 @@ __global__ void __launch_bounds__(kGather ? kGatherThreads : kThreads, 1)
       }
     }
     // No copy may land after the CTA has gone.
-    if (lane == 0)
+    if (lane == 0) {
+      const long long now = clock64();
       for (uint32_t s = 0; s < (uint32_t)C::kStages && s < fills; ++s)
-        drain_bar(bar(kBarFull + s), ((fills - 1 - s) / C::kStages) & 1);
+        drain_bar(bar(kBarFull + s), ((fills - 1 - s) / C::kStages) & 1, now);
+    }
     __syncwarp();
   } else if (kGather && warp >= 10) {
     uint32_t fills = 0, e = 0;
@@ -647,9 +649,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGather ? kGatherThr
       }
     }
     // No copy may land after the CTAs have gone.
-    if (lane == 0 && rank == 0)
+    if (lane == 0 && rank == 0) {
+      const long long now = clock64();
       for (uint32_t s = 0; s < (uint32_t)kStages && s < fills; ++s)
-        drain_bar(bar(kFullBar + s), ((fills - 1 - s) / kStages) & 1);
+        drain_bar(bar(kFullBar + s), ((fills - 1 - s) / kStages) & 1, now);
+    }
     __syncwarp();
   } else if (kGather && warp >= 10) {
     uint32_t fills = 0, e = 0;

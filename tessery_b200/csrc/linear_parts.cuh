@@ -30,10 +30,13 @@ __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile
     }
   }
 }
-__device__ __forceinline__ void drain_bar(uint32_t bar, uint32_t parity) {
-  const long long t0 = clock64();
-  while (!mbar_test(bar, parity) && clock64() - t0 < kDrainCycles) {
+// since: where several are drained in turn, when the first began.
+__device__ __forceinline__ void drain_bar(uint32_t bar, uint32_t parity, long long since) {
+  while (!mbar_test(bar, parity) && clock64() - since < kDrainCycles) {
   }
+}
+__device__ __forceinline__ void drain_bar(uint32_t bar, uint32_t parity) {
+  drain_bar(bar, parity, clock64());
 }
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, uint32_t src, int x, int y) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(

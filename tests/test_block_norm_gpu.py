@@ -116,6 +116,25 @@ def test_joined_rows(runtime, cols, top_k, dtype):
         check(block_norm(None, y, runtime=runtime, **kw), None, yf, **exact)
 
 
+@pytest.mark.parametrize("rows,cols", [(9000, 72), (9000, 50), (5000, 264), (3000, 600), (2500, 1024),
+                                       (2500, 1030), (700, 4096), (400, 9000)])
+def test_many_rows(runtime, rows, cols):
+    """More rows than are in work at once, plain and joined."""
+    rng = np.random.default_rng(rows)
+    x, xf = values(rng, (rows, cols))
+    n, ne = norm_of(rng, cols, "layer", "f32", bias=True)
+    for top_k in (0, 2):
+        y, yf = values(rng, (rows * max(1, top_k), cols), "bf16")
+        kw = {}
+        if top_k:
+            kw = dict(places=rng.permutation(rows * top_k).reshape(rows, top_k),
+                      weights=rng.random((rows, top_k)).astype(np.float32))
+        gate, gf = values(rng, (7, cols))
+        seq = -(-rows // 7)
+        check(block_norm(x, y, after=n, before=n, gate=gate, seq=seq, runtime=runtime, **kw), xf, yf,
+              after=ne, before=ne, gate=gf, gate_row=np.arange(rows) // seq, **kw)
+
+
 @pytest.mark.parametrize("gate_dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("cols", [40, 41, 1500])
 def test_gates(runtime, cols, gate_dtype):
@@ -228,7 +247,7 @@ def test_refusals(runtime):
                dict(after={**norm, "size": 3}), dict(after={**norm, "eps": -1.0}),
                dict(after={**norm, "eps": np.nan}), dict(before={**norm, "weight": p + 2}),
                dict(before={**norm, "dtype": 2}), dict(before={**norm, "offset": np.inf}),
-               {**join, "top_k": 0}, {**join, "weights": None}, {**join, "places": p + 2},
+               {**join, "top_k": 0}, {**join, "top_k": 33}, {**join, "weights": None}, {**join, "places": p + 2},
                {**join, "out": p + 512}, {**gate, "gate_rows": 2}, {**gate, "gate_rows": 0},
                {**gate, "gate_rows": 3, "seq": 1}, {**gate, "ldg": 8}, {**gate, "gate_dtype": 2},
                {**gate, "cu_seqlens": p, "seq": 4}, {**gate, "cu_seqlens": p + 1},

@@ -20,11 +20,13 @@ through the sigmoid, and 2^-8 of a row's largest logit (5 or more) is allowed to
 
 import importlib.util
 import sys
+import threading
 from pathlib import Path
 
 import numpy as np
 import pytest
 
+import tessery_b200 as tx
 from oracle import layers as oracle
 from tessery_b200 import rotary_frequencies, rotary_pair_axes
 from tessery_b200.workloads import from_bf16_bits, to_bf16_bits
@@ -137,3 +139,37 @@ def test_layer(runtime, heads, kv_heads, dim, sections, experts, top_k, groups, 
     assert np.array_equal(dev[0].cpu().numpy(), got) and np.array_equal(chosen.cpu().numpy(), ids)
     del graph
     layer.close()
+
+
+def test_threads_on_one_runtime(runtime):
+    """The operators on arrays from three threads: each call's result is the one it has alone."""
+    rng = np.random.default_rng(1)
+    cases = []
+    for n in (40, 300, 1100):
+        logits = rng.standard_normal((n, 16)).astype(np.float32)
+        x = to_bf16_bits(rng.standard_normal((n, 64)).astype(np.float32))
+        w = to_bf16_bits(rng.standard_normal((16, 96, 64)).astype(np.float32))
+        r = tx.experts_route(logits, 2, runtime=runtime)
+        cases.append((
+            lambda v=logits: np.concatenate([a.ravel() for a in tx.experts_route(v, 2, runtime=runtime)]),
+            lambda x=x, w=w, r=r: tx.experts_linear(x, w, r.offsets, order=r.order, top_k=2,
+                                                    runtime=runtime),
+            lambda x=x: tx.block_norm(x, x, before=dict(kind="layer"), runtime=runtime)[1]))
+    want = [[call() for call in case] for case in cases]
+    wrong = []
+
+    def work(i):
+        try:
+            for _ in range(15):
+                for call, w in zip(cases[i], want[i], strict=True):
+                    if not np.array_equal(call(), w):
+                        wrong.append(i)
+        except Exception as e:  # noqa: BLE001 - reported below
+            wrong.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong

@@ -10,7 +10,7 @@ import numpy as np
 import pytest
 
 from oracle import layers as oracle
-from tessery_b200 import InvalidInputError, TX_BF16, TX_F32
+from tessery_b200 import DeviceTimeoutError, InvalidInputError, TX_BF16, TX_F32
 from tessery_b200.layers import experts_linear
 from tessery_b200.workloads import from_bf16_bits, to_bf16_bits
 
@@ -103,6 +103,37 @@ def test_long_sums_and_several_tiles(runtime, rows, experts, n, k, gated, out):
     assert np.array_equal(got, experts_linear(x, w, offsets, out_dtype=out, runtime=runtime, **kw))
 
 
+@pytest.mark.parametrize("gated,n,k,out", [(True, 150, 200, "bf16"), (True, 128, 64, "float32"),
+                                           (False, 300, 72, "bf16"), (False, 257, 513, "bf16"),
+                                           (False, 512, 130, "float32")])
+@pytest.mark.parametrize("gather", [False, True])
+def test_tiles_of_two_blocks(runtime, gated, n, k, out, gather):
+    """Rows enough for tiles of 256 rows: experts without rows, with one, with half a tile, with several."""
+    rng = np.random.default_rng(n + k)
+    counts = np.array([0, 3000, 1, 127, 128, 129, 0, 257, 5000, 300, 255, 0])
+    rows, experts, top_k = int(counts.sum()), len(counts), 2
+    offsets = np.r_[0, np.cumsum(counts)]
+    tokens = -(-rows // top_k) + 40  # some tokens without an expert
+    order = np.full(tokens * top_k, -1)
+    order[:rows] = rng.permutation(tokens * top_k)[:rows]
+    x, xf = bf16(rng, (tokens if gather else rows, k))
+    wide = 2 * n if gated else n
+    w, wf = bf16(rng, (experts, wide, k), k**-0.5)
+    bias = rng.standard_normal((experts, wide)).astype(np.float32)
+    kw = dict(gated=gated, activation="silu" if gated else "gelu_tanh", bias=bias)
+    plan = dict(order=order, top_k=top_k) if gather else {}
+    got = experts_linear(x, w, offsets, out_dtype=out, runtime=runtime, **kw, **plan)
+    some = np.unique(np.r_[0, offsets[1:] - 1, offsets[:-1], rng.integers(0, rows, 150)])
+    some = some[(some >= 0) & (some < rows)]
+    of = np.searchsorted(offsets, some, side="right") - 1
+    small = np.searchsorted(of, np.arange(experts + 1))
+    check(got[some], xf[order[some] // top_k if gather else some], wf, small, **kw)
+    assert not got[rows:].any()
+    for _ in range(3):
+        again = experts_linear(x, w, offsets, out_dtype=out, runtime=runtime, **kw, **plan)
+        assert np.array_equal(got, again)
+
+
 def device_call(runtime, dtype=torch.bfloat16, rows=37, n=24, k=40, experts=4, ldx=56, ldw=48, ldo=29,
                 offsets=(0, 9, 9, 30, 33), **kw):
     """A call whose x, w and out lie inside wider rows: (out, untouched mask, exact)."""
@@ -189,6 +220,37 @@ def test_streams_and_a_graph(runtime):
     assert torch.equal(out, want)
     del graph
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("rows,n", [(9000, 256), (100, 40)])
+@pytest.mark.parametrize("gather", [False, True])
+def test_wait_limit_is_reported_and_the_runtime_goes_on(runtime, rows, n, gather):
+    """A limit of one cycle runs out in the waits of either kernel; the next call is right again."""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    x = torch.randn(rows, 4096, generator=g, device="cuda").bfloat16()
+    w = torch.randn(2, n, 4096, generator=g, device="cuda").mul(2.0**-6).bfloat16()
+    cut = rows // 3
+    offsets = torch.tensor([0, cut, rows], dtype=torch.int32, device="cuda")
+    order = torch.arange(rows, dtype=torch.int32, device="cuda")
+    out = torch.zeros(rows, n, device="cuda").bfloat16()
+    want = torch.cat([x[:cut].double() @ w[0].double().t(), x[cut:].double() @ w[1].double().t()])
+    torch.cuda.synchronize()
+
+    def call():
+        runtime.experts_linear_device(
+            x.data_ptr(), w.data_ptr(), out.data_ptr(), offsets=offsets.data_ptr(), tokens=rows,
+            top_k=1, num_experts=2, n=n, k=4096, order=order.data_ptr() if gather else None)
+        runtime.sync()
+
+    runtime.set_wait_limit(1)
+    try:
+        with pytest.raises(DeviceTimeoutError):
+            call()
+    finally:
+        runtime.set_wait_limit(0)
+    call()
+    # bf16's 2^-8 of the value, and 4096 / 16 + 16 cut additions of 2^-23 of sums of about 64.
+    assert ((out.double() - want).abs() <= 2.0**-8 * want.abs() + 272 * 2.0**-23 * 64).all()
 
 
 def test_refusals(runtime):

@@ -147,6 +147,55 @@ def test_plans_of_many_tokens(runtime, tokens, experts, top_k):
     np.testing.assert_allclose(got.weights.sum(1), 1.0, rtol=2.0**-20)
 
 
+@pytest.mark.parametrize("tokens,experts,top_k,groups,top_groups,best", [
+    (6000, 256, 8, 8, 4, 2), (6000, 160, 6, 8, 3, 1), (5000, 60, 6, 4, 3, 1), (5000, 128, 8, 1, 1, 2),
+    (3000, 512, 8, 16, 5, 2), (4000, 64, 7, 1, 1, 2), (2000, 256, 12, 8, 4, 2)])
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("kind", ["fp32", "bf16 values", "bias"])
+def test_choices_of_many_tokens(runtime, tokens, experts, top_k, groups, top_groups, best, scores, kind):
+    """Enough tokens that some have neighbours, and sums of groups, next to one another."""
+    rng = np.random.default_rng(tokens + experts)
+    x = (1.5 * rng.standard_normal((tokens, experts))).astype(np.float32)
+    if kind == "bf16 values":
+        x = from_bf16_bits(to_bf16_bits(x))
+    bias = (0.1 * rng.standard_normal(experts)).astype(np.float32) if kind == "bias" else None
+    got = experts_route(x, top_k, scores=scores, bias=bias, groups=groups, top_groups=top_groups,
+                        group_best=best, runtime=runtime)
+    z = x.astype(np.float64)
+    if scores == "softmax":
+        s = np.exp(z - z.max(1, keepdims=True))
+        s /= s.sum(1, keepdims=True)
+    else:
+        s = 1 / (1 + np.exp(-z))
+    c = s if bias is None else s + bias
+    per = experts // groups
+    if groups > 1:
+        sums = np.sort(c.reshape(tokens, groups, per), axis=-1)[..., -best:].sum(-1)
+        kept = np.argsort(-sums, axis=1, kind="stable")[:, :top_groups]
+        mask = np.zeros((tokens, groups), bool)
+        np.put_along_axis(mask, kept, True, axis=1)
+        c = np.where(np.repeat(mask, per, axis=1), c, -np.inf)
+    want = np.argsort(-c, axis=1, kind="stable")[:, :top_k]
+    np.testing.assert_array_equal(got.experts, want)
+    w = np.take_along_axis(s, want, 1)
+    np.testing.assert_allclose(got.weights, w / w.sum(1, keepdims=True), rtol=2.0**-18)
+
+
+@pytest.mark.parametrize("experts", [20, 64, 128, 200, 400])
+def test_logits_an_ulp_apart(runtime, experts):
+    """fp32 logits of few values, each also an ulp up and down: equals, neighbours, and more candidates
+    for the last place than are put in order at once."""
+    rng = np.random.default_rng(experts)
+    base = np.float32(rng.standard_normal(6))
+    x = base[rng.integers(0, 6, (800, experts))]
+    step = rng.integers(-1, 2, x.shape)
+    x = np.where(step > 0, np.nextafter(x, np.float32(9)), np.where(step < 0, np.nextafter(
+        x, np.float32(-9)), x)).astype(np.float32)
+    for top_k in (1, 5, 8):
+        got = experts_route(x, top_k, runtime=runtime)
+        np.testing.assert_array_equal(got.experts, np.argsort(-x, axis=1, kind="stable")[:, :top_k])
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("ld,start", [(64, 0), (67, 1), (72, 8), (65, 3)])
 def test_row_strides_and_rows_behind(runtime, dtype, ld, start):
@@ -244,7 +293,7 @@ def test_refusals(runtime):
     plan = dict(offsets=p + 4096, order=p + 8192, places=p + 12288)
     runtime.experts_route_device(p, p + 16384, p + 32768, **ok, **plan)
     for kw in (dict(num_experts=0), dict(num_experts=1025), dict(top_k=0), dict(top_k=17),
-               dict(groups=3), dict(groups=0), dict(top_groups=2), dict(groups=4, top_groups=5),
+               dict(groups=3), dict(groups=0), dict(num_experts=128, groups=128), dict(top_groups=2), dict(groups=4, top_groups=5),
                dict(groups=8, top_groups=1, top_k=3), dict(groups=4, top_groups=2, group_best=3),
                dict(scores="other"), dict(scale=np.inf), dict(scale=np.nan), dict(ld=15),
                dict(logits_dtype=2), dict(lengths=p), dict(bias=p + 2), dict(order=None),
