@@ -10,8 +10,10 @@
 // gate columns and the same up columns side by side in tensor memory.
 // pair_kernel: 256 x 256 tiles by two CTAs, for calls of many rows.
 //
-// Measured: 65536 rows over 64 experts, gated, n 512, k 1024, gathered: 118 us, 1160 TFLOP/s (128 x 256
-// tiles: 121 us); n 1024, k 512, rows by expert: 68 us, 1010 TFLOP/s and 3.9 TB/s (78 us).
+// Measured: 65536 rows over 64 experts, gated, n 512, k 1024, gathered: 118 us from rest, 1160 TFLOP/s, and
+// 149 us in a loop under the power limit (128 x 256 tiles by one CTA: 121 from rest); n 1024, k 512, rows by
+// expert: 65 us, 1060 TFLOP/s and 4.1 TB/s, and 86 us in a loop (78 from rest).  Bound: the tensor pipe with
+// its power, 11 % more rows than there are in experts' last tiles, and for the latter the writes of out.
 #include <cuda.h>
 
 #include <algorithm>
@@ -61,6 +63,11 @@ enum : uint32_t { kOffTmem = 8 * kNumBars, kOffAbort = kOffTmem + 4 };
 static_assert(kOffAbort + 4 <= 512, "misc area");
 enum : int { kSiteEmpty = 1, kSiteFull = 2, kSiteAcc = 3, kSiteFree = 4 };
 
+__device__ __forceinline__ void pause_cycles(long long n) {
+  const long long t0 = clock64();
+  while (clock64() - t0 < n) {
+  }
+}
 // wait_bar by a whole warp, with one answer.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag,
                                           const ExpertsProblem &p, int site) {
@@ -575,6 +582,7 @@ enum : uint32_t { kFullBar = 0, kGathered = kStages, kEmpty = 2 * kStages, kAcc 
                   kFree = kAcc + 2, kDrain = kFree + 2, kBars = kDrain + 1 };
 static_assert(8 * kBars + 8 <= 512, "misc area");
 enum : int { kSiteGathered = 5 };
+constexpr long long kLandCycles = 1 << 20;  // 0.5 ms
 }  // namespace pair
 
 template <bool kGated, bool kGather>
@@ -654,6 +662,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGather ? kGatherThr
       for (uint32_t s = 0; s < (uint32_t)kStages && s < fills; ++s)
         drain_bar(bar(kFullBar + s), ((fills - 1 - s) / kStages) & 1, now);
     }
+    // The odd CTA's copies arrive at barriers that it cannot test.  Those in flight when a wait has ended get
+    // time to land.
+    if (!ok && rank == 1) pause_cycles(kLandCycles);
     __syncwarp();
   } else if (kGather && warp >= 10) {
     uint32_t fills = 0, e = 0;
@@ -822,8 +833,14 @@ cudaError_t launch_pairs(const ExpertsProblem &p, int num_sms, cudaStream_t stre
 template <bool kGated, bool kLong, bool kGather>
 cudaError_t launch_wide(const ExpertsProblem &p, int num_sms, cudaStream_t stream) {
   const uint32_t wide = p.n * (kGated ? 2 : 1);
+  // Tiles of two CTAs where an expert has 128 rows or more and there is work for them.  Against tiles of 128,
+  // gated, n 512, k 1024: 8192 rows over 8 experts 24.6 / 32.7 us, over 64 40.8 / 43.0; 4096 rows over 8
+  // 18.4 / 20.5, over 64 36.9 / 34.8; 2048 over 8 18.4 / 16.4; 65536 over 1024 432 / 420.  n 256, k 768, 16
+  // experts: 8192 rows 16.3 / 12.4, 16384 16.4 / 16.4, 65536 30.7 / 38.8.
   if constexpr (!kLong)
-    if (wide > 128 && p.rows > 128 * 64) return launch_pairs<kGated, kGather>(p, num_sms, stream);
+    if (wide > 128 && p.rows >= 128 * p.experts &&
+        (p.rows > 8192 || (uint64_t)p.rows * wide * p.k >= 1ull << 32))
+      return launch_pairs<kGated, kGather>(p, num_sms, stream);
   // 64 columns a tile where tiles of 128 would leave half the SMs without one (the expert ranges are not
   // known here: at most a tile for each row or expert, and one for every 128 rows): 18 / 12 us for 2 to 32
   // rows over 8 experts, n 768, k 768; but 27 / 35 us for 64 rows over 64 experts, gated, n 512, k 1024.

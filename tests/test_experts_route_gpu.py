@@ -118,6 +118,30 @@ def test_nan_ranks_below_every_number(runtime):
     assert np.isfinite(got.weights[0]).all() and np.isnan(got.weights[1, 1:]).all()
 
 
+@pytest.mark.parametrize("experts,top_k", [(16, 4), (40, 4), (64, 10), (640, 4)])
+def test_nan_among_softmax_scores(runtime, experts, top_k):
+    """One NaN logit leaves the choice among the others as it is without that expert."""
+    rng = np.random.default_rng(experts)
+    x = rng.standard_normal((9, experts)).astype(np.float32)
+    bias = rng.standard_normal(experts).astype(np.float32)
+    x[np.arange(9), rng.integers(0, experts, 9)] = np.nan
+    without = np.where(np.isnan(x), np.float32(-np.inf), x)
+    for kw in (dict(bias=bias), dict(groups=4, top_groups=2), dict(bias=bias, groups=8, top_groups=4)):
+        got = experts_route(x, top_k, runtime=runtime, **kw)
+        np.testing.assert_array_equal(got.experts, oracle.experts_route(without, top_k, **kw)[0])
+
+
+@pytest.mark.parametrize("experts,top_k", [(16, 4), (64, 8), (64, 12), (640, 16)])
+@pytest.mark.parametrize("level", [100.0, -800.0])
+def test_scores_without_a_bias_are_told_apart_by_their_logits(runtime, experts, top_k, level):
+    """Sigmoids that 64 bits do not tell apart, in groups of which all stay."""
+    rng = np.random.default_rng(experts)
+    x = np.float32(level) + rng.permuted(np.tile(np.arange(experts, dtype=np.float32), (7, 1)), axis=1) / 16
+    got = experts_route(x, top_k, scores="sigmoid", groups=4, top_groups=4, renormalise=False,
+                        runtime=runtime)
+    np.testing.assert_array_equal(got.experts, np.argsort(-x, axis=1, kind="stable")[:, :top_k])
+
+
 def test_far_logits(runtime):
     """Weights whose exponentials leave fp32's range unless a common factor is taken out."""
     x = np.float32([[-120, -121, -300, -119], [200, 199, 198, -200]])
