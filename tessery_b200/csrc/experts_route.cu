@@ -16,10 +16,11 @@
 // its rank among the warp's; place_kernel adds what lies before, of the warps and blocks before it.  A few
 // tokens are one block, which does both.
 //
-// Bound: instructions and their latency.  Measured: 65536 tokens of 128 bf16 logits, 8 of each, 28.7 us (HBM
-// would take 3.8); 16384 tokens of 256, 8 of each from 4 in 8 groups, with a bias, 35 us (2.9); 8 tokens of
-// 64, one launch, 8.2.  With a round for each chosen expert, in place of the lanes' eight largest together,
-// the first took 50 us, the second 48.
+// Bound: instructions and their latency.  Measured: 65536 tokens of 128 bf16 logits, 8 of each, 24.6 us (HBM
+// would take 3.8; 28.7 with place_kernel launched behind the runs and its pairs loaded behind the counts);
+// 16384 tokens of 256, 8 of each from 4 in 8 groups, with a bias, 31 us (2.9); 8 tokens of 64, one launch,
+// 8.2.  With a round for each chosen expert, in place of the lanes' eight largest together, the first took
+// 50 us, the second 48.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -607,6 +608,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
     __syncthreads();
   }
   __syncwarp();
+  asm volatile("griddepcontrol.launch_dependents;");
   uint32_t first, end;
   warp_tokens(p, blockIdx.x, warp, &first, &end);
   bool told = !kScored && p.logits_dtype == TX_BF16;
@@ -937,10 +939,23 @@ __global__ void __launch_bounds__(kPlaceThreads, 1)
     place_kernel(const __grid_constant__ RouteProblem p) {
   __shared__ uint32_t total[1024], base[1024], offset[1025], parts[32];
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, runs = gridDim.x;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // for the runs, see run_warps
+  const uint64_t first = min((uint64_t)blockIdx.x * p.run, (uint64_t)p.tokens) * p.top_k;
+  const uint64_t end = min((uint64_t)(blockIdx.x + 1) * p.run, (uint64_t)p.tokens) * p.top_k;
+  // The block's first pairs travel while the counts are summed.
+  constexpr int kHeld = 4;
+  int32_t held_e[kHeld], held_rank[kHeld];
+#pragma unroll
+  for (int h = 0; h < kHeld; ++h) {
+    const uint64_t i = first + threadIdx.x + h * kPlaceThreads;
+    held_e[h] = i < end ? __ldcg(p.chosen + i) : -1;
+    held_rank[h] = i < end ? __ldcg(p.places + i) : 0;
+  }
   // A warp sums the counts of an expert over the runs, and of those before this one; the loads of four
   // experts are on their way at once.
   for (uint32_t e0 = warp * 4; e0 < p.experts; e0 += kPlaceThreads / 8) {
     uint32_t all[4] = {}, before[4] = {};
+#pragma unroll 5
     for (uint32_t b = lane; b < runs; b += 32) {
 #pragma unroll
       for (uint32_t i = 0; i < 4; ++i) {
@@ -964,17 +979,18 @@ __global__ void __launch_bounds__(kPlaceThreads, 1)
     for (uint32_t e = threadIdx.x; e <= p.experts; e += kPlaceThreads) p.offsets[e] = (int32_t)offset[e];
   for (uint32_t e = threadIdx.x; e < p.experts; e += kPlaceThreads) base[e] += offset[e];
   __syncthreads();
-  const uint64_t first = min((uint64_t)blockIdx.x * p.run, (uint64_t)p.tokens) * p.top_k;
-  const uint64_t end = min((uint64_t)(blockIdx.x + 1) * p.run, (uint64_t)p.tokens) * p.top_k;
+  auto place = [&](uint64_t i, int32_t e, int32_t rank) {
+    if (e < 0) return;
+    const uint32_t at = base[e] + (uint32_t)rank;
+    p.places[i] = (int32_t)at;
+    p.order[at] = (int32_t)i;
+  };
+#pragma unroll
+  for (int h = 0; h < kHeld; ++h)
+    place(first + threadIdx.x + h * kPlaceThreads, held_e[h], held_rank[h]);
 #pragma unroll 4
-  for (uint64_t i = first + threadIdx.x; i < end; i += kPlaceThreads) {
-    const int32_t e = p.chosen[i], rank = p.places[i];
-    if (e >= 0) {
-      const uint32_t at = base[e] + (uint32_t)rank;
-      p.places[i] = (int32_t)at;
-      p.order[at] = (int32_t)i;
-    }
-  }
+  for (uint64_t i = first + threadIdx.x + kHeld * kPlaceThreads; i < end; i += kPlaceThreads)
+    place(i, p.chosen[i], p.places[i]);
 }
 
 template <int kLanes, int V, bool kScored, int kWarps, bool kTop8>
@@ -993,8 +1009,17 @@ cudaError_t run_warps(RouteProblem p, cudaStream_t stream) {
   if (e != cudaSuccess) return e;
   route_kernel<kLanes, V, kScored, kWarps, kTop8><<<p.blocks, 32 * kWarps, bytes, stream>>>(p);
   if ((e = cudaGetLastError()) != cudaSuccess || p.blocks == 1 || !p.order) return e;
-  place_kernel<<<p.blocks, kPlaceThreads, 0, stream>>>(p);
-  return cudaGetLastError();
+  // Launched while the runs finish (griddepcontrol), it waits for them on the device.
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(p.blocks);
+  config.blockDim = dim3(kPlaceThreads);
+  config.stream = stream;
+  cudaLaunchAttribute early = {};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &early;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, place_kernel, p);
 }
 // Few warps where a round of theirs takes all tokens: a block of 32 is slower to start and to add up (8 tokens
 // of 64 experts: 8.2 against 9.5 us).
