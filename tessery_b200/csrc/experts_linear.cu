@@ -87,17 +87,19 @@ __device__ __forceinline__ void copies_wait() {
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-// The rows that four warps gather for a tile.  Eight lanes copy a row's 128 bytes of a stage, a warp 32 rows
-// in eight steps, into the 128-byte swizzle.  A tile's entries of `order` are fetched while the tile before
+// The rows that kWarps warps gather for a tile.  Eight lanes copy a row's 128 bytes of a stage, four warps 32
+// rows each in eight steps, into the 128-byte swizzle.  A tile's entries of `order` are fetched while the tile before
 // it is copied: waiting for them at its start took 3400 cycles, more than the stages ahead last.
+template <uint32_t kWarps>
 struct Gather {
-  const uint16_t *from[8];
-  int32_t pair[8];
+  static constexpr uint32_t kEach = 32 / kWarps;  // rows of a thread
+  const uint16_t *from[kEach];
+  int32_t pair[kEach];
   uint32_t first, chunk, rows, next_rows;
-  // warp: 0 .. 3
+  // warp: 0 .. kWarps - 1
   __device__ __forceinline__ explicit Gather(uint32_t warp) {
     const uint32_t lane = threadIdx.x & 31;
-    first = warp * 32 + lane / 8;
+    first = warp * (128 / kWarps) + lane / 8;
     chunk = lane % 8;
     next_rows = 0;
   }
@@ -105,7 +107,7 @@ struct Gather {
   __device__ __forceinline__ void fetch(const ExpertsProblem &p, uint32_t r0, uint32_t tile_rows) {
     next_rows = tile_rows;
 #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i)
+    for (uint32_t i = 0; i < kEach; ++i)
       pair[i] = first + i * 4 < tile_rows ? __ldg(p.order + r0 + first + i * 4) : 0;
   }
   // Turns to the tile fetched last.
@@ -113,7 +115,7 @@ struct Gather {
     rows = next_rows;
     const uint16_t *x = static_cast<const uint16_t *>(p.x) + chunk * 8;
 #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) {
+    for (uint32_t i = 0; i < kEach; ++i) {
       // pair / top_k by the reciprocal floor(2^32 / top_k) + 1, which is one too much at most.
       uint32_t at = p.top_k > 1 ? __umulhi((uint32_t)pair[i], p.top_k_inv) : (uint32_t)pair[i];
       if (at * p.top_k > (uint32_t)pair[i]) --at;
@@ -129,7 +131,7 @@ struct Gather {
     const uint32_t col = kb * kBK + chunk * 8;
     const uint32_t bytes = col < p.k ? min((p.k - col) * 2, 16u) : 0;
 #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) {
+    for (uint32_t i = 0; i < kEach; ++i) {
       const uint32_t r = first + i * 4;
       if (r < rows)
         copy16(dst + r * 128 + ((chunk ^ (r & 7)) << 4), bytes ? from[i] + kb * kBK : from[i], bytes);
@@ -349,7 +351,25 @@ __device__ __forceinline__ void load_columns(uint32_t at, float (&v)[kStep]) {
   for (uint32_t t = 0; t < kStep; ++t) v[t] = __uint_as_float(a[t]);
 }
 
-// kLong: the sum is taken in parts of 512 K that are added in fp32 registers.
+template <uint32_t kStep>
+__device__ __forceinline__ void zero(float (&v)[kStep]) {
+#pragma unroll
+  for (uint32_t t = 0; t < kStep; ++t) v[t] = 0.f;
+}
+// v += the columns, eight at a time: sums hold most registers here.
+template <uint32_t kStep>
+__device__ __forceinline__ void add_columns(uint32_t at, float (&v)[kStep]) {
+#pragma unroll
+  for (uint32_t t = 0; t < kStep; t += 8) {
+    float a[8];
+    load_columns<8>(at + t, a);
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) v[t + i] += a[i];
+  }
+}
+
+// kLong: the sum is taken in parts of 512 K that are added in fp32 registers.  (Added from zero on: with the
+// first part taken as it is the compiler held them twice.)
 template <int kBN, bool kGated, bool kLong, bool kGather>
 __global__ void __launch_bounds__(kGather ? kGatherThreads : kThreads, 1)
     experts_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
@@ -429,7 +449,7 @@ __global__ void __launch_bounds__(kGather ? kGatherThreads : kThreads, 1)
   } else if (kGather && warp >= 10) {
     uint32_t fills = 0, e = 0;
     bool ok = true;
-    Gather rows((uint32_t)warp - 10);
+    Gather<4> rows((uint32_t)warp - 10);
     auto fetch = [&](uint32_t tile) {
       if (tile >= total) return;
       e = expert_of(tiles, p.experts, tile / nt, e);
@@ -506,7 +526,14 @@ __global__ void __launch_bounds__(kGather ? kGatherThreads : kThreads, 1)
       if constexpr (kLong) {
         constexpr uint32_t kHeld = kCols / kStep;
         float v[kHeld][kStep], u[kGated ? kHeld : 1][kGated ? kStep : 1];
+#pragma unroll
+        for (uint32_t c = 0; c < kHeld; ++c) zero(v[c]);
+        if constexpr (kGated) {
+#pragma unroll
+          for (uint32_t c = 0; c < kHeld; ++c) zero(u[c]);
+        }
         const uint32_t parts = (nk + kPart - 1) / kPart;
+#pragma unroll 1
         for (uint32_t part = 0; part < parts; ++part, ++done) {
           const uint32_t b = done & 1, t0 = tmem + b * kBN + half * kCols + lanes;
           if (!(ok = __all_sync(kFull, wait_bar(bar(kBarAcc + b), (done >> 1) & 1, abort_flag, p.status,
@@ -515,15 +542,8 @@ __global__ void __launch_bounds__(kGather ? kGatherThreads : kThreads, 1)
           tc_fence_after();
 #pragma unroll
           for (uint32_t c = 0; c < kHeld; ++c) {
-            float a[kStep];
-            load_columns<kStep>(t0 + c * kStep, a);
-#pragma unroll
-            for (uint32_t t = 0; t < kStep; ++t) v[c][t] = part ? v[c][t] + a[t] : a[t];
-            if constexpr (kGated) {
-              load_columns<kStep>(t0 + kOut + c * kStep, a);
-#pragma unroll
-              for (uint32_t t = 0; t < kStep; ++t) u[c][t] = part ? u[c][t] + a[t] : a[t];
-            }
+            add_columns(t0 + c * kStep, v[c]);
+            if constexpr (kGated) add_columns(t0 + kOut + c * kStep, u[c]);
           }
           tc_fence_before();
           mbar_arrive(bar(kBarFree + b));
@@ -567,14 +587,18 @@ __global__ void __launch_bounds__(kGather ? kGatherThreads : kThreads, 1)
 // holds 128 of the rows and 128 of the columns, so that a stage of 64 K takes 32 KB of shared memory a CTA
 // where the tiles above take 48 KB: with those the way from L2 into shared memory is the bound.
 namespace pair {
-constexpr int kStages = 6;
 constexpr uint32_t kHalfBytes = 128 * 128, kStageBytes = 2 * kHalfBytes;
 constexpr uint32_t kRows = 256, kWide = 256, kMaxExperts = 1024;
+constexpr int kStages = 6;
 constexpr uint32_t kOffStaging = kStages * kStageBytes;
 constexpr uint32_t kOffMisc = kOffStaging + 8 * (kBufBytes + kBiasBytes);
 constexpr uint32_t kOffTables = kOffMisc + 512;
 constexpr uint32_t kSmemBytes = kOffTables + 2 * (kMaxExperts + 1) * 4;
 static_assert(kSmemBytes <= 232448, "shared memory");
+// Warps that gather.  kLong: two, since each epilogue thread holds 128 sums and the others' registers are
+// those that it lacks (with four, sums went through local memory).
+template <bool kLong>
+constexpr uint32_t kGathering = kLong ? 2 : 4;
 constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | ((kWide >> 3) << 17) |
                             ((kRows >> 4) << 24);
 // kFull: of the even CTA, the copies of both (and the odd one's gathered rows); kGathered: this CTA's.
@@ -585,8 +609,9 @@ enum : int { kSiteGathered = 5 };
 constexpr long long kLandCycles = 1 << 20;  // 0.5 ms
 }  // namespace pair
 
-template <bool kGated, bool kGather>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGather ? kGatherThreads : kThreads, 1)
+template <bool kGated, bool kLong, bool kGather>
+__global__ void __cluster_dims__(2, 1, 1)
+    __launch_bounds__(kThreads + (kGather ? 32 * pair::kGathering<kLong> : 0), 1)
     pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                 const __grid_constant__ ExpertsProblem p) {
   using namespace pair;
@@ -605,7 +630,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGather ? kGatherThr
     prefetch_tmap(&tm_w);
     for (int s = 0; s < kStages; ++s) {
       mbar_init(bar(kFullBar + s), kGather ? 2 : 1);
-      mbar_init(bar(kGathered + s), 128);
+      mbar_init(bar(kGathered + s), 32 * kGathering<kLong>);
       mbar_init(bar(kEmpty + s), 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -669,7 +694,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGather ? kGatherThr
   } else if (kGather && warp >= 10) {
     uint32_t fills = 0, e = 0;
     bool ok = true;
-    Gather rows((uint32_t)warp - 10);
+    Gather<kGathering<kLong>> rows((uint32_t)warp - 10);
     auto fetch = [&](uint32_t tile) {
       if (tile >= total) return;
       e = expert_of(tiles, p.experts, tile / nt, e);
@@ -694,31 +719,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGather ? kGatherThr
     if (rank == 0) {
       uint32_t step = 0, done = 0;
       bool ok = true;
-      for (uint32_t tile = first_tile; ok && tile < total; tile += tile_step, ++done) {
-        const uint32_t b = done & 1, acc = tmem + b * kWide;
-        if (done >= 2 && !(ok = warp_wait(bar(kFree + b), ((done >> 1) - 1) & 1, abort_flag, p, kSiteFree)))
-          break;
-        tc_fence_after();
-        for (uint32_t kb = 0; kb < nk; ++kb, ++step) {
-          const uint32_t s = step % kStages, parity = (step / kStages) & 1;
-          if (!(ok = warp_wait(bar(kFullBar + s), parity, abort_flag, p, kSiteFull))) break;
-          if constexpr (kGather) {
-            if (!(ok = warp_wait(bar(kGathered + s), parity, abort_flag, p, kSiteGathered))) break;
-            fence_proxy_async();
-          }
+      for (uint32_t tile = first_tile; ok && tile < total; tile += tile_step) {
+        for (uint32_t kb = 0; ok && kb < nk; ++done) {
+          const uint32_t b = done & 1, acc = tmem + b * kWide;
+          if (done >= 2 &&
+              !(ok = warp_wait(bar(kFree + b), ((done >> 1) - 1) & 1, abort_flag, p, kSiteFree)))
+            break;
           tc_fence_after();
-          const uint32_t st = sbase + s * kStageBytes;
-          const uint64_t ad = sw128_desc(st, 16, 1024), bd = sw128_desc(st + kHalfBytes, 16, 1024);
-          if (elect_one()) {
+          const uint32_t end = kLong ? min(kb + kPart, nk) : nk;
+          for (uint32_t first = kb; kb < end; ++kb, ++step) {
+            const uint32_t s = step % kStages, parity = (step / kStages) & 1;
+            if (!(ok = warp_wait(bar(kFullBar + s), parity, abort_flag, p, kSiteFull))) break;
+            if constexpr (kGather) {
+              if (!(ok = warp_wait(bar(kGathered + s), parity, abort_flag, p, kSiteGathered))) break;
+              fence_proxy_async();
+            }
+            tc_fence_after();
+            const uint32_t st = sbase + s * kStageBytes;
+            const uint64_t ad = sw128_desc(st, 16, 1024), bd = sw128_desc(st + kHalfBytes, 16, 1024);
+            if (elect_one()) {
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks)
-              umma_pair(acc, ad + ks * 2, bd + ks * 2, kIdesc, kb > 0 || ks > 0);
-            umma_commit_pair(bar(kEmpty + s));
+              for (int ks = 0; ks < 4; ++ks)
+                umma_pair(acc, ad + ks * 2, bd + ks * 2, kIdesc, kb > first || ks > 0);
+              umma_commit_pair(bar(kEmpty + s));
+            }
+            __syncwarp();
           }
+          if (ok && elect_one()) umma_commit_pair(bar(kAcc + b));
           __syncwarp();
         }
-        if (ok && elect_one()) umma_commit_pair(bar(kAcc + b));
-        __syncwarp();
       }
       if (elect_one()) umma_commit_pair(bar(kDrain));
       __syncwarp();
@@ -747,6 +776,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGather ? kGatherThr
     static_assert(kCols * (kGated ? 8 : 4) <= kBiasBytes, "bias area");
     uint32_t done = 0, e = 0;
     bool ok = true;
+    auto wait_acc = [&] {
+      const bool is = __all_sync(kFull, wait_bar(bar(kAcc + (done & 1)), (done >> 1) & 1, abort_flag,
+                                                 p.status, kSiteAcc, p.wait_cycles));
+      tc_fence_after();
+      return is;
+    };
+    auto give_acc = [&] {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(cluster_addr(bar(kFree + (done & 1)), 0));
+      ++done;
+    };
     for (uint32_t tile = first_tile; ok && tile < total; tile += tile_step) {
       const uint32_t mt = tile / nt;
       e = expert_of(tiles, p.experts, mt, e);
@@ -754,25 +795,47 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGather ? kGatherThr
       const uint32_t n0 = tile % nt * kOut + half * kCols;
       const Finish f{r0, start[e + 1] > r0 ? min(start[e + 1] - r0, 32u) : 0, staging, bias};
       if (p.bias && f.rows) fetch_bias<kGated, kCols>(p, bias, e, n0);
-      const uint32_t b = done & 1, t0 = tmem + b * kWide + half * kCols + lanes;
-      ok = __all_sync(kFull, wait_bar(bar(kAcc + b), (done >> 1) & 1, abort_flag, p.status,
-                                              kSiteAcc, p.wait_cycles));
-      if (!ok) break;
-      tc_fence_after();
-      ++done;
-      if (f.rows) {
-#pragma unroll 1
-        for (uint32_t c = 0; c < kCols; c += kStep) {
-          float v[kStep], u[kGated ? kStep : 1];
-          load_columns<kStep>(t0 + c, v);
-          if constexpr (kGated) load_columns<kStep>(t0 + kOut + c, u);
-          finish_columns<kGated, kCols, kStep>(p, f, n0, c, v, u);
-          __syncwarp();
+      const uint32_t t0 = tmem + half * kCols + lanes;
+      if constexpr (kLong) {
+        constexpr uint32_t kHeld = kCols / kStep;
+        float v[kHeld][kStep], u[kGated ? kHeld : 1][kGated ? kStep : 1];
+#pragma unroll
+        for (uint32_t c = 0; c < kHeld; ++c) zero(v[c]);
+        if constexpr (kGated) {
+#pragma unroll
+          for (uint32_t c = 0; c < kHeld; ++c) zero(u[c]);
         }
+        const uint32_t parts = (nk + kPart - 1) / kPart;
+#pragma unroll 1
+        for (uint32_t i = 0; i < parts; ++i) {
+          if (!(ok = wait_acc())) break;
+          const uint32_t at = t0 + (done & 1) * kWide;
+#pragma unroll
+          for (uint32_t c = 0; c < kHeld; ++c) {
+            add_columns(at + c * kStep, v[c]);
+            if constexpr (kGated) add_columns(at + kOut + c * kStep, u[c]);
+          }
+          give_acc();
+        }
+        if (!ok) break;
+#pragma unroll
+        for (uint32_t c = 0; c < kHeld; ++c)
+          finish_columns<kGated, kCols, kStep>(p, f, n0, c * kStep, v[c], u[kGated ? c : 0]);
+      } else {
+        if (!(ok = wait_acc())) break;
+        const uint32_t at = t0 + (done & 1) * kWide;
+        if (f.rows) {
+#pragma unroll 1
+          for (uint32_t c = 0; c < kCols; c += kStep) {
+            float v[kStep], u[kGated ? kStep : 1];
+            load_columns<kStep>(at + c, v);
+            if constexpr (kGated) load_columns<kStep>(at + kOut + c, u);
+            finish_columns<kGated, kCols, kStep>(p, f, n0, c, v, u);
+            __syncwarp();
+          }
+        }
+        give_acc();
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(cluster_addr(bar(kFree + b), 0));
     }
   }
 
@@ -818,15 +881,16 @@ cudaError_t launch_tiles(const ExpertsProblem &p, int num_sms, cudaStream_t stre
   return cudaGetLastError();
 }
 
-template <bool kGated, bool kGather>
+template <bool kGated, bool kLong, bool kGather>
 cudaError_t launch_pairs(const ExpertsProblem &p, int num_sms, cudaStream_t stream) {
   CUtensorMap mx, mw;
   if (!make_maps(&mx, &mw, p, 128)) return cudaErrorInvalidValue;
   static std::atomic<uint64_t> seen{0};
-  cudaError_t e = allow_smem((const void *)pair_kernel<kGated, kGather>, (int)pair::kSmemBytes, seen);
+  cudaError_t e =
+      allow_smem((const void *)pair_kernel<kGated, kLong, kGather>, (int)pair::kSmemBytes, seen);
   if (e != cudaSuccess) return e;
-  pair_kernel<kGated, kGather><<<num_sms / 2 * 2, kGather ? kGatherThreads : kThreads, pair::kSmemBytes,
-                                 stream>>>(mx, mw, p);
+  const uint32_t threads = kThreads + (kGather ? 32 * pair::kGathering<kLong> : 0);
+  pair_kernel<kGated, kLong, kGather><<<num_sms / 2 * 2, threads, pair::kSmemBytes, stream>>>(mx, mw, p);
   return cudaGetLastError();
 }
 
@@ -836,11 +900,13 @@ cudaError_t launch_wide(const ExpertsProblem &p, int num_sms, cudaStream_t strea
   // Tiles of two CTAs where an expert has 128 rows or more and there is work for them.  Against tiles of 128,
   // gated, n 512, k 1024: 8192 rows over 8 experts 24.6 / 32.7 us, over 64 40.8 / 43.0; 4096 rows over 8
   // 18.4 / 20.5, over 64 36.9 / 34.8; 2048 over 8 18.4 / 16.4; 65536 over 1024 432 / 420.  n 256, k 768, 16
-  // experts: 8192 rows 16.3 / 12.4, 16384 16.4 / 16.4, 65536 30.7 / 38.8.
-  if constexpr (!kLong)
-    if (wide > 128 && p.rows >= 128 * p.experts &&
-        (p.rows > 8192 || (uint64_t)p.rows * wide * p.k >= 1ull << 32))
-      return launch_pairs<kGated, kGather>(p, num_sms, stream);
+  // experts: 8192 rows 16.3 / 12.4, 16384 16.4 / 16.4, 65536 30.7 / 38.8.  In partial sums the tile's own end
+  // is longer, n 1024: 16384 rows over 8 experts, k 1024 47 / 49, 8192 rows 33 / 31, k 2048 43 / 49; 65536 over
+  // 64, k 1024 135 / 162, k 576 127 / 115.
+  const uint64_t work = (uint64_t)p.rows * wide * p.k;
+  const bool pairs = kLong ? p.k >= 1024 && work >= 1ull << 34 : p.rows > 8192 || work >= 1ull << 32;
+  if (wide > 128 && p.rows >= 128 * p.experts && pairs)
+    return launch_pairs<kGated, kLong, kGather>(p, num_sms, stream);
   // 64 columns a tile where tiles of 128 would leave half the SMs without one (the expert ranges are not
   // known here: at most a tile for each row or expert, and one for every 128 rows): 18 / 12 us for 2 to 32
   // rows over 8 experts, n 768, k 768; but 27 / 35 us for 64 rows over 64 experts, gated, n 512, k 1024.

@@ -305,6 +305,14 @@ __device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[16]) {
                : "r"(taddr)
                : "memory");
 }
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+      : "r"(taddr)
+      : "memory");
+}
 __device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[1]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x1.b32 {"

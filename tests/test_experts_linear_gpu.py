@@ -105,7 +105,8 @@ def test_long_sums_and_several_tiles(runtime, rows, experts, n, k, gated, out):
 
 @pytest.mark.parametrize("gated,n,k,out", [(True, 150, 200, "bf16"), (True, 128, 64, "float32"),
                                            (False, 300, 72, "bf16"), (False, 257, 513, "bf16"),
-                                           (False, 512, 130, "float32")])
+                                           (False, 512, 130, "float32"), (False, 1000, 2056, "float32"),
+                                           (True, 520, 2056, "float32")])
 @pytest.mark.parametrize("gather", [False, True])
 def test_tiles_of_two_blocks(runtime, gated, n, k, out, gather):
     """Rows enough for tiles of 256 rows: experts without rows, with one, with half a tile, with several."""
