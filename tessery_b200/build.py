@@ -55,6 +55,7 @@ def build(verbose: bool = False, force: bool = False) -> Path:
         "-lineinfo",
         "-O3",
         "-std=c++17",
+        "--threads=0",  # sources side by side
         "-Xcompiler",
         "-fPIC,-O3",
         "-shared",
