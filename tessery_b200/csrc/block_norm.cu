@@ -398,10 +398,16 @@ cudaError_t run_fours(const BlockNormProblem &p, int num_sms, cudaStream_t strea
   if (warps <= 16) return run<Any, Any, 8, 4, 2>(p, num_sms, stream);
   return run<Any, Any, 16, 4, 8>(p, num_sms, stream);
 }
+// Rows that start anywhere, element by element, eight a thread where 16 warps hold them: bound by instructions
+// and waits (8192 rows of 1023 take 72 us, of 1024 21).  Half as many warps as the next width wants: 33500 rows
+// of 383 110 us with two warps, 144 with four; 2000 rows of 5001 with 16 elements a thread 174, with 32 312.
 cudaError_t run_ones(const BlockNormProblem &p, int num_sms, cudaStream_t stream) {
   if (p.cols <= 32 * 8) return run<Any, Any, 1, 1, 8>(p, num_sms, stream);
+  if (p.cols <= 64 * 8) return run<Any, Any, 2, 1, 8>(p, num_sms, stream);
   if (p.cols <= 128 * 8) return run<Any, Any, 4, 1, 8>(p, num_sms, stream);
+  if (p.cols <= 256 * 8) return run<Any, Any, 8, 1, 8>(p, num_sms, stream);
   if (p.cols <= 512 * 8) return run<Any, Any, 16, 1, 8>(p, num_sms, stream);
+  if (p.cols <= 512 * 16) return run<Any, Any, 16, 1, 16>(p, num_sms, stream);
   return run<Any, Any, 16, 1, 32>(p, num_sms, stream);
 }
 

@@ -117,7 +117,8 @@ def test_joined_rows(runtime, cols, top_k, dtype):
 
 
 @pytest.mark.parametrize("rows,cols", [(9000, 72), (9000, 50), (5000, 264), (3000, 600), (2500, 1024),
-                                       (2500, 1030), (700, 4096), (400, 9000)])
+                                       (2500, 1030), (700, 4096), (400, 9000), (3000, 383),
+                                       (1500, 2001), (500, 5001)])
 def test_many_rows(runtime, rows, cols):
     """More rows than are in work at once, plain and joined."""
     rng = np.random.default_rng(rows)
