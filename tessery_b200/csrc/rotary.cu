@@ -99,7 +99,8 @@ __device__ __forceinline__ float axis_position(const RotaryProblem &p, uint32_t 
 // (interleaved).  kLanes lanes cover a head with kSlots slots each, so a warp takes
 // 32 / kLanes heads at a time; one warp per token, so the sines and cosines of a lane's slots
 // serve every head of the token.
-// kAxes: a pair turns by its own axis' position of the token.
+// kAxes: a pair turns by its own axis' position of the token (65536 tokens with norms, 16 + 8 heads of 128 inside
+// fused rows, three axes: 156 us, 5.2 TB/s; with one position for all pairs 151).
 template <typename TI, typename TO, int V, int kLanes, int kSlots, bool kAxes>
 __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ RotaryProblem p) {
   constexpr uint32_t kHeads = 32 / kLanes;  // heads per step of a warp
