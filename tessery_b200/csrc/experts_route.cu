@@ -129,13 +129,21 @@ __device__ __forceinline__ float score_tolerance(bool softmax, float inv_sum) {
   return softmax ? (float)((V + 16) * 1.1920929e-7f) * inv_sum : 7.2e-7f;
 }
 
+// A group's sum is off by the rounding of both its terms, 2^-24 of each (s + bias) however little of them the
+// sum leaves, and of itself, besides what the scores are off by.  So two sums are told apart beyond 3 of the
+// scores' tolerances and 4 roundings of the larger terms: kSumRoundings of |best| + |second|.
+constexpr float kSumRoundings = 2.4e-7f;
+__device__ __forceinline__ float terms_of(float best, float second, bool both) {
+  return fabsf(best) + (both ? fabsf(second) : 0.f);
+}
+
 // keep_groups for groups that cut through lanes: one after the other over all lanes.
 template <int kLanes, int V>
 __device__ __noinline__ uint32_t keep_any_groups(const RouteProblem &p, uint32_t sub, uint32_t slot,
                                                  const float (&c)[V], float tol, bool *near) {
   const float none = -INFINITY;
   const uint32_t per = p.experts / p.groups;
-  auto sum_of = [&](uint32_t g) {
+  auto sum_of = [&](uint32_t g, float *terms) {
     float a = none, b = none;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -150,11 +158,13 @@ __device__ __noinline__ uint32_t keep_any_groups(const RouteProblem &p, uint32_t
       b = fmaxf(fminf(a, x), fmaxf(b, y));
       a = fmaxf(a, x);
     }
-    return p.group_best > 1 && b > none ? a + b : a;
+    const bool both = p.group_best > 1 && b > none;
+    *terms = terms_of(a, b, both);
+    return both ? a + b : a;
   };
   // The lane keeps the sums of groups sub, sub + kLanes, ...: 64 groups at most.
   constexpr int kSums = 64 / kLanes;
-  float sums[kSums];
+  float sums[kSums], size[kSums];
   uint32_t before[kSums];
 #pragma unroll
   for (int m = 0; m < kSums; ++m) {
@@ -162,10 +172,14 @@ __device__ __noinline__ uint32_t keep_any_groups(const RouteProblem &p, uint32_t
     before[m] = 0;
   }
   for (uint32_t g = 0; g < p.groups; ++g) {
-    const float s = sum_of(g);
+    float terms;
+    const float s = sum_of(g, &terms);
 #pragma unroll
     for (int m = 0; m < kSums; ++m)
-      if (g == sub + m * kLanes) sums[m] = s;
+      if (g == sub + m * kLanes) {
+        sums[m] = s;
+        size[m] = terms;
+      }
   }
   for (uint32_t h = 0; h < p.groups; ++h) {
     float other = none;
@@ -178,31 +192,33 @@ __device__ __noinline__ uint32_t keep_any_groups(const RouteProblem &p, uint32_t
       before[m] += other > sums[m] || (other == sums[m] && h < sub + m * kLanes);
   }
   uint32_t mask = 0;
-  float low = INFINITY, high = none;  // the lowest sum kept, the highest left out
+  // What the lowest sum kept may come down to, and the highest left out up to.
+  float low = INFINITY, high = none;
   for (uint32_t g = 0; g < p.groups; ++g) {
-    float s = none;
+    float s = none, off = 0.f;
     uint32_t n = 0;
 #pragma unroll
     for (int m = 0; m < kSums; ++m)
       if (g / kLanes == m) {
         s = sums[m];
+        off = size[m] * (0.5f * kSumRoundings);
         n = before[m];
       }
     s = __shfl_sync(kFull, s, slot * kLanes + g % kLanes);
+    off = __shfl_sync(kFull, off, slot * kLanes + g % kLanes);
     n = __shfl_sync(kFull, n, slot * kLanes + g % kLanes);
     if (n < p.top_groups) {
-      low = fminf(low, s);
+      low = fminf(low, s - off);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const uint32_t e = sub * p.per_lane + i;
         if (e >= g * per && e < (g + 1) * per) mask |= 1u << i;
       }
-    } else {
-      high = fmaxf(high, s);
+    } else if (s > none) {
+      high = fmaxf(high, s + off);
     }
   }
-  if (high > none)
-    *near |= low - high <= 3.f * tol + fabsf(low) * 2.4e-7f;
+  if (high > none) *near |= !(low - high > 3.f * tol);
   return mask;
 }
 // Whether the lane's experts lie in a group that stays, bit i for its i-th; c[i] is -inf where closed or
@@ -232,14 +248,17 @@ __device__ __forceinline__ uint32_t keep_groups(const RouteProblem &p, uint32_t 
       second = fmaxf(fminf(best, x), fmaxf(second, y));
       best = fmaxf(best, x);
     }
-    const float sum = p.group_best > 1 && second > none ? best + second : best;
-    const float close = 3.f * tol + fabsf(sum) * 2.4e-7f;
+    const bool both = p.group_best > 1 && second > none;
+    const float sum = both ? best + second : best;
+    // (Of two groups the one with the larger terms sees the other.)
+    const float close = 3.f * tol + terms_of(best, second, both) * kSumRoundings;
+    auto near_to = [&](float other) { return !(fabsf(other - sum) > close); };
     uint32_t before = 0;
     bool touch = false;
     for (uint32_t h = 0; h < p.groups; ++h) {
       const float other = __shfl_sync(kFull, sum, slot * kLanes + h * p.group_lanes);
       before += other > sum || (other == sum && h < g);
-      touch |= h != g && other <= sum + close && other >= sum - close;
+      touch |= h != g && near_to(other);
     }
     bool kept = before < p.top_groups;
     if (__any_sync(kFull, touch && g < p.groups && sum > none)) {
@@ -247,8 +266,7 @@ __device__ __forceinline__ uint32_t keep_groups(const RouteProblem &p, uint32_t 
       for (uint32_t h = 0; h < p.groups; ++h) {
         const float other = __shfl_sync(kFull, sum, slot * kLanes + h * p.group_lanes);
         const bool stays = __shfl_sync(kFull, (int)kept, slot * kLanes + h * p.group_lanes);
-        doubt |= g < p.groups && sum > none && stays != kept && other <= sum + close &&
-                 other >= sum - close;
+        doubt |= g < p.groups && sum > none && stays != kept && near_to(other);
       }
       if (p.softmax && p.bias) {
         *near |= doubt;  // the scores' sum is needed in 64 bits

@@ -1,0 +1,55 @@
+"""Routing of tokens to experts on a B200 where its choice or its weights hang on what fp32 does not
+hold: groups whose sums cancel, experts closed by their bias, groups far below the largest logit.
+Experts have to be equal to those of the formula in 64 bits; weights to 2^-18 of the value, as in
+test_experts_route_gpu.py (two logits at most 24 apart: their difference is off by 2^-20)."""
+
+import numpy as np
+import pytest
+
+from oracle import layers as oracle
+from tessery_b200.layers import experts_route
+
+pytestmark = pytest.mark.gpu
+
+
+def scores_of(x, scores):
+    x = x.astype(np.float64)
+    if scores == "sigmoid":
+        return 1 / (1 + np.exp(-x))
+    s = np.exp(x - x.max(-1, keepdims=True))
+    return s / s.sum(-1, keepdims=True)
+
+
+def best_of_groups(c, groups):
+    """The sum of the best two of each group."""
+    return np.sort(c.reshape(groups, -1), axis=1)[:, -2:].sum(1)
+
+
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("size", [2.0, 40.0, 1000.0])
+@pytest.mark.parametrize("experts,groups,top_groups,top_k", [
+    (64, 8, 4, 8), (128, 8, 3, 6), (128, 32, 9, 8), (256, 8, 4, 8), (256, 64, 20, 8), (60, 4, 2, 5),
+    (256, 8, 4, 12), (1024, 16, 5, 8)])
+def test_groups_whose_sums_cancel(runtime, scores, size, experts, groups, top_groups, top_k):
+    """The best two of every group lie near `size` and -`size`, and one bias brings the first group
+    that is left out next to the last one that stays: their sums are told apart by what the rounding
+    of each term to fp32 takes away."""
+    rng = np.random.default_rng(experts + groups + top_k)
+    per, close = experts // groups, 0
+    for _ in range(50):
+        x = rng.standard_normal((1, experts)).astype(np.float32)
+        s = scores_of(x[0], scores)
+        bias = np.full(experts, -3 * size, np.float32)
+        pairs = np.array([g * per + rng.permutation(per)[:2] for g in range(groups)])
+        bias[pairs[:, 0]] = size * rng.uniform(0.97, 1.03, groups)
+        bias[pairs[:, 1]] = -size * rng.uniform(0.97, 1.03, groups)
+        sums = best_of_groups(s + bias, groups)
+        by = np.argsort(-sums, kind="stable")
+        stays, leaves = by[top_groups - 1], by[top_groups]
+        bias[pairs[leaves, 1]] += sums[stays] - sums[leaves]
+        sums = best_of_groups(s + bias, groups)
+        close += abs(sums[stays] - sums[leaves]) <= size * 2.0**-23
+        kw = dict(scores=scores, bias=bias, groups=groups, top_groups=top_groups)
+        got = experts_route(x, top_k, runtime=runtime, **kw)
+        np.testing.assert_array_equal(got.experts, oracle.experts_route(x, top_k, **kw)[0])
+    assert close > 40
