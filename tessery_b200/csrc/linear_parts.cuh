@@ -50,7 +50,8 @@ __device__ __forceinline__ float rcp(float x) {
   return y;
 }
 
-// TX_ACT_GELU for fp32 results: a kernel of its own.
+// TX_ACT_GELU for fp32 results, and where the value is multiplied (gated products): a kernel of its own, or
+// chosen as the tile ends.
 constexpr int kGeluF32 = TX_ACT_SILU + 1;
 
 // The hardware exponential and reciprocal (2^-22 of the value each) in place of exp and a
