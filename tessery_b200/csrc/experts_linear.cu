@@ -4,16 +4,17 @@
 //
 // 128 x BN tiles on tcgen05 as in linear_fused.cu: one tile is up to 128 rows of one expert, and with the
 // ranges known on the device alone each CTA counts the tiles of every expert first.  Rows of x that do not
-// lie by expert are gathered by four warps with 16-byte asynchronous copies into the layout that TMA
+// lie by expert are gathered by two or four warps with 16-byte asynchronous copies into the layout that TMA
 // writes, so nothing is sorted into memory first.  (TMA gathers of four rows took 80 cycles each, 2600 a
 // stage where the products take 512: 336 against 138 us for the largest case.)  A gated tile holds BN / 2
 // gate columns and the same up columns side by side in tensor memory.
-// pair_kernel: 256 x 256 tiles by two CTAs, for calls of many rows.
+// pair_kernel: 256 x 256 tiles by two CTAs, for calls of many rows that lie by expert.  Gathered rows would
+// have to be handed from one CTA's threads to the other's products, with an arrival that waits for all copies
+// in flight: 244 us where 128 x 256 tiles by one CTA take 117.
 //
-// Measured: 65536 rows over 64 experts, gated, n 512, k 1024, gathered: 118 us from rest, 1160 TFLOP/s, and
-// 149 us in a loop under the power limit (128 x 256 tiles by one CTA: 121 from rest); n 1024, k 512, rows by
-// expert: 65 us, 1060 TFLOP/s and 4.1 TB/s, and 86 us in a loop (78 from rest).  Bound: the tensor pipe with
-// its power, 11 % more rows than there are in experts' last tiles, and for the latter the writes of out.
+// Measured: 65536 rows over 64 experts, gated, n 512, k 1024, gathered: 117 us from rest, 1175 TFLOP/s, and
+// 142 us in a loop under the power limit; n 1024, k 512, rows by expert: 64 us, 1080 TFLOP/s and 4.2 TB/s, and
+// 83 to 87 us in a loop.  Bound: the tensor pipe with its power, and for the latter the writes of out.
 #include <cuda.h>
 
 #include <algorithm>
@@ -32,8 +33,8 @@ using namespace lfused;
 
 constexpr int kBM = 128;
 constexpr uint32_t kBK = 64;
-// warp 0 TMA, warp 1 MMA, warps 2-9 epilogue, and to gather rows warps 10-13
-constexpr int kThreads = 320, kGatherThreads = 448;
+// warp 0 TMA, warp 1 MMA, warps 2-9 epilogue, and to gather rows those from warp 10 on
+constexpr int kThreads = 320;
 constexpr int kMaxStages = 8;
 constexpr uint32_t kPart = 8;  // K stages (512 columns) of one partial sum
 constexpr uint32_t kBufBytes = 32 * 64;  // staging of an epilogue warp: 32 rows of 64 bytes
@@ -69,9 +70,10 @@ __device__ __forceinline__ void pause_cycles(long long n) {
   }
 }
 // wait_bar by a whole warp, with one answer.
+template <bool kCluster = false>
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag,
                                           const ExpertsProblem &p, int site) {
-  return __all_sync(kFull, wait_bar(bar, parity, abort_flag, p.status, site, p.wait_cycles));
+  return __all_sync(kFull, wait_bar<kCluster>(bar, parity, abort_flag, p.status, site, p.wait_cycles));
 }
 // 16 bytes from global to shared memory, of which the first `bytes` are read and the others zeros.
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, uint32_t bytes) {
@@ -370,12 +372,17 @@ __device__ __forceinline__ void add_columns(uint32_t at, float (&v)[kStep]) {
 
 // kLong: the sum is taken in parts of 512 K that are added in fp32 registers.  (Added from zero on: with the
 // first part taken as it is the compiler held them twice.)
+// Two warps gather where each epilogue thread holds 128 sums and the others' registers are those that it lacks
+// (with four, sums went through local memory), otherwise four.
+template <int kBN, bool kLong>
+constexpr uint32_t kGathering = kLong && kBN == 256 ? 2 : 4;
 template <int kBN, bool kGated, bool kLong, bool kGather>
-__global__ void __launch_bounds__(kGather ? kGatherThreads : kThreads, 1)
+__global__ void __launch_bounds__(kThreads + (kGather ? 32 * kGathering<kBN, kLong> : 0), 1)
     experts_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                    const __grid_constant__ ExpertsProblem p) {
   using C = Cfg<kBN>;
   constexpr uint32_t kOut = kGated ? kBN / 2 : kBN;  // output columns of a tile
+  constexpr uint32_t kGathers = kGathering<kBN, kLong>;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sbase = smem_addr(smem), bars = sbase + C::kOffMisc;
   auto bar = [&](uint32_t i) { return bars + 8u * i; };
@@ -388,7 +395,7 @@ __global__ void __launch_bounds__(kGather ? kGatherThreads : kThreads, 1)
     prefetch_tmap(&tm_x);
     prefetch_tmap(&tm_w);
     for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(bar(kBarFull + s), kGather ? 129 : 1);  // the TMA copies, and each gathering thread
+      mbar_init(bar(kBarFull + s), kGather ? 1 + 32 * kGathers : 1);  // the TMA copies, and each gathering thread
       mbar_init(bar(kBarEmpty + s), 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -449,7 +456,7 @@ __global__ void __launch_bounds__(kGather ? kGatherThreads : kThreads, 1)
   } else if (kGather && warp >= 10) {
     uint32_t fills = 0, e = 0;
     bool ok = true;
-    Gather<4> rows((uint32_t)warp - 10);
+    Gather<kGathers> rows((uint32_t)warp - 10);
     auto fetch = [&](uint32_t tile) {
       if (tile >= total) return;
       e = expert_of(tiles, p.experts, tile / nt, e);
@@ -585,7 +592,8 @@ __global__ void __launch_bounds__(kGather ? kGatherThreads : kThreads, 1)
 // ---- two CTAs a tile ------------------------------------------------------------------------
 // 256 rows x 256 columns of products a tile, by the two CTAs of a cluster (cta_group::2): each brings and
 // holds 128 of the rows and 128 of the columns, so that a stage of 64 K takes 32 KB of shared memory a CTA
-// where the tiles above take 48 KB: with those the way from L2 into shared memory is the bound.
+// where 128 x 256 tiles take 48 KB.  Between the two CTAs go copies by TMA and products alone, which complete
+// at barriers, and tensor memory handed back between its fences.
 namespace pair {
 constexpr uint32_t kHalfBytes = 128 * 128, kStageBytes = 2 * kHalfBytes;
 constexpr uint32_t kRows = 256, kWide = 256, kMaxExperts = 1024;
@@ -595,23 +603,17 @@ constexpr uint32_t kOffMisc = kOffStaging + 8 * (kBufBytes + kBiasBytes);
 constexpr uint32_t kOffTables = kOffMisc + 512;
 constexpr uint32_t kSmemBytes = kOffTables + 2 * (kMaxExperts + 1) * 4;
 static_assert(kSmemBytes <= 232448, "shared memory");
-// Warps that gather.  kLong: two, since each epilogue thread holds 128 sums and the others' registers are
-// those that it lacks (with four, sums went through local memory).
-template <bool kLong>
-constexpr uint32_t kGathering = kLong ? 2 : 4;
 constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | ((kWide >> 3) << 17) |
                             ((kRows >> 4) << 24);
-// kFull: of the even CTA, the copies of both (and the odd one's gathered rows); kGathered: this CTA's.
-enum : uint32_t { kFullBar = 0, kGathered = kStages, kEmpty = 2 * kStages, kAcc = 3 * kStages,
-                  kFree = kAcc + 2, kDrain = kFree + 2, kBars = kDrain + 1 };
+// kFullBar: of the even CTA, the copies of both.
+enum : uint32_t { kFullBar = 0, kEmpty = kStages, kAcc = 2 * kStages, kFree = kAcc + 2,
+                  kDrain = kFree + 2, kBars = kDrain + 1 };
 static_assert(8 * kBars + 8 <= 512, "misc area");
-enum : int { kSiteGathered = 5 };
 constexpr long long kLandCycles = 1 << 20;  // 0.5 ms
 }  // namespace pair
 
-template <bool kGated, bool kLong, bool kGather>
-__global__ void __cluster_dims__(2, 1, 1)
-    __launch_bounds__(kThreads + (kGather ? 32 * pair::kGathering<kLong> : 0), 1)
+template <bool kGated, bool kLong>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                 const __grid_constant__ ExpertsProblem p) {
   using namespace pair;
@@ -629,8 +631,7 @@ __global__ void __cluster_dims__(2, 1, 1)
     prefetch_tmap(&tm_x);
     prefetch_tmap(&tm_w);
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(bar(kFullBar + s), kGather ? 2 : 1);
-      mbar_init(bar(kGathered + s), 32 * kGathering<kLong>);
+      mbar_init(bar(kFullBar + s), 1);
       mbar_init(bar(kEmpty + s), 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -659,7 +660,7 @@ __global__ void __cluster_dims__(2, 1, 1)
   auto full_at_even = [&](uint32_t s) { return cluster_addr(bar(kFullBar + s), 0); };
 
   if (warp == 0) {
-    // This CTA's rows (unless gathered) and columns of every stage.
+    // This CTA's rows and columns of every stage.
     uint32_t fills = 0, e = 0;
     bool ok = true;
     for (uint32_t tile = first_tile; ok && tile < total; tile += tile_step) {
@@ -669,12 +670,12 @@ __global__ void __cluster_dims__(2, 1, 1)
       const int n0 = (int)(tile % nt * kOut + rank * (kGated ? p.n : 128));
       for (uint32_t kb = 0; kb < nk; ++kb) {
         const uint32_t s = fills % kStages, round = fills / kStages;
-        if (round && !(ok = warp_wait(bar(kEmpty + s), (round - 1) & 1, abort_flag, p, kSiteEmpty)))
+        if (round && !(ok = warp_wait<true>(bar(kEmpty + s), (round - 1) & 1, abort_flag, p, kSiteEmpty)))
           break;
         const uint32_t dst = sbase + s * kStageBytes, full = full_at_even(s);
         if (elect_one()) {
-          if (rank == 0) mbar_expect_tx(bar(kFullBar + s), (kGather ? 2 : 4) * kHalfBytes);
-          if constexpr (!kGather) tma_load_2d_pair(dst, &tm_x, full, (int)(kb * kBK), r0);
+          if (rank == 0) mbar_expect_tx(bar(kFullBar + s), 4 * kHalfBytes);
+          tma_load_2d_pair(dst, &tm_x, full, (int)(kb * kBK), r0);
           tma_load_3d_pair(dst + kHalfBytes, &tm_w, full, (int)(kb * kBK), n0, (int)e);
         }
         __syncwarp();
@@ -685,36 +686,12 @@ __global__ void __cluster_dims__(2, 1, 1)
     if (lane == 0 && rank == 0) {
       const long long now = clock64();
       for (uint32_t s = 0; s < (uint32_t)kStages && s < fills; ++s)
-        drain_bar(bar(kFullBar + s), ((fills - 1 - s) / kStages) & 1, now);
+        drain_bar<true>(bar(kFullBar + s), ((fills - 1 - s) / kStages) & 1, now);
     }
     // The odd CTA's copies arrive at barriers that it cannot test.  Those in flight when a wait has ended get
     // time to land.
     if (!ok && rank == 1) pause_cycles(kLandCycles);
     __syncwarp();
-  } else if (kGather && warp >= 10) {
-    uint32_t fills = 0, e = 0;
-    bool ok = true;
-    Gather<kGathering<kLong>> rows((uint32_t)warp - 10);
-    auto fetch = [&](uint32_t tile) {
-      if (tile >= total) return;
-      e = expert_of(tiles, p.experts, tile / nt, e);
-      const uint32_t r0 = start[e] + (tile / nt - tiles[e]) * kRows + rank * 128;
-      rows.fetch(p, r0, start[e + 1] > r0 ? min(start[e + 1] - r0, 128u) : 0);
-    };
-    fetch(first_tile);
-    for (uint32_t tile = first_tile; ok && tile < total; tile += tile_step) {
-      rows.turn(p);
-      fetch(tile + tile_step);
-      for (uint32_t kb = 0; kb < nk; ++kb) {
-        const uint32_t s = fills % kStages, round = fills / kStages;
-        if (round && !(ok = warp_wait(bar(kEmpty + s), (round - 1) & 1, abort_flag, p, kSiteEmpty)))
-          break;
-        rows.stage(p, sbase + s * kStageBytes, kb);
-        copies_arrive(bar(kGathered + s));
-        ++fills;
-      }
-    }
-    copies_wait();
   } else if (warp == 1) {
     if (rank == 0) {
       uint32_t step = 0, done = 0;
@@ -723,17 +700,13 @@ __global__ void __cluster_dims__(2, 1, 1)
         for (uint32_t kb = 0; ok && kb < nk; ++done) {
           const uint32_t b = done & 1, acc = tmem + b * kWide;
           if (done >= 2 &&
-              !(ok = warp_wait(bar(kFree + b), ((done >> 1) - 1) & 1, abort_flag, p, kSiteFree)))
+              !(ok = warp_wait<true>(bar(kFree + b), ((done >> 1) - 1) & 1, abort_flag, p, kSiteFree)))
             break;
           tc_fence_after();
           const uint32_t end = kLong ? min(kb + kPart, nk) : nk;
           for (uint32_t first = kb; kb < end; ++kb, ++step) {
             const uint32_t s = step % kStages, parity = (step / kStages) & 1;
-            if (!(ok = warp_wait(bar(kFullBar + s), parity, abort_flag, p, kSiteFull))) break;
-            if constexpr (kGather) {
-              if (!(ok = warp_wait(bar(kGathered + s), parity, abort_flag, p, kSiteGathered))) break;
-              fence_proxy_async();
-            }
+            if (!(ok = warp_wait<true>(bar(kFullBar + s), parity, abort_flag, p, kSiteFull))) break;
             tc_fence_after();
             const uint32_t st = sbase + s * kStageBytes;
             const uint64_t ad = sw128_desc(st, 16, 1024), bd = sw128_desc(st + kHalfBytes, 16, 1024);
@@ -751,21 +724,8 @@ __global__ void __cluster_dims__(2, 1, 1)
       }
       if (elect_one()) umma_commit_pair(bar(kDrain));
       __syncwarp();
-    } else if constexpr (kGather) {
-      // The odd CTA's gathered rows, passed on to the thread that multiplies.
-      uint32_t step = 0;
-      bool ok = true;
-      for (uint32_t tile = first_tile; ok && tile < total; tile += tile_step)
-        for (uint32_t kb = 0; kb < nk; ++kb, ++step) {
-          const uint32_t s = step % kStages;
-          if (!(ok = warp_wait(bar(kGathered + s), (step / kStages) & 1, abort_flag, p, kSiteGathered)))
-            break;
-          fence_proxy_async();
-          if (elect_one()) mbar_arrive_cluster(full_at_even(s));
-          __syncwarp();
-        }
     }
-    drain_bar(bar(kDrain), 0);
+    drain_bar<true>(bar(kDrain), 0);
   } else {
     // Warp w finishes output columns [half * kCols, +kCols) of the 32 rows of its tensor-memory quarter.
     constexpr uint32_t kCols = kOut / 2, kStep = 32;
@@ -777,7 +737,7 @@ __global__ void __cluster_dims__(2, 1, 1)
     uint32_t done = 0, e = 0;
     bool ok = true;
     auto wait_acc = [&] {
-      const bool is = __all_sync(kFull, wait_bar(bar(kAcc + (done & 1)), (done >> 1) & 1, abort_flag,
+      const bool is = __all_sync(kFull, wait_bar<true>(bar(kAcc + (done & 1)), (done >> 1) & 1, abort_flag,
                                                  p.status, kSiteAcc, p.wait_cycles));
       tc_fence_after();
       return is;
@@ -876,37 +836,47 @@ cudaError_t launch_tiles(const ExpertsProblem &p, int num_sms, cudaStream_t stre
   cudaError_t e =
       allow_smem((const void *)experts_kernel<kBN, kGated, kLong, kGather>, (int)smem, seen);
   if (e != cudaSuccess) return e;
-  experts_kernel<kBN, kGated, kLong, kGather>
-      <<<num_sms, kGather ? kGatherThreads : kThreads, smem, stream>>>(mx, mw, p);
+  constexpr uint32_t threads = kThreads + (kGather ? 32 * kGathering<kBN, kLong> : 0);
+  experts_kernel<kBN, kGated, kLong, kGather><<<num_sms, threads, smem, stream>>>(mx, mw, p);
   return cudaGetLastError();
 }
 
-template <bool kGated, bool kLong, bool kGather>
+template <bool kGated, bool kLong>
 cudaError_t launch_pairs(const ExpertsProblem &p, int num_sms, cudaStream_t stream) {
   CUtensorMap mx, mw;
   if (!make_maps(&mx, &mw, p, 128)) return cudaErrorInvalidValue;
   static std::atomic<uint64_t> seen{0};
-  cudaError_t e =
-      allow_smem((const void *)pair_kernel<kGated, kLong, kGather>, (int)pair::kSmemBytes, seen);
+  cudaError_t e = allow_smem((const void *)pair_kernel<kGated, kLong>, (int)pair::kSmemBytes, seen);
   if (e != cudaSuccess) return e;
-  const uint32_t threads = kThreads + (kGather ? 32 * pair::kGathering<kLong> : 0);
-  pair_kernel<kGated, kLong, kGather><<<num_sms / 2 * 2, threads, pair::kSmemBytes, stream>>>(mx, mw, p);
+  pair_kernel<kGated, kLong><<<num_sms / 2 * 2, kThreads, pair::kSmemBytes, stream>>>(mx, mw, p);
   return cudaGetLastError();
 }
 
 template <bool kGated, bool kLong, bool kGather>
 cudaError_t launch_wide(const ExpertsProblem &p, int num_sms, cudaStream_t stream) {
   const uint32_t wide = p.n * (kGated ? 2 : 1);
-  // Tiles of two CTAs where an expert has 128 rows or more and there is work for them.  Against tiles of 128,
-  // gated, n 512, k 1024: 8192 rows over 8 experts 24.6 / 32.7 us, over 64 40.8 / 43.0; 4096 rows over 8
-  // 18.4 / 20.5, over 64 36.9 / 34.8; 2048 over 8 18.4 / 16.4; 65536 over 1024 432 / 420.  n 256, k 768, 16
-  // experts: 8192 rows 16.3 / 12.4, 16384 16.4 / 16.4, 65536 30.7 / 38.8.  In partial sums the tile's own end
-  // is longer, n 1024: 16384 rows over 8 experts, k 1024 47 / 49, 8192 rows 33 / 31, k 2048 43 / 49; 65536 over
-  // 64, k 1024 135 / 162, k 576 127 / 115.
-  const uint64_t work = (uint64_t)p.rows * wide * p.k;
-  const bool pairs = kLong ? p.k >= 1024 && work >= 1ull << 34 : p.rows > 8192 || work >= 1ull << 32;
-  if (wide > 128 && p.rows >= 128 * p.experts && pairs)
-    return launch_pairs<kGated, kLong, kGather>(p, num_sms, stream);
+  if constexpr (kGather) {
+    // 256 columns a tile where tiles of 128 are more than the SMs and an expert has 64 rows or more.  Tiles of
+    // 128 against 256 columns, gated, n 512, k 1024: 2048 rows over 8 experts 20 / 17 us, 8192 over 8 33 / 25,
+    // 4096 over 64 35 / 33, 65536 over 64 191 / 123, over 512 262 / 222.  n 1024, k 1024: 1024 rows over 8
+    // 17 / 19, 2048 24 / 21; n 256, k 768, 16 experts: 8192 rows 14 / 16, 16384 19 / 16; n 264, k 512: 32768
+    // over 64 32 / 29.  In partial sums, n 1024, k 1024: 8192 over 8 37 / 33, 65536 over 64 218 / 172; k 576
+    // 155 / 131; gated, n 512, k 1024 212 / 162.
+    if (wide > 128 && p.rows >= 64 * p.experts &&
+        (p.rows / kBM + (uint64_t)p.experts / 2) * ((wide + 127) / 128) > (uint64_t)num_sms)
+      return launch_tiles<256, kGated, kLong, true>(p, num_sms, stream);
+  } else {
+    // Tiles of two CTAs where an expert has 128 rows or more and there is work for them.  Tiles of 128 columns
+    // against them, gated, n 512, k 1024: 2048 rows over 8 experts 19 / 18 us, 8192 over 8 29 / 23, over 64
+    // 40 / 38, 65536 over 64 152 / 100, over 512 228 / 222, 4096 over 64 33 / 37 (but 4096 over 8 19 / 23).
+    // n 256, k 768, 16 experts: 8192 rows 13 / 16, 16384 16 / 16, 65536 39 / 30.  In partial sums the tile's own
+    // end is longer, n 1024, k 1024: 4096 rows over 8 21 / 31, 8192 31 / 31, 16384 51 / 47; 65536 over 64
+    // 164 / 137, k 576 115 / 141 in a loop.
+    const uint64_t work = (uint64_t)p.rows * wide * p.k;
+    const bool pairs = kLong ? p.k >= 1024 && work >= 1ull << 34 : p.rows > 8192 || work >= 1ull << 32;
+    if (wide > 128 && p.rows >= 128 * p.experts && pairs)
+      return launch_pairs<kGated, kLong>(p, num_sms, stream);
+  }
   // 64 columns a tile where tiles of 128 would leave half the SMs without one (the expert ranges are not
   // known here: at most a tile for each row or expert, and one for every 128 rows): 18 / 12 us for 2 to 32
   // rows over 8 experts, n 768, k 768; but 27 / 35 us for 64 rows over 64 experts, gated, n 512, k 1024.

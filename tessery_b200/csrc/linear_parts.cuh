@@ -16,12 +16,21 @@ using namespace ptx;
 
 constexpr long long kDrainCycles = 2000000000ll;
 
+// kCluster: threads or products of the other CTA of a pair arrive at the barrier.
+template <bool kCluster>
+__device__ __forceinline__ bool test_bar(uint32_t bar, uint32_t parity) {
+  if constexpr (kCluster)
+    return mbar_test_cluster(bar, parity);
+  else
+    return mbar_test(bar, parity);
+}
+template <bool kCluster = false>
 __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile int *abort_flag,
                                          int *status, int site, long long limit) {
-  if (mbar_test(bar, parity)) return true;
+  if (test_bar<kCluster>(bar, parity)) return true;
   const long long t0 = clock64();
   while (true) {
-    if (mbar_test(bar, parity)) return true;
+    if (test_bar<kCluster>(bar, parity)) return true;
     if (*abort_flag) return false;
     if (clock64() - t0 > limit) {
       *abort_flag = 1;
@@ -31,12 +40,14 @@ __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile
   }
 }
 // since: where several are drained in turn, when the first began.
+template <bool kCluster = false>
 __device__ __forceinline__ void drain_bar(uint32_t bar, uint32_t parity, long long since) {
-  while (!mbar_test(bar, parity) && clock64() - since < kDrainCycles) {
+  while (!test_bar<kCluster>(bar, parity) && clock64() - since < kDrainCycles) {
   }
 }
+template <bool kCluster = false>
 __device__ __forceinline__ void drain_bar(uint32_t bar, uint32_t parity) {
-  drain_bar(bar, parity, clock64());
+  drain_bar<kCluster>(bar, parity, clock64());
 }
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, uint32_t src, int x, int y) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(

@@ -65,11 +65,25 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
                    : "memory");
 }
-// Arrives at a barrier of another CTA of the cluster (an address from cluster_addr).  Orders what is in
-// this CTA alone before it, such as copies into this CTA's shared memory that the pair's product reads
-// there: with .release.cluster each such arrival took 1400 cycles while copies were in flight.
+// Arrives at a barrier of any CTA of the cluster (an address from cluster_addr).  It tells whoever waits with
+// mbar_test_cluster that this thread has come so far, and between tc_fence_before here and tc_fence_after there
+// orders tensor memory.  Writes to other memory it does not order: with .release, which does, an arrival waits
+// for all stores and copies in flight (1400 cycles beside gathered rows; 78 against 63 us for 65536 rows, n 1024,
+// k 512).
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// mbar_test for a barrier of this CTA at which threads or products of the other CTA arrive as well.
+__device__ __forceinline__ bool mbar_test_cluster(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
 }
 // Copies into this CTA's shared memory that count at a barrier of either CTA of the pair.
 __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap *map, uint32_t bar,

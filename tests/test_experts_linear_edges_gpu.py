@@ -6,8 +6,9 @@ import math
 import numpy as np
 import pytest
 
+from oracle import layers as oracle
 from tessery_b200.layers import experts_linear
-from tessery_b200.workloads import from_bf16_bits
+from tessery_b200.workloads import from_bf16_bits, to_bf16_bits
 
 pytestmark = pytest.mark.gpu
 
@@ -40,3 +41,39 @@ def test_gates_far_below_zero(runtime, act, out):
     want = FORMULA[act](b[:, :n]) * b[:, n:]
     rel = 2.0**-8 + 2.0**-17 if out == "bf16" else 2.0**-17
     np.testing.assert_array_less(np.abs(got - want), rel * np.abs(want) + 1e-30)
+
+
+@pytest.mark.parametrize("gated,n,k,out", [(False, 129, 72, "bf16"), (False, 160, 200, "float32"),
+                                           (False, 255, 40, "bf16"), (False, 520, 1100, "float32"),
+                                           (True, 65, 72, "bf16"), (True, 130, 700, "float32"),
+                                           (True, 257, 200, "bf16")])
+def test_widest_tiles_of_gathered_rows(runtime, gated, n, k, out):
+    """Rows of tokens in any order, enough that tiles are 256 columns wide: last columns and rows of
+    every kind, experts without rows, with one and with several tiles.  Tolerance as in
+    test_experts_linear_gpu.py."""
+    rng = np.random.default_rng(n)
+    counts = np.array([0, 4000, 1, 127, 128, 129, 0, 6001, 5, 300, 0])
+    rows, experts, top_k = int(counts.sum()), len(counts), 3
+    offsets = np.r_[0, np.cumsum(counts)]
+    tokens = -(-rows // top_k) + 50
+    order = np.full(tokens * top_k, -1)
+    order[:rows] = rng.permutation(tokens * top_k)[:rows]
+    wide = 2 * n if gated else n
+    x = to_bf16_bits(rng.standard_normal((tokens, k)).astype(np.float32))
+    w = to_bf16_bits((k**-0.5 * rng.standard_normal((experts, wide, k))).astype(np.float32))
+    bias = rng.standard_normal((experts, wide)).astype(np.float32)
+    kw = dict(gated=gated, activation="silu" if gated else "relu", bias=bias)
+    got = experts_linear(x, w, offsets, order=order, top_k=top_k, out_dtype=out, runtime=runtime, **kw)
+    assert not got[rows:].any()
+    for _ in range(2):
+        again = experts_linear(x, w, offsets, order=order, top_k=top_k, out_dtype=out, runtime=runtime,
+                               **kw)
+        assert np.array_equal(got, again)
+    some = np.unique(np.r_[offsets[1:] - 1, offsets[:-1], rng.integers(0, rows, 200)]).clip(0, rows - 1)
+    small = np.searchsorted(np.searchsorted(offsets, some, side="right") - 1, np.arange(experts + 1))
+    want, mass = oracle.experts_linear(from_bf16_bits(x)[order[some] // top_k], from_bf16_bits(w), small,
+                                       **kw)
+    got = from_bf16_bits(got) if out == "bf16" else got
+    tol = 1.13 * (k / 16 + 16) * 2.0**-23 * 1.001 * mass + 2.0**-20 * mass
+    tol = tol + (2.0**-8 * np.abs(want) if out == "bf16" else 0)
+    np.testing.assert_array_less(np.abs(got[some] - want), tol + 1e-30)
