@@ -547,9 +547,11 @@ enum { TX_SCORES_SOFTMAX = 0, TX_SCORES_SIGMOID = 1 };
  * of the top_groups groups are eligible whose best group_best (1 or 2) values of s + bias have the
  * largest sums.  A weight is the expert's s, divided by the sum of the chosen ones' with `renormalise`,
  * times scale.  The choice is that of exact arithmetic on the fp32 values of logits and bias, as far
- * as 64 bits tell s + bias and its sums apart.  An expert whose logit or bias is -inf is closed; NaN
- * ranks below every number and counts in no sum that the choice needs.  Where a token has fewer open experts than top_k, and for the rows of a padded batch past their
- * sequence's length, the remaining entries are expert -1 with weight 0. */
+ * as 64 bits tell s + bias and its sums apart.  An expert whose logit or bias is -inf is closed; the
+ * bias closes it to the choice alone, and in a softmax its logit counts as before.  NaN ranks below
+ * every number and counts in no sum that the choice needs.  Where a token has fewer open experts than
+ * top_k, and for the rows of a padded batch past their sequence's length, the remaining entries are
+ * expert -1 with weight 0. */
 typedef struct {
   const void *logits;      /* [tokens, experts] TX_F32 or TX_BF16 */
   uint64_t ld;             /* row stride in elements */

@@ -152,8 +152,8 @@ def experts_route(logits: NDArray, top_k: int, *, scores="softmax", bias=None, g
             continue
         with np.errstate(over="ignore", invalid="ignore"):
             if scores == "softmax":
-                s = np.exp(row - np.nanmax(row[open_]))
-                s = s / s[open_].sum()
+                s = np.exp(row - np.nanmax(row))
+                s = s / s.sum()
             else:
                 s = 1.0 / (1.0 + np.exp(-row))
         c = s + bias

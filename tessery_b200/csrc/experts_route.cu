@@ -326,8 +326,7 @@ __device__ __noinline__ void choose_exact(const RouteProblem &p, uint32_t *chose
 #pragma unroll 4
   for (int i = 0; i < V; ++i) {
     const uint32_t e = first + i;
-    float l = valid && i < (int)p.per_lane && e < p.experts ? logit_at(p, token, e) : -INFINITY;
-    if (l != -INFINITY && p.bias && p.bias[e] == -INFINITY) l = -INFINITY;
+    const float l = valid && i < (int)p.per_lane && e < p.experts ? logit_at(p, token, e) : -INFINITY;
     top = fmaxf(top, l);
     c[i] = l;
   }
@@ -344,7 +343,10 @@ __device__ __noinline__ void choose_exact(const RouteProblem &p, uint32_t *chose
     const double inv = p.softmax ? 1.0 / lanes_sum<kLanes>(sum) : 1.0;
 #pragma unroll 1
     for (int i = 0; i < V; ++i)
-      if (c[i] != -INFINITY) c[i] = c[i] * inv + (p.bias ? (double)p.bias[first + i] : 0.0);
+      if (c[i] != -INFINITY) {
+        const double b = p.bias ? (double)p.bias[first + i] : 0.0;
+        c[i] = b == -INFINITY ? b : c[i] * inv + b;
+      }
   }
   // NaN ranks below every number: -inf from here on, with a mark.
 #pragma unroll 1
@@ -652,11 +654,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
     {
       float c[V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        c[i] = __uint_as_float(raw.w[i]);
-        if constexpr (kScored)
-          if (bias[i * kLanes + sub] == -INFINITY) c[i] = -INFINITY;
-      }
+      for (int i = 0; i < V; ++i) c[i] = __uint_as_float(raw.w[i]);
       if (p.softmax && (kScored || !p.renormalise)) {
         all_top = c[0];
 #pragma unroll
@@ -691,7 +689,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           const float s = p.softmax ? quick_exp(c[i] - all_top) * inv : sigmoid(c[i]);
-          c[i] = c[i] == -INFINITY ? -INFINITY : s + bias[i * kLanes + sub];
+          c[i] = c[i] == -INFINITY ? -INFINITY : s + bias[i * kLanes + sub];  // closed by either's -inf
           far |= c[i] != c[i];
         }
         tol = score_tolerance<V>(p.softmax, inv);

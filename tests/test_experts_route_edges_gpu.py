@@ -53,3 +53,47 @@ def test_groups_whose_sums_cancel(runtime, scores, size, experts, groups, top_gr
         got = experts_route(x, top_k, runtime=runtime, **kw)
         np.testing.assert_array_equal(got.experts, oracle.experts_route(x, top_k, **kw)[0])
     assert close > 40
+
+
+@pytest.mark.parametrize("experts,groups,top_groups,top_k", [
+    (16, 1, 1, 4), (64, 1, 1, 8), (64, 8, 4, 8), (64, 1, 1, 12), (200, 1, 1, 8), (256, 64, 20, 8),
+    (640, 1, 1, 4), (1024, 16, 5, 9)])
+@pytest.mark.parametrize("renormalise", [False, True])
+@pytest.mark.parametrize("kind", ["spread", "neighbours"])
+def test_a_bias_takes_part_in_the_choice_alone(runtime, experts, groups, top_groups, top_k, renormalise,
+                                               kind):
+    """Experts closed by a bias of -inf, the one with the largest logit among them, keep their place
+    in the softmax: the scores by which the others are chosen, and their weights, are those of all
+    logits."""
+    rng = np.random.default_rng(experts + top_k)
+    x = (1.5 * rng.standard_normal((40, experts))).astype(np.float32).clip(-12, 11)
+    shut = rng.permutation(experts)[:max(1, experts // 8)]
+    x[:, shut[0]] = rng.uniform(2, 12, 40)
+    bias = (0.01 * rng.standard_normal(experts)).astype(np.float32)
+    bias[shut] = -np.inf
+    s = scores_of(x, "softmax")
+    if kind == "neighbours":  # of the first token: fp32 does not tell two experts apart
+        a, b = [e for e in np.argsort(-(s[0] + bias)) if np.isfinite(bias[e])][:2]
+        bias[b] = s[0, a] + bias[a] - s[0, b]
+    c = s + bias
+    per = experts // groups
+    want = []
+    for row in c:
+        top = np.sort(row.reshape(groups, per), axis=1)[:, -2:]
+        # A closed expert is in no sum; a group of closed experts alone comes behind all others.
+        sums = np.where(top[:, -1] == -np.inf, -np.inf, np.where(np.isinf(top), 0.0, top).sum(1))
+        kept = np.argsort(-sums, kind="stable")[:top_groups]
+        row = np.where(np.isin(np.arange(experts) // per, kept), row, -np.inf)
+        want.append(np.argsort(-row, kind="stable")[:top_k])
+    want = np.array(want)
+    assert np.isfinite(np.take_along_axis(c, want, 1)).all()
+    w = np.take_along_axis(s, want, 1)
+    if renormalise:
+        w = w / w.sum(1, keepdims=True)
+    kw = dict(bias=bias, groups=groups, top_groups=top_groups, renormalise=renormalise, scale=1.5)
+    got = experts_route(x, top_k, runtime=runtime, **kw)
+    np.testing.assert_array_equal(got.experts, want)
+    np.testing.assert_allclose(got.weights, 1.5 * w, rtol=2.0**-18)
+    restated = oracle.experts_route(x, top_k, **kw)
+    np.testing.assert_array_equal(restated[0], want)
+    np.testing.assert_allclose(restated[1], 1.5 * w, rtol=1e-12)
