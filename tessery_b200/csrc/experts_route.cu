@@ -60,11 +60,12 @@ __device__ __forceinline__ float quick_rcp(float x) {
   return y;
 }
 __device__ __forceinline__ float sigmoid(float l) { return quick_rcp(1.f + quick_exp(-l)); }
-// e^x in 64 bits without a branch, so that a lane's many overlap: x = k ln 2 + r with ln 2 in two parts, the
-// Taylor series of e^r to r^13 (|r| < 0.35: 4e-18 is left), and k into the exponent.  To 0 below -700.
+// e^x of x <= 0 in 64 bits without a branch, so that a lane's many overlap: x = k ln 2 + r, with ln 2 as the
+// nearest double and what that leaves, the Taylor series of e^r to r^13 (|r| < 0.35: 4e-18 is left), and 2^k in
+// two steps, of which the second rounds where the value is subnormal.  (e^-746 is 0.)
 __device__ __forceinline__ double exp_of(double x) {
-  const double z = fmin(fmax(x, -700.0), 700.0), k = rint(z * 1.4426950408889634);
-  const double r = fma(k, -1.9082149292705877e-10, fma(k, -0.693147180369123816490, z));
+  const double z = fmax(x, -746.0), k = rint(z * 1.4426950408889634);
+  const double r = fma(k, -2.3190468138462996e-17, fma(k, -0.6931471805599453, z));
   double y = 1.0 / 6227020800.0;
   y = fma(y, r, 1.0 / 479001600.0);
   y = fma(y, r, 1.0 / 39916800.0);
@@ -79,7 +80,7 @@ __device__ __forceinline__ double exp_of(double x) {
   y = fma(y, r, 0.5);
   y = fma(y, r, 1.0);
   y = fma(y, r, 1.0);
-  y = __longlong_as_double(__double_as_longlong(y) + ((long long)(int)k << 52));
+  y = __longlong_as_double(__double_as_longlong(y) + ((long long)((int)k + 600) << 52)) * 0x1p-600;
   return x != x ? x : y;
 }
 // 1 / (1 + e^-l): the reciprocal by Newton's steps from the hardware's.

@@ -97,3 +97,22 @@ def test_a_bias_takes_part_in_the_choice_alone(runtime, experts, groups, top_gro
     restated = oracle.experts_route(x, top_k, **kw)
     np.testing.assert_array_equal(restated[0], want)
     np.testing.assert_allclose(restated[1], 1.5 * w, rtol=1e-12)
+
+
+@pytest.mark.parametrize("experts,groups", [(32, 4), (60, 5), (256, 64), (640, 4), (1024, 8)])
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+def test_groups_far_below_the_largest_logit(runtime, experts, groups, scores):
+    """Scores down to e^-740, of which 64 bits hold a few bits yet, tell groups apart."""
+    per = experts // groups
+    rng = np.random.default_rng(experts)
+    for level in (-600, -690, -710, -720, -738):
+        x = (level - 60 + rng.uniform(0, 1, (6, experts))).astype(np.float32)  # in no group's best
+        stays = rng.integers(groups // 2, groups, 6)
+        for t, g in enumerate(stays):
+            for group in range(groups):
+                best = level + 2 * (group == g) if group else level + 4 if scores == "sigmoid" else 0
+                x[t, group * per:group * per + 2] = best
+        got = experts_route(x, 4, scores=scores, groups=groups, top_groups=2, renormalise=False,
+                            runtime=runtime)
+        want = [[0, 1, g * per, g * per + 1] for g in stays]
+        np.testing.assert_array_equal(got.experts, want)
