@@ -603,6 +603,8 @@ def block_norm(
     elif weights is not None or (y is not None and len(y) != rows):
         raise InvalidInputError()
     if gate is not None:
+        if rows and not len(gate):
+            raise InvalidInputError()
         kw.update(gate_rows=len(gate), gate_dtype=_dtype_code(gate), seq=seq)
     if cu_seqlens is not None:
         cu = _int32(cu_seqlens)
