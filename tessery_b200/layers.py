@@ -459,6 +459,8 @@ def experts_route(
     if logits.ndim != 2 or not logits.shape[1]:
         raise InvalidInputError()
     code, (tokens, experts) = _dtype_code(logits), logits.shape
+    if top_k > experts:  # before memory for as many is taken
+        raise InvalidInputError()
     if bias is not None and np.shape(bias) != (experts,):
         raise InvalidInputError()
     if lengths is not None:

@@ -17,3 +17,20 @@ def test_a_gate_without_rows(seq):
     block_norm(F, F, gate=F[:2], seq=3, runtime=Host())
     with pytest.raises(InvalidInputError):
         block_norm(F, F, gate=F[:0], seq=seq, runtime=Host())
+
+
+class NoMemory(Host):
+    """Host, of which a call may not take more than a few rows' memory before it is refused."""
+
+    def workspace(self, name, size):
+        assert size < 1 << 20
+        return super().workspace(name, size)
+
+
+@pytest.mark.parametrize("top_k", [17, 2**20, 2**45, 2**70])
+def test_more_choices_than_experts(top_k):
+    """Before room for as many is taken on the device, and filled on the host."""
+    with pytest.raises(InvalidInputError):
+        experts_route(F, top_k, runtime=NoMemory())
+    with pytest.raises(InvalidInputError):
+        experts_route(F[:0], top_k, runtime=NoMemory())
