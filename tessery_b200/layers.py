@@ -54,6 +54,14 @@ def _int32(a) -> NDArray[np.int32]:
     return held
 
 
+def _values(a) -> NDArray[np.float32]:
+    """`a` as float32; uint16 arrays, which hold bf16 patterns elsewhere here, are refused."""
+    a = np.asarray(a)
+    if a.dtype == np.uint16:
+        raise InvalidInputError()
+    return np.ascontiguousarray(a, dtype=np.float32)
+
+
 def _one_at_a_time(operator):
     """Holds the runtime for a whole call.  The named workspaces that inputs and results go through
     are the runtime's: between an upload and the read-back another thread's call would overwrite
@@ -461,7 +469,8 @@ def experts_route(
     code, (tokens, experts) = _dtype_code(logits), logits.shape
     if top_k > experts:  # before memory for as many is taken
         raise InvalidInputError()
-    if bias is not None and np.shape(bias) != (experts,):
+    bias = None if bias is None else _values(bias)
+    if bias is not None and bias.shape != (experts,):
         raise InvalidInputError()
     if lengths is not None:
         if seq < 1:
@@ -478,7 +487,7 @@ def experts_route(
     rt.experts_route_device(
         _upload(rt, "route_logits", logits) if tokens else at[0], at[0], at[1], tokens=tokens,
         num_experts=experts, top_k=top_k, logits_dtype=code,
-        bias=None if bias is None else _upload(rt, "route_bias", np.asarray(bias, np.float32)),
+        bias=None if bias is None else _upload(rt, "route_bias", bias),
         scores=scores, groups=groups, top_groups=top_groups, group_best=group_best,
         renormalise=renormalise, scale=scale, seq=seq,
         lengths=None if lengths is None or not tokens else _upload(rt, "route_lengths", lengths),
@@ -532,7 +541,8 @@ def experts_linear(
     offsets = _plan_offsets(offsets, rows)
     if offsets.size != experts + 1 or activation not in native.ACTIVATIONS:
         raise InvalidInputError()
-    if bias is not None and np.shape(bias) != (experts, wide):
+    bias = None if bias is None else _values(bias)
+    if bias is not None and bias.shape != (experts, wide):
         raise InvalidInputError()
     if order is not None:
         used = order[:offsets[-1]]
@@ -554,7 +564,7 @@ def experts_linear(
         offsets=_upload(rt, "experts_offsets", offsets), tokens=rows // top_k, top_k=top_k,
         num_experts=experts, n=n, k=k, gated=gated, activation=activation, ldx=ld, ldw=ld,
         order=None if order is None else _upload(rt, "experts_order", order),
-        bias=None if bias is None else _upload(rt, "experts_bias", np.asarray(bias, np.float32)),
+        bias=None if bias is None else _upload(rt, "experts_bias", bias),
         out_dtype=out_code)
     rt.sync()
     got = _read(rt, out, (rows, n), out_code)
@@ -598,6 +608,7 @@ def block_norm(
     kw: dict = {}
     if places is not None:
         places = _int32(places)
+        weights = None if weights is None else _values(weights)
         if (y is None or places.ndim != 2 or places.shape[0] != rows or np.shape(weights) != places.shape
                 or not places.shape[1] or np.any(places >= len(y))):
             raise InvalidInputError()
@@ -631,7 +642,7 @@ def block_norm(
             kw[name + "_dtype"] = _dtype_code(a)
     at = {name: _upload(rt, "norm_" + name, a)
           for name, a in (("x", x), ("y", y), ("gate", gate), ("places", places),
-                          ("weights", None if places is None else np.asarray(weights, np.float32)),
+                          ("weights", weights),
                           ("cu_seqlens", None if cu_seqlens is None else cu))
           if a is not None and a.size}
     for which, norm in zip(("after", "before"), norms, strict=True):

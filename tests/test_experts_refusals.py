@@ -34,3 +34,16 @@ def test_more_choices_than_experts(top_k):
         experts_route(F, top_k, runtime=NoMemory())
     with pytest.raises(InvalidInputError):
         experts_route(F[:0], top_k, runtime=NoMemory())
+
+
+@pytest.mark.parametrize("call", [
+    lambda a: experts_route(F, 2, bias=a(16), runtime=Host()),
+    lambda a: experts_linear(F.astype(np.uint16), np.ones((3, 8, 16), np.uint16), [0, 2, 4, 6],
+                             bias=a(3, 8), runtime=Host()),
+    lambda a: block_norm(F, F, places=np.zeros((6, 2), int), weights=a(6, 2), runtime=Host())])
+def test_bf16_patterns_where_values_are_wanted(call):
+    """As numbers the patterns would be other values."""
+    call(lambda *shape: np.ones(shape))
+    call(lambda *shape: np.ones(shape, int))
+    with pytest.raises(InvalidInputError):
+        call(lambda *shape: np.full(shape, 0x3F80, np.uint16))
