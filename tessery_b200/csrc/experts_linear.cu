@@ -118,10 +118,11 @@ struct Gather {
     const uint16_t *x = static_cast<const uint16_t *>(p.x) + chunk * 8;
 #pragma unroll
     for (uint32_t i = 0; i < kEach; ++i) {
-      // pair / top_k by the reciprocal floor(2^32 / top_k) + 1, which is one too much at most.
+      // pair / top_k by the reciprocal floor(2^32 / top_k) + 1, which is one too much at most.  (A negative
+      // pair is far up among the unsigned ones, where its quotient may yet be a row.)
       uint32_t at = p.top_k > 1 ? __umulhi((uint32_t)pair[i], p.top_k_inv) : (uint32_t)pair[i];
       if (at * p.top_k > (uint32_t)pair[i]) --at;
-      if (at >= p.x_rows) {
+      if (pair[i] < 0 || at >= p.x_rows) {
         report_status(p.status, kStatusBadArg);
         at = p.x_rows - 1;
       }

@@ -7,10 +7,12 @@ import numpy as np
 import pytest
 
 from oracle import layers as oracle
+from tessery_b200 import TX_F32, InvalidInputError
 from tessery_b200.layers import experts_linear
 from tessery_b200.workloads import from_bf16_bits, to_bf16_bits
 
 pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
 
 ERFC = np.vectorize(math.erfc)
 FORMULA = {
@@ -77,3 +79,25 @@ def test_widest_tiles_of_gathered_rows(runtime, gated, n, k, out):
     tol = 1.13 * (k / 16 + 16) * 2.0**-23 * 1.001 * mass + 2.0**-20 * mass
     tol = tol + (2.0**-8 * np.abs(want) if out == "bf16" else 0)
     np.testing.assert_array_less(np.abs(got[some] - want), tol + 1e-30)
+
+
+def test_negative_entries_of_a_plan_of_many_choices(runtime):
+    """Of 1000 choices a token, 2^32 - 1 is one of token 4294967, which is there: the library's own
+    call takes a number of rows of x apart from that of the plan."""
+    x = torch.ones(4_300_000, 8, device="cuda").bfloat16()
+    w = torch.ones(1, 8, 8, device="cuda").bfloat16()
+    out = torch.zeros(6, 8, device="cuda")
+    offsets = torch.tensor([0, 6], dtype=torch.int32, device="cuda")
+    for entries, bad in (([0, 1, 2, 4000, 4, 5], False), ([0, 1, 2, -1, 4, 5], True)):
+        order = torch.tensor(entries, dtype=torch.int32, device="cuda")
+        torch.cuda.synchronize()
+        rc = runtime._lib.tx_experts_linear(
+            runtime._pointer, x.data_ptr(), 8, len(x), w.data_ptr(), 8, 64, None, out.data_ptr(), TX_F32,
+            8, offsets.data_ptr(), order.data_ptr(), 6, 1, 1000, 8, 8, 0, 0, None)
+        assert rc == 0
+        if bad:
+            with pytest.raises(InvalidInputError):
+                runtime.sync()
+        else:
+            runtime.sync()
+        assert (out == 8).all()
