@@ -101,3 +101,36 @@ def test_negative_entries_of_a_plan_of_many_choices(runtime):
         else:
             runtime.sync()
         assert (out == 8).all()
+
+
+def parts_bound(k):
+    """What an fp32 result may be off by, relative to the sum of its terms' magnitudes: in parts of 512
+    columns each of 32 additions of 16 products cuts less than a step of 2^-23 off, each part is added
+    with a rounding, and 16 more for the 16 products' own alignment, as in test_experts_linear_gpu.py."""
+    return (512 / 16 + -(-k // 512) + 16) * 2.0**-23
+
+
+@pytest.mark.parametrize("rows,experts,n,k,gather", [
+    (3, 2, 16, 16384, True), (40, 3, 130, 20000, False), (300, 2, 260, 16392, True),
+    (4000, 2, 512, 16384, False), (4000, 2, 300, 16384, True)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_long_sums_of_one_sign(runtime, rows, experts, n, k, gather, gated):
+    """Where every addition cuts off in the same direction: a single accumulator over k would be off by
+    more than twice the bound (test_experts_sums.py)."""
+    rng = np.random.default_rng(rows + k)
+    wide = 2 * n if gated else n
+    x = to_bf16_bits(rng.uniform(0.5, 1, (rows, k)).astype(np.float32))
+    w = to_bf16_bits((rng.uniform(0.5, 1, (experts, wide, k)) / k).astype(np.float32))
+    offsets = np.linspace(0, rows, experts + 1).astype(int)
+    order = rng.permutation(rows) if gather else None
+    got = experts_linear(x, w, offsets, order=order, gated=gated, out_dtype="float32", runtime=runtime)
+    some = np.unique(np.r_[offsets[1:] - 1, offsets[:-1], rng.integers(0, rows, 60)])
+    some = some[some < rows]
+    small = np.searchsorted(np.searchsorted(offsets, some, side="right") - 1, np.arange(experts + 1))
+    want, _ = oracle.experts_linear(from_bf16_bits(x)[order[some] if gather else some],
+                                    from_bf16_bits(w), small, gated=gated)
+    rel = np.abs(got[some] - want) / want
+    # Gated, both sums' errors are in the product, and its rounding.
+    bound = parts_bound(k) * (2.001 if gated else 1) + 2.0**-23
+    print(f"worst {rel.max() * 2**23:.1f}, bound {bound * 2**23:.1f} of 2^-23")
+    assert rel.max() <= bound
