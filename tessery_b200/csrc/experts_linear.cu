@@ -903,9 +903,9 @@ cudaError_t launch_experts_linear(ExpertsProblem p, int num_sms, cudaStream_t st
   // The short form of GELU is off by 1.4e-6 of the sum, 5 % of the value at -5, which is nothing beside 1 but
   // not where the value is multiplied by the up half.
   if (p.act == TX_ACT_GELU && (p.out_dtype == TX_F32 || p.gated)) p.act = kGeluF32;
-  // The accumulator cuts bits off at each of its additions: over 512 K that is far below bf16's rounding,
-  // for an fp32 result it is not.
-  const bool parts = p.out_dtype == TX_F32 && p.k > kPart * kBK;
+  // The accumulator cuts up to 2^-23 off at each of its additions of 16 K: over 32768 that is a twentieth of
+  // half a bf16 step at most, but 1 % of the value over 2^21, and for an fp32 result too much over 512 already.
+  const bool parts = p.k > (p.out_dtype == TX_F32 ? kPart * kBK : 32768);
   if (p.gated)
     return parts ? launch_rows<true, true>(p, num_sms, stream)
                  : launch_rows<true, false>(p, num_sms, stream);

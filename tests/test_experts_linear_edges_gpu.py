@@ -134,3 +134,18 @@ def test_long_sums_of_one_sign(runtime, rows, experts, n, k, gather, gated):
     bound = parts_bound(k) * (2.001 if gated else 1) + 2.0**-23
     print(f"worst {rel.max() * 2**23:.1f}, bound {bound * 2**23:.1f} of 2^-23")
     assert rel.max() <= bound
+
+
+@pytest.mark.parametrize("gated", [False, True])
+def test_bf16_results_of_very_long_sums(runtime, gated):
+    """2^21 columns of one sign: half a step of bf16 and no more (a single accumulator cuts off about
+    2^-23 at each of 131072 additions, 1 % in all)."""
+    rng = np.random.default_rng(21)
+    rows, n, k = 2, 8, 1 << 21
+    wide = 2 * n if gated else n
+    x = to_bf16_bits(rng.uniform(0.5, 1, (rows, k)).astype(np.float32))
+    w = to_bf16_bits((rng.uniform(0.5, 1, (1, wide, k)) / k).astype(np.float32))
+    got = from_bf16_bits(experts_linear(x, w, [0, rows], gated=gated, runtime=runtime))
+    want, _ = oracle.experts_linear(from_bf16_bits(x), from_bf16_bits(w), [0, rows], gated=gated)
+    # The parts' own: 4096 of them added with a rounding each (2^-12 at worst; 2^-18 in the mean).
+    np.testing.assert_array_less(np.abs(got - want), (2.0**-8 + 2.0**-12 * (1 + gated)) * want)
