@@ -903,7 +903,7 @@ cudaError_t launch_experts_linear(ExpertsProblem p, int num_sms, cudaStream_t st
   // The short form of GELU is off by 1.4e-6 of the sum, 5 % of the value at -5, which is nothing beside 1 but
   // not where the value is multiplied by the up half.
   if (p.act == TX_ACT_GELU && (p.out_dtype == TX_F32 || p.gated)) p.act = kGeluF32;
-  // The accumulator cuts up to 2^-23 off at each of its additions of 16 K: over 32768 that is a twentieth of
+  // The accumulator cuts up to 2^-23 off at each of its additions of 16 K: over 32768 that is a sixteenth of
   // half a bf16 step at most, but 1 % of the value over 2^21, and for an fp32 result too much over 512 already.
   const bool parts = p.k > (p.out_dtype == TX_F32 ? kPart * kBK : 32768);
   if (p.gated)

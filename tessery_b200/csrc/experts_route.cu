@@ -170,6 +170,7 @@ __device__ __noinline__ uint32_t keep_any_groups(const RouteProblem &p, uint32_t
 #pragma unroll
   for (int m = 0; m < kSums; ++m) {
     sums[m] = none;
+    size[m] = 0.f;
     before[m] = 0;
   }
   for (uint32_t g = 0; g < p.groups; ++g) {
@@ -192,31 +193,34 @@ __device__ __noinline__ uint32_t keep_any_groups(const RouteProblem &p, uint32_t
     for (int m = 0; m < kSums; ++m)
       before[m] += other > sums[m] || (other == sums[m] && h < sub + m * kLanes);
   }
+  // What a sum that is kept may come down to, and one that is left out up to.
+#pragma unroll
+  for (int m = 0; m < kSums; ++m) {
+    const float off = size[m] * (0.5f * kSumRoundings);
+    if (sums[m] > none) sums[m] += before[m] < p.top_groups ? -off : off;
+  }
   uint32_t mask = 0;
-  // What the lowest sum kept may come down to, and the highest left out up to.
-  float low = INFINITY, high = none;
+  float low = INFINITY, high = none;  // the lowest of those kept, the highest of those left out
   for (uint32_t g = 0; g < p.groups; ++g) {
-    float s = none, off = 0.f;
+    float s = none;
     uint32_t n = 0;
 #pragma unroll
     for (int m = 0; m < kSums; ++m)
       if (g / kLanes == m) {
         s = sums[m];
-        off = size[m] * (0.5f * kSumRoundings);
         n = before[m];
       }
     s = __shfl_sync(kFull, s, slot * kLanes + g % kLanes);
-    off = __shfl_sync(kFull, off, slot * kLanes + g % kLanes);
     n = __shfl_sync(kFull, n, slot * kLanes + g % kLanes);
     if (n < p.top_groups) {
-      low = fminf(low, s - off);
+      low = fminf(low, s);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const uint32_t e = sub * p.per_lane + i;
         if (e >= g * per && e < (g + 1) * per) mask |= 1u << i;
       }
-    } else if (s > none) {
-      high = fmaxf(high, s + off);
+    } else {
+      high = fmaxf(high, s);
     }
   }
   if (high > none) *near |= !(low - high > 3.f * tol);
