@@ -573,6 +573,7 @@ typedef struct {
 
 /* experts at most 1024, groups at most 64, top_k at most 32 and at most the eligible experts, tokens *
  * top_k below 2^31.
+ * Weights are computed in fp32 (2^-18 of the value for logits of at most 12; 4e-7 measured).
  * More than a few hundred tokens take two launches and scratch of the context (or, on a stream that is
  * being captured, of the graph). */
 int tx_experts_route(void *ctx, const TxRoute *route, uint32_t tokens, uint32_t experts,
@@ -587,7 +588,13 @@ int tx_experts_route(void *ctx, const TxRoute *route, uint32_t tokens, uint32_t 
  * k; x and w 16-byte aligned with ldx, ldw and expert_stride multiples of 8 (columns past k may hold
  * anything).  experts at most 1024.  Rows past offsets[experts] are left as they were.  An offset that
  * falls or leaves 0 .. rows is cut to fit, a row of x that is not there replaced by the last; both are
- * reported as TX_EINVAL by the next tx_sync. */
+ * reported as TX_EINVAL by the next tx_sync.
+ * Accuracy, besides out's rounding: sums are taken in parts of 512 columns for fp32 results, and for
+ * bf16 ones of more than 32768 columns; a part is off by at most 48 of 2^-23 of its terms' magnitudes
+ * (2 to 8 measured), a whole sum by k / 16 + 16 of them.
+ * Activations: SiLU 6e-7 of the value for |y| <= 8, GELU 3e-6, GELU (tanh) 8e-6, by the hardware's
+ * exponential and reciprocal; GELU of a bf16 result without a gate 1.4e-6 of |y|, which is 5 % of the
+ * value at -5. */
 int tx_experts_linear(void *ctx, const void *x, uint64_t ldx, uint32_t x_rows, const void *w,
                       uint64_t ldw, uint64_t expert_stride, const float *bias, void *out,
                       int out_dtype, uint64_t ldo, const int32_t *offsets, const int32_t *order,

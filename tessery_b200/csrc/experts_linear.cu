@@ -12,9 +12,10 @@
 // have to be handed from one CTA's threads to the other's products, with an arrival that waits for all copies
 // in flight: 244 us where 128 x 256 tiles by one CTA take 117.
 //
-// Measured: 65536 rows over 64 experts, gated, n 512, k 1024, gathered: 117 us from rest, 1175 TFLOP/s, and
-// 142 us in a loop under the power limit; n 1024, k 512, rows by expert: 64 us, 1080 TFLOP/s and 4.2 TB/s, and
-// 83 to 87 us in a loop.  Bound: the tensor pipe with its power, and for the latter the writes of out.
+// Measured: 65536 rows over 64 experts, gated, n 512, k 1024, gathered: 115 us from rest, 1195 TFLOP/s, and
+// 139 to 146 us in a loop under the power limit; n 1024, k 512, rows by expert: 61 us, 1120 TFLOP/s, and 83 to
+// 85 us in a loop.  Bound: the tensor pipe, 60 % of whose cycles are used, beside L2's way in (12.5 TB/s), and for
+// the latter the writes of out; 5.9 and 12.9 % of the rows multiplied, in experts' last tiles, are not there.
 #include <cuda.h>
 
 #include <algorithm>
@@ -372,7 +373,8 @@ __device__ __forceinline__ void add_columns(uint32_t at, float (&v)[kStep]) {
 }
 
 // kLong: the sum is taken in parts of 512 K that are added in fp32 registers.  (Added from zero on: with the
-// first part taken as it is the compiler held them twice.)
+// first part taken as it is the compiler held them twice.  Tiles of 256 columns, gated, still pass 24 to 32 bytes
+// a thread through local memory.)
 // Two warps gather where each epilogue thread holds 128 sums and the others' registers are those that it lacks
 // (with four, sums went through local memory), otherwise four.
 template <int kBN, bool kLong>

@@ -16,11 +16,14 @@
 // its rank among the warp's; place_kernel adds what lies before, of the warps and blocks before it.  A few
 // tokens are one block, which does both.
 //
-// Bound: instructions and their latency.  Measured: 65536 tokens of 128 bf16 logits, 8 of each, 24.6 us (HBM
-// would take 3.8; 28.7 with place_kernel launched behind the runs and its pairs loaded behind the counts);
-// 16384 tokens of 256, 8 of each from 4 in 8 groups, with a bias, 31 us (2.9); 8 tokens of 64, one launch,
-// 8.2.  With a round for each chosen expert, in place of the lanes' eight largest together, the first took
-// 50 us, the second 48.
+// Bound: instructions and their latency, and place_kernel (10 to 12 us), each block of which sums the counts of
+// all runs.  Measured: 65536 tokens of 128 bf16 logits, 8 of each, 24.6 us (HBM would take 3.8; 28.7 with
+// place_kernel launched behind the runs and its pairs loaded behind the counts); 16384 tokens of 256, 8 of each
+// from 4 in 8 groups, with a bias, 31 us (2.9), from 4 in 8 by softmax with a bias, where every doubt takes
+// the exact choice, 102, from 20 in 64 groups that cut through lanes 313; 8 tokens of 64, one launch, 9.2.  With
+// a round for each chosen expert, in place of the lanes' eight largest together, the first took 50 us, the second
+// 48; the rounds that are left: 16384 tokens, 12 of 256 in groups, 65 us, 16 of 128 41; 8192 tokens, 8 of
+// 1024 105, 32 of 1024 289.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -1046,7 +1049,9 @@ cudaError_t run_warps(RouteProblem p, cudaStream_t stream) {
 // of 64 experts: 8.2 against 9.5 us).
 template <int kLanes, int V, bool kScored, bool kTop8>
 cudaError_t run(const RouteProblem &p, cudaStream_t stream) {
-  constexpr int kWarps = V <= 8 || kTop8 ? kMostWarps : kMostWarps / 2;  // as registers allow
+  // 64 registers a thread with 32 warps, 128 with 16.  64 are few: 17 of the 18 forms of 32 warps keep some in
+  // local memory (4 to 616 bytes stored; the two of the large cases above 132 and 12).
+  constexpr int kWarps = V <= 8 || kTop8 ? kMostWarps : kMostWarps / 2;
   if (p.tokens <= 4 * (32 / kLanes)) return run_warps<kLanes, V, kScored, 4, kTop8>(p, stream);
   return run_warps<kLanes, V, kScored, kWarps, kTop8>(p, stream);
 }
