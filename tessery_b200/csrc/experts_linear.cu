@@ -860,13 +860,15 @@ cudaError_t launch_wide(const ExpertsProblem &p, int num_sms, cudaStream_t strea
   const uint32_t wide = p.n * (kGated ? 2 : 1);
   if constexpr (kGather) {
     // 256 columns a tile where tiles of 128 are more than the SMs and an expert has 64 rows or more.  Tiles of
-    // 128 against 256 columns, gated, n 512, k 1024: 2048 rows over 8 experts 20 / 17 us, 8192 over 8 33 / 25,
+    // 128 against 256 columns, gated, n 512, k 1024: 2048 rows over 8 experts 20 / 18 us, 8192 over 8 34 / 25,
     // 4096 over 64 35 / 33, 65536 over 64 191 / 123, over 512 262 / 222.  n 1024, k 1024: 1024 rows over 8
-    // 17 / 19, 2048 24 / 21; n 256, k 768, 16 experts: 8192 rows 14 / 16, 16384 19 / 16; n 264, k 512: 32768
-    // over 64 32 / 29.  In partial sums, n 1024, k 1024: 8192 over 8 37 / 33, 65536 over 64 218 / 172; k 576
-    // 155 / 131; gated, n 512, k 1024 212 / 162.
+    // 16 / 17, 2048 21 / 18; n 512, k 2048: 4096 over 8 21 / 24, 6000 31 / 25; n 256, k 768, 16 experts: 8192 rows
+    // 14 / 16, 16384 19 / 16; n 264, k 512: 32768 over 64 32 / 29.  In partial sums the tile's own end is longer,
+    // and three tiles of 128 for each SM are the border: n 1024, k 1024: 4096 over 8 25 / 29, 6000 31 / 35, 8192
+    // 38 / 33, 65536 over 64 218 / 172; k 576 155 / 131; gated, n 512, k 1024: 6000 over 8 29 / 32, 8192 36 / 33,
+    // 65536 over 64 212 / 162.
     if (wide > 128 && p.rows >= 64 * p.experts &&
-        (p.rows / kBM + (uint64_t)p.experts / 2) * ((wide + 127) / 128) > (uint64_t)num_sms)
+        (p.rows / kBM + (uint64_t)p.experts / 2) * ((wide + 127) / 128) > (kLong ? 3ull : 1ull) * num_sms)
       return launch_tiles<256, kGated, kLong, true>(p, num_sms, stream);
   } else {
     // Tiles of two CTAs where an expert has 128 rows or more and there is work for them.  Tiles of 128 columns
